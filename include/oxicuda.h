@@ -613,6 +613,104 @@ oxc_status oxc_layer_norm_bwd_noalloc(const float* x, const float* w, const floa
                                       float* dx, float* dw, float* db, int64_t rows, int64_t cols,
                                       int32_t act, int32_t grad_mode, void* stream);
 
+/* ---- layers of a recurrent draft model --------------------------------------
+ * No counterpart in the reference: what a small recurrent language model needs
+ * beside the layers above when it is distilled from a larger one and drafts
+ * tokens for it.  Where `dtype` appears, the void* tensors hold float32
+ * (OXC_F32) or bfloat16 (OXC_BF16) elements; everything declared float* is
+ * float32 either way, and all arithmetic is f32 with one rounding to the
+ * tensor's type.  Strides are in elements; the last dim is dense. */
+#define OXC_F32 0
+#define OXC_BF16 1
+
+/* r = x + residual; y = r / sqrt(mean_row(r^2) + eps) * w.
+ * x, residual: [rows, cols] with row strides; y (dtype), r (f32) dense; rstd
+ * [rows] is what the VJP needs.  cols <= 32768. */
+oxc_status oxc_add_rms_norm_fwd(const void* x, int64_t x_stride, const float* residual,
+                                int64_t residual_stride, const float* w, void* y, float* r,
+                                float* rstd, int64_t rows, int64_t cols, int32_t dtype, float eps,
+                                void* stream);
+/* The same norm in 8 bits: per row and block of `block` columns (128, or 0 for
+ * the whole row) scale = max(amax(|y|) / 448, 2^-126) and q = e4m3(y / scale),
+ * to nearest even.  q: [rows, cols] e4m3 bytes; scale: [rows, ceil(cols /
+ * block)]; r as above. */
+oxc_status oxc_add_rms_norm_quant(const void* x, int64_t x_stride, const float* residual,
+                                  int64_t residual_stride, const float* w, uint8_t* q,
+                                  float* scale, float* r, int64_t rows, int64_t cols,
+                                  int64_t block, int32_t dtype, float eps, void* stream);
+/* dresidual (f32) = dr + the norm's gradient for dy (dtype); dr may be NULL
+ * (zero).  dx = dresidual in bf16 when dtype is OXC_BF16 (in f32 it is
+ * dresidual itself, and dx is not used); dw: [cols].  grad_mode as for
+ * oxc_rms_norm_bwd. */
+size_t oxc_add_rms_norm_bwd_workspace_size(int64_t rows, int64_t cols);
+oxc_status oxc_add_rms_norm_bwd(const float* r, const float* w, const float* rstd, const void* dy,
+                                int64_t dy_stride, const float* dr, int64_t dr_stride,
+                                float* dresidual, void* dx, float* dw, int64_t rows, int64_t cols,
+                                int32_t dtype, int32_t grad_mode, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/* Gated linear recurrence: h_t = a_t h_{t-1} + (1 - a_t) x_t, a = sigmoid(gate),
+ * over dim 1 of [batch, length, dim]; x, gate, dh take batch and time strides.
+ * starts (uint8 [batch, length], may be NULL): where nonzero, a new sequence
+ * begins and the state before that token is zero.  h0 (f32 [batch, dim], NULL =
+ * zero) is the state before the first token; last (may be NULL) receives the
+ * state after the last.  h is dense.  carry: oxc_gated_scan_carry_size floats
+ * that the VJP reads (NULL when there will be none).  The VJP's dh may be NULL
+ * (zero), as may dlast; dx, dgate are dense, dh0 may be NULL.
+ * One workspace size for both directions. */
+int64_t oxc_gated_scan_carry_size(int64_t batch, int64_t length, int64_t dim);
+size_t oxc_gated_scan_workspace_size(int64_t batch, int64_t length, int64_t dim);
+oxc_status oxc_gated_scan_fwd(const void* x, int64_t x_sb, int64_t x_st, const void* gate,
+                              int64_t g_sb, int64_t g_st, const uint8_t* starts, const float* h0,
+                              void* h, float* last, float* carry, int64_t batch, int64_t length,
+                              int64_t dim, int32_t dtype, void* workspace, size_t workspace_bytes,
+                              void* stream);
+oxc_status oxc_gated_scan_bwd(const void* x, int64_t x_sb, int64_t x_st, const void* gate,
+                              int64_t g_sb, int64_t g_st, const uint8_t* starts,
+                              const float* carry, const void* dh, int64_t dh_sb, int64_t dh_st,
+                              const float* dlast, void* dx, void* dgate, float* dh0, int64_t batch,
+                              int64_t length, int64_t dim, int32_t dtype, void* workspace,
+                              size_t workspace_bytes, void* stream);
+/* One token: state_out = a state + (1 - a) x and h = state_out in dtype, for
+ * [batch, dim]; state_out may be state. */
+oxc_status oxc_gated_step(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,
+                          const float* state, float* state_out, void* h, int64_t batch,
+                          int64_t dim, int32_t dtype, void* stream);
+
+/* Distillation from a teacher's top logits: loss[0] = tau^2 / total_rows *
+ * sum_rows sum_k p_k (log p_k - log q(id_k)), p = softmax(teacher_logits / tau)
+ * over the row's entries, q = softmax(logits / tau) over the vocabulary, and
+ * (unless dlogits is NULL) dlogits = grad_loss[0] * d loss / d logits, dense, in
+ * the same pass; grad_loss NULL = 1.  teacher_logits f32, teacher_ids int64:
+ * [rows, top].  An entry with a negative id or a -inf logit is absent; a row
+ * without entries gives loss 0 and gradient 0.  An id >= vocab is recorded in
+ * err_flag (int32[4], may be NULL) and, like a NaN teacher logit, makes the
+ * row's loss and gradient NaN.  row_loss: [rows] scratch (the per-row sums). */
+oxc_status oxc_distill_loss(const void* logits, int64_t logits_stride, const float* teacher_logits,
+                            const int64_t* teacher_ids, int64_t top, float temperature,
+                            const float* grad_loss, float* loss, float* row_loss, void* dlogits,
+                            int64_t rows, int64_t vocab, int64_t total_rows, int32_t dtype,
+                            int32_t* err_flag, void* stream);
+/* x[0..n) *= g[0] in place, g on the device; reads and writes nothing of x when
+ * g[0] is 1. */
+oxc_status oxc_scale_by(void* x, int64_t n, int32_t dtype, const float* g, void* stream);
+
+/* Verification of drafted tokens.  target: f32 probabilities [batch, drafted +
+ * 1, vocab], draft: [batch, drafted, vocab] (both with batch and place
+ * strides; draft NULL = the drafted token had probability 1); tokens, lengths
+ * (NULL = drafted): how many of tokens[b] count; uniform: [batch, drafted] in
+ * [0, 1); race: [batch, vocab] exponential variates.  Token k is kept while
+ * uniform * q < p; out_tokens [batch, drafted + 1] gets the kept tokens, then
+ * argmax max(p - q, 0) / race at the first one not kept (p / race after the
+ * last), then -1; accepted[b] is how many were kept.  A token outside [0,
+ * vocab) is recorded in err_flag and not kept. */
+oxc_status oxc_verify_draft(const float* target, int64_t target_sb, int64_t target_sk,
+                            const float* draft, int64_t draft_sb, int64_t draft_sk,
+                            const int64_t* tokens, const int64_t* lengths, const float* uniform,
+                            const float* race, int64_t batch, int64_t drafted, int64_t vocab,
+                            int64_t* out_tokens, int64_t* accepted, int32_t* err_flag,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -30,6 +30,8 @@ GRAD_REF = 0
 GRAD_EXACT = 1
 ACT_NONE = 0
 ACT_GELU_TANH = 1
+F32 = 0
+BF16 = 1
 
 MAX_DIMS = 8
 
@@ -196,6 +198,25 @@ SIGNATURES = {
                                         _P]),
     "oxc_upload": (_I32, [_P, _P, _I64, _P]),
     "oxc_download": (_I32, [_P, _P, _I64, _P]),
+    "oxc_add_rms_norm_fwd": (_I32, [_P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I32, _F32,
+                                    _P]),
+    "oxc_add_rms_norm_quant": (_I32, [_P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I32,
+                                      _F32, _P]),
+    "oxc_add_rms_norm_bwd_workspace_size": (_SZ, [_I64, _I64]),
+    "oxc_add_rms_norm_bwd": (_I32, [_P, _P, _P, _P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I32,
+                                    _I32, _P, _SZ, _P]),
+    "oxc_gated_scan_carry_size": (_I64, [_I64, _I64, _I64]),
+    "oxc_gated_scan_workspace_size": (_SZ, [_I64, _I64, _I64]),
+    "oxc_gated_scan_fwd": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64,
+                                  _I64, _I32, _P, _SZ, _P]),
+    "oxc_gated_scan_bwd": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _P,
+                                  _P, _P, _I64, _I64, _I64, _I32, _P, _SZ, _P]),
+    "oxc_gated_step": (_I32, [_P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I32, _P]),
+    "oxc_distill_loss": (_I32, [_P, _I64, _P, _P, _I64, _F32, _P, _P, _P, _P, _I64, _I64, _I64,
+                                _I32, _P, _P]),
+    "oxc_scale_by": (_I32, [_P, _I64, _I32, _P, _P]),
+    "oxc_verify_draft": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64,
+                                _P, _P, _P, _P]),
 }
 
 NOALLOC_SCRATCH_BYTES = 16 * 1024 * 1024

@@ -522,3 +522,408 @@ def silu(x):
 def swiglu(gate, up):
     """silu(gate) * up, the decoder-MLP gate (composed by callers of F.silu)."""
     return _SwiGLU.apply(gate, up)
+
+
+# ---- layers of a recurrent draft model -------------------------------------------------
+#
+# What a small recurrent language model needs beside the layers above when it is
+# distilled from a larger one and then drafts tokens for it.  The reference has
+# no counterpart.  Activations and logits may be float32 or bfloat16; the
+# residual stream, weights, recurrent states, scales and probabilities are
+# float32, and so is all arithmetic (a bfloat16 result is rounded once).
+
+_DTYPES = {torch.float32: N.F32, torch.bfloat16: N.BF16}
+
+
+def _dtype_id(name, t):
+    """The dtype id of a float32 / bfloat16 CUDA tensor on the current device."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch CUDA tensor")
+    if not t.is_cuda:
+        raise ValueError(f"invalid argument: {name} must live on a CUDA device "
+                         "(oxitorch_b200 has no CPU path)")
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"invalid argument: {name} lives on {t.device}, the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"invalid argument: {name} must be float32 or bfloat16, got {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+def _operand(name, t, shape, dtype, device):
+    """Checks one more tensor of a call: its shape, type and device."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch CUDA tensor")
+    if t.device != device:
+        raise ValueError(f"invalid argument: {name} must live on {device}, got {t.device}")
+    if t.dtype != dtype:
+        raise ValueError(f"invalid argument: {name} must be {str(dtype)[6:]}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"shape mismatch: {name} {list(t.shape)} vs {list(shape)}")
+
+
+def _dense_any(t):
+    if t.is_contiguous():
+        return t
+    return dense(t) if t.dtype == torch.float32 else t.contiguous()
+
+
+def _rows2d(t):
+    """t as [rows, cols] over its last dim with any row stride; a copy only if
+    the leading dims do not collapse or the last one is not dense."""
+    cols = t.shape[-1]
+    if t.dim() != 2:
+        try:
+            t = t.view(-1, cols) if cols else t.reshape(0, 0)
+        except RuntimeError:
+            t = _dense_any(t).view(-1, cols)
+    if cols > 1 and t.stride(1) != 1:
+        t = _dense_any(t)
+    return t
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+# ---- residual addition + RMSNorm ---------------------------------------------------------
+
+def _add_rms_args(x, residual, weight):
+    dt = _dtype_id("x", x)
+    if x.dim() == 0:
+        raise ValueError("invalid argument: dim -1 out of range for 0-D tensor")
+    _operand("residual", residual, x.shape, torch.float32, x.device)
+    _operand("weight", weight, (x.shape[-1],), torch.float32, x.device)
+    return dt, _rows2d(x), _rows2d(residual), dense(weight)
+
+
+def add_rms_norm_fwd(x, residual, weight, eps=1e-6):
+    """Returns (y, r, rstd): r = x + residual (float32), y = rms_norm(r) * weight
+    in x's type, rstd the saved row factor."""
+    dt, x2, res2, w = _add_rms_args(x, residual, weight)
+    rows, cols = x2.shape
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    r = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    N.check(N.load().oxc_add_rms_norm_fwd(
+        x2.data_ptr(), x2.stride(0), res2.data_ptr(), res2.stride(0), w.data_ptr(), y.data_ptr(),
+        r.data_ptr(), rstd.data_ptr(), rows, cols, dt, float(eps), _stream()), "add_rms_norm")
+    return y, r, rstd
+
+
+def add_rms_norm_bwd(r, weight, rstd, dy, dr=None, grad_mode="ref"):
+    """Returns (dx, dresidual, dweight) for dy (the type of y) and dr (float32,
+    None = zero); in float32 dx and dresidual are one tensor."""
+    dt = _dtype_id("dy", dy)
+    _operand("r", r, dy.shape, torch.float32, dy.device)
+    r, dy2, w = dense(r), _rows2d(dy), dense(weight)
+    rows, cols = dy2.shape
+    if dr is not None:
+        _operand("dr", dr, r.shape, torch.float32, r.device)
+        dr = _rows2d(dr)
+    dres = torch.empty_like(r)
+    dx = dres if dt == N.F32 else torch.empty(r.shape, dtype=dy.dtype, device=r.device)
+    dw = torch.empty(cols, dtype=torch.float32, device=r.device)
+    L = N.load()
+    ws = _workspace(L.oxc_add_rms_norm_bwd_workspace_size(rows, cols), r.device)
+    N.check(L.oxc_add_rms_norm_bwd(
+        r.data_ptr(), w.data_ptr(), rstd.data_ptr(), dy2.data_ptr(), dy2.stride(0), _ptr(dr),
+        0 if dr is None else dr.stride(0), dres.data_ptr(), dx.data_ptr(), dw.data_ptr(), rows,
+        cols, dt, _MODES[grad_mode], ws.data_ptr(), ws.numel(), _stream()),
+        "add_rms_norm backward")
+    return dx, dres, dw
+
+
+class _AddRMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps, grad_mode):
+        y, r, rstd = add_rms_norm_fwd(x, residual, weight, eps)
+        ctx.save_for_backward(r, weight, rstd)
+        ctx.grad_mode, ctx.dtype = grad_mode, x.dtype
+        ctx.set_materialize_grads(False)
+        return y, r
+
+    @staticmethod
+    def backward(ctx, dy, dr):
+        r, weight, rstd = ctx.saved_tensors
+        if dy is None:  # only the residual stream was used
+            if dr is None:
+                return None, None, None, None, None
+            return dr.to(ctx.dtype), dr, torch.zeros_like(weight), None, None
+        dx, dres, dw = add_rms_norm_bwd(r, weight, rstd, dy, dr, ctx.grad_mode)
+        return dx, dres, dw, None, None
+
+
+def add_rms_norm(x, residual, weight, eps=1e-6, grad_mode="ref"):
+    """The residual's addition and the norm after it in one kernel each way:
+    returns (y, r) with r = x + residual and y = rms_norm(r, weight, eps).
+
+    x [..., cols] is float32 or bfloat16 and y has its type; residual and r, the
+    residual stream, and weight [cols] are float32.  Rows may be strided."""
+    if grad_mode not in _MODES:
+        raise ValueError(f"invalid argument: unknown grad mode {grad_mode!r}")
+    return _AddRMSNorm.apply(x, residual, weight, eps, grad_mode)
+
+
+def add_rms_norm_quant(x, residual, weight, eps=1e-6, block=128):
+    """add_rms_norm with y in 8 bits: returns (q, scale, r).
+
+    Each row is cut into blocks of 128 columns (``block=None``: one block a
+    row); scale [..., blocks] is max(amax(|y|) / 448, 2^-126) of a block and q,
+    of type float8_e4m3fn, is y / scale rounded to nearest, so y is q * scale.
+    For inference: it has no gradient."""
+    dt, x2, res2, w = _add_rms_args(x, residual, weight)
+    if block not in (128, None):
+        raise ValueError(f"invalid argument: block must be 128 or None, got {block}")
+    rows, cols = x2.shape
+    blocks = -(-cols // block) if block else 1
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(*x.shape[:-1], blocks, dtype=torch.float32, device=x.device)
+    r = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+    N.check(N.load().oxc_add_rms_norm_quant(
+        x2.data_ptr(), x2.stride(0), res2.data_ptr(), res2.stride(0), w.data_ptr(), q.data_ptr(),
+        scale.data_ptr(), r.data_ptr(), rows, cols, block or 0, dt, float(eps), _stream()),
+        "add_rms_norm_quant")
+    return q, scale, r
+
+
+# ---- gated linear recurrence ---------------------------------------------------------------
+
+def _sequence(t):
+    """A [batch, length, dim] operand whose last dim is dense; others are copied."""
+    return t if t.shape[2] <= 1 or t.stride(2) == 1 else _dense_any(t)
+
+
+def _starts_tensor(starts, x):
+    if starts is None:
+        return None
+    if isinstance(starts, torch.Tensor) and starts.dtype == torch.bool:
+        starts = starts.view(torch.uint8)
+    _operand("starts", starts, x.shape[:2], torch.uint8, x.device)
+    return starts.contiguous()
+
+
+def gated_scan_fwd(x, gate, h0=None, starts=None, save=True):
+    """Returns (h, last, carry); carry (None without ``save``) is what the VJP needs."""
+    dt = _dtype_id("x", x)
+    if x.dim() != 3:
+        raise ValueError(f"invalid argument: gated_scan expects [batch, length, dim], got {list(x.shape)}")
+    _operand("gate", gate, x.shape, x.dtype, x.device)
+    B, T, D = x.shape
+    x, gate, starts = _sequence(x), _sequence(gate), _starts_tensor(starts, x)
+    if h0 is not None:
+        _operand("h0", h0, (B, D), torch.float32, x.device)
+        h0 = dense(h0)
+    L = N.load()
+    h = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
+    last = torch.empty(B, D, dtype=torch.float32, device=x.device)
+    carry = None
+    if save:
+        carry = torch.empty(L.oxc_gated_scan_carry_size(B, T, D), dtype=torch.float32, device=x.device)
+    ws = _workspace(L.oxc_gated_scan_workspace_size(B, T, D), x.device)
+    N.check(L.oxc_gated_scan_fwd(
+        x.data_ptr(), x.stride(0), x.stride(1), gate.data_ptr(), gate.stride(0), gate.stride(1),
+        _ptr(starts), _ptr(h0), h.data_ptr(), last.data_ptr(), _ptr(carry), B, T, D, dt,
+        ws.data_ptr(), ws.numel(), _stream()), "gated_scan")
+    return h, last, carry
+
+
+def gated_scan_bwd(x, gate, carry, dh=None, dlast=None, starts=None):
+    """Returns (dx, dgate, dh0) for the gradients of h and of the last state
+    (None = zero)."""
+    dt = _dtype_id("x", x)
+    B, T, D = x.shape
+    x, gate, starts = _sequence(x), _sequence(gate), _starts_tensor(starts, x)
+    if dh is not None:
+        _operand("dh", dh, x.shape, x.dtype, x.device)
+        dh = _sequence(dh)
+    if dlast is not None:
+        _operand("dlast", dlast, (B, D), torch.float32, x.device)
+        dlast = dense(dlast)
+    L = N.load()
+    dx = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
+    dgate = torch.empty_like(dx)
+    dh0 = torch.empty(B, D, dtype=torch.float32, device=x.device)
+    ws = _workspace(L.oxc_gated_scan_workspace_size(B, T, D), x.device)
+    dsb, dst = (0, 0) if dh is None else dh.stride()[:2]
+    N.check(L.oxc_gated_scan_bwd(
+        x.data_ptr(), x.stride(0), x.stride(1), gate.data_ptr(), gate.stride(0), gate.stride(1),
+        _ptr(starts), carry.data_ptr(), _ptr(dh), dsb, dst, _ptr(dlast), dx.data_ptr(),
+        dgate.data_ptr(), dh0.data_ptr(), B, T, D, dt, ws.data_ptr(), ws.numel(), _stream()),
+        "gated_scan backward")
+    return dx, dgate, dh0
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, h0, starts):
+        h, last, carry = gated_scan_fwd(x, gate, h0, starts)
+        ctx.save_for_backward(x, gate, carry, starts)
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    def backward(ctx, dh, dlast):
+        x, gate, carry, starts = ctx.saved_tensors
+        if dh is None and dlast is None:
+            return None, None, None, None
+        dx, dgate, dh0 = gated_scan_bwd(x, gate, carry, dh, dlast, starts)
+        return dx, dgate, dh0 if ctx.needs_input_grad[2] else None, None
+
+
+def gated_scan(x, gate, h0=None, starts=None):
+    """The gated linear recurrence over dim 1 of x [batch, length, dim]:
+    h_t = a_t h_{t-1} + (1 - a_t) x_t with a = sigmoid(gate).  Returns (h, last),
+    last [batch, dim] being the state after the last token.
+
+    x and gate have one type (float32 or bfloat16) and any batch and time
+    strides, so halves of one projection need no copy; the state h0 (zero if
+    None) and last are float32.  ``starts`` (bool [batch, length]) marks where a
+    new sequence begins in a packed row: the state before such a token is zero."""
+    grads = (x, gate) if h0 is None else (x, gate, h0)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in grads):
+        return _GatedScan.apply(x, gate, h0, starts)
+    return gated_scan_fwd(x, gate, h0, starts, save=False)[:2]
+
+
+def gated_step(x, gate, state, out=None):
+    """One token of gated_scan for x, gate [batch, dim]: writes the state after
+    it to ``out`` (``state`` itself if None) and returns h, that state in x's
+    type.  For inference: it has no gradient."""
+    dt = _dtype_id("x", x)
+    if x.dim() != 2:
+        raise ValueError(f"invalid argument: gated_step expects [batch, dim], got {list(x.shape)}")
+    _operand("gate", gate, x.shape, x.dtype, x.device)
+    _operand("state", state, x.shape, torch.float32, x.device)
+    if out is None:
+        out = state
+    else:
+        _operand("out", out, x.shape, torch.float32, x.device)
+    if not (state.is_contiguous() and out.is_contiguous()):
+        raise ValueError("invalid argument: state and out must be contiguous")
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad):
+        raise ValueError("invalid argument: gated_step has no gradient; train with gated_scan")
+    x, gate = _rows2d(x), _rows2d(gate)
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    N.check(N.load().oxc_gated_step(
+        x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0), state.data_ptr(),
+        out.data_ptr(), h.data_ptr(), x.shape[0], x.shape[1], dt, _stream()), "gated_step")
+    return h
+
+
+# ---- distillation ------------------------------------------------------------------------
+
+def distill_loss_fwd(logits, teacher_logits, teacher_ids, temperature=1.0, total_rows=None,
+                     grad=True, grad_loss=None, flag=None):
+    """Returns (loss[1], dlogits): the gradient (times grad_loss[0] if given)
+    comes from the same pass; None without ``grad``."""
+    dt = _dtype_id("logits", logits)
+    if logits.dim() < 2:
+        raise ValueError(f"invalid argument: distill_loss expects [n, classes] logits, got {list(logits.shape)}")
+    if not isinstance(teacher_ids, torch.Tensor) or teacher_ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError("invalid argument: teacher_ids must be an int64 or int32 tensor")
+    if not isinstance(teacher_logits, torch.Tensor) or teacher_logits.dtype not in _DTYPES:
+        raise ValueError("invalid argument: teacher_logits must be a float32 or bfloat16 tensor")
+    if teacher_ids.shape[:-1] != logits.shape[:-1] or teacher_ids.dim() != logits.dim():
+        raise ValueError(f"shape mismatch: teacher_ids {list(teacher_ids.shape)} vs logits {list(logits.shape)}")
+    tl = _dense_any(teacher_logits.detach()).to(torch.float32)
+    ti = teacher_ids.to(torch.int64).contiguous()
+    _operand("teacher_ids", ti, ti.shape, torch.int64, logits.device)
+    _operand("teacher_logits", tl, ti.shape, torch.float32, logits.device)
+    x = _rows2d(logits)
+    rows, vocab = x.shape
+    loss = torch.empty(1, dtype=torch.float32, device=x.device)
+    row_loss = torch.empty(rows, dtype=torch.float32, device=x.device)
+    dlogits = torch.empty(logits.shape, dtype=x.dtype, device=x.device) if grad else None
+    N.check(N.load().oxc_distill_loss(
+        x.data_ptr(), x.stride(0), tl.data_ptr(), ti.data_ptr(), ti.shape[-1], float(temperature),
+        _ptr(grad_loss), loss.data_ptr(), row_loss.data_ptr(), _ptr(dlogits), rows, vocab,
+        int(total_rows or rows), dt, _ptr(flag), _stream()), "distill_loss")
+    return loss, dlogits
+
+
+class _DistillLoss(torch.autograd.Function):
+    """The forward pass leaves the gradient for a loss gradient of 1; backward
+    hands it out, scaled in place on the device if it is another.  A second
+    backward (retain_graph) computes it again."""
+
+    @staticmethod
+    def forward(ctx, logits, teacher_logits, teacher_ids, temperature, total_rows):
+        loss, ctx.dlogits = distill_loss_fwd(logits, teacher_logits, teacher_ids, temperature, total_rows)
+        ctx.save_for_backward(logits, teacher_logits, teacher_ids)
+        ctx.args = temperature, total_rows
+        return loss.reshape(())
+
+    @staticmethod
+    def backward(ctx, g):
+        logits, teacher_logits, teacher_ids = ctx.saved_tensors
+        g = g.reshape(1).to(torch.float32).contiguous()
+        d, ctx.dlogits = ctx.dlogits, None
+        if d is None:
+            d = distill_loss_fwd(logits, teacher_logits, teacher_ids, *ctx.args, grad_loss=g)[1]
+        else:
+            N.check(N.load().oxc_scale_by(d.data_ptr(), d.numel(), _DTYPES[d.dtype], g.data_ptr(),
+                                          _stream()), "distill_loss backward")
+        return d, None, None, None, None
+
+
+def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, total_rows=None):
+    """Distillation from a teacher's top logits: temperature^2 times the mean over
+    rows of KL(p || q), p the softmax of teacher_logits / temperature over the
+    row's entries and q the student's softmax of logits / temperature over the
+    whole vocabulary.
+
+    logits [..., vocab] float32 or bfloat16; teacher_logits and teacher_ids
+    (int64 or int32) [..., top] with the same leading dims.  An entry with a
+    negative id or a -inf logit is absent; a row without entries adds 0 to the
+    mean and has a zero gradient.  An id >= vocab makes the loss NaN.
+    total_rows: the divisor of the mean (the rows of this call if None), as in
+    a sharded batch.  The gradient reaches logits only."""
+    if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
+        return _DistillLoss.apply(logits, teacher_logits, teacher_ids, temperature, total_rows)
+    return distill_loss_fwd(logits, teacher_logits, teacher_ids, temperature, total_rows,
+                            grad=False)[0].reshape(())
+
+
+# ---- verification of drafted tokens --------------------------------------------------------
+
+def verify_draft(target, draft, tokens, uniform, race, lengths=None, flag=None):
+    """Which drafted tokens the target keeps, and the token after them, from given
+    random numbers.  Returns (out [batch, drafted + 1], accepted [batch]), int64.
+
+    target [batch, drafted + 1, vocab] and draft [batch, drafted, vocab] are
+    float32 probabilities (None for draft: each token was drafted with
+    probability 1); tokens [batch, drafted] int64, of which lengths[b] (all if
+    None) count.  Token k is kept while uniform[b, k] * q < p.  out[b] holds the
+    accepted[b] kept tokens, then the token sampled after them as the first
+    argmax of max(p - q, 0) / race[b] (p / race[b] when all were kept or nothing
+    is left), then -1.  uniform [batch, drafted] is in [0, 1), race [batch,
+    vocab] holds exponential variates.  Tokens outside the vocabulary are not
+    kept, and recorded in ``flag`` (int32[4], zeroed by the caller) if given."""
+    _require_cuda_f32("target", target)
+    _dtype_id("target", target)
+    if target.dim() != 3 or target.shape[1] < 1:
+        raise ValueError("invalid argument: verify_draft expects target [batch, drafted + 1, vocab], "
+                         f"got {list(target.shape)}")
+    B, K, V = target.shape[0], target.shape[1] - 1, target.shape[2]
+    dev = target.device
+    if draft is not None:
+        _operand("draft", draft, (B, K, V), torch.float32, dev)
+        draft = _sequence(draft)
+    _operand("tokens", tokens, (B, K), torch.int64, dev)
+    _operand("uniform", uniform, (B, K), torch.float32, dev)
+    _operand("race", race, (B, V), torch.float32, dev)
+    if lengths is not None:
+        _operand("lengths", lengths, (B,), torch.int64, dev)
+        lengths = lengths.contiguous()
+    if flag is not None:
+        _operand("flag", flag, (4,), torch.int32, dev)
+    target, tokens, uniform, race = _sequence(target), tokens.contiguous(), dense(uniform), dense(race)
+    out = torch.empty(B, K + 1, dtype=torch.int64, device=dev)
+    accepted = torch.empty(B, dtype=torch.int64, device=dev)
+    qsb, qsk = (0, 0) if draft is None else draft.stride()[:2]
+    N.check(N.load().oxc_verify_draft(
+        target.data_ptr(), target.stride(0), target.stride(1), _ptr(draft), qsb, qsk,
+        tokens.data_ptr(), _ptr(lengths), uniform.data_ptr(), race.data_ptr(), B, K, V,
+        out.data_ptr(), accepted.data_ptr(), _ptr(flag), _stream()), "verify_draft")
+    return out, accepted
