@@ -18,92 +18,495 @@
 // each chunk of kScanChunk tokens, so the VJP does not read h back: 5 elements
 // of traffic per token and channel instead of 6, and no rounding of h to bf16
 // in the gradient.
+//
+// Both kernels cut the sequence into chunks of 64 tokens and the channels into
+// tiles, one CTA each.  h_t = a_t h_{t-1} + v_t is an affine map of the state
+// and maps compose, so a CTA first reduces its chunk to one map per channel (A,
+// H), publishes it, finds the state that enters the chunk, and then runs the
+// recurrence from it on the values that it kept in registers: x and gate are
+// read once.  The VJP's mu runs through the same A from the other end.
+//
+// The state that enters a chunk (Chain, below): chunks form groups of 16.  A
+// chunk applies, one after the other, the maps of the chunks before it in its
+// group to the state entering the group; that one in turn comes from the
+// nearest group whose entering state is known and the group maps between.  So
+// the number of dependent steps is length / 1024, the reads per chunk are at
+// most 15 maps and a few group words, and since every state is defined by one
+// fixed sequence of operations -- whoever computes it, from however far back --
+// the results do not depend on timing.
 #include <algorithm>
 
+#include "pipeline.cuh"
 #include "typed.cuh"
 
 namespace oxc {
 
-constexpr int kScanChunk = 64;
+constexpr int kScanWarps = 8;
+constexpr int kScanSteps = 8;                        // tokens per warp
+constexpr int kScanChunk = kScanWarps * kScanSteps;  // tokens per CTA
+constexpr int kScanGroup = 16;                       // chunks per group
 
 // A [batch, length, dim] operand: the last dim dense, strides in elements.
 template <typename T>
 struct SeqView {
   const T* p;
   int64_t sb, st;
-  __device__ __forceinline__ const T* at(int64_t b, int64_t t, int64_t d) const {
-    return p + b * sb + t * st + d;
+};
+
+// a = sigmoid(g) and b = 1 - a, both relatively accurate (b is not formed by
+// subtraction, which would lose it for large gates): with e = exp(-|g|) they
+// are 1 / (1 + e) and e / (1 + e).  exp(-|g|) = 2^t, t = -|g| log2(e) in two
+// parts: ex2 takes the rounded one, the rest enters to first order.
+__device__ __forceinline__ void gate_pair(float g, float& a, float& b) {
+  const float n = -fabsf(g);
+  const float t = n * 1.44269502f;
+  const float lo = fmaf(n, 1.44269502f, -t) + n * 1.92596299e-8f;
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  e = t < -126.0f ? 0.0f : fmaf(e, lo * 0.693147181f, e);  // (an infinite t has lo = NaN)
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  const float er = e * r;
+  a = g > 0.0f ? r : er;
+  b = g > 0.0f ? er : r;
+}
+
+// ---- maps of the state ---------------------------------------------------------------
+//
+// s -> A s + H, A a product of sigmoids and so never negative.  A = -0 marks a
+// map that forgets its argument (a sequence starts inside): it is selected, not
+// multiplied, and keeps its mark in compositions.
+__device__ __forceinline__ bool forgets(float A) { return __float_as_uint(A) == 0x80000000u; }
+__device__ __forceinline__ float map_apply(float A, float H, float s) {
+  return forgets(A) ? H : fmaf(A, s, H);
+}
+// (A, H) after (A1, H1)
+__device__ __forceinline__ void map_compose(float& A, float& H, float A1, float H1) {
+  if (!forgets(A)) {
+    H = fmaf(A, H1, H);
+    A = forgets(A1) ? -0.0f : A * A1;
+  }
+}
+
+// ---- the state that enters a chunk -----------------------------------------------------
+//
+// Words of 64 bits, written once and read whole, so a word carries its own
+// "ready": a map (A low, H high) is empty while A's bits are all ones (no A has
+// them: a NaN is stored as 0x7fffffff), an entering state (tag low, state high)
+// while the tag's are.  The caller's workspace is set to all ones before the
+// launch.  Chunks are counted along the direction of the scan.
+struct Chain {
+  unsigned int* ticket;       // the next tile to hand out, less one
+  unsigned long long* map;    // [chunks, batch * dim]
+  unsigned long long* group;  // [groups, batch * dim] the map of a whole group
+  unsigned long long* enter;  // [groups, batch * dim] the state entering it
+  int64_t stride;             // batch * dim
+};
+
+__device__ __forceinline__ unsigned long long word_load(const unsigned long long* p) {
+  unsigned long long v;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void word_store(unsigned long long* p, float lo, float hi) {
+  const unsigned long long v =
+      ((unsigned long long)__float_as_uint(hi) << 32) | __float_as_uint(lo);
+  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
+}
+__device__ __forceinline__ void map_store(unsigned long long* p, float A, float H) {
+  word_store(p, A != A ? __uint_as_float(0x7fffffffu) : A, H);
+}
+__device__ __forceinline__ bool word_ready(unsigned long long w) {
+  return (uint32_t)w != 0xffffffffu;
+}
+__device__ __forceinline__ float word_lo(unsigned long long w) { return __uint_as_float((uint32_t)w); }
+__device__ __forceinline__ float word_hi(unsigned long long w) {
+  return __uint_as_float((uint32_t)(w >> 32));
+}
+
+// Bounds a spin: false once kWaitTimeoutNs have passed since the first call.
+struct Patience {
+  unsigned long long t0 = 0;
+  __device__ __forceinline__ bool more() {
+    const unsigned long long t = globaltimer_ns();
+    if (t0 == 0) t0 = t;
+    if (t - t0 <= kWaitTimeoutNs) return true;
+    atomicOr(&g_kernel_error, OXC_KERR_PIPELINE_TIMEOUT);
+    return false;
   }
 };
 
-// a = sigmoid(g) and b = 1 - a, both to f32 accuracy (b is not formed by
-// subtraction, which would lose it for large gates).
-__device__ __forceinline__ void gate_pair(float g, float& a, float& b) {
-  const float e = expf(-fabsf(g));
-  const float big = __frcp_rn(1.0f + e);
-  const float small = e * big;
-  a = g >= 0.0f ? big : small;
-  b = g >= 0.0f ? small : big;
-  if (g != g) a = b = g;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(128) scan_fwd_kernel(SeqView<T> x, SeqView<T> gate,
-                                                       const uint8_t* __restrict__ starts,
-                                                       const float* __restrict__ h0,
-                                                       T* __restrict__ h, float* __restrict__ last,
-                                                       float* __restrict__ carry, int64_t length,
-                                                       int64_t dim) {
-  const int64_t d = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t bi = blockIdx.y;
-  if (d >= dim) return;
-  const int64_t chunks = (length + kScanChunk - 1) / kScanChunk;
-  float s = h0 ? h0[bi * dim + d] : 0.0f;
-  for (int64_t t = 0; t < length; ++t) {
-    if (carry && t % kScanChunk == 0) carry[(bi * chunks + t / kScanChunk) * dim + d] = s;
-    float a, b;
-    gate_pair(to_f32(*gate.at(bi, t, d)), a, b);
-    const float v = b * to_f32(*x.at(bi, t, d));
-    s = starts && starts[bi * length + t] ? v : fmaf(a, s, v);
-    h[(bi * length + t) * dim + d] = from_f32<T>(s);
+// The word at p once it is ready; a NaN map if that takes too long.
+__device__ __forceinline__ unsigned long long word_wait(const unsigned long long* p,
+                                                        unsigned long long w) {
+  Patience patience;
+  while (!word_ready(w)) {
+    if (!patience.more()) return 0x7fffffff7fffffffull;
+    w = word_load(p);
   }
-  if (last) last[bi * dim + d] = s;
+  return w;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(128) scan_bwd_kernel(
+// The state entering group g >= 0 at channel offset `off`.
+__device__ __forceinline__ float chain_enter_group(const Chain& c, int64_t g, int64_t off,
+                                                   float first) {
+  constexpr int kBack = 4;
+  Patience patience;
+  while (g > 0) {
+    unsigned long long e[kBack], m[kBack];
+#pragma unroll
+    for (int i = 0; i < kBack; ++i) {  // e[i]: entering g - i; m[i]: the group before it
+      e[i] = g - i > 0 ? word_load(c.enter + (g - i) * c.stride + off) : 0ull;
+      m[i] = g - i > 0 ? word_load(c.group + (g - i - 1) * c.stride + off) : 0ull;
+    }
+    int at = kBack;
+#pragma unroll
+    for (int i = kBack - 1; i >= 0; --i) {
+      if (word_ready(e[i])) at = i;                         // nearest known state so far
+      else if (at < kBack && !word_ready(m[i])) at = kBack;  // a map missing on the way
+    }
+    if (at < kBack) {
+      float s = 0.0f;
+#pragma unroll
+      for (int i = kBack - 1; i >= 0; --i) {
+        if (i == at) s = g - i > 0 ? word_hi(e[i]) : first;
+        else if (i < at) s = map_apply(word_lo(m[i]), word_hi(m[i]), s);
+      }
+      return s;
+    }
+    if (!patience.more()) return __uint_as_float(0x7fffffffu);
+  }
+  return first;
+}
+
+// Called by one thread per channel with the map (A, H) of chunk k: publishes what
+// later chunks need and returns the state entering chunk k.
+__device__ __forceinline__ float chain_state(const Chain& c, int64_t k, int64_t chunks,
+                                             int64_t off, float A, float H, float first) {
+  constexpr int kBatch = 5;  // maps in flight
+  const int64_t g = k / kScanGroup, k0 = g * kScanGroup;
+  const bool ends_group = k + 1 - k0 == kScanGroup;
+  if (k + 1 < chunks) {
+    if (!ends_group) {
+      map_store(c.map + k * c.stride + off, A, H);
+    } else {
+      // the group's map, composed from its last chunk backwards
+      for (int64_t j = k - 1; j >= k0; j -= kBatch) {
+        unsigned long long w[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) w[i] = word_load(c.map + (j - i) * c.stride + off);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          w[i] = word_wait(c.map + (j - i) * c.stride + off, w[i]);
+          map_compose(A, H, word_lo(w[i]), word_hi(w[i]));
+        }
+      }
+      map_store(c.group + g * c.stride + off, A, H);
+    }
+  }
+  float s = chain_enter_group(c, g, off, first);
+  if (k == k0 && g > 0 && k + 1 < chunks) word_store(c.enter + g * c.stride + off, 0.0f, s);
+  for (int64_t j = k0; j < k; j += kBatch) {
+    unsigned long long w[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      w[i] = j + i < k ? word_load(c.map + (j + i) * c.stride + off) : 0ull;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (j + i < k) {
+        w[i] = word_wait(c.map + (j + i) * c.stride + off, w[i]);
+        s = map_apply(word_lo(w[i]), word_hi(w[i]), s);
+      }
+    }
+  }
+  return s;
+}
+static_assert((kScanGroup - 1) % 5 == 0, "a group's maps are read in batches of 5");
+
+// Which tile a CTA takes.  Tiles are handed out in the order of the scan, every
+// batch row and channel tile of a chunk before the next chunk, so the tiles that
+// one waits for are always already running.
+struct Tile {
+  int64_t chunk, b;
+  int64_t d0;
+};
+__device__ __forceinline__ Tile take_tile(const Chain& c, int64_t batch, int64_t dtiles,
+                                          int channels) {
+  __shared__ unsigned int mine;
+  if (threadIdx.x == 0) mine = c.ticket ? atomicAdd(c.ticket, 1u) + 1u : blockIdx.x;
+  __syncthreads();
+  const int64_t id = mine, per = batch * dtiles, chunk = id / per, rest = id - chunk * per;
+  return {chunk, rest / dtiles, (rest % dtiles) * channels};
+}
+
+// VW channels of one token, in f32.  VEC: consecutive ones, in one load; else
+// 32 apart (lane l takes l, l + 32, ...), each guarded.
+template <typename T, int VW, bool VEC>
+struct Lane {
+  static constexpr int kChannels = 32 * VW;
+  int64_t d;   // the lane's first channel
+  int live;    // how many of its channels exist
+  __device__ __forceinline__ Lane(int64_t d0, int64_t dim) {
+    const int lane = threadIdx.x & 31;
+    d = VEC ? d0 + lane * VW : d0 + lane;
+    live = 0;
+#pragma unroll
+    for (int k = 0; k < VW; ++k) live += d + (VEC ? k : 32 * k) < dim;
+  }
+  __device__ __forceinline__ int channel(int k) const {  // within the tile
+    const int lane = threadIdx.x & 31;
+    return VEC ? lane * VW + k : lane + 32 * k;
+  }
+  __device__ __forceinline__ void load(float (&v)[VW], const T* row) const {
+    if constexpr (VEC) {
+      if (live) load_as_f32<VW>(v, row + d);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        float one[1] = {0.0f};
+        if (k < live) load_as_f32<1>(one, row + d + 32 * k);
+        v[k] = one[0];
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* row, const float (&v)[VW]) const {
+    if constexpr (VEC) {
+      if (live) store_from_f32<VW>(row + d, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        const float one[1] = {v[k]};
+        if (k < live) store_from_f32<1>(row + d + 32 * k, one);
+      }
+    }
+  }
+};
+
+// The warp's tokens at which a sequence starts, a bit each.
+__device__ __forceinline__ unsigned int start_bits(const uint8_t* starts, int64_t row, int64_t t0,
+                                                   int64_t length) {
+  if (!starts) return 0u;
+  const int lane = threadIdx.x & 31;
+  const bool s = lane < kScanSteps && t0 + lane < length && starts[row * length + t0 + lane];
+  return __ballot_sync(0xffffffffu, s);
+}
+
+template <typename T, int VW, bool VEC>
+__global__ void __launch_bounds__(kScanWarps * 32, 2) scan_fwd_kernel(
+    SeqView<T> x, SeqView<T> gate, const uint8_t* __restrict__ starts,
+    const float* __restrict__ h0, T* __restrict__ h, float* __restrict__ last,
+    float* __restrict__ carry, Chain chain, int64_t batch, int64_t length, int64_t dim,
+    int64_t chunks, int64_t dtiles) {
+  using L = Lane<T, VW, VEC>;
+  __shared__ float mapA[kScanWarps][L::kChannels], mapH[kScanWarps][L::kChannels];
+  const Tile tile = take_tile(chain, batch, dtiles, L::kChannels);
+  const L lane(tile.d0, dim);
+  const int warp = threadIdx.x >> 5;
+  const int64_t t0 = tile.chunk * kScanChunk + warp * kScanSteps;
+  const int steps = (int)max((int64_t)0, min((int64_t)kScanSteps, length - t0));
+  const unsigned int fresh = start_bits(starts, tile.b, t0, length);
+
+  float a[kScanSteps][VW], v[kScanSteps][VW];
+#pragma unroll
+  for (int i = 0; i < kScanSteps; ++i) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) a[i][k] = v[i][k] = 0.0f;
+    if (i < steps) {
+      lane.load(a[i], gate.p + tile.b * gate.sb + (t0 + i) * gate.st);
+      lane.load(v[i], x.p + tile.b * x.sb + (t0 + i) * x.st);
+    }
+  }
+  float A[VW], H[VW];
+#pragma unroll
+  for (int k = 0; k < VW; ++k) { A[k] = 1.0f; H[k] = 0.0f; }
+#pragma unroll
+  for (int i = 0; i < kScanSteps; ++i) {
+    if (i < steps) {
+      const bool s = (fresh >> i) & 1u;
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        float b;
+        gate_pair(a[i][k], a[i][k], b);
+        v[i][k] *= b;
+        H[k] = s ? v[i][k] : fmaf(a[i][k], H[k], v[i][k]);
+        A[k] = s ? -0.0f : A[k] * a[i][k];
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < VW; ++k) {
+    mapA[warp][lane.channel(k)] = A[k];
+    mapH[warp][lane.channel(k)] = H[k];
+  }
+  __syncthreads();
+  const int c = threadIdx.x;
+  if (c < L::kChannels && tile.d0 + c < dim) {
+    const int64_t off = tile.b * dim + tile.d0 + c;
+    float s = h0 ? h0[off] : 0.0f;
+    if (chunks > 1) {
+      float tA = mapA[kScanWarps - 1][c], tH = mapH[kScanWarps - 1][c];
+#pragma unroll
+      for (int w = kScanWarps - 2; w >= 0; --w) map_compose(tA, tH, mapA[w][c], mapH[w][c]);
+      s = chain_state(chain, tile.chunk, chunks, off, tA, tH, s);
+    }
+    if (carry) carry[(tile.b * chunks + tile.chunk) * dim + tile.d0 + c] = s;
+#pragma unroll
+    for (int w = 0; w < kScanWarps; ++w) {  // mapH becomes the state entering warp w
+      const float next = map_apply(mapA[w][c], mapH[w][c], s);
+      mapH[w][c] = s;
+      s = next;
+    }
+  }
+  __syncthreads();
+  float s[VW];
+#pragma unroll
+  for (int k = 0; k < VW; ++k) s[k] = mapH[warp][lane.channel(k)];
+#pragma unroll
+  for (int i = 0; i < kScanSteps; ++i) {
+    if (i < steps) {
+      const bool f = (fresh >> i) & 1u;
+#pragma unroll
+      for (int k = 0; k < VW; ++k) s[k] = f ? v[i][k] : fmaf(a[i][k], s[k], v[i][k]);
+      lane.store(h + (tile.b * length + t0 + i) * dim, s);
+    }
+  }
+  if (last && steps > 0 && t0 + steps == length) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k)
+      if (k < lane.live) last[tile.b * dim + tile.d0 + lane.channel(k)] = s[k];
+  }
+}
+
+template <typename T, int VW, bool VEC>
+__global__ void __launch_bounds__(kScanWarps * 32, 2) scan_bwd_kernel(
     SeqView<T> x, SeqView<T> gate, const uint8_t* __restrict__ starts,
     const float* __restrict__ carry, SeqView<T> dh, const float* __restrict__ dlast,
-    T* __restrict__ dx, T* __restrict__ dgate, float* __restrict__ dh0, int64_t length,
-    int64_t dim) {
-  const int64_t d = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t bi = blockIdx.y;
-  if (d >= dim) return;
-  const int64_t chunks = (length + kScanChunk - 1) / kScanChunk;
-  float mu = dlast ? dlast[bi * dim + d] : 0.0f;
-  for (int64_t c = chunks - 1; c >= 0; --c) {
-    const int64_t t0 = c * kScanChunk, t1 = min(length, t0 + kScanChunk);
-    float before[kScanChunk];  // the state before each token of the chunk
-    float s = carry[(bi * chunks + c) * dim + d];
-    for (int64_t t = t0; t < t1; ++t) {
-      float a, b;
-      gate_pair(to_f32(*gate.at(bi, t, d)), a, b);
-      if (starts && starts[bi * length + t]) s = 0.0f;
-      before[t - t0] = s;
-      s = fmaf(a, s, b * to_f32(*x.at(bi, t, d)));
-    }
-    for (int64_t t = t1 - 1; t >= t0; --t) {
-      float a, b;
-      gate_pair(to_f32(*gate.at(bi, t, d)), a, b);
-      const float lam = (dh.p ? to_f32(*dh.at(bi, t, d)) : 0.0f) + mu;
-      const float db = lam * b;
-      const int64_t o = (bi * length + t) * dim + d;
-      dx[o] = from_f32<T>(db);
-      dgate[o] = from_f32<T>(db * a * (before[t - t0] - to_f32(*x.at(bi, t, d))));
-      mu = starts && starts[bi * length + t] ? 0.0f : a * lam;
+    T* __restrict__ dx, T* __restrict__ dgate, float* __restrict__ dh0, Chain chain, int64_t batch,
+    int64_t length, int64_t dim, int64_t chunks, int64_t dtiles) {
+  using L = Lane<T, VW, VEC>;
+  // per warp: its map's A, the state's H and mu's H; then the state entering it
+  // from the left and the mu from the right
+  __shared__ float mapA[kScanWarps][L::kChannels], mapS[kScanWarps][L::kChannels],
+      mapM[kScanWarps][L::kChannels];
+  Tile tile = take_tile(chain, batch, dtiles, L::kChannels);
+  tile.chunk = chunks - 1 - tile.chunk;  // from the end of the sequence
+  const L lane(tile.d0, dim);
+  const int warp = threadIdx.x >> 5;
+  const int64_t t0 = tile.chunk * kScanChunk + warp * kScanSteps;
+  const int steps = (int)max((int64_t)0, min((int64_t)kScanSteps, length - t0));
+  const unsigned int fresh = start_bits(starts, tile.b, t0, length);
+
+  float g[kScanSteps][VW], v[kScanSteps][VW], lam[kScanSteps][VW];
+#pragma unroll
+  for (int i = 0; i < kScanSteps; ++i) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) g[i][k] = v[i][k] = lam[i][k] = 0.0f;
+    if (i < steps) {
+      lane.load(g[i], gate.p + tile.b * gate.sb + (t0 + i) * gate.st);
+      lane.load(v[i], x.p + tile.b * x.sb + (t0 + i) * x.st);
+      if (dh.p) lane.load(lam[i], dh.p + tile.b * dh.sb + (t0 + i) * dh.st);
     }
   }
-  if (dh0) dh0[bi * dim + d] = mu;
+  float a[kScanSteps][VW], b[kScanSteps][VW];
+  float A[VW], S[VW], M[VW];
+#pragma unroll
+  for (int k = 0; k < VW; ++k) { A[k] = 1.0f; S[k] = 0.0f; M[k] = 0.0f; }
+#pragma unroll
+  for (int i = 0; i < kScanSteps; ++i) {
+    if (i < steps) {
+      const bool s = (fresh >> i) & 1u;
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        gate_pair(g[i][k], a[i][k], b[i][k]);
+        S[k] = s ? b[i][k] * v[i][k] : fmaf(a[i][k], S[k], b[i][k] * v[i][k]);
+        A[k] = s ? -0.0f : A[k] * a[i][k];
+      }
+    }
+  }
+#pragma unroll
+  for (int i = kScanSteps - 1; i >= 0; --i) {
+    if (i < steps) {
+      const bool s = (fresh >> i) & 1u;
+#pragma unroll
+      for (int k = 0; k < VW; ++k) M[k] = s ? 0.0f : a[i][k] * (lam[i][k] + M[k]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < VW; ++k) {
+    mapA[warp][lane.channel(k)] = A[k];
+    mapS[warp][lane.channel(k)] = S[k];
+    mapM[warp][lane.channel(k)] = M[k];
+  }
+  __syncthreads();
+  // the mu of the chunk after this one and the state before it, by two sets of
+  // threads
+  const int c = threadIdx.x % L::kChannels, part = threadIdx.x / L::kChannels;
+  if (part < 2 && tile.d0 + c < dim) {
+    const int64_t off = tile.b * dim + tile.d0 + c;
+    if (part == 0) {
+      float m = dlast ? dlast[off] : 0.0f;
+      if (chunks > 1) {
+        float tA = mapA[0][c], tM = mapM[0][c];
+#pragma unroll
+        for (int w = 1; w < kScanWarps; ++w) map_compose(tA, tM, mapA[w][c], mapM[w][c]);
+        m = chain_state(chain, chunks - 1 - tile.chunk, chunks, off, tA, tM, m);
+      }
+#pragma unroll
+      for (int w = kScanWarps - 1; w >= 0; --w) {
+        const float next = map_apply(mapA[w][c], mapM[w][c], m);
+        mapM[w][c] = m;
+        m = next;
+      }
+    } else {
+      float s = carry[(tile.b * chunks + tile.chunk) * dim + tile.d0 + c];
+#pragma unroll
+      for (int w = 0; w < kScanWarps; ++w) {
+        const float next = map_apply(mapA[w][c], mapS[w][c], s);
+        mapS[w][c] = s;
+        s = next;
+      }
+    }
+  }
+  __syncthreads();
+  float s[VW], m[VW];
+#pragma unroll
+  for (int k = 0; k < VW; ++k) {
+    s[k] = mapS[warp][lane.channel(k)];
+    m[k] = mapM[warp][lane.channel(k)];
+  }
+#pragma unroll
+  for (int i = 0; i < kScanSteps; ++i) {
+    if (i < steps) {
+      const bool f = (fresh >> i) & 1u;
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        const float before = f ? 0.0f : s[k];
+        s[k] = fmaf(a[i][k], before, b[i][k] * v[i][k]);
+        v[i][k] = before - v[i][k];  // what d h_t / d a_t is
+      }
+    }
+  }
+#pragma unroll
+  for (int i = kScanSteps - 1; i >= 0; --i) {
+    if (i < steps) {
+      const bool f = (fresh >> i) & 1u;
+      float ox[VW], og[VW];
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        const float l = lam[i][k] + m[k];
+        ox[k] = l * b[i][k];
+        og[k] = ox[k] * a[i][k] * v[i][k];
+        m[k] = f ? 0.0f : a[i][k] * l;
+      }
+      const int64_t o = (tile.b * length + t0 + i) * dim;
+      lane.store(dx + o, ox);
+      lane.store(dgate + o, og);
+    }
+  }
+  if (dh0 && tile.chunk == 0 && warp == 0) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k)
+      if (k < lane.live) dh0[tile.b * dim + tile.d0 + lane.channel(k)] = m[k];
+  }
 }
 
 // One token: state_out (which may be state itself) and h = state_out rounded.
@@ -138,6 +541,90 @@ static oxc_status scan_check(const char* fn, int32_t dtype, int64_t batch, int64
 }
 
 static int64_t scan_chunks(int64_t length) { return (length + kScanChunk - 1) / kScanChunk; }
+static int64_t scan_groups(int64_t length) {
+  return (scan_chunks(length) + kScanGroup - 1) / kScanGroup;
+}
+
+// Lays the chain out in the workspace and empties it; a single chunk has none.
+static oxc_status scan_chain(const char* fn, int64_t batch, int64_t length, int64_t dim,
+                             void* workspace, size_t workspace_bytes, cudaStream_t s, Chain* c) {
+  const size_t need = oxc_gated_scan_workspace_size(batch, length, dim);
+  *c = Chain{nullptr, nullptr, nullptr, nullptr, batch * dim};
+  if (need == 0) return OXC_OK;
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    return fail(OXC_ERR_INVALID_ARGUMENT,
+                "invalid argument: %s needs a 16-byte aligned %zu-byte workspace, got %zu", fn,
+                need, workspace_bytes);
+  c->ticket = static_cast<unsigned int*>(workspace);
+  c->map = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + 16);
+  c->group = c->map + scan_chunks(length) * c->stride;
+  c->enter = c->group + scan_groups(length) * c->stride;
+  const cudaError_t e = cudaMemsetAsync(workspace, 0xff, need, s);
+  return e == cudaSuccess ? OXC_OK : cuda_fail(e, fn);
+}
+
+// VW channels of an operand in one access.
+template <typename T, int VW>
+static bool seq_vec(const void* p, int64_t sb, int64_t st, int64_t dim) {
+  return dim % VW == 0 && sb % VW == 0 && st % VW == 0 && aligned_to(p, VW * sizeof(T));
+}
+
+static oxc_status scan_grid(const char* fn, int64_t batch, int64_t length, int64_t dim,
+                            int channels, int64_t* dtiles, unsigned* grid) {
+  *dtiles = (dim + channels - 1) / channels;
+  const int64_t per = batch * *dtiles;
+  if (scan_chunks(length) > 0x7fffffff / per)
+    return fail(OXC_ERR_NOT_IMPLEMENTED, "not implemented: %s: [%lld, %lld, %lld]", fn,
+                (long long)batch, (long long)length, (long long)dim);
+  *grid = (unsigned)(scan_chunks(length) * per);
+  return OXC_OK;
+}
+
+template <typename T>
+static oxc_status scan_fwd_launch(const void* x, int64_t x_sb, int64_t x_st, const void* gate,
+                                  int64_t g_sb, int64_t g_st, const uint8_t* starts,
+                                  const float* h0, void* h, float* last, float* carry,
+                                  const Chain& chain, int64_t batch, int64_t length, int64_t dim,
+                                  cudaStream_t s) {
+  constexpr int VW = 4;
+  int64_t dtiles;
+  unsigned grid;
+  oxc_status st = scan_grid("gated_scan", batch, length, dim, 32 * VW, &dtiles, &grid);
+  if (st) return st;
+  const bool vec = seq_vec<T, VW>(x, x_sb, x_st, dim) && seq_vec<T, VW>(gate, g_sb, g_st, dim) &&
+                   seq_vec<T, VW>(h, 0, 0, dim);
+  const SeqView<T> xv{static_cast<const T*>(x), x_sb, x_st};
+  const SeqView<T> gv{static_cast<const T*>(gate), g_sb, g_st};
+  auto kernel = vec ? scan_fwd_kernel<T, VW, true> : scan_fwd_kernel<T, VW, false>;
+  kernel<<<grid, kScanWarps * 32, 0, s>>>(xv, gv, starts, h0, static_cast<T*>(h), last, carry,
+                                          chain, batch, length, dim, scan_chunks(length), dtiles);
+  return check_launch("oxc_gated_scan_fwd");
+}
+
+template <typename T>
+static oxc_status scan_bwd_launch(const void* x, int64_t x_sb, int64_t x_st, const void* gate,
+                                  int64_t g_sb, int64_t g_st, const uint8_t* starts,
+                                  const float* carry, const void* dh, int64_t dh_sb, int64_t dh_st,
+                                  const float* dlast, void* dx, void* dgate, float* dh0,
+                                  const Chain& chain, int64_t batch, int64_t length, int64_t dim,
+                                  cudaStream_t s) {
+  constexpr int VW = 2;
+  int64_t dtiles;
+  unsigned grid;
+  oxc_status st = scan_grid("gated_scan backward", batch, length, dim, 32 * VW, &dtiles, &grid);
+  if (st) return st;
+  const bool vec = seq_vec<T, VW>(x, x_sb, x_st, dim) && seq_vec<T, VW>(gate, g_sb, g_st, dim) &&
+                   seq_vec<T, VW>(dh, dh_sb, dh_st, dim) && seq_vec<T, VW>(dx, 0, 0, dim) &&
+                   seq_vec<T, VW>(dgate, 0, 0, dim);
+  const SeqView<T> xv{static_cast<const T*>(x), x_sb, x_st};
+  const SeqView<T> gv{static_cast<const T*>(gate), g_sb, g_st};
+  const SeqView<T> dv{static_cast<const T*>(dh), dh_sb, dh_st};
+  auto kernel = vec ? scan_bwd_kernel<T, VW, true> : scan_bwd_kernel<T, VW, false>;
+  kernel<<<grid, kScanWarps * 32, 0, s>>>(xv, gv, starts, carry, dv, dlast, static_cast<T*>(dx),
+                                          static_cast<T*>(dgate), dh0, chain, batch, length, dim,
+                                          scan_chunks(length), dtiles);
+  return check_launch("oxc_gated_scan_bwd");
+}
 
 }  // namespace oxc
 
@@ -150,9 +637,12 @@ int64_t oxc_gated_scan_carry_size(int64_t batch, int64_t length, int64_t dim) {
   return batch * scan_chunks(length) * dim;
 }
 
+// The same for both directions: a ticket, a map per chunk and channel, a map and
+// a state per group.
 size_t oxc_gated_scan_workspace_size(int64_t batch, int64_t length, int64_t dim) {
-  (void)batch; (void)length; (void)dim;
-  return 0;
+  if (batch <= 0 || length <= kScanChunk || dim <= 0) return 0;
+  return 16 + (size_t)(scan_chunks(length) + 2 * scan_groups(length)) * (size_t)batch *
+                  (size_t)dim * sizeof(unsigned long long);
 }
 
 oxc_status oxc_gated_scan_fwd(const void* x, int64_t x_sb, int64_t x_st, const void* gate,
@@ -173,18 +663,14 @@ oxc_status oxc_gated_scan_fwd(const void* x, int64_t x_sb, int64_t x_st, const v
   }
   if (!x || !gate || !h)
     return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: gated_scan: null pointer");
-  const dim3 grid((unsigned)((dim + 127) / 128), (unsigned)batch);
+  Chain chain;
+  st = scan_chain("gated_scan", batch, length, dim, workspace, workspace_bytes, s, &chain);
+  if (st) return st;
   if (dtype == OXC_BF16)
-    scan_fwd_kernel<bf16><<<grid, 128, 0, s>>>({static_cast<const bf16*>(x), x_sb, x_st},
-                                               {static_cast<const bf16*>(gate), g_sb, g_st},
-                                               starts, h0, static_cast<bf16*>(h), last, carry,
-                                               length, dim);
-  else
-    scan_fwd_kernel<float><<<grid, 128, 0, s>>>({static_cast<const float*>(x), x_sb, x_st},
-                                                {static_cast<const float*>(gate), g_sb, g_st},
-                                                starts, h0, static_cast<float*>(h), last, carry,
-                                                length, dim);
-  return check_launch("oxc_gated_scan_fwd");
+    return scan_fwd_launch<bf16>(x, x_sb, x_st, gate, g_sb, g_st, starts, h0, h, last, carry,
+                                 chain, batch, length, dim, s);
+  return scan_fwd_launch<float>(x, x_sb, x_st, gate, g_sb, g_st, starts, h0, h, last, carry, chain,
+                                batch, length, dim, s);
 }
 
 oxc_status oxc_gated_scan_bwd(const void* x, int64_t x_sb, int64_t x_st, const void* gate,
@@ -206,18 +692,14 @@ oxc_status oxc_gated_scan_bwd(const void* x, int64_t x_sb, int64_t x_st, const v
   }
   if (!x || !gate || !carry || !dx || !dgate)
     return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: gated_scan backward: null pointer");
-  const dim3 grid((unsigned)((dim + 127) / 128), (unsigned)batch);
+  Chain chain;
+  st = scan_chain("gated_scan backward", batch, length, dim, workspace, workspace_bytes, s, &chain);
+  if (st) return st;
   if (dtype == OXC_BF16)
-    scan_bwd_kernel<bf16><<<grid, 128, 0, s>>>(
-        {static_cast<const bf16*>(x), x_sb, x_st}, {static_cast<const bf16*>(gate), g_sb, g_st},
-        starts, carry, {static_cast<const bf16*>(dh), dh_sb, dh_st}, dlast,
-        static_cast<bf16*>(dx), static_cast<bf16*>(dgate), dh0, length, dim);
-  else
-    scan_bwd_kernel<float><<<grid, 128, 0, s>>>(
-        {static_cast<const float*>(x), x_sb, x_st}, {static_cast<const float*>(gate), g_sb, g_st},
-        starts, carry, {static_cast<const float*>(dh), dh_sb, dh_st}, dlast,
-        static_cast<float*>(dx), static_cast<float*>(dgate), dh0, length, dim);
-  return check_launch("oxc_gated_scan_bwd");
+    return scan_bwd_launch<bf16>(x, x_sb, x_st, gate, g_sb, g_st, starts, carry, dh, dh_sb, dh_st,
+                                 dlast, dx, dgate, dh0, chain, batch, length, dim, s);
+  return scan_bwd_launch<float>(x, x_sb, x_st, gate, g_sb, g_st, starts, carry, dh, dh_sb, dh_st,
+                                dlast, dx, dgate, dh0, chain, batch, length, dim, s);
 }
 
 oxc_status oxc_gated_step(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,

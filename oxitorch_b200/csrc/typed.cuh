@@ -31,14 +31,17 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 
 // VW consecutive elements as f32, evict-first; VW > 1 needs VW * sizeof(T)
-// alignment.  VW = 1, 4 (16 bytes of f32, 8 of bf16) or 8 (bf16 only).
+// alignment.  VW = 1, 2, 4, or 8 (bf16 only).
 template <int VW>
 __device__ __forceinline__ void load_as_f32(float (&d)[VW], const float* p) {
   if constexpr (VW == 4) {
     const float4 t = ld_stream(reinterpret_cast<const float4*>(p));
     d[0] = t.x; d[1] = t.y; d[2] = t.z; d[3] = t.w;
+  } else if constexpr (VW == 2) {
+    const float2 t = __ldcs(reinterpret_cast<const float2*>(p));
+    d[0] = t.x; d[1] = t.y;
   } else {
-    static_assert(VW == 1, "f32 vectors hold 1 or 4 elements");
+    static_assert(VW == 1, "f32 vectors hold 1, 2 or 4 elements");
     d[0] = ld_stream(p);
   }
 }
@@ -52,8 +55,11 @@ __device__ __forceinline__ void load_as_f32(float (&d)[VW], const bf16* p) {
   } else if constexpr (VW == 4) {
     const uint2 t = __ldcs(reinterpret_cast<const uint2*>(p));
     d[0] = bf16_lo(t.x); d[1] = bf16_hi(t.x); d[2] = bf16_lo(t.y); d[3] = bf16_hi(t.y);
+  } else if constexpr (VW == 2) {
+    const uint32_t t = __ldcs(reinterpret_cast<const uint32_t*>(p));
+    d[0] = bf16_lo(t); d[1] = bf16_hi(t);
   } else {
-    static_assert(VW == 1, "bf16 vectors hold 1, 4 or 8 elements");
+    static_assert(VW == 1, "bf16 vectors hold 1, 2, 4 or 8 elements");
     d[0] = bf16_lo(__ldcs(reinterpret_cast<const unsigned short*>(p)));
   }
 }
@@ -61,8 +67,10 @@ template <int VW>
 __device__ __forceinline__ void store_from_f32(float* p, const float (&d)[VW]) {
   if constexpr (VW == 4) {
     st_stream(reinterpret_cast<float4*>(p), make_float4(d[0], d[1], d[2], d[3]));
+  } else if constexpr (VW == 2) {
+    __stcs(reinterpret_cast<float2*>(p), make_float2(d[0], d[1]));
   } else {
-    static_assert(VW == 1, "f32 vectors hold 1 or 4 elements");
+    static_assert(VW == 1, "f32 vectors hold 1, 2 or 4 elements");
     st_stream(p, d[0]);
   }
 }
@@ -73,8 +81,10 @@ __device__ __forceinline__ void store_from_f32(bf16* p, const float (&d)[VW]) {
                                                    pack_bf16(d[4], d[5]), pack_bf16(d[6], d[7])));
   } else if constexpr (VW == 4) {
     __stcs(reinterpret_cast<uint2*>(p), make_uint2(pack_bf16(d[0], d[1]), pack_bf16(d[2], d[3])));
+  } else if constexpr (VW == 2) {
+    __stcs(reinterpret_cast<uint32_t*>(p), pack_bf16(d[0], d[1]));
   } else {
-    static_assert(VW == 1, "bf16 vectors hold 1, 4 or 8 elements");
+    static_assert(VW == 1, "bf16 vectors hold 1, 2, 4 or 8 elements");
     __stcs(reinterpret_cast<unsigned short*>(p), __bfloat16_as_ushort(__float2bfloat16_rn(d[0])));
   }
 }
