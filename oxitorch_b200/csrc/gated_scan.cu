@@ -35,6 +35,7 @@
 // fixed sequence of operations -- whoever computes it, from however far back --
 // the results do not depend on timing.
 #include <algorithm>
+#include <type_traits>
 
 #include "pipeline.cuh"
 #include "typed.cuh"
@@ -45,6 +46,8 @@ constexpr int kScanWarps = 8;
 constexpr int kScanSteps = 8;                        // tokens per warp
 constexpr int kScanChunk = kScanWarps * kScanSteps;  // tokens per CTA
 constexpr int kScanGroup = 16;                       // chunks per group
+constexpr int kScanFwdCtas = 3;                      // resident per SM
+constexpr int kScanBwdCtas = 2;
 
 // A [batch, length, dim] operand: the last dim dense, strides in elements.
 template <typename T>
@@ -53,21 +56,40 @@ struct SeqView {
   int64_t sb, st;
 };
 
-// a = sigmoid(g) and b = 1 - a, both relatively accurate (b is not formed by
-// subtraction, which would lose it for large gates): with e = exp(-|g|) they
-// are 1 / (1 + e) and e / (1 + e).  exp(-|g|) = 2^t, t = -|g| log2(e) in two
-// parts: ex2 takes the rounded one, the rest enters to first order.
-__device__ __forceinline__ void gate_pair(float g, float& a, float& b) {
-  const float n = -fabsf(g);
-  const float t = n * 1.44269502f;
-  const float lo = fmaf(n, 1.44269502f, -t) + n * 1.92596299e-8f;
-  float e, r;
+// a = sigmoid(g) and b = 1 - a for two channels, both relatively accurate (b is
+// not formed by subtraction, which would lose it for large gates): with e =
+// exp(-|g|) they are 1 / (1 + e) and e / (1 + e).  e = 2^t exp(n - t ln 2) with
+// n = -|g| and t = n log2(e) rounded; the second factor, the rounding's share,
+// to first order.  Below -100 e is 0 anyway, so n stops there (and stays finite
+// for infinite gates; max.NaN keeps a NaN).  Two channels at a time on the packed
+// f32x2 pipe: at 16 bits the kernels would otherwise be bound by the issue of
+// these instructions rather than by memory.
+__device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float gate_arg(float g) {
+  float n;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(n) : "f"(-fabsf(g)), "f"(-100.0f));
+  return n;
+}
+__device__ __forceinline__ float ex2_approx(float t) {
+  float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  e = t < -126.0f ? 0.0f : fmaf(e, lo * 0.693147181f, e);  // (an infinite t has lo = NaN)
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  const float er = e * r;
-  a = g > 0.0f ? r : er;
-  b = g > 0.0f ? er : r;
+  return e;
+}
+__device__ __forceinline__ float rcp_approx(float t) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return r;
+}
+__device__ __forceinline__ void gate_pair(float2 g, float2& a, float2& b) {
+  const float2 n = make_float2(gate_arg(g.x), gate_arg(g.y));
+  const float2 t = __fmul2_rn(n, f2(1.44269502f));
+  float2 e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
+  e = __ffma2_rn(e, __ffma2_rn(t, f2(-0.693147181f), n), e);
+  const float2 d = __fadd2_rn(e, f2(1.0f));
+  const float2 r = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+  const float2 q = __fmul2_rn(e, r);
+  a = make_float2(g.x > 0.0f ? r.x : q.x, g.y > 0.0f ? r.y : q.y);
+  b = make_float2(g.x > 0.0f ? q.x : r.x, g.y > 0.0f ? q.y : r.y);
 }
 
 // ---- maps of the state ---------------------------------------------------------------
@@ -222,29 +244,102 @@ __device__ __forceinline__ float chain_state(const Chain& c, int64_t k, int64_t 
 }
 static_assert((kScanGroup - 1) % 5 == 0, "a group's maps are read in batches of 5");
 
-// Which tile a CTA takes.  Tiles are handed out in the order of the scan, every
-// batch row and channel tile of a chunk before the next chunk, so the tiles that
-// one waits for are always already running.
+// ---- tiles -------------------------------------------------------------------------------
+
 struct Tile {
-  int64_t chunk, b;
-  int64_t d0;
+  int64_t chunk, b, d0;
 };
-__device__ __forceinline__ Tile take_tile(const Chain& c, int64_t batch, int64_t dtiles,
-                                          int channels) {
-  __shared__ unsigned int mine;
-  if (threadIdx.x == 0) mine = c.ticket ? atomicAdd(c.ticket, 1u) + 1u : blockIdx.x;
-  __syncthreads();
-  const int64_t id = mine, per = batch * dtiles, chunk = id / per, rest = id - chunk * per;
-  return {chunk, rest / dtiles, (rest % dtiles) * channels};
+
+// Hands out tiles to persistent CTAs, in the order of the scan: every batch row
+// and channel tile of a chunk before the next chunk, so whatever a tile waits
+// for belongs to a tile handed out before it, and the earliest unfinished tile
+// never waits.  The ticket for the next tile is drawn while the current one is
+// computed.  Without a chain (one chunk) the tiles are strided over the grid.
+struct Tiles {
+  unsigned int* next;  // shared
+  unsigned int drawn;
+
+  __device__ __forceinline__ void draw(const Chain& c, unsigned int now) {
+    if (threadIdx.x == blockDim.x - 1)
+      drawn = c.ticket ? atomicAdd(c.ticket, 1u) + 1u : now + gridDim.x;
+  }
+  __device__ __forceinline__ void post() {
+    if (threadIdx.x == blockDim.x - 1) *next = drawn;
+  }
+};
+
+__device__ __forceinline__ Tile tile_at(unsigned int id, int64_t batch, int64_t dtiles,
+                                        int channels) {
+  const uint32_t per = (uint32_t)(batch * dtiles), chunk = id / per, rest = id - chunk * per;
+  const uint32_t b = rest / (uint32_t)dtiles;
+  return {chunk, b, (int64_t)(rest - b * (uint32_t)dtiles) * channels};
 }
 
-// VW channels of one token, in f32.  VEC: consecutive ones, in one load; else
-// 32 apart (lane l takes l, l + 32, ...), each guarded.
+// VW channels of one token as loaded.  VEC: consecutive ones, in one access; else
+// 32 apart (lane l takes l, l + 32, ...), each guarded.  The loads are predicated
+// rather than branched around, so that all of a thread's loads are in flight
+// before the first is used.
+template <typename T, int VW, bool VEC>
+struct Raw;
+
+template <int VW, bool VEC>
+struct Raw<float, VW, VEC> {
+  float v[VW];
+  __device__ __forceinline__ void fill(float f) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) v[k] = f;
+  }
+  __device__ __forceinline__ void load(const float* p, int live) {
+    if constexpr (VEC && VW == 4) {
+      asm("{.reg .pred p; setp.gt.s32 p, %5, 0; @p ld.global.cs.v4.f32 {%0, %1, %2, %3}, [%4];}"
+          : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]) : "l"(p), "r"(live));
+    } else if constexpr (VEC && VW == 2) {
+      asm("{.reg .pred p; setp.gt.s32 p, %3, 0; @p ld.global.cs.v2.f32 {%0, %1}, [%2];}"
+          : "+f"(v[0]), "+f"(v[1]) : "l"(p), "r"(live));
+    } else {
+#pragma unroll
+      for (int k = 0; k < VW; ++k)
+        asm("{.reg .pred p; setp.gt.s32 p, %2, %3; @p ld.global.cs.f32 %0, [%1];}"
+            : "+f"(v[k]) : "l"(p + 32 * k), "r"(live), "r"(k));
+    }
+  }
+  __device__ __forceinline__ float2 pair(int j) const { return make_float2(v[2 * j], v[2 * j + 1]); }
+};
+
+template <int VW, bool VEC>
+struct Raw<bf16, VW, VEC> {
+  uint32_t w[VEC ? VW / 2 : VW];  // two to a word, or one in the upper half
+  __device__ __forceinline__ void fill(float f) {
+    const uint32_t u = __float_as_uint(f);  // 0 or infinity: the lower half is 0
+#pragma unroll
+    for (int k = 0; k < (VEC ? VW / 2 : VW); ++k) w[k] = VEC ? u | (u >> 16) : u >> 16;
+  }
+  __device__ __forceinline__ void load(const bf16* p, int live) {
+    if constexpr (VEC && VW == 4) {
+      asm("{.reg .pred p; setp.gt.s32 p, %3, 0; @p ld.global.cs.v2.u32 {%0, %1}, [%2];}"
+          : "+r"(w[0]), "+r"(w[1]) : "l"(p), "r"(live));
+    } else if constexpr (VEC && VW == 2) {
+      asm("{.reg .pred p; setp.gt.s32 p, %2, 0; @p ld.global.cs.u32 %0, [%1];}"
+          : "+r"(w[0]) : "l"(p), "r"(live));
+    } else {
+#pragma unroll
+      for (int k = 0; k < VW; ++k)
+        asm("{.reg .pred p; setp.gt.s32 p, %2, %3; @p ld.global.cs.u16 %0, [%1];}"
+            : "+r"(w[k]) : "l"(p + 32 * k), "r"(live), "r"(k));
+    }
+  }
+  __device__ __forceinline__ float2 pair(int j) const {
+    if constexpr (VEC) return make_float2(bf16_lo(w[j]), bf16_hi(w[j]));
+    else return make_float2(bf16_lo(w[2 * j]), bf16_lo(w[2 * j + 1]));
+  }
+};
+
+// A lane's channels of a tile.
 template <typename T, int VW, bool VEC>
 struct Lane {
   static constexpr int kChannels = 32 * VW;
-  int64_t d;   // the lane's first channel
-  int live;    // how many of its channels exist
+  int64_t d;  // the first
+  int live;   // how many exist
   __device__ __forceinline__ Lane(int64_t d0, int64_t dim) {
     const int lane = threadIdx.x & 31;
     d = VEC ? d0 + lane * VW : d0 + lane;
@@ -256,27 +351,37 @@ struct Lane {
     const int lane = threadIdx.x & 31;
     return VEC ? lane * VW + k : lane + 32 * k;
   }
-  __device__ __forceinline__ void load(float (&v)[VW], const T* row) const {
+  __device__ __forceinline__ void store(T* row, const float2 (&v)[VW / 2]) const {
+    float f[VW];
+#pragma unroll
+    for (int j = 0; j < VW / 2; ++j) { f[2 * j] = v[j].x; f[2 * j + 1] = v[j].y; }
     if constexpr (VEC) {
-      if (live) load_as_f32<VW>(v, row + d);
+      if (live) store_from_f32<VW>(row + d, f);
     } else {
 #pragma unroll
       for (int k = 0; k < VW; ++k) {
-        float one[1] = {0.0f};
-        if (k < live) load_as_f32<1>(one, row + d + 32 * k);
-        v[k] = one[0];
+        const float one[1] = {f[k]};
+        if (k < live) store_from_f32<1>(row + d + 32 * k, one);
       }
     }
   }
-  __device__ __forceinline__ void store(T* row, const float (&v)[VW]) const {
-    if constexpr (VEC) {
-      if (live) store_from_f32<VW>(row + d, v);
-    } else {
+  // this lane's entries of a [kChannels] row in shared memory
+  __device__ __forceinline__ void put(float* row, const float2 (&v)[VW / 2]) const {
 #pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        const float one[1] = {v[k]};
-        if (k < live) store_from_f32<1>(row + d + 32 * k, one);
+    for (int j = 0; j < VW / 2; ++j) {
+      if constexpr (VEC) {
+        *reinterpret_cast<float2*>(row + channel(2 * j)) = v[j];
+      } else {
+        row[channel(2 * j)] = v[j].x;
+        row[channel(2 * j + 1)] = v[j].y;
       }
+    }
+  }
+  __device__ __forceinline__ void get(const float* row, float2 (&v)[VW / 2]) const {
+#pragma unroll
+    for (int j = 0; j < VW / 2; ++j) {
+      if constexpr (VEC) v[j] = *reinterpret_cast<const float2*>(row + channel(2 * j));
+      else v[j] = make_float2(row[channel(2 * j)], row[channel(2 * j + 1)]);
     }
   }
 };
@@ -290,222 +395,272 @@ __device__ __forceinline__ unsigned int start_bits(const uint8_t* starts, int64_
   return __ballot_sync(0xffffffffu, s);
 }
 
-template <typename T, int VW, bool VEC>
-__global__ void __launch_bounds__(kScanWarps * 32, 2) scan_fwd_kernel(
+// Runs f(std::true_type) if any of the warp's tokens starts a sequence, else
+// f(std::false_type), whose loops need no selects.
+template <typename F>
+__device__ __forceinline__ void by_fresh(unsigned int fresh, F f) {
+  if (fresh) f(std::true_type{});
+  else f(std::false_type{});
+}
+
+// Tokens beyond the length are given an infinite gate and x = 0: a = 1, b = 0,
+// the identity.  Only their loads and stores are left out.
+template <typename T, int VW, bool VEC, int CTAS>
+__global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_fwd_kernel(
     SeqView<T> x, SeqView<T> gate, const uint8_t* __restrict__ starts,
     const float* __restrict__ h0, T* __restrict__ h, float* __restrict__ last,
     float* __restrict__ carry, Chain chain, int64_t batch, int64_t length, int64_t dim,
-    int64_t chunks, int64_t dtiles) {
+    int64_t chunks, int64_t dtiles, unsigned int tiles) {
   using L = Lane<T, VW, VEC>;
-  __shared__ float mapA[kScanWarps][L::kChannels], mapH[kScanWarps][L::kChannels];
-  const Tile tile = take_tile(chain, batch, dtiles, L::kChannels);
-  const L lane(tile.d0, dim);
+  using R = Raw<T, VW, VEC>;
+  constexpr int P = VW / 2;
+  __shared__ __align__(16) float mapA[kScanWarps][L::kChannels];
+  __shared__ __align__(16) float mapH[kScanWarps][L::kChannels];
+  __shared__ unsigned int next;
+  Tiles order{&next, blockIdx.x};
   const int warp = threadIdx.x >> 5;
-  const int64_t t0 = tile.chunk * kScanChunk + warp * kScanSteps;
-  const int steps = (int)max((int64_t)0, min((int64_t)kScanSteps, length - t0));
-  const unsigned int fresh = start_bits(starts, tile.b, t0, length);
-
-  float a[kScanSteps][VW], v[kScanSteps][VW];
+  if (chain.ticket) order.draw(chain, 0u);
+  order.post();
+  for (;;) {
+    __syncthreads();  // `next` is posted, the maps of the tile before are read
+    const unsigned int id = next;
+    if (id >= tiles) return;
+    const Tile tile = tile_at(id, batch, dtiles, L::kChannels);
+    const L lane(tile.d0, dim);
+    const int64_t t0 = tile.chunk * kScanChunk + warp * kScanSteps;
+    const int steps = (int)max((int64_t)0, min((int64_t)kScanSteps, length - t0));
+    R rg[kScanSteps], rx[kScanSteps];
+    {
+      const T* pg = gate.p + tile.b * gate.sb + t0 * gate.st + lane.d;
+      const T* px = x.p + tile.b * x.sb + t0 * x.st + lane.d;
 #pragma unroll
-  for (int i = 0; i < kScanSteps; ++i) {
-#pragma unroll
-    for (int k = 0; k < VW; ++k) a[i][k] = v[i][k] = 0.0f;
-    if (i < steps) {
-      lane.load(a[i], gate.p + tile.b * gate.sb + (t0 + i) * gate.st);
-      lane.load(v[i], x.p + tile.b * x.sb + (t0 + i) * x.st);
-    }
-  }
-  float A[VW], H[VW];
-#pragma unroll
-  for (int k = 0; k < VW; ++k) { A[k] = 1.0f; H[k] = 0.0f; }
-#pragma unroll
-  for (int i = 0; i < kScanSteps; ++i) {
-    if (i < steps) {
-      const bool s = (fresh >> i) & 1u;
-#pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        float b;
-        gate_pair(a[i][k], a[i][k], b);
-        v[i][k] *= b;
-        H[k] = s ? v[i][k] : fmaf(a[i][k], H[k], v[i][k]);
-        A[k] = s ? -0.0f : A[k] * a[i][k];
+      for (int i = 0; i < kScanSteps; ++i) {
+        rg[i].fill(INFINITY);
+        rx[i].fill(0.0f);
+        rg[i].load(pg, i < steps ? lane.live : 0);
+        rx[i].load(px, i < steps ? lane.live : 0);
+        pg += gate.st;
+        px += x.st;
       }
     }
-  }
+    const unsigned int fresh = start_bits(starts, tile.b, t0, length);
+    order.draw(chain, id);
+    float2 a[kScanSteps][P], v[kScanSteps][P], A[P], H[P];
 #pragma unroll
-  for (int k = 0; k < VW; ++k) {
-    mapA[warp][lane.channel(k)] = A[k];
-    mapH[warp][lane.channel(k)] = H[k];
-  }
-  __syncthreads();
-  const int c = threadIdx.x;
-  if (c < L::kChannels && tile.d0 + c < dim) {
-    const int64_t off = tile.b * dim + tile.d0 + c;
-    float s = h0 ? h0[off] : 0.0f;
-    if (chunks > 1) {
-      float tA = mapA[kScanWarps - 1][c], tH = mapH[kScanWarps - 1][c];
+    for (int j = 0; j < P; ++j) { A[j] = f2(1.0f); H[j] = f2(0.0f); }
 #pragma unroll
-      for (int w = kScanWarps - 2; w >= 0; --w) map_compose(tA, tH, mapA[w][c], mapH[w][c]);
-      s = chain_state(chain, tile.chunk, chunks, off, tA, tH, s);
+    for (int i = 0; i < kScanSteps; ++i)
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        float2 b;
+        gate_pair(rg[i].pair(j), a[i][j], b);
+        v[i][j] = __fmul2_rn(b, rx[i].pair(j));
+      }
+    by_fresh(fresh, [&](auto some) {
+#pragma unroll
+      for (int i = 0; i < kScanSteps; ++i)
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          H[j] = __ffma2_rn(a[i][j], H[j], v[i][j]);
+          A[j] = __fmul2_rn(A[j], a[i][j]);
+          if (decltype(some)::value && ((fresh >> i) & 1u)) { H[j] = v[i][j]; A[j] = f2(-0.0f); }
+        }
+    });
+    lane.put(mapA[warp], A);
+    lane.put(mapH[warp], H);
+    __syncthreads();
+    order.post();
+    const int c = threadIdx.x;
+    if (c < L::kChannels && tile.d0 + c < dim) {
+      const int64_t off = tile.b * dim + tile.d0 + c;
+      float s = h0 ? h0[off] : 0.0f;
+      if (chunks > 1) {
+        float tA = mapA[kScanWarps - 1][c], tH = mapH[kScanWarps - 1][c];
+#pragma unroll
+        for (int w = kScanWarps - 2; w >= 0; --w) map_compose(tA, tH, mapA[w][c], mapH[w][c]);
+        s = chain_state(chain, tile.chunk, chunks, off, tA, tH, s);
+      }
+      if (carry) carry[(tile.b * chunks + tile.chunk) * dim + tile.d0 + c] = s;
+#pragma unroll
+      for (int w = 0; w < kScanWarps; ++w) {  // mapH becomes the state entering warp w
+        const float after = map_apply(mapA[w][c], mapH[w][c], s);
+        mapH[w][c] = s;
+        s = after;
+      }
     }
-    if (carry) carry[(tile.b * chunks + tile.chunk) * dim + tile.d0 + c] = s;
+    __syncthreads();
+    float2 s[P];
+    lane.get(mapH[warp], s);
+    by_fresh(fresh, [&](auto some) {
+      T* ph = h + (tile.b * length + t0) * dim;
 #pragma unroll
-    for (int w = 0; w < kScanWarps; ++w) {  // mapH becomes the state entering warp w
-      const float next = map_apply(mapA[w][c], mapH[w][c], s);
-      mapH[w][c] = s;
-      s = next;
+      for (int i = 0; i < kScanSteps; ++i) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          s[j] = __ffma2_rn(a[i][j], s[j], v[i][j]);
+          if (decltype(some)::value && ((fresh >> i) & 1u)) s[j] = v[i][j];
+        }
+        if (i < steps) lane.store(ph, s);
+        ph += dim;
+      }
+    });
+    if (last && steps > 0 && t0 + steps == length) {
+#pragma unroll
+      for (int k = 0; k < VW; ++k)
+        if (k < lane.live)
+          last[tile.b * dim + tile.d0 + lane.channel(k)] = k & 1 ? s[k / 2].y : s[k / 2].x;
     }
-  }
-  __syncthreads();
-  float s[VW];
-#pragma unroll
-  for (int k = 0; k < VW; ++k) s[k] = mapH[warp][lane.channel(k)];
-#pragma unroll
-  for (int i = 0; i < kScanSteps; ++i) {
-    if (i < steps) {
-      const bool f = (fresh >> i) & 1u;
-#pragma unroll
-      for (int k = 0; k < VW; ++k) s[k] = f ? v[i][k] : fmaf(a[i][k], s[k], v[i][k]);
-      lane.store(h + (tile.b * length + t0 + i) * dim, s);
-    }
-  }
-  if (last && steps > 0 && t0 + steps == length) {
-#pragma unroll
-    for (int k = 0; k < VW; ++k)
-      if (k < lane.live) last[tile.b * dim + tile.d0 + lane.channel(k)] = s[k];
   }
 }
 
-template <typename T, int VW, bool VEC>
-__global__ void __launch_bounds__(kScanWarps * 32, 2) scan_bwd_kernel(
+template <typename T, int VW, bool VEC, int CTAS>
+__global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
     SeqView<T> x, SeqView<T> gate, const uint8_t* __restrict__ starts,
     const float* __restrict__ carry, SeqView<T> dh, const float* __restrict__ dlast,
     T* __restrict__ dx, T* __restrict__ dgate, float* __restrict__ dh0, Chain chain, int64_t batch,
-    int64_t length, int64_t dim, int64_t chunks, int64_t dtiles) {
+    int64_t length, int64_t dim, int64_t chunks, int64_t dtiles, unsigned int tiles) {
   using L = Lane<T, VW, VEC>;
+  using R = Raw<T, VW, VEC>;
+  constexpr int P = VW / 2;
   // per warp: its map's A, the state's H and mu's H; then the state entering it
   // from the left and the mu from the right
-  __shared__ float mapA[kScanWarps][L::kChannels], mapS[kScanWarps][L::kChannels],
-      mapM[kScanWarps][L::kChannels];
-  Tile tile = take_tile(chain, batch, dtiles, L::kChannels);
-  tile.chunk = chunks - 1 - tile.chunk;  // from the end of the sequence
-  const L lane(tile.d0, dim);
+  __shared__ __align__(16) float mapA[kScanWarps][L::kChannels];
+  __shared__ __align__(16) float mapS[kScanWarps][L::kChannels];
+  __shared__ __align__(16) float mapM[kScanWarps][L::kChannels];
+  __shared__ unsigned int next;
+  Tiles order{&next, blockIdx.x};
   const int warp = threadIdx.x >> 5;
-  const int64_t t0 = tile.chunk * kScanChunk + warp * kScanSteps;
-  const int steps = (int)max((int64_t)0, min((int64_t)kScanSteps, length - t0));
-  const unsigned int fresh = start_bits(starts, tile.b, t0, length);
-
-  float g[kScanSteps][VW], v[kScanSteps][VW], lam[kScanSteps][VW];
+  if (chain.ticket) order.draw(chain, 0u);
+  order.post();
+  for (;;) {
+    __syncthreads();  // `next` is posted, the maps of the tile before are read
+    const unsigned int id = next;
+    if (id >= tiles) return;
+    Tile tile = tile_at(id, batch, dtiles, L::kChannels);
+    tile.chunk = chunks - 1 - tile.chunk;  // from the end of the sequence
+    const L lane(tile.d0, dim);
+    const int64_t t0 = tile.chunk * kScanChunk + warp * kScanSteps;
+    const int steps = (int)max((int64_t)0, min((int64_t)kScanSteps, length - t0));
+    R rg[kScanSteps], rx[kScanSteps], rd[kScanSteps];
+    {
+      const T* pg = gate.p + tile.b * gate.sb + t0 * gate.st + lane.d;
+      const T* px = x.p + tile.b * x.sb + t0 * x.st + lane.d;
+      const T* pd = dh.p + tile.b * dh.sb + t0 * dh.st + lane.d;
 #pragma unroll
-  for (int i = 0; i < kScanSteps; ++i) {
-#pragma unroll
-    for (int k = 0; k < VW; ++k) g[i][k] = v[i][k] = lam[i][k] = 0.0f;
-    if (i < steps) {
-      lane.load(g[i], gate.p + tile.b * gate.sb + (t0 + i) * gate.st);
-      lane.load(v[i], x.p + tile.b * x.sb + (t0 + i) * x.st);
-      if (dh.p) lane.load(lam[i], dh.p + tile.b * dh.sb + (t0 + i) * dh.st);
-    }
-  }
-  float a[kScanSteps][VW], b[kScanSteps][VW];
-  float A[VW], S[VW], M[VW];
-#pragma unroll
-  for (int k = 0; k < VW; ++k) { A[k] = 1.0f; S[k] = 0.0f; M[k] = 0.0f; }
-#pragma unroll
-  for (int i = 0; i < kScanSteps; ++i) {
-    if (i < steps) {
-      const bool s = (fresh >> i) & 1u;
-#pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        gate_pair(g[i][k], a[i][k], b[i][k]);
-        S[k] = s ? b[i][k] * v[i][k] : fmaf(a[i][k], S[k], b[i][k] * v[i][k]);
-        A[k] = s ? -0.0f : A[k] * a[i][k];
+      for (int i = 0; i < kScanSteps; ++i) {
+        rg[i].fill(INFINITY);
+        rx[i].fill(0.0f);
+        rd[i].fill(0.0f);
+        rg[i].load(pg, i < steps ? lane.live : 0);
+        rx[i].load(px, i < steps ? lane.live : 0);
+        rd[i].load(pd, i < steps && dh.p ? lane.live : 0);
+        pg += gate.st;
+        px += x.st;
+        pd += dh.st;
       }
     }
-  }
+    const unsigned int fresh = start_bits(starts, tile.b, t0, length);
+    order.draw(chain, id);
+    float2 a[kScanSteps][P], b[kScanSteps][P], A[P], S[P], M[P];
 #pragma unroll
-  for (int i = kScanSteps - 1; i >= 0; --i) {
-    if (i < steps) {
-      const bool s = (fresh >> i) & 1u;
+    for (int j = 0; j < P; ++j) { A[j] = f2(1.0f); S[j] = M[j] = f2(0.0f); }
 #pragma unroll
-      for (int k = 0; k < VW; ++k) M[k] = s ? 0.0f : a[i][k] * (lam[i][k] + M[k]);
-    }
-  }
+    for (int i = 0; i < kScanSteps; ++i)
 #pragma unroll
-  for (int k = 0; k < VW; ++k) {
-    mapA[warp][lane.channel(k)] = A[k];
-    mapS[warp][lane.channel(k)] = S[k];
-    mapM[warp][lane.channel(k)] = M[k];
-  }
-  __syncthreads();
-  // the mu of the chunk after this one and the state before it, by two sets of
-  // threads
-  const int c = threadIdx.x % L::kChannels, part = threadIdx.x / L::kChannels;
-  if (part < 2 && tile.d0 + c < dim) {
-    const int64_t off = tile.b * dim + tile.d0 + c;
-    if (part == 0) {
-      float m = dlast ? dlast[off] : 0.0f;
-      if (chunks > 1) {
-        float tA = mapA[0][c], tM = mapM[0][c];
+      for (int j = 0; j < P; ++j) gate_pair(rg[i].pair(j), a[i][j], b[i][j]);
+    by_fresh(fresh, [&](auto some) {
 #pragma unroll
-        for (int w = 1; w < kScanWarps; ++w) map_compose(tA, tM, mapA[w][c], mapM[w][c]);
-        m = chain_state(chain, chunks - 1 - tile.chunk, chunks, off, tA, tM, m);
-      }
+      for (int i = 0; i < kScanSteps; ++i)
 #pragma unroll
-      for (int w = kScanWarps - 1; w >= 0; --w) {
-        const float next = map_apply(mapA[w][c], mapM[w][c], m);
-        mapM[w][c] = m;
-        m = next;
-      }
-    } else {
-      float s = carry[(tile.b * chunks + tile.chunk) * dim + tile.d0 + c];
+        for (int j = 0; j < P; ++j) {
+          const float2 v = __fmul2_rn(b[i][j], rx[i].pair(j));
+          S[j] = __ffma2_rn(a[i][j], S[j], v);
+          A[j] = __fmul2_rn(A[j], a[i][j]);
+          if (decltype(some)::value && ((fresh >> i) & 1u)) { S[j] = v; A[j] = f2(-0.0f); }
+        }
 #pragma unroll
-      for (int w = 0; w < kScanWarps; ++w) {
-        const float next = map_apply(mapA[w][c], mapS[w][c], s);
-        mapS[w][c] = s;
-        s = next;
-      }
-    }
-  }
-  __syncthreads();
-  float s[VW], m[VW];
+      for (int i = kScanSteps - 1; i >= 0; --i)
 #pragma unroll
-  for (int k = 0; k < VW; ++k) {
-    s[k] = mapS[warp][lane.channel(k)];
-    m[k] = mapM[warp][lane.channel(k)];
-  }
+        for (int j = 0; j < P; ++j) {
+          M[j] = __fmul2_rn(a[i][j], __fadd2_rn(rd[i].pair(j), M[j]));
+          if (decltype(some)::value && ((fresh >> i) & 1u)) M[j] = f2(0.0f);
+        }
+    });
+    lane.put(mapA[warp], A);
+    lane.put(mapS[warp], S);
+    lane.put(mapM[warp], M);
+    __syncthreads();
+    order.post();
+    // the mu of the chunk after this one and the state before it, by two sets of
+    // threads
+    const int c = threadIdx.x % L::kChannels, part = threadIdx.x / L::kChannels;
+    if (part < 2 && tile.d0 + c < dim) {
+      const int64_t off = tile.b * dim + tile.d0 + c;
+      if (part == 0) {
+        float m = dlast ? dlast[off] : 0.0f;
+        if (chunks > 1) {
+          float tA = mapA[0][c], tM = mapM[0][c];
 #pragma unroll
-  for (int i = 0; i < kScanSteps; ++i) {
-    if (i < steps) {
-      const bool f = (fresh >> i) & 1u;
+          for (int w = 1; w < kScanWarps; ++w) map_compose(tA, tM, mapA[w][c], mapM[w][c]);
+          m = chain_state(chain, chunks - 1 - tile.chunk, chunks, off, tA, tM, m);
+        }
 #pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        const float before = f ? 0.0f : s[k];
-        s[k] = fmaf(a[i][k], before, b[i][k] * v[i][k]);
-        v[i][k] = before - v[i][k];  // what d h_t / d a_t is
+        for (int w = kScanWarps - 1; w >= 0; --w) {
+          const float before = map_apply(mapA[w][c], mapM[w][c], m);
+          mapM[w][c] = m;
+          m = before;
+        }
+      } else {
+        float s = carry[(tile.b * chunks + tile.chunk) * dim + tile.d0 + c];
+#pragma unroll
+        for (int w = 0; w < kScanWarps; ++w) {
+          const float after = map_apply(mapA[w][c], mapS[w][c], s);
+          mapS[w][c] = s;
+          s = after;
+        }
       }
     }
-  }
+    __syncthreads();
+    float2 s[P], m[P], gap[kScanSteps][P];  // gap: h_{t-1} - x_t, what d h_t / d a_t is
+    lane.get(mapS[warp], s);
+    lane.get(mapM[warp], m);
+    by_fresh(fresh, [&](auto some) {
 #pragma unroll
-  for (int i = kScanSteps - 1; i >= 0; --i) {
-    if (i < steps) {
-      const bool f = (fresh >> i) & 1u;
-      float ox[VW], og[VW];
+      for (int i = 0; i < kScanSteps; ++i)
 #pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        const float l = lam[i][k] + m[k];
-        ox[k] = l * b[i][k];
-        og[k] = ox[k] * a[i][k] * v[i][k];
-        m[k] = f ? 0.0f : a[i][k] * l;
+        for (int j = 0; j < P; ++j) {
+          const float2 v = rx[i].pair(j);
+          if (decltype(some)::value && ((fresh >> i) & 1u)) s[j] = f2(0.0f);
+          gap[i][j] = __fadd2_rn(s[j], make_float2(-v.x, -v.y));
+          s[j] = __ffma2_rn(a[i][j], s[j], __fmul2_rn(b[i][j], v));
+        }
+      T* px = dx + (tile.b * length + t0 + kScanSteps - 1) * dim;
+      T* pg = dgate + (tile.b * length + t0 + kScanSteps - 1) * dim;
+#pragma unroll
+      for (int i = kScanSteps - 1; i >= 0; --i) {
+        float2 ox[P], og[P];
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          const float2 l = __fadd2_rn(rd[i].pair(j), m[j]);
+          ox[j] = __fmul2_rn(l, b[i][j]);
+          m[j] = __fmul2_rn(a[i][j], l);
+          og[j] = __fmul2_rn(__fmul2_rn(m[j], b[i][j]), gap[i][j]);
+          if (decltype(some)::value && ((fresh >> i) & 1u)) m[j] = f2(0.0f);
+        }
+        if (i < steps) {
+          lane.store(px, ox);
+          lane.store(pg, og);
+        }
+        px -= dim;
+        pg -= dim;
       }
-      const int64_t o = (tile.b * length + t0 + i) * dim;
-      lane.store(dx + o, ox);
-      lane.store(dgate + o, og);
-    }
-  }
-  if (dh0 && tile.chunk == 0 && warp == 0) {
+    });
+    if (dh0 && tile.chunk == 0 && warp == 0) {
 #pragma unroll
-    for (int k = 0; k < VW; ++k)
-      if (k < lane.live) dh0[tile.b * dim + tile.d0 + lane.channel(k)] = m[k];
+      for (int k = 0; k < VW; ++k)
+        if (k < lane.live)
+          dh0[tile.b * dim + tile.d0 + lane.channel(k)] = k & 1 ? m[k / 2].y : m[k / 2].x;
+    }
   }
 }
 
@@ -519,9 +674,9 @@ __global__ void __launch_bounds__(128) scan_step_kernel(const T* __restrict__ x,
   const int64_t d = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int64_t bi = blockIdx.y;
   if (d >= dim) return;
-  float a, b;
-  gate_pair(to_f32(gate[bi * gate_stride + d]), a, b);
-  const float s = fmaf(a, state[bi * dim + d], b * to_f32(x[bi * x_stride + d]));
+  float2 a, b;
+  gate_pair(f2(to_f32(gate[bi * gate_stride + d])), a, b);
+  const float s = fmaf(a.x, state[bi * dim + d], b.x * to_f32(x[bi * x_stride + d]));
   state_out[bi * dim + d] = s;
   h[bi * dim + d] = from_f32<T>(s);
 }
@@ -569,60 +724,67 @@ static bool seq_vec(const void* p, int64_t sb, int64_t st, int64_t dim) {
   return dim % VW == 0 && sb % VW == 0 && st % VW == 0 && aligned_to(p, VW * sizeof(T));
 }
 
-static oxc_status scan_grid(const char* fn, int64_t batch, int64_t length, int64_t dim,
-                            int channels, int64_t* dtiles, unsigned* grid) {
+// The number of tiles, and a grid that is resident at once.
+static oxc_status scan_grid(const char* fn, const void* kernel, int64_t batch, int64_t length,
+                            int64_t dim, int channels, int64_t* dtiles, unsigned* tiles,
+                            unsigned* grid) {
   *dtiles = (dim + channels - 1) / channels;
   const int64_t per = batch * *dtiles;
   if (scan_chunks(length) > 0x7fffffff / per)
     return fail(OXC_ERR_NOT_IMPLEMENTED, "not implemented: %s: [%lld, %lld, %lld]", fn,
                 (long long)batch, (long long)length, (long long)dim);
-  *grid = (unsigned)(scan_chunks(length) * per);
+  *tiles = (unsigned)(scan_chunks(length) * per);
+  const unsigned resident = (unsigned)(sm_count() * occupancy(kernel, kScanWarps * 32, 0));
+  *grid = std::min(*tiles, resident);
   return OXC_OK;
 }
 
-template <typename T>
+template <typename T, int VW>
 static oxc_status scan_fwd_launch(const void* x, int64_t x_sb, int64_t x_st, const void* gate,
                                   int64_t g_sb, int64_t g_st, const uint8_t* starts,
                                   const float* h0, void* h, float* last, float* carry,
                                   const Chain& chain, int64_t batch, int64_t length, int64_t dim,
                                   cudaStream_t s) {
-  constexpr int VW = 4;
-  int64_t dtiles;
-  unsigned grid;
-  oxc_status st = scan_grid("gated_scan", batch, length, dim, 32 * VW, &dtiles, &grid);
-  if (st) return st;
   const bool vec = seq_vec<T, VW>(x, x_sb, x_st, dim) && seq_vec<T, VW>(gate, g_sb, g_st, dim) &&
                    seq_vec<T, VW>(h, 0, 0, dim);
+  auto kernel = vec ? scan_fwd_kernel<T, VW, true, kScanFwdCtas>
+                    : scan_fwd_kernel<T, VW, false, kScanFwdCtas>;
+  int64_t dtiles;
+  unsigned tiles, grid;
+  oxc_status st = scan_grid("gated_scan", (const void*)kernel, batch, length, dim, 32 * VW, &dtiles,
+                            &tiles, &grid);
+  if (st) return st;
   const SeqView<T> xv{static_cast<const T*>(x), x_sb, x_st};
   const SeqView<T> gv{static_cast<const T*>(gate), g_sb, g_st};
-  auto kernel = vec ? scan_fwd_kernel<T, VW, true> : scan_fwd_kernel<T, VW, false>;
   kernel<<<grid, kScanWarps * 32, 0, s>>>(xv, gv, starts, h0, static_cast<T*>(h), last, carry,
-                                          chain, batch, length, dim, scan_chunks(length), dtiles);
+                                          chain, batch, length, dim, scan_chunks(length), dtiles,
+                                          tiles);
   return check_launch("oxc_gated_scan_fwd");
 }
 
-template <typename T>
+template <typename T, int VW>
 static oxc_status scan_bwd_launch(const void* x, int64_t x_sb, int64_t x_st, const void* gate,
                                   int64_t g_sb, int64_t g_st, const uint8_t* starts,
                                   const float* carry, const void* dh, int64_t dh_sb, int64_t dh_st,
                                   const float* dlast, void* dx, void* dgate, float* dh0,
                                   const Chain& chain, int64_t batch, int64_t length, int64_t dim,
                                   cudaStream_t s) {
-  constexpr int VW = 2;
-  int64_t dtiles;
-  unsigned grid;
-  oxc_status st = scan_grid("gated_scan backward", batch, length, dim, 32 * VW, &dtiles, &grid);
-  if (st) return st;
   const bool vec = seq_vec<T, VW>(x, x_sb, x_st, dim) && seq_vec<T, VW>(gate, g_sb, g_st, dim) &&
                    seq_vec<T, VW>(dh, dh_sb, dh_st, dim) && seq_vec<T, VW>(dx, 0, 0, dim) &&
                    seq_vec<T, VW>(dgate, 0, 0, dim);
+  auto kernel = vec ? scan_bwd_kernel<T, VW, true, kScanBwdCtas>
+                    : scan_bwd_kernel<T, VW, false, kScanBwdCtas>;
+  int64_t dtiles;
+  unsigned tiles, grid;
+  oxc_status st = scan_grid("gated_scan backward", (const void*)kernel, batch, length, dim, 32 * VW,
+                            &dtiles, &tiles, &grid);
+  if (st) return st;
   const SeqView<T> xv{static_cast<const T*>(x), x_sb, x_st};
   const SeqView<T> gv{static_cast<const T*>(gate), g_sb, g_st};
   const SeqView<T> dv{static_cast<const T*>(dh), dh_sb, dh_st};
-  auto kernel = vec ? scan_bwd_kernel<T, VW, true> : scan_bwd_kernel<T, VW, false>;
   kernel<<<grid, kScanWarps * 32, 0, s>>>(xv, gv, starts, carry, dv, dlast, static_cast<T*>(dx),
                                           static_cast<T*>(dgate), dh0, chain, batch, length, dim,
-                                          scan_chunks(length), dtiles);
+                                          scan_chunks(length), dtiles, tiles);
   return check_launch("oxc_gated_scan_bwd");
 }
 
@@ -667,9 +829,9 @@ oxc_status oxc_gated_scan_fwd(const void* x, int64_t x_sb, int64_t x_st, const v
   st = scan_chain("gated_scan", batch, length, dim, workspace, workspace_bytes, s, &chain);
   if (st) return st;
   if (dtype == OXC_BF16)
-    return scan_fwd_launch<bf16>(x, x_sb, x_st, gate, g_sb, g_st, starts, h0, h, last, carry,
+    return scan_fwd_launch<bf16, 4>(x, x_sb, x_st, gate, g_sb, g_st, starts, h0, h, last, carry,
                                  chain, batch, length, dim, s);
-  return scan_fwd_launch<float>(x, x_sb, x_st, gate, g_sb, g_st, starts, h0, h, last, carry, chain,
+  return scan_fwd_launch<float, 4>(x, x_sb, x_st, gate, g_sb, g_st, starts, h0, h, last, carry, chain,
                                 batch, length, dim, s);
 }
 
@@ -696,9 +858,9 @@ oxc_status oxc_gated_scan_bwd(const void* x, int64_t x_sb, int64_t x_st, const v
   st = scan_chain("gated_scan backward", batch, length, dim, workspace, workspace_bytes, s, &chain);
   if (st) return st;
   if (dtype == OXC_BF16)
-    return scan_bwd_launch<bf16>(x, x_sb, x_st, gate, g_sb, g_st, starts, carry, dh, dh_sb, dh_st,
+    return scan_bwd_launch<bf16, 2>(x, x_sb, x_st, gate, g_sb, g_st, starts, carry, dh, dh_sb, dh_st,
                                  dlast, dx, dgate, dh0, chain, batch, length, dim, s);
-  return scan_bwd_launch<float>(x, x_sb, x_st, gate, g_sb, g_st, starts, carry, dh, dh_sb, dh_st,
+  return scan_bwd_launch<float, 2>(x, x_sb, x_st, gate, g_sb, g_st, starts, carry, dh, dh_sb, dh_st,
                                 dlast, dx, dgate, dh0, chain, batch, length, dim, s);
 }
 
