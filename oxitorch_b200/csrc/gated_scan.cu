@@ -26,12 +26,12 @@
 // recurrence from it on the values that it kept in registers: x and gate are
 // read once.  The VJP's mu runs through the same A from the other end.
 //
-// The state that enters a chunk (Chain, below): chunks form groups of 16.  A
+// The state that enters a chunk (Chain, below): chunks form groups of 8.  A
 // chunk applies, one after the other, the maps of the chunks before it in its
 // group to the state entering the group; that one in turn comes from the
 // nearest group whose entering state is known and the group maps between.  So
-// the number of dependent steps is length / 1024, the reads per chunk are at
-// most 15 maps and a few group words, and since every state is defined by one
+// the number of dependent steps is length / 512, the reads per chunk are at
+// most 7 maps and a few group words, and since every state is defined by one
 // fixed sequence of operations -- whoever computes it, from however far back --
 // the results do not depend on timing.
 #include <algorithm>
@@ -45,8 +45,8 @@ namespace oxc {
 constexpr int kScanWarps = 8;
 constexpr int kScanSteps = 8;                        // tokens per warp
 constexpr int kScanChunk = kScanWarps * kScanSteps;  // tokens per CTA
-constexpr int kScanGroup = 16;                       // chunks per group
-constexpr int kScanFwdCtas = 3;                      // resident per SM
+constexpr int kScanGroup = 8;                        // chunks per group
+constexpr int kScanFwdCtas = 2;                      // resident per SM
 constexpr int kScanBwdCtas = 2;
 
 // A [batch, length, dim] operand: the last dim dense, strides in elements.
@@ -101,11 +101,41 @@ __device__ __forceinline__ bool forgets(float A) { return __float_as_uint(A) == 
 __device__ __forceinline__ float map_apply(float A, float H, float s) {
   return forgets(A) ? H : fmaf(A, s, H);
 }
-// (A, H) after (A1, H1)
+// (A, H) after (A1, H1); branch-free, as these run in long dependent chains
 __device__ __forceinline__ void map_compose(float& A, float& H, float A1, float H1) {
-  if (!forgets(A)) {
-    H = fmaf(A, H1, H);
-    A = forgets(A1) ? -0.0f : A * A1;
+  const bool f = forgets(A);
+  H = f ? H : fmaf(A, H1, H);
+  A = f || forgets(A1) ? -0.0f : A * A1;
+}
+// The composition of N maps in a column of shared memory (row stride in floats),
+// the first applied first; all of them are read before the first is used.
+template <int N, bool REVERSE>
+__device__ __forceinline__ void map_compose_column(const float* a, const float* h, int stride,
+                                                   float& A, float& H) {
+  float va[N], vh[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    va[i] = a[(REVERSE ? N - 1 - i : i) * stride];
+    vh[i] = h[(REVERSE ? N - 1 - i : i) * stride];
+  }
+  A = va[N - 1];
+  H = vh[N - 1];
+#pragma unroll
+  for (int i = N - 2; i >= 0; --i) map_compose(A, H, va[i], vh[i]);
+}
+// Replaces h of the N maps by the argument each gets, starting from s.
+template <int N, bool REVERSE>
+__device__ __forceinline__ void map_arguments_column(const float* a, float* h, int stride, float s) {
+  float va[N], vh[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    va[i] = a[(REVERSE ? N - 1 - i : i) * stride];
+    vh[i] = h[(REVERSE ? N - 1 - i : i) * stride];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    h[(REVERSE ? N - 1 - i : i) * stride] = s;
+    s = map_apply(va[i], vh[i], s);
   }
 }
 
@@ -145,13 +175,15 @@ __device__ __forceinline__ float word_hi(unsigned long long w) {
   return __uint_as_float((uint32_t)(w >> 32));
 }
 
-// Bounds a spin: false once kWaitTimeoutNs have passed since the first call.
+// Bounds a spin: false once kWaitCycles (some four seconds) have passed since the
+// first call.  The SM's own clock: the global timer takes far longer to read.
+constexpr long long kWaitCycles = 8000000000ll;
 struct Patience {
-  unsigned long long t0 = 0;
+  long long t0 = 0;
   __device__ __forceinline__ bool more() {
-    const unsigned long long t = globaltimer_ns();
+    const long long t = clock64();
     if (t0 == 0) t0 = t;
-    if (t - t0 <= kWaitTimeoutNs) return true;
+    if (t - t0 <= kWaitCycles) return true;
     atomicOr(&g_kernel_error, OXC_KERR_PIPELINE_TIMEOUT);
     return false;
   }
@@ -169,16 +201,19 @@ __device__ __forceinline__ unsigned long long word_wait(const unsigned long long
 }
 
 // The state entering group g >= 0 at channel offset `off`.
-__device__ __forceinline__ float chain_enter_group(const Chain& c, int64_t g, int64_t off,
+__device__ __forceinline__ float chain_enter_group(const Chain& c, int g, int64_t off,
                                                    float first) {
   constexpr int kBack = 4;
   Patience patience;
-  while (g > 0) {
+  if (g == 0) return first;
+  const unsigned long long* pe = c.enter + g * c.stride + off;
+  const unsigned long long* pm = c.group + (g - 1) * c.stride + off;
+  for (;;) {
     unsigned long long e[kBack], m[kBack];
 #pragma unroll
     for (int i = 0; i < kBack; ++i) {  // e[i]: entering g - i; m[i]: the group before it
-      e[i] = g - i > 0 ? word_load(c.enter + (g - i) * c.stride + off) : 0ull;
-      m[i] = g - i > 0 ? word_load(c.group + (g - i - 1) * c.stride + off) : 0ull;
+      e[i] = g - i > 0 ? word_load(pe - i * c.stride) : 0ull;
+      m[i] = g - i > 0 && i + 1 < kBack ? word_load(pm - i * c.stride) : 0ull;
     }
     int at = kBack;
 #pragma unroll
@@ -197,103 +232,124 @@ __device__ __forceinline__ float chain_enter_group(const Chain& c, int64_t g, in
     }
     if (!patience.more()) return __uint_as_float(0x7fffffffu);
   }
-  return first;
 }
 
-// Called by one thread per channel with the map (A, H) of chunk k: publishes what
-// later chunks need and returns the state entering chunk k.
-__device__ __forceinline__ float chain_state(const Chain& c, int64_t k, int64_t chunks,
-                                             int64_t off, float A, float H, float first) {
-  constexpr int kBatch = 5;  // maps in flight
-  const int64_t g = k / kScanGroup, k0 = g * kScanGroup;
-  const bool ends_group = k + 1 - k0 == kScanGroup;
-  if (k + 1 < chunks) {
-    if (!ends_group) {
-      map_store(c.map + k * c.stride + off, A, H);
-    } else {
-      // the group's map, composed from its last chunk backwards
-      for (int64_t j = k - 1; j >= k0; j -= kBatch) {
-        unsigned long long w[kBatch];
+// The state entering chunk k comes together from two sets of threads, one thread
+// per channel each:
+// chain_maps, with the map (A, H) of chunk k, publishes what later chunks need
+// and leaves the maps of the chunks before k in its group in `before` [kScanGroup -
+// 1][channels], a column per channel;
+// chain_enter publishes and returns the state entering the group.
+// Applying the former to the latter, chain_state, gives the state.  Both are
+// waits on other CTAs' words, hence side by side.
+template <int CHANNELS>
+__device__ __forceinline__ void chain_maps(const Chain& c, int k, int chunks, int64_t off,
+                                           float A, float H, float2 (*before)[CHANNELS],
+                                           int channel) {
+  constexpr int kBatch = 8;  // maps in flight
+  const int n = k % kScanGroup;
+  const bool ends_group = n + 1 == kScanGroup;
+  const unsigned long long* p = c.map + (k - n) * c.stride + off;
+  if (k + 1 < chunks && !ends_group) map_store(c.map + k * c.stride + off, A, H);
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) w[i] = word_load(c.map + (j - i) * c.stride + off);
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          w[i] = word_wait(c.map + (j - i) * c.stride + off, w[i]);
-          map_compose(A, H, word_lo(w[i]), word_hi(w[i]));
-        }
-      }
-      map_store(c.group + g * c.stride + off, A, H);
-    }
-  }
-  float s = chain_enter_group(c, g, off, first);
-  if (k == k0 && g > 0 && k + 1 < chunks) word_store(c.enter + g * c.stride + off, 0.0f, s);
-  for (int64_t j = k0; j < k; j += kBatch) {
+  for (int j0 = 0; j0 < kScanGroup - 1; j0 += kBatch) {
     unsigned long long w[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
-      w[i] = j + i < k ? word_load(c.map + (j + i) * c.stride + off) : 0ull;
+      w[i] = j0 + i < n ? word_load(p + (j0 + i) * c.stride) : 0ull;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      if (j + i < k) {
-        w[i] = word_wait(c.map + (j + i) * c.stride + off, w[i]);
-        s = map_apply(word_lo(w[i]), word_hi(w[i]), s);
+      if (j0 + i < n) {
+        w[i] = word_wait(p + (j0 + i) * c.stride, w[i]);
+        before[j0 + i][channel] = make_float2(word_lo(w[i]), word_hi(w[i]));
       }
     }
   }
+  if (k + 1 < chunks && ends_group) {
+    for (int j = n - 1; j >= 0; --j) map_compose(A, H, before[j][channel].x, before[j][channel].y);
+    map_store(c.group + k / kScanGroup * c.stride + off, A, H);
+  }
+}
+
+__device__ __forceinline__ float chain_enter(const Chain& c, int k, int chunks, int64_t off,
+                                             float first) {
+  const int g = k / kScanGroup;
+  const float s = chain_enter_group(c, g, off, first);
+  if (k % kScanGroup == 0 && g > 0 && k + 1 < chunks)
+    word_store(c.enter + g * c.stride + off, 0.0f, s);
   return s;
 }
-static_assert((kScanGroup - 1) % 5 == 0, "a group's maps are read in batches of 5");
+
+template <int CHANNELS>
+__device__ __forceinline__ float chain_state(int k, const float2 (*before)[CHANNELS],
+                                             int channel, float s) {
+  const int n = k % kScanGroup;
+#pragma unroll
+  for (int j = 0; j < kScanGroup - 1; ++j) {
+    const float2 m = before[j][channel];  // (not written beyond n)
+    s = j < n ? map_apply(m.x, m.y, s) : s;
+  }
+  return s;
+}
 
 // ---- tiles -------------------------------------------------------------------------------
 
 struct Tile {
-  int64_t chunk, b, d0;
+  int chunk, b, d0, rank;  // rank: the tile's place in the order; negative at the end
 };
 
 // Hands out tiles to persistent CTAs, in the order of the scan: every batch row
 // and channel tile of a chunk before the next chunk, so whatever a tile waits
 // for belongs to a tile handed out before it, and the earliest unfinished tile
 // never waits.  The ticket for the next tile is drawn while the current one is
-// computed.  Without a chain (one chunk) the tiles are strided over the grid.
+// written, not before: a CTA that held one while it still waited for its state
+// delayed every later tile (238 us instead of 182 at [1, 65537, 1024] bf16).
+// Without a chain (one chunk) the tiles are strided over the grid.  One thread
+// draws, works out the coordinates and posts them.
 struct Tiles {
-  unsigned int* next;  // shared
-  unsigned int drawn;
+  Tile* next;  // shared
+  unsigned int drawn, dtiles, per, tiles;
+  int channels;
 
+  __device__ __forceinline__ bool mine() const { return threadIdx.x == blockDim.x - 1; }
   __device__ __forceinline__ void draw(const Chain& c, unsigned int now) {
-    if (threadIdx.x == blockDim.x - 1)
-      drawn = c.ticket ? atomicAdd(c.ticket, 1u) + 1u : now + gridDim.x;
+    if (mine()) drawn = c.ticket ? atomicAdd(c.ticket, 1u) + 1u : now + gridDim.x;
   }
   __device__ __forceinline__ void post() {
-    if (threadIdx.x == blockDim.x - 1) *next = drawn;
+    if (mine()) {
+      const unsigned int chunk = drawn / per, rest = drawn - chunk * per, b = rest / dtiles;
+      *next = {(int)chunk, (int)b, (int)(rest - b * dtiles) * channels,
+               drawn < tiles ? (int)drawn : -1};
+    }
   }
 };
 
-__device__ __forceinline__ Tile tile_at(unsigned int id, int64_t batch, int64_t dtiles,
-                                        int channels) {
-  const uint32_t per = (uint32_t)(batch * dtiles), chunk = id / per, rest = id - chunk * per;
-  const uint32_t b = rest / (uint32_t)dtiles;
-  return {chunk, b, (int64_t)(rest - b * (uint32_t)dtiles) * channels};
-}
-
 // VW channels of one token as loaded.  VEC: consecutive ones, in one access; else
-// 32 apart (lane l takes l, l + 32, ...), each guarded.  The loads are predicated
-// rather than branched around, so that all of a thread's loads are in flight
-// before the first is used.
+// 32 apart (lane l takes l, l + 32, ...).  load_some takes the first `live` of
+// them and `fill` for the rest; its loads are predicated rather than branched
+// around, so that all of a thread's loads are in flight before the first is used.
 template <typename T, int VW, bool VEC>
 struct Raw;
 
 template <int VW, bool VEC>
 struct Raw<float, VW, VEC> {
   float v[VW];
-  __device__ __forceinline__ void fill(float f) {
+  __device__ __forceinline__ void load(const float* p) {
+    if constexpr (VEC) {
+      load_as_f32<VW>(v, p);
+    } else {
 #pragma unroll
-    for (int k = 0; k < VW; ++k) v[k] = f;
+      for (int k = 0; k < VW; ++k) v[k] = ld_stream(p + 32 * k);
+    }
   }
-  __device__ __forceinline__ void load(const float* p, int live) {
+  __device__ __forceinline__ void load_some(const float* p, int live, float fill) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) v[k] = fill;
     if constexpr (VEC && VW == 4) {
       asm("{.reg .pred p; setp.gt.s32 p, %5, 0; @p ld.global.cs.v4.f32 {%0, %1, %2, %3}, [%4];}"
           : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]) : "l"(p), "r"(live));
-    } else if constexpr (VEC && VW == 2) {
+    } else if constexpr (VEC) {
+      static_assert(!VEC || VW == 2 || VW == 4, "vectors of 2 or 4 channels");
       asm("{.reg .pred p; setp.gt.s32 p, %3, 0; @p ld.global.cs.v2.f32 {%0, %1}, [%2];}"
           : "+f"(v[0]), "+f"(v[1]) : "l"(p), "r"(live));
     } else {
@@ -308,17 +364,28 @@ struct Raw<float, VW, VEC> {
 
 template <int VW, bool VEC>
 struct Raw<bf16, VW, VEC> {
-  uint32_t w[VEC ? VW / 2 : VW];  // two to a word, or one in the upper half
-  __device__ __forceinline__ void fill(float f) {
-    const uint32_t u = __float_as_uint(f);  // 0 or infinity: the lower half is 0
+  uint32_t w[VEC ? VW / 2 : VW];  // two to a word, or one in the lower half
+  __device__ __forceinline__ void load(const bf16* p) {
+    if constexpr (VEC && VW == 4) {
+      const uint2 t = __ldcs(reinterpret_cast<const uint2*>(p));
+      w[0] = t.x;
+      w[1] = t.y;
+    } else if constexpr (VEC) {
+      w[0] = __ldcs(reinterpret_cast<const uint32_t*>(p));
+    } else {
+#pragma unroll
+      for (int k = 0; k < VW; ++k) w[k] = __ldcs(reinterpret_cast<const unsigned short*>(p + 32 * k));
+    }
+  }
+  __device__ __forceinline__ void load_some(const bf16* p, int live, float fill) {
+    const uint32_t u = __float_as_uint(fill);  // 0 or infinity: the lower half is 0
 #pragma unroll
     for (int k = 0; k < (VEC ? VW / 2 : VW); ++k) w[k] = VEC ? u | (u >> 16) : u >> 16;
-  }
-  __device__ __forceinline__ void load(const bf16* p, int live) {
     if constexpr (VEC && VW == 4) {
       asm("{.reg .pred p; setp.gt.s32 p, %3, 0; @p ld.global.cs.v2.u32 {%0, %1}, [%2];}"
           : "+r"(w[0]), "+r"(w[1]) : "l"(p), "r"(live));
-    } else if constexpr (VEC && VW == 2) {
+    } else if constexpr (VEC) {
+      static_assert(!VEC || VW == 2 || VW == 4, "vectors of 2 or 4 channels");
       asm("{.reg .pred p; setp.gt.s32 p, %2, 0; @p ld.global.cs.u32 %0, [%1];}"
           : "+r"(w[0]) : "l"(p), "r"(live));
     } else {
@@ -410,41 +477,53 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_fwd_kernel(
     SeqView<T> x, SeqView<T> gate, const uint8_t* __restrict__ starts,
     const float* __restrict__ h0, T* __restrict__ h, float* __restrict__ last,
     float* __restrict__ carry, Chain chain, int64_t batch, int64_t length, int64_t dim,
-    int64_t chunks, int64_t dtiles, unsigned int tiles) {
+    int chunks, unsigned int dtiles,
+    unsigned int tiles) {
   using L = Lane<T, VW, VEC>;
   using R = Raw<T, VW, VEC>;
   constexpr int P = VW / 2;
   __shared__ __align__(16) float mapA[kScanWarps][L::kChannels];
   __shared__ __align__(16) float mapH[kScanWarps][L::kChannels];
-  __shared__ unsigned int next;
-  Tiles order{&next, blockIdx.x};
+  __shared__ float2 before[kScanGroup - 1][L::kChannels];
+  __shared__ float enter[L::kChannels];
+  __shared__ __align__(16) Tile next;
+  Tiles order{&next, blockIdx.x, dtiles, (unsigned int)batch * dtiles, tiles, L::kChannels};
   const int warp = threadIdx.x >> 5;
   if (chain.ticket) order.draw(chain, 0u);
   order.post();
   for (;;) {
     __syncthreads();  // `next` is posted, the maps of the tile before are read
-    const unsigned int id = next;
-    if (id >= tiles) return;
-    const Tile tile = tile_at(id, batch, dtiles, L::kChannels);
+    const Tile tile = next;
+    if (tile.rank < 0) return;
     const L lane(tile.d0, dim);
-    const int64_t t0 = tile.chunk * kScanChunk + warp * kScanSteps;
+    const int64_t t0 = (int64_t)tile.chunk * kScanChunk + warp * kScanSteps;
+    const int64_t row0 = tile.b * length + t0;
     const int steps = (int)max((int64_t)0, min((int64_t)kScanSteps, length - t0));
     R rg[kScanSteps], rx[kScanSteps];
     {
-      const T* pg = gate.p + tile.b * gate.sb + t0 * gate.st + lane.d;
+      const T* pg = gate.p + (int64_t)tile.b * gate.sb + t0 * gate.st + lane.d;
       const T* px = x.p + tile.b * x.sb + t0 * x.st + lane.d;
+      const bool whole = steps == kScanSteps && tile.d0 + L::kChannels <= dim;
+      if (whole) {
 #pragma unroll
-      for (int i = 0; i < kScanSteps; ++i) {
-        rg[i].fill(INFINITY);
-        rx[i].fill(0.0f);
-        rg[i].load(pg, i < steps ? lane.live : 0);
-        rx[i].load(px, i < steps ? lane.live : 0);
-        pg += gate.st;
-        px += x.st;
+        for (int i = 0; i < kScanSteps; ++i) {
+          rg[i].load(pg);
+          rx[i].load(px);
+          pg += gate.st;
+          px += x.st;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kScanSteps; ++i) {
+          const int live = i < steps ? lane.live : 0;
+          rg[i].load_some(pg, live, INFINITY);
+          rx[i].load_some(px, live, 0.0f);
+          pg += gate.st;
+          px += x.st;
+        }
       }
     }
     const unsigned int fresh = start_bits(starts, tile.b, t0, length);
-    order.draw(chain, id);
     float2 a[kScanSteps][P], v[kScanSteps][P], A[P], H[P];
 #pragma unroll
     for (int j = 0; j < P; ++j) { A[j] = f2(1.0f); H[j] = f2(0.0f); }
@@ -469,30 +548,30 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_fwd_kernel(
     lane.put(mapA[warp], A);
     lane.put(mapH[warp], H);
     __syncthreads();
-    order.post();
-    const int c = threadIdx.x;
-    if (c < L::kChannels && tile.d0 + c < dim) {
-      const int64_t off = tile.b * dim + tile.d0 + c;
-      float s = h0 ? h0[off] : 0.0f;
-      if (chunks > 1) {
-        float tA = mapA[kScanWarps - 1][c], tH = mapH[kScanWarps - 1][c];
-#pragma unroll
-        for (int w = kScanWarps - 2; w >= 0; --w) map_compose(tA, tH, mapA[w][c], mapH[w][c]);
-        s = chain_state(chain, tile.chunk, chunks, off, tA, tH, s);
-      }
-      if (carry) carry[(tile.b * chunks + tile.chunk) * dim + tile.d0 + c] = s;
-#pragma unroll
-      for (int w = 0; w < kScanWarps; ++w) {  // mapH becomes the state entering warp w
-        const float after = map_apply(mapA[w][c], mapH[w][c], s);
-        mapH[w][c] = s;
-        s = after;
-      }
+    const int c = threadIdx.x % L::kChannels, part = threadIdx.x / L::kChannels;
+    const bool mine = tile.d0 + c < dim;
+    const int64_t off = tile.b * dim + tile.d0 + c;
+    if (mine && part == 0 && chunks > 1) {
+      float tA, tH;
+      map_compose_column<kScanWarps, false>(&mapA[0][c], &mapH[0][c], L::kChannels, tA, tH);
+      chain_maps(chain, tile.chunk, chunks, off, tA, tH, before, c);
+    } else if (mine && part == 1) {
+      const float s = h0 ? h0[off] : 0.0f;
+      enter[c] = chunks > 1 ? chain_enter(chain, tile.chunk, chunks, off, s) : s;
     }
     __syncthreads();
+    if (mine && part == 0) {
+      const float s = chain_state(tile.chunk, before, c, enter[c]);
+      if (carry) carry[((int64_t)tile.b * chunks + tile.chunk) * dim + tile.d0 + c] = s;
+      // mapH becomes the state entering each warp
+      map_arguments_column<kScanWarps, false>(&mapA[0][c], &mapH[0][c], L::kChannels, s);
+    }
+    __syncthreads();
+    order.draw(chain, tile.rank);
     float2 s[P];
     lane.get(mapH[warp], s);
     by_fresh(fresh, [&](auto some) {
-      T* ph = h + (tile.b * length + t0) * dim;
+      T* ph = h + row0 * dim;
 #pragma unroll
       for (int i = 0; i < kScanSteps; ++i) {
 #pragma unroll
@@ -510,6 +589,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_fwd_kernel(
         if (k < lane.live)
           last[tile.b * dim + tile.d0 + lane.channel(k)] = k & 1 ? s[k / 2].y : s[k / 2].x;
     }
+    order.post();
   }
 }
 
@@ -518,7 +598,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
     SeqView<T> x, SeqView<T> gate, const uint8_t* __restrict__ starts,
     const float* __restrict__ carry, SeqView<T> dh, const float* __restrict__ dlast,
     T* __restrict__ dx, T* __restrict__ dgate, float* __restrict__ dh0, Chain chain, int64_t batch,
-    int64_t length, int64_t dim, int64_t chunks, int64_t dtiles, unsigned int tiles) {
+    int64_t length, int64_t dim, int chunks, unsigned int dtiles,
+    unsigned int tiles) {
   using L = Lane<T, VW, VEC>;
   using R = Raw<T, VW, VEC>;
   constexpr int P = VW / 2;
@@ -527,40 +608,52 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
   __shared__ __align__(16) float mapA[kScanWarps][L::kChannels];
   __shared__ __align__(16) float mapS[kScanWarps][L::kChannels];
   __shared__ __align__(16) float mapM[kScanWarps][L::kChannels];
-  __shared__ unsigned int next;
-  Tiles order{&next, blockIdx.x};
+  __shared__ float2 before[kScanGroup - 1][L::kChannels];
+  __shared__ float enter[L::kChannels];
+  __shared__ __align__(16) Tile next;
+  Tiles order{&next, blockIdx.x, dtiles, (unsigned int)batch * dtiles, tiles, L::kChannels};
   const int warp = threadIdx.x >> 5;
   if (chain.ticket) order.draw(chain, 0u);
   order.post();
   for (;;) {
     __syncthreads();  // `next` is posted, the maps of the tile before are read
-    const unsigned int id = next;
-    if (id >= tiles) return;
-    Tile tile = tile_at(id, batch, dtiles, L::kChannels);
+    Tile tile = next;
+    if (tile.rank < 0) return;
     tile.chunk = chunks - 1 - tile.chunk;  // from the end of the sequence
     const L lane(tile.d0, dim);
-    const int64_t t0 = tile.chunk * kScanChunk + warp * kScanSteps;
+    const int64_t t0 = (int64_t)tile.chunk * kScanChunk + warp * kScanSteps;
+    const int64_t row0 = tile.b * length + t0;
     const int steps = (int)max((int64_t)0, min((int64_t)kScanSteps, length - t0));
     R rg[kScanSteps], rx[kScanSteps], rd[kScanSteps];
     {
-      const T* pg = gate.p + tile.b * gate.sb + t0 * gate.st + lane.d;
+      const T* pg = gate.p + (int64_t)tile.b * gate.sb + t0 * gate.st + lane.d;
       const T* px = x.p + tile.b * x.sb + t0 * x.st + lane.d;
       const T* pd = dh.p + tile.b * dh.sb + t0 * dh.st + lane.d;
+      const bool whole = steps == kScanSteps && tile.d0 + L::kChannels <= dim && dh.p;
+      if (whole) {
 #pragma unroll
-      for (int i = 0; i < kScanSteps; ++i) {
-        rg[i].fill(INFINITY);
-        rx[i].fill(0.0f);
-        rd[i].fill(0.0f);
-        rg[i].load(pg, i < steps ? lane.live : 0);
-        rx[i].load(px, i < steps ? lane.live : 0);
-        rd[i].load(pd, i < steps && dh.p ? lane.live : 0);
-        pg += gate.st;
-        px += x.st;
-        pd += dh.st;
+        for (int i = 0; i < kScanSteps; ++i) {
+          rg[i].load(pg);
+          rd[i].load(pd);
+          rx[i].load(px);
+          pg += gate.st;
+          pd += dh.st;
+          px += x.st;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kScanSteps; ++i) {
+          const int live = i < steps ? lane.live : 0;
+          rg[i].load_some(pg, live, INFINITY);
+          rd[i].load_some(pd, dh.p ? live : 0, 0.0f);
+          rx[i].load_some(px, live, 0.0f);
+          pg += gate.st;
+          pd += dh.st;
+          px += x.st;
+        }
       }
     }
     const unsigned int fresh = start_bits(starts, tile.b, t0, length);
-    order.draw(chain, id);
     float2 a[kScanSteps][P], b[kScanSteps][P], A[P], S[P], M[P];
 #pragma unroll
     for (int j = 0; j < P; ++j) { A[j] = f2(1.0f); S[j] = M[j] = f2(0.0f); }
@@ -590,37 +683,31 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
     lane.put(mapS[warp], S);
     lane.put(mapM[warp], M);
     __syncthreads();
-    order.post();
-    // the mu of the chunk after this one and the state before it, by two sets of
-    // threads
+    // the mu of the chunk after this one (two sets of threads) and the state before
+    // it (a third)
     const int c = threadIdx.x % L::kChannels, part = threadIdx.x / L::kChannels;
-    if (part < 2 && tile.d0 + c < dim) {
-      const int64_t off = tile.b * dim + tile.d0 + c;
-      if (part == 0) {
-        float m = dlast ? dlast[off] : 0.0f;
-        if (chunks > 1) {
-          float tA = mapA[0][c], tM = mapM[0][c];
-#pragma unroll
-          for (int w = 1; w < kScanWarps; ++w) map_compose(tA, tM, mapA[w][c], mapM[w][c]);
-          m = chain_state(chain, chunks - 1 - tile.chunk, chunks, off, tA, tM, m);
-        }
-#pragma unroll
-        for (int w = kScanWarps - 1; w >= 0; --w) {
-          const float before = map_apply(mapA[w][c], mapM[w][c], m);
-          mapM[w][c] = m;
-          m = before;
-        }
-      } else {
-        float s = carry[(tile.b * chunks + tile.chunk) * dim + tile.d0 + c];
-#pragma unroll
-        for (int w = 0; w < kScanWarps; ++w) {
-          const float after = map_apply(mapA[w][c], mapS[w][c], s);
-          mapS[w][c] = s;
-          s = after;
-        }
-      }
+    const bool mine = tile.d0 + c < dim;
+    const int64_t off = tile.b * dim + tile.d0 + c;
+    const int k = chunks - 1 - tile.chunk;
+    if (mine && part == 0 && chunks > 1) {
+      float tA, tM;
+      map_compose_column<kScanWarps, true>(&mapA[0][c], &mapM[0][c], L::kChannels, tA, tM);
+      chain_maps(chain, k, chunks, off, tA, tM, before, c);
+    } else if (mine && part == 1) {
+      const float m = dlast ? dlast[off] : 0.0f;
+      enter[c] = chunks > 1 ? chain_enter(chain, k, chunks, off, m) : m;
+    } else if (mine && part == 2) {
+      map_arguments_column<kScanWarps, false>(
+          &mapA[0][c], &mapS[0][c], L::kChannels,
+          carry[((int64_t)tile.b * chunks + tile.chunk) * dim + tile.d0 + c]);
     }
     __syncthreads();
+    if (mine && part == 0) {
+      const float m = chain_state(k, before, c, enter[c]);
+      map_arguments_column<kScanWarps, true>(&mapA[0][c], &mapM[0][c], L::kChannels, m);
+    }
+    __syncthreads();
+    order.draw(chain, tile.rank);
     float2 s[P], m[P], gap[kScanSteps][P];  // gap: h_{t-1} - x_t, what d h_t / d a_t is
     lane.get(mapS[warp], s);
     lane.get(mapM[warp], m);
@@ -634,8 +721,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
           gap[i][j] = __fadd2_rn(s[j], make_float2(-v.x, -v.y));
           s[j] = __ffma2_rn(a[i][j], s[j], __fmul2_rn(b[i][j], v));
         }
-      T* px = dx + (tile.b * length + t0 + kScanSteps - 1) * dim;
-      T* pg = dgate + (tile.b * length + t0 + kScanSteps - 1) * dim;
+      T* px = dx + (row0 + kScanSteps - 1) * dim;
+      T* pg = dgate + (row0 + kScanSteps - 1) * dim;
 #pragma unroll
       for (int i = kScanSteps - 1; i >= 0; --i) {
         float2 ox[P], og[P];
@@ -661,6 +748,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
         if (k < lane.live)
           dh0[tile.b * dim + tile.d0 + lane.channel(k)] = k & 1 ? m[k / 2].y : m[k / 2].x;
     }
+    order.post();
   }
 }
 
@@ -757,8 +845,8 @@ static oxc_status scan_fwd_launch(const void* x, int64_t x_sb, int64_t x_st, con
   const SeqView<T> xv{static_cast<const T*>(x), x_sb, x_st};
   const SeqView<T> gv{static_cast<const T*>(gate), g_sb, g_st};
   kernel<<<grid, kScanWarps * 32, 0, s>>>(xv, gv, starts, h0, static_cast<T*>(h), last, carry,
-                                          chain, batch, length, dim, scan_chunks(length), dtiles,
-                                          tiles);
+                                          chain, batch, length, dim, (int)scan_chunks(length),
+                                          (unsigned)dtiles, tiles);
   return check_launch("oxc_gated_scan_fwd");
 }
 
@@ -784,7 +872,8 @@ static oxc_status scan_bwd_launch(const void* x, int64_t x_sb, int64_t x_st, con
   const SeqView<T> dv{static_cast<const T*>(dh), dh_sb, dh_st};
   kernel<<<grid, kScanWarps * 32, 0, s>>>(xv, gv, starts, carry, dv, dlast, static_cast<T*>(dx),
                                           static_cast<T*>(dgate), dh0, chain, batch, length, dim,
-                                          scan_chunks(length), dtiles, tiles);
+                                          (int)scan_chunks(length),
+                                          (unsigned)dtiles, tiles);
   return check_launch("oxc_gated_scan_bwd");
 }
 
