@@ -9,6 +9,14 @@
 // An entry is absent when its id is negative or its logit is -inf; a row with
 // no entry has loss 0 and gradient 0, whatever its logits hold.  An id listed
 // twice counts twice.
+//
+// Bound by HBM: 2 sizeof(T) bytes a logit, the row read once and its gradient
+// written once.  So a row stays in registers between the two: a cluster of 1 to 8
+// CTAs shares it, 32 logits a thread, as exponentials relative to the CTA's own
+// maximum; (max, sum) pairs are exchanged through distributed shared memory, and
+// one multiplication an element remains.  Rows wider than that (262144) take the
+// three-pass kernel, which re-reads them from L2 or HBM.
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include <algorithm>
@@ -18,6 +26,9 @@
 namespace oxc {
 
 constexpr int kDistillMaxTop = 4096;
+constexpr int kDistillEach = 32;      // logits per thread
+constexpr int kDistillCluster = 8;    // CTAs per row at most
+constexpr int kDistillMaxThreads = 1024;
 
 // Records the first bad id: flag[0] = 2 (dim 1), flag[1..2] = id, flag[3] = vocab.
 __device__ __forceinline__ void record_bad_id(int32_t* flag, int64_t id, int64_t vocab) {
@@ -28,78 +39,324 @@ __device__ __forceinline__ void record_bad_id(int32_t* flag, int64_t id, int64_t
   }
 }
 
-// One CTA per row, three passes over it.
+// exp(d / tau) for d = x - max <= 0, c = log2(e) / tau.  The subtraction comes
+// first, so the large terms see only ex2's own error; results below 2^-126 are 0.
+__device__ __forceinline__ float exp_scaled(float d, float c) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * c));
+  return r;
+}
+
+// The teacher's side of a row, in shared memory: prob[k] (0 for absent entries)
+// and id[k] (-1).
+struct Teacher {
+  float* prob;
+  int* id;
+  int* table;  // hash of the ids, 2^bits entries
+  int bits;
+};
+
+__host__ __device__ inline int teacher_bits(int top) {
+  int b = 5;
+  while ((1 << b) < 2 * top) ++b;
+  return b;
+}
+__host__ __device__ inline size_t teacher_smem(int top) {
+  return (size_t)top * 8 + (sizeof(int) << teacher_bits(top));
+}
+
+struct TeacherRow {
+  float log_sum;  // of exp((t - max) / tau)
+  float max;
+  bool none, bad, repeated;
+};
+
+// Fills the teacher's side of one row; every thread gets the summary.
+__device__ __forceinline__ TeacherRow teacher_row(const Teacher& s, const float* tl,
+                                                  const int64_t* ti, int top, float c, int vocab,
+                                                  int32_t* err, float* scratch) {
+  TeacherRow r;
+  for (int i = threadIdx.x; i < (1 << s.bits); i += blockDim.x) s.table[i] = -1;
+  float tm = -INFINITY;
+  int bad = 0;
+  for (int k = threadIdx.x; k < top; k += blockDim.x) {
+    const int64_t id = ti[k];
+    const float v = id >= 0 ? tl[k] : -INFINITY;
+    if (id >= vocab) { record_bad_id(err, id, vocab); bad = 1; }
+    if (v != v) bad = 1;
+    s.id[k] = id >= 0 && id < vocab && v != -INFINITY ? (int)id : -1;
+    s.prob[k] = v;
+    tm = fmaxf(tm, v);
+  }
+  r.bad = __syncthreads_or(bad);
+  tm = block_max(tm, scratch);
+  r.max = tm;
+  r.none = tm == -INFINITY && !r.bad;
+  r.repeated = false;
+  r.log_sum = 0.0f;
+  if (r.none || r.bad) return r;
+  float ts = 0.0f;
+  int twice = 0;
+  for (int k = threadIdx.x; k < top; k += blockDim.x) {
+    const float e = exp_scaled(s.prob[k] - tm, c);
+    s.prob[k] = e;
+    ts += e;
+    const int id = s.id[k];
+    if (id >= 0) {  // insert; finding the id there already means it is listed twice
+      unsigned int h = ((unsigned int)id * 2654435769u) >> (32 - s.bits);
+      for (int n = 0; n < (1 << s.bits); ++n) {
+        const int was = atomicCAS(&s.table[h], -1, id);
+        if (was == -1) break;
+        if (was == id) { twice = 1; break; }
+        h = (h + 1) & ((1u << s.bits) - 1);
+      }
+    }
+  }
+  ts = block_sum(ts, scratch);
+  r.repeated = __syncthreads_or(twice);
+  r.log_sum = logf(ts);
+  const float inv = __fdiv_rn(1.0f, ts);
+  for (int k = threadIdx.x; k < top; k += blockDim.x) s.prob[k] *= inv;
+  __syncthreads();
+  return r;
+}
+
+// The probability that all entries of s.id[k]'s token have together, 0 if an
+// earlier entry is that token's; in the order of the entries.
+__device__ __forceinline__ float teacher_prob(const Teacher& s, const TeacherRow& r, int k, int top,
+                                              bool* first) {
+  *first = true;
+  if (!r.repeated) return s.prob[k];
+  float p = 0.0f;
+  for (int j = 0; j < top; ++j) {
+    if (s.id[j] != s.id[k]) continue;
+    if (j < k) *first = false;
+    p += s.prob[j];
+  }
+  return p;
+}
+
+// This thread's share of sum_k p_k (log p_k - log q_k).
+__device__ __forceinline__ float teacher_loss(const Teacher& s, const TeacherRow& r, const float* tl,
+                                              int top, float inv_tau, float log_q0,
+                                              float (*logit)(const void*, int), const void* row,
+                                              float m) {
+  float loss = 0.0f;
+  for (int k = threadIdx.x; k < top; k += blockDim.x) {
+    const float p = s.prob[k];
+    if (s.id[k] >= 0 && p > 0.0f)
+      loss += p * (((tl[k] - r.max) * inv_tau - r.log_sum) -
+                   ((logit(row, s.id[k]) - m) * inv_tau - log_q0));
+  }
+  return loss;
+}
 template <typename T>
-__global__ void __launch_bounds__(512) distill_kernel(
-    const T* __restrict__ logits, int64_t stride, const float* __restrict__ tl,
-    const int64_t* __restrict__ ti, int top, float inv_tau, float grad_scale,
-    const float* __restrict__ grad_loss, float* __restrict__ row_loss, T* __restrict__ dlogits,
-    int64_t rows, int vocab, int32_t* err) {
-  extern __shared__ float prob[];  // [top]
+__device__ float logit_at(const void* row, int i) {
+  return to_f32(static_cast<const T*>(row)[i]);
+}
+
+struct DistillArgs {
+  const float* tl;
+  const int64_t* ti;
+  int top;
+  float inv_tau, c;   // c = log2(e) / tau
+  float grad_scale;   // tau / total_rows
+  const float* grad_loss;
+  float* row_loss;
+  int64_t rows;
+  int vocab;
+  int32_t* err;
+};
+
+// One cluster per row.  The row's bytes are cut at 16-byte boundaries of memory:
+// `body` whole vectors, CTA r of the cluster taking [r, r + 1) / size of them,
+// thread t the vectors t, t + THREADS, ...; the elements before the first
+// boundary and after the last (fewer than a vector each) are single elements of
+// the last CTA's warp 0.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restrict__ dlogits,
+                       DistillArgs a) {
+  namespace cg = cooperative_groups;
+  constexpr int kVec = 16 / (int)sizeof(T);
+  constexpr int kVecs = kDistillEach / kVec;
+  extern __shared__ float smem[];
   __shared__ float scratch[33];
-  const float gs = grad_loss ? grad_scale * __ldg(grad_loss) : grad_scale;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const T* xr = logits + row * stride;
-    T* dr = dlogits ? dlogits + row * (int64_t)vocab : nullptr;
-    const float* tr = tl + row * top;
-    const int64_t* ir = ti + row * top;
-    // the teacher's probabilities
-    float tm = -INFINITY;
-    int bad = 0;
-    for (int k = threadIdx.x; k < top; k += blockDim.x) {
-      const int64_t id = ir[k];
-      if (id >= vocab) { record_bad_id(err, id, vocab); bad = 1; }
-      const float v = id >= 0 ? tr[k] : -INFINITY;
-      prob[k] = v;
-      tm = fmaxf(tm, v);
-      if (v != v) bad = 1;
+  __shared__ float2 mine;  // this CTA's (max, sum)
+  const Teacher teach{smem, reinterpret_cast<int*>(smem) + a.top,
+                      reinterpret_cast<int*>(smem) + 2 * a.top, teacher_bits(a.top)};
+  cg::cluster_group cluster = cg::this_cluster();
+  const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int64_t row = blockIdx.x / size;
+  const T* xr = logits + row * stride;
+  const int head = min(a.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(xr) & 15)) & 15) / (int)sizeof(T));
+  const int body = (a.vocab - head) / kVec, each = (body + size - 1) / size;
+  const int v0 = min(body, rank * each), v1 = min(body, v0 + each);
+  const int edges = a.vocab - body * kVec;  // head + tail
+  const bool has_edge = rank == size - 1 && (int)threadIdx.x < edges;
+  const int edge_at = (int)threadIdx.x < head ? threadIdx.x : body * kVec + threadIdx.x;
+  uint4 raw[kVecs];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int v = v0 + i * THREADS + threadIdx.x;
+    if (v < v1) raw[i] = __ldcs(reinterpret_cast<const uint4*>(xr + head) + v);
+  }
+  float edge = has_edge ? to_f32(xr[edge_at]) : -INFINITY;
+  const float* tl = a.tl + row * a.top;
+  const TeacherRow t = teacher_row(teach, tl, a.ti + row * a.top, a.top, a.c, a.vocab,
+                                   rank == 0 ? a.err : nullptr, scratch);
+  T* dr = dlogits ? dlogits + row * (int64_t)a.vocab : nullptr;
+  float e[kDistillEach];
+  float scale = 0.0f, base = 0.0f, row_max = 0.0f, log_sum = 0.0f;
+  if (!t.none && !t.bad) {
+    float m = edge;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      const bool in = v0 + i * THREADS + (int)threadIdx.x < v1;
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) {
+        float f;
+        if constexpr (sizeof(T) == 4) f = __uint_as_float(w[k]);
+        else f = k & 1 ? bf16_hi(w[k / 2]) : bf16_lo(w[k / 2]);
+        e[i * kVec + k] = in ? f : -INFINITY;
+        m = fmaxf(m, e[i * kVec + k]);
+      }
     }
-    bad = __syncthreads_or(bad);
-    tm = block_max(tm, scratch);
-    if (tm == -INFINITY && !bad) {
-      for (int c = threadIdx.x; dr && c < vocab; c += blockDim.x) dr[c] = from_f32<T>(0.0f);
-      if (threadIdx.x == 0) row_loss[row] = 0.0f;
-      continue;
-    }
-    float ts = 0.0f;
-    for (int k = threadIdx.x; k < top; k += blockDim.x) ts += expf((prob[k] - tm) * inv_tau);
-    ts = block_sum(ts, scratch);
-    // the student's row
-    float m = -INFINITY;
-    for (int c = threadIdx.x; c < vocab; c += blockDim.x) m = fmaxf(m, to_f32(xr[c]));
     m = block_max(m, scratch);
-    float sum = 0.0f;
-    for (int c = threadIdx.x; c < vocab; c += blockDim.x) sum += expf((to_f32(xr[c]) - m) * inv_tau);
-    sum = block_sum(sum, scratch);
-    const float log_ts = logf(ts), log_sum = logf(sum);
-    float loss = 0.0f;
-    for (int k = threadIdx.x; k < top; k += blockDim.x) {
-      const int64_t id = ir[k];
-      const float z = (prob[k] - tm) * inv_tau;
-      const float p = expf(z) / ts;
-      prob[k] = p;
-      if (id >= 0 && id < vocab && p > 0.0f)
-        loss += p * ((z - log_ts) - ((to_f32(xr[id]) - m) * inv_tau - log_sum));
+    base = m == -INFINITY ? 0.0f : m;
+    float s = has_edge ? exp_scaled(edge - base, a.c) : 0.0f;
+    edge = s;
+#pragma unroll
+    for (int i = 0; i < kDistillEach; ++i) {
+      e[i] = exp_scaled(e[i] - base, a.c);
+      s += e[i];
     }
-    loss = block_sum(loss, scratch);
-    if (threadIdx.x == 0) row_loss[row] = bad ? NAN : loss;
-    if (dr) {
-      const float inv_sum = 1.0f / sum;
-      for (int c = threadIdx.x; c < vocab; c += blockDim.x)
-        dr[c] = from_f32<T>(bad ? NAN : gs * (expf((to_f32(xr[c]) - m) * inv_tau) * inv_sum));
-      __syncthreads();
-      if (!bad) {
-        for (int k = threadIdx.x; k < top; k += blockDim.x) {
-          const int64_t id = ir[k];
-          if (id < 0) continue;
-          float p = 0.0f;  // all entries of this id, in order
-          for (int j = 0; j < top; ++j)
-            if (ir[j] == id) p += prob[j];
-          dr[id] = from_f32<T>(gs * (expf((to_f32(xr[id]) - m) * inv_tau) * inv_sum - p));
+    s = block_sum(s, scratch);
+    // the row's maximum and sum from the CTAs' (a row of -inf alone has sum NaN)
+    row_max = m;
+    float total = s;
+    if (size > 1) {
+      if (threadIdx.x == 0) mine = make_float2(m, s);
+      cluster.sync();
+      float2 part[kDistillCluster];
+#pragma unroll
+      for (int r = 0; r < kDistillCluster; ++r)
+        part[r] = r < size ? *cluster.map_shared_rank(&mine, r) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+      for (int r = 0; r < kDistillCluster; ++r) row_max = fmaxf(row_max, part[r].x);
+      total = 0.0f;
+#pragma unroll
+      for (int r = 0; r < kDistillCluster; ++r)
+        if (part[r].x != -INFINITY || part[r].y != 0.0f)
+          total += part[r].x == -INFINITY ? part[r].y
+                                          : part[r].y * exp_scaled(part[r].x - row_max, a.c);
+    }
+    if (row_max == -INFINITY) total = NAN;
+    const float gs = a.grad_loss ? a.grad_scale * __ldg(a.grad_loss) : a.grad_scale;
+    const float share = m == -INFINITY ? 1.0f : exp_scaled(m - row_max, a.c);
+    scale = gs * (share * __fdiv_rn(1.0f, total));
+    log_sum = logf(total);
+  } else {
+    const float f = t.none ? 0.0f : NAN;
+#pragma unroll
+    for (int i = 0; i < kDistillEach; ++i) e[i] = f;
+    edge = f;
+    scale = 1.0f;
+  }
+  if (dr) {
+    const bool vector = ((reinterpret_cast<uintptr_t>(dr + head) & 15) == 0);
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int v = v0 + i * THREADS + threadIdx.x;
+      if (v < v1) {
+        float g[kVec];
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) g[k] = e[i * kVec + k] * scale;
+        T* out = dr + head + (int64_t)v * kVec;
+        if (vector) {
+          store_from_f32<kVec>(out, g);
+        } else {  // the gradient's rows lie otherwise within their 16 bytes
+#pragma unroll
+          for (int k = 0; k < kVec; ++k) out[k] = from_f32<T>(g[k]);
         }
       }
     }
-    __syncthreads();  // prob is read; the next row overwrites it
+    if (has_edge) dr[edge_at] = from_f32<T>(edge * scale);
+  }
+  if (!t.none && !t.bad) {
+    // the teacher's tokens in this CTA's part: q - p instead of q, over what was
+    // just written
+    const float gs = a.grad_loss ? a.grad_scale * __ldg(a.grad_loss) : a.grad_scale;
+    if (dr) {
+      __syncthreads();
+      for (int k = threadIdx.x; k < a.top; k += THREADS) {
+        const int id = teach.id[k];
+        if (id < 0) continue;
+        const int v = id < head ? -1 : (id - head) / kVec;
+        if (v < 0 || v >= body ? rank != size - 1 : v < v0 || v >= v1) continue;
+        bool first;
+        const float p = teacher_prob(teach, t, k, a.top, &first);
+        if (first) dr[id] = from_f32<T>(exp_scaled(to_f32(xr[id]) - base, a.c) * scale - gs * p);
+      }
+    }
+    if (rank == 0) {
+      const float loss = block_sum(
+          teacher_loss(teach, t, tl, a.top, a.inv_tau, log_sum, logit_at<T>, xr, row_max), scratch);
+      if (threadIdx.x == 0) a.row_loss[row] = loss;
+    }
+  } else if (rank == 0 && threadIdx.x == 0) {
+    a.row_loss[row] = t.none ? 0.0f : NAN;
+  }
+  if (size > 1) cluster.sync();  // `mine` may still be read by the others
+}
+
+// One CTA per row at a time, three passes over it: any width.
+template <typename T>
+__global__ void __launch_bounds__(512) distill_wide_kernel(const T* __restrict__ logits,
+                                                           int64_t stride, T* __restrict__ dlogits,
+                                                           DistillArgs a) {
+  extern __shared__ float smem[];
+  __shared__ float scratch[33];
+  const Teacher teach{smem, reinterpret_cast<int*>(smem) + a.top,
+                      reinterpret_cast<int*>(smem) + 2 * a.top, teacher_bits(a.top)};
+  const float gs = a.grad_loss ? a.grad_scale * __ldg(a.grad_loss) : a.grad_scale;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* xr = logits + row * stride;
+    T* dr = dlogits ? dlogits + row * (int64_t)a.vocab : nullptr;
+    const float* tl = a.tl + row * a.top;
+    const TeacherRow t = teacher_row(teach, tl, a.ti + row * a.top, a.top, a.c, a.vocab, a.err, scratch);
+    if (t.none || t.bad) {
+      const float f = t.none ? 0.0f : NAN;
+      for (int i = threadIdx.x; dr && i < a.vocab; i += blockDim.x) dr[i] = from_f32<T>(f);
+      if (threadIdx.x == 0) a.row_loss[row] = f;
+      __syncthreads();
+      continue;
+    }
+    float m = -INFINITY;
+    for (int i = threadIdx.x; i < a.vocab; i += blockDim.x) m = fmaxf(m, to_f32(xr[i]));
+    m = block_max(m, scratch);
+    float sum = 0.0f;
+    for (int i = threadIdx.x; i < a.vocab; i += blockDim.x)
+      sum += exp_scaled(to_f32(xr[i]) - m, a.c);
+    sum = block_sum(sum, scratch);
+    if (dr) {
+      const float scale = gs * __fdiv_rn(1.0f, sum);
+      for (int i = threadIdx.x; i < a.vocab; i += blockDim.x)
+        dr[i] = from_f32<T>(exp_scaled(to_f32(xr[i]) - m, a.c) * scale);
+      __syncthreads();
+      for (int k = threadIdx.x; k < a.top; k += blockDim.x) {
+        const int id = teach.id[k];
+        if (id < 0) continue;
+        bool first;
+        const float p = teacher_prob(teach, t, k, a.top, &first);
+        if (first) dr[id] = from_f32<T>(exp_scaled(to_f32(xr[id]) - m, a.c) * scale - gs * p);
+      }
+    }
+    const float loss = block_sum(
+        teacher_loss(teach, t, tl, a.top, a.inv_tau, logf(sum), logit_at<T>, xr, m), scratch);
+    if (threadIdx.x == 0) a.row_loss[row] = loss;
+    __syncthreads();  // the teacher's side is read; the next row overwrites it
   }
 }
 
@@ -108,6 +365,7 @@ __global__ void __launch_bounds__(1024) distill_loss_kernel(const float* __restr
                                                             int64_t rows, double scale,
                                                             float* __restrict__ loss) {
   __shared__ double scratch[33];
+  pdl_wait();  // row_loss is the previous kernel's output
   double acc = 0.0;
   for (int64_t r = threadIdx.x; r < rows; r += blockDim.x) acc += (double)row_loss[r];
   const double sum = block_sum(acc, scratch);
@@ -123,6 +381,73 @@ __global__ void __launch_bounds__(256) scale_by_kernel(T* __restrict__ x, int64_
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
        i += (int64_t)gridDim.x * blockDim.x)
     x[i] = from_f32<T>(to_f32(x[i]) * s);
+}
+
+// Threads and CTAs per row.  CTAs of 256 threads (or fewer, for narrow rows) as
+// long as a cluster of 8 holds the row, else of 512 and 1024; 0 threads: none
+// does.  More CTAs than the row needs while that leaves SMs idle.
+static void distill_geometry(int64_t rows, int64_t vocab, int* threads, int* size) {
+  *threads = 0;
+  for (int n : {64, 128, 256}) {
+    if ((int64_t)n * kDistillEach >= vocab) {
+      *threads = n;
+      *size = 1;
+      break;
+    }
+  }
+  for (int n = 256; *threads == 0 && n <= kDistillMaxThreads; n *= 2)
+    for (int k = 1; *threads == 0 && k <= kDistillCluster; k *= 2)
+      if ((int64_t)n * k * kDistillEach >= vocab) {
+        *threads = n;
+        *size = k;
+      }
+  if (*threads == 0) return;
+  while (*size < kDistillCluster && rows * *size < sm_count() &&
+         vocab >= (int64_t)*size * 2 * *threads * 4)
+    *size *= 2;
+}
+
+template <typename T>
+static oxc_status distill_launch(const void* logits, int64_t stride, void* dlogits,
+                                 const DistillArgs& a, cudaStream_t s) {
+  const T* x = static_cast<const T*>(logits);
+  T* d = static_cast<T*>(dlogits);
+  const size_t smem = teacher_smem(a.top);
+  int threads, size;
+  distill_geometry(a.rows, a.vocab, &threads, &size);
+  void (*kernel)(const T*, int64_t, T*, DistillArgs) = distill_wide_kernel<T>;
+  switch (threads) {
+    case 64: kernel = distill_cluster_kernel<T, 64>; break;
+    case 128: kernel = distill_cluster_kernel<T, 128>; break;
+    case 256: kernel = distill_cluster_kernel<T, 256>; break;
+    case 512: kernel = distill_cluster_kernel<T, 512>; break;
+    case 1024: kernel = distill_cluster_kernel<T, 1024>; break;
+    default: break;
+  }
+  if (smem > 40 * 1024) {  // beyond what a kernel may use unasked
+    const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return cuda_fail(e, "oxc_distill_loss");
+  }
+  if (threads == 0) {
+    kernel<<<(unsigned)std::min<int64_t>(a.rows, (int64_t)sm_count() * 4), 512, smem, s>>>(x, stride, d, a);
+    return check_launch("oxc_distill_loss");
+  }
+  if (a.rows > 0x7fffffff / size)
+    return fail(OXC_ERR_NOT_IMPLEMENTED, "not implemented: distill_loss: %lld rows", (long long)a.rows);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.rows * size));
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)size;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, x, stride, d, a);
+  return e == cudaSuccess ? check_launch("oxc_distill_loss") : cuda_fail(e, "oxc_distill_loss");
 }
 
 }  // namespace oxc
@@ -161,24 +486,18 @@ oxc_status oxc_distill_loss(const void* logits, int64_t logits_stride, const flo
   if (rows > 0) {
     if (!logits || !row_loss || (top > 0 && (!teacher_logits || !teacher_ids)))
       return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: distill_loss: null pointer");
-    const unsigned grid = (unsigned)std::min<int64_t>(rows, (int64_t)sm_count() * 64);
-    const float inv_tau = (float)(1.0 / (double)temperature);
-    const float gs = (float)((double)temperature / (double)total_rows);
-    const size_t smem = (size_t)top * sizeof(float);
-    if (dtype == OXC_BF16)
-      distill_kernel<bf16><<<grid, 512, smem, s>>>(
-          static_cast<const bf16*>(logits), logits_stride, teacher_logits, teacher_ids, (int)top,
-          inv_tau, gs, grad_loss, row_loss, static_cast<bf16*>(dlogits), rows, (int)vocab, err_flag);
-    else
-      distill_kernel<float><<<grid, 512, smem, s>>>(
-          static_cast<const float*>(logits), logits_stride, teacher_logits, teacher_ids, (int)top,
-          inv_tau, gs, grad_loss, row_loss, static_cast<float*>(dlogits), rows, (int)vocab,
-          err_flag);
-    oxc_status st = check_launch("oxc_distill_loss");
+    const double tau = (double)temperature;
+    const DistillArgs a{teacher_logits, teacher_ids, (int)top, (float)(1.0 / tau),
+                        (float)(1.4426950408889634 / tau), (float)(tau / (double)total_rows),
+                        grad_loss, row_loss, rows, (int)vocab, err_flag};
+    const oxc_status st = dtype == OXC_BF16
+                              ? distill_launch<bf16>(logits, logits_stride, dlogits, a, s)
+                              : distill_launch<float>(logits, logits_stride, dlogits, a, s);
     if (st) return st;
   }
   const double scale = (double)temperature * (double)temperature / (double)total_rows;
-  distill_loss_kernel<<<1, 1024, 0, s>>>(row_loss, rows, scale, loss);
+  launch_dependent(distill_loss_kernel, dim3(1), dim3(1024), s, (const float*)row_loss, rows, scale,
+                   loss);
   return check_launch("oxc_distill_loss (sum)");
 }
 
