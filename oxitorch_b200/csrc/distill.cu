@@ -123,10 +123,10 @@ __device__ __forceinline__ TeacherRow teacher_row(const Teacher& s, const float*
 
 // The probability that all entries of s.id[k]'s token have together, 0 if an
 // earlier entry is that token's; in the order of the entries.
-__device__ __forceinline__ float teacher_prob(const Teacher& s, const TeacherRow& r, int k, int top,
+__device__ __forceinline__ float teacher_prob(const Teacher& s, bool repeated, int k, int top,
                                               bool* first) {
   *first = true;
-  if (!r.repeated) return s.prob[k];
+  if (!repeated) return s.prob[k];
   float p = 0.0f;
   for (int j = 0; j < top; ++j) {
     if (s.id[j] != s.id[k]) continue;
@@ -134,25 +134,6 @@ __device__ __forceinline__ float teacher_prob(const Teacher& s, const TeacherRow
     p += s.prob[j];
   }
   return p;
-}
-
-// This thread's share of sum_k p_k (log p_k - log q_k).
-__device__ __forceinline__ float teacher_loss(const Teacher& s, const TeacherRow& r, const float* tl,
-                                              int top, float inv_tau, float log_q0,
-                                              float (*logit)(const void*, int), const void* row,
-                                              float m) {
-  float loss = 0.0f;
-  for (int k = threadIdx.x; k < top; k += blockDim.x) {
-    const float p = s.prob[k];
-    if (s.id[k] >= 0 && p > 0.0f)
-      loss += p * (((tl[k] - r.max) * inv_tau - r.log_sum) -
-                   ((logit(row, s.id[k]) - m) * inv_tau - log_q0));
-  }
-  return loss;
-}
-template <typename T>
-__device__ float logit_at(const void* row, int i) {
-  return to_f32(static_cast<const T*>(row)[i]);
 }
 
 struct DistillArgs {
@@ -168,11 +149,33 @@ struct DistillArgs {
   int32_t* err;
 };
 
+// (max, sum of exponentials relative to it) of two sets; -inf with 0 is the empty
+// one.  A sum that is not 0 beside a maximum of -inf is NaN and stays.
+__device__ __forceinline__ float2 pair_merge(float2 a, float2 b, float c) {
+  const float m = fmaxf(a.x, b.x);
+  const float sa = a.x == m ? a.y : a.y * exp_scaled(a.x - m, c);
+  const float sb = b.x == m ? b.y : b.y * exp_scaled(b.x - m, c);
+  return make_float2(m, sa + sb);
+}
+__device__ __forceinline__ float2 warp_merge(float2 v, float c) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    v = pair_merge(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o),
+                                  __shfl_xor_sync(0xffffffffu, v.y, o)), c);
+  return v;
+}
+
 // One cluster per row.  The row's bytes are cut at 16-byte boundaries of memory:
-// `body` whole vectors, CTA r of the cluster taking [r, r + 1) / size of them,
+// `body` whole vectors, CTA r of the cluster taking the r-th share of them,
 // thread t the vectors t, t + THREADS, ...; the elements before the first
 // boundary and after the last (fewer than a vector each) are single elements of
 // the last CTA's warp 0.
+//
+// A CTA lives for a few microseconds, so what counts beside the bytes in flight
+// is how rarely its warps meet.  Each warp reduces its logits, and its share of
+// the teacher's entries, to a (max, sum) pair of its own; one cluster barrier
+// exchanges all pairs; the gradient is written; one more barrier, within the CTA,
+// precedes the corrections at the teacher's tokens.
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restrict__ dlogits,
@@ -180,13 +183,15 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
   namespace cg = cooperative_groups;
   constexpr int kVec = 16 / (int)sizeof(T);
   constexpr int kVecs = kDistillEach / kVec;
+  constexpr int kWarps = THREADS / 32;
   extern __shared__ float smem[];
-  __shared__ float scratch[33];
-  __shared__ float2 mine;  // this CTA's (max, sum)
+  __shared__ float2 student[kWarps], teacher[kWarps];
+  __shared__ float partial[kWarps];
   const Teacher teach{smem, reinterpret_cast<int*>(smem) + a.top,
                       reinterpret_cast<int*>(smem) + 2 * a.top, teacher_bits(a.top)};
   cg::cluster_group cluster = cg::this_cluster();
   const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x / size;
   const T* xr = logits + row * stride;
   const int head = min(a.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(xr) & 15)) & 15) / (int)sizeof(T));
@@ -202,68 +207,82 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
     if (v < v1) raw[i] = __ldcs(reinterpret_cast<const uint4*>(xr + head) + v);
   }
   float edge = has_edge ? to_f32(xr[edge_at]) : -INFINITY;
+
+  // the teacher's entries k with (k / 32) % kWarps == warp: exponentials relative
+  // to the warp's maximum, 0 and id -1 for absent ones.  An id that is too large
+  // or a NaN logit makes the sum NaN, and with it the row.
   const float* tl = a.tl + row * a.top;
-  const TeacherRow t = teacher_row(teach, tl, a.ti + row * a.top, a.top, a.c, a.vocab,
-                                   rank == 0 ? a.err : nullptr, scratch);
-  T* dr = dlogits ? dlogits + row * (int64_t)a.vocab : nullptr;
-  float e[kDistillEach];
-  float scale = 0.0f, base = 0.0f, row_max = 0.0f, log_sum = 0.0f;
-  if (!t.none && !t.bad) {
-    float m = edge;
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-      const bool in = v0 + i * THREADS + (int)threadIdx.x < v1;
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        float f;
-        if constexpr (sizeof(T) == 4) f = __uint_as_float(w[k]);
-        else f = k & 1 ? bf16_hi(w[k / 2]) : bf16_lo(w[k / 2]);
-        e[i * kVec + k] = in ? f : -INFINITY;
-        m = fmaxf(m, e[i * kVec + k]);
-      }
+  const int64_t* ti = a.ti + row * a.top;
+  for (int i = threadIdx.x; i < (1 << teach.bits); i += THREADS) teach.table[i] = -1;
+  float2 tp = make_float2(-INFINITY, 0.0f);
+  for (int k = threadIdx.x; k < a.top; k += THREADS) {
+    const int64_t id = ti[k];
+    float v = tl[k];
+    if (id < 0) v = -INFINITY;
+    if (id >= a.vocab) {
+      if (rank == 0) record_bad_id(a.err, id, a.vocab);
+      v = NAN;
     }
-    m = block_max(m, scratch);
-    base = m == -INFINITY ? 0.0f : m;
-    float s = has_edge ? exp_scaled(edge - base, a.c) : 0.0f;
-    edge = s;
-#pragma unroll
-    for (int i = 0; i < kDistillEach; ++i) {
-      e[i] = exp_scaled(e[i] - base, a.c);
-      s += e[i];
-    }
-    s = block_sum(s, scratch);
-    // the row's maximum and sum from the CTAs' (a row of -inf alone has sum NaN)
-    row_max = m;
-    float total = s;
-    if (size > 1) {
-      if (threadIdx.x == 0) mine = make_float2(m, s);
-      cluster.sync();
-      float2 part[kDistillCluster];
-#pragma unroll
-      for (int r = 0; r < kDistillCluster; ++r)
-        part[r] = r < size ? *cluster.map_shared_rank(&mine, r) : make_float2(-INFINITY, 0.0f);
-#pragma unroll
-      for (int r = 0; r < kDistillCluster; ++r) row_max = fmaxf(row_max, part[r].x);
-      total = 0.0f;
-#pragma unroll
-      for (int r = 0; r < kDistillCluster; ++r)
-        if (part[r].x != -INFINITY || part[r].y != 0.0f)
-          total += part[r].x == -INFINITY ? part[r].y
-                                          : part[r].y * exp_scaled(part[r].x - row_max, a.c);
-    }
-    if (row_max == -INFINITY) total = NAN;
-    const float gs = a.grad_loss ? a.grad_scale * __ldg(a.grad_loss) : a.grad_scale;
-    const float share = m == -INFINITY ? 1.0f : exp_scaled(m - row_max, a.c);
-    scale = gs * (share * __fdiv_rn(1.0f, total));
-    log_sum = logf(total);
-  } else {
-    const float f = t.none ? 0.0f : NAN;
-#pragma unroll
-    for (int i = 0; i < kDistillEach; ++i) e[i] = f;
-    edge = f;
-    scale = 1.0f;
+    teach.id[k] = id < a.vocab && v != -INFINITY ? (int)id : -1;
+    teach.prob[k] = v;
+    tp.x = fmaxf(tp.x, v);
+    if (v != v) tp.y = NAN;
   }
+  tp.x = warp_max(tp.x);
+  for (int k = threadIdx.x; k < a.top; k += THREADS) {
+    const float e = teach.id[k] < 0 ? 0.0f : exp_scaled(teach.prob[k] - tp.x, a.c);
+    teach.prob[k] = e;
+    tp.y += e;
+  }
+  tp.y = warp_sum(tp.y);
+
+  float e[kDistillEach];
+  float2 sp = make_float2(edge, 0.0f);
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    const bool in = v0 + i * THREADS + (int)threadIdx.x < v1;
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      float f;
+      if constexpr (sizeof(T) == 4) f = __uint_as_float(w[k]);
+      else f = k & 1 ? bf16_hi(w[k / 2]) : bf16_lo(w[k / 2]);
+      e[i * kVec + k] = in ? f : -INFINITY;
+      sp.x = fmaxf(sp.x, e[i * kVec + k]);
+    }
+  }
+  sp.x = warp_max(sp.x);
+  const float base = sp.x == -INFINITY ? 0.0f : sp.x;
+  edge = has_edge ? exp_scaled(edge - base, a.c) : 0.0f;
+  sp.y = edge;
+#pragma unroll
+  for (int i = 0; i < kDistillEach; ++i) {
+    e[i] = exp_scaled(e[i] - base, a.c);
+    sp.y += e[i];
+  }
+  sp.y = warp_sum(sp.y);
+  if (lane == 0) {
+    student[warp] = sp;
+    teacher[warp] = tp;
+  }
+  if (size > 1) cluster.sync();
+  else __syncthreads();
+  const float own_max = sp.x;
+  sp = make_float2(-INFINITY, 0.0f);
+  for (int i = lane; i < size * kWarps; i += 32) {
+    const float2* s = size > 1 ? cluster.map_shared_rank(student, i / kWarps) : student;
+    sp = pair_merge(sp, s[i % kWarps], a.c);
+  }
+  if (size > 1) cluster.barrier_arrive();  // the others' pairs are read
+  sp = warp_merge(sp, a.c);
+  tp = warp_merge(lane < kWarps ? teacher[lane] : make_float2(-INFINITY, 0.0f), a.c);
+  const bool none = tp.x == -INFINITY && tp.y == 0.0f, bad = tp.y != tp.y;
+  const float gs = a.grad_loss ? a.grad_scale * __ldg(a.grad_loss) : a.grad_scale;
+  // a row of -inf alone has no softmax: its sum counts as NaN
+  const float unit = gs * __fdiv_rn(1.0f, sp.x == -INFINITY ? NAN : sp.y);
+  float scale = own_max == -INFINITY ? unit : unit * exp_scaled(own_max - sp.x, a.c);
+  if (bad) scale = NAN;
+  T* dr = dlogits ? dlogits + row * (int64_t)a.vocab : nullptr;
   if (dr) {
     const bool vector = ((reinterpret_cast<uintptr_t>(dr + head) & 15) == 0);
 #pragma unroll
@@ -272,7 +291,7 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
       if (v < v1) {
         float g[kVec];
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) g[k] = e[i * kVec + k] * scale;
+        for (int k = 0; k < kVec; ++k) g[k] = none ? 0.0f : e[i * kVec + k] * scale;
         T* out = dr + head + (int64_t)v * kVec;
         if (vector) {
           store_from_f32<kVec>(out, g);
@@ -282,33 +301,53 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
         }
       }
     }
-    if (has_edge) dr[edge_at] = from_f32<T>(edge * scale);
+    if (has_edge) dr[edge_at] = from_f32<T>(none ? 0.0f : edge * scale);
   }
-  if (!t.none && !t.bad) {
-    // the teacher's tokens in this CTA's part: q - p instead of q, over what was
-    // just written
-    const float gs = a.grad_loss ? a.grad_scale * __ldg(a.grad_loss) : a.grad_scale;
-    if (dr) {
-      __syncthreads();
-      for (int k = threadIdx.x; k < a.top; k += THREADS) {
-        const int id = teach.id[k];
-        if (id < 0) continue;
-        const int v = id < head ? -1 : (id - head) / kVec;
-        if (v < 0 || v >= body ? rank != size - 1 : v < v0 || v >= v1) continue;
-        bool first;
-        const float p = teacher_prob(teach, t, k, a.top, &first);
-        if (first) dr[id] = from_f32<T>(exp_scaled(to_f32(xr[id]) - base, a.c) * scale - gs * p);
-      }
+  // this thread's entries: their part of the loss (rank 0), and whether an id is
+  // there twice (finding it in the table already means it is)
+  const float t_unit = __fdiv_rn(1.0f, tp.y), t_log = logf(tp.y), s_log = logf(sp.y);
+  const float t_share = teacher[warp].x == -INFINITY ? 0.0f : t_unit * exp_scaled(teacher[warp].x - tp.x, a.c);
+  float loss = 0.0f;
+  int twice = 0;
+  for (int k = threadIdx.x; k < a.top; k += THREADS) {
+    const int id = teach.id[k];
+    const float p = teach.prob[k] * t_share;
+    teach.prob[k] = p;
+    if (id < 0) continue;
+    if (rank == 0 && p > 0.0f)
+      loss += p * (((tl[k] - tp.x) * a.inv_tau - t_log) -
+                   ((to_f32(xr[id]) - sp.x) * a.inv_tau - s_log));
+    unsigned int h = ((unsigned int)id * 2654435769u) >> (32 - teach.bits);
+    for (int n = 0; n < (1 << teach.bits); ++n) {
+      const int was = atomicCAS(&teach.table[h], -1, id);
+      if (was == -1) break;
+      if (was == id) { twice = 1; break; }
+      h = (h + 1) & ((1u << teach.bits) - 1);
     }
-    if (rank == 0) {
-      const float loss = block_sum(
-          teacher_loss(teach, t, tl, a.top, a.inv_tau, log_sum, logit_at<T>, xr, row_max), scratch);
-      if (threadIdx.x == 0) a.row_loss[row] = loss;
-    }
-  } else if (rank == 0 && threadIdx.x == 0) {
-    a.row_loss[row] = t.none ? 0.0f : NAN;
   }
-  if (size > 1) cluster.sync();  // `mine` may still be read by the others
+  if (rank == 0) {
+    loss = warp_sum(loss);
+    if (lane == 0) partial[warp] = loss;
+  }
+  const bool repeated = __syncthreads_or(twice);
+  if (rank == 0 && threadIdx.x == 0) {
+    float sum = 0.0f;
+    for (int w = 0; w < kWarps; ++w) sum += partial[w];
+    a.row_loss[row] = none ? 0.0f : bad || sp.x == -INFINITY ? NAN : sum;
+  }
+  // the teacher's tokens in this CTA's part: q - p over the q just written
+  if (dr && !none && !bad) {
+    for (int k = threadIdx.x; k < a.top; k += THREADS) {
+      const int id = teach.id[k];
+      if (id < 0) continue;
+      const int v = id < head ? -1 : (id - head) / kVec;
+      if (v < 0 || v >= body ? rank != size - 1 : v < v0 || v >= v1) continue;
+      bool first;
+      const float p = teacher_prob(teach, repeated, k, a.top, &first);
+      if (first) dr[id] = from_f32<T>(exp_scaled(to_f32(xr[id]) - sp.x, a.c) * unit - gs * p);
+    }
+  }
+  if (size > 1) cluster.barrier_wait();  // no CTA leaves while its pairs are read
 }
 
 // One CTA per row at a time, three passes over it: any width.
@@ -349,12 +388,19 @@ __global__ void __launch_bounds__(512) distill_wide_kernel(const T* __restrict__
         const int id = teach.id[k];
         if (id < 0) continue;
         bool first;
-        const float p = teacher_prob(teach, t, k, a.top, &first);
+        const float p = teacher_prob(teach, t.repeated, k, a.top, &first);
         if (first) dr[id] = from_f32<T>(exp_scaled(to_f32(xr[id]) - m, a.c) * scale - gs * p);
       }
     }
-    const float loss = block_sum(
-        teacher_loss(teach, t, tl, a.top, a.inv_tau, logf(sum), logit_at<T>, xr, m), scratch);
+    const float s_log = logf(sum);
+    float loss = 0.0f;
+    for (int k = threadIdx.x; k < a.top; k += blockDim.x) {
+      const float p = teach.prob[k];
+      if (teach.id[k] >= 0 && p > 0.0f)
+        loss += p * (((tl[k] - t.max) * a.inv_tau - t.log_sum) -
+                     ((to_f32(xr[teach.id[k]]) - m) * a.inv_tau - s_log));
+    }
+    loss = block_sum(loss, scratch);
     if (threadIdx.x == 0) a.row_loss[row] = loss;
     __syncthreads();  // the teacher's side is read; the next row overwrites it
   }
