@@ -685,7 +685,9 @@ oxc_status oxc_gated_step(const void* x, int64_t x_stride, const void* gate, int
  * [rows, top].  An entry with a negative id or a -inf logit is absent; a row
  * without entries gives loss 0 and gradient 0.  An id >= vocab is recorded in
  * err_flag (int32[4], may be NULL) and, like a NaN teacher logit, makes the
- * row's loss and gradient NaN.  row_loss: [rows] scratch (the per-row sums). */
+ * row's loss and gradient NaN.  row_loss: OXC_DISTILL_PARTS * rows floats of
+ * scratch (the parts of each row's loss). */
+#define OXC_DISTILL_PARTS 8
 oxc_status oxc_distill_loss(const void* logits, int64_t logits_stride, const float* teacher_logits,
                             const int64_t* teacher_ids, int64_t top, float temperature,
                             const float* grad_loss, float* loss, float* row_loss, void* dlogits,

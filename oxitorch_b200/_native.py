@@ -32,6 +32,7 @@ ACT_NONE = 0
 ACT_GELU_TANH = 1
 F32 = 0
 BF16 = 1
+DISTILL_PARTS = 8
 
 MAX_DIMS = 8
 

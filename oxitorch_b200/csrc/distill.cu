@@ -11,24 +11,26 @@
 // twice counts twice.
 //
 // Bound by HBM: 2 sizeof(T) bytes a logit, the row read once and its gradient
-// written once.  So a row stays in registers between the two: a cluster of 1 to 8
-// CTAs shares it, 32 logits a thread, as exponentials relative to the CTA's own
-// maximum; (max, sum) pairs are exchanged through distributed shared memory, and
-// one multiplication an element remains.  Rows wider than that (262144) take the
-// three-pass kernel, which re-reads them from L2 or HBM.
+// written once.  So a row stays in shared memory between the two, shared by a
+// cluster of 1 to 8 CTAs that exchange (max, sum) pairs through distributed shared
+// memory.  Rows wider than a cluster holds (1.25 MB) take the three-pass kernel,
+// which re-reads them from L2 or HBM.
 #include <cooperative_groups.h>
 #include <math.h>
 
 #include <algorithm>
 
+#include "pipeline.cuh"
 #include "typed.cuh"
 
 namespace oxc {
 
 constexpr int kDistillMaxTop = 4096;
-constexpr int kDistillEach = 32;      // logits per thread
-constexpr int kDistillCluster = 8;    // CTAs per row at most
-constexpr int kDistillMaxThreads = 1024;
+constexpr int kDistillThreads = 256;
+constexpr int kDistillCopies = 4;             // bulk copies per part of a row
+constexpr int kDistillPart = 64 * 1024;       // bytes of a row per CTA, if a cluster can
+constexpr int kDistillMaxPart = 160 * 1024;   // and at most
+constexpr int kDistillCluster = OXC_DISTILL_PARTS;  // CTAs per row at most
 
 // Records the first bad id: flag[0] = 2 (dim 1), flag[1..2] = id, flag[3] = vocab.
 __device__ __forceinline__ void record_bad_id(int32_t* flag, int64_t id, int64_t vocab) {
@@ -39,16 +41,17 @@ __device__ __forceinline__ void record_bad_id(int32_t* flag, int64_t id, int64_t
   }
 }
 
-// exp(d / tau) for d = x - max <= 0, c = log2(e) / tau.  The subtraction comes
-// first, so the large terms see only ex2's own error; results below 2^-126 are 0.
-__device__ __forceinline__ float exp_scaled(float d, float c) {
+__device__ __forceinline__ float ex2_approx(float t) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * c));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
 }
+// exp(d / tau) for d = x - max <= 0, c = log2(e) / tau.  The subtraction comes
+// first, so the large terms see only ex2's own error; results below 2^-126 are 0.
+__device__ __forceinline__ float exp_scaled(float d, float c) { return ex2_approx(d * c); }
 
-// The teacher's side of a row, in shared memory: prob[k] (0 for absent entries)
-// and id[k] (-1).
+// The teacher's side of a row, in shared memory: its logits, then probabilities,
+// and ids (negative for entries that do not count).
 struct Teacher {
   float* prob;
   int* id;
@@ -62,7 +65,7 @@ __host__ __device__ inline int teacher_bits(int top) {
   return b;
 }
 __host__ __device__ inline size_t teacher_smem(int top) {
-  return (size_t)top * 8 + (sizeof(int) << teacher_bits(top));
+  return (size_t)top * 12 + (sizeof(int) << teacher_bits(top));
 }
 
 struct TeacherRow {
@@ -165,189 +168,275 @@ __device__ __forceinline__ float2 warp_merge(float2 v, float c) {
   return v;
 }
 
-// One cluster per row.  The row's bytes are cut at 16-byte boundaries of memory:
-// `body` whole vectors, CTA r of the cluster taking the r-th share of them,
-// thread t the vectors t, t + THREADS, ...; the elements before the first
-// boundary and after the last (fewer than a vector each) are single elements of
-// the last CTA's warp 0.
-//
-// A CTA lives for a few microseconds, so what counts beside the bytes in flight
-// is how rarely its warps meet.  Each warp reduces its logits, and its share of
-// the teacher's entries, to a (max, sum) pair of its own; one cluster barrier
-// exchanges all pairs; the gradient is written; one more barrier, within the CTA,
-// precedes the corrections at the teacher's tokens.
-template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+// A row's bytes are cut at 16-byte boundaries of memory: `body` whole vectors,
+// CTA r of the cluster taking the r-th share of them, thread t the vectors t,
+// t + THREADS, ... of it; the elements before the first boundary and after the
+// last (fewer than a vector each) are single elements of the last CTA's warp 0.
+template <typename T>
+struct RowCut {
+  static constexpr int kVec = 16 / (int)sizeof(T);
+  const T* row;
+  int head, body, v0, v1;
+  __device__ __forceinline__ RowCut(const T* row, int vocab, int rank, int size) : row(row) {
+    head = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T));
+    body = (vocab - head) / kVec;
+    const int each = (body + size - 1) / size;
+    v0 = min(body, rank * each);
+    v1 = min(body, v0 + each);
+  }
+  __device__ __forceinline__ const T* part() const { return row + head + (int64_t)v0 * kVec; }
+};
+
+// Folds N logits (N even) into a running (max, sum of exponentials): the maximum
+// of the N first, a rescale of the sum when it grows, then N terms.
+template <int N>
+__device__ __forceinline__ void pair_fold(float2& p, const float2 (&v)[N / 2], float c) {
+  float m = p.x;
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) m = fmaxf(m, fmaxf(v[i].x, v[i].y));
+  if (m > p.x) {
+    p.y *= exp_scaled(p.x - m, c);
+    p.x = m;
+  }
+  const float base = m == -INFINITY ? 0.0f : -m;
+  float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    const float2 d = __fmul2_rn(__fadd2_rn(v[i], make_float2(base, base)), make_float2(c, c));
+    s = __fadd2_rn(s, make_float2(ex2_approx(d.x), ex2_approx(d.y)));
+  }
+  p.y += s.x + s.y;
+}
+
+// The elements of a 16-byte vector, in pairs.
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& q, float2 (&v)[8 / (int)sizeof(T)]) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 8 / (int)sizeof(T); ++i) {
+    if constexpr (sizeof(T) == 4)
+      v[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else
+      v[i] = make_float2(bf16_lo(w[i]), bf16_hi(w[i]));
+  }
+}
+
+// Persistent clusters, a row at a time.  A CTA's part of the row arrives in
+// shared memory by bulk copies; one pass over it makes the (max, sum) pair, a
+// second the gradient, and then the copies of the next row's part are started,
+// whose bytes L2 was asked for when the second pass began.  The teacher's side of
+// a row is worked out while its logits are on the way.  The warps of a row meet
+// twice: each reduces its logits, and its share of the teacher's entries, to a
+// (max, sum) pair of its own, and one cluster barrier exchanges all of them; a
+// barrier within the CTA precedes the corrections at the teacher's tokens.  Each
+// CTA sums the loss over the tokens in its part: row_loss[row][rank].
+template <typename T>
+__global__ void __launch_bounds__(kDistillThreads)
 distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restrict__ dlogits,
-                       DistillArgs a) {
+                       DistillArgs a, int part_bytes) {
   namespace cg = cooperative_groups;
-  constexpr int kVec = 16 / (int)sizeof(T);
-  constexpr int kVecs = kDistillEach / kVec;
+  using Cut = RowCut<T>;
+  constexpr int THREADS = kDistillThreads;
+  constexpr int kVec = Cut::kVec, kPairs = kVec / 2;
   constexpr int kWarps = THREADS / 32;
-  extern __shared__ float smem[];
-  __shared__ float2 student[kWarps], teacher[kWarps];
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float2 student[2][kWarps], teacher[kWarps];
   __shared__ float partial[kWarps];
-  const Teacher teach{smem, reinterpret_cast<int*>(smem) + a.top,
-                      reinterpret_cast<int*>(smem) + 2 * a.top, teacher_bits(a.top)};
+  __shared__ uint64_t full[kDistillCopies];
   cg::cluster_group cluster = cg::this_cluster();
   const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = blockIdx.x / size;
-  const T* xr = logits + row * stride;
-  const int head = min(a.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(xr) & 15)) & 15) / (int)sizeof(T));
-  const int body = (a.vocab - head) / kVec, each = (body + size - 1) / size;
-  const int v0 = min(body, rank * each), v1 = min(body, v0 + each);
-  const int edges = a.vocab - body * kVec;  // head + tail
-  const bool has_edge = rank == size - 1 && (int)threadIdx.x < edges;
-  const int edge_at = (int)threadIdx.x < head ? threadIdx.x : body * kVec + threadIdx.x;
-  uint4 raw[kVecs];
-#pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int v = v0 + i * THREADS + threadIdx.x;
-    if (v < v1) raw[i] = __ldcs(reinterpret_cast<const uint4*>(xr + head) + v);
-  }
-  float edge = has_edge ? to_f32(xr[edge_at]) : -INFINITY;
-
-  // the teacher's entries k with (k / 32) % kWarps == warp: exponentials relative
-  // to the warp's maximum, 0 and id -1 for absent ones.  An id that is too large
-  // or a NaN logit makes the sum NaN, and with it the row.
-  const float* tl = a.tl + row * a.top;
-  const int64_t* ti = a.ti + row * a.top;
-  for (int i = threadIdx.x; i < (1 << teach.bits); i += THREADS) teach.table[i] = -1;
-  float2 tp = make_float2(-INFINITY, 0.0f);
-  for (int k = threadIdx.x; k < a.top; k += THREADS) {
-    const int64_t id = ti[k];
-    float v = tl[k];
-    if (id < 0) v = -INFINITY;
-    if (id >= a.vocab) {
-      if (rank == 0) record_bad_id(a.err, id, a.vocab);
-      v = NAN;
-    }
-    teach.id[k] = id < a.vocab && v != -INFINITY ? (int)id : -1;
-    teach.prob[k] = v;
-    tp.x = fmaxf(tp.x, v);
-    if (v != v) tp.y = NAN;
-  }
-  tp.x = warp_max(tp.x);
-  for (int k = threadIdx.x; k < a.top; k += THREADS) {
-    const float e = teach.id[k] < 0 ? 0.0f : exp_scaled(teach.prob[k] - tp.x, a.c);
-    teach.prob[k] = e;
-    tp.y += e;
-  }
-  tp.y = warp_sum(tp.y);
-
-  float e[kDistillEach];
-  float2 sp = make_float2(edge, 0.0f);
-#pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-    const bool in = v0 + i * THREADS + (int)threadIdx.x < v1;
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) {
-      float f;
-      if constexpr (sizeof(T) == 4) f = __uint_as_float(w[k]);
-      else f = k & 1 ? bf16_hi(w[k / 2]) : bf16_lo(w[k / 2]);
-      e[i * kVec + k] = in ? f : -INFINITY;
-      sp.x = fmaxf(sp.x, e[i * kVec + k]);
-    }
-  }
-  sp.x = warp_max(sp.x);
-  const float base = sp.x == -INFINITY ? 0.0f : sp.x;
-  edge = has_edge ? exp_scaled(edge - base, a.c) : 0.0f;
-  sp.y = edge;
-#pragma unroll
-  for (int i = 0; i < kDistillEach; ++i) {
-    e[i] = exp_scaled(e[i] - base, a.c);
-    sp.y += e[i];
-  }
-  sp.y = warp_sum(sp.y);
-  if (lane == 0) {
-    student[warp] = sp;
-    teacher[warp] = tp;
-  }
-  if (size > 1) cluster.sync();
-  else __syncthreads();
-  const float own_max = sp.x;
-  sp = make_float2(-INFINITY, 0.0f);
-  for (int i = lane; i < size * kWarps; i += 32) {
-    const float2* s = size > 1 ? cluster.map_shared_rank(student, i / kWarps) : student;
-    sp = pair_merge(sp, s[i % kWarps], a.c);
-  }
-  if (size > 1) cluster.barrier_arrive();  // the others' pairs are read
-  sp = warp_merge(sp, a.c);
-  tp = warp_merge(lane < kWarps ? teacher[lane] : make_float2(-INFINITY, 0.0f), a.c);
-  const bool none = tp.x == -INFINITY && tp.y == 0.0f, bad = tp.y != tp.y;
+  const uint4* buffer = reinterpret_cast<const uint4*>(smem);
+  float* rest = reinterpret_cast<float*>(smem + part_bytes);
+  const Teacher teach{rest, reinterpret_cast<int*>(rest) + a.top,
+                      reinterpret_cast<int*>(rest) + 2 * a.top, teacher_bits(a.top)};
+  float* logit_k = rest + 2 * a.top + (1 << teach.bits);  // the student's logit at id[k]
   const float gs = a.grad_loss ? a.grad_scale * __ldg(a.grad_loss) : a.grad_scale;
-  // a row of -inf alone has no softmax: its sum counts as NaN
-  const float unit = gs * __fdiv_rn(1.0f, sp.x == -INFINITY ? NAN : sp.y);
-  float scale = own_max == -INFINITY ? unit : unit * exp_scaled(own_max - sp.x, a.c);
-  if (bad) scale = NAN;
-  T* dr = dlogits ? dlogits + row * (int64_t)a.vocab : nullptr;
-  if (dr) {
-    const bool vector = ((reinterpret_cast<uintptr_t>(dr + head) & 15) == 0);
+  const int64_t rows_apart = gridDim.x / size;
+
+  // vectors [copy_start(i), copy_start(i + 1)) of a part of n are copy i's: whole
+  // rounds of the threads
+  auto copy_start = [](int n, int i) {
+    const int rounds = (n + THREADS - 1) / THREADS;
+    return min(n, (rounds * i + kDistillCopies - 1) / kDistillCopies * THREADS);
+  };
+  auto fetch = [&](int64_t row) {  // thread 0
+    const Cut cut(logits + row * stride, a.vocab, rank, size);
+    const int n = cut.v1 - cut.v0;
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int v = v0 + i * THREADS + threadIdx.x;
-      if (v < v1) {
-        float g[kVec];
-#pragma unroll
-        for (int k = 0; k < kVec; ++k) g[k] = none ? 0.0f : e[i * kVec + k] * scale;
-        T* out = dr + head + (int64_t)v * kVec;
-        if (vector) {
-          store_from_f32<kVec>(out, g);
-        } else {  // the gradient's rows lie otherwise within their 16 bytes
-#pragma unroll
-          for (int k = 0; k < kVec; ++k) out[k] = from_f32<T>(g[k]);
-        }
+    for (int i = 0; i < kDistillCopies; ++i) {
+      const int from = copy_start(n, i), bytes = 16 * (copy_start(n, i + 1) - from);
+      if (bytes > 0) {
+        mbar_arrive_expect_tx(&full[i], (uint32_t)bytes);
+        bulk_g2s(smem + 16 * from, cut.part() + (int64_t)from * kVec, (uint32_t)bytes, &full[i]);
+      } else {
+        mbar_arrive(&full[i]);
       }
     }
-    if (has_edge) dr[edge_at] = from_f32<T>(none ? 0.0f : edge * scale);
+  };
+  int64_t row = blockIdx.x / size;
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 0; i < kDistillCopies; ++i) mbar_init(&full[i], 1);
+    fence_barrier_init();
+    if (row < a.rows) fetch(row);
   }
-  // this thread's entries: their part of the loss (rank 0), and whether an id is
-  // there twice (finding it in the table already means it is)
-  const float t_unit = __fdiv_rn(1.0f, tp.y), t_log = logf(tp.y), s_log = logf(sp.y);
-  const float t_share = teacher[warp].x == -INFINITY ? 0.0f : t_unit * exp_scaled(teacher[warp].x - tp.x, a.c);
-  float loss = 0.0f;
-  int twice = 0;
-  for (int k = threadIdx.x; k < a.top; k += THREADS) {
-    const int id = teach.id[k];
-    const float p = teach.prob[k] * t_share;
-    teach.prob[k] = p;
-    if (id < 0) continue;
-    if (rank == 0 && p > 0.0f)
-      loss += p * (((tl[k] - tp.x) * a.inv_tau - t_log) -
-                   ((to_f32(xr[id]) - sp.x) * a.inv_tau - s_log));
-    unsigned int h = ((unsigned int)id * 2654435769u) >> (32 - teach.bits);
-    for (int n = 0; n < (1 << teach.bits); ++n) {
-      const int was = atomicCAS(&teach.table[h], -1, id);
-      if (was == -1) break;
-      if (was == id) { twice = 1; break; }
-      h = (h + 1) & ((1u << teach.bits) - 1);
+  __syncthreads();
+  for (uint32_t n = 0; row < a.rows; row += rows_apart, ++n) {
+    const Cut cut(logits + row * stride, a.vocab, rank, size);
+    const int vecs = cut.v1 - cut.v0;
+    const int edges = a.vocab - cut.body * kVec;  // before the body and after it
+    const bool has_edge = rank == size - 1 && (int)threadIdx.x < edges;
+    const int edge_at = (int)threadIdx.x < cut.head ? threadIdx.x : cut.body * kVec + threadIdx.x;
+    const float edge = has_edge ? to_f32(cut.row[edge_at]) : -INFINITY;
+
+    // the teacher's entries k with (k / 32) % kWarps == warp: absent ones get id
+    // -1.  An id that is too large or a NaN logit makes the sum NaN, and with it
+    // the row.
+    for (int i = threadIdx.x; i < (1 << teach.bits); i += THREADS) teach.table[i] = -1;
+    float2 tp = make_float2(-INFINITY, 0.0f);
+    for (int k = threadIdx.x; k < a.top; k += THREADS) {
+      const int64_t id = __ldcs(a.ti + row * a.top + k);
+      float v = __ldcs(a.tl + row * a.top + k);
+      if (id < 0) v = -INFINITY;
+      if (id >= a.vocab) {
+        if (rank == 0) record_bad_id(a.err, id, a.vocab);
+        v = NAN;
+      }
+      teach.id[k] = id < a.vocab && v != -INFINITY ? (int)id : -1;
+      teach.prob[k] = v;
+      tp.x = fmaxf(tp.x, v);
+      if (v != v) tp.y = NAN;
     }
-  }
-  if (rank == 0) {
-    loss = warp_sum(loss);
-    if (lane == 0) partial[warp] = loss;
-  }
-  const bool repeated = __syncthreads_or(twice);
-  if (rank == 0 && threadIdx.x == 0) {
-    float sum = 0.0f;
-    for (int w = 0; w < kWarps; ++w) sum += partial[w];
-    a.row_loss[row] = none ? 0.0f : bad || sp.x == -INFINITY ? NAN : sum;
-  }
-  // the teacher's tokens in this CTA's part: q - p over the q just written
-  if (dr && !none && !bad) {
+    tp.x = warp_max(tp.x);
+    for (int k = threadIdx.x; k < a.top; k += THREADS)
+      if (teach.id[k] >= 0) tp.y += exp_scaled(teach.prob[k] - tp.x, a.c);
+    tp.y = warp_sum(tp.y);
+
+    float2 sp = make_float2(edge, edge == -INFINITY ? 0.0f : edge - edge + 1.0f);
+#pragma unroll
+    for (int i = 0; i < kDistillCopies; ++i) {
+      if (!mbar_wait(&full[i], n & 1u)) atomicOr(&g_kernel_error, OXC_KERR_PIPELINE_TIMEOUT);
+      int v = copy_start(vecs, i) + threadIdx.x;
+      const int end = copy_start(vecs, i + 1);
+      constexpr int U = 16 / kVec;  // vectors at a time
+      for (; v + (U - 1) * THREADS < end; v += U * THREADS) {
+        float2 f[8];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          unpack<T>(buffer[v + u * THREADS], reinterpret_cast<float2(&)[kPairs]>(f[u * kPairs]));
+        pair_fold<16>(sp, f, a.c);
+      }
+      for (; v < end; v += THREADS) {
+        float2 f[kPairs];
+        unpack<T>(buffer[v], f);
+        pair_fold<kVec>(sp, f, a.c);
+      }
+    }
+    // the student's logits at this thread's entries; ids of other CTAs' parts turn
+    // negative
     for (int k = threadIdx.x; k < a.top; k += THREADS) {
       const int id = teach.id[k];
       if (id < 0) continue;
-      const int v = id < head ? -1 : (id - head) / kVec;
-      if (v < 0 || v >= body ? rank != size - 1 : v < v0 || v >= v1) continue;
-      bool first;
-      const float p = teacher_prob(teach, repeated, k, a.top, &first);
-      if (first) dr[id] = from_f32<T>(exp_scaled(to_f32(xr[id]) - sp.x, a.c) * unit - gs * p);
+      const int v = id < cut.head ? -1 : (id - cut.head) / kVec;
+      const bool in_body = v >= 0 && v < cut.body;
+      if (in_body ? v < cut.v0 || v >= cut.v1 : rank != size - 1) teach.id[k] = -2 - id;
+      else logit_k[k] = to_f32(in_body ? reinterpret_cast<const T*>(smem)[id - cut.head - cut.v0 * kVec] : cut.row[id]);
     }
+    sp = warp_merge(sp, a.c);
+    if (lane == 0) {
+      student[n & 1u][warp] = sp;
+      teacher[warp] = tp;
+    }
+    if (size > 1) cluster.sync();
+    else __syncthreads();
+    const int64_t next = row + rows_apart;
+    if (threadIdx.x == 0 && next < a.rows) {
+      const Cut ahead(logits + next * stride, a.vocab, rank, size);
+      if (ahead.v1 > ahead.v0)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(ahead.part()),
+                     "r"((ahead.v1 - ahead.v0) * 16) : "memory");
+    }
+    sp = make_float2(-INFINITY, 0.0f);
+    for (int i = lane; i < size * kWarps; i += 32) {
+      const float2* s = size > 1 ? cluster.map_shared_rank(student[n & 1u], i / kWarps) : student[n & 1u];
+      sp = pair_merge(sp, s[i % kWarps], a.c);
+    }
+    sp = warp_merge(sp, a.c);
+    tp = warp_merge(lane < kWarps ? teacher[lane] : make_float2(-INFINITY, 0.0f), a.c);
+    const bool none = tp.x == -INFINITY && tp.y == 0.0f, bad = tp.y != tp.y;
+    // a row of -inf alone has no softmax: its sum counts as NaN
+    if (sp.x == -INFINITY) sp.y = NAN;
+    const float unit = bad ? NAN : gs * __fdiv_rn(1.0f, sp.y);
+    T* dr = dlogits ? dlogits + row * (int64_t)a.vocab : nullptr;
+    if (dr) {
+      T* out = dr + cut.head + (int64_t)cut.v0 * kVec;
+      const bool vector = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+      const float2 shift = make_float2(-sp.x, -sp.x), c2 = make_float2(a.c, a.c),
+                   unit2 = make_float2(unit, unit);
+#pragma unroll 4
+      for (int v = threadIdx.x; v < vecs; v += THREADS) {
+        float2 f[kPairs];
+        unpack<T>(buffer[v], f);
+        float g[kVec];
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+          const float2 d = __fmul2_rn(__fadd2_rn(f[k], shift), c2);
+          const float2 o = __fmul2_rn(make_float2(ex2_approx(d.x), ex2_approx(d.y)), unit2);
+          g[2 * k] = none ? 0.0f : o.x;
+          g[2 * k + 1] = none ? 0.0f : o.y;
+        }
+        if (vector) {
+          store_from_f32<kVec>(out + (int64_t)v * kVec, g);
+        } else {  // the gradient's rows lie otherwise within their 16 bytes
+#pragma unroll
+          for (int k = 0; k < kVec; ++k) out[(int64_t)v * kVec + k] = from_f32<T>(g[k]);
+        }
+      }
+      if (has_edge) dr[edge_at] = from_f32<T>(none ? 0.0f : exp_scaled(edge - sp.x, a.c) * unit);
+    }
+    // this thread's entries: the loss at those in this part, and whether an id is
+    // there twice (finding it in the table already means it is)
+    const float t_log = logf(tp.y), s_log = logf(sp.y), t_unit = __fdiv_rn(1.0f, tp.y);
+    float loss = 0.0f;
+    int twice = 0;
+    for (int k = threadIdx.x; k < a.top; k += THREADS) {
+      const int id = teach.id[k];
+      if (id < 0) continue;
+      const float z = (teach.prob[k] - tp.x), p = exp_scaled(z, a.c) * t_unit;
+      teach.prob[k] = p;
+      if (p > 0.0f)
+        loss += p * ((z * a.inv_tau - t_log) - ((logit_k[k] - sp.x) * a.inv_tau - s_log));
+      unsigned int h = ((unsigned int)id * 2654435769u) >> (32 - teach.bits);
+      for (int i = 0; i < (1 << teach.bits); ++i) {
+        const int was = atomicCAS(&teach.table[h], -1, id);
+        if (was == -1) break;
+        if (was == id) { twice = 1; break; }
+        h = (h + 1) & ((1u << teach.bits) - 1);
+      }
+    }
+    loss = warp_sum(loss);
+    if (lane == 0) partial[warp] = loss;
+    const bool repeated = __syncthreads_or(twice);
+    if (threadIdx.x == 0) {
+      if (next < a.rows) fetch(next);  // the part has been read twice
+      float sum = 0.0f;
+      for (int w = 0; w < kWarps; ++w) sum += partial[w];
+      a.row_loss[row * size + rank] = none ? 0.0f : bad || sp.y != sp.y ? NAN : sum;
+    }
+    // q - p over the q just written
+    if (dr && !none && !bad) {
+      for (int k = threadIdx.x; k < a.top; k += THREADS) {
+        const int id = teach.id[k];
+        if (id < 0) continue;
+        bool first;
+        const float p = teacher_prob(teach, repeated, k, a.top, &first);
+        if (first) dr[id] = from_f32<T>(exp_scaled(logit_k[k] - sp.x, a.c) * unit - gs * p);
+      }
+    }
+    if (repeated) __syncthreads();  // the other threads' entries are read
   }
-  if (size > 1) cluster.barrier_wait();  // no CTA leaves while its pairs are read
+  if (size > 1) cluster.sync();  // no CTA leaves while its pairs are read
 }
 
 // One CTA per row at a time, three passes over it: any width.
@@ -355,10 +444,11 @@ template <typename T>
 __global__ void __launch_bounds__(512) distill_wide_kernel(const T* __restrict__ logits,
                                                            int64_t stride, T* __restrict__ dlogits,
                                                            DistillArgs a) {
-  extern __shared__ float smem[];
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* rest = reinterpret_cast<float*>(smem);
   __shared__ float scratch[33];
-  const Teacher teach{smem, reinterpret_cast<int*>(smem) + a.top,
-                      reinterpret_cast<int*>(smem) + 2 * a.top, teacher_bits(a.top)};
+  const Teacher teach{rest, reinterpret_cast<int*>(rest) + a.top,
+                      reinterpret_cast<int*>(rest) + 2 * a.top, teacher_bits(a.top)};
   const float gs = a.grad_loss ? a.grad_scale * __ldg(a.grad_loss) : a.grad_scale;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* xr = logits + row * stride;
@@ -429,60 +519,43 @@ __global__ void __launch_bounds__(256) scale_by_kernel(T* __restrict__ x, int64_
     x[i] = from_f32<T>(to_f32(x[i]) * s);
 }
 
-// Threads and CTAs per row.  CTAs of 256 threads (or fewer, for narrow rows) as
-// long as a cluster of 8 holds the row, else of 512 and 1024; 0 threads: none
-// does.  More CTAs than the row needs while that leaves SMs idle.
-static void distill_geometry(int64_t rows, int64_t vocab, int* threads, int* size) {
-  *threads = 0;
-  for (int n : {64, 128, 256}) {
-    if ((int64_t)n * kDistillEach >= vocab) {
-      *threads = n;
-      *size = 1;
-      break;
-    }
-  }
-  for (int n = 256; *threads == 0 && n <= kDistillMaxThreads; n *= 2)
-    for (int k = 1; *threads == 0 && k <= kDistillCluster; k *= 2)
-      if ((int64_t)n * k * kDistillEach >= vocab) {
-        *threads = n;
-        *size = k;
-      }
-  if (*threads == 0) return;
-  while (*size < kDistillCluster && rows * *size < sm_count() &&
-         vocab >= (int64_t)*size * 2 * *threads * 4)
-    *size *= 2;
+// CTAs per row: parts of 64 KB, three of them resident on an SM, as long as a
+// cluster of 8 holds the row, larger ones beyond; 0 if they would be too large.
+// More CTAs than the row needs while that leaves SMs idle and each has some work.
+static int distill_cluster(int64_t rows, int64_t bytes) {
+  int size = 1;
+  while (size < kDistillCluster && bytes > (int64_t)size * kDistillPart) size *= 2;
+  if (bytes > (int64_t)size * kDistillMaxPart) return 0;
+  while (size < kDistillCluster && rows * size * 2 <= sm_count() &&
+         bytes >= (int64_t)size * 2 * kDistillThreads * 16)
+    size *= 2;
+  return size;
 }
 
 template <typename T>
 static oxc_status distill_launch(const void* logits, int64_t stride, void* dlogits,
-                                 const DistillArgs& a, cudaStream_t s) {
+                                 const DistillArgs& a, int* losses, cudaStream_t s) {
   const T* x = static_cast<const T*>(logits);
   T* d = static_cast<T*>(dlogits);
-  const size_t smem = teacher_smem(a.top);
-  int threads, size;
-  distill_geometry(a.rows, a.vocab, &threads, &size);
-  void (*kernel)(const T*, int64_t, T*, DistillArgs) = distill_wide_kernel<T>;
-  switch (threads) {
-    case 64: kernel = distill_cluster_kernel<T, 64>; break;
-    case 128: kernel = distill_cluster_kernel<T, 128>; break;
-    case 256: kernel = distill_cluster_kernel<T, 256>; break;
-    case 512: kernel = distill_cluster_kernel<T, 512>; break;
-    case 1024: kernel = distill_cluster_kernel<T, 1024>; break;
-    default: break;
-  }
+  const int size = distill_cluster(a.rows, (int64_t)a.vocab * sizeof(T));
+  // the largest part: its share of the row's vectors
+  const int vecs = a.vocab / (16 / (int)sizeof(T)), part = size ? 16 * ((vecs + size - 1) / size) : 0;
+  const size_t smem = teacher_smem(a.top) + part;
+  const void* kernel = size ? (const void*)distill_cluster_kernel<T> : (const void*)distill_wide_kernel<T>;
   if (smem > 40 * 1024) {  // beyond what a kernel may use unasked
-    const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return cuda_fail(e, "oxc_distill_loss");
   }
-  if (threads == 0) {
-    kernel<<<(unsigned)std::min<int64_t>(a.rows, (int64_t)sm_count() * 4), 512, smem, s>>>(x, stride, d, a);
+  *losses = size ? size : 1;
+  if (size == 0) {
+    distill_wide_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, (int64_t)sm_count() * 4), 512, smem, s>>>(x, stride, d, a);
     return check_launch("oxc_distill_loss");
   }
-  if (a.rows > 0x7fffffff / size)
-    return fail(OXC_ERR_NOT_IMPLEMENTED, "not implemented: distill_loss: %lld rows", (long long)a.rows);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.rows * size));
-  cfg.blockDim = dim3((unsigned)threads);
+  const int64_t resident = std::max<int64_t>(
+      1, (int64_t)sm_count() * occupancy(kernel, kDistillThreads, smem) / size);
+  cfg.gridDim = dim3((unsigned)(std::min(a.rows, resident) * size));
+  cfg.blockDim = dim3(kDistillThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -492,7 +565,7 @@ static oxc_status distill_launch(const void* logits, int64_t stride, void* dlogi
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, x, stride, d, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, distill_cluster_kernel<T>, x, stride, d, a, part);
   return e == cudaSuccess ? check_launch("oxc_distill_loss") : cuda_fail(e, "oxc_distill_loss");
 }
 
@@ -529,6 +602,7 @@ oxc_status oxc_distill_loss(const void* logits, int64_t logits_stride, const flo
   if (rows > 0 && vocab == 0)
     return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: distill_loss over zero classes");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int losses = 1;  // per row
   if (rows > 0) {
     if (!logits || !row_loss || (top > 0 && (!teacher_logits || !teacher_ids)))
       return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: distill_loss: null pointer");
@@ -537,12 +611,13 @@ oxc_status oxc_distill_loss(const void* logits, int64_t logits_stride, const flo
                         (float)(1.4426950408889634 / tau), (float)(tau / (double)total_rows),
                         grad_loss, row_loss, rows, (int)vocab, err_flag};
     const oxc_status st = dtype == OXC_BF16
-                              ? distill_launch<bf16>(logits, logits_stride, dlogits, a, s)
-                              : distill_launch<float>(logits, logits_stride, dlogits, a, s);
+                              ? distill_launch<bf16>(logits, logits_stride, dlogits, a, &losses, s)
+                              : distill_launch<float>(logits, logits_stride, dlogits, a, &losses, s);
     if (st) return st;
   }
   const double scale = (double)temperature * (double)temperature / (double)total_rows;
-  launch_dependent(distill_loss_kernel, dim3(1), dim3(1024), s, (const float*)row_loss, rows, scale,
+  launch_dependent(distill_loss_kernel, dim3(1), dim3(1024), s, (const float*)row_loss, rows * losses,
+                   scale,
                    loss);
   return check_launch("oxc_distill_loss (sum)");
 }

@@ -833,7 +833,7 @@ def distill_loss_fwd(logits, teacher_logits, teacher_ids, temperature=1.0, total
     x = _rows2d(logits)
     rows, vocab = x.shape
     loss = torch.empty(1, dtype=torch.float32, device=x.device)
-    row_loss = torch.empty(rows, dtype=torch.float32, device=x.device)
+    row_loss = torch.empty(rows * N.DISTILL_PARTS, dtype=torch.float32, device=x.device)
     dlogits = torch.empty(logits.shape, dtype=x.dtype, device=x.device) if grad else None
     N.check(N.load().oxc_distill_loss(
         x.data_ptr(), x.stride(0), tl.data_ptr(), ti.data_ptr(), ti.shape[-1], float(temperature),
