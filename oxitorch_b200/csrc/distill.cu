@@ -26,9 +26,15 @@
 namespace oxc {
 
 constexpr int kDistillMaxTop = 4096;
-constexpr int kDistillThreads = 256;
+constexpr int kDistillThreads = 256;          // per CTA at most
+#ifndef DVEC
+#define DVEC 8
+#endif
+#ifndef DPART
+#define DPART 64
+#endif
 constexpr int kDistillCopies = 4;             // bulk copies per part of a row
-constexpr int kDistillPart = 64 * 1024;       // bytes of a row per CTA, if a cluster can
+constexpr int kDistillPart = DPART * 1024;       // bytes of a row per CTA, if a cluster can
 constexpr int kDistillMaxPart = 160 * 1024;   // and at most
 constexpr int kDistillCluster = OXC_DISTILL_PARTS;  // CTAs per row at most
 
@@ -46,9 +52,21 @@ __device__ __forceinline__ float ex2_approx(float t) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
 }
+__device__ __forceinline__ float rcp_approx(float t) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return r;
+}
 // exp(d / tau) for d = x - max <= 0, c = log2(e) / tau.  The subtraction comes
 // first, so the large terms see only ex2's own error; results below 2^-126 are 0.
 __device__ __forceinline__ float exp_scaled(float d, float c) { return ex2_approx(d * c); }
+
+// Maximum over the warp, NaN ignored.
+__device__ __forceinline__ float warp_max_fast(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
 
 // The teacher's side of a row, in shared memory: its logits, then probabilities,
 // and ids (negative for entries that do not count).
@@ -161,11 +179,8 @@ __device__ __forceinline__ float2 pair_merge(float2 a, float2 b, float c) {
   return make_float2(m, sa + sb);
 }
 __device__ __forceinline__ float2 warp_merge(float2 v, float c) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    v = pair_merge(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o),
-                                  __shfl_xor_sync(0xffffffffu, v.y, o)), c);
-  return v;
+  const float m = warp_max_fast(v.x);
+  return make_float2(m, warp_sum(m == -INFINITY ? v.y : v.y * exp_scaled(v.x - m, c)));
 }
 
 // A row's bytes are cut at 16-byte boundaries of memory: `body` whole vectors,
@@ -177,10 +192,10 @@ struct RowCut {
   static constexpr int kVec = 16 / (int)sizeof(T);
   const T* row;
   int head, body, v0, v1;
-  __device__ __forceinline__ RowCut(const T* row, int vocab, int rank, int size) : row(row) {
+  __device__ __forceinline__ RowCut(const T* row, int vocab, int rank, int log_size) : row(row) {
     head = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T));
     body = (vocab - head) / kVec;
-    const int each = (body + size - 1) / size;
+    const int each = (body + (1 << log_size) - 1) >> log_size;
     v0 = min(body, rank * each);
     v1 = min(body, v0 + each);
   }
@@ -230,13 +245,12 @@ __device__ __forceinline__ void unpack(const uint4& q, float2 (&v)[8 / (int)size
 // (max, sum) pair of its own, and one cluster barrier exchanges all of them; a
 // barrier within the CTA precedes the corrections at the teacher's tokens.  Each
 // CTA sums the loss over the tokens in its part: row_loss[row][rank].
-template <typename T>
-__global__ void __launch_bounds__(kDistillThreads)
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS)
 distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restrict__ dlogits,
                        DistillArgs a, int part_bytes) {
   namespace cg = cooperative_groups;
   using Cut = RowCut<T>;
-  constexpr int THREADS = kDistillThreads;
   constexpr int kVec = Cut::kVec, kPairs = kVec / 2;
   constexpr int kWarps = THREADS / 32;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -245,6 +259,7 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
   __shared__ uint64_t full[kDistillCopies];
   cg::cluster_group cluster = cg::this_cluster();
   const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int log_size = 31 - __clz(size);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint4* buffer = reinterpret_cast<const uint4*>(smem);
   float* rest = reinterpret_cast<float*>(smem + part_bytes);
@@ -252,20 +267,20 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
                       reinterpret_cast<int*>(rest) + 2 * a.top, teacher_bits(a.top)};
   float* logit_k = rest + 2 * a.top + (1 << teach.bits);  // the student's logit at id[k]
   const float gs = a.grad_loss ? a.grad_scale * __ldg(a.grad_loss) : a.grad_scale;
-  const int64_t rows_apart = gridDim.x / size;
+  const int64_t rows_apart = gridDim.x >> log_size;
+  const int entry_warps = min(kWarps, (a.top + 31) / 32);  // warps with entries of the teacher
 
-  // vectors [copy_start(i), copy_start(i + 1)) of a part of n are copy i's: whole
-  // rounds of the threads
-  auto copy_start = [](int n, int i) {
-    const int rounds = (n + THREADS - 1) / THREADS;
-    return min(n, (rounds * i + kDistillCopies - 1) / kDistillCopies * THREADS);
+  // copy i of a part of n vectors: [i, i + 1) * copy_vecs(n) of them, whole rounds
+  // of the threads
+  auto copy_vecs = [](int n) {
+    return (n + kDistillCopies * THREADS - 1) / (kDistillCopies * THREADS) * THREADS;
   };
   auto fetch = [&](int64_t row) {  // thread 0
-    const Cut cut(logits + row * stride, a.vocab, rank, size);
-    const int n = cut.v1 - cut.v0;
+    const Cut cut(logits + row * stride, a.vocab, rank, log_size);
+    const int n = cut.v1 - cut.v0, each = copy_vecs(n);
 #pragma unroll
     for (int i = 0; i < kDistillCopies; ++i) {
-      const int from = copy_start(n, i), bytes = 16 * (copy_start(n, i + 1) - from);
+      const int from = i * each, bytes = 16 * (min(n, from + each) - from);
       if (bytes > 0) {
         mbar_arrive_expect_tx(&full[i], (uint32_t)bytes);
         bulk_g2s(smem + 16 * from, cut.part() + (int64_t)from * kVec, (uint32_t)bytes, &full[i]);
@@ -274,7 +289,7 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
       }
     }
   };
-  int64_t row = blockIdx.x / size;
+  int64_t row = blockIdx.x >> log_size;
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int i = 0; i < kDistillCopies; ++i) mbar_init(&full[i], 1);
@@ -282,9 +297,16 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
     if (row < a.rows) fetch(row);
   }
   __syncthreads();
+  // this thread's first entry of the teacher, a row ahead
+  int64_t next_id = -1;
+  float next_t = 0.0f;
+  if ((int)threadIdx.x < a.top && row < a.rows) {
+    next_id = __ldcs(a.ti + row * a.top + threadIdx.x);
+    next_t = __ldcs(a.tl + row * a.top + threadIdx.x);
+  }
   for (uint32_t n = 0; row < a.rows; row += rows_apart, ++n) {
-    const Cut cut(logits + row * stride, a.vocab, rank, size);
-    const int vecs = cut.v1 - cut.v0;
+    const Cut cut(logits + row * stride, a.vocab, rank, log_size);
+    const int vecs = cut.v1 - cut.v0, copy = copy_vecs(vecs);
     const int edges = a.vocab - cut.body * kVec;  // before the body and after it
     const bool has_edge = rank == size - 1 && (int)threadIdx.x < edges;
     const int edge_at = (int)threadIdx.x < cut.head ? threadIdx.x : cut.body * kVec + threadIdx.x;
@@ -296,8 +318,9 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
     for (int i = threadIdx.x; i < (1 << teach.bits); i += THREADS) teach.table[i] = -1;
     float2 tp = make_float2(-INFINITY, 0.0f);
     for (int k = threadIdx.x; k < a.top; k += THREADS) {
-      const int64_t id = __ldcs(a.ti + row * a.top + k);
-      float v = __ldcs(a.tl + row * a.top + k);
+      const bool first = k < THREADS;
+      const int64_t id = first ? next_id : a.ti[row * a.top + k];
+      float v = first ? next_t : a.tl[row * a.top + k];
       if (id < 0) v = -INFINITY;
       if (id >= a.vocab) {
         if (rank == 0) record_bad_id(a.err, id, a.vocab);
@@ -308,17 +331,20 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
       tp.x = fmaxf(tp.x, v);
       if (v != v) tp.y = NAN;
     }
-    tp.x = warp_max(tp.x);
-    for (int k = threadIdx.x; k < a.top; k += THREADS)
-      if (teach.id[k] >= 0) tp.y += exp_scaled(teach.prob[k] - tp.x, a.c);
-    tp.y = warp_sum(tp.y);
+    if (warp < entry_warps) {
+      tp.x = warp_max_fast(tp.x);
+      for (int k = threadIdx.x; k < a.top; k += THREADS)
+        if (teach.id[k] >= 0) tp.y += exp_scaled(teach.prob[k] - tp.x, a.c);
+      tp.y = warp_sum(tp.y);
+      if (lane == 0) teacher[warp] = tp;
+    }
 
     float2 sp = make_float2(edge, edge == -INFINITY ? 0.0f : edge - edge + 1.0f);
 #pragma unroll
     for (int i = 0; i < kDistillCopies; ++i) {
       if (!mbar_wait(&full[i], n & 1u)) atomicOr(&g_kernel_error, OXC_KERR_PIPELINE_TIMEOUT);
-      int v = copy_start(vecs, i) + threadIdx.x;
-      const int end = copy_start(vecs, i + 1);
+      int v = i * copy + threadIdx.x;
+      const int end = min(vecs, (i + 1) * copy);
       constexpr int U = 16 / kVec;  // vectors at a time
       for (; v + (U - 1) * THREADS < end; v += U * THREADS) {
         float2 f[8];
@@ -344,18 +370,21 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
       else logit_k[k] = to_f32(in_body ? reinterpret_cast<const T*>(smem)[id - cut.head - cut.v0 * kVec] : cut.row[id]);
     }
     sp = warp_merge(sp, a.c);
-    if (lane == 0) {
-      student[n & 1u][warp] = sp;
-      teacher[warp] = tp;
-    }
+    if (lane == 0) student[n & 1u][warp] = sp;
     if (size > 1) cluster.sync();
     else __syncthreads();
     const int64_t next = row + rows_apart;
-    if (threadIdx.x == 0 && next < a.rows) {
-      const Cut ahead(logits + next * stride, a.vocab, rank, size);
-      if (ahead.v1 > ahead.v0)
-        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(ahead.part()),
-                     "r"((ahead.v1 - ahead.v0) * 16) : "memory");
+    if (next < a.rows) {
+      if (threadIdx.x == 0) {
+        const Cut ahead(logits + next * stride, a.vocab, rank, log_size);
+        if (ahead.v1 > ahead.v0)
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(ahead.part()),
+                       "r"((ahead.v1 - ahead.v0) * 16) : "memory");
+      }
+      if ((int)threadIdx.x < a.top) {
+        next_id = __ldcs(a.ti + next * a.top + threadIdx.x);
+        next_t = __ldcs(a.tl + next * a.top + threadIdx.x);
+      }
     }
     sp = make_float2(-INFINITY, 0.0f);
     for (int i = lane; i < size * kWarps; i += 32) {
@@ -363,11 +392,11 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
       sp = pair_merge(sp, s[i % kWarps], a.c);
     }
     sp = warp_merge(sp, a.c);
-    tp = warp_merge(lane < kWarps ? teacher[lane] : make_float2(-INFINITY, 0.0f), a.c);
+    tp = warp_merge(lane < entry_warps ? teacher[lane] : make_float2(-INFINITY, 0.0f), a.c);
     const bool none = tp.x == -INFINITY && tp.y == 0.0f, bad = tp.y != tp.y;
     // a row of -inf alone has no softmax: its sum counts as NaN
     if (sp.x == -INFINITY) sp.y = NAN;
-    const float unit = bad ? NAN : gs * __fdiv_rn(1.0f, sp.y);
+    const float unit = bad ? NAN : gs * rcp_approx(sp.y);
     T* dr = dlogits ? dlogits + row * (int64_t)a.vocab : nullptr;
     if (dr) {
       T* out = dr + cut.head + (int64_t)cut.v0 * kVec;
@@ -397,31 +426,33 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
     }
     // this thread's entries: the loss at those in this part, and whether an id is
     // there twice (finding it in the table already means it is)
-    const float t_log = logf(tp.y), s_log = logf(sp.y), t_unit = __fdiv_rn(1.0f, tp.y);
-    float loss = 0.0f;
     int twice = 0;
-    for (int k = threadIdx.x; k < a.top; k += THREADS) {
-      const int id = teach.id[k];
-      if (id < 0) continue;
-      const float z = (teach.prob[k] - tp.x), p = exp_scaled(z, a.c) * t_unit;
-      teach.prob[k] = p;
-      if (p > 0.0f)
-        loss += p * ((z * a.inv_tau - t_log) - ((logit_k[k] - sp.x) * a.inv_tau - s_log));
-      unsigned int h = ((unsigned int)id * 2654435769u) >> (32 - teach.bits);
-      for (int i = 0; i < (1 << teach.bits); ++i) {
-        const int was = atomicCAS(&teach.table[h], -1, id);
-        if (was == -1) break;
-        if (was == id) { twice = 1; break; }
-        h = (h + 1) & ((1u << teach.bits) - 1);
+    if (warp < entry_warps) {
+      const float t_log = logf(tp.y), s_log = logf(sp.y), t_unit = rcp_approx(tp.y);
+      float loss = 0.0f;
+      for (int k = threadIdx.x; k < a.top; k += THREADS) {
+        const int id = teach.id[k];
+        if (id < 0) continue;
+        const float z = (teach.prob[k] - tp.x), p = exp_scaled(z, a.c) * t_unit;
+        teach.prob[k] = p;
+        if (p > 0.0f)
+          loss += p * ((z * a.inv_tau - t_log) - ((logit_k[k] - sp.x) * a.inv_tau - s_log));
+        unsigned int h = ((unsigned int)id * 2654435769u) >> (32 - teach.bits);
+        for (int i = 0; i < (1 << teach.bits); ++i) {
+          const int was = atomicCAS(&teach.table[h], -1, id);
+          if (was == -1) break;
+          if (was == id) { twice = 1; break; }
+          h = (h + 1) & ((1u << teach.bits) - 1);
+        }
       }
+      loss = warp_sum(loss);
+      if (lane == 0) partial[warp] = loss;
     }
-    loss = warp_sum(loss);
-    if (lane == 0) partial[warp] = loss;
     const bool repeated = __syncthreads_or(twice);
     if (threadIdx.x == 0) {
       if (next < a.rows) fetch(next);  // the part has been read twice
       float sum = 0.0f;
-      for (int w = 0; w < kWarps; ++w) sum += partial[w];
+      for (int w = 0; w < entry_warps; ++w) sum += partial[w];
       a.row_loss[row * size + rank] = none ? 0.0f : bad || sp.y != sp.y ? NAN : sum;
     }
     // q - p over the q just written
@@ -541,7 +572,11 @@ static oxc_status distill_launch(const void* logits, int64_t stride, void* dlogi
   // the largest part: its share of the row's vectors
   const int vecs = a.vocab / (16 / (int)sizeof(T)), part = size ? 16 * ((vecs + size - 1) / size) : 0;
   const size_t smem = teacher_smem(a.top) + part;
-  const void* kernel = size ? (const void*)distill_cluster_kernel<T> : (const void*)distill_wide_kernel<T>;
+  const int threads = part <= 64 * 16 * DVEC ? 64 : part <= 128 * 16 * DVEC ? 128 : 256;
+  auto cluster = threads == 64    ? distill_cluster_kernel<T, 64>
+                 : threads == 128 ? distill_cluster_kernel<T, 128>
+                                  : distill_cluster_kernel<T, 256>;
+  const void* kernel = size ? (const void*)cluster : (const void*)distill_wide_kernel<T>;
   if (smem > 40 * 1024) {  // beyond what a kernel may use unasked
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return cuda_fail(e, "oxc_distill_loss");
@@ -553,9 +588,9 @@ static oxc_status distill_launch(const void* logits, int64_t stride, void* dlogi
   }
   cudaLaunchConfig_t cfg = {};
   const int64_t resident = std::max<int64_t>(
-      1, (int64_t)sm_count() * occupancy(kernel, kDistillThreads, smem) / size);
+      1, (int64_t)sm_count() * occupancy(kernel, threads, smem) / size);
   cfg.gridDim = dim3((unsigned)(std::min(a.rows, resident) * size));
-  cfg.blockDim = dim3(kDistillThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -565,7 +600,7 @@ static oxc_status distill_launch(const void* logits, int64_t stride, void* dlogi
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, distill_cluster_kernel<T>, x, stride, d, a, part);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, cluster, x, stride, d, a, part);
   return e == cudaSuccess ? check_launch("oxc_distill_loss") : cuda_fail(e, "oxc_distill_loss");
 }
 
