@@ -27,14 +27,8 @@ namespace oxc {
 
 constexpr int kDistillMaxTop = 4096;
 constexpr int kDistillThreads = 256;          // per CTA at most
-#ifndef DVEC
-#define DVEC 8
-#endif
-#ifndef DPART
-#define DPART 64
-#endif
 constexpr int kDistillCopies = 4;             // bulk copies per part of a row
-constexpr int kDistillPart = DPART * 1024;       // bytes of a row per CTA, if a cluster can
+constexpr int kDistillPart = 100 * 1024;      // bytes of a row per CTA, if a cluster can
 constexpr int kDistillMaxPart = 160 * 1024;   // and at most
 constexpr int kDistillCluster = OXC_DISTILL_PARTS;  // CTAs per row at most
 
@@ -550,7 +544,7 @@ __global__ void __launch_bounds__(256) scale_by_kernel(T* __restrict__ x, int64_
     x[i] = from_f32<T>(to_f32(x[i]) * s);
 }
 
-// CTAs per row: parts of 64 KB, three of them resident on an SM, as long as a
+// CTAs per row: parts of up to 100 KB, two or more resident on an SM, as long as a
 // cluster of 8 holds the row, larger ones beyond; 0 if they would be too large.
 // More CTAs than the row needs while that leaves SMs idle and each has some work.
 static int distill_cluster(int64_t rows, int64_t bytes) {
@@ -572,7 +566,7 @@ static oxc_status distill_launch(const void* logits, int64_t stride, void* dlogi
   // the largest part: its share of the row's vectors
   const int vecs = a.vocab / (16 / (int)sizeof(T)), part = size ? 16 * ((vecs + size - 1) / size) : 0;
   const size_t smem = teacher_smem(a.top) + part;
-  const int threads = part <= 64 * 16 * DVEC ? 64 : part <= 128 * 16 * DVEC ? 128 : 256;
+  const int threads = part <= 64 * 16 * 8 ? 64 : part <= 128 * 16 * 8 ? 128 : 256;
   auto cluster = threads == 64    ? distill_cluster_kernel<T, 64>
                  : threads == 128 ? distill_cluster_kernel<T, 128>
                                   : distill_cluster_kernel<T, 256>;
@@ -587,9 +581,7 @@ static oxc_status distill_launch(const void* logits, int64_t stride, void* dlogi
     return check_launch("oxc_distill_loss");
   }
   cudaLaunchConfig_t cfg = {};
-  const int64_t resident = std::max<int64_t>(
-      1, (int64_t)sm_count() * occupancy(kernel, threads, smem) / size);
-  cfg.gridDim = dim3((unsigned)(std::min(a.rows, resident) * size));
+  cfg.gridDim = dim3((unsigned)size);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -600,6 +592,16 @@ static oxc_status distill_launch(const void* logits, int64_t stride, void* dlogi
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  // as many clusters as are resident at once: with more, the rest would run as a
+  // second wave (a cluster's CTAs share a GPC, so not every SM can be used)
+  int64_t resident = (int64_t)sm_count() * occupancy(kernel, threads, smem) / size;
+  if (size > 1 && a.rows > resident / 2) {
+    int n = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+    if (e != cudaSuccess) return cuda_fail(e, "oxc_distill_loss");
+    resident = n;
+  }
+  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(a.rows, std::max<int64_t>(resident, 1)) * size));
   const cudaError_t e = cudaLaunchKernelEx(&cfg, cluster, x, stride, d, a, part);
   return e == cudaSuccess ? check_launch("oxc_distill_loss") : cuda_fail(e, "oxc_distill_loss");
 }
