@@ -196,27 +196,6 @@ struct RowCut {
   __device__ __forceinline__ const T* part() const { return row + head + (int64_t)v0 * kVec; }
 };
 
-// Folds N logits (N even) into a running (max, sum of exponentials): the maximum
-// of the N first, a rescale of the sum when it grows, then N terms.
-template <int N>
-__device__ __forceinline__ void pair_fold(float2& p, const float2 (&v)[N / 2], float c) {
-  float m = p.x;
-#pragma unroll
-  for (int i = 0; i < N / 2; ++i) m = fmaxf(m, fmaxf(v[i].x, v[i].y));
-  if (m > p.x) {
-    p.y *= exp_scaled(p.x - m, c);
-    p.x = m;
-  }
-  const float base = m == -INFINITY ? 0.0f : -m;
-  float2 s = make_float2(0.0f, 0.0f);
-#pragma unroll
-  for (int i = 0; i < N / 2; ++i) {
-    const float2 d = __fmul2_rn(__fadd2_rn(v[i], make_float2(base, base)), make_float2(c, c));
-    s = __fadd2_rn(s, make_float2(ex2_approx(d.x), ex2_approx(d.y)));
-  }
-  p.y += s.x + s.y;
-}
-
 // The elements of a 16-byte vector, in pairs.
 template <typename T>
 __device__ __forceinline__ void unpack(const uint4& q, float2 (&v)[8 / (int)sizeof(T)]) {
@@ -230,15 +209,67 @@ __device__ __forceinline__ void unpack(const uint4& q, float2 (&v)[8 / (int)size
   }
 }
 
+// Folds V vectors of logits into a running (max, sum of exponentials): the maximum
+// of all first (of bf16, two at a time), a rescale of the sum when it grows, then
+// the terms.
+template <typename T, int V>
+__device__ __forceinline__ void pair_fold(float2& p, const uint4 (&q)[V], float c) {
+  constexpr int kPairs = 8 / (int)sizeof(T);
+  float m = p.x;
+  if constexpr (sizeof(T) == 2) {
+    __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&q[0].x);
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      const uint32_t w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h = __hmax2(h, *reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+    }
+    m = fmaxf(m, fmaxf(__low2float(h), __high2float(h)));
+  } else {
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      m = fmaxf(m, fmaxf(__uint_as_float(q[u].x), __uint_as_float(q[u].y)));
+      m = fmaxf(m, fmaxf(__uint_as_float(q[u].z), __uint_as_float(q[u].w)));
+    }
+  }
+  if (m > p.x) {
+    p.y *= exp_scaled(p.x - m, c);
+    p.x = m;
+  }
+  const float base = m == -INFINITY ? 0.0f : -m;
+  float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for (int u = 0; u < V; ++u) {
+    float2 v[kPairs];
+    unpack<T>(q[u], v);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const float2 d = __fmul2_rn(__fadd2_rn(v[i], make_float2(base, base)), make_float2(c, c));
+      s = __fadd2_rn(s, make_float2(ex2_approx(d.x), ex2_approx(d.y)));
+    }
+  }
+  p.y += s.x + s.y;
+}
+
+// Sends v to `to` in CTA `rank` of the cluster, completing 8 bytes on its `bar`.
+__device__ __forceinline__ void send_pair(const float2* to, uint64_t* bar, int rank, float2 v) {
+  uint32_t dst, rbar;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(to)), "r"(rank));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(rbar) : "r"(smem_u32(bar)), "r"(rank));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];"
+               ::"r"(dst), "f"(v.x), "f"(v.y), "r"(rbar) : "memory");
+}
+
 // Persistent clusters, a row at a time.  A CTA's part of the row arrives in
 // shared memory by bulk copies; one pass over it makes the (max, sum) pair, a
 // second the gradient, and then the copies of the next row's part are started,
 // whose bytes L2 was asked for when the second pass began.  The teacher's side of
 // a row is worked out while its logits are on the way.  The warps of a row meet
-// twice: each reduces its logits, and its share of the teacher's entries, to a
-// (max, sum) pair of its own, and one cluster barrier exchanges all of them; a
-// barrier within the CTA precedes the corrections at the teacher's tokens.  Each
-// CTA sums the loss over the tokens in its part: row_loss[row][rank].
+// twice: each reduces its logits to a (max, sum) pair and sends it to every CTA of
+// the cluster (a cluster barrier would also wait for the gradient's stores of the
+// row before); a barrier within the CTA precedes the corrections at the teacher's
+// tokens.  Each CTA sums the loss over the tokens in its part:
+// row_loss[row][rank].
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restrict__ dlogits,
@@ -248,7 +279,11 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
   constexpr int kVec = Cut::kVec, kPairs = kVec / 2;
   constexpr int kWarps = THREADS / 32;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float2 student[2][kWarps], teacher[kWarps];
+  // by the parity of the row: a CTA that is a row ahead of another sends into the
+  // set that the other is not reading
+  __shared__ float2 student[2][kDistillCluster * kWarps];
+  __shared__ uint64_t met[2];
+  __shared__ float2 teacher[kWarps];
   __shared__ float partial[kWarps];
   __shared__ uint64_t full[kDistillCopies];
   cg::cluster_group cluster = cg::this_cluster();
@@ -287,10 +322,13 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int i = 0; i < kDistillCopies; ++i) mbar_init(&full[i], 1);
+    mbar_init(&met[0], 1);
+    mbar_init(&met[1], 1);
     fence_barrier_init();
     if (row < a.rows) fetch(row);
   }
-  __syncthreads();
+  if (size > 1) cluster.sync();  // nobody sends before the barriers are there
+  else __syncthreads();
   // this thread's first entry of the teacher, a row ahead
   int64_t next_id = -1;
   float next_t = 0.0f;
@@ -305,6 +343,8 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
     const bool has_edge = rank == size - 1 && (int)threadIdx.x < edges;
     const int edge_at = (int)threadIdx.x < cut.head ? threadIdx.x : cut.body * kVec + threadIdx.x;
     const float edge = has_edge ? to_f32(cut.row[edge_at]) : -INFINITY;
+    // the row's pairs: one from each warp of the cluster
+    if (threadIdx.x == 0) mbar_arrive_expect_tx(&met[n & 1u], (uint32_t)(size * kWarps * sizeof(float2)));
 
     // the teacher's entries k with (k / 32) % kWarps == warp: absent ones get id
     // -1.  An id that is too large or a NaN logit makes the sum NaN, and with it
@@ -341,16 +381,14 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
       const int end = min(vecs, (i + 1) * copy);
       constexpr int U = 16 / kVec;  // vectors at a time
       for (; v + (U - 1) * THREADS < end; v += U * THREADS) {
-        float2 f[8];
+        uint4 q[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          unpack<T>(buffer[v + u * THREADS], reinterpret_cast<float2(&)[kPairs]>(f[u * kPairs]));
-        pair_fold<16>(sp, f, a.c);
+        for (int u = 0; u < U; ++u) q[u] = buffer[v + u * THREADS];
+        pair_fold<T, U>(sp, q, a.c);
       }
       for (; v < end; v += THREADS) {
-        float2 f[kPairs];
-        unpack<T>(buffer[v], f);
-        pair_fold<kVec>(sp, f, a.c);
+        const uint4 q[1] = {buffer[v]};
+        pair_fold<T, 1>(sp, q, a.c);
       }
     }
     // the student's logits at this thread's entries; ids of other CTAs' parts turn
@@ -364,9 +402,7 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
       else logit_k[k] = to_f32(in_body ? reinterpret_cast<const T*>(smem)[id - cut.head - cut.v0 * kVec] : cut.row[id]);
     }
     sp = warp_merge(sp, a.c);
-    if (lane == 0) student[n & 1u][warp] = sp;
-    if (size > 1) cluster.sync();
-    else __syncthreads();
+    if (lane < size) send_pair(&student[n & 1u][rank * kWarps + warp], &met[n & 1u], lane, sp);
     const int64_t next = row + rows_apart;
     if (next < a.rows) {
       if (threadIdx.x == 0) {
@@ -380,11 +416,10 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
         next_t = __ldcs(a.tl + next * a.top + threadIdx.x);
       }
     }
+    __syncthreads();  // the teacher's pairs are there
+    if (!mbar_wait(&met[n & 1u], (n >> 1) & 1u)) atomicOr(&g_kernel_error, OXC_KERR_PIPELINE_TIMEOUT);
     sp = make_float2(-INFINITY, 0.0f);
-    for (int i = lane; i < size * kWarps; i += 32) {
-      const float2* s = size > 1 ? cluster.map_shared_rank(student[n & 1u], i / kWarps) : student[n & 1u];
-      sp = pair_merge(sp, s[i % kWarps], a.c);
-    }
+    for (int i = lane; i < size * kWarps; i += 32) sp = pair_merge(sp, student[n & 1u][i], a.c);
     sp = warp_merge(sp, a.c);
     tp = warp_merge(lane < entry_warps ? teacher[lane] : make_float2(-INFINITY, 0.0f), a.c);
     const bool none = tp.x == -INFINITY && tp.y == 0.0f, bad = tp.y != tp.y;
@@ -406,8 +441,12 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
         for (int k = 0; k < kPairs; ++k) {
           const float2 d = __fmul2_rn(__fadd2_rn(f[k], shift), c2);
           const float2 o = __fmul2_rn(make_float2(ex2_approx(d.x), ex2_approx(d.y)), unit2);
-          g[2 * k] = none ? 0.0f : o.x;
-          g[2 * k + 1] = none ? 0.0f : o.y;
+          g[2 * k] = o.x;
+          g[2 * k + 1] = o.y;
+        }
+        if (none) {
+#pragma unroll
+          for (int k = 0; k < kVec; ++k) g[k] = 0.0f;
         }
         if (vector) {
           store_from_f32<kVec>(out + (int64_t)v * kVec, g);
@@ -461,7 +500,6 @@ distill_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restri
     }
     if (repeated) __syncthreads();  // the other threads' entries are read
   }
-  if (size > 1) cluster.sync();  // no CTA leaves while its pairs are read
 }
 
 // One CTA per row at a time, three passes over it: any width.
