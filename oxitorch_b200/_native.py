@@ -223,12 +223,15 @@ SIGNATURES = {
 NOALLOC_SCRATCH_BYTES = 16 * 1024 * 1024
 
 _lib = None
+_device_seen = False
 
 
 def load(require_device: bool = True):
     """Loads the library (once).  Raises if it is missing; with
     ``require_device`` also raises when no CUDA device is visible."""
-    global _lib
+    global _lib, _device_seen
+    if _device_seen:
+        return _lib
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise RuntimeError(
@@ -240,8 +243,10 @@ def load(require_device: bool = True):
             fn.restype = res
             fn.argtypes = args
         _lib = lib
-    if require_device and _lib.oxc_device_count() <= 0:
-        raise RuntimeError("oxitorch_b200: no CUDA device is visible (there is no CPU fallback)")
+    if require_device:
+        if _lib.oxc_device_count() <= 0:
+            raise RuntimeError("oxitorch_b200: no CUDA device is visible (there is no CPU fallback)")
+        _device_seen = True
     return _lib
 
 

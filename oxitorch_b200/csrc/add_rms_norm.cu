@@ -16,10 +16,21 @@
 //
 // 8-bit output: per row, each block of `block` columns has the scale
 // s = max(amax(|y|) / 448, 2^-126) and q = e4m3(y / s), 448 being e4m3's
-// largest value.  y is not rounded to x's type in between.
+// largest value (y times the scale's reciprocal: a tie may fall to the other side
+// when y / s is within two roundings of it).  y is not rounded to x's type in
+// between.
 //
 // All are bound by HBM traffic: 8 + 2 sizeof(T) bytes an element forward, 9 +
-// sizeof(T) with the 8-bit output.
+// sizeof(T) with the 8-bit output, 12 + sizeof(T) (and 2 more at 16 bits) for the
+// VJP.  A row is held in registers by a group of 1 to 32 warps (as many as its
+// width needs at 4 vectors a thread, 2 in the VJP; narrow rows share a CTA), all
+// of its loads issued before the first is used.
+//
+// Vectors are 4 elements at addresses that are multiples of 4 elements.  Where the
+// columns are not a multiple of 4, a row starts `o` = 0 to 3 elements after such an
+// address, the same in every tensor (row_shift); the row's first and last vectors
+// are then partial ones, read and written by element.  Tensors that differ in
+// that take the kernels for single elements.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -35,8 +46,351 @@ __device__ __forceinline__ uint8_t to_e4m3(float v) {
   return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
 }
 
-// One CTA per row, the row in registers: thread t holds the VPT vectors
-// [(i * blockDim + t) * VW, +VW).
+__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
+// A block's scale from the bits of its largest |y|, which order like the values,
+// NaN above infinity: a NaN in a block makes its scale NaN.
+__device__ __forceinline__ float quant_scale(uint32_t amax) {
+  const float a = __uint_as_float(amax);
+  return a != a ? a : fmaxf(__fdiv_rn(a, 448.0f), 1.17549435e-38f);
+}
+
+// ---- rows in groups of warps ------------------------------------------------------------
+
+// Four elements as loaded: 16 bytes of f32, 8 of bf16.
+__device__ __forceinline__ float4 load_raw(const float* p) { return ld_stream(reinterpret_cast<const float4*>(p)); }
+__device__ __forceinline__ uint2 load_raw(const bf16* p) { return __ldcs(reinterpret_cast<const uint2*>(p)); }
+__device__ __forceinline__ void raw_f32(float (&d)[4], const float4& t) {
+  d[0] = t.x; d[1] = t.y; d[2] = t.z; d[3] = t.w;
+}
+__device__ __forceinline__ void raw_f32(float (&d)[4], const uint2& t) {
+  d[0] = bf16_lo(t.x); d[1] = bf16_hi(t.x); d[2] = bf16_lo(t.y); d[3] = bf16_hi(t.y);
+}
+template <typename T>
+using raw_t = decltype(load_raw(static_cast<const T*>(nullptr)));
+
+// A thread's place in its row: vector i covers columns [e(i), e(i) + 4) of which
+// those outside [0, cols) do not exist.  Without EDGE the shift is 0 and a vector
+// exists whole or not at all.
+template <bool EDGE>
+struct RowSlots {
+  int cols, o, first, step;  // columns; shift; the thread's first vector, from one to the next
+  __device__ __forceinline__ int e(int i) const { return 4 * (first + i * step) - (EDGE ? o : 0); }
+  __device__ __forceinline__ bool partial(int e) const { return EDGE && (e < 0 || e + 4 > cols); }
+  // the nearest vector that is whole: somewhere to load from without a branch
+  __device__ __forceinline__ int whole(int e) const {
+    if constexpr (!EDGE) return min(e, cols - 4);
+    return max(min(e, ((cols + o) & ~3) - 4 - o), o ? 4 - o : 0);
+  }
+  template <typename T>
+  __device__ __forceinline__ void take(float (&d)[4], const raw_t<T>& raw, const T* row, int e) const {
+    raw_f32(d, raw);
+    if (!EDGE) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) d[k] = e < cols ? d[k] : 0.0f;
+    } else if (partial(e)) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) d[k] = e + k >= 0 && e + k < cols ? to_f32(row[e + k]) : 0.0f;
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void put(T* row, int e, const float (&d)[4]) const {
+    if (!partial(e)) {
+      store_from_f32<4>(row + e, d);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (e + k >= 0 && e + k < cols) row[e + k] = from_f32<T>(d[k]);
+    }
+  }
+  // a [cols] parameter, 16-byte aligned
+  __device__ __forceinline__ void weights(float (&d)[4], const float* w, int e) const {
+    if (!EDGE || (o == 0 && !partial(e))) {
+      raw_f32(d, __ldg(reinterpret_cast<const float4*>(w + whole(e))));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) d[k] = __ldg(w + min(max(e + k, 0), cols - 1));
+    }
+  }
+};
+
+// Barrier and sum over a group of warps; `scratch` has a place for each of its
+// warps and is not written again before the group's next barrier.
+__device__ __forceinline__ void group_sync(int group, int warps) {
+  if (warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * warps) : "memory");
+  else __syncwarp();
+}
+__device__ __forceinline__ float group_total(float v, float* scratch, int group, int warps) {
+  v = warp_sum(v);
+  if (warps == 1) return v;
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - group * warps;
+  if (lane == 0) scratch[warp] = v;
+  group_sync(group, warps);
+  return warp_sum(lane < warps ? scratch[lane] : 0.0f);
+}
+
+constexpr int kMaxGroups = 8;  // per CTA
+
+template <typename T, int VPT, int MAXT, bool QUANT, bool EDGE>
+__global__ void __launch_bounds__(MAXT) add_rms_fwd_rows_kernel(
+    const T* __restrict__ x, int64_t x_stride, const float* __restrict__ res, int64_t res_stride,
+    const float* __restrict__ w, T* __restrict__ y, uint8_t* __restrict__ q,
+    float* __restrict__ scale, int block_cols, float* __restrict__ r, float* __restrict__ rstd,
+    int64_t rows, int cols, float eps, int group_warps) {
+  __shared__ float scratch[32];
+  __shared__ uint32_t amax[QUANT ? kQuantMaxBlocks + 1 : 1];
+  const int lane = threadIdx.x & 31, group = (threadIdx.x >> 5) / group_warps;
+  const int in_group = threadIdx.x - group * group_warps * 32;
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / (32 * group_warps)) + group;
+  if (row >= rows) return;  // the whole group
+  const RowSlots<EDGE> s{cols, EDGE ? (int)((row * cols) & 3) : 0, in_group, group_warps * 32};
+  const T* xr = x + row * x_stride;
+  const float* rr = res + row * res_stride;
+  raw_t<T> rx[VPT];
+  float4 rv[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int e = s.whole(s.e(i));
+    rx[i] = load_raw(xr + e);
+    rv[i] = load_raw(rr + e);
+  }
+  const int blocks = QUANT ? (cols + block_cols - 1) / block_cols : 0;
+  uint32_t* am = amax + (QUANT ? group * blocks : 0);
+  if constexpr (QUANT) {
+    for (int b = in_group; b < blocks; b += 32 * group_warps) am[b] = 0u;
+  }
+  float v[VPT][4];
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int e = s.e(i);
+    float a[4];
+    s.take(a, rx[i], xr, e);
+    s.take(v[i], rv[i], rr, e);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[i][k] += a[k];
+      ss = fmaf(v[i][k], v[i][k], ss);
+    }
+    if (e < cols) s.put(r + row * (int64_t)cols, e, v[i]);
+  }
+  ss = group_total(ss, scratch + group * group_warps, group, group_warps);
+  const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)cols) + eps));
+  if constexpr (!QUANT) {
+    if (in_group == 0) rstd[row] = inv;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int e = s.e(i);
+      if (e < cols) {
+        float wv[4], o[4];
+        s.weights(wv, w, e);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = v[i][k] * inv * wv[k];
+        s.put(y + row * (int64_t)cols, e, o);
+      }
+    }
+  } else if (!EDGE && block_cols == 128) {  // a scale is a warp's own affair
+    uint8_t* qr = q + row * (int64_t)cols;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int e = s.e(i);
+      float wv[4];
+      s.weights(wv, w, e);
+      uint32_t m = 0u;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[i][k] *= inv * wv[k];
+        m = max(m, __float_as_uint(fabsf(v[i][k])));
+      }
+      const float sc = quant_scale(__reduce_max_sync(0xffffffffu, e < cols ? m : 0u));
+      const float to = __fdiv_rn(1.0f, sc);
+      if (e < cols) {
+        *reinterpret_cast<uint32_t*>(qr + e) = to_e4m3x4(v[i][0] * to, v[i][1] * to, v[i][2] * to, v[i][3] * to);
+        if (lane == 0) scale[row * blocks + e / 128] = sc;
+      }
+    }
+  } else {
+    uint32_t m[VPT];
+    if (group_warps == 1) __syncwarp();
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int e = s.e(i);
+      float wv[4];
+      s.weights(wv, w, e);
+      uint32_t before = 0u;  // of the columns of the block before the warp's
+      m[i] = 0u;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[i][k] *= inv * wv[k];
+        const bool in = e + k >= 0 && e + k < cols;
+        const uint32_t u = in ? __float_as_uint(fabsf(v[i][k])) : 0u;
+        if (lane == 0 && k < s.o) before = max(before, u);
+        else m[i] = max(m[i], u);
+      }
+      m[i] = __reduce_max_sync(0xffffffffu, m[i]);
+      const int e0 = __shfl_sync(0xffffffffu, e, 0) + s.o;  // a multiple of 128
+      if (lane == 0 && e0 < cols + s.o) {
+        if (e0 < cols) atomicMax(&am[e0 / block_cols], m[i]);
+        if (s.o && e0 > 0) atomicMax(&am[(e0 - 1) / block_cols], before);
+      }
+    }
+    group_sync(group, group_warps);
+    // each block's scale once; its reciprocal takes the maximum's place
+    for (int b = in_group; b < blocks; b += 32 * group_warps) {
+      const float sc = quant_scale(am[b]);
+      scale[row * blocks + b] = sc;
+      am[b] = __float_as_uint(__fdiv_rn(1.0f, sc));
+    }
+    group_sync(group, group_warps);
+    uint8_t* qr = q + row * (int64_t)cols;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int e = s.e(i);
+      if (e >= cols) continue;
+      // at most two blocks meet in a vector
+      const int b0 = max(e, 0) / block_cols, b1 = min(e + 3, cols - 1) / block_cols;
+      const float to0 = __uint_as_float(am[b0]), to1 = __uint_as_float(am[b1]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[i][k] *= e + k < (b0 + 1) * block_cols ? to0 : to1;
+      const uint32_t o = to_e4m3x4(v[i][0], v[i][1], v[i][2], v[i][3]);
+      if (!s.partial(e)) {
+        *reinterpret_cast<uint32_t*>(qr + e) = o;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (e + k >= 0 && e + k < cols) qr[e + k] = (uint8_t)(o >> (8 * k));
+      }
+    }
+  }
+}
+
+// Persistent VJP.  Rows whose shift is equal (`period` apart) belong to one CTA, so
+// a thread's columns, and with them its dw sums, stay the same; the CTA's groups
+// are added in shared memory, in order, into its partial parts[b][cols].
+template <typename T, int VPT, int MAXT, int MODE, bool EDGE>
+__global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_bwd_rows_kernel(
+    const float* __restrict__ r, const float* __restrict__ w, const float* __restrict__ rstd,
+    const T* __restrict__ dy, int64_t dy_stride, const float* __restrict__ dr, int64_t dr_stride,
+    float* __restrict__ dres, T* __restrict__ dx, float* __restrict__ parts, int64_t rows, int cols,
+    int period, int group_warps) {
+  pdl_launch_dependents();  // the dweight finisher waits for this grid
+  __shared__ float scratch[2][32];
+  extern __shared__ __align__(16) float sums[];  // by column (several groups) or by vector
+  const int group = (threadIdx.x >> 5) / group_warps, groups = blockDim.x / (32 * group_warps);
+  const int in_group = threadIdx.x - group * group_warps * 32;
+  const int part = blockIdx.x % period;
+  const int64_t ctas = (gridDim.x - part + period - 1) / period;
+  const RowSlots<EDGE> s{cols, EDGE ? (int)(((int64_t)part * cols) & 3) : 0, in_group, group_warps * 32};
+  // the dw sums: registers, or this thread's own vectors of shared memory in wide
+  // rows (one group a CTA)
+  constexpr bool kShared = VPT >= 4;
+  float4* own_sums = reinterpret_cast<float4*>(sums) + in_group;
+  float wv[VPT][4], acc[kShared ? 1 : VPT][4];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    s.weights(wv[i], w, s.e(i));
+    if constexpr (kShared) {
+      own_sums[i * s.step] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[i][k] = 0.0f;
+    }
+  }
+  const float inv_n = __fdiv_rn(1.0f, (float)cols);
+  int parity = 0;
+  for (int64_t row = part + period * ((blockIdx.x / period) * groups + group); row < rows;
+       row += period * ctas * groups, parity ^= 1) {
+    const float* ur = r + row * (int64_t)cols;
+    const T* gr = dy + row * dy_stride;
+    const float* pr = dr ? dr + row * dr_stride : nullptr;
+    float4 ru[VPT], rd[VPT];
+    raw_t<T> rg[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int e = s.whole(s.e(i));
+      ru[i] = load_raw(ur + e);
+      rg[i] = load_raw(gr + e);
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      rd[i] = pr ? load_raw(pr + s.whole(s.e(i))) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float inv = __ldg(rstd + row);
+    float u[VPT][4], g[VPT][4];
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      s.take(u[i], ru[i], ur, s.e(i));
+      s.take(g[i], rg[i], gr, s.e(i));
+      float now[4];
+      if constexpr (kShared) raw_f32(now, own_sums[i * s.step]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        u[i][k] *= inv;
+        if constexpr (kShared) now[k] = fmaf(g[i][k], u[i][k], now[k]);
+        else acc[i][k] = fmaf(g[i][k], u[i][k], acc[i][k]);
+        g[i][k] *= wv[i][k];
+        sum = fmaf(g[i][k], u[i][k], sum);
+      }
+      if constexpr (kShared) own_sums[i * s.step] = make_float4(now[0], now[1], now[2], now[3]);
+    }
+    float mean = 0.0f;
+    if constexpr (MODE == OXC_GRAD_EXACT)
+      mean = group_total(sum, scratch[parity] + group * group_warps, group, group_warps) * inv_n;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int e = s.e(i);
+      if (e >= cols) continue;
+      float d[4];
+      if (pr) s.take(d, rd[i], pr, e);
+      else raw_f32(d, rd[i]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (MODE == OXC_GRAD_EXACT) g[i][k] = fmaf(-u[i][k], mean, g[i][k]);
+        d[k] = fmaf(inv, g[i][k], d[k]);
+      }
+      s.put(dres + row * (int64_t)cols, e, d);
+      if constexpr (sizeof(T) == 2) s.put(dx + row * (int64_t)cols, e, d);
+    }
+  }
+  float* pr = parts + (int64_t)blockIdx.x * cols;
+  if constexpr (kShared) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float now[4];
+      raw_f32(now, own_sums[i * s.step]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int c = s.e(i) + k;
+        if (c >= 0 && c < cols) pr[c] = now[k];
+      }
+    }
+    return;
+  }
+  for (int gi = 0; gi < groups; ++gi) {  // one group after the other
+    if (group == gi) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int c = s.e(i) + k;
+          if (c < 0 || c >= cols) continue;
+          const float a = gi > 0 ? sums[c] + acc[kShared ? 0 : i][k] : acc[kShared ? 0 : i][k];
+          if (gi + 1 < groups) sums[c] = a;
+          else pr[c] = a;
+        }
+    }
+    __syncthreads();
+  }
+}
+
+// ---- single elements: rows that no common shift fits --------------------------------------
+
+// One CTA per row, the row in registers: thread t holds the elements t, t +
+// blockDim, ...
 template <typename T, int VW, int VPT, int MAXT, bool QUANT>
 __global__ void __launch_bounds__(MAXT) add_rms_fwd_kernel(
     const T* __restrict__ x, int64_t x_stride, const float* __restrict__ res, int64_t res_stride,
@@ -103,11 +457,10 @@ __global__ void __launch_bounds__(MAXT) add_rms_fwd_kernel(
         const int e = (i * blockDim.x + threadIdx.x) * VW;
         if (e < cols) {
           const int b = e / block_cols;
-          const float a = __uint_as_float(amax[b]);
-          const float s = a != a ? a : fmaxf(__fdiv_rn(a, 448.0f), 1.17549435e-38f);
+          const float s = quant_scale(amax[b]), to = __fdiv_rn(1.0f, s);
           uint8_t o[VW];
 #pragma unroll
-          for (int k = 0; k < VW; ++k) o[k] = to_e4m3(__fdiv_rn(v[i][k], s));
+          for (int k = 0; k < VW; ++k) o[k] = to_e4m3(v[i][k] * to);
           uint8_t* qp = q + row * (int64_t)cols + e;
           if constexpr (VW == 4)
             *reinterpret_cast<uchar4*>(qp) = make_uchar4(o[0], o[1], o[2], o[3]);
@@ -195,11 +548,30 @@ __global__ void __launch_bounds__(MAXT) add_rms_bwd_kernel(
   }
 }
 
-static int64_t add_rms_bwd_ctas(int64_t rows) {
-  int64_t g = 2 * (int64_t)sm_count();
-  const int64_t by_rows = (rows + 7) / 8;
-  if (g > by_rows) g = by_rows;
-  return g < 1 ? 1 : g;
+// Warps per row, rows per CTA and vectors per thread, for rows of `slots` vectors:
+// `vpt` vectors a thread where 32 warps suffice, more beyond.
+struct GroupGeom {
+  int vpt, warps, groups;
+  int threads() const { return 32 * warps * groups; }
+};
+static GroupGeom group_geom(int64_t cols, int vpt) {
+  const int64_t slots = (cols + (cols % 4 ? 3 : 0) + 3) / 4;
+  while (vpt > 1 && slots <= 32 * (vpt / 2)) vpt /= 2;
+  while (slots > 32 * 32 * vpt) vpt *= 2;
+  const int warps = (int)((slots + 32 * vpt - 1) / (32 * vpt));
+  return {vpt, warps, warps >= kMaxGroups ? 1 : kMaxGroups / warps};
+}
+constexpr int kFwdVecs = 4;
+// 2 vectors a thread in the VJP: its 64 registers let 1024 threads share an SM.
+static GroupGeom bwd_geom(int64_t cols) { return group_geom(cols, 2); }
+
+// CTAs of the VJP: as many as are resident, at least 4 rows a group; 4 at least,
+// one for each shift of the rows.
+static int64_t add_rms_bwd_ctas(int64_t rows, int64_t cols) {
+  const GroupGeom g = bwd_geom(cols);
+  const int64_t per_sm = std::max(1, 1024 / g.threads());
+  const int64_t by_rows = (rows + 4 * g.groups - 1) / (4 * g.groups);
+  return std::max<int64_t>(4, std::min<int64_t>(per_sm * sm_count(), by_rows));
 }
 
 static oxc_status add_rms_check(const char* fn, int32_t dtype, int64_t rows, int64_t cols) {
@@ -216,12 +588,13 @@ static oxc_status add_rms_check(const char* fn, int32_t dtype, int64_t rows, int
   return OXC_OK;
 }
 
-// Vectors of 4 when every row of x and of the f32 tensors starts on one.
+// Whether every row of x (and of the f32 tensor f) starts where the rows of the
+// dense tensors do, relative to a multiple of 4 elements.
 template <typename T>
-static bool rows_vec4(const void* x, int64_t x_stride, const void* f, int64_t f_stride,
-                      int64_t cols) {
-  return cols % 4 == 0 && x_stride % 4 == 0 && f_stride % 4 == 0 &&
-         aligned_to(x, 4 * sizeof(T)) && aligned16(f);
+static bool row_shift(const void* x, int64_t x_stride, const void* f, int64_t f_stride,
+                      int64_t cols, int64_t rows) {
+  return cols >= 8 && aligned_to(x, 4 * sizeof(T)) && aligned16(f) &&
+         (rows == 1 || ((x_stride - cols) % 4 == 0 && (f_stride - cols) % 4 == 0));
 }
 
 template <typename T, bool QUANT>
@@ -230,19 +603,39 @@ static oxc_status add_rms_fwd_launch(const char* fn, const void* x, int64_t x_st
                                      uint8_t* q, float* scale, int block_cols, float* r,
                                      float* rstd, int64_t rows, int64_t cols, float eps,
                                      cudaStream_t s) {
-  const bool v4 = rows_vec4<T>(x, x_stride, res, res_stride, cols) && aligned16(w) &&
-                  aligned16(r) && (QUANT ? aligned_to(q, 4) : aligned_to(y, 4 * sizeof(T)));
-  RowGeom g = row_geom(cols, v4);
-  if (v4) {
-    const RowGeom d = row_geom_deep(cols);
-    if (d.ok && d.block <= 512) g = d;
+  if (row_shift<T>(x, x_stride, res, res_stride, cols, rows) && aligned16(w) && aligned16(r) &&
+      (QUANT ? aligned_to(q, 4) : aligned_to(y, 4 * sizeof(T)))) {
+    const GroupGeom g = group_geom(cols, kFwdVecs);
+    const int64_t grid = (rows + g.groups - 1) / g.groups;
+    if (grid > 0x7fffffff)
+      return fail(OXC_ERR_NOT_IMPLEMENTED, "not implemented: %s: %lld rows", fn, (long long)rows);
+#define LAUNCH(VPT, MAXT)                                                                       \
+  (cols % 4 ? add_rms_fwd_rows_kernel<T, VPT, MAXT, QUANT, true>                                \
+            : add_rms_fwd_rows_kernel<T, VPT, MAXT, QUANT, false>)<<<(unsigned)grid, g.threads(), 0, s>>>( \
+      static_cast<const T*>(x), x_stride, res, res_stride, w, static_cast<T*>(y), q, scale,     \
+      block_cols, r, rstd, rows, (int)cols, eps, g.warps)
+    if (g.vpt == 1) LAUNCH(1, 256);
+    else if (g.vpt == 2) LAUNCH(2, 256);
+    else if (g.vpt == 4 && g.threads() <= 512) LAUNCH(4, 512);
+    else if (g.vpt == 4) LAUNCH(4, 1024);
+    else LAUNCH(8, 1024);
+#undef LAUNCH
+    return check_launch(fn);
   }
+  const RowGeom g = row_geom(cols, false);
   const unsigned grid = (unsigned)std::min<int64_t>(rows, 0x7fffffff);
-#define LAUNCH(VW, VPT, MAXT)                                                                   \
-  add_rms_fwd_kernel<T, VW, VPT, MAXT, QUANT><<<grid, g.block, 0, s>>>(                         \
+#define LAUNCH(VPT)                                                                             \
+  add_rms_fwd_kernel<T, 1, VPT, 1024, QUANT><<<grid, g.block, 0, s>>>(                          \
       static_cast<const T*>(x), x_stride, res, res_stride, w, static_cast<T*>(y), q, scale,     \
       block_cols, r, rstd, rows, (int)cols, eps)
-  OXC_DISPATCH_ROW(g, LAUNCH);
+  switch (g.vpt) {
+    case 1: LAUNCH(1); break;
+    case 2: LAUNCH(2); break;
+    case 4: LAUNCH(4); break;
+    case 8: LAUNCH(8); break;
+    case 16: LAUNCH(16); break;
+    default: LAUNCH(32); break;
+  }
 #undef LAUNCH
   return check_launch(fn);
 }
@@ -253,25 +646,60 @@ static oxc_status add_rms_bwd_launch(const float* r, const float* w, const float
                                      int64_t dr_stride, float* dres, void* dx, float* dw,
                                      int64_t rows, int64_t cols, int32_t mode, float* parts,
                                      cudaStream_t s) {
-  const bool v4 = rows_vec4<T>(dy, dy_stride, dr, dr ? dr_stride : 0, cols) && aligned16(r) &&
-                  aligned16(w) && aligned16(dres) && aligned16(parts) &&
-                  (sizeof(T) == 4 || aligned_to(dx, 4 * sizeof(T)));
-  const RowGeom g = row_geom(cols, v4, 512);
-  const int64_t ctas = add_rms_bwd_ctas(rows);
-  const int64_t chunk = (rows + ctas - 1) / ctas;
-#define LAUNCH(VW, VPT, MAXT)                                                                   \
+  const int64_t ctas = add_rms_bwd_ctas(rows, cols);
+  if (row_shift<T>(dy, dy_stride, dr, dr ? dr_stride : cols, cols, rows) && aligned16(r) &&
+      aligned16(w) && aligned16(dres) && (sizeof(T) == 4 || aligned_to(dx, 4 * sizeof(T)))) {
+    const GroupGeom g = bwd_geom(cols);
+    const int period = cols % 4 == 0 ? 1 : cols % 2 == 0 ? 2 : 4;
+    const size_t smem = g.vpt >= 4      ? (size_t)g.vpt * g.threads() * sizeof(float4)
+                        : g.groups > 1 ? (size_t)cols * sizeof(float)
+                                       : 0;
+    const bool edge = cols % 4 != 0, exact = mode == OXC_GRAD_EXACT;
+#define LAUNCH(VPT, MAXT)                                                                       \
+  do {                                                                                          \
+    auto kernel = exact ? edge ? add_rms_bwd_rows_kernel<T, VPT, MAXT, OXC_GRAD_EXACT, true>    \
+                               : add_rms_bwd_rows_kernel<T, VPT, MAXT, OXC_GRAD_EXACT, false>   \
+                  : edge       ? add_rms_bwd_rows_kernel<T, VPT, MAXT, OXC_GRAD_REF, true>      \
+                               : add_rms_bwd_rows_kernel<T, VPT, MAXT, OXC_GRAD_REF, false>;    \
+    if (smem > 40 * 1024) {                                                                     \
+      const cudaError_t e = cudaFuncSetAttribute(                                               \
+          (const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);         \
+      if (e != cudaSuccess) return cuda_fail(e, "oxc_add_rms_norm_bwd");                        \
+    }                                                                                           \
+    kernel<<<(unsigned)ctas, g.threads(), smem, s>>>(                                           \
+        r, w, rstd, static_cast<const T*>(dy), dy_stride, dr, dr_stride, dres,                  \
+        static_cast<T*>(dx), parts, rows, (int)cols, period, g.warps);                          \
+  } while (0)
+    if (g.vpt == 1) LAUNCH(1, 256);
+    else if (g.vpt == 2 && g.threads() <= 512) LAUNCH(2, 512);
+    else if (g.vpt == 2) LAUNCH(2, 1024);
+    else if (g.vpt == 4) LAUNCH(4, 1024);
+    else LAUNCH(8, 1024);
+#undef LAUNCH
+  } else {
+    const RowGeom g = row_geom(cols, false, 512);
+    const int64_t chunk = (rows + ctas - 1) / ctas;
+#define LAUNCH(VPT)                                                                             \
   do {                                                                                          \
     if (mode == OXC_GRAD_REF)                                                                   \
-      add_rms_bwd_kernel<T, VW, VPT, MAXT, OXC_GRAD_REF><<<(unsigned)ctas, g.block, 0, s>>>(    \
+      add_rms_bwd_kernel<T, 1, VPT, 1024, OXC_GRAD_REF><<<(unsigned)ctas, g.block, 0, s>>>(     \
           r, w, rstd, static_cast<const T*>(dy), dy_stride, dr, dr_stride, dres,                \
           static_cast<T*>(dx), parts, rows, (int)cols, chunk);                                  \
     else                                                                                        \
-      add_rms_bwd_kernel<T, VW, VPT, MAXT, OXC_GRAD_EXACT><<<(unsigned)ctas, g.block, 0, s>>>(  \
+      add_rms_bwd_kernel<T, 1, VPT, 1024, OXC_GRAD_EXACT><<<(unsigned)ctas, g.block, 0, s>>>(   \
           r, w, rstd, static_cast<const T*>(dy), dy_stride, dr, dr_stride, dres,                \
           static_cast<T*>(dx), parts, rows, (int)cols, chunk);                                  \
   } while (0)
-  OXC_DISPATCH_ROW(g, LAUNCH);
+    switch (g.vpt) {
+      case 1: LAUNCH(1); break;
+      case 2: LAUNCH(2); break;
+      case 4: LAUNCH(4); break;
+      case 8: LAUNCH(8); break;
+      case 16: LAUNCH(16); break;
+      default: LAUNCH(32); break;
+    }
 #undef LAUNCH
+  }
   oxc_status st = check_launch("oxc_add_rms_norm_bwd");
   if (st) return st;
   launch_colsum_partials(parts, (int)ctas, cols, dw, s);
@@ -330,7 +758,7 @@ oxc_status oxc_add_rms_norm_quant(const void* x, int64_t x_stride, const float* 
 
 size_t oxc_add_rms_norm_bwd_workspace_size(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  return (size_t)add_rms_bwd_ctas(rows) * (size_t)cols * sizeof(float);
+  return (size_t)add_rms_bwd_ctas(rows, cols) * (size_t)cols * sizeof(float);
 }
 
 oxc_status oxc_add_rms_norm_bwd(const float* r, const float* w, const float* rstd, const void* dy,

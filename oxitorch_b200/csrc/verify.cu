@@ -15,6 +15,13 @@
 //
 // Each weight is one subtraction and one division in f32, correctly rounded,
 // so the choice is the same on every machine and in every order of reduction.
+//
+// Three rows of the vocabulary are read per sequence, 12 bytes an entry.  A cluster
+// of up to 8 CTAs shares a sequence, so that few sequences still use many SMs;
+// every CTA works the acceptance out for itself (a few dozen loads) and the
+// argmax's keys meet in distributed shared memory.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "common.cuh"
@@ -45,26 +52,77 @@ __device__ __forceinline__ unsigned long long warp_max_key(unsigned long long k)
   return k;
 }
 
-// One CTA per sequence.
-__global__ void __launch_bounds__(512) verify_kernel(
+constexpr int kVerifyThreads = 256;
+constexpr int kVerifyCluster = 8;
+
+// The largest key of vocabulary entries [v0, v1) in weights p - q (q may be null;
+// token x counts 0).  The rows start anywhere: vectors where their addresses agree
+// modulo 16 bytes, else single entries.
+__device__ __forceinline__ unsigned long long race_best(const float* p, const float* q,
+                                                        const float* e, int64_t x, int64_t v0,
+                                                        int64_t v1) {
+  unsigned long long k = 0ull;
+  auto one = [&](float pv, float qv, float ev, int64_t v) {
+    k = max(k, race_key(v == x ? 0.0f : __fsub_rn(pv, qv), ev, (uint32_t)v));
+  };
+  const uintptr_t o = reinterpret_cast<uintptr_t>(p + v0) & 15;
+  int64_t from = v1, to = v1;  // the part read by vectors
+  if (o == (reinterpret_cast<uintptr_t>(e + v0) & 15) &&
+      (!q || o == (reinterpret_cast<uintptr_t>(q + v0) & 15))) {
+    from = min(v1, v0 + (int64_t)((16 - o) & 15) / 4);
+    to = from + ((v1 - from) & ~(int64_t)3);
+  }
+  constexpr int U = 2;  // vectors in flight per row
+  for (int64_t v = from + 4 * threadIdx.x; v < to; v += 4 * U * kVerifyThreads) {
+    float4 pv[U], qv[U], ev[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = min(v + 4 * u * kVerifyThreads, to - 4);  // twice the last is no harm
+      pv[u] = ld_stream(reinterpret_cast<const float4*>(p + at));
+      ev[u] = ld_stream(reinterpret_cast<const float4*>(e + at));
+      qv[u] = q ? ld_stream(reinterpret_cast<const float4*>(q + at)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = min(v + 4 * u * kVerifyThreads, to - 4);
+      one(pv[u].x, qv[u].x, ev[u].x, at);
+      one(pv[u].y, qv[u].y, ev[u].y, at + 1);
+      one(pv[u].z, qv[u].z, ev[u].z, at + 2);
+      one(pv[u].w, qv[u].w, ev[u].w, at + 3);
+    }
+  }
+  // what the vectors leave: before `from` and from `to` on
+  const int64_t single = (from - v0) + (v1 - to);
+  for (int64_t i = threadIdx.x; i < (from == v1 ? v1 - v0 : single); i += kVerifyThreads) {
+    const int64_t v = i < from - v0 ? v0 + i : to + (i - (from - v0));
+    one(p[v], q ? q[v] : 0.0f, e[v], v);
+  }
+  return k;
+}
+
+// One cluster per sequence.
+__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(
     const float* __restrict__ target, int64_t t_sb, int64_t t_sk, const float* __restrict__ draft,
     int64_t d_sb, int64_t d_sk, const int64_t* __restrict__ tokens,
     const int64_t* __restrict__ lengths, const float* __restrict__ uniform,
     const float* __restrict__ race, int drafted, int64_t vocab, int64_t* __restrict__ out_tokens,
     int64_t* __restrict__ accepted, int32_t* err) {
-  __shared__ unsigned long long best[16];
+  namespace cg = cooperative_groups;
+  __shared__ unsigned long long best[kVerifyThreads / 32], mine[2];
   __shared__ int first;
-  const int64_t b = blockIdx.x;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int64_t b = blockIdx.x / size;
   const int64_t* tok = tokens + b * drafted;
-  int64_t want = lengths ? lengths[b] : drafted;
+  const int64_t want = lengths ? lengths[b] : drafted;
   const int n = (int)(want < 0 ? 0 : want > drafted ? drafted : want);
   if (threadIdx.x == 0) first = n;
   __syncthreads();
-  for (int k = threadIdx.x; k < n; k += blockDim.x) {
+  for (int k = threadIdx.x; k < n; k += kVerifyThreads) {
     const int64_t x = tok[k];
     bool keep = false;
     if (x < 0 || x >= vocab) {
-      record_bad_token(err, x, vocab);
+      if (rank == 0) record_bad_token(err, x, vocab);
     } else {
       const float p = target[b * t_sb + k * t_sk + x];
       const float q = draft ? draft[b * d_sb + k * d_sk + x] : 1.0f;
@@ -75,28 +133,36 @@ __global__ void __launch_bounds__(512) verify_kernel(
   __syncthreads();
   const int j = first;
   const float* p = target + b * t_sb + j * t_sk;
-  const float* q = j < n && draft ? draft + b * d_sb + j * d_sk : nullptr;
-  const int64_t x = j < n && !draft ? tok[j] : -1;
   const float* e = race + b * vocab;
+  // this CTA's entries: a share in multiples of 4
+  const int64_t each = ((vocab + size - 1) / size + 3) & ~(int64_t)3;
+  const int64_t v0 = min(vocab, rank * each), v1 = min(vocab, v0 + each);
   unsigned long long k = 0ull;
   for (int pass = 0; pass < 2; ++pass) {  // the second from p alone, if nothing was left
-    for (int64_t v = threadIdx.x; v < vocab; v += blockDim.x) {
-      float w = p[v];
-      if (pass == 0) w = q ? __fsub_rn(w, q[v]) : v == x ? 0.0f : w;
-      k = max(k, race_key(w, e[v], (uint32_t)v));
-    }
+    const bool beyond = pass == 0 && j < n;
+    k = race_best(p, beyond && draft ? draft + b * d_sb + j * d_sk : nullptr, e,
+                  beyond && !draft ? tok[j] : -1, v0, v1);
     k = warp_max_key(k);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) best[threadIdx.x >> 5] = k;
     __syncthreads();
     k = 0ull;
-    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) k = max(k, best[w]);
-    if (k != 0ull) break;
+    for (int w = 0; w < kVerifyThreads / 32; ++w) k = max(k, best[w]);
+    if (size > 1) {
+      if (threadIdx.x == 0) mine[pass] = k;
+      cluster.sync();
+      k = 0ull;
+      for (int r = 0; r < size; ++r) k = max(k, *cluster.map_shared_rank(&mine[pass], r));
+    }
+    if (k != 0ull || j == n) break;  // (the same in every CTA)
   }
-  const int64_t next = k ? (int64_t)(0xffffffffu - (uint32_t)k) : -1;
-  for (int i = threadIdx.x; i <= drafted; i += blockDim.x)
-    out_tokens[b * (drafted + 1) + i] = i < j ? tok[i] : i == j ? next : -1;
-  if (threadIdx.x == 0) accepted[b] = j;
+  if (rank == 0) {
+    const int64_t next = k ? (int64_t)(0xffffffffu - (uint32_t)k) : -1;
+    for (int i = threadIdx.x; i <= drafted; i += kVerifyThreads)
+      out_tokens[b * (drafted + 1) + i] = i < j ? tok[i] : i == j ? next : -1;
+    if (threadIdx.x == 0) accepted[b] = j;
+  }
+  if (size > 1) cluster.sync();  // no CTA leaves while its key is read
 }
 
 }  // namespace oxc
@@ -122,10 +188,28 @@ oxc_status oxc_verify_draft(const float* target, int64_t target_sb, int64_t targ
   if (!target || !race || !out_tokens || !accepted || (drafted > 0 && (!tokens || !uniform)))
     return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: verify_draft: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  verify_kernel<<<(unsigned)batch, 512, 0, s>>>(target, target_sb, target_sk, draft, draft_sb,
-                                                draft_sk, tokens, lengths, uniform, race,
-                                                (int)drafted, vocab, out_tokens, accepted,
-                                                err_flag);
+  // CTAs per sequence: doubled while that leaves room on the SMs (four CTAs each)
+  // and every CTA has a few thousand entries
+  int size = 1;
+  while (size < kVerifyCluster && batch * size * 2 <= 4 * (int64_t)sm_count() &&
+         vocab >= (int64_t)size * 2 * 2048)
+    size *= 2;
+  if (batch > 0x7fffffff / size) size = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(batch * size));
+  cfg.blockDim = dim3(kVerifyThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)size;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, verify_kernel, target, target_sb, target_sk, draft,
+                                           draft_sb, draft_sk, tokens, lengths, uniform, race,
+                                           (int)drafted, vocab, out_tokens, accepted, err_flag);
+  if (e != cudaSuccess) return cuda_fail(e, "oxc_verify_draft");
   return check_launch("oxc_verify_draft");
 }
 

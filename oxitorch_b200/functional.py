@@ -26,7 +26,8 @@ _MODES = {"ref": N.GRAD_REF, "exact": N.GRAD_EXACT}
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # torch.cuda.current_stream().cuda_stream without the Stream object around it
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _require_cuda_f32(name, t):
@@ -542,12 +543,13 @@ def _dtype_id(name, t):
     if not t.is_cuda:
         raise ValueError(f"invalid argument: {name} must live on a CUDA device "
                          "(oxitorch_b200 has no CPU path)")
-    if t.get_device() != torch.cuda.current_device():
+    if t.get_device() != torch._C._cuda_getDevice():
         raise ValueError(f"invalid argument: {name} lives on {t.device}, the current device is "
                          f"cuda:{torch.cuda.current_device()}")
-    if t.dtype not in _DTYPES:
+    dt = _DTYPES.get(t.dtype)
+    if dt is None:
         raise ValueError(f"invalid argument: {name} must be float32 or bfloat16, got {t.dtype}")
-    return _DTYPES[t.dtype]
+    return dt
 
 
 def _operand(name, t, shape, dtype, device):
@@ -558,7 +560,7 @@ def _operand(name, t, shape, dtype, device):
         raise ValueError(f"invalid argument: {name} must live on {device}, got {t.device}")
     if t.dtype != dtype:
         raise ValueError(f"invalid argument: {name} must be {str(dtype)[6:]}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"shape mismatch: {name} {list(t.shape)} vs {list(shape)}")
 
 
@@ -856,11 +858,11 @@ class _DistillLoss(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        logits, teacher_logits, teacher_ids = ctx.saved_tensors
-        g = g.reshape(1).to(torch.float32).contiguous()
+        if g.dtype != torch.float32:
+            g = g.to(torch.float32)
         d, ctx.dlogits = ctx.dlogits, None
         if d is None:
-            d = distill_loss_fwd(logits, teacher_logits, teacher_ids, *ctx.args, grad_loss=g)[1]
+            d = distill_loss_fwd(*ctx.saved_tensors, *ctx.args, grad_loss=g)[1]
         else:
             N.check(N.load().oxc_scale_by(d.data_ptr(), d.numel(), _DTYPES[d.dtype], g.data_ptr(),
                                           _stream()), "distill_loss backward")
