@@ -46,8 +46,7 @@ constexpr int kScanWarps = 8;
 constexpr int kScanSteps = 8;                        // tokens per warp
 constexpr int kScanChunk = kScanWarps * kScanSteps;  // tokens per CTA
 constexpr int kScanGroup = 8;                        // chunks per group
-constexpr int kScanFwdCtas = 2;                      // resident per SM
-constexpr int kScanBwdCtas = 2;
+constexpr int kScanCtas = 2;                         // resident per SM
 
 // A [batch, length, dim] operand: the last dim dense, strides in elements.
 template <typename T>
@@ -684,8 +683,9 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
     lane.put(mapM[warp], M);
     __syncthreads();
     // the mu of the chunk after this one (two sets of threads) and the state before
-    // it (a third)
+    // it (a third, or the second first)
     const int c = threadIdx.x % L::kChannels, part = threadIdx.x / L::kChannels;
+    constexpr int kStatePart = kScanWarps * 32 >= 3 * L::kChannels ? 2 : 1;
     const bool mine = tile.d0 + c < dim;
     const int64_t off = tile.b * dim + tile.d0 + c;
     const int k = chunks - 1 - tile.chunk;
@@ -693,13 +693,14 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
       float tA, tM;
       map_compose_column<kScanWarps, true>(&mapA[0][c], &mapM[0][c], L::kChannels, tA, tM);
       chain_maps(chain, k, chunks, off, tA, tM, before, c);
-    } else if (mine && part == 1) {
-      const float m = dlast ? dlast[off] : 0.0f;
-      enter[c] = chunks > 1 ? chain_enter(chain, k, chunks, off, m) : m;
-    } else if (mine && part == 2) {
+    }
+    if (mine && part == kStatePart)
       map_arguments_column<kScanWarps, false>(
           &mapA[0][c], &mapS[0][c], L::kChannels,
           carry[((int64_t)tile.b * chunks + tile.chunk) * dim + tile.d0 + c]);
+    if (mine && part == 1) {
+      const float m = dlast ? dlast[off] : 0.0f;
+      enter[c] = chunks > 1 ? chain_enter(chain, k, chunks, off, m) : m;
     }
     __syncthreads();
     if (mine && part == 0) {
@@ -835,8 +836,8 @@ static oxc_status scan_fwd_launch(const void* x, int64_t x_sb, int64_t x_st, con
                                   cudaStream_t s) {
   const bool vec = seq_vec<T, VW>(x, x_sb, x_st, dim) && seq_vec<T, VW>(gate, g_sb, g_st, dim) &&
                    seq_vec<T, VW>(h, 0, 0, dim);
-  auto kernel = vec ? scan_fwd_kernel<T, VW, true, kScanFwdCtas>
-                    : scan_fwd_kernel<T, VW, false, kScanFwdCtas>;
+  auto kernel = vec ? scan_fwd_kernel<T, VW, true, kScanCtas>
+                    : scan_fwd_kernel<T, VW, false, kScanCtas>;
   int64_t dtiles;
   unsigned tiles, grid;
   oxc_status st = scan_grid("gated_scan", (const void*)kernel, batch, length, dim, 32 * VW, &dtiles,
@@ -860,8 +861,8 @@ static oxc_status scan_bwd_launch(const void* x, int64_t x_sb, int64_t x_st, con
   const bool vec = seq_vec<T, VW>(x, x_sb, x_st, dim) && seq_vec<T, VW>(gate, g_sb, g_st, dim) &&
                    seq_vec<T, VW>(dh, dh_sb, dh_st, dim) && seq_vec<T, VW>(dx, 0, 0, dim) &&
                    seq_vec<T, VW>(dgate, 0, 0, dim);
-  auto kernel = vec ? scan_bwd_kernel<T, VW, true, kScanBwdCtas>
-                    : scan_bwd_kernel<T, VW, false, kScanBwdCtas>;
+  auto kernel = vec ? scan_bwd_kernel<T, VW, true, kScanCtas>
+                    : scan_bwd_kernel<T, VW, false, kScanCtas>;
   int64_t dtiles;
   unsigned tiles, grid;
   oxc_status st = scan_grid("gated_scan backward", (const void*)kernel, batch, length, dim, 32 * VW,
@@ -917,11 +918,11 @@ oxc_status oxc_gated_scan_fwd(const void* x, int64_t x_sb, int64_t x_st, const v
   Chain chain;
   st = scan_chain("gated_scan", batch, length, dim, workspace, workspace_bytes, s, &chain);
   if (st) return st;
-  if (dtype == OXC_BF16)
-    return scan_fwd_launch<bf16, 4>(x, x_sb, x_st, gate, g_sb, g_st, starts, h0, h, last, carry,
-                                 chain, batch, length, dim, s);
-  return scan_fwd_launch<float, 4>(x, x_sb, x_st, gate, g_sb, g_st, starts, h0, h, last, carry, chain,
-                                batch, length, dim, s);
+  // 4 channels a thread, half as many where a tile would be wider than the tensor
+  auto launch = dtype == OXC_BF16 ? (dim <= 64 ? scan_fwd_launch<bf16, 2> : scan_fwd_launch<bf16, 4>)
+                                  : (dim <= 64 ? scan_fwd_launch<float, 2> : scan_fwd_launch<float, 4>);
+  return launch(x, x_sb, x_st, gate, g_sb, g_st, starts, h0, h, last, carry, chain, batch, length,
+                dim, s);
 }
 
 oxc_status oxc_gated_scan_bwd(const void* x, int64_t x_sb, int64_t x_st, const void* gate,
@@ -946,11 +947,16 @@ oxc_status oxc_gated_scan_bwd(const void* x, int64_t x_sb, int64_t x_st, const v
   Chain chain;
   st = scan_chain("gated_scan backward", batch, length, dim, workspace, workspace_bytes, s, &chain);
   if (st) return st;
-  if (dtype == OXC_BF16)
-    return scan_bwd_launch<bf16, 2>(x, x_sb, x_st, gate, g_sb, g_st, starts, carry, dh, dh_sb, dh_st,
-                                 dlast, dx, dgate, dh0, chain, batch, length, dim, s);
-  return scan_bwd_launch<float, 2>(x, x_sb, x_st, gate, g_sb, g_st, starts, carry, dh, dh_sb, dh_st,
-                                dlast, dx, dgate, dh0, chain, batch, length, dim, s);
+  // 2 channels a thread; 4 where bf16 is read by vectors, which then cost half the
+  // instructions (94 us instead of 117 at [4, 2048, 4096]; f32 needs the registers,
+  // 141 us against 150)
+  const bool wide = dtype == OXC_BF16 && dim > 64 && seq_vec<bf16, 4>(x, x_sb, x_st, dim) &&
+                    seq_vec<bf16, 4>(gate, g_sb, g_st, dim) && seq_vec<bf16, 4>(dh, dh_sb, dh_st, dim) &&
+                    seq_vec<bf16, 4>(dx, 0, 0, dim) && seq_vec<bf16, 4>(dgate, 0, 0, dim);
+  auto launch = dtype == OXC_BF16 ? (wide ? scan_bwd_launch<bf16, 4> : scan_bwd_launch<bf16, 2>)
+                                  : scan_bwd_launch<float, 2>;
+  return launch(x, x_sb, x_st, gate, g_sb, g_st, starts, carry, dh, dh_sb, dh_st, dlast, dx, dgate,
+                dh0, chain, batch, length, dim, s);
 }
 
 oxc_status oxc_gated_step(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,
