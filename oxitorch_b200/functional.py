@@ -616,16 +616,21 @@ def add_rms_norm_fwd(x, residual, weight, eps=1e-6):
 def add_rms_norm_bwd(r, weight, rstd, dy, dr=None, grad_mode="ref"):
     """Returns (dx, dresidual, dweight) for dy (the type of y) and dr (float32,
     None = zero); in float32 dx and dresidual are one tensor."""
-    dt = _dtype_id("dy", dy)
+    _dtype_id("dy", dy)
     _operand("r", r, dy.shape, torch.float32, dy.device)
-    r, dy2, w = dense(r), _rows2d(dy), dense(weight)
-    rows, cols = dy2.shape
     if dr is not None:
         _operand("dr", dr, r.shape, torch.float32, r.device)
+    return _add_rms_norm_bwd(dense(r), dense(weight), rstd, dy, dr, grad_mode)
+
+
+def _add_rms_norm_bwd(r, w, rstd, dy, dr, grad_mode):
+    dt, dy2 = _DTYPES[dy.dtype], _rows2d(dy)
+    rows, cols = dy2.shape
+    if dr is not None:
         dr = _rows2d(dr)
     dres = torch.empty_like(r)
     dx = dres if dt == N.F32 else torch.empty(r.shape, dtype=dy.dtype, device=r.device)
-    dw = torch.empty(cols, dtype=torch.float32, device=r.device)
+    dw = torch.empty_like(w)
     L = N.load()
     ws = _workspace(L.oxc_add_rms_norm_bwd_workspace_size(rows, cols), r.device)
     N.check(L.oxc_add_rms_norm_bwd(
@@ -652,8 +657,7 @@ class _AddRMSNorm(torch.autograd.Function):
             if dr is None:
                 return None, None, None, None, None
             return dr.to(ctx.dtype), dr, torch.zeros_like(weight), None, None
-        dx, dres, dw = add_rms_norm_bwd(r, weight, rstd, dy, dr, ctx.grad_mode)
-        return dx, dres, dw, None, None
+        return *_add_rms_norm_bwd(r, dense(weight), rstd, dy, dr, ctx.grad_mode), None, None
 
 
 def add_rms_norm(x, residual, weight, eps=1e-6, grad_mode="ref"):
@@ -899,8 +903,9 @@ def verify_draft(target, draft, tokens, uniform, race, lengths=None, flag=None):
     None) count.  Token k is kept while uniform[b, k] * q < p.  out[b] holds the
     accepted[b] kept tokens, then the token sampled after them as the first
     argmax of max(p - q, 0) / race[b] (p / race[b] when all were kept or nothing
-    is left), then -1.  uniform [batch, drafted] is in [0, 1), race [batch,
-    vocab] holds exponential variates.  Tokens outside the vocabulary are not
+    is left), then -1.  uniform [batch, drafted] is in [0, 1); race [batch,
+    vocab] holds exponential variates, which are positive (a zero would win its
+    race whatever its weight).  Tokens outside the vocabulary are not
     kept, and recorded in ``flag`` (int32[4], zeroed by the caller) if given."""
     _require_cuda_f32("target", target)
     _dtype_id("target", target)
