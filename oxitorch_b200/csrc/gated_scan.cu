@@ -461,6 +461,12 @@ __device__ __forceinline__ unsigned int start_bits(const uint8_t* starts, int64_
   return __ballot_sync(0xffffffffu, s);
 }
 
+// N pairs of a thread in shared memory.
+template <int N>
+struct __align__(8 * N > 16 ? 16 : 8 * N) Held {
+  float2 v[N];
+};
+
 // Runs f(std::true_type) if any of the warp's tokens starts a sequence, else
 // f(std::false_type), whose loops need no selects.
 template <typename F>
@@ -469,25 +475,31 @@ __device__ __forceinline__ void by_fresh(unsigned int fresh, F f) {
   else f(std::false_type{});
 }
 
+// A tile is one chunk, or two (HALVES): then the gates and values of the first
+// half wait in shared memory and those of the second in registers, and the chain,
+// whose waits a long sequence of few channels mostly consists of, is entered half
+// as often.
 // Tokens beyond the length are given an infinite gate and x = 0: a = 1, b = 0,
 // the identity.  Only their loads and stores are left out.
-template <typename T, int VW, bool VEC, int CTAS>
-__global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_fwd_kernel(
+template <typename T, int VW, bool VEC, int HALVES>
+__global__ void __launch_bounds__(kScanWarps * 32, kScanCtas) scan_fwd_kernel(
     SeqView<T> x, SeqView<T> gate, const uint8_t* __restrict__ starts,
     const float* __restrict__ h0, T* __restrict__ h, float* __restrict__ last,
     float* __restrict__ carry, Chain chain, int64_t batch, int64_t length, int64_t dim,
-    int chunks, unsigned int dtiles,
-    unsigned int tiles) {
+    int tiles_long, unsigned int dtiles, unsigned int tiles) {
   using L = Lane<T, VW, VEC>;
   using R = Raw<T, VW, VEC>;
-  constexpr int P = VW / 2;
-  __shared__ __align__(16) float mapA[kScanWarps][L::kChannels];
-  __shared__ __align__(16) float mapH[kScanWarps][L::kChannels];
+  constexpr int P = VW / 2, kMaps = HALVES * kScanWarps;
+  __shared__ __align__(16) float mapA[kMaps][L::kChannels];
+  __shared__ __align__(16) float mapH[kMaps][L::kChannels];
   __shared__ float2 before[kScanGroup - 1][L::kChannels];
   __shared__ float enter[L::kChannels];
   __shared__ __align__(16) Tile next;
+  extern __shared__ __align__(16) unsigned char held_bytes[];
+  auto* held = reinterpret_cast<Held<2 * P>*>(held_bytes) + threadIdx.x;
   Tiles order{&next, blockIdx.x, dtiles, (unsigned int)batch * dtiles, tiles, L::kChannels};
   const int warp = threadIdx.x >> 5;
+  const int64_t chunks = (length + kScanChunk - 1) / kScanChunk;
   if (chain.ticket) order.draw(chain, 0u);
   order.post();
   for (;;) {
@@ -495,15 +507,18 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_fwd_kernel(
     const Tile tile = next;
     if (tile.rank < 0) return;
     const L lane(tile.d0, dim);
-    const int64_t t0 = (int64_t)tile.chunk * kScanChunk + warp * kScanSteps;
-    const int64_t row0 = tile.b * length + t0;
-    const int steps = (int)max((int64_t)0, min((int64_t)kScanSteps, length - t0));
-    R rg[kScanSteps], rx[kScanSteps];
-    {
+    float2 a[kScanSteps][P], v[kScanSteps][P];
+    unsigned int fresh[HALVES];
+    int steps[HALVES];
+    const int64_t tile_t0 = (int64_t)tile.chunk * (HALVES * kScanChunk) + warp * kScanSteps;
+#pragma unroll
+    for (int half = 0; half < HALVES; ++half) {
+      const int64_t t0 = tile_t0 + half * kScanChunk;
+      steps[half] = (int)max((int64_t)0, min((int64_t)kScanSteps, length - t0));
+      R rg[kScanSteps], rx[kScanSteps];
       const T* pg = gate.p + (int64_t)tile.b * gate.sb + t0 * gate.st + lane.d;
-      const T* px = x.p + tile.b * x.sb + t0 * x.st + lane.d;
-      const bool whole = steps == kScanSteps && tile.d0 + L::kChannels <= dim;
-      if (whole) {
+      const T* px = x.p + (int64_t)tile.b * x.sb + t0 * x.st + lane.d;
+      if (steps[half] == kScanSteps && tile.d0 + L::kChannels <= dim) {
 #pragma unroll
         for (int i = 0; i < kScanSteps; ++i) {
           rg[i].load(pg);
@@ -514,79 +529,103 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_fwd_kernel(
       } else {
 #pragma unroll
         for (int i = 0; i < kScanSteps; ++i) {
-          const int live = i < steps ? lane.live : 0;
+          const int live = i < steps[half] ? lane.live : 0;
           rg[i].load_some(pg, live, INFINITY);
           rx[i].load_some(px, live, 0.0f);
           pg += gate.st;
           px += x.st;
         }
       }
-    }
-    const unsigned int fresh = start_bits(starts, tile.b, t0, length);
-    float2 a[kScanSteps][P], v[kScanSteps][P], A[P], H[P];
+      fresh[half] = start_bits(starts, tile.b, t0, length);
+      float2 A[P], H[P];
 #pragma unroll
-    for (int j = 0; j < P; ++j) { A[j] = f2(1.0f); H[j] = f2(0.0f); }
-#pragma unroll
-    for (int i = 0; i < kScanSteps; ++i)
-#pragma unroll
-      for (int j = 0; j < P; ++j) {
-        float2 b;
-        gate_pair(rg[i].pair(j), a[i][j], b);
-        v[i][j] = __fmul2_rn(b, rx[i].pair(j));
-      }
-    by_fresh(fresh, [&](auto some) {
+      for (int k = 0; k < P; ++k) { A[k] = f2(1.0f); H[k] = f2(0.0f); }
 #pragma unroll
       for (int i = 0; i < kScanSteps; ++i)
 #pragma unroll
-        for (int j = 0; j < P; ++j) {
-          H[j] = __ffma2_rn(a[i][j], H[j], v[i][j]);
-          A[j] = __fmul2_rn(A[j], a[i][j]);
-          if (decltype(some)::value && ((fresh >> i) & 1u)) { H[j] = v[i][j]; A[j] = f2(-0.0f); }
+        for (int k = 0; k < P; ++k) {
+          float2 b;
+          gate_pair(rg[i].pair(k), a[i][k], b);
+          v[i][k] = __fmul2_rn(b, rx[i].pair(k));
         }
-    });
-    lane.put(mapA[warp], A);
-    lane.put(mapH[warp], H);
+      by_fresh(fresh[half], [&](auto some) {
+#pragma unroll
+        for (int i = 0; i < kScanSteps; ++i)
+#pragma unroll
+          for (int k = 0; k < P; ++k) {
+            H[k] = __ffma2_rn(a[i][k], H[k], v[i][k]);
+            A[k] = __fmul2_rn(A[k], a[i][k]);
+            if (decltype(some)::value && ((fresh[half] >> i) & 1u)) { H[k] = v[i][k]; A[k] = f2(-0.0f); }
+          }
+      });
+      lane.put(mapA[half * kScanWarps + warp], A);
+      lane.put(mapH[half * kScanWarps + warp], H);
+      if (half + 1 < HALVES) {
+#pragma unroll
+        for (int i = 0; i < kScanSteps; ++i) {
+          Held<2 * P> keep;
+#pragma unroll
+          for (int k = 0; k < P; ++k) { keep.v[k] = a[i][k]; keep.v[P + k] = v[i][k]; }
+          held[i * kScanWarps * 32] = keep;
+        }
+      }
+    }
     __syncthreads();
     const int c = threadIdx.x % L::kChannels, part = threadIdx.x / L::kChannels;
     const bool mine = tile.d0 + c < dim;
     const int64_t off = tile.b * dim + tile.d0 + c;
-    if (mine && part == 0 && chunks > 1) {
+    if (mine && part == 0 && tiles_long > 1) {
       float tA, tH;
-      map_compose_column<kScanWarps, false>(&mapA[0][c], &mapH[0][c], L::kChannels, tA, tH);
-      chain_maps(chain, tile.chunk, chunks, off, tA, tH, before, c);
+      map_compose_column<kMaps, false>(&mapA[0][c], &mapH[0][c], L::kChannels, tA, tH);
+      chain_maps(chain, tile.chunk, tiles_long, off, tA, tH, before, c);
     } else if (mine && part == 1) {
       const float s = h0 ? h0[off] : 0.0f;
-      enter[c] = chunks > 1 ? chain_enter(chain, tile.chunk, chunks, off, s) : s;
+      enter[c] = tiles_long > 1 ? chain_enter(chain, tile.chunk, tiles_long, off, s) : s;
     }
     __syncthreads();
     if (mine && part == 0) {
       const float s = chain_state(tile.chunk, before, c, enter[c]);
-      if (carry) carry[((int64_t)tile.b * chunks + tile.chunk) * dim + tile.d0 + c] = s;
       // mapH becomes the state entering each warp
-      map_arguments_column<kScanWarps, false>(&mapA[0][c], &mapH[0][c], L::kChannels, s);
+      map_arguments_column<kMaps, false>(&mapA[0][c], &mapH[0][c], L::kChannels, s);
+      if (carry) {
+#pragma unroll
+        for (int half = 0; half < HALVES; ++half) {
+          const int64_t k = (int64_t)tile.chunk * HALVES + half;
+          if (k < chunks)
+            carry[((int64_t)tile.b * chunks + k) * dim + tile.d0 + c] = mapH[half * kScanWarps][c];
+        }
+      }
     }
     __syncthreads();
     order.draw(chain, tile.rank);
-    float2 s[P];
-    lane.get(mapH[warp], s);
-    by_fresh(fresh, [&](auto some) {
-      T* ph = h + row0 * dim;
 #pragma unroll
-      for (int i = 0; i < kScanSteps; ++i) {
+    for (int half = 0; half < HALVES; ++half) {
+      const int64_t t0 = tile_t0 + half * kScanChunk;
+      float2 s[P];
+      lane.get(mapH[half * kScanWarps + warp], s);
+      by_fresh(fresh[half], [&](auto some) {
+        T* ph = h + (tile.b * length + t0) * dim;
 #pragma unroll
-        for (int j = 0; j < P; ++j) {
-          s[j] = __ffma2_rn(a[i][j], s[j], v[i][j]);
-          if (decltype(some)::value && ((fresh >> i) & 1u)) s[j] = v[i][j];
+        for (int i = 0; i < kScanSteps; ++i) {
+          Held<2 * P> kept;
+          if (half + 1 < HALVES) kept = held[i * kScanWarps * 32];
+#pragma unroll
+          for (int k = 0; k < P; ++k) {
+            const float2 ai = half + 1 < HALVES ? kept.v[k] : a[i][k];
+            const float2 vi = half + 1 < HALVES ? kept.v[P + k] : v[i][k];
+            s[k] = __ffma2_rn(ai, s[k], vi);
+            if (decltype(some)::value && ((fresh[half] >> i) & 1u)) s[k] = vi;
+          }
+          if (i < steps[half]) lane.store(ph, s);
+          ph += dim;
         }
-        if (i < steps) lane.store(ph, s);
-        ph += dim;
-      }
-    });
-    if (last && steps > 0 && t0 + steps == length) {
+      });
+      if (last && steps[half] > 0 && t0 + steps[half] == length) {
 #pragma unroll
-      for (int k = 0; k < VW; ++k)
-        if (k < lane.live)
-          last[tile.b * dim + tile.d0 + lane.channel(k)] = k & 1 ? s[k / 2].y : s[k / 2].x;
+        for (int k = 0; k < VW; ++k)
+          if (k < lane.live)
+            last[tile.b * dim + tile.d0 + lane.channel(k)] = k & 1 ? s[k / 2].y : s[k / 2].x;
+      }
     }
     order.post();
   }
@@ -790,19 +829,22 @@ static int64_t scan_groups(int64_t length) {
 }
 
 // Lays the chain out in the workspace and empties it; a single chunk has none.
-static oxc_status scan_chain(const char* fn, int64_t batch, int64_t length, int64_t dim,
+static oxc_status scan_chain(const char* fn, int64_t batch, int64_t length, int64_t dim, int halves,
                              void* workspace, size_t workspace_bytes, cudaStream_t s, Chain* c) {
-  const size_t need = oxc_gated_scan_workspace_size(batch, length, dim);
+  const size_t size = oxc_gated_scan_workspace_size(batch, length, dim);
+  const int64_t tiles = (scan_chunks(length) + halves - 1) / halves;
+  const int64_t groups = (tiles + kScanGroup - 1) / kScanGroup;
   *c = Chain{nullptr, nullptr, nullptr, nullptr, batch * dim};
-  if (need == 0) return OXC_OK;
-  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+  if (size && (!workspace || workspace_bytes < size || !aligned16(workspace)))
     return fail(OXC_ERR_INVALID_ARGUMENT,
                 "invalid argument: %s needs a 16-byte aligned %zu-byte workspace, got %zu", fn,
-                need, workspace_bytes);
+                size, workspace_bytes);
+  if (tiles == 1) return OXC_OK;
+  const size_t need = 16 + (size_t)((tiles + 2 * groups) * c->stride) * sizeof(unsigned long long);
   c->ticket = static_cast<unsigned int*>(workspace);
   c->map = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + 16);
-  c->group = c->map + scan_chunks(length) * c->stride;
-  c->enter = c->group + scan_groups(length) * c->stride;
+  c->group = c->map + tiles * c->stride;
+  c->enter = c->group + groups * c->stride;
   const cudaError_t e = cudaMemsetAsync(workspace, 0xff, need, s);
   return e == cudaSuccess ? OXC_OK : cuda_fail(e, fn);
 }
@@ -813,41 +855,46 @@ static bool seq_vec(const void* p, int64_t sb, int64_t st, int64_t dim) {
   return dim % VW == 0 && sb % VW == 0 && st % VW == 0 && aligned_to(p, VW * sizeof(T));
 }
 
-// The number of tiles, and a grid that is resident at once.
-static oxc_status scan_grid(const char* fn, const void* kernel, int64_t batch, int64_t length,
-                            int64_t dim, int channels, int64_t* dtiles, unsigned* tiles,
-                            unsigned* grid) {
-  *dtiles = (dim + channels - 1) / channels;
-  const int64_t per = batch * *dtiles;
-  if (scan_chunks(length) > 0x7fffffff / per)
-    return fail(OXC_ERR_NOT_IMPLEMENTED, "not implemented: %s: [%lld, %lld, %lld]", fn,
-                (long long)batch, (long long)length, (long long)dim);
-  *tiles = (unsigned)(scan_chunks(length) * per);
-  const unsigned resident = (unsigned)(sm_count() * occupancy(kernel, kScanWarps * 32, 0));
-  *grid = std::min(*tiles, resident);
-  return OXC_OK;
+// Tiles of the tensor with `halves` chunks each, or -1 if they cannot be counted.
+static int64_t scan_tiles(int64_t batch, int64_t length, int64_t dim, int channels, int halves) {
+  const int64_t per = batch * ((dim + channels - 1) / channels);
+  const int64_t along = (scan_chunks(length) + halves - 1) / halves;
+  return along > 0x7fffffff / per ? -1 : along * per;
 }
 
-template <typename T, int VW>
+// A grid that is resident at once.
+static unsigned scan_grid(const void* kernel, int64_t tiles, size_t smem) {
+  return (unsigned)std::min<int64_t>(tiles, (int64_t)sm_count() * occupancy(kernel, kScanWarps * 32, smem));
+}
+
+template <typename T, int VW, int HALVES>
 static oxc_status scan_fwd_launch(const void* x, int64_t x_sb, int64_t x_st, const void* gate,
                                   int64_t g_sb, int64_t g_st, const uint8_t* starts,
                                   const float* h0, void* h, float* last, float* carry,
-                                  const Chain& chain, int64_t batch, int64_t length, int64_t dim,
-                                  cudaStream_t s) {
+                                  int64_t batch, int64_t length, int64_t dim, void* workspace,
+                                  size_t workspace_bytes, cudaStream_t s) {
+  const int64_t tiles = scan_tiles(batch, length, dim, 32 * VW, HALVES);
+  if (tiles < 0)
+    return fail(OXC_ERR_NOT_IMPLEMENTED, "not implemented: gated_scan: [%lld, %lld, %lld]",
+                (long long)batch, (long long)length, (long long)dim);
+  Chain chain;
+  oxc_status st = scan_chain("gated_scan", batch, length, dim, HALVES, workspace, workspace_bytes,
+                             s, &chain);
+  if (st) return st;
   const bool vec = seq_vec<T, VW>(x, x_sb, x_st, dim) && seq_vec<T, VW>(gate, g_sb, g_st, dim) &&
                    seq_vec<T, VW>(h, 0, 0, dim);
-  auto kernel = vec ? scan_fwd_kernel<T, VW, true, kScanCtas>
-                    : scan_fwd_kernel<T, VW, false, kScanCtas>;
-  int64_t dtiles;
-  unsigned tiles, grid;
-  oxc_status st = scan_grid("gated_scan", (const void*)kernel, batch, length, dim, 32 * VW, &dtiles,
-                            &tiles, &grid);
-  if (st) return st;
+  auto kernel = vec ? scan_fwd_kernel<T, VW, true, HALVES> : scan_fwd_kernel<T, VW, false, HALVES>;
+  const size_t smem = (HALVES - 1) * (size_t)kScanSteps * kScanWarps * 32 * 2 * VW * sizeof(float);
+  if (smem) {
+    const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return cuda_fail(e, "oxc_gated_scan_fwd");
+  }
+  const int64_t dtiles = (dim + 32 * VW - 1) / (32 * VW);
   const SeqView<T> xv{static_cast<const T*>(x), x_sb, x_st};
   const SeqView<T> gv{static_cast<const T*>(gate), g_sb, g_st};
-  kernel<<<grid, kScanWarps * 32, 0, s>>>(xv, gv, starts, h0, static_cast<T*>(h), last, carry,
-                                          chain, batch, length, dim, (int)scan_chunks(length),
-                                          (unsigned)dtiles, tiles);
+  kernel<<<scan_grid((const void*)kernel, tiles, smem), kScanWarps * 32, smem, s>>>(
+      xv, gv, starts, h0, static_cast<T*>(h), last, carry, chain, batch, length, dim,
+      (int)(tiles / (batch * dtiles)), (unsigned)dtiles, (unsigned)tiles);
   return check_launch("oxc_gated_scan_fwd");
 }
 
@@ -856,25 +903,27 @@ static oxc_status scan_bwd_launch(const void* x, int64_t x_sb, int64_t x_st, con
                                   int64_t g_sb, int64_t g_st, const uint8_t* starts,
                                   const float* carry, const void* dh, int64_t dh_sb, int64_t dh_st,
                                   const float* dlast, void* dx, void* dgate, float* dh0,
-                                  const Chain& chain, int64_t batch, int64_t length, int64_t dim,
-                                  cudaStream_t s) {
+                                  int64_t batch, int64_t length, int64_t dim, void* workspace,
+                                  size_t workspace_bytes, cudaStream_t s) {
+  const int64_t tiles = scan_tiles(batch, length, dim, 32 * VW, 1);
+  if (tiles < 0)
+    return fail(OXC_ERR_NOT_IMPLEMENTED, "not implemented: gated_scan backward: [%lld, %lld, %lld]",
+                (long long)batch, (long long)length, (long long)dim);
+  Chain chain;
+  oxc_status st = scan_chain("gated_scan backward", batch, length, dim, 1, workspace,
+                             workspace_bytes, s, &chain);
+  if (st) return st;
   const bool vec = seq_vec<T, VW>(x, x_sb, x_st, dim) && seq_vec<T, VW>(gate, g_sb, g_st, dim) &&
                    seq_vec<T, VW>(dh, dh_sb, dh_st, dim) && seq_vec<T, VW>(dx, 0, 0, dim) &&
                    seq_vec<T, VW>(dgate, 0, 0, dim);
-  auto kernel = vec ? scan_bwd_kernel<T, VW, true, kScanCtas>
-                    : scan_bwd_kernel<T, VW, false, kScanCtas>;
-  int64_t dtiles;
-  unsigned tiles, grid;
-  oxc_status st = scan_grid("gated_scan backward", (const void*)kernel, batch, length, dim, 32 * VW,
-                            &dtiles, &tiles, &grid);
-  if (st) return st;
+  auto kernel = vec ? scan_bwd_kernel<T, VW, true, kScanCtas> : scan_bwd_kernel<T, VW, false, kScanCtas>;
+  const int64_t dtiles = (dim + 32 * VW - 1) / (32 * VW);
   const SeqView<T> xv{static_cast<const T*>(x), x_sb, x_st};
   const SeqView<T> gv{static_cast<const T*>(gate), g_sb, g_st};
   const SeqView<T> dv{static_cast<const T*>(dh), dh_sb, dh_st};
-  kernel<<<grid, kScanWarps * 32, 0, s>>>(xv, gv, starts, carry, dv, dlast, static_cast<T*>(dx),
-                                          static_cast<T*>(dgate), dh0, chain, batch, length, dim,
-                                          (int)scan_chunks(length),
-                                          (unsigned)dtiles, tiles);
+  kernel<<<scan_grid((const void*)kernel, tiles, 0), kScanWarps * 32, 0, s>>>(
+      xv, gv, starts, carry, dv, dlast, static_cast<T*>(dx), static_cast<T*>(dgate), dh0, chain,
+      batch, length, dim, (int)(tiles / (batch * dtiles)), (unsigned)dtiles, (unsigned)tiles);
   return check_launch("oxc_gated_scan_bwd");
 }
 
@@ -915,14 +964,21 @@ oxc_status oxc_gated_scan_fwd(const void* x, int64_t x_sb, int64_t x_st, const v
   }
   if (!x || !gate || !h)
     return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: gated_scan: null pointer");
-  Chain chain;
-  st = scan_chain("gated_scan", batch, length, dim, workspace, workspace_bytes, s, &chain);
-  if (st) return st;
-  // 4 channels a thread, half as many where a tile would be wider than the tensor
-  auto launch = dtype == OXC_BF16 ? (dim <= 64 ? scan_fwd_launch<bf16, 2> : scan_fwd_launch<bf16, 4>)
-                                  : (dim <= 64 ? scan_fwd_launch<float, 2> : scan_fwd_launch<float, 4>);
-  return launch(x, x_sb, x_st, gate, g_sb, g_st, starts, h0, h, last, carry, chain, batch, length,
-                dim, s);
+  // 4 channels a thread, half as many where a tile would be wider than the tensor.
+  // Tiles of two chunks where few channels leave many chunks of one chain in flight
+  // (bf16 [1, 65537, 1024]: 144 us instead of 163; with 128 tiles side by side, f32
+  // [4, 2048, 4096], 97 against 80), if there are several tiles for each CTA.
+  const bool narrow = dim <= 64;
+  const int channels = narrow ? 64 : 128;
+  const bool two = batch * ((dim + channels - 1) / channels) * 8 <= sm_count() &&
+                   scan_tiles(batch, length, dim, channels, 2) >= 4 * (int64_t)sm_count();
+  auto launch = dtype == OXC_BF16
+                    ? (narrow ? (two ? scan_fwd_launch<bf16, 2, 2> : scan_fwd_launch<bf16, 2, 1>)
+                              : (two ? scan_fwd_launch<bf16, 4, 2> : scan_fwd_launch<bf16, 4, 1>))
+                    : (narrow ? (two ? scan_fwd_launch<float, 2, 2> : scan_fwd_launch<float, 2, 1>)
+                              : (two ? scan_fwd_launch<float, 4, 2> : scan_fwd_launch<float, 4, 1>));
+  return launch(x, x_sb, x_st, gate, g_sb, g_st, starts, h0, h, last, carry, batch, length, dim,
+                workspace, workspace_bytes, s);
 }
 
 oxc_status oxc_gated_scan_bwd(const void* x, int64_t x_sb, int64_t x_st, const void* gate,
@@ -944,9 +1000,6 @@ oxc_status oxc_gated_scan_bwd(const void* x, int64_t x_sb, int64_t x_st, const v
   }
   if (!x || !gate || !carry || !dx || !dgate)
     return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: gated_scan backward: null pointer");
-  Chain chain;
-  st = scan_chain("gated_scan backward", batch, length, dim, workspace, workspace_bytes, s, &chain);
-  if (st) return st;
   // 2 channels a thread; 4 where bf16 is read by vectors, which then cost half the
   // instructions (94 us instead of 117 at [4, 2048, 4096]; f32 needs the registers,
   // 141 us against 150)
@@ -956,7 +1009,7 @@ oxc_status oxc_gated_scan_bwd(const void* x, int64_t x_sb, int64_t x_st, const v
   auto launch = dtype == OXC_BF16 ? (wide ? scan_bwd_launch<bf16, 4> : scan_bwd_launch<bf16, 2>)
                                   : scan_bwd_launch<float, 2>;
   return launch(x, x_sb, x_st, gate, g_sb, g_st, starts, carry, dh, dh_sb, dh_st, dlast, dx, dgate,
-                dh0, chain, batch, length, dim, s);
+                dh0, batch, length, dim, workspace, workspace_bytes, s);
 }
 
 oxc_status oxc_gated_step(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,

@@ -188,7 +188,8 @@ def test_add_rms_norm_empty_and_refusals():
 # ---- gated_scan -----------------------------------------------------------------------
 
 SCAN_SHAPES = [(1, 1, 1), (2, 1, 130), (1, 2, 64), (3, 63, 33), (2, 64, 128), (2, 65, 256), (1, 127, 100),
-               (2, 129, 512), (1, 700, 40), (1, 2049, 260), (5, 300, 1001), (1, 9001, 8)]
+               (2, 129, 512), (1, 700, 40), (1, 2049, 260), (5, 300, 1001), (1, 9001, 8), (16, 5001, 64),
+               (3, 12900, 130)]
 
 
 def _scan_inputs(B, T, D, dtype, seed=0, starts=False):
