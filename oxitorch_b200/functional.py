@@ -17,6 +17,7 @@ mathematical gradient.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 import ctypes
 
@@ -531,7 +532,8 @@ def swiglu(gate, up):
 # distilled from a larger one and then drafts tokens for it.  The reference has
 # no counterpart.  Activations and logits may be float32 or bfloat16; the
 # residual stream, weights, recurrent states, scales and probabilities are
-# float32, and so is all arithmetic (a bfloat16 result is rounded once).
+# float32, and so is all arithmetic (a bfloat16 result is rounded once).  Their
+# gradients cannot be differentiated again; torch refuses to.
 
 _DTYPES = {torch.float32: N.F32, torch.bfloat16: N.BF16}
 
@@ -651,6 +653,7 @@ class _AddRMSNorm(torch.autograd.Function):
         return y, r
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dr):
         r, weight, rstd = ctx.saved_tensors
         if dy is None:  # only the residual stream was used
@@ -769,6 +772,7 @@ class _GatedScan(torch.autograd.Function):
         return h, last
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dh, dlast):
         x, gate, carry, starts = ctx.saved_tensors
         if dh is None and dlast is None:
@@ -807,6 +811,8 @@ def gated_step(x, gate, state, out=None):
         _operand("out", out, x.shape, torch.float32, x.device)
     if not (state.is_contiguous() and out.is_contiguous()):
         raise ValueError("invalid argument: state and out must be contiguous")
+    if 0 < abs(out.data_ptr() - state.data_ptr()) < 4 * state.numel():
+        raise ValueError("invalid argument: out must be state or not overlap it")
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad):
         raise ValueError("invalid argument: gated_step has no gradient; train with gated_scan")
     x, gate = _rows2d(x), _rows2d(gate)
@@ -861,6 +867,7 @@ class _DistillLoss(torch.autograd.Function):
         return loss.reshape(())
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         if g.dtype != torch.float32:
             g = g.to(torch.float32)

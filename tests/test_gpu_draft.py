@@ -371,6 +371,23 @@ def test_gated_step_continues_a_scan(B, D, dtype):
                 lambda: F.gated_step(x[:, 0].clone().requires_grad_(), gate[:, 0], state)):
         with pytest.raises(ValueError):
             bad()
+    pair = torch.zeros(2 * B * D, device="cuda")
+    if B * D > 1:
+        with pytest.raises(ValueError, match="overlap"):
+            F.gated_step(x[:, 0], gate[:, 0], pair[:B * D].view(B, D), out=pair[1:B * D + 1].view(B, D))
+
+
+def test_gradients_refuse_to_be_differentiated_again():
+    import torch
+    from oxitorch_b200 import functional as F
+    x = torch.randn(2, 4, 8, device="cuda").requires_grad_()
+    h, _ = F.gated_scan(x, x)
+    y, _ = F.add_rms_norm(x, x, torch.ones(8, device="cuda"))
+    loss = F.distill_loss(x, torch.zeros(2, 4, 1, device="cuda"), torch.zeros(2, 4, 1, dtype=torch.int64, device="cuda"))
+    for out in (h.sum(), y.sum(), loss):
+        (g,) = torch.autograd.grad(out, x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
 
 
 # ---- distill_loss ------------------------------------------------------------------------
