@@ -391,8 +391,8 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_bwd_rows_kernel(
 
 // One CTA per row, the row in registers: thread t holds the elements t, t +
 // blockDim, ...
-template <typename T, int VW, int VPT, int MAXT, bool QUANT>
-__global__ void __launch_bounds__(MAXT) add_rms_fwd_kernel(
+template <typename T, int VPT, bool QUANT>
+__global__ void __launch_bounds__(1024) add_rms_fwd_kernel(
     const T* __restrict__ x, int64_t x_stride, const float* __restrict__ res, int64_t res_stride,
     const float* __restrict__ w, T* __restrict__ y, uint8_t* __restrict__ q,
     float* __restrict__ scale, int block_cols, float* __restrict__ r, float* __restrict__ rstd,
@@ -401,73 +401,41 @@ __global__ void __launch_bounds__(MAXT) add_rms_fwd_kernel(
   __shared__ uint32_t amax[QUANT ? kQuantMaxBlocks : 1];
   const int blocks = QUANT ? (cols + block_cols - 1) / block_cols : 0;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    float v[VPT][VW];
-    float ss = 0.0f;
+    const T* xr = x + row * x_stride;
+    const float* rr = res + row * res_stride;
+    const int64_t out = row * (int64_t)cols;
     if constexpr (QUANT) {
       for (int b = threadIdx.x; b < blocks; b += blockDim.x) amax[b] = 0u;
     }
+    float v[VPT];
+    float ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int e = (i * blockDim.x + threadIdx.x) * VW;
-      if (e < cols) {
-        float a[VW];
-        load_as_f32<VW>(a, x + row * x_stride + e);
-        load_as_f32<VW>(v[i], res + row * res_stride + e);
-#pragma unroll
-        for (int k = 0; k < VW; ++k) v[i][k] += a[k];
-        store_from_f32<VW>(r + row * (int64_t)cols + e, v[i]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < VW; ++k) v[i][k] = 0.0f;
-      }
+      const int e = i * blockDim.x + threadIdx.x;
+      v[i] = e < cols ? to_f32(xr[e]) + ld_stream(rr + e) : 0.0f;
+      ss = fmaf(v[i], v[i], ss);
     }
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int k = 0; k < VW; ++k) ss = fmaf(v[i][k], v[i][k], ss);
     ss = block_sum(ss, scratch);
     const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)cols) + eps));
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int e = (i * blockDim.x + threadIdx.x) * VW;
-      if (e < cols) {
-        float wv[VW];
-        load_vec<VW>(wv, w + e, false);
-#pragma unroll
-        for (int k = 0; k < VW; ++k) v[i][k] = v[i][k] * inv * wv[k];
-        if constexpr (!QUANT) store_from_f32<VW>(y + row * (int64_t)cols + e, v[i]);
-      }
+      const int e = i * blockDim.x + threadIdx.x;
+      if (e >= cols) continue;
+      st_stream(r + out + e, v[i]);
+      v[i] = v[i] * inv * __ldg(w + e);
+      if constexpr (QUANT) atomicMax(&amax[e / block_cols], __float_as_uint(fabsf(v[i])));
+      else y[out + e] = from_f32<T>(v[i]);
     }
     if constexpr (QUANT) {
-      // |y|'s bits order like its values, NaN above infinity: a NaN in a block
-      // makes its scale NaN
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int e = (i * blockDim.x + threadIdx.x) * VW;
-        if (e < cols) {
-          uint32_t m = 0u;
-#pragma unroll
-          for (int k = 0; k < VW; ++k) m = max(m, __float_as_uint(fabsf(v[i][k])));
-          atomicMax(&amax[e / block_cols], m);
-        }
-      }
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        const int e = (i * blockDim.x + threadIdx.x) * VW;
-        if (e < cols) {
-          const int b = e / block_cols;
-          const float s = quant_scale(amax[b]), to = __fdiv_rn(1.0f, s);
-          uint8_t o[VW];
-#pragma unroll
-          for (int k = 0; k < VW; ++k) o[k] = to_e4m3(v[i][k] * to);
-          uint8_t* qp = q + row * (int64_t)cols + e;
-          if constexpr (VW == 4)
-            *reinterpret_cast<uchar4*>(qp) = make_uchar4(o[0], o[1], o[2], o[3]);
-          else
-            qp[0] = o[0];
-          if (e == b * block_cols) scale[row * blocks + b] = s;
-        }
+        const int e = i * blockDim.x + threadIdx.x;
+        if (e >= cols) continue;
+        const int b = e / block_cols;
+        const float s = quant_scale(amax[b]);
+        q[out + e] = to_e4m3(v[i] * __fdiv_rn(1.0f, s));
+        if (e == b * block_cols) scale[row * blocks + b] = s;
       }
       __syncthreads();  // amax is read; the next row clears it
     } else if (threadIdx.x == 0) {
@@ -476,10 +444,10 @@ __global__ void __launch_bounds__(MAXT) add_rms_fwd_kernel(
   }
 }
 
-// Persistent VJP: CTA b handles rows [b * chunk, min((b + 1) * chunk, rows))
-// and writes its dw partial to parts[b][cols].
-template <typename T, int VW, int VPT, int MAXT, int MODE>
-__global__ void __launch_bounds__(MAXT) add_rms_bwd_kernel(
+// Persistent VJP: CTA b handles rows [b * chunk, min((b + 1) * chunk, rows)) and
+// writes its dw partial to parts[b][cols].
+template <typename T, int VPT, int MODE>
+__global__ void __launch_bounds__(1024) add_rms_bwd_kernel(
     const float* __restrict__ r, const float* __restrict__ w, const float* __restrict__ rstd,
     const T* __restrict__ dy, int64_t dy_stride, const float* __restrict__ dr, int64_t dr_stride,
     float* __restrict__ dres, T* __restrict__ dx, float* __restrict__ parts, int64_t rows, int cols,
@@ -488,63 +456,45 @@ __global__ void __launch_bounds__(MAXT) add_rms_bwd_kernel(
   __shared__ float scratch[33];
   const int64_t r0 = (int64_t)blockIdx.x * chunk;
   const int64_t r1 = min(rows, r0 + chunk);
-  float wv[VPT][VW], acc[VPT][VW];
+  float wv[VPT], acc[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int e = (i * blockDim.x + threadIdx.x) * VW;
-#pragma unroll
-    for (int k = 0; k < VW; ++k) { acc[i][k] = 0.0f; wv[i][k] = 0.0f; }
-    if (e < cols) load_vec<VW>(wv[i], w + e, false);
+    const int e = i * blockDim.x + threadIdx.x;
+    acc[i] = 0.0f;
+    wv[i] = e < cols ? __ldg(w + e) : 0.0f;
   }
   const float inv_n = __fdiv_rn(1.0f, (float)cols);
   for (int64_t row = r0; row < r1; ++row) {
-    float u[VPT][VW], g[VPT][VW], d[VPT][VW];
     const float inv = __ldg(rstd + row);
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int e = (i * blockDim.x + threadIdx.x) * VW;
-#pragma unroll
-      for (int k = 0; k < VW; ++k) { u[i][k] = 0.0f; g[i][k] = 0.0f; d[i][k] = 0.0f; }
-      if (e < cols) {
-        load_vec<VW>(u[i], r + row * (int64_t)cols + e, true);
-        load_as_f32<VW>(g[i], dy + row * dy_stride + e);
-        if (dr) load_as_f32<VW>(d[i], dr + row * dr_stride + e);
-      }
-    }
+    const int64_t out = row * (int64_t)cols;
+    float u[VPT], g[VPT];
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        u[i][k] *= inv;
-        acc[i][k] = fmaf(g[i][k], u[i][k], acc[i][k]);
-        g[i][k] *= wv[i][k];
-        s = fmaf(g[i][k], u[i][k], s);
-      }
+    for (int i = 0; i < VPT; ++i) {
+      const int e = i * blockDim.x + threadIdx.x;
+      u[i] = e < cols ? ld_stream(r + out + e) * inv : 0.0f;
+      g[i] = e < cols ? to_f32(dy[row * dy_stride + e]) : 0.0f;
+      acc[i] = fmaf(g[i], u[i], acc[i]);
+      g[i] *= wv[i];
+      s = fmaf(g[i], u[i], s);
+    }
     float mean = 0.0f;
     if constexpr (MODE == OXC_GRAD_EXACT) mean = block_sum(s, scratch) * inv_n;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int e = (i * blockDim.x + threadIdx.x) * VW;
-      if (e < cols) {
-#pragma unroll
-        for (int k = 0; k < VW; ++k) {
-          if constexpr (MODE == OXC_GRAD_EXACT) g[i][k] = fmaf(-u[i][k], mean, g[i][k]);
-          d[i][k] = fmaf(inv, g[i][k], d[i][k]);
-        }
-        store_from_f32<VW>(dres + row * (int64_t)cols + e, d[i]);
-        if constexpr (sizeof(T) == 2) store_from_f32<VW>(dx + row * (int64_t)cols + e, d[i]);
-      }
+      const int e = i * blockDim.x + threadIdx.x;
+      if (e >= cols) continue;
+      if constexpr (MODE == OXC_GRAD_EXACT) g[i] = fmaf(-u[i], mean, g[i]);
+      const float d = fmaf(inv, g[i], dr ? ld_stream(dr + row * dr_stride + e) : 0.0f);
+      st_stream(dres + out + e, d);
+      if constexpr (sizeof(T) == 2) dx[out + e] = from_f32<T>(d);
     }
   }
   float* pr = parts + (int64_t)blockIdx.x * cols;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int e = (i * blockDim.x + threadIdx.x) * VW;
-    if (e < cols) {
-#pragma unroll
-      for (int k = 0; k < VW; ++k) pr[e + k] = acc[i][k];
-    }
+    const int e = i * blockDim.x + threadIdx.x;
+    if (e < cols) pr[e] = acc[i];
   }
 }
 
@@ -625,7 +575,7 @@ static oxc_status add_rms_fwd_launch(const char* fn, const void* x, int64_t x_st
   const RowGeom g = row_geom(cols, false);
   const unsigned grid = (unsigned)std::min<int64_t>(rows, 0x7fffffff);
 #define LAUNCH(VPT)                                                                             \
-  add_rms_fwd_kernel<T, 1, VPT, 1024, QUANT><<<grid, g.block, 0, s>>>(                          \
+  add_rms_fwd_kernel<T, VPT, QUANT><<<grid, g.block, 0, s>>>(                          \
       static_cast<const T*>(x), x_stride, res, res_stride, w, static_cast<T*>(y), q, scale,     \
       block_cols, r, rstd, rows, (int)cols, eps)
   switch (g.vpt) {
@@ -682,11 +632,11 @@ static oxc_status add_rms_bwd_launch(const float* r, const float* w, const float
 #define LAUNCH(VPT)                                                                             \
   do {                                                                                          \
     if (mode == OXC_GRAD_REF)                                                                   \
-      add_rms_bwd_kernel<T, 1, VPT, 1024, OXC_GRAD_REF><<<(unsigned)ctas, g.block, 0, s>>>(     \
+      add_rms_bwd_kernel<T, VPT, OXC_GRAD_REF><<<(unsigned)ctas, g.block, 0, s>>>(     \
           r, w, rstd, static_cast<const T*>(dy), dy_stride, dr, dr_stride, dres,                \
           static_cast<T*>(dx), parts, rows, (int)cols, chunk);                                  \
     else                                                                                        \
-      add_rms_bwd_kernel<T, 1, VPT, 1024, OXC_GRAD_EXACT><<<(unsigned)ctas, g.block, 0, s>>>(   \
+      add_rms_bwd_kernel<T, VPT, OXC_GRAD_EXACT><<<(unsigned)ctas, g.block, 0, s>>>(   \
           r, w, rstd, static_cast<const T*>(dy), dy_stride, dr, dr_stride, dres,                \
           static_cast<T*>(dx), parts, rows, (int)cols, chunk);                                  \
   } while (0)

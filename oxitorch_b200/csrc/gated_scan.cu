@@ -55,14 +55,14 @@ struct SeqView {
   int64_t sb, st;
 };
 
-// a = sigmoid(g) and b = 1 - a for two channels, both relatively accurate (b is
-// not formed by subtraction, which would lose it for large gates): with e =
-// exp(-|g|) they are 1 / (1 + e) and e / (1 + e).  e = 2^t exp(n - t ln 2) with
-// n = -|g| and t = n log2(e) rounded; the second factor, the rounding's share,
-// to first order.  Below -100 e is 0 anyway, so n stops there (and stays finite
-// for infinite gates; max.NaN keeps a NaN).  Two channels at a time on the packed
-// f32x2 pipe: at 16 bits the kernels would otherwise be bound by the issue of
-// these instructions rather than by memory.
+// a = sigmoid(g) and b = 1 - a for two channels, both relatively accurate: with e
+// = exp(-|g|) the smaller of the two is e / (1 + e), and the larger 1 minus that,
+// which rounds once (a reciprocal's error in an a close to 1 would grow with the
+// hundreds of tokens that such a gate remembers).  e = 2^t exp(n - t ln 2) with n =
+// -|g| and t = n log2(e) rounded; the second factor, the rounding's share, to first
+// order.  Below -100 e is 0 anyway, so n stops there (and stays finite for infinite
+// gates; max.NaN keeps a NaN).  Two channels at a time on the packed f32x2 pipe: at
+// 16 bits the kernels are bound by the issue of instructions as much as by memory.
 __device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float gate_arg(float g) {
   float n;
@@ -86,9 +86,9 @@ __device__ __forceinline__ void gate_pair(float2 g, float2& a, float2& b) {
   e = __ffma2_rn(e, __ffma2_rn(t, f2(-0.693147181f), n), e);
   const float2 d = __fadd2_rn(e, f2(1.0f));
   const float2 r = make_float2(rcp_approx(d.x), rcp_approx(d.y));
-  const float2 q = __fmul2_rn(e, r);
-  a = make_float2(g.x > 0.0f ? r.x : q.x, g.y > 0.0f ? r.y : q.y);
-  b = make_float2(g.x > 0.0f ? q.x : r.x, g.y > 0.0f ? q.y : r.y);
+  const float2 q = __fmul2_rn(e, r), o = __ffma2_rn(q, f2(-1.0f), f2(1.0f));
+  a = make_float2(g.x > 0.0f ? o.x : q.x, g.y > 0.0f ? o.y : q.y);
+  b = make_float2(g.x > 0.0f ? q.x : o.x, g.y > 0.0f ? q.y : o.y);
 }
 
 // ---- maps of the state ---------------------------------------------------------------

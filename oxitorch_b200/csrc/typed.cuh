@@ -31,7 +31,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 
 // VW consecutive elements as f32, evict-first; VW > 1 needs VW * sizeof(T)
-// alignment.  VW = 1, 2, 4, or 8 (bf16 only).
+// alignment.  VW = 1, 2 or 4, and 8 for storing bf16.
 template <int VW>
 __device__ __forceinline__ void load_as_f32(float (&d)[VW], const float* p) {
   if constexpr (VW == 4) {
@@ -47,19 +47,14 @@ __device__ __forceinline__ void load_as_f32(float (&d)[VW], const float* p) {
 }
 template <int VW>
 __device__ __forceinline__ void load_as_f32(float (&d)[VW], const bf16* p) {
-  if constexpr (VW == 8) {
-    const uint4 t = __ldcs(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { d[2 * i] = bf16_lo(w[i]); d[2 * i + 1] = bf16_hi(w[i]); }
-  } else if constexpr (VW == 4) {
+  if constexpr (VW == 4) {
     const uint2 t = __ldcs(reinterpret_cast<const uint2*>(p));
     d[0] = bf16_lo(t.x); d[1] = bf16_hi(t.x); d[2] = bf16_lo(t.y); d[3] = bf16_hi(t.y);
   } else if constexpr (VW == 2) {
     const uint32_t t = __ldcs(reinterpret_cast<const uint32_t*>(p));
     d[0] = bf16_lo(t); d[1] = bf16_hi(t);
   } else {
-    static_assert(VW == 1, "bf16 vectors hold 1, 2, 4 or 8 elements");
+    static_assert(VW == 1, "bf16 vectors hold 1, 2 or 4 elements");
     d[0] = bf16_lo(__ldcs(reinterpret_cast<const unsigned short*>(p)));
   }
 }

@@ -8,6 +8,9 @@ torch CUDA float32 tensors: torch supplies device memory, the stream and the
 autograd graph bookkeeping (``torch.autograd.Function``); all arithmetic on
 the path is ours.
 
+The last part of the file, the layers of a recurrent draft model, has no
+counterpart in the reference and takes bfloat16 activations too.
+
 ``grad_mode`` selects the backward semantics of the norms:
 ``"ref"`` (default) reproduces the reference graph, where ``rsqrt`` is
 detached (crates/oxi-bindings/src/lib.rs:682-697); ``"exact"`` is the full

@@ -162,6 +162,37 @@ def test_add_rms_norm_strided_rows_and_leading_dims(dtype):
     _check(rs.grad, d, bd, "dresidual of a sum")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(5, 260), (9, 133), (3, 4100), (40, 7)])
+def test_add_rms_norm_rows_that_start_anywhere(rows, cols, dtype):
+    """Operands whose rows no common alignment fits: views at odd offsets and strides."""
+    import torch
+    from oxitorch_b200 import functional as F
+    x, res, w, dy, dr = _norm_inputs(rows, cols, dtype, seed=3)
+
+    def odd(t, offset, extra):
+        wide = torch.full((rows, cols + extra), float("nan"), device="cuda", dtype=t.dtype)
+        wide[:, offset:offset + cols] = t
+        return wide[:, offset:offset + cols]
+    xo, ro, gyo, gro = odd(x, 1, 6), odd(res, 2, 3), odd(dy, 3, 7), odd(dr, 1, 2)
+    want_y, want_r, _ = R.add_rms_norm(_n(x), _n(res), _n(w), 1e-5)
+    y, r, rstd = F.add_rms_norm_fwd(xo, ro, w, 1e-5)
+    _check(y, want_y, 56 * R.EPS * np.abs(want_y), "y")
+    assert (r == x.float() + res).all()
+    for mode in ("ref", "exact"):
+        dx, dres, dw = F.add_rms_norm_bwd(r, w, rstd, gyo, gro, mode)
+        (d, want_dw), (bd, bdw) = R.add_rms_norm_grad(_n(x), _n(res), _n(w), 1e-5, _n(dy), _n(dr), mode == "exact")
+        _check(dres, d, bd, "dresidual")
+        _check(dx, d, bd, "dx")
+        _check(dw, want_dw, bdw, "dweight")
+    for block in (128, None):
+        q, scale, r = F.add_rms_norm_quant(xo, ro, w, 1e-5, block=block)
+        want = R.block_scales(want_y, block)
+        _check(scale, want, 60 * R.EPS * want, "scale")
+        z = want_y / np.repeat(want, block or cols, -1)[:, :cols]
+        _check(q.to(torch.float32), z, R.e4m3_half_step(z) * (1 + 2.0 ** -10) + 120 * R.EPS * np.abs(z), "q")
+
+
 def test_add_rms_norm_empty_and_refusals():
     import torch
     from oxitorch_b200 import functional as F
