@@ -331,7 +331,7 @@ template <typename T, int VW, bool VEC>
 struct Raw;
 
 template <int VW, bool VEC>
-struct Raw<float, VW, VEC> {
+struct __align__(VEC ? 4 * VW : 4) Raw<float, VW, VEC> {
   float v[VW];
   __device__ __forceinline__ void load(const float* p) {
     if constexpr (VEC) {
@@ -362,7 +362,7 @@ struct Raw<float, VW, VEC> {
 };
 
 template <int VW, bool VEC>
-struct Raw<bf16, VW, VEC> {
+struct __align__(VEC ? 2 * VW : 4) Raw<bf16, VW, VEC> {
   uint32_t w[VEC ? VW / 2 : VW];  // two to a word, or one in the lower half
   __device__ __forceinline__ void load(const bf16* p) {
     if constexpr (VEC && VW == 4) {
@@ -631,8 +631,22 @@ __global__ void __launch_bounds__(kScanWarps * 32, kScanCtas) scan_fwd_kernel(
   }
 }
 
-template <typename T, int VW, bool VEC, int CTAS>
-__global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
+// 8 or 16 bytes to shared memory without passing the registers; zeros unless `on`.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool on) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
+                 "r"(on ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(dst)), "l"(src),
+                 "r"(on ? 8 : 0) : "memory");
+}
+
+// With 4 channels a thread, x and dh are staged: copied to shared memory, each
+// thread's own vectors, and read there where they are needed, which leaves the
+// registers to the gates.
+template <typename T, int VW, bool VEC>
+__global__ void __launch_bounds__(kScanWarps * 32, kScanCtas) scan_bwd_kernel(
     SeqView<T> x, SeqView<T> gate, const uint8_t* __restrict__ starts,
     const float* __restrict__ carry, SeqView<T> dh, const float* __restrict__ dlast,
     T* __restrict__ dx, T* __restrict__ dgate, float* __restrict__ dh0, Chain chain, int64_t batch,
@@ -640,7 +654,10 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
     unsigned int tiles) {
   using L = Lane<T, VW, VEC>;
   using R = Raw<T, VW, VEC>;
-  constexpr int P = VW / 2;
+  constexpr int P = VW / 2, kThreads = kScanWarps * 32;
+  constexpr bool kStaged = VW == 4;
+  constexpr bool kGapStaged = kStaged && sizeof(T) == 4;  // h_{t-1} - x_t in the place of x_t
+  static_assert(!kStaged || VEC, "vectors are staged");
   // per warp: its map's A, the state's H and mu's H; then the state entering it
   // from the left and the mu from the right
   __shared__ __align__(16) float mapA[kScanWarps][L::kChannels];
@@ -649,6 +666,9 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
   __shared__ float2 before[kScanGroup - 1][L::kChannels];
   __shared__ float enter[L::kChannels];
   __shared__ __align__(16) Tile next;
+  extern __shared__ __align__(16) unsigned char staged_bytes[];
+  R* stage_x = reinterpret_cast<R*>(staged_bytes) + threadIdx.x;
+  R* stage_d = stage_x + kScanSteps * kThreads;
   Tiles order{&next, blockIdx.x, dtiles, (unsigned int)batch * dtiles, tiles, L::kChannels};
   const int warp = threadIdx.x >> 5;
   if (chain.ticket) order.draw(chain, 0u);
@@ -662,8 +682,22 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
     const int64_t t0 = (int64_t)tile.chunk * kScanChunk + warp * kScanSteps;
     const int64_t row0 = tile.b * length + t0;
     const int steps = (int)max((int64_t)0, min((int64_t)kScanSteps, length - t0));
-    R rg[kScanSteps], rx[kScanSteps], rd[kScanSteps];
-    {
+    R rg[kScanSteps], rx[kStaged ? 1 : kScanSteps], rd[kStaged ? 1 : kScanSteps];
+    if constexpr (kStaged) {
+      const T* pg = gate.p + (int64_t)tile.b * gate.sb + t0 * gate.st + lane.d;
+      const T* px = x.p + tile.b * x.sb + t0 * x.st + lane.d;
+      const T* pd = dh.p + tile.b * dh.sb + t0 * dh.st + lane.d;
+#pragma unroll
+      for (int i = 0; i < kScanSteps; ++i) {
+        const bool on = i < steps && lane.live;
+        rg[i].load_some(pg, on, INFINITY);
+        copy_async<sizeof(R)>(stage_x + i * kThreads, on ? px : x.p, on);
+        copy_async<sizeof(R)>(stage_d + i * kThreads, on && dh.p ? pd : x.p, on && dh.p);
+        pg += gate.st;
+        pd += dh.st;
+        px += x.st;
+      }
+    } else {
       const T* pg = gate.p + (int64_t)tile.b * gate.sb + t0 * gate.st + lane.d;
       const T* px = x.p + tile.b * x.sb + t0 * x.st + lane.d;
       const T* pd = dh.p + tile.b * dh.sb + t0 * dh.st + lane.d;
@@ -691,6 +725,21 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
         }
       }
     }
+    // the i-th token's x (then h_{t-1} - x) and dh
+    auto get_x = [&](int i, float2 (&o)[P]) {
+      const R* r;
+      if constexpr (kStaged) r = stage_x + i * kThreads;
+      else r = rx + i;
+#pragma unroll
+      for (int j = 0; j < P; ++j) o[j] = r->pair(j);
+    };
+    auto get_d = [&](int i, float2 (&o)[P]) {
+      const R* r;
+      if constexpr (kStaged) r = stage_d + i * kThreads;
+      else r = rd + i;
+#pragma unroll
+      for (int j = 0; j < P; ++j) o[j] = r->pair(j);
+    };
     const unsigned int fresh = start_bits(starts, tile.b, t0, length);
     float2 a[kScanSteps][P], b[kScanSteps][P], A[P], S[P], M[P];
 #pragma unroll
@@ -699,23 +748,30 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
     for (int i = 0; i < kScanSteps; ++i)
 #pragma unroll
       for (int j = 0; j < P; ++j) gate_pair(rg[i].pair(j), a[i][j], b[i][j]);
+    if constexpr (kStaged) asm volatile("cp.async.wait_all;" ::: "memory");
     by_fresh(fresh, [&](auto some) {
 #pragma unroll
-      for (int i = 0; i < kScanSteps; ++i)
+      for (int i = 0; i < kScanSteps; ++i) {
+        float2 xi[P];
+        get_x(i, xi);
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-          const float2 v = __fmul2_rn(b[i][j], rx[i].pair(j));
+          const float2 v = __fmul2_rn(b[i][j], xi[j]);
           S[j] = __ffma2_rn(a[i][j], S[j], v);
           A[j] = __fmul2_rn(A[j], a[i][j]);
           if (decltype(some)::value && ((fresh >> i) & 1u)) { S[j] = v; A[j] = f2(-0.0f); }
         }
+      }
 #pragma unroll
-      for (int i = kScanSteps - 1; i >= 0; --i)
+      for (int i = kScanSteps - 1; i >= 0; --i) {
+        float2 di[P];
+        get_d(i, di);
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-          M[j] = __fmul2_rn(a[i][j], __fadd2_rn(rd[i].pair(j), M[j]));
+          M[j] = __fmul2_rn(a[i][j], __fadd2_rn(di[j], M[j]));
           if (decltype(some)::value && ((fresh >> i) & 1u)) M[j] = f2(0.0f);
         }
+      }
     });
     lane.put(mapA[warp], A);
     lane.put(mapS[warp], S);
@@ -748,30 +804,43 @@ __global__ void __launch_bounds__(kScanWarps * 32, CTAS) scan_bwd_kernel(
     }
     __syncthreads();
     order.draw(chain, tile.rank);
-    float2 s[P], m[P], gap[kScanSteps][P];  // gap: h_{t-1} - x_t, what d h_t / d a_t is
+    float2 s[P], m[P], gap[kGapStaged ? 1 : kScanSteps][P];  // h_{t-1} - x_t, what d h_t / d a_t is
     lane.get(mapS[warp], s);
     lane.get(mapM[warp], m);
     by_fresh(fresh, [&](auto some) {
 #pragma unroll
-      for (int i = 0; i < kScanSteps; ++i)
+      for (int i = 0; i < kScanSteps; ++i) {
+        float2 xi[P];
+        get_x(i, xi);
+        [[maybe_unused]] R g;
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-          const float2 v = rx[i].pair(j);
           if (decltype(some)::value && ((fresh >> i) & 1u)) s[j] = f2(0.0f);
-          gap[i][j] = __fadd2_rn(s[j], make_float2(-v.x, -v.y));
-          s[j] = __ffma2_rn(a[i][j], s[j], __fmul2_rn(b[i][j], v));
+          const float2 q = __fadd2_rn(s[j], make_float2(-xi[j].x, -xi[j].y));
+          s[j] = __ffma2_rn(a[i][j], s[j], __fmul2_rn(b[i][j], xi[j]));
+          if constexpr (kGapStaged) g.v[2 * j] = q.x, g.v[2 * j + 1] = q.y;
+          else gap[i][j] = q;
         }
+        if constexpr (kGapStaged) stage_x[i * kThreads] = g;
+      }
       T* px = dx + (row0 + kScanSteps - 1) * dim;
       T* pg = dgate + (row0 + kScanSteps - 1) * dim;
 #pragma unroll
       for (int i = kScanSteps - 1; i >= 0; --i) {
-        float2 ox[P], og[P];
+        float2 ox[P], og[P], gi[P], di[P];
+        if constexpr (kGapStaged) {
+          get_x(i, gi);
+        } else {
+#pragma unroll
+          for (int j = 0; j < P; ++j) gi[j] = gap[i][j];
+        }
+        get_d(i, di);
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-          const float2 l = __fadd2_rn(rd[i].pair(j), m[j]);
+          const float2 l = __fadd2_rn(di[j], m[j]);
           ox[j] = __fmul2_rn(l, b[i][j]);
           m[j] = __fmul2_rn(a[i][j], l);
-          og[j] = __fmul2_rn(__fmul2_rn(m[j], b[i][j]), gap[i][j]);
+          og[j] = __fmul2_rn(__fmul2_rn(m[j], b[i][j]), gi[j]);
           if (decltype(some)::value && ((fresh >> i) & 1u)) m[j] = f2(0.0f);
         }
         if (i < steps) {
@@ -916,12 +985,22 @@ static oxc_status scan_bwd_launch(const void* x, int64_t x_sb, int64_t x_st, con
   const bool vec = seq_vec<T, VW>(x, x_sb, x_st, dim) && seq_vec<T, VW>(gate, g_sb, g_st, dim) &&
                    seq_vec<T, VW>(dh, dh_sb, dh_st, dim) && seq_vec<T, VW>(dx, 0, 0, dim) &&
                    seq_vec<T, VW>(dgate, 0, 0, dim);
-  auto kernel = vec ? scan_bwd_kernel<T, VW, true, kScanCtas> : scan_bwd_kernel<T, VW, false, kScanCtas>;
+  auto kernel = scan_bwd_kernel<T, VW, true>;
+  if constexpr (VW == 2)
+    kernel = vec ? kernel : scan_bwd_kernel<T, VW, false>;
+  else if (!vec)
+    return fail(OXC_ERR_OTHER, "internal: gated_scan backward: operands not aligned");
+  const size_t smem = VW == 4 ? 2 * kScanSteps * kScanWarps * 32 * VW * sizeof(T) : 0;
+  if (smem) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        (const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return cuda_fail(e, "oxc_gated_scan_bwd");
+  }
   const int64_t dtiles = (dim + 32 * VW - 1) / (32 * VW);
   const SeqView<T> xv{static_cast<const T*>(x), x_sb, x_st};
   const SeqView<T> gv{static_cast<const T*>(gate), g_sb, g_st};
   const SeqView<T> dv{static_cast<const T*>(dh), dh_sb, dh_st};
-  kernel<<<scan_grid((const void*)kernel, tiles, 0), kScanWarps * 32, 0, s>>>(
+  kernel<<<scan_grid((const void*)kernel, tiles, smem), kScanWarps * 32, smem, s>>>(
       xv, gv, starts, carry, dv, dlast, static_cast<T*>(dx), static_cast<T*>(dgate), dh0, chain,
       batch, length, dim, (int)(tiles / (batch * dtiles)), (unsigned)dtiles, (unsigned)tiles);
   return check_launch("oxc_gated_scan_bwd");
@@ -1000,14 +1079,19 @@ oxc_status oxc_gated_scan_bwd(const void* x, int64_t x_sb, int64_t x_st, const v
   }
   if (!x || !gate || !carry || !dx || !dgate)
     return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: gated_scan backward: null pointer");
-  // 2 channels a thread; 4 where bf16 is read by vectors, which then cost half the
-  // instructions (94 us instead of 117 at [4, 2048, 4096]; f32 needs the registers,
-  // 141 us against 150)
-  const bool wide = dtype == OXC_BF16 && dim > 64 && seq_vec<bf16, 4>(x, x_sb, x_st, dim) &&
-                    seq_vec<bf16, 4>(gate, g_sb, g_st, dim) && seq_vec<bf16, 4>(dh, dh_sb, dh_st, dim) &&
-                    seq_vec<bf16, 4>(dx, 0, 0, dim) && seq_vec<bf16, 4>(dgate, 0, 0, dim);
-  auto launch = dtype == OXC_BF16 ? (wide ? scan_bwd_launch<bf16, 4> : scan_bwd_launch<bf16, 2>)
-                                  : scan_bwd_launch<float, 2>;
+  // 2 channels a thread; 4, with x and dh staged, where vectors can be read: wider
+  // tiles, so fewer entries to the chain, and less of the addressing.  At [4, 2048,
+  // 4096] 94 us instead of 117 in bf16 and 134 instead of 143 in f32; in f32 not with
+  // a single chunk, which enters no chain ([16, 64, 8192]: 40 us against 34).
+  auto vec4 = [&](const void* p, int64_t sb, int64_t st) {
+    return dtype == OXC_BF16 ? seq_vec<bf16, 4>(p, sb, st, dim) : seq_vec<float, 4>(p, sb, st, dim);
+  };
+  const bool wide = dim > 64 && vec4(x, x_sb, x_st) && vec4(gate, g_sb, g_st) &&
+                    vec4(dh, dh_sb, dh_st) && vec4(dx, 0, 0) && vec4(dgate, 0, 0) &&
+                    (dtype == OXC_BF16 || length > kScanChunk);
+  auto launch = dtype == OXC_BF16
+                    ? (wide ? scan_bwd_launch<bf16, 4> : scan_bwd_launch<bf16, 2>)
+                    : (wide ? scan_bwd_launch<float, 4> : scan_bwd_launch<float, 2>);
   return launch(x, x_sb, x_st, gate, g_sb, g_st, starts, carry, dh, dh_sb, dh_st, dlast, dx, dgate,
                 dh0, batch, length, dim, workspace, workspace_bytes, s);
 }
