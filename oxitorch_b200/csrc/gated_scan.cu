@@ -306,7 +306,7 @@ struct Tile {
 // Without a chain (one chunk) the tiles are strided over the grid.  One thread
 // draws, works out the coordinates and posts them.
 struct Tiles {
-  Tile* next;  // shared
+  Tile* next;  // shared: the next tile, and the one a round of the grid after it
   unsigned int drawn, dtiles, per, tiles;
   int channels;
 
@@ -316,12 +316,34 @@ struct Tiles {
   }
   __device__ __forceinline__ void post() {
     if (mine()) {
-      const unsigned int chunk = drawn / per, rest = drawn - chunk * per, b = rest / dtiles;
-      *next = {(int)chunk, (int)b, (int)(rest - b * dtiles) * channels,
-               drawn < tiles ? (int)drawn : -1};
+      next[0] = at(drawn);
+      next[1] = at(per < tiles ? drawn + gridDim.x : tiles);  // one chunk: none
     }
   }
+  __device__ __forceinline__ Tile at(unsigned int rank) const {
+    const unsigned int chunk = rank / per, rest = rank - chunk * per, b = rest / dtiles;
+    return {(int)chunk, (int)b, (int)(rest - b * dtiles) * channels,
+            rank < tiles ? (int)rank : -1};
+  }
 };
+
+// Asks L2 for a tile's part of an operand.  The kernels do so for the tile a round of
+// the grid ahead (someone's next one: each tile is asked for once) before they wait
+// for the chain, which the loads from HBM would otherwise follow: f32 [4, 2048, 4096]
+// 75 us instead of 81 and 122 instead of 135 in the VJP.  With a single chunk there
+// is no wait to fill, and the VJP of bf16 [16, 64, 8192] took 27 us instead of 26.
+template <int TOKENS, int CHANNELS, typename T>
+__device__ __forceinline__ void ask_ahead(const SeqView<T>& v, const Tile& tile, int64_t length,
+                                          int64_t dim) {
+  constexpr int kPerLine = 128 / sizeof(T), kLines = CHANNELS / kPerLine;
+  if (tile.rank < 0) return;
+#pragma unroll
+  for (int i = threadIdx.x; i < TOKENS * kLines; i += kScanWarps * 32) {
+    const int64_t t = (int64_t)tile.chunk * TOKENS + i / kLines, d = tile.d0 + i % kLines * kPerLine;
+    if (t < length && d < dim)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(v.p + tile.b * v.sb + t * v.st + d));
+  }
+}
 
 // VW channels of one token as loaded.  VEC: consecutive ones, in one access; else
 // 32 apart (lane l takes l, l + 32, ...).  load_some takes the first `live` of
@@ -494,17 +516,17 @@ __global__ void __launch_bounds__(kScanWarps * 32, kScanCtas) scan_fwd_kernel(
   __shared__ __align__(16) float mapH[kMaps][L::kChannels];
   __shared__ float2 before[kScanGroup - 1][L::kChannels];
   __shared__ float enter[L::kChannels];
-  __shared__ __align__(16) Tile next;
+  __shared__ __align__(16) Tile next[2];
   extern __shared__ __align__(16) unsigned char held_bytes[];
   auto* held = reinterpret_cast<Held<2 * P>*>(held_bytes) + threadIdx.x;
-  Tiles order{&next, blockIdx.x, dtiles, (unsigned int)batch * dtiles, tiles, L::kChannels};
+  Tiles order{next, blockIdx.x, dtiles, (unsigned int)batch * dtiles, tiles, L::kChannels};
   const int warp = threadIdx.x >> 5;
   const int64_t chunks = (length + kScanChunk - 1) / kScanChunk;
   if (chain.ticket) order.draw(chain, 0u);
   order.post();
   for (;;) {
     __syncthreads();  // `next` is posted, the maps of the tile before are read
-    const Tile tile = next;
+    const Tile tile = next[0];
     if (tile.rank < 0) return;
     const L lane(tile.d0, dim);
     float2 a[kScanSteps][P], v[kScanSteps][P];
@@ -570,6 +592,9 @@ __global__ void __launch_bounds__(kScanWarps * 32, kScanCtas) scan_fwd_kernel(
         }
       }
     }
+    Tile ahead = next[1];
+    ask_ahead<HALVES * kScanChunk, L::kChannels>(gate, ahead, length, dim);
+    ask_ahead<HALVES * kScanChunk, L::kChannels>(x, ahead, length, dim);
     __syncthreads();
     const int c = threadIdx.x % L::kChannels, part = threadIdx.x / L::kChannels;
     const bool mine = tile.d0 + c < dim;
@@ -665,17 +690,17 @@ __global__ void __launch_bounds__(kScanWarps * 32, kScanCtas) scan_bwd_kernel(
   __shared__ __align__(16) float mapM[kScanWarps][L::kChannels];
   __shared__ float2 before[kScanGroup - 1][L::kChannels];
   __shared__ float enter[L::kChannels];
-  __shared__ __align__(16) Tile next;
+  __shared__ __align__(16) Tile next[2];
   extern __shared__ __align__(16) unsigned char staged_bytes[];
   R* stage_x = reinterpret_cast<R*>(staged_bytes) + threadIdx.x;
   R* stage_d = stage_x + kScanSteps * kThreads;
-  Tiles order{&next, blockIdx.x, dtiles, (unsigned int)batch * dtiles, tiles, L::kChannels};
+  Tiles order{next, blockIdx.x, dtiles, (unsigned int)batch * dtiles, tiles, L::kChannels};
   const int warp = threadIdx.x >> 5;
   if (chain.ticket) order.draw(chain, 0u);
   order.post();
   for (;;) {
     __syncthreads();  // `next` is posted, the maps of the tile before are read
-    Tile tile = next;
+    Tile tile = next[0];
     if (tile.rank < 0) return;
     tile.chunk = chunks - 1 - tile.chunk;  // from the end of the sequence
     const L lane(tile.d0, dim);
@@ -776,6 +801,11 @@ __global__ void __launch_bounds__(kScanWarps * 32, kScanCtas) scan_bwd_kernel(
     lane.put(mapA[warp], A);
     lane.put(mapS[warp], S);
     lane.put(mapM[warp], M);
+        Tile ahead = next[1];
+    ahead.chunk = chunks - 1 - ahead.chunk;
+    ask_ahead<kScanChunk, L::kChannels>(gate, ahead, length, dim);
+    ask_ahead<kScanChunk, L::kChannels>(x, ahead, length, dim);
+    if (dh.p) ask_ahead<kScanChunk, L::kChannels>(dh, ahead, length, dim);
     __syncthreads();
     // the mu of the chunk after this one (two sets of threads) and the state before
     // it (a third, or the second first)
@@ -1045,8 +1075,8 @@ oxc_status oxc_gated_scan_fwd(const void* x, int64_t x_sb, int64_t x_st, const v
     return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: gated_scan: null pointer");
   // 4 channels a thread, half as many where a tile would be wider than the tensor.
   // Tiles of two chunks where few channels leave many chunks of one chain in flight
-  // (bf16 [1, 65537, 1024]: 144 us instead of 163; with 128 tiles side by side, f32
-  // [4, 2048, 4096], 97 against 80), if there are several tiles for each CTA.
+  // (bf16 [1, 65537, 1024]: 141 us instead of 160; with 128 tiles side by side, f32
+  // [4, 2048, 4096], 81 against 75), if there are several tiles for each CTA.
   const bool narrow = dim <= 64;
   const int channels = narrow ? 64 : 128;
   const bool two = batch * ((dim + channels - 1) / channels) * 8 <= sm_count() &&
@@ -1081,7 +1111,7 @@ oxc_status oxc_gated_scan_bwd(const void* x, int64_t x_sb, int64_t x_st, const v
     return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: gated_scan backward: null pointer");
   // 2 channels a thread; 4, with x and dh staged, where vectors can be read: wider
   // tiles, so fewer entries to the chain, and less of the addressing.  At [4, 2048,
-  // 4096] 94 us instead of 117 in bf16 and 134 instead of 143 in f32; in f32 not with
+  // 4096] 94 us instead of 117 in bf16 and 135 instead of 143 in f32; in f32 not with
   // a single chunk, which enters no chain ([16, 64, 8192]: 40 us against 34).
   auto vec4 = [&](const void* p, int64_t sb, int64_t st) {
     return dtype == OXC_BF16 ? seq_vec<bf16, 4>(p, sb, st, dim) : seq_vec<float, 4>(p, sb, st, dim);
