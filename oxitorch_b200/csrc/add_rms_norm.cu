@@ -75,26 +75,34 @@ using raw_t = decltype(load_raw(static_cast<const T*>(nullptr)));
 
 // A thread's place in its row: vector i covers columns [e(i), e(i) + 4) of which
 // those outside [0, cols) do not exist.  Without EDGE the shift is 0 and a vector
-// exists whole or not at all.
+// exists whole or not at all.  With it the row's first and last vectors are loaded
+// whole like the others and then masked: what they hold beside the row is memory of
+// the rows before and after it, or between them -- except after the last row, whose
+// last vector is read by element.
 template <bool EDGE>
 struct RowSlots {
   int cols, o, first, step;  // columns; shift; the thread's first vector, from one to the next
   __device__ __forceinline__ int e(int i) const { return 4 * (first + i * step) - (EDGE ? o : 0); }
   __device__ __forceinline__ bool partial(int e) const { return EDGE && (e < 0 || e + 4 > cols); }
-  // the nearest vector that is whole: somewhere to load from without a branch
-  __device__ __forceinline__ int whole(int e) const {
+  // the nearest vector that can be loaded: somewhere to load from without a branch
+  __device__ __forceinline__ int near(int e, bool last_row) const {
     if constexpr (!EDGE) return min(e, cols - 4);
-    return max(min(e, ((cols + o) & ~3) - 4 - o), o ? 4 - o : 0);
+    return min(e, ((cols + o + (last_row ? 0 : 3)) & ~3) - 4 - o);
   }
   template <typename T>
-  __device__ __forceinline__ void take(float (&d)[4], const raw_t<T>& raw, const T* row, int e) const {
+  __device__ __forceinline__ void take(float (&d)[4], const raw_t<T>& raw, const T* row, int e,
+                                       bool last_row) const {
     raw_f32(d, raw);
     if (!EDGE) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) d[k] = e < cols ? d[k] : 0.0f;
     } else if (partial(e)) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) d[k] = e + k >= 0 && e + k < cols ? to_f32(row[e + k]) : 0.0f;
+      for (int k = 0; k < 4; ++k) d[k] = e + k >= 0 && e + k < cols ? d[k] : 0.0f;
+      if (last_row && e < cols && e + 4 > cols) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) d[k] = e + k < cols ? to_f32(row[e + k]) : 0.0f;
+      }
     }
   }
   template <typename T>
@@ -110,7 +118,7 @@ struct RowSlots {
   // a [cols] parameter, 16-byte aligned
   __device__ __forceinline__ void weights(float (&d)[4], const float* w, int e) const {
     if (!EDGE || (o == 0 && !partial(e))) {
-      raw_f32(d, __ldg(reinterpret_cast<const float4*>(w + whole(e))));
+      raw_f32(d, __ldg(reinterpret_cast<const float4*>(w + near(e, true))));
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) d[k] = __ldg(w + min(max(e + k, 0), cols - 1));
@@ -139,7 +147,7 @@ template <typename T, int VPT, int MAXT, bool QUANT, bool EDGE>
 __global__ void __launch_bounds__(MAXT) add_rms_fwd_rows_kernel(
     const T* __restrict__ x, int64_t x_stride, const float* __restrict__ res, int64_t res_stride,
     const float* __restrict__ w, T* __restrict__ y, uint8_t* __restrict__ q,
-    float* __restrict__ scale, int block_cols, float* __restrict__ r, float* __restrict__ rstd,
+    float* __restrict__ scale, int block_shift, float* __restrict__ r, float* __restrict__ rstd,
     int64_t rows, int cols, float eps, int group_warps) {
   __shared__ float scratch[32];
   __shared__ uint32_t amax[QUANT ? kQuantMaxBlocks + 1 : 1];
@@ -150,15 +158,16 @@ __global__ void __launch_bounds__(MAXT) add_rms_fwd_rows_kernel(
   const RowSlots<EDGE> s{cols, EDGE ? (int)((row * cols) & 3) : 0, in_group, group_warps * 32};
   const T* xr = x + row * x_stride;
   const float* rr = res + row * res_stride;
+  const bool last_row = row == rows - 1;
   raw_t<T> rx[VPT];
   float4 rv[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int e = s.whole(s.e(i));
+    const int e = s.near(s.e(i), last_row);
     rx[i] = load_raw(xr + e);
     rv[i] = load_raw(rr + e);
   }
-  const int blocks = QUANT ? (cols + block_cols - 1) / block_cols : 0;
+  const int blocks = QUANT ? ((cols - 1) >> block_shift) + 1 : 0;
   uint32_t* am = amax + (QUANT ? group * blocks : 0);
   if constexpr (QUANT) {
     for (int b = in_group; b < blocks; b += 32 * group_warps) am[b] = 0u;
@@ -169,8 +178,8 @@ __global__ void __launch_bounds__(MAXT) add_rms_fwd_rows_kernel(
   for (int i = 0; i < VPT; ++i) {
     const int e = s.e(i);
     float a[4];
-    s.take(a, rx[i], xr, e);
-    s.take(v[i], rv[i], rr, e);
+    s.take(a, rx[i], xr, e, last_row);
+    s.take(v[i], rv[i], rr, e, last_row);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       v[i][k] += a[k];
@@ -193,7 +202,7 @@ __global__ void __launch_bounds__(MAXT) add_rms_fwd_rows_kernel(
         s.put(y + row * (int64_t)cols, e, o);
       }
     }
-  } else if (!EDGE && block_cols == 128) {  // a scale is a warp's own affair
+  } else if (!EDGE && block_shift == 7) {  // a scale is a warp's own affair
     uint8_t* qr = q + row * (int64_t)cols;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -234,8 +243,8 @@ __global__ void __launch_bounds__(MAXT) add_rms_fwd_rows_kernel(
       m[i] = __reduce_max_sync(0xffffffffu, m[i]);
       const int e0 = __shfl_sync(0xffffffffu, e, 0) + s.o;  // a multiple of 128
       if (lane == 0 && e0 < cols + s.o) {
-        if (e0 < cols) atomicMax(&am[e0 / block_cols], m[i]);
-        if (s.o && e0 > 0) atomicMax(&am[(e0 - 1) / block_cols], before);
+        if (e0 < cols) atomicMax(&am[e0 >> block_shift], m[i]);
+        if (s.o && e0 > 0) atomicMax(&am[(e0 - 1) >> block_shift], before);
       }
     }
     group_sync(group, group_warps);
@@ -252,10 +261,10 @@ __global__ void __launch_bounds__(MAXT) add_rms_fwd_rows_kernel(
       const int e = s.e(i);
       if (e >= cols) continue;
       // at most two blocks meet in a vector
-      const int b0 = max(e, 0) / block_cols, b1 = min(e + 3, cols - 1) / block_cols;
+      const int b0 = max(e, 0) >> block_shift, b1 = min(e + 3, cols - 1) >> block_shift;
       const float to0 = __uint_as_float(am[b0]), to1 = __uint_as_float(am[b1]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[i][k] *= e + k < (b0 + 1) * block_cols ? to0 : to1;
+      for (int k = 0; k < 4; ++k) v[i][k] *= (max(e + k, 0) >> block_shift) == b0 ? to0 : to1;
       const uint32_t o = to_e4m3x4(v[i][0], v[i][1], v[i][2], v[i][3]);
       if (!s.partial(e)) {
         *reinterpret_cast<uint32_t*>(qr + e) = o;
@@ -307,24 +316,25 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_bwd_rows_kernel(
     const float* ur = r + row * (int64_t)cols;
     const T* gr = dy + row * dy_stride;
     const float* pr = dr ? dr + row * dr_stride : nullptr;
+    const bool last_row = row == rows - 1;
     float4 ru[VPT], rd[VPT];
     raw_t<T> rg[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int e = s.whole(s.e(i));
+      const int e = s.near(s.e(i), last_row);
       ru[i] = load_raw(ur + e);
       rg[i] = load_raw(gr + e);
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
-      rd[i] = pr ? load_raw(pr + s.whole(s.e(i))) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      rd[i] = pr ? load_raw(pr + s.near(s.e(i), last_row)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const float inv = __ldg(rstd + row);
     float u[VPT][4], g[VPT][4];
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      s.take(u[i], ru[i], ur, s.e(i));
-      s.take(g[i], rg[i], gr, s.e(i));
+      s.take(u[i], ru[i], ur, s.e(i), last_row);
+      s.take(g[i], rg[i], gr, s.e(i), last_row);
       float now[4];
       if constexpr (kShared) raw_f32(now, own_sums[i * s.step]);
 #pragma unroll
@@ -345,7 +355,7 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_bwd_rows_kernel(
       const int e = s.e(i);
       if (e >= cols) continue;
       float d[4];
-      if (pr) s.take(d, rd[i], pr, e);
+      if (pr) s.take(d, rd[i], pr, e, last_row);
       else raw_f32(d, rd[i]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -395,11 +405,11 @@ template <typename T, int VPT, bool QUANT>
 __global__ void __launch_bounds__(1024) add_rms_fwd_kernel(
     const T* __restrict__ x, int64_t x_stride, const float* __restrict__ res, int64_t res_stride,
     const float* __restrict__ w, T* __restrict__ y, uint8_t* __restrict__ q,
-    float* __restrict__ scale, int block_cols, float* __restrict__ r, float* __restrict__ rstd,
+    float* __restrict__ scale, int block_shift, float* __restrict__ r, float* __restrict__ rstd,
     int64_t rows, int cols, float eps) {
   __shared__ float scratch[33];
   __shared__ uint32_t amax[QUANT ? kQuantMaxBlocks : 1];
-  const int blocks = QUANT ? (cols + block_cols - 1) / block_cols : 0;
+  const int blocks = QUANT ? ((cols - 1) >> block_shift) + 1 : 0;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * x_stride;
     const float* rr = res + row * res_stride;
@@ -423,7 +433,7 @@ __global__ void __launch_bounds__(1024) add_rms_fwd_kernel(
       if (e >= cols) continue;
       st_stream(r + out + e, v[i]);
       v[i] = v[i] * inv * __ldg(w + e);
-      if constexpr (QUANT) atomicMax(&amax[e / block_cols], __float_as_uint(fabsf(v[i])));
+      if constexpr (QUANT) atomicMax(&amax[e >> block_shift], __float_as_uint(fabsf(v[i])));
       else y[out + e] = from_f32<T>(v[i]);
     }
     if constexpr (QUANT) {
@@ -432,10 +442,10 @@ __global__ void __launch_bounds__(1024) add_rms_fwd_kernel(
       for (int i = 0; i < VPT; ++i) {
         const int e = i * blockDim.x + threadIdx.x;
         if (e >= cols) continue;
-        const int b = e / block_cols;
+        const int b = e >> block_shift;
         const float s = quant_scale(amax[b]);
         q[out + e] = to_e4m3(v[i] * __fdiv_rn(1.0f, s));
-        if (e == b * block_cols) scale[row * blocks + b] = s;
+        if (e == b << block_shift) scale[row * blocks + b] = s;
       }
       __syncthreads();  // amax is read; the next row clears it
     } else if (threadIdx.x == 0) {
@@ -539,18 +549,20 @@ static oxc_status add_rms_check(const char* fn, int32_t dtype, int64_t rows, int
 }
 
 // Whether every row of x (and of the f32 tensor f) starts where the rows of the
-// dense tensors do, relative to a multiple of 4 elements.
+// dense tensors do, relative to a multiple of 4 elements, and where vectors are
+// partial (columns not a multiple of 4) at least 4 elements after the row before.
 template <typename T>
 static bool row_shift(const void* x, int64_t x_stride, const void* f, int64_t f_stride,
                       int64_t cols, int64_t rows) {
   return cols >= 8 && aligned_to(x, 4 * sizeof(T)) && aligned16(f) &&
-         (rows == 1 || ((x_stride - cols) % 4 == 0 && (f_stride - cols) % 4 == 0));
+         (rows == 1 || ((x_stride - cols) % 4 == 0 && (f_stride - cols) % 4 == 0 &&
+                        (cols % 4 == 0 || std::min(x_stride, f_stride) >= 4)));
 }
 
 template <typename T, bool QUANT>
 static oxc_status add_rms_fwd_launch(const char* fn, const void* x, int64_t x_stride,
                                      const float* res, int64_t res_stride, const float* w, void* y,
-                                     uint8_t* q, float* scale, int block_cols, float* r,
+                                     uint8_t* q, float* scale, int block_shift, float* r,
                                      float* rstd, int64_t rows, int64_t cols, float eps,
                                      cudaStream_t s) {
   if (row_shift<T>(x, x_stride, res, res_stride, cols, rows) && aligned16(w) && aligned16(r) &&
@@ -563,7 +575,7 @@ static oxc_status add_rms_fwd_launch(const char* fn, const void* x, int64_t x_st
   (cols % 4 ? add_rms_fwd_rows_kernel<T, VPT, MAXT, QUANT, true>                                \
             : add_rms_fwd_rows_kernel<T, VPT, MAXT, QUANT, false>)<<<(unsigned)grid, g.threads(), 0, s>>>( \
       static_cast<const T*>(x), x_stride, res, res_stride, w, static_cast<T*>(y), q, scale,     \
-      block_cols, r, rstd, rows, (int)cols, eps, g.warps)
+      block_shift, r, rstd, rows, (int)cols, eps, g.warps)
     if (g.vpt == 1) LAUNCH(1, 256);
     else if (g.vpt == 2) LAUNCH(2, 256);
     else if (g.vpt == 4 && g.threads() <= 512) LAUNCH(4, 512);
@@ -577,7 +589,7 @@ static oxc_status add_rms_fwd_launch(const char* fn, const void* x, int64_t x_st
 #define LAUNCH(VPT)                                                                             \
   add_rms_fwd_kernel<T, VPT, QUANT><<<grid, g.block, 0, s>>>(                          \
       static_cast<const T*>(x), x_stride, res, res_stride, w, static_cast<T*>(y), q, scale,     \
-      block_cols, r, rstd, rows, (int)cols, eps)
+      block_shift, r, rstd, rows, (int)cols, eps)
   switch (g.vpt) {
     case 1: LAUNCH(1); break;
     case 2: LAUNCH(2); break;
@@ -696,13 +708,13 @@ oxc_status oxc_add_rms_norm_quant(const void* x, int64_t x_stride, const float* 
   if (!x || !residual || !w || !q || !scale || !r)
     return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: add_rms_norm_quant: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int block_cols = block ? (int)block : (int)cols;
+  const int block_shift = block ? 7 : 31;  // a column's block
   if (dtype == OXC_BF16)
     return add_rms_fwd_launch<bf16, true>("oxc_add_rms_norm_quant", x, x_stride, residual,
-                                          residual_stride, w, nullptr, q, scale, block_cols, r,
+                                          residual_stride, w, nullptr, q, scale, block_shift, r,
                                           nullptr, rows, cols, eps, s);
   return add_rms_fwd_launch<float, true>("oxc_add_rms_norm_quant", x, x_stride, residual,
-                                         residual_stride, w, nullptr, q, scale, block_cols, r,
+                                         residual_stride, w, nullptr, q, scale, block_shift, r,
                                          nullptr, rows, cols, eps, s);
 }
 
