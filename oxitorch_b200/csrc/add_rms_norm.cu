@@ -277,6 +277,15 @@ __global__ void __launch_bounds__(MAXT) add_rms_fwd_rows_kernel(
   }
 }
 
+// Asks L2 for n elements, but those that share 16 bytes with what lies after them.
+template <typename T>
+__device__ __forceinline__ void ask_row(const T* p, int n) {
+  const uintptr_t from = reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15;
+  const uint32_t bytes = (uint32_t)(reinterpret_cast<uintptr_t>(p + n) - from) & ~15u;
+  if (bytes)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(bytes) : "memory");
+}
+
 // Persistent VJP.  Rows whose shift is equal (`period` apart) belong to one CTA, so
 // a thread's columns, and with them its dw sums, stay the same; the CTA's groups
 // are added in shared memory, in order, into its partial parts[b][cols].
@@ -294,21 +303,32 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_bwd_rows_kernel(
   const int part = blockIdx.x % period;
   const int64_t ctas = (gridDim.x - part + period - 1) / period;
   const RowSlots<EDGE> s{cols, EDGE ? (int)(((int64_t)part * cols) & 3) : 0, in_group, group_warps * 32};
-  // the dw sums: registers, or this thread's own vectors of shared memory in wide
-  // rows (one group a CTA)
-  constexpr bool kShared = VPT >= 4;
-  float4* own_sums = reinterpret_cast<float4*>(sums) + in_group;
-  float wv[VPT][4], acc[kShared ? 1 : VPT][4];
+  // the dw sums and the weights: registers, or this thread's own vectors of shared
+  // memory in wide rows (one group a CTA; beyond 4 vectors the weights are read anew
+  // for each row)
+  constexpr bool kShared = VPT >= 4, kOwnW = kShared && VPT <= 4;
+  float4* own_sums = reinterpret_cast<float4*>(sums) + threadIdx.x;
+  float4* own_w = own_sums + VPT * blockDim.x;
+  float w_held[kShared ? 1 : VPT][4], acc[kShared ? 1 : VPT][4];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    s.weights(wv[i], w, s.e(i));
     if constexpr (kShared) {
-      own_sums[i * s.step] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      own_sums[i * blockDim.x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if constexpr (kOwnW) {
+        float wv[4];
+        s.weights(wv, w, s.e(i));
+        own_w[i * blockDim.x] = make_float4(wv[0], wv[1], wv[2], wv[3]);
+      }
     } else {
+      s.weights(w_held[i], w, s.e(i));
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[i][k] = 0.0f;
     }
   }
+  // With few threads on the SM, nobody else loads while these add up and write: L2 is
+  // asked for the CTA's next row (bf16 [8192, 5000] 122 us instead of 141; with 1024
+  // threads in several CTAs, [16384, 4096], 184 instead of 174).
+  constexpr bool kAhead = MAXT > 512 || MAXT == 384;
   const float inv_n = __fdiv_rn(1.0f, (float)cols);
   int parity = 0;
   for (int64_t row = part + period * ((blockIdx.x / period) * groups + group); row < rows;
@@ -325,9 +345,20 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_bwd_rows_kernel(
       ru[i] = load_raw(ur + e);
       rg[i] = load_raw(gr + e);
     }
+    auto load_dr = [&] {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      rd[i] = pr ? load_raw(pr + s.near(s.e(i), last_row)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int i = 0; i < VPT; ++i)
+        rd[i] = pr ? load_raw(pr + s.near(s.e(i), last_row)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    };
+    if constexpr (!kShared) load_dr();
+    if (kAhead && threadIdx.x == 0) {
+      const int64_t next = row + period * ctas * groups;
+      if (next < rows) {
+        ask_row(r + next * cols, cols);
+        ask_row(dy + next * dy_stride, cols);
+        if (dr) ask_row(dr + next * dr_stride, cols);
+      }
+    }
     const float inv = __ldg(rstd + row);
     float u[VPT][4], g[VPT][4];
     float sum = 0.0f;
@@ -335,18 +366,21 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_bwd_rows_kernel(
     for (int i = 0; i < VPT; ++i) {
       s.take(u[i], ru[i], ur, s.e(i), last_row);
       s.take(g[i], rg[i], gr, s.e(i), last_row);
-      float now[4];
-      if constexpr (kShared) raw_f32(now, own_sums[i * s.step]);
+      float now[4], wv[4];
+      if constexpr (kShared) raw_f32(now, own_sums[i * blockDim.x]);
+      if constexpr (kOwnW) raw_f32(wv, own_w[i * blockDim.x]);
+      else if constexpr (kShared) s.weights(wv, w, s.e(i));
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         u[i][k] *= inv;
         if constexpr (kShared) now[k] = fmaf(g[i][k], u[i][k], now[k]);
         else acc[i][k] = fmaf(g[i][k], u[i][k], acc[i][k]);
-        g[i][k] *= wv[i][k];
+        g[i][k] *= kShared ? wv[k] : w_held[kShared ? 0 : i][k];
         sum = fmaf(g[i][k], u[i][k], sum);
       }
-      if constexpr (kShared) own_sums[i * s.step] = make_float4(now[0], now[1], now[2], now[3]);
+      if constexpr (kShared) own_sums[i * blockDim.x] = make_float4(now[0], now[1], now[2], now[3]);
     }
+    if constexpr (kShared) load_dr();  // all three at once would not fit the registers
     float mean = 0.0f;
     if constexpr (MODE == OXC_GRAD_EXACT)
       mean = group_total(sum, scratch[parity] + group * group_warps, group, group_warps) * inv_n;
@@ -371,7 +405,7 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_bwd_rows_kernel(
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       float now[4];
-      raw_f32(now, own_sums[i * s.step]);
+      raw_f32(now, own_sums[i * blockDim.x]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int c = s.e(i) + k;
@@ -613,10 +647,11 @@ static oxc_status add_rms_bwd_launch(const float* r, const float* w, const float
       aligned16(w) && aligned16(dres) && (sizeof(T) == 4 || aligned_to(dx, 4 * sizeof(T)))) {
     const GroupGeom g = bwd_geom(cols);
     const int period = cols % 4 == 0 ? 1 : cols % 2 == 0 ? 2 : 4;
-    const size_t smem = g.vpt >= 4      ? (size_t)g.vpt * g.threads() * sizeof(float4)
+    const bool edge = cols % 4 != 0, exact = mode == OXC_GRAD_EXACT;
+    const size_t smem = g.vpt >= 4
+                            ? (size_t)g.vpt * g.threads() * sizeof(float4) * (g.vpt <= 4 ? 2 : 1)
                         : g.groups > 1 ? (size_t)cols * sizeof(float)
                                        : 0;
-    const bool edge = cols % 4 != 0, exact = mode == OXC_GRAD_EXACT;
 #define LAUNCH(VPT, MAXT)                                                                       \
   do {                                                                                          \
     auto kernel = exact ? edge ? add_rms_bwd_rows_kernel<T, VPT, MAXT, OXC_GRAD_EXACT, true>    \
@@ -633,7 +668,9 @@ static oxc_status add_rms_bwd_launch(const float* r, const float* w, const float
         static_cast<T*>(dx), parts, rows, (int)cols, period, g.warps);                          \
   } while (0)
     if (g.vpt == 1) LAUNCH(1, 256);
+    else if (g.vpt == 2 && g.threads() <= 384 && g.threads() > 1024 / 3) LAUNCH(2, 384);
     else if (g.vpt == 2 && g.threads() <= 512) LAUNCH(2, 512);
+    else if (g.vpt == 2 && g.threads() <= 640) LAUNCH(2, 640);
     else if (g.vpt == 2) LAUNCH(2, 1024);
     else if (g.vpt == 4) LAUNCH(4, 1024);
     else LAUNCH(8, 1024);
