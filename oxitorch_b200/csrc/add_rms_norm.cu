@@ -144,13 +144,13 @@ __device__ __forceinline__ float group_total(float v, float* scratch, int group,
 constexpr int kMaxGroups = 8;  // per CTA
 
 template <typename T, int VPT, int MAXT, bool QUANT, bool EDGE>
-__global__ void __launch_bounds__(MAXT) add_rms_fwd_rows_kernel(
+__global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_fwd_rows_kernel(
     const T* __restrict__ x, int64_t x_stride, const float* __restrict__ res, int64_t res_stride,
     const float* __restrict__ w, T* __restrict__ y, uint8_t* __restrict__ q,
     float* __restrict__ scale, int block_shift, float* __restrict__ r, float* __restrict__ rstd,
     int64_t rows, int cols, float eps, int group_warps) {
   __shared__ float scratch[32];
-  __shared__ uint32_t amax[QUANT ? kQuantMaxBlocks + 1 : 1];
+  __shared__ uint32_t amax[!QUANT ? 1 : EDGE ? kQuantMaxBlocks + 1 : 32];  // of blocks or warps
   const int lane = threadIdx.x & 31, group = (threadIdx.x >> 5) / group_warps;
   const int in_group = threadIdx.x - group * group_warps * 32;
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x / (32 * group_warps)) + group;
@@ -167,9 +167,9 @@ __global__ void __launch_bounds__(MAXT) add_rms_fwd_rows_kernel(
     rx[i] = load_raw(xr + e);
     rv[i] = load_raw(rr + e);
   }
-  const int blocks = QUANT ? ((cols - 1) >> block_shift) + 1 : 0;
-  uint32_t* am = amax + (QUANT ? group * blocks : 0);
-  if constexpr (QUANT) {
+  const int blocks = QUANT && EDGE ? ((cols - 1) >> block_shift) + 1 : 0;
+  uint32_t* am = amax + group * blocks;
+  if constexpr (QUANT && EDGE) {
     for (int b = in_group; b < blocks; b += 32 * group_warps) am[b] = 0u;
   }
   float v[VPT][4];
@@ -202,27 +202,39 @@ __global__ void __launch_bounds__(MAXT) add_rms_fwd_rows_kernel(
         s.put(y + row * (int64_t)cols, e, o);
       }
     }
-  } else if (!EDGE && block_shift == 7) {  // a scale is a warp's own affair
-    uint8_t* qr = q + row * (int64_t)cols;
+  } else if constexpr (!EDGE) {  // a block of 128 columns is a warp's own affair
+    const bool by_block = block_shift == 7;
+    uint32_t m[VPT], all = 0u;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int e = s.e(i);
       float wv[4];
       s.weights(wv, w, e);
-      uint32_t m = 0u;
+      m[i] = 0u;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         v[i][k] *= inv * wv[k];
-        m = max(m, __float_as_uint(fabsf(v[i][k])));
+        m[i] = max(m[i], e < cols ? __float_as_uint(fabsf(v[i][k])) : 0u);
       }
-      const float sc = quant_scale(__reduce_max_sync(0xffffffffu, e < cols ? m : 0u));
-      const float to = __fdiv_rn(1.0f, sc);
+      m[i] = __reduce_max_sync(0xffffffffu, m[i]);
+      all = max(all, m[i]);
+    }
+    if (!by_block && group_warps > 1) {
+      if (lane == 0) amax[threadIdx.x >> 5] = all;
+      group_sync(group, group_warps);
+      all = __reduce_max_sync(0xffffffffu, lane < group_warps ? amax[group * group_warps + lane] : 0u);
+    }
+    uint8_t* qr = q + row * (int64_t)cols;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int e = s.e(i);
+      const float sc = quant_scale(by_block ? m[i] : all), to = __fdiv_rn(1.0f, sc);
       if (e < cols) {
         *reinterpret_cast<uint32_t*>(qr + e) = to_e4m3x4(v[i][0] * to, v[i][1] * to, v[i][2] * to, v[i][3] * to);
-        if (lane == 0) scale[row * blocks + e / 128] = sc;
+        if (lane == 0 && (by_block || e == 0)) scale[by_block ? row * ((cols + 127) / 128) + e / 128 : row] = sc;
       }
     }
-  } else {
+  } else {  // with a shift the blocks lie across warps
     uint32_t m[VPT];
     if (group_warps == 1) __syncwarp();
 #pragma unroll
@@ -286,11 +298,17 @@ __device__ __forceinline__ void ask_row(const T* p, int n) {
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(bytes) : "memory");
 }
 
+// CTAs of the VJP on an SM.
+__host__ __device__ constexpr int bwd_ctas(int vpt, bool edge, int threads) {
+  const int n = vpt >= 4 ? 1 : (edge && vpt == 2 ? 768 : 1024) / threads;
+  return n > 1 ? n : 1;
+}
+
 // Persistent VJP.  Rows whose shift is equal (`period` apart) belong to one CTA, so
 // a thread's columns, and with them its dw sums, stay the same; the CTA's groups
 // are added in shared memory, in order, into its partial parts[b][cols].
 template <typename T, int VPT, int MAXT, int MODE, bool EDGE>
-__global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_bwd_rows_kernel(
+__global__ void __launch_bounds__(MAXT, bwd_ctas(VPT, EDGE, MAXT)) add_rms_bwd_rows_kernel(
     const float* __restrict__ r, const float* __restrict__ w, const float* __restrict__ rstd,
     const T* __restrict__ dy, int64_t dy_stride, const float* __restrict__ dr, int64_t dr_stride,
     float* __restrict__ dres, T* __restrict__ dx, float* __restrict__ parts, int64_t rows, int cols,
@@ -328,7 +346,7 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_bwd_rows_kernel(
   // With few threads on the SM, nobody else loads while these add up and write: L2 is
   // asked for the CTA's next row (bf16 [8192, 5000] 122 us instead of 141; with 1024
   // threads in several CTAs, [16384, 4096], 184 instead of 174).
-  constexpr bool kAhead = MAXT > 512 || MAXT == 384;
+  constexpr bool kAhead = (EDGE && VPT > 1) || MAXT > 512 || MAXT == 384;
   const float inv_n = __fdiv_rn(1.0f, (float)cols);
   int parity = 0;
   for (int64_t row = part + period * ((blockIdx.x / period) * groups + group); row < rows;
@@ -412,22 +430,22 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_bwd_rows_kernel(
         if (c >= 0 && c < cols) pr[c] = now[k];
       }
     }
-    return;
-  }
-  for (int gi = 0; gi < groups; ++gi) {  // one group after the other
-    if (group == gi) {
+  } else {
+    for (int gi = 0; gi < groups; ++gi) {  // one group after the other
+      if (group == gi) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i)
+        for (int i = 0; i < VPT; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int c = s.e(i) + k;
-          if (c < 0 || c >= cols) continue;
-          const float a = gi > 0 ? sums[c] + acc[kShared ? 0 : i][k] : acc[kShared ? 0 : i][k];
-          if (gi + 1 < groups) sums[c] = a;
-          else pr[c] = a;
-        }
+          for (int k = 0; k < 4; ++k) {
+            const int c = s.e(i) + k;
+            if (c < 0 || c >= cols) continue;
+            const float a = gi > 0 ? sums[c] + acc[i][k] : acc[i][k];
+            if (gi + 1 < groups) sums[c] = a;
+            else pr[c] = a;
+          }
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -557,13 +575,17 @@ static GroupGeom group_geom(int64_t cols, int vpt) {
 }
 constexpr int kFwdVecs = 4;
 // 2 vectors a thread in the VJP: its 64 registers let 1024 threads share an SM.
-static GroupGeom bwd_geom(int64_t cols) { return group_geom(cols, 2); }
+static GroupGeom bwd_geom(int64_t cols) {
+  const GroupGeom g = group_geom(cols, 2);
+  if (cols % 4 && g.vpt == 2 && g.threads() > 640) return group_geom(cols, 4);
+  return g;
+}
 
 // CTAs of the VJP: as many as are resident, at least 4 rows a group; 4 at least,
 // one for each shift of the rows.
 static int64_t add_rms_bwd_ctas(int64_t rows, int64_t cols) {
   const GroupGeom g = bwd_geom(cols);
-  const int64_t per_sm = std::max(1, 1024 / g.threads());
+  const int64_t per_sm = bwd_ctas(g.vpt, cols % 4 != 0, g.threads());
   const int64_t by_rows = (rows + 4 * g.groups - 1) / (4 * g.groups);
   return std::max<int64_t>(4, std::min<int64_t>(per_sm * sm_count(), by_rows));
 }
@@ -652,12 +674,10 @@ static oxc_status add_rms_bwd_launch(const float* r, const float* w, const float
                             ? (size_t)g.vpt * g.threads() * sizeof(float4) * (g.vpt <= 4 ? 2 : 1)
                         : g.groups > 1 ? (size_t)cols * sizeof(float)
                                        : 0;
-#define LAUNCH(VPT, MAXT)                                                                       \
+#define LAUNCH(VPT, MAXT, EDGE)                                                                 \
   do {                                                                                          \
-    auto kernel = exact ? edge ? add_rms_bwd_rows_kernel<T, VPT, MAXT, OXC_GRAD_EXACT, true>    \
-                               : add_rms_bwd_rows_kernel<T, VPT, MAXT, OXC_GRAD_EXACT, false>   \
-                  : edge       ? add_rms_bwd_rows_kernel<T, VPT, MAXT, OXC_GRAD_REF, true>      \
-                               : add_rms_bwd_rows_kernel<T, VPT, MAXT, OXC_GRAD_REF, false>;    \
+    auto kernel = exact ? add_rms_bwd_rows_kernel<T, VPT, MAXT, OXC_GRAD_EXACT, EDGE>           \
+                        : add_rms_bwd_rows_kernel<T, VPT, MAXT, OXC_GRAD_REF, EDGE>;            \
     if (smem > 40 * 1024) {                                                                     \
       const cudaError_t e = cudaFuncSetAttribute(                                               \
           (const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);         \
@@ -667,13 +687,26 @@ static oxc_status add_rms_bwd_launch(const float* r, const float* w, const float
         r, w, rstd, static_cast<const T*>(dy), dy_stride, dr, dr_stride, dres,                  \
         static_cast<T*>(dx), parts, rows, (int)cols, period, g.warps);                          \
   } while (0)
-    if (g.vpt == 1) LAUNCH(1, 256);
-    else if (g.vpt == 2 && g.threads() <= 384 && g.threads() > 1024 / 3) LAUNCH(2, 384);
-    else if (g.vpt == 2 && g.threads() <= 512) LAUNCH(2, 512);
-    else if (g.vpt == 2 && g.threads() <= 640) LAUNCH(2, 640);
-    else if (g.vpt == 2) LAUNCH(2, 1024);
-    else if (g.vpt == 4) LAUNCH(4, 1024);
-    else LAUNCH(8, 1024);
+    const int n = g.threads();
+    if (edge) {
+      if (g.vpt == 1) LAUNCH(1, 256, true);
+      else if (g.vpt == 2 && n <= 256) LAUNCH(2, 256, true);
+      else if (g.vpt == 2 && n <= 384) LAUNCH(2, 384, true);
+      else if (g.vpt == 2) LAUNCH(2, 640, true);
+      else if (g.vpt == 4 && n <= 512) LAUNCH(4, 512, true);
+      else if (g.vpt == 4 && n <= 768) LAUNCH(4, 768, true);
+      else if (g.vpt == 4) LAUNCH(4, 1024, true);
+      else LAUNCH(8, 1024, true);
+    } else {
+      if (g.vpt == 1) LAUNCH(1, 256, false);
+      else if (g.vpt == 2 && n <= 384 && n > 1024 / 3) LAUNCH(2, 384, false);
+      else if (g.vpt == 2 && n <= 512) LAUNCH(2, 512, false);
+      else if (g.vpt == 2 && n <= 640) LAUNCH(2, 640, false);
+      else if (g.vpt == 2) LAUNCH(2, 1024, false);
+      else if (g.vpt == 4 && n <= 768) LAUNCH(4, 768, false);
+      else if (g.vpt == 4) LAUNCH(4, 1024, false);
+      else LAUNCH(8, 1024, false);
+    }
 #undef LAUNCH
   } else {
     const RowGeom g = row_geom(cols, false, 512);
