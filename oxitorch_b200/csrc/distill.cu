@@ -14,7 +14,10 @@
 // written once.  So a row stays in shared memory between the two, shared by a
 // cluster of 1 to 8 CTAs that exchange (max, sum) pairs through distributed shared
 // memory.  Rows wider than a cluster holds (1.25 MB) take the three-pass kernel,
-// which re-reads them from L2 or HBM.
+// which re-reads them from L2 or HBM.  Measured, of the copy bandwidth: f32 [4096,
+// 131072] 701 us (94%), [8192, 32000] 364 (88%); bf16 [8192, 32000] 204 (78%), [8192,
+// 131072] 863 (76%), where the issue of instructions and the exponentials are as
+// busy as the memory.
 #include <cooperative_groups.h>
 #include <math.h>
 

@@ -34,6 +34,11 @@
 // most 7 maps and a few group words, and since every state is defined by one
 // fixed sequence of operations -- whoever computes it, from however far back --
 // the results do not depend on timing.
+//
+// Bound by HBM in f32: [4, 2048, 4096] 75 us forward (82% of the copy bandwidth), 122
+// us VJP (84%).  At 16 bits half the bytes leave the waits for the chain and the
+// issue of instructions in sight: 66 and 91 us (46%, 57%), and [1, 65537, 1024], 1025
+// chunks in a row, 141 and 197 us (44%, 52%).
 #include <algorithm>
 #include <type_traits>
 

@@ -9,9 +9,9 @@
 //   w = max(p_j - q_j, 0) for j < n,  w = p_n for j = n,
 // as argmax_v w_v / e_v with e exponential variates (the first of equal ones),
 // which picks v with probability w_v / sum(w).  Should w be zero everywhere,
-// p_j takes its place; -1 if that has no positive entry either.  Without draft probabilities q_k is 1 at x_k and 0
-// elsewhere (a draft that was not sampled).  A NaN probability keeps no token
-// and is never the argmax.
+// p_j takes its place; -1 if that has no positive entry either.  Without draft
+// probabilities q_k is 1 at x_k and 0 elsewhere (a draft that was not sampled).  A
+// NaN probability keeps no token and is never the argmax.
 //
 // Each weight is one subtraction and one division in f32, correctly rounded,
 // so the choice is the same on every machine and in every order of reduction.
@@ -19,7 +19,9 @@
 // Three rows of the vocabulary are read per sequence, 12 bytes an entry.  A cluster
 // of up to 8 CTAs shares a sequence, so that few sequences still use many SMs;
 // every CTA works the acceptance out for itself (a few dozen loads) and the
-// argmax's keys meet in distributed shared memory.
+// argmax's keys meet in distributed shared memory.  Measured: 256 sequences of
+// 131072 entries 78.5 us (78% of the copy bandwidth), 64 of them 27 us (57%), where
+// the launch, the acceptance and the meeting are not hidden by other sequences.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -75,8 +77,8 @@ __device__ __forceinline__ Race warp_merge(Race r) {
 
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyCluster = 8;
-// Resident per SM: capped at 64 registers for a fourth (64 x 131072: 25.7 us instead
-// of 32.7 with three).
+// Resident per SM: capped at 64 registers for a fourth (64 x 131072: 27 us; three
+// took 7 us more).
 constexpr int kVerifyCtas = 4;
 
 // The best of the vocabulary entries [v0, v1) with weights p - q (q may be null;
