@@ -41,7 +41,7 @@ def add_rms_norm_grad(x, residual, w, eps, dy, dr, exact=True):
     # row mean as many again
     bound_d = EPS * (2 * np.abs(dr) + np.abs(inv) * (56 * np.abs(g) + 160 * np.abs(u) * mean_abs))
     rows = dy.size // r.shape[-1]
-    # dw: in a row within a CTA (at least 8 rows each, 296 CTAs at least on 148
+    # dw: in a row within a CTA (at least 8 rows each, 148 CTAs at least on 148
     # SMs), then the partials
     bound_dw = EPS * (rows / 64 + 128) * np.abs(dy * u).reshape(-1, r.shape[-1]).sum(0)
     return (d, dw), (bound_d, bound_dw)

@@ -193,6 +193,42 @@ def test_add_rms_norm_rows_that_start_anywhere(rows, cols, dtype):
         _check(q.to(torch.float32), z, R.e4m3_half_step(z) * (1 + 2.0 ** -10) + 120 * R.EPS * np.abs(z), "q")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(700, 6), (650, 1001), (600, 1537), (400, 2999), (400, 3000), (300, 3333),
+                                       (300, 5001), (200, 5804), (200, 7003), (30, 9000), (30, 10002), (20, 12999),
+                                       (9, 16383), (9, 20001)])
+def test_add_rms_norm_rows_between_nans(rows, cols, dtype):
+    """Rows read by whole vectors that reach into what lies between them: every
+    width's own kernel, several rows to a group."""
+    import torch
+    from oxitorch_b200 import functional as F
+    x, res, w, dy, dr = _norm_inputs(rows, cols, dtype, seed=4)
+
+    def apart(t, extra):  # the last row ends with the buffer
+        flat = torch.full(((rows - 1) * (cols + extra) + cols,), float("nan"), device="cuda", dtype=t.dtype)
+        view = flat.as_strided((rows, cols), (cols + extra, 1))
+        view.copy_(t)
+        return view
+    xa, ra, gya, gra = apart(x, 4), apart(res, 8), apart(dy, 4), apart(dr, 12)
+    want_y, _, _ = R.add_rms_norm(_n(x), _n(res), _n(w), 1e-5)
+    for dense in (False, True):
+        y, r, rstd = F.add_rms_norm_fwd(x if dense else xa, res if dense else ra, w, 1e-5)
+        _check(y, want_y, 56 * R.EPS * np.abs(want_y), "y")
+        assert (r == x.float() + res).all()
+        dx, dres, dw = F.add_rms_norm_bwd(r, w, rstd, dy if dense else gya, dr if dense else gra, "exact")
+        (d, want_dw), (bd, bdw) = R.add_rms_norm_grad(_n(x), _n(res), _n(w), 1e-5, _n(dy), _n(dr), True)
+        _check(dres, d, bd, "dresidual")
+        _check(dx, d, bd, "dx")
+        _check(dw, want_dw, bdw, "dweight")
+    for block in (128, None):
+        q, scale, r = F.add_rms_norm_quant(xa, ra, w, 1e-5, block=block)
+        assert (r == x.float() + res).all()
+        want = R.block_scales(want_y, block)
+        _check(scale, want, 60 * R.EPS * want, "scale")
+        z = want_y / np.repeat(want, block or cols, -1)[:, :cols]
+        _check(q.to(torch.float32), z, R.e4m3_half_step(z) * (1 + 2.0 ** -10) + 120 * R.EPS * np.abs(z), "q")
+
+
 def test_add_rms_norm_empty_and_refusals():
     import torch
     from oxitorch_b200 import functional as F
