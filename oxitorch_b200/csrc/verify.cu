@@ -20,7 +20,7 @@
 // of up to 8 CTAs shares a sequence, so that few sequences still use many SMs;
 // every CTA works the acceptance out for itself (a few dozen loads) and the
 // argmax's keys meet in distributed shared memory.  Measured: 256 sequences of
-// 131072 entries 78.5 us (78% of the copy bandwidth), 64 of them 27 us (57%), where
+// 131072 entries 71 us (86% of the copy bandwidth), 64 of them 25 us (61%), where
 // the launch, the acceptance and the meeting are not hidden by other sequences.
 #include <cooperative_groups.h>
 
@@ -75,76 +75,80 @@ __device__ __forceinline__ Race warp_merge(Race r) {
   return r;
 }
 
-constexpr int kVerifyThreads = 256;
 constexpr int kVerifyCluster = 8;
-// Resident per SM: capped at 64 registers for a fourth (64 x 131072: 27 us; three
-// took 7 us more).
+// CTAs of 256 threads per SM: capped at 64 registers for a fourth (three took 7 us
+// more at 64 x 131072).
 constexpr int kVerifyCtas = 4;
 
 // The best of the vocabulary entries [v0, v1) with weights p - q (q may be null;
 // token x counts 0).  The rows start anywhere: vectors where their addresses agree
 // modulo 16 bytes, else single entries.
+template <int THREADS>
 __device__ __forceinline__ Race race_best(const float* p, const float* q,
                                           const float* e, int64_t x, int64_t v0, int64_t v1) {
   Race k;
-  auto one = [&](float pv, float qv, float ev, int64_t v) {
-    k.add(v == x ? 0.0f : __fsub_rn(pv, qv), ev, (uint32_t)v);
+  p += v0;
+  e += v0;
+  if (q) q += v0;
+  const uint32_t n = (uint32_t)(v1 - v0);
+  const int64_t own = x - v0;
+  auto one = [&](float pv, float qv, float ev, uint32_t at) {
+    k.add(at == own ? 0.0f : __fsub_rn(pv, qv), ev, (uint32_t)(v0 + at));
   };
-  const uintptr_t o = reinterpret_cast<uintptr_t>(p + v0) & 15;
-  int64_t from = v1, to = v1;  // the part read by vectors
-  if (o == (reinterpret_cast<uintptr_t>(e + v0) & 15) &&
-      (!q || o == (reinterpret_cast<uintptr_t>(q + v0) & 15))) {
-    from = min(v1, v0 + (int64_t)((16 - o) & 15) / 4);
-    to = from + ((v1 - from) & ~(int64_t)3);
-  }
-  constexpr int U = 2;  // vectors in flight per row
-  for (int64_t v = from + 4 * threadIdx.x; v < to; v += 4 * U * kVerifyThreads) {
-    float4 pv[U], qv[U], ev[U];
+  const uintptr_t o = reinterpret_cast<uintptr_t>(p) & 15;
+  if (o == (reinterpret_cast<uintptr_t>(e) & 15) && (!q || o == (reinterpret_cast<uintptr_t>(q) & 15))) {
+    const uint32_t from = min(n, (uint32_t)((16 - o) & 15) / 4), to = from + ((n - from) & ~3u);
+    constexpr int U = 2;  // vectors in flight per row
+    for (uint32_t v = from + 4 * threadIdx.x; v < to; v += 4 * U * THREADS) {
+      float4 pv[U], qv[U], ev[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = min(v + 4 * u * kVerifyThreads, to - 4);  // twice the last is no harm
-      pv[u] = ld_stream(reinterpret_cast<const float4*>(p + at));
-      ev[u] = ld_stream(reinterpret_cast<const float4*>(e + at));
-      qv[u] = q ? ld_stream(reinterpret_cast<const float4*>(q + at)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int u = 0; u < U; ++u) {
+        const uint32_t at = min(v + 4 * u * THREADS, to - 4);  // twice the last is no harm
+        pv[u] = ld_stream(reinterpret_cast<const float4*>(p + at));
+        ev[u] = ld_stream(reinterpret_cast<const float4*>(e + at));
+        qv[u] = q ? ld_stream(reinterpret_cast<const float4*>(q + at)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t at = min(v + 4 * u * THREADS, to - 4);
+        one(pv[u].x, qv[u].x, ev[u].x, at);
+        one(pv[u].y, qv[u].y, ev[u].y, at + 1);
+        one(pv[u].z, qv[u].z, ev[u].z, at + 2);
+        one(pv[u].w, qv[u].w, ev[u].w, at + 3);
+      }
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = min(v + 4 * u * kVerifyThreads, to - 4);
-      one(pv[u].x, qv[u].x, ev[u].x, at);
-      one(pv[u].y, qv[u].y, ev[u].y, at + 1);
-      one(pv[u].z, qv[u].z, ev[u].z, at + 2);
-      one(pv[u].w, qv[u].w, ev[u].w, at + 3);
+    if (threadIdx.x < from + (n - to)) {  // before the vectors and after them
+      const uint32_t at = threadIdx.x < from ? threadIdx.x : to + threadIdx.x - from;
+      one(p[at], q ? q[at] : 0.0f, e[at], at);
     }
-  }
-  // what the vectors leave: before `from` and from `to` on, or everything
-  const int64_t head = from - v0, singles = from == v1 ? v1 - v0 : head + (v1 - to);
-  constexpr int S = 4;  // entries in flight per row
-  for (int64_t i = threadIdx.x; i < singles; i += S * kVerifyThreads) {
-    float pv[S], qv[S], ev[S];
-    int64_t at[S];
+  } else {
+    constexpr int S = 8;  // entries in flight per row (64 x 131071: 29 us; with 4, 31)
+    for (uint32_t i = threadIdx.x; i < n; i += S * THREADS) {
+      float pv[S], qv[S], ev[S];
 #pragma unroll
-    for (int u = 0; u < S; ++u) {
-      const int64_t n = min(i + u * kVerifyThreads, singles - 1);  // twice the last is no harm
-      at[u] = n < head ? v0 + n : to + (n - head);
-      pv[u] = ld_stream(p + at[u]);
-      ev[u] = ld_stream(e + at[u]);
-      qv[u] = q ? ld_stream(q + at[u]) : 0.0f;
+      for (int u = 0; u < S; ++u) {
+        const uint32_t at = min(i + u * THREADS, n - 1);  // twice the last is no harm
+        pv[u] = ld_stream(p + at);
+        ev[u] = ld_stream(e + at);
+        qv[u] = q ? ld_stream(q + at) : 0.0f;
+      }
+#pragma unroll
+      for (int u = 0; u < S; ++u) one(pv[u], qv[u], ev[u], min(i + u * THREADS, n - 1));
     }
-#pragma unroll
-    for (int u = 0; u < S; ++u) one(pv[u], qv[u], ev[u], at[u]);
   }
   return k;
 }
 
 // One cluster per sequence.
-__global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas) verify_kernel(
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(
     const float* __restrict__ target, int64_t t_sb, int64_t t_sk, const float* __restrict__ draft,
     int64_t d_sb, int64_t d_sk, const int64_t* __restrict__ tokens,
     const int64_t* __restrict__ lengths, const float* __restrict__ uniform,
     const float* __restrict__ race, int drafted, int64_t vocab, int64_t* __restrict__ out_tokens,
     int64_t* __restrict__ accepted, int32_t* err) {
   namespace cg = cooperative_groups;
-  constexpr int kWarps = kVerifyThreads / 32;
+  constexpr int kWarps = THREADS / 32;
   __shared__ unsigned long long best_key[kWarps], mine_key[2];
   __shared__ uint32_t best_zero[kWarps], mine_zero[2];
   __shared__ int first;
@@ -156,7 +160,7 @@ __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas) verify_kernel(
   const int n = (int)(want < 0 ? 0 : want > drafted ? drafted : want);
   if (threadIdx.x == 0) first = n;
   __syncthreads();
-  for (int k = threadIdx.x; k < n; k += kVerifyThreads) {
+  for (int k = threadIdx.x; k < n; k += THREADS) {
     const int64_t x = tok[k];
     bool keep = false;
     if (x < 0 || x >= vocab) {
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas) verify_kernel(
   Race k;
   for (int pass = 0; pass < 2; ++pass) {  // the second from p alone, if nothing was left
     const bool beyond = pass == 0 && j < n;
-    k = race_best(p, beyond && draft ? draft + b * d_sb + j * d_sk : nullptr, e,
+    k = race_best<THREADS>(p, beyond && draft ? draft + b * d_sb + j * d_sk : nullptr, e,
                   beyond && !draft ? tok[j] : -1, v0, v1);
     k = warp_merge(k);
     __syncthreads();
@@ -203,7 +207,7 @@ __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas) verify_kernel(
   }
   if (rank == 0) {
     const int64_t next = k.token();
-    for (int i = threadIdx.x; i <= drafted; i += kVerifyThreads)
+    for (int i = threadIdx.x; i <= drafted; i += THREADS)
       out_tokens[b * (drafted + 1) + i] = i < j ? tok[i] : i == j ? next : -1;
     if (threadIdx.x == 0) accepted[b] = j;
   }
@@ -240,9 +244,17 @@ oxc_status oxc_verify_draft(const float* target, int64_t target_sb, int64_t targ
          vocab >= (int64_t)size * 2 * 2048)
     size *= 2;
   if (batch > 0x7fffffff / size) size = 1;
+  // and larger CTAs where there are few (8 x 200003: 19 us instead of 27): as long as
+  // they fill three quarters of the SMs at most, since a cluster's share a GPC, which
+  // leaves some idle (16 x 131072 with a CTA an SM: 24 us instead of 19)
+  int threads = 256;
+  while (threads < 1024 && batch * size * threads * 2 <= 768 * (int64_t)sm_count() &&
+         vocab >= (int64_t)size * threads * 2 * 4)
+    threads *= 2;
+  auto kernel = threads == 256 ? verify_kernel<256> : threads == 512 ? verify_kernel<512> : verify_kernel<1024>;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(batch * size));
-  cfg.blockDim = dim3(kVerifyThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -251,7 +263,7 @@ oxc_status oxc_verify_draft(const float* target, int64_t target_sb, int64_t targ
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, verify_kernel, target, target_sb, target_sk, draft,
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, target, target_sb, target_sk, draft,
                                            draft_sb, draft_sk, tokens, lengths, uniform, race,
                                            (int)drafted, vocab, out_tokens, accepted, err_flag);
   if (e != cudaSuccess) return cuda_fail(e, "oxc_verify_draft");

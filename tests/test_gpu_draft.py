@@ -674,6 +674,14 @@ def test_verify_draft(B, K, V):
     _verify_check(p, None, tokens, u, e, lengths)
 
 
+@pytest.mark.parametrize("B,K,V", [(20, 2, 20001), (20, 2, 20004), (3, 1, 65536), (1, 2, 200003), (40, 1, 16388)])
+def test_verify_draft_few_long_rows(B, K, V):
+    """Larger CTAs, several of them to a sequence; rows aligned alike and not."""
+    p, q, tokens, u, e, lengths = _verify_inputs(B, K, V)
+    _verify_check(p, q, tokens, u, e, lengths)
+    _verify_check(p, None, tokens, u, e)
+
+
 def test_verify_draft_ties_equal_rows_and_zero_weights():
     p, q, tokens, u, e, _ = _verify_inputs(6, 3, 64)
     q[:] = p[:, :3]
