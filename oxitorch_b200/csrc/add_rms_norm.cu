@@ -16,17 +16,16 @@
 //
 // 8-bit output: per row, each block of `block` columns has the scale
 // s = max(amax(|y|) / 448, 2^-126) and q = e4m3(y / s), 448 being e4m3's
-// largest value (y times the scale's reciprocal: a tie may fall to the other side
-// when y / s is within two roundings of it).  y is not rounded to x's type in
-// between.
+// largest value.  y is not rounded to x's type in between, and its f32 product is
+// the one that the forward rounds.
 //
 // All are bound by HBM traffic: 8 + 2 sizeof(T) bytes an element forward, 9 +
 // sizeof(T) with the 8-bit output, 12 + sizeof(T) (and 2 more at 16 bits) for the
 // VJP.  A row is held in registers by a group of 1 to 32 warps (as many as its
 // width needs at 4 vectors a thread, 2 in the VJP; narrow rows share a CTA), all
 // of its loads issued before the first is used.  Measured, of the copy bandwidth:
-// [16384, 4096] f32 162 us forward (100%), 173 us VJP (95%), bf16 8-bit output 120
-// us (94%); bf16 [8192, 5001] 85, 124 and 107 us (88%, 81%, 64%: the blocks of 128
+// [16384, 4096] f32 162 us forward (100%), 173 us VJP (95%), bf16 8-bit output 122
+// us (92%); bf16 [8192, 5001] 85, 124 and 111 us (88%, 81%, 62%: the blocks of 128
 // columns of such a row lie across warps).
 //
 // Vectors are 4 elements at addresses that are multiples of 4 elements.  Where the
@@ -49,9 +48,9 @@ __device__ __forceinline__ uint8_t to_e4m3(float v) {
   return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
 }
 
-__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ uint32_t to_e4m3x4(float2 a, float2 b) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3);
   return lo | (hi << 16);
 }
 
@@ -60,6 +59,25 @@ __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d
 __device__ __forceinline__ float quant_scale(uint32_t amax) {
   const float a = __uint_as_float(amax);
   return a != a ? a : fmaxf(__fdiv_rn(a, 448.0f), 1.17549435e-38f);
+}
+
+// y / s for a pair of columns, rounded to nearest: z = y * RN(1 / s) is off by up to 1.5
+// ulp, y - z s is exact in one fma, and a second fma adds what it is worth (Markstein,
+// IBM J. Res. Dev. 34, 1990).  Two packed operations more than z alone, whose code is
+// the other one beside a tie in some 10 of 24 million elements; __fdiv_rn gives the
+// same codes at 3 to 19% more of the kernel's time instead of 2 to 8%.  An infinite scale
+// has no remainder: 0 for finite y, NaN for infinite.  (Where y is near the smallest
+// normal number the remainder may lie under 2^-149, and z stands.)
+struct Divisor {
+  float minus_s, rcp;
+};
+__device__ __forceinline__ Divisor divisor(float s) {
+  return {s == INFINITY ? 0.0f : -s, __fdiv_rn(1.0f, s)};
+}
+__device__ __forceinline__ float2 quotients(float2 y, const Divisor& a, const Divisor& b) {
+  const float2 rcp = make_float2(a.rcp, b.rcp);
+  const float2 z = __fmul2_rn(y, rcp);
+  return __ffma2_rn(__ffma2_rn(z, make_float2(a.minus_s, b.minus_s), y), rcp, z);
 }
 
 // ---- rows in groups of warps ------------------------------------------------------------
@@ -154,6 +172,7 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_fwd_rows_kernel(
     int64_t rows, int cols, float eps, int group_warps) {
   __shared__ float scratch[32];
   __shared__ uint32_t amax[!QUANT ? 1 : EDGE ? kQuantMaxBlocks + 1 : 32];  // of blocks or warps
+  __shared__ Divisor divisors[QUANT && EDGE ? kQuantMaxBlocks + 1 : 1];
   const int lane = threadIdx.x & 31, group = (threadIdx.x >> 5) / group_warps;
   const int in_group = threadIdx.x - group * group_warps * 32;
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x / (32 * group_warps)) + group;
@@ -216,7 +235,7 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_fwd_rows_kernel(
       m[i] = 0u;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        v[i][k] *= inv * wv[k];
+        v[i][k] = v[i][k] * inv * wv[k];
         m[i] = max(m[i], e < cols ? __float_as_uint(fabsf(v[i][k])) : 0u);
       }
       m[i] = __reduce_max_sync(0xffffffffu, m[i]);
@@ -231,9 +250,11 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_fwd_rows_kernel(
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int e = s.e(i);
-      const float sc = quant_scale(by_block ? m[i] : all), to = __fdiv_rn(1.0f, sc);
+      const float sc = quant_scale(by_block ? m[i] : all);
+      const Divisor by = divisor(sc);
       if (e < cols) {
-        *reinterpret_cast<uint32_t*>(qr + e) = to_e4m3x4(v[i][0] * to, v[i][1] * to, v[i][2] * to, v[i][3] * to);
+        *reinterpret_cast<uint32_t*>(qr + e) = to_e4m3x4(quotients(make_float2(v[i][0], v[i][1]), by, by),
+                                                         quotients(make_float2(v[i][2], v[i][3]), by, by));
         if (lane == 0 && (by_block || e == 0)) scale[by_block ? row * ((cols + 127) / 128) + e / 128 : row] = sc;
       }
     }
@@ -249,7 +270,7 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_fwd_rows_kernel(
       m[i] = 0u;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        v[i][k] *= inv * wv[k];
+        v[i][k] = v[i][k] * inv * wv[k];
         const bool in = e + k >= 0 && e + k < cols;
         const uint32_t u = in ? __float_as_uint(fabsf(v[i][k])) : 0u;
         if (lane == 0 && k < s.o) before = max(before, u);
@@ -263,11 +284,12 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_fwd_rows_kernel(
       }
     }
     group_sync(group, group_warps);
-    // each block's scale once; its reciprocal takes the maximum's place
+    // each block's scale and reciprocal once
+    Divisor* by = divisors + group * blocks;
     for (int b = in_group; b < blocks; b += 32 * group_warps) {
       const float sc = quant_scale(am[b]);
       scale[row * blocks + b] = sc;
-      am[b] = __float_as_uint(__fdiv_rn(1.0f, sc));
+      by[b] = divisor(sc);
     }
     group_sync(group, group_warps);
     uint8_t* qr = q + row * (int64_t)cols;
@@ -277,10 +299,10 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) add_rms_fwd_rows_kernel(
       if (e >= cols) continue;
       // at most two blocks meet in a vector
       const int b0 = max(e, 0) >> block_shift, b1 = min(e + 3, cols - 1) >> block_shift;
-      const float to0 = __uint_as_float(am[b0]), to1 = __uint_as_float(am[b1]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[i][k] *= (max(e + k, 0) >> block_shift) == b0 ? to0 : to1;
-      const uint32_t o = to_e4m3x4(v[i][0], v[i][1], v[i][2], v[i][3]);
+      const Divisor d0 = by[b0], d1 = by[b1];
+      auto of = [&](int k) { return (max(e + k, 0) >> block_shift) == b0 ? d0 : d1; };
+      const uint32_t o = to_e4m3x4(quotients(make_float2(v[i][0], v[i][1]), of(0), of(1)),
+                                   quotients(make_float2(v[i][2], v[i][3]), of(2), of(3)));
       if (!s.partial(e)) {
         *reinterpret_cast<uint32_t*>(qr + e) = o;
       } else {
@@ -499,7 +521,8 @@ __global__ void __launch_bounds__(1024) add_rms_fwd_kernel(
         if (e >= cols) continue;
         const int b = e >> block_shift;
         const float s = quant_scale(amax[b]);
-        q[out + e] = to_e4m3(v[i] * __fdiv_rn(1.0f, s));
+        const Divisor by = divisor(s);
+        q[out + e] = to_e4m3(quotients(make_float2(v[i], v[i]), by, by).x);
         if (e == b << block_shift) scale[row * blocks + b] = s;
       }
       __syncthreads();  // amax is read; the next row clears it

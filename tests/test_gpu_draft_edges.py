@@ -1,0 +1,44 @@
+"""The recurrent draft model's operators where they can go wrong: ties of the
+8-bit codes, the widest rows, variates of zero, NaN beside a sequence start,
+long teacher lists, derivatives that there are none of, and operands that do not
+fit each other.  Error bounds come from tests/draft_reference.py."""
+
+import numpy as np
+import pytest
+
+import draft_reference as R
+from test_gpu_draft import DTYPES, _check, _distill_inputs, _n, _norm_inputs, _scan_inputs, _t, _verify_inputs
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- add_rms_norm --------------------------------------------------------------------
+
+@pytest.mark.parametrize("block", [128, None])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,offset", [(24576, 1024, 0), (24576, 1001, 0), (24576, 1000, 1)])
+def test_add_rms_norm_quant_codes_are_quotients(rows, cols, offset, dtype, block):
+    """The code is y / scale, an f32 division, rounded to nearest even, with the y that
+    add_rms_norm_fwd gives: bit for bit, by vectors, by shifted vectors and by single
+    elements.  Of 24 million codes several lie within an f32 rounding of a tie."""
+    import torch
+    from oxitorch_b200 import functional as F
+    g = torch.Generator(device="cuda")
+    g.manual_seed(rows + cols + offset)
+
+    def rows_at(t):  # `offset` elements after an aligned address
+        wide = torch.empty(rows, cols + 4, device="cuda", dtype=t.dtype)
+        wide[:, offset:offset + cols] = t
+        return wide[:, offset:offset + cols]
+    x = rows_at(torch.randn(rows, cols, device="cuda", generator=g).to(getattr(torch, dtype)))
+    res = rows_at(torch.randn(rows, cols, device="cuda", generator=g) * 3)
+    w = torch.rand(cols, device="cuda", generator=g) + 0.5
+    q, scale, _ = F.add_rms_norm_quant(x, res, w, 1e-5, block=block)
+    y, _, _ = F.add_rms_norm_fwd(rows_at(x.float()), res, w, 1e-5)
+    b = block or cols
+    largest = torch.stack([v.abs().amax(-1) for v in y.split(b, -1)], -1)
+    want = (largest / torch.full_like(largest, R.E4M3_MAX)).clamp(min=2.0 ** -126)
+    assert torch.equal(scale, want)
+    codes = (y / want.repeat_interleave(b, -1)[:, :cols]).to(torch.float8_e4m3fn)
+    off = int((codes.view(torch.uint8) != q.view(torch.uint8)).sum())
+    assert off == 0, f"{off} codes of {codes.numel()}"
