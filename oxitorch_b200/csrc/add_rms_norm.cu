@@ -32,7 +32,7 @@
 // columns are not a multiple of 4, a row starts `o` = 0 to 3 elements after such an
 // address, the same in every tensor (row_shift); the row's first and last vectors
 // are then partial ones, read and written by element.  Tensors that differ in
-// that take the kernels for single elements.
+// that take the kernels for single elements, as do rows of 32766 and 32767 columns.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -591,6 +591,9 @@ __global__ void __launch_bounds__(1024) add_rms_bwd_kernel(
 struct GroupGeom {
   int vpt, warps, groups;
   int threads() const { return 32 * warps * groups; }
+  // 8 vectors a thread at most: all rows but those of 32766 and 32767 columns, whose
+  // shifts touch up to 8193 vectors (the single-element kernels hold them)
+  bool held() const { return vpt <= 8; }
 };
 static GroupGeom group_geom(int64_t cols, int vpt) {
   const int64_t slots = (cols + (cols % 4 ? 3 : 0) + 3) / 4;
@@ -650,8 +653,8 @@ static oxc_status add_rms_fwd_launch(const char* fn, const void* x, int64_t x_st
                                      uint8_t* q, float* scale, int block_shift, float* r,
                                      float* rstd, int64_t rows, int64_t cols, float eps,
                                      cudaStream_t s) {
-  if (row_shift<T>(x, x_stride, res, res_stride, cols, rows) && aligned16(w) && aligned16(r) &&
-      (QUANT ? aligned_to(q, 4) : aligned_to(y, 4 * sizeof(T)))) {
+  if (group_geom(cols, kFwdVecs).held() && row_shift<T>(x, x_stride, res, res_stride, cols, rows) &&
+      aligned16(w) && aligned16(r) && (QUANT ? aligned_to(q, 4) : aligned_to(y, 4 * sizeof(T)))) {
     const GroupGeom g = group_geom(cols, kFwdVecs);
     const int64_t grid = (rows + g.groups - 1) / g.groups;
     if (grid > 0x7fffffff)
@@ -694,8 +697,9 @@ static oxc_status add_rms_bwd_launch(const float* r, const float* w, const float
                                      int64_t rows, int64_t cols, int32_t mode, float* parts,
                                      cudaStream_t s) {
   const int64_t ctas = add_rms_bwd_ctas(rows, cols);
-  if (row_shift<T>(dy, dy_stride, dr, dr ? dr_stride : cols, cols, rows) && aligned16(r) &&
-      aligned16(w) && aligned16(dres) && (sizeof(T) == 4 || aligned_to(dx, 4 * sizeof(T)))) {
+  if (bwd_geom(cols).held() && row_shift<T>(dy, dy_stride, dr, dr ? dr_stride : cols, cols, rows) &&
+      aligned16(r) && aligned16(w) && aligned16(dres) &&
+      (sizeof(T) == 4 || aligned_to(dx, 4 * sizeof(T)))) {
     const GroupGeom g = bwd_geom(cols);
     const int period = cols % 4 == 0 ? 1 : cols % 2 == 0 ? 2 : 4;
     const bool edge = cols % 4 != 0, exact = mode == OXC_GRAD_EXACT;

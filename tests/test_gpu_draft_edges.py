@@ -42,3 +42,30 @@ def test_add_rms_norm_quant_codes_are_quotients(rows, cols, offset, dtype, block
     codes = (y / want.repeat_interleave(b, -1)[:, :cols]).to(torch.float8_e4m3fn)
     off = int((codes.view(torch.uint8) != q.view(torch.uint8)).sum())
     assert off == 0, f"{off} codes of {codes.numel()}"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [32763, 32765, 32766, 32767])
+def test_add_rms_norm_widest_rows(cols, dtype):
+    """Just under the limit: a row that starts 3 elements after an aligned address
+    touches 8193 vectors of 4."""
+    import torch
+    from oxitorch_b200 import functional as F
+    x, res, w, dy, dr = _norm_inputs(6, cols, dtype, seed=5)
+    want_y, _, _ = R.add_rms_norm(_n(x), _n(res), _n(w), 1e-5)
+    y, r, rstd = F.add_rms_norm_fwd(x, res, w, 1e-5)
+    _check(y, want_y, 56 * R.EPS * np.abs(want_y), "y")
+    assert (r == x.float() + res).all()
+    for mode in ("ref", "exact"):
+        dx, dres, dw = F.add_rms_norm_bwd(r, w, rstd, dy, dr, mode)
+        (d, want_dw), (bd, bdw) = R.add_rms_norm_grad(_n(x), _n(res), _n(w), 1e-5, _n(dy), _n(dr), mode == "exact")
+        _check(dres, d, bd, "dresidual")
+        _check(dx, d, bd, "dx")
+        _check(dw, want_dw, bdw, "dweight")
+    for block in (128, None):
+        q, scale, r = F.add_rms_norm_quant(x, res, w, 1e-5, block=block)
+        assert (r == x.float() + res).all()
+        want = R.block_scales(want_y, block)
+        _check(scale, want, 60 * R.EPS * want, "scale")
+        z = want_y / np.repeat(want, block or cols, -1)[:, :cols]
+        _check(q.to(torch.float32), z, R.e4m3_half_step(z) * (1 + 2.0 ** -10) + 120 * R.EPS * np.abs(z), "q")
