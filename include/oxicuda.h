@@ -701,9 +701,9 @@ oxc_status oxc_scale_by(void* x, int64_t n, int32_t dtype, const float* g, void*
  * 1, vocab], draft: [batch, drafted, vocab] (both with batch and place
  * strides; draft NULL = the drafted token had probability 1); tokens, lengths
  * (NULL = drafted): how many of tokens[b] count; uniform: [batch, drafted] in
- * [0, 1); race: [batch, vocab] exponential variates, positive (a zero wins
- * whatever its weight).  Token k is kept while
- * uniform * q < p; out_tokens [batch, drafted + 1] gets the kept tokens, then
+ * [0, 1); race: [batch, vocab] exponential variates (one of zero makes the
+ * quotient of a positive weight infinite; a token without weight is never
+ * chosen).  Token k is kept while uniform * q < p; out_tokens [batch, drafted + 1] gets the kept tokens, then
  * argmax max(p - q, 0) / race at the first one not kept (p / race after the
  * last), then -1; accepted[b] is how many were kept.  A token outside [0,
  * vocab) is recorded in err_flag and not kept. */

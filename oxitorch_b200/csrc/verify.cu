@@ -20,7 +20,7 @@
 // of up to 8 CTAs shares a sequence, so that few sequences still use many SMs;
 // every CTA works the acceptance out for itself (a few dozen loads) and the
 // argmax's keys meet in distributed shared memory.  Measured: 256 sequences of
-// 131072 entries 71 us (86% of the copy bandwidth), 64 of them 25 us (61%), where
+// 131072 entries 65 us (94% of the copy bandwidth), 64 of them 24 us (64%), where
 // the launch, the acceptance and the meeting are not hidden by other sequences.
 #include <cooperative_groups.h>
 
@@ -38,41 +38,20 @@ __device__ __forceinline__ void record_bad_token(int32_t* flag, int64_t id, int6
   }
 }
 
-// The best of a set of tokens.  A key is the quotient's bits above the index's
-// complement, so the largest key is the largest quotient at the lowest index; 0 is
-// none (any other has a nonzero low half).  zero: of the quotients 0 / 0, by index
-// alone; they count only if some weight is positive.
-struct Race {
-  unsigned long long key = 0ull;
-  uint32_t zero = 0u;
-  __device__ __forceinline__ void add(float w, float e, uint32_t v) {
-    const uint32_t low = 0xffffffffu - v;
-    if (w > 0.0f) {
-      const float s = __fdiv_rn(w, e);
-      if (s == s) key = max(key, ((unsigned long long)__float_as_uint(s) << 32) | low);
-    } else if (e == 0.0f && w <= 0.0f) {
-      zero = max(zero, low);
-    }
-  }
-  __device__ __forceinline__ void merge(const Race& o) {
-    key = max(key, o.key);
-    zero = max(zero, o.zero);
-  }
-  __device__ __forceinline__ bool found() const { return key != 0ull; }
-  __device__ __forceinline__ int64_t token() const {
-    return found() ? (int64_t)(0xffffffffu - (zero ? zero : (uint32_t)key)) : -1;
-  }
-};
+// w / e as an ordered key with the index's complement below it, so the largest
+// key is the largest quotient at the lowest index; 0 for no weight or a NaN (any
+// other key has a nonzero low half).  A variate of zero gives a positive weight an
+// infinite quotient; a token without weight never wins, whatever its variate.
+__device__ __forceinline__ unsigned long long race_key(float w, float e, uint32_t v) {
+  if (!(w > 0.0f)) return 0ull;
+  const float s = __fdiv_rn(w, e);
+  return s >= 0.0f ? ((unsigned long long)__float_as_uint(s) << 32) | (0xffffffffu - v) : 0ull;
+}
 
-__device__ __forceinline__ Race warp_merge(Race r) {
+__device__ __forceinline__ unsigned long long warp_max_key(unsigned long long k) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Race other;
-    other.key = __shfl_xor_sync(0xffffffffu, r.key, o);
-    other.zero = __shfl_xor_sync(0xffffffffu, r.zero, o);
-    r.merge(other);
-  }
-  return r;
+  for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
+  return k;
 }
 
 constexpr int kVerifyCluster = 8;
@@ -80,20 +59,21 @@ constexpr int kVerifyCluster = 8;
 // more at 64 x 131072).
 constexpr int kVerifyCtas = 4;
 
-// The best of the vocabulary entries [v0, v1) with weights p - q (q may be null;
+// The largest key of the vocabulary entries [v0, v1) with weights p - q (q may be null;
 // token x counts 0).  The rows start anywhere: vectors where their addresses agree
 // modulo 16 bytes, else single entries.
 template <int THREADS>
-__device__ __forceinline__ Race race_best(const float* p, const float* q,
-                                          const float* e, int64_t x, int64_t v0, int64_t v1) {
-  Race k;
+__device__ __forceinline__ unsigned long long race_best(const float* p, const float* q,
+                                                        const float* e, int64_t x, int64_t v0,
+                                                        int64_t v1) {
+  unsigned long long k = 0ull;
   p += v0;
   e += v0;
   if (q) q += v0;
   const uint32_t n = (uint32_t)(v1 - v0);
   const int64_t own = x - v0;
   auto one = [&](float pv, float qv, float ev, uint32_t at) {
-    k.add(at == own ? 0.0f : __fsub_rn(pv, qv), ev, (uint32_t)(v0 + at));
+    k = max(k, race_key(at == own ? 0.0f : __fsub_rn(pv, qv), ev, (uint32_t)(v0 + at)));
   };
   const uintptr_t o = reinterpret_cast<uintptr_t>(p) & 15;
   if (o == (reinterpret_cast<uintptr_t>(e) & 15) && (!q || o == (reinterpret_cast<uintptr_t>(q) & 15))) {
@@ -149,8 +129,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(
     int64_t* __restrict__ accepted, int32_t* err) {
   namespace cg = cooperative_groups;
   constexpr int kWarps = THREADS / 32;
-  __shared__ unsigned long long best_key[kWarps], mine_key[2];
-  __shared__ uint32_t best_zero[kWarps], mine_zero[2];
+  __shared__ unsigned long long best[kWarps], mine[2];
   __shared__ int first;
   cg::cluster_group cluster = cg::this_cluster();
   const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -179,34 +158,27 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(
   // this CTA's entries: a share in multiples of 4
   const int64_t each = ((vocab + size - 1) / size + 3) & ~(int64_t)3;
   const int64_t v0 = min(vocab, rank * each), v1 = min(vocab, v0 + each);
-  Race k;
+  unsigned long long k = 0ull;
   for (int pass = 0; pass < 2; ++pass) {  // the second from p alone, if nothing was left
     const bool beyond = pass == 0 && j < n;
     k = race_best<THREADS>(p, beyond && draft ? draft + b * d_sb + j * d_sk : nullptr, e,
                   beyond && !draft ? tok[j] : -1, v0, v1);
-    k = warp_merge(k);
+    k = warp_max_key(k);
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) {
-      best_key[threadIdx.x >> 5] = k.key;
-      best_zero[threadIdx.x >> 5] = k.zero;
-    }
+    if ((threadIdx.x & 31) == 0) best[threadIdx.x >> 5] = k;
     __syncthreads();
-    k = Race();
-    for (int w = 0; w < kWarps; ++w) k.merge({best_key[w], best_zero[w]});
+    k = 0ull;
+    for (int w = 0; w < kWarps; ++w) k = max(k, best[w]);
     if (size > 1) {
-      if (threadIdx.x == 0) {
-        mine_key[pass] = k.key;
-        mine_zero[pass] = k.zero;
-      }
+      if (threadIdx.x == 0) mine[pass] = k;
       cluster.sync();
-      k = Race();
-      for (int r = 0; r < size; ++r)
-        k.merge({*cluster.map_shared_rank(&mine_key[pass], r), *cluster.map_shared_rank(&mine_zero[pass], r)});
+      k = 0ull;
+      for (int r = 0; r < size; ++r) k = max(k, *cluster.map_shared_rank(&mine[pass], r));
     }
-    if (k.found() || j == n) break;  // (the same in every CTA)
+    if (k != 0ull || j == n) break;  // (the same in every CTA)
   }
   if (rank == 0) {
-    const int64_t next = k.token();
+    const int64_t next = k ? (int64_t)(0xffffffffu - (uint32_t)k) : -1;
     for (int i = threadIdx.x; i <= drafted; i += THREADS)
       out_tokens[b * (drafted + 1) + i] = i < j ? tok[i] : i == j ? next : -1;
     if (threadIdx.x == 0) accepted[b] = j;

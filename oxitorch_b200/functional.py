@@ -914,9 +914,9 @@ def verify_draft(target, draft, tokens, uniform, race, lengths=None, flag=None):
     accepted[b] kept tokens, then the token sampled after them as the first
     argmax of max(p - q, 0) / race[b] (p / race[b] when all were kept or nothing
     is left), then -1.  uniform [batch, drafted] is in [0, 1); race [batch,
-    vocab] holds exponential variates, which are positive (a zero would win its
-    race whatever its weight).  Tokens outside the vocabulary are not
-    kept, and recorded in ``flag`` (int32[4], zeroed by the caller) if given."""
+    vocab] holds exponential variates (one of zero makes the quotient of a
+    positive weight infinite; a token without weight is never chosen).  Tokens
+    outside the vocabulary are not kept, and recorded in ``flag`` (int32[4], zeroed by the caller) if given."""
     _require_cuda_f32("target", target)
     _dtype_id("target", target)
     if target.dim() != 3 or target.shape[1] < 1:

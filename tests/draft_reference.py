@@ -187,8 +187,7 @@ def verify(target, draft, tokens, uniform, race, lengths=None):
                 score = np.where(weights > 0, weights / race[b], -1.0)
             score = np.where(np.isnan(score), -1.0, score)
             if score.max() >= 0:
-                none = (weights <= 0) & (race[b] == 0)  # 0 / 0 ranks first, as argmax has it
-                out[b, j] = int(none.argmax()) if none.any() else int(score.argmax())
+                out[b, j] = int(score.argmax())
                 break
         accepted[b] = j
     return out, accepted

@@ -69,3 +69,32 @@ def test_add_rms_norm_widest_rows(cols, dtype):
         _check(scale, want, 60 * R.EPS * want, "scale")
         z = want_y / np.repeat(want, block or cols, -1)[:, :cols]
         _check(q.to(torch.float32), z, R.e4m3_half_step(z) * (1 + 2.0 ** -10) + 120 * R.EPS * np.abs(z), "q")
+
+
+# ---- verify_draft --------------------------------------------------------------------
+
+@pytest.mark.parametrize("B,V", [(40, 50), (3, 40003), (200, 20004)])
+def test_verify_draft_zero_variates_pick_no_token_without_weight(B, V):
+    """A variate of zero gives a positive weight an infinite quotient and a weight of
+    zero nothing: the token after the kept ones always has weight."""
+    import torch
+    from oxitorch_b200 import functional as F
+    p, q, tokens, u, e, lengths = _verify_inputs(B, 2, V, seed=9)
+    g = np.random.default_rng(B + V)
+    e[g.random((B, V)) < 4 / V] = 0.0
+    e[0], e[1, : V // 2] = 0.0, 0.0
+    for draft in (q, None):
+        dev = [None if a is None else torch.from_numpy(np.array(a)).cuda() for a in (p, draft, tokens, u, e, lengths)]
+        out, accepted = (a.cpu().numpy() for a in F.verify_draft(*dev))
+        for b in range(B):
+            n, j = int(lengths[b]), int(accepted[b])
+            w = p[b, j].copy()
+            if j < n and draft is not None:
+                w = p[b, j] - q[b, j]
+            elif j < n:
+                w[tokens[b, j]] = 0.0
+            some = w > 0
+            assert some.any()
+            with np.errstate(divide="ignore", invalid="ignore"):
+                score = np.where(some, w / e[b], -1.0)
+            assert out[b, j] == score.argmax() and w[out[b, j]] > 0
