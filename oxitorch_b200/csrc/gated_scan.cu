@@ -35,8 +35,8 @@
 // fixed sequence of operations -- whoever computes it, from however far back --
 // the results do not depend on timing.
 //
-// Bound by HBM in f32: [4, 2048, 4096] 75 us forward (82% of the copy bandwidth), 122
-// us VJP (84%).  At 16 bits half the bytes leave the waits for the chain and the
+// Bound by HBM in f32: [4, 2048, 4096] 75 us forward (82% of the copy bandwidth), 125
+// us VJP (82%).  At 16 bits half the bytes leave the waits for the chain and the
 // issue of instructions in sight: 66 and 91 us (46%, 57%), and [1, 65537, 1024], 1025
 // chunks in a row, 141 and 197 us (44%, 52%).
 #include <algorithm>
@@ -102,6 +102,13 @@ __device__ __forceinline__ void gate_pair(float2 g, float2& a, float2& b) {
 // map that forgets its argument (a sequence starts inside): it is selected, not
 // multiplied, and keeps its mark in compositions.
 __device__ __forceinline__ bool forgets(float A) { return __float_as_uint(A) == 0x80000000u; }
+// Sets the mark once a warp's tokens are composed: a NaN gate among them would have
+// turned it into a NaN, and mu would reach the sequence before.
+template <int P>
+__device__ __forceinline__ void mark_forgets(float2 (&A)[P]) {
+#pragma unroll
+  for (int j = 0; j < P; ++j) A[j] = f2(-0.0f);
+}
 __device__ __forceinline__ float map_apply(float A, float H, float s) {
   return forgets(A) ? H : fmaf(A, s, H);
 }
@@ -582,8 +589,9 @@ __global__ void __launch_bounds__(kScanWarps * 32, kScanCtas) scan_fwd_kernel(
           for (int k = 0; k < P; ++k) {
             H[k] = __ffma2_rn(a[i][k], H[k], v[i][k]);
             A[k] = __fmul2_rn(A[k], a[i][k]);
-            if (decltype(some)::value && ((fresh[half] >> i) & 1u)) { H[k] = v[i][k]; A[k] = f2(-0.0f); }
+            if (decltype(some)::value && ((fresh[half] >> i) & 1u)) H[k] = v[i][k];
           }
+        if (decltype(some)::value) mark_forgets(A);
       });
       lane.put(mapA[half * kScanWarps + warp], A);
       lane.put(mapH[half * kScanWarps + warp], H);
@@ -789,9 +797,10 @@ __global__ void __launch_bounds__(kScanWarps * 32, kScanCtas) scan_bwd_kernel(
           const float2 v = __fmul2_rn(b[i][j], xi[j]);
           S[j] = __ffma2_rn(a[i][j], S[j], v);
           A[j] = __fmul2_rn(A[j], a[i][j]);
-          if (decltype(some)::value && ((fresh >> i) & 1u)) { S[j] = v; A[j] = f2(-0.0f); }
+          if (decltype(some)::value && ((fresh >> i) & 1u)) S[j] = v;
         }
       }
+      if (decltype(some)::value) mark_forgets(A);
 #pragma unroll
       for (int i = kScanSteps - 1; i >= 0; --i) {
         float2 di[P];

@@ -98,3 +98,34 @@ def test_verify_draft_zero_variates_pick_no_token_without_weight(B, V):
             with np.errstate(divide="ignore", invalid="ignore"):
                 score = np.where(some, w / e[b], -1.0)
             assert out[b, j] == score.argmax() and w[out[b, j]] > 0
+
+
+# ---- gated_scan ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [72, 130, 256])
+def test_gated_scan_starts_stop_a_nan_gate(D, dtype):
+    """A NaN gate at a start or at one of the tokens after it, in the same warp's eight
+    tokens, the same chunk or a later one, does not reach what lies before the start."""
+    import torch
+    from oxitorch_b200 import functional as F
+    T = 300
+    x, gate, h0, dh, dlast, _ = _scan_inputs(1, T, D, dtype)
+    for new in (1, 64, 130, 255):
+        starts = torch.zeros(1, T, dtype=torch.bool, device="cuda")
+        starts[:, new] = True
+        (wx, wg, w0), (bx, bg, b0) = R.gated_scan_grad(_n(x)[:, :new], _n(gate)[:, :new], _n(h0), None,
+                                                       _n(dh)[:, :new], None)
+        want, _, bound = R.gated_scan(_n(x)[:, :new], _n(gate)[:, :new], _n(h0))
+        for after in (0, 1, 2, 5, 6, 7, 11, 40):
+            bad = gate.clone()
+            bad[:, new + after] = float("nan")
+            leaves = [t.clone().requires_grad_() for t in (x, bad, h0)]
+            h, last = F.gated_scan(*leaves, starts)
+            dx, dg, dh0 = torch.autograd.grad((h, last), leaves, (dh, dlast))
+            where = f"NaN {after} after the start at {new}"
+            _check(h[:, :new], want, bound, "h, " + where)
+            assert torch.isnan(h[:, new + after:].float()).all() and torch.isnan(last).all()
+            _check(dx[:, :new], wx, bx, "dx, " + where)
+            _check(dg[:, :new], wg, bg, "dgate, " + where)
+            _check(dh0, w0, b0, "dh0, " + where)
