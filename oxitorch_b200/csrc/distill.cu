@@ -13,11 +13,11 @@
 // Bound by HBM: 2 sizeof(T) bytes a logit, the row read once and its gradient
 // written once.  So a row stays in shared memory between the two, shared by a
 // cluster of 1 to 8 CTAs that exchange (max, sum) pairs through distributed shared
-// memory.  Rows wider than a cluster holds (1.25 MB) take the three-pass kernel,
-// which re-reads them from L2 or HBM.  Measured, of the copy bandwidth: f32 [4096,
-// 131072] 701 us (94%), [8192, 32000] 364 (88%); bf16 [8192, 32000] 204 (78%), [8192,
-// 131072] 863 (76%), where the issue of instructions and the exponentials are as
-// busy as the memory.
+// memory.  Rows wider than a cluster holds (1.25 MB; 1.13 MB beside the 80 KB of 4096
+// entries) take the three-pass kernel, which re-reads them from L2 or HBM.  Measured,
+// of the copy bandwidth: f32 [4096, 131072] 701 us (94%), [8192, 32000] 364 (88%); bf16
+// [8192, 32000] 204 (78%), [8192, 131072] 863 (76%), where the issue of instructions
+// and the exponentials are as busy as the memory.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -33,6 +33,8 @@ constexpr int kDistillThreads = 256;          // per CTA at most
 constexpr int kDistillCopies = 4;             // bulk copies per part of a row
 constexpr int kDistillPart = 100 * 1024;      // bytes of a row per CTA, if a cluster can
 constexpr int kDistillMaxPart = 160 * 1024;   // and at most
+constexpr int kDistillSmem = 225 * 1024;      // a part and the teacher's side: the 227 KB
+                                              // that a CTA can have, less the kernel's own
 constexpr int kDistillCluster = OXC_DISTILL_PARTS;  // CTAs per row at most
 
 // Records the first bad id: flag[0] = 2 (dim 1), flag[1..2] = id, flag[3] = vocab.
@@ -586,12 +588,14 @@ __global__ void __launch_bounds__(256) scale_by_kernel(T* __restrict__ x, int64_
 }
 
 // CTAs per row: parts of up to 100 KB, two or more resident on an SM, as long as a
-// cluster of 8 holds the row, larger ones beyond; 0 if they would be too large.
+// cluster of 8 holds the row, larger ones beyond; 0 if they would be too large, by
+// themselves or beside the `teacher` bytes of a long list.
 // More CTAs than the row needs while that leaves SMs idle and each has some work.
-static int distill_cluster(int64_t rows, int64_t bytes) {
+static int distill_cluster(int64_t rows, int64_t bytes, int64_t teacher) {
   int size = 1;
   while (size < kDistillCluster && bytes > (int64_t)size * kDistillPart) size *= 2;
   if (bytes > (int64_t)size * kDistillMaxPart) return 0;
+  if (bytes / size + 16 + teacher > kDistillSmem) return 0;
   while (size < kDistillCluster && rows * size * 2 <= sm_count() &&
          bytes >= (int64_t)size * 2 * kDistillThreads * 16)
     size *= 2;
@@ -603,7 +607,7 @@ static oxc_status distill_launch(const void* logits, int64_t stride, void* dlogi
                                  const DistillArgs& a, int* losses, cudaStream_t s) {
   const T* x = static_cast<const T*>(logits);
   T* d = static_cast<T*>(dlogits);
-  const int size = distill_cluster(a.rows, (int64_t)a.vocab * sizeof(T));
+  const int size = distill_cluster(a.rows, (int64_t)a.vocab * sizeof(T), teacher_smem(a.top));
   // the largest part: its share of the row's vectors
   const int vecs = a.vocab / (16 / (int)sizeof(T)), part = size ? 16 * ((vecs + size - 1) / size) : 0;
   const size_t smem = teacher_smem(a.top) + part;

@@ -129,3 +129,24 @@ def test_gated_scan_starts_stop_a_nan_gate(D, dtype):
             _check(dx[:, :new], wx, bx, "dx, " + where)
             _check(dg[:, :new], wg, bg, "dgate, " + where)
             _check(dh0, w0, b0, "dh0, " + where)
+
+
+# ---- distill_loss --------------------------------------------------------------------
+
+def _distill_against_reference(logits, teacher, ids, tau):
+    import torch
+    from oxitorch_b200 import functional as F
+    leaf = logits.detach().requires_grad_()
+    loss = F.distill_loss(leaf, teacher, ids, tau)
+    (grad,) = torch.autograd.grad(loss, leaf)
+    want = R.distill(_n(logits), _n(teacher), ids.cpu().numpy(), tau)
+    _check(loss, want[0], want[2], "loss")
+    _check(grad, want[1], want[3], "dlogits")
+
+
+@pytest.mark.parametrize("dtype,vocab", [("float32", 290000), ("float32", 300000), ("float32", 320000),
+                                         ("float32", 327680), ("bfloat16", 600000), ("bfloat16", 650000)])
+def test_distill_loss_long_teacher_lists_beside_wide_rows(dtype, vocab):
+    """The longest lists take 80 KB of shared memory beside a row's part of up to 160 KB."""
+    for top in (2900, 4096):
+        _distill_against_reference(*_distill_inputs(2, vocab, top, dtype), 1.0)
