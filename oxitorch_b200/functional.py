@@ -20,6 +20,7 @@ mathematical gradient.
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 import ctypes
@@ -536,7 +537,8 @@ def swiglu(gate, up):
 # no counterpart.  Activations and logits may be float32 or bfloat16; the
 # residual stream, weights, recurrent states, scales and probabilities are
 # float32, and so is all arithmetic (a bfloat16 result is rounded once).  Their
-# gradients cannot be differentiated again; torch refuses to.
+# gradients cannot be differentiated again, and none has a forward-mode derivative:
+# either is refused.
 
 _DTYPES = {torch.float32: N.F32, torch.bfloat16: N.BF16}
 
@@ -591,6 +593,13 @@ def _rows2d(t):
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _has_tangent(*tensors):
+    """Whether forward-mode differentiation runs through one of them.  Then a call goes
+    through its autograd function, which refuses, or refuses itself: the kernels would
+    drop the tangent, and a missing one counts as zero."""
+    return any(isinstance(t, torch.Tensor) and unpack_dual(t).tangent is not None for t in tensors)
 
 
 # ---- residual addition + RMSNorm ---------------------------------------------------------
@@ -687,6 +696,8 @@ def add_rms_norm_quant(x, residual, weight, eps=1e-6, block=128):
     dt, x2, res2, w = _add_rms_args(x, residual, weight)
     if block not in (128, None):
         raise ValueError(f"invalid argument: block must be 128 or None, got {block}")
+    if _has_tangent(x, residual, weight):
+        raise ValueError("invalid argument: add_rms_norm_quant has no derivative; train with add_rms_norm")
     rows, cols = x2.shape
     blocks = -(-cols // block) if block else 1
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
@@ -794,7 +805,8 @@ def gated_scan(x, gate, h0=None, starts=None):
     None) and last are float32.  ``starts`` (bool [batch, length]) marks where a
     new sequence begins in a packed row: the state before such a token is zero."""
     grads = (x, gate) if h0 is None else (x, gate, h0)
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in grads):
+    if (torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in grads)
+            or _has_tangent(*grads)):
         return _GatedScan.apply(x, gate, h0, starts)
     return gated_scan_fwd(x, gate, h0, starts, save=False)[:2]
 
@@ -816,7 +828,8 @@ def gated_step(x, gate, state, out=None):
         raise ValueError("invalid argument: state and out must be contiguous")
     if 0 < abs(out.data_ptr() - state.data_ptr()) < 4 * state.numel():
         raise ValueError("invalid argument: out must be state or not overlap it")
-    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad):
+    if (torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad)
+            or _has_tangent(x, gate, state)):
         raise ValueError("invalid argument: gated_step has no gradient; train with gated_scan")
     x, gate = _rows2d(x), _rows2d(gate)
     h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -895,7 +908,8 @@ def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, total_row
     mean and has a zero gradient.  An id >= vocab makes the loss NaN.
     total_rows: the divisor of the mean (the rows of this call if None), as in
     a sharded batch.  The gradient reaches logits only."""
-    if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
+    if (torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad
+            or _has_tangent(logits, teacher_logits)):
         return _DistillLoss.apply(logits, teacher_logits, teacher_ids, temperature, total_rows)
     return distill_loss_fwd(logits, teacher_logits, teacher_ids, temperature, total_rows,
                             grad=False)[0].reshape(())

@@ -150,3 +150,29 @@ def test_distill_loss_long_teacher_lists_beside_wide_rows(dtype, vocab):
     """The longest lists take 80 KB of shared memory beside a row's part of up to 160 KB."""
     for top in (2900, 4096):
         _distill_against_reference(*_distill_inputs(2, vocab, top, dtype), 1.0)
+
+
+# ---- derivatives ---------------------------------------------------------------------
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent that would be dropped is an error, whether or not the tensor also wants
+    a gradient."""
+    import torch
+    import torch.autograd.forward_ad as fwAD
+    from oxitorch_b200 import functional as F
+    x, t = torch.randn(2, 4, 8, device="cuda"), torch.randn(2, 4, 8, device="cuda")
+    h0, ones = torch.zeros(2, 8, device="cuda"), torch.ones(8, device="cuda")
+    tl, ti = torch.zeros(2, 4, 2, device="cuda"), torch.arange(2, device="cuda").expand(2, 4, 2)
+    with fwAD.dual_level():
+        d, d0, dl = fwAD.make_dual(x, t), fwAD.make_dual(h0, h0.clone()), fwAD.make_dual(tl, tl.clone())
+        for call in (lambda: F.gated_scan(d, x), lambda: F.gated_scan(x, d), lambda: F.gated_scan(x, x, d0),
+                     lambda: F.distill_loss(d, tl, ti), lambda: F.distill_loss(x, dl, ti),
+                     lambda: F.gated_step(d[:, 0], x[:, 0], h0), lambda: F.gated_step(x[:, 0], x[:, 0], d0),
+                     lambda: F.add_rms_norm(d, x, ones), lambda: F.add_rms_norm_quant(x, d, ones)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises((RuntimeError, ValueError)):
+                    call()
+        # without a tangent nothing is refused inside a level
+        F.gated_scan(x, x, h0)
+        F.distill_loss(x, tl, ti)
+        F.gated_step(x[:, 0], x[:, 0], h0)
