@@ -692,12 +692,14 @@ def add_rms_norm_quant(x, residual, weight, eps=1e-6, block=128):
     Each row is cut into blocks of 128 columns (``block=None``: one block a
     row); scale [..., blocks] is max(amax(|y|) / 448, 2^-126) of a block and q,
     of type float8_e4m3fn, is y / scale rounded to nearest, so y is q * scale.
-    For inference: it has no gradient."""
+    For inference: it has no gradient, and where one is recorded an argument that
+    requires it is refused (r would be cut from it)."""
     dt, x2, res2, w = _add_rms_args(x, residual, weight)
     if block not in (128, None):
         raise ValueError(f"invalid argument: block must be 128 or None, got {block}")
-    if _has_tangent(x, residual, weight):
-        raise ValueError("invalid argument: add_rms_norm_quant has no derivative; train with add_rms_norm")
+    if (torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or weight.requires_grad)
+            or _has_tangent(x, residual, weight)):
+        raise ValueError("invalid argument: add_rms_norm_quant has no gradient; train with add_rms_norm")
     rows, cols = x2.shape
     blocks = -(-cols // block) if block else 1
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)

@@ -176,3 +176,18 @@ def test_forward_mode_derivatives_are_refused():
         F.gated_scan(x, x, h0)
         F.distill_loss(x, tl, ti)
         F.gated_step(x[:, 0], x[:, 0], h0)
+
+
+def test_add_rms_norm_quant_refuses_to_cut_a_gradient():
+    """Its outputs have no gradient, the residual stream among them."""
+    import torch
+    from oxitorch_b200 import functional as F
+    x, w = torch.randn(3, 8, device="cuda"), torch.ones(8, device="cuda")
+    for at in range(3):
+        args = [x, x, w]
+        args[at] = args[at].clone().requires_grad_()
+        with pytest.raises(ValueError, match="gradient"):
+            F.add_rms_norm_quant(*args)
+        with torch.no_grad():
+            q, scale, r = F.add_rms_norm_quant(*args)
+        assert not r.requires_grad
