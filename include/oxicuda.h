@@ -619,7 +619,7 @@ oxc_status oxc_layer_norm_bwd_noalloc(const float* x, const float* w, const floa
  * tokens for it.  Where `dtype` appears, the void* tensors hold float32
  * (OXC_F32) or bfloat16 (OXC_BF16) elements; everything declared float* is
  * float32 either way, and all arithmetic is f32 with one rounding to the
- * tensor's type.  Strides are in elements; the last dim is dense. */
+ * tensor's type per call.  Strides are in elements; the last dim is dense. */
 #define OXC_F32 0
 #define OXC_BF16 1
 
@@ -694,7 +694,8 @@ oxc_status oxc_distill_loss(const void* logits, int64_t logits_stride, const flo
                             int64_t rows, int64_t vocab, int64_t total_rows, int32_t dtype,
                             int32_t* err_flag, void* stream);
 /* x[0..n) *= g[0] in place, g on the device; reads and writes nothing of x when
- * g[0] is 1. */
+ * g[0] is 1.  A bf16 x is rounded again (exact for powers of two); where the factor
+ * is known in time, grad_loss above scales before the only rounding. */
 oxc_status oxc_scale_by(void* x, int64_t n, int32_t dtype, const float* g, void* stream);
 
 /* Verification of drafted tokens.  target: f32 probabilities [batch, drafted +

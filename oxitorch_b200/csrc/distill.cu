@@ -576,7 +576,9 @@ __global__ void __launch_bounds__(1024) distill_loss_kernel(const float* __restr
   if (threadIdx.x == 0) loss[0] = (float)(sum * scale);
 }
 
-// x *= g[0]; nothing to do, and nothing read, when g[0] is 1.
+// x *= g[0]; nothing to do, and nothing read, when g[0] is 1.  A bf16 gradient is
+// rounded a second time here, 2^-9 relative at most: kept for the pass over the logits
+// that a factor known only in backward would otherwise cost.
 template <typename T>
 __global__ void __launch_bounds__(256) scale_by_kernel(T* __restrict__ x, int64_t n,
                                                        const float* __restrict__ g) {

@@ -536,9 +536,10 @@ def swiglu(gate, up):
 # distilled from a larger one and then drafts tokens for it.  The reference has
 # no counterpart.  Activations and logits may be float32 or bfloat16; the
 # residual stream, weights, recurrent states, scales and probabilities are
-# float32, and so is all arithmetic (a bfloat16 result is rounded once).  Their
-# gradients cannot be differentiated again, and none has a forward-mode derivative:
-# either is refused.
+# float32, and so is all arithmetic (a bfloat16 result is rounded once; the gradient
+# of distill_loss a second time by a factor on the loss).  Their gradients cannot
+# be differentiated again, and none has a forward-mode derivative: either is
+# refused.
 
 _DTYPES = {torch.float32: N.F32, torch.bfloat16: N.BF16}
 
@@ -875,7 +876,10 @@ def distill_loss_fwd(logits, teacher_logits, teacher_ids, temperature=1.0, total
 class _DistillLoss(torch.autograd.Function):
     """The forward pass leaves the gradient for a loss gradient of 1; backward
     hands it out, scaled in place on the device if it is another.  A second
-    backward (retain_graph) computes it again."""
+    backward (retain_graph) computes it again and scales it likewise, so that the
+    bits do not depend on which one asks.  In bfloat16 a factor that is no power of
+    two rounds the gradient a second time, by up to half a unit in its last place:
+    the first rounding came before the factor was known."""
 
     @staticmethod
     def forward(ctx, logits, teacher_logits, teacher_ids, temperature, total_rows):
@@ -891,10 +895,9 @@ class _DistillLoss(torch.autograd.Function):
             g = g.to(torch.float32)
         d, ctx.dlogits = ctx.dlogits, None
         if d is None:
-            d = distill_loss_fwd(*ctx.saved_tensors, *ctx.args, grad_loss=g)[1]
-        else:
-            N.check(N.load().oxc_scale_by(d.data_ptr(), d.numel(), _DTYPES[d.dtype], g.data_ptr(),
-                                          _stream()), "distill_loss backward")
+            d = distill_loss_fwd(*ctx.saved_tensors, *ctx.args)[1]
+        N.check(N.load().oxc_scale_by(d.data_ptr(), d.numel(), _DTYPES[d.dtype], g.data_ptr(),
+                                      _stream()), "distill_loss backward")
         return d, None, None, None, None
 
 
@@ -909,7 +912,8 @@ def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, total_row
     negative id or a -inf logit is absent; a row without entries adds 0 to the
     mean and has a zero gradient.  An id >= vocab makes the loss NaN.
     total_rows: the divisor of the mean (the rows of this call if None), as in
-    a sharded batch.  The gradient reaches logits only."""
+    a sharded batch.  The gradient reaches logits only; in bfloat16 it is rounded
+    for a factor of 1 on the loss and again when another one scales it."""
     if (torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad
             or _has_tangent(logits, teacher_logits)):
         return _DistillLoss.apply(logits, teacher_logits, teacher_ids, temperature, total_rows)

@@ -191,3 +191,26 @@ def test_add_rms_norm_quant_refuses_to_cut_a_gradient():
         with torch.no_grad():
             q, scale, r = F.add_rms_norm_quant(*args)
         assert not r.requires_grad
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("factor", [3.0, 0.1, -0.7])
+def test_distill_loss_gradient_is_the_same_whichever_backward_asks(dtype, factor):
+    """The factor on the loss gives the same bits in the first backward and in later
+    ones, within its own rounding of the gradient for a factor of 1."""
+    import torch
+    from oxitorch_b200 import functional as F
+    logits, teacher, ids = _distill_inputs(9, 1003, 12, dtype)
+    leaf = logits.detach().requires_grad_()
+    loss = F.distill_loss(leaf, teacher, ids, 2.0)
+    (first,) = torch.autograd.grad(factor * loss, leaf, retain_graph=True)
+    (second,) = torch.autograd.grad(factor * loss, leaf, retain_graph=True)
+    (one,) = torch.autograd.grad(loss, leaf, retain_graph=True)
+    (third,) = torch.autograd.grad(factor * loss, leaf)
+    assert torch.equal(first, second) and torch.equal(first, third)
+    _, want, _, bound = R.distill(_n(logits), _n(teacher), ids.cpu().numpy(), 2.0)
+    _check(one, want, bound, "factor 1")
+    f = float(np.float32(factor))
+    # the rounding for a factor of 1, times the factor, and (in _check) the second one
+    once = 2.0 ** -8 * (np.abs(want) + bound) if dtype == "bfloat16" else R.EPS * np.abs(want)
+    _check(first, f * want, abs(f) * (bound + once + 2.0 ** -133), "factor")
