@@ -756,9 +756,16 @@ def gated_scan_fwd(x, gate, h0=None, starts=None, save=True):
 
 def gated_scan_bwd(x, gate, carry, dh=None, dlast=None, starts=None):
     """Returns (dx, dgate, dh0) for the gradients of h and of the last state
-    (None = zero)."""
+    (None = zero); carry is gated_scan_fwd's for the same shape."""
     dt = _dtype_id("x", x)
+    if x.dim() != 3:
+        raise ValueError(f"invalid argument: gated_scan expects [batch, length, dim], got {list(x.shape)}")
     B, T, D = x.shape
+    L = N.load()
+    _operand("gate", gate, x.shape, x.dtype, x.device)
+    _operand("carry", carry, (L.oxc_gated_scan_carry_size(B, T, D),), torch.float32, x.device)
+    if not carry.is_contiguous():
+        raise ValueError("invalid argument: carry must be contiguous")
     x, gate, starts = _sequence(x), _sequence(gate), _starts_tensor(starts, x)
     if dh is not None:
         _operand("dh", dh, x.shape, x.dtype, x.device)
@@ -766,7 +773,6 @@ def gated_scan_bwd(x, gate, carry, dh=None, dlast=None, starts=None):
     if dlast is not None:
         _operand("dlast", dlast, (B, D), torch.float32, x.device)
         dlast = dense(dlast)
-    L = N.load()
     dx = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
     dgate = torch.empty_like(dx)
     dh0 = torch.empty(B, D, dtype=torch.float32, device=x.device)

@@ -214,3 +214,24 @@ def test_distill_loss_gradient_is_the_same_whichever_backward_asks(dtype, factor
     # the rounding for a factor of 1, times the factor, and (in _check) the second one
     once = 2.0 ** -8 * (np.abs(want) + bound) if dtype == "bfloat16" else R.EPS * np.abs(want)
     _check(first, f * want, abs(f) * (bound + once + 2.0 ** -133), "factor")
+
+
+# ---- operands that do not fit each other ---------------------------------------------
+
+def test_gated_scan_bwd_refuses_operands_that_do_not_fit():
+    import torch
+    from oxitorch_b200 import functional as F
+    x = torch.randn(2, 130, 8, device="cuda")
+    gate = torch.randn_like(x)
+    _, _, carry = F.gated_scan_fwd(x, gate)
+    _, _, short = F.gated_scan_fwd(x[:, :64], gate[:, :64])
+    F.gated_scan_bwd(x, gate, carry)
+    for bad in (lambda: F.gated_scan_bwd(x, gate[:, :129], carry), lambda: F.gated_scan_bwd(x, gate[:1], carry),
+                lambda: F.gated_scan_bwd(x, gate.bfloat16(), carry), lambda: F.gated_scan_bwd(x, gate.cpu(), carry),
+                lambda: F.gated_scan_bwd(x, gate, short), lambda: F.gated_scan_bwd(x, gate, carry.bfloat16()),
+                lambda: F.gated_scan_bwd(x, gate, carry.repeat_interleave(2)[::2]),
+                lambda: F.gated_scan_bwd(x, gate, carry.cpu()), lambda: F.gated_scan_bwd(x[0], gate[0], carry)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        F.gated_scan_bwd(x, gate, None)
