@@ -632,10 +632,16 @@ def add_rms_norm_bwd(r, weight, rstd, dy, dr=None, grad_mode="ref"):
     """Returns (dx, dresidual, dweight) for dy (the type of y) and dr (float32,
     None = zero); in float32 dx and dresidual are one tensor."""
     _dtype_id("dy", dy)
+    if dy.dim() == 0:
+        raise ValueError("invalid argument: dim -1 out of range for 0-D tensor")
+    if grad_mode not in _MODES:
+        raise ValueError(f"invalid argument: unknown grad mode {grad_mode!r}")
     _operand("r", r, dy.shape, torch.float32, dy.device)
+    _operand("weight", weight, (dy.shape[-1],), torch.float32, dy.device)
+    _operand("rstd", rstd, dy.shape[:-1], torch.float32, dy.device)
     if dr is not None:
         _operand("dr", dr, r.shape, torch.float32, r.device)
-    return _add_rms_norm_bwd(dense(r), dense(weight), rstd, dy, dr, grad_mode)
+    return _add_rms_norm_bwd(dense(r), dense(weight), dense(rstd), dy, dr, grad_mode)
 
 
 def _add_rms_norm_bwd(r, w, rstd, dy, dr, grad_mode):

@@ -235,3 +235,24 @@ def test_gated_scan_bwd_refuses_operands_that_do_not_fit():
             bad()
     with pytest.raises(TypeError):
         F.gated_scan_bwd(x, gate, None)
+
+
+def test_add_rms_norm_bwd_refuses_operands_that_do_not_fit():
+    import torch
+    from oxitorch_b200 import functional as F
+    x, w = torch.randn(5, 3, 16, device="cuda"), torch.ones(16, device="cuda")
+    _, r, rstd = F.add_rms_norm_fwd(x, x, w)
+    want = F.add_rms_norm_bwd(r, w, rstd, x)
+    for bad in (lambda: F.add_rms_norm_bwd(r, w[:8], rstd, x), lambda: F.add_rms_norm_bwd(r, w.bfloat16(), rstd, x),
+                lambda: F.add_rms_norm_bwd(r, w, rstd[:2], x), lambda: F.add_rms_norm_bwd(r, w, rstd.double(), x),
+                lambda: F.add_rms_norm_bwd(r, w.cpu(), rstd, x), lambda: F.add_rms_norm_bwd(r, w, rstd.cpu(), x),
+                lambda: F.add_rms_norm_bwd(r[0], w, rstd, x), lambda: F.add_rms_norm_bwd(r, w, rstd, x, grad_mode="half"),
+                lambda: F.add_rms_norm_bwd(r[0, 0, 0], w, rstd, x[0, 0, 0])):
+        with pytest.raises(ValueError):
+            bad()
+    # strided ones are read where they are
+    apart = torch.full((5, 3, 2), float("nan"), device="cuda")
+    apart[..., 0] = rstd
+    twice = torch.stack([w, w * 9], -1)
+    got = F.add_rms_norm_bwd(r, twice[:, 0], apart[..., 0], x)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
