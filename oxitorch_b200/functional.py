@@ -572,6 +572,13 @@ def _operand(name, t, shape, dtype, device):
         raise ValueError(f"shape mismatch: {name} {list(t.shape)} vs {list(shape)}")
 
 
+def _flag(t, device):
+    """Checks an error flag: four dense int32."""
+    _operand("flag", t, (4,), torch.int32, device)
+    if not t.is_contiguous():
+        raise ValueError("invalid argument: flag must be contiguous")
+
+
 def _dense_any(t):
     if t.is_contiguous():
         return t
@@ -873,6 +880,11 @@ def distill_loss_fwd(logits, teacher_logits, teacher_ids, temperature=1.0, total
     ti = teacher_ids.to(torch.int64).contiguous()
     _operand("teacher_ids", ti, ti.shape, torch.int64, logits.device)
     _operand("teacher_logits", tl, ti.shape, torch.float32, logits.device)
+    if grad_loss is not None:
+        one = isinstance(grad_loss, torch.Tensor) and grad_loss.numel() == 1
+        _operand("grad_loss", grad_loss, grad_loss.shape if one else (1,), torch.float32, logits.device)
+    if flag is not None:
+        _flag(flag, logits.device)
     x = _rows2d(logits)
     rows, vocab = x.shape
     loss = torch.empty(1, dtype=torch.float32, device=x.device)
@@ -966,7 +978,7 @@ def verify_draft(target, draft, tokens, uniform, race, lengths=None, flag=None):
         _operand("lengths", lengths, (B,), torch.int64, dev)
         lengths = lengths.contiguous()
     if flag is not None:
-        _operand("flag", flag, (4,), torch.int32, dev)
+        _flag(flag, dev)
     target, tokens, uniform, race = _sequence(target), tokens.contiguous(), dense(uniform), dense(race)
     out = torch.empty(B, K + 1, dtype=torch.int64, device=dev)
     accepted = torch.empty(B, dtype=torch.int64, device=dev)

@@ -256,3 +256,24 @@ def test_add_rms_norm_bwd_refuses_operands_that_do_not_fit():
     twice = torch.stack([w, w * 9], -1)
     got = F.add_rms_norm_bwd(r, twice[:, 0], apart[..., 0], x)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_flags_and_factors_that_do_not_fit_are_refused():
+    import torch
+    from oxitorch_b200 import functional as F
+    p = torch.softmax(torch.randn(2, 2, 10, device="cuda"), -1)
+    tok, u, e = torch.zeros(2, 1, dtype=torch.int64, device="cuda"), torch.rand(2, 1, device="cuda"), torch.ones(2, 10, device="cuda")
+    x, tl, ti = torch.randn(3, 10, device="cuda"), torch.zeros(3, 2, device="cuda"), torch.zeros(3, 2, dtype=torch.int64, device="cuda")
+    flag = torch.zeros(8, dtype=torch.int32, device="cuda")
+    F.verify_draft(p, p[:, :1], tok, u, e, flag=flag[:4])
+    F.distill_loss_fwd(x, tl, ti, grad_loss=torch.ones(1, device="cuda"), flag=flag[4:])
+    F.distill_loss_fwd(x, tl, ti, grad_loss=torch.ones((), device="cuda"))
+    for bad in (flag[::2], flag, flag[:4].long(), flag[:4].cpu()):
+        with pytest.raises(ValueError):
+            F.verify_draft(p, p[:, :1], tok, u, e, flag=bad)
+        with pytest.raises(ValueError):
+            F.distill_loss_fwd(x, tl, ti, flag=bad)
+    for bad in (torch.ones(2, device="cuda"), torch.ones(1, device="cuda").double(), torch.ones(1),
+                torch.ones(0, device="cuda")):
+        with pytest.raises(ValueError):
+            F.distill_loss_fwd(x, tl, ti, grad_loss=bad)
