@@ -676,7 +676,7 @@ oxc_status oxc_distill_loss(const void* logits, int64_t logits_stride, const flo
     return fail(OXC_ERR_INVALID_ARGUMENT,
                 "invalid argument: distill_loss: temperature must be positive, got %g",
                 (double)temperature);
-  if (vocab > 0x7fffffff)
+  if (vocab > 0x7fffffff - 1024)  // a thread's int index steps past the last token
     return fail(OXC_ERR_NOT_IMPLEMENTED, "not implemented: distill_loss: rows wider than 2^31");
   if (top > kDistillMaxTop)
     return fail(OXC_ERR_NOT_IMPLEMENTED,

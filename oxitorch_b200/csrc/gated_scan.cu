@@ -933,6 +933,8 @@ static oxc_status scan_check(const char* fn, int32_t dtype, int64_t batch, int64
   if (batch > 65535)
     return fail(OXC_ERR_NOT_IMPLEMENTED, "not implemented: %s: batch of %lld > 65535", fn,
                 (long long)batch);
+  if (dim > 0x7fffffff - 1024)  // a tile's channels are counted in int, past the last one
+    return fail(OXC_ERR_NOT_IMPLEMENTED, "not implemented: %s: %lld channels", fn, (long long)dim);
   return OXC_OK;
 }
 
