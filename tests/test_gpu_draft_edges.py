@@ -277,3 +277,96 @@ def test_flags_and_factors_that_do_not_fit_are_refused():
                 torch.ones(0, device="cuda")):
         with pytest.raises(ValueError):
             F.distill_loss_fwd(x, tl, ti, grad_loss=bad)
+
+
+# ---- distill_loss: many rows to a cluster, and the kernel for any width ------------------
+
+def _mixed_rows(n, vocab, top, dtype):
+    """Rows as in training, among them ones without a teacher, with an entry of -inf,
+    with ids listed twice or more, and with masked logits."""
+    import torch
+    logits, teacher, ids = _distill_inputs(n, vocab, top, dtype)
+    ids[::5, top // 2:] = ids[::5, :top - top // 2]
+    ids[1::7] = -1
+    teacher[2::9, 0] = float("-inf")
+    logits[3::11, vocab // 3:vocab // 2] = float("-inf")
+    keep = torch.zeros_like(ids, dtype=torch.bool)
+    keep[3::11] = (ids[3::11] >= vocab // 3) & (ids[3::11] < vocab // 2)
+    ids[keep] = 0
+    return logits, teacher, ids
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,vocab,top", [(9001, 1003, 40), (1501, 32001, 64), (333, 131073, 300)])
+def test_distill_loss_many_rows_to_a_cluster(n, vocab, top, dtype):
+    """Several rows in turn through each cluster of 1, 2, 4 or 8 CTAs, not the same
+    number for each."""
+    _distill_against_reference(*_mixed_rows(n, vocab, top, dtype), 1.5)
+
+
+@pytest.mark.parametrize("dtype,vocab", [("float32", 330001), ("bfloat16", 660001)])
+def test_distill_loss_rows_wider_than_a_cluster_holds(dtype, vocab):
+    import torch
+    from oxitorch_b200 import functional as F
+    logits, teacher, ids = _mixed_rows(13, vocab, 50, dtype)
+    for tau in (1.0, 0.7):
+        _distill_against_reference(logits, teacher, ids, tau)
+    ids[:, 0] = 3
+    clean = ids.clone()
+    ids[4, 1] = vocab
+    t = teacher.clone()
+    t[6, 0] = float("nan")
+    x = logits.clone()
+    x[8, 17] = float("nan")
+    x[10] = float("-inf")
+    flag = torch.zeros(4, dtype=torch.int32, device="cuda")
+    loss, grad = F.distill_loss_fwd(x, t, ids, flag=flag)
+    assert torch.isnan(loss).all() and flag.tolist() == [2, vocab, 0, vocab]
+    bad = [4, 6, 8, 10]
+    assert torch.isnan(grad[bad]).all()
+    good = [i for i in range(13) if i not in bad]
+    _, want = F.distill_loss_fwd(logits, teacher, clean)
+    assert torch.equal(grad[good], want[good])
+
+
+# ---- graphs --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_draft_ops_captured_in_a_graph(dtype):
+    """A replay on new inputs in the captured buffers gives the bits of an eager call."""
+    import torch
+    from oxitorch_b200 import functional as F
+    scan, norm = _scan_inputs(2, 700, 264, dtype, starts=True), _norm_inputs(300, 1032, dtype)
+    dist = _distill_inputs(40, 33000, 30, dtype)
+    ver = [torch.from_numpy(np.array(a)).cuda() for a in _verify_inputs(9, 3, 20003)]
+
+    def everything():
+        x, gate, h0, dh, dlast, starts = scan
+        h, last, carry = F.gated_scan_fwd(x, gate, h0, starts)
+        nx, nr, nw, ndy, ndr = norm
+        y, r, rstd = F.add_rms_norm_fwd(nx, nr, nw)
+        q, scale, _ = F.add_rms_norm_quant(nx, nr, nw)
+        out = torch.empty_like(h0)
+        step = F.gated_step(x[:, 3], gate[:, 3], h0, out=out)
+        p, d, tokens, u, e, lengths = ver
+        return [h, last, *F.gated_scan_bwd(x, gate, carry, dh, dlast, starts), y, r,
+                *F.add_rms_norm_bwd(r, nw, rstd, ndy, ndr, "exact"), q.view(torch.uint8), scale, step, out,
+                *F.distill_loss_fwd(*dist), *F.verify_draft(p, d, tokens, u, e, lengths)]
+    everything()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = everything()
+    for seed in (1, 2):
+        for t, s in zip(scan[:5], _scan_inputs(2, 700, 264, dtype, seed)[:5]):
+            t.copy_(s)
+        for t, s in zip(norm, _norm_inputs(300, 1032, dtype, seed)):
+            t.copy_(s)
+        for t, s in zip(dist, _distill_inputs(40, 33000, 30, dtype, seed)):
+            t.copy_(s)
+        for t, s in zip(ver, _verify_inputs(9, 3, 20003, seed)):
+            t.copy_(torch.from_numpy(np.array(s)))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in got]
+        assert all(torch.equal(a, b) for a, b in zip(kept, everything()))
+    assert __import__("oxitorch_b200")._native.kernel_error_bits() == 0
