@@ -592,7 +592,8 @@ struct GroupGeom {
   int vpt, warps, groups;
   int threads() const { return 32 * warps * groups; }
   // 8 vectors a thread at most: all rows but those of 32766 and 32767 columns, whose
-  // shifts touch up to 8193 vectors (the single-element kernels hold them)
+  // shifts touch up to 8193 vectors (the single-element kernels hold them: bf16 [2000,
+  // 32766] 264 us, 1.09 ms VJP; 32765 columns 158 us and 1.02 ms, as 8 vectors spill)
   bool held() const { return vpt <= 8; }
 };
 static GroupGeom group_geom(int64_t cols, int vpt) {
@@ -731,6 +732,8 @@ static oxc_status add_rms_bwd_launch(const float* r, const float* w, const float
       else if (g.vpt == 4) LAUNCH(4, 1024, true);
       else LAUNCH(8, 1024, true);
     } else {
+      // 352 and 384 threads: two CTAs fit an SM, a third neither at 64 registers, so
+      // they take 85 ([16384, 2944] f32 120 us instead of 132, bf16 127 instead of 140)
       if (g.vpt == 1) LAUNCH(1, 256, false);
       else if (g.vpt == 2 && n <= 384 && n > 1024 / 3) LAUNCH(2, 384, false);
       else if (g.vpt == 2 && n <= 512) LAUNCH(2, 512, false);

@@ -26,10 +26,12 @@
 // recurrence from it on the values that it kept in registers: x and gate are
 // read once.  The VJP's mu runs through the same A from the other end.
 //
-// The state that enters a chunk (Chain, below): chunks form groups of 8.  A
-// chunk applies, one after the other, the maps of the chunks before it in its
-// group to the state entering the group; that one in turn comes from the
-// nearest group whose entering state is known and the group maps between.  So
+// The state that enters a chunk (Chain, below) is found by looking back, as in the
+// published single-pass scans with decoupled look-back (Merrill and Garland, 2016),
+// over two levels: chunks form groups of 8.  A chunk applies, one after the other,
+// the maps of the chunks before it in its group to the state entering the group;
+// that one in turn comes from the nearest group whose entering state is known and the
+// group maps between.  So
 // the number of dependent steps is length / 512, the reads per chunk are at
 // most 7 maps and a few group words, and since every state is defined by one
 // fixed sequence of operations -- whoever computes it, from however far back --
@@ -815,7 +817,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, kScanCtas) scan_bwd_kernel(
     lane.put(mapA[warp], A);
     lane.put(mapS[warp], S);
     lane.put(mapM[warp], M);
-        Tile ahead = next[1];
+    Tile ahead = next[1];
     ahead.chunk = chunks - 1 - ahead.chunk;
     ask_ahead<kScanChunk, L::kChannels>(gate, ahead, length, dim);
     ask_ahead<kScanChunk, L::kChannels>(x, ahead, length, dim);

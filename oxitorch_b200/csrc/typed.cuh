@@ -85,7 +85,6 @@ __device__ __forceinline__ void store_from_f32(bf16* p, const float (&d)[VW]) {
 }
 
 inline bool known_dtype(int32_t t) { return t == OXC_F32 || t == OXC_BF16; }
-inline int dtype_size(int32_t t) { return t == OXC_BF16 ? 2 : 4; }
 inline bool aligned_to(const void* p, size_t n) {
   return reinterpret_cast<uintptr_t>(p) % n == 0;
 }

@@ -55,8 +55,8 @@ __device__ __forceinline__ unsigned long long warp_max_key(unsigned long long k)
 }
 
 constexpr int kVerifyCluster = 8;
-// CTAs of 256 threads per SM: capped at 64 registers for a fourth (three took 7 us
-// more at 64 x 131072).
+// CTAs of 256 threads per SM: capped at 64 registers for a fourth (64 x 131072 24 us,
+// with three 30; 256 x 131072 65 and 95).
 constexpr int kVerifyCtas = 4;
 
 // The largest key of the vocabulary entries [v0, v1) with weights p - q (q may be null;
@@ -102,7 +102,7 @@ __device__ __forceinline__ unsigned long long race_best(const float* p, const fl
       one(p[at], q ? q[at] : 0.0f, e[at], at);
     }
   } else {
-    constexpr int S = 8;  // entries in flight per row (64 x 131071: 29 us; with 4, 31)
+    constexpr int S = 8;  // entries in flight per row (64 x 131071: 27 us; with 4, 32)
     for (uint32_t i = threadIdx.x; i < n; i += S * THREADS) {
       float pv[S], qv[S], ev[S];
 #pragma unroll
@@ -216,9 +216,9 @@ oxc_status oxc_verify_draft(const float* target, int64_t target_sb, int64_t targ
          vocab >= (int64_t)size * 2 * 2048)
     size *= 2;
   if (batch > 0x7fffffff / size) size = 1;
-  // and larger CTAs where there are few (8 x 200003: 19 us instead of 27): as long as
+  // and larger CTAs where there are few (8 x 200003: 18 us instead of 28): as long as
   // they fill three quarters of the SMs at most, since a cluster's share a GPC, which
-  // leaves some idle (16 x 131072 with a CTA an SM: 24 us instead of 19)
+  // leaves some idle (16 x 131072 with a CTA an SM: 22 us instead of 18)
   int threads = 256;
   while (threads < 1024 && batch * size * threads * 2 <= 768 * (int64_t)sm_count() &&
          vocab >= (int64_t)size * threads * 2 * 4)
