@@ -607,7 +607,10 @@ def _has_tangent(*tensors):
     """Whether forward-mode differentiation runs through one of them.  Then a call goes
     through its autograd function, which refuses, or refuses itself: the kernels would
     drop the tangent, and a missing one counts as zero."""
-    return any(isinstance(t, torch.Tensor) and unpack_dual(t).tangent is not None for t in tensors)
+    for t in tensors:  # (0.3 us each; a generator costs another 0.5)
+        if unpack_dual(t).tangent is not None:
+            return True
+    return False
 
 
 # ---- residual addition + RMSNorm ---------------------------------------------------------
