@@ -715,6 +715,110 @@ oxc_status oxc_verify_draft(const float* target, int64_t target_sb, int64_t targ
                             int64_t* out_tokens, int64_t* accepted, int32_t* err_flag,
                             void* stream);
 
+/* ---- a selective state space model's training step and serving ---------------
+ * No counterpart in the reference either: mixing layers with a state larger than
+ * the width, the loss on sampled tokens that such a draft model is trained further
+ * with, and the clipping of its gradients.  Types and strides as above. */
+
+/* Short causal convolution over dim 1 of x [batch, length, dim] (batch and time
+ * strides), channel by channel: u_t = bias + sum_k w[:, k] x_{t - width + 1 + k},
+ * y = silu(u) where `silu`, else u.  w: [dim, width], width 1 to 8; bias [dim]
+ * may be NULL.  Tokens before the first are x0 [batch, width - 1, dim] (dtype, NULL
+ * = zeros).  starts as for oxc_gated_scan_fwd: taps do not reach before the start of
+ * a token's sequence.  last (like x0, may be NULL): the inputs that a continuation
+ * of the row takes as x0 (zero before the start of its last sequence).
+ * VJP: dy, dlast may be NULL (zero), as may dx0; dw: dim * (width + 1) floats, the
+ * gradient of w, then that of bias. */
+oxc_status oxc_causal_conv_fwd(const void* x, int64_t x_sb, int64_t x_st, const float* w,
+                               const float* bias, const void* x0, const uint8_t* starts, void* y,
+                               void* last, int64_t batch, int64_t length, int64_t dim,
+                               int64_t width, int32_t silu, int32_t dtype, void* stream);
+size_t oxc_causal_conv_bwd_workspace_size(int64_t batch, int64_t length, int64_t dim,
+                                          int64_t width);
+oxc_status oxc_causal_conv_bwd(const void* x, int64_t x_sb, int64_t x_st, const float* w,
+                               const float* bias, const void* x0, const uint8_t* starts,
+                               const void* dy, int64_t dy_sb, int64_t dy_st, const void* dlast,
+                               void* dx, void* dx0, float* dw, int64_t batch, int64_t length,
+                               int64_t dim, int64_t width, int32_t silu, int32_t dtype,
+                               void* workspace, size_t workspace_bytes, void* stream);
+/* One token x [batch, dim] after the inputs in state [batch, width - 1, dim];
+ * state_out (which may be state) keeps those for the next. */
+oxc_status oxc_causal_conv_step(const void* x, int64_t x_stride, const float* w, const float* bias,
+                                const void* state, void* state_out, void* y, int64_t batch,
+                                int64_t dim, int64_t width, int32_t silu, int32_t dtype,
+                                void* stream);
+
+/* Selective state space scan over dim 1 of x, delta, z [batch, length, dim], with A
+ * [dim, state], B, C [batch, length, state] (batch and time strides):
+ *   dt = softplus(delta + delta_bias), h_t = exp(dt A) h_{t-1} + dt x B_t,
+ *   y = (sum_n C_t h_t + D x) silu(z)
+ * delta_bias, D [dim] and z may be NULL (0, 0, no gate).  h0 [batch, dim, state]
+ * f32 (NULL = zero) and last (may be NULL): the state before the first token and
+ * after the last; starts as for oxc_gated_scan_fwd.  state: 1 to 128.  carry:
+ * oxc_selective_scan_carry_size floats that the VJP reads (NULL when there will be
+ * none).  VJP: dy, dlast may be NULL (zero), dh0 too; sums: dim * (state + 2)
+ * floats, the gradients of A, D and delta_bias one after the other; dz only with z. */
+int64_t oxc_selective_scan_carry_size(int64_t batch, int64_t length, int64_t dim, int64_t state);
+size_t oxc_selective_scan_workspace_size(int64_t batch, int64_t length, int64_t dim, int64_t state,
+                                         int32_t backward);
+oxc_status oxc_selective_scan_fwd(const void* x, int64_t x_sb, int64_t x_st, const void* delta,
+                                  int64_t delta_sb, int64_t delta_st, const float* A, const void* B,
+                                  int64_t B_sb, int64_t B_st, const void* C, int64_t C_sb,
+                                  int64_t C_st, const float* D, const void* z, int64_t z_sb,
+                                  int64_t z_st, const float* delta_bias, const uint8_t* starts,
+                                  const float* h0, void* y, float* last, float* carry,
+                                  int64_t batch, int64_t length, int64_t dim, int64_t state,
+                                  int32_t dtype, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+oxc_status oxc_selective_scan_bwd(const void* x, int64_t x_sb, int64_t x_st, const void* delta,
+                                  int64_t delta_sb, int64_t delta_st, const float* A, const void* B,
+                                  int64_t B_sb, int64_t B_st, const void* C, int64_t C_sb,
+                                  int64_t C_st, const float* D, const void* z, int64_t z_sb,
+                                  int64_t z_st, const float* delta_bias, const uint8_t* starts,
+                                  const float* carry, const void* dy, int64_t dy_sb, int64_t dy_st,
+                                  const float* dlast, void* dx, void* ddelta, float* sums, void* dB,
+                                  void* dC, void* dz, float* dh0, int64_t batch, int64_t length,
+                                  int64_t dim, int64_t state, int32_t dtype, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+/* One token of it, x, delta, z [batch, dim] and B, C [batch, state] with batch
+ * strides, from state_in [batch, dim, state] to state_out (which may be state_in). */
+oxc_status oxc_selective_step(const void* x, int64_t x_sb, const void* delta, int64_t delta_sb,
+                              const float* A, const void* B, int64_t B_sb, const void* C,
+                              int64_t C_sb, const float* D, const void* z, int64_t z_sb,
+                              const float* delta_bias, const float* state_in, float* state_out,
+                              void* y, int64_t batch, int64_t dim, int64_t state, int32_t dtype,
+                              void* stream);
+
+/* Clipped policy loss of sampled tokens: with logp the token's log-probability in
+ * softmax(logits / temperature) and r = exp(logp - old_logp), loss[0] = 1 / total_rows *
+ * sum_rows -min(r A, clamp(r, 1 - clip_below, 1 + clip_above) A) + kl_coef *
+ * (exp(ref_logp - logp) - (ref_logp - logp) - 1), A the row's advantage, and (unless
+ * dlogits is NULL) dlogits = grad_loss[0] * d loss / d logits, dense, in the same
+ * pass; grad_loss NULL = 1.  logp [rows] is written too.  A row with a negative token
+ * is padding: loss, gradient and logp 0.  A token >= vocab is recorded in err_flag
+ * (int32[4], may be NULL) and makes them NaN.  ref_logp may be NULL where kl_coef is
+ * 0.  loss NULL: only logp is computed (advantages, old_logp, row_loss are not used,
+ * dlogits is NULL).  row_loss: `rows` floats of scratch. */
+oxc_status oxc_policy_loss(const void* logits, int64_t logits_stride, const int64_t* tokens,
+                           const float* old_logp, const float* advantages, const float* ref_logp,
+                           float clip_below, float clip_above, float kl_coef, float temperature,
+                           const float* grad_loss, float* loss, float* logp, float* row_loss,
+                           void* dlogits, int64_t rows, int64_t vocab, int64_t total_rows,
+                           int32_t dtype, int32_t* err_flag, void* stream);
+
+/* The norm over `count` dense tensors (addresses, element counts and dtypes in host
+ * arrays), summed in f64, into norm[0] on the device; and the clipping by it: out[i] =
+ * tensor i times max_norm / (norm + 1e-6) where that is below 1 (the tensor itself
+ * where it is not, also when the norm is NaN).  out NULL: in place.  The tensors do
+ * not overlap; out[i] is tensor i or overlaps none. */
+size_t oxc_clip_global_norm_workspace_size(int64_t count);
+oxc_status oxc_global_norm(const int64_t* tensors, const int64_t* sizes, const int32_t* dtypes,
+                           int64_t count, float* norm, void* workspace, size_t workspace_bytes,
+                           void* stream);
+oxc_status oxc_clip_global_norm(const int64_t* grads, const int64_t* out, const int64_t* sizes,
+                                const int32_t* dtypes, int64_t count, double max_norm, float* norm,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

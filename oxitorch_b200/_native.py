@@ -218,6 +218,29 @@ SIGNATURES = {
     "oxc_scale_by": (_I32, [_P, _I64, _I32, _P, _P]),
     "oxc_verify_draft": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64,
                                 _P, _P, _P, _P]),
+    "oxc_causal_conv_fwd": (_I32, [_P, _I64, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
+                                   _I32, _I32, _P]),
+    "oxc_causal_conv_bwd_workspace_size": (_SZ, [_I64, _I64, _I64, _I64]),
+    "oxc_causal_conv_bwd": (_I32, [_P, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P,
+                                   _I64, _I64, _I64, _I64, _I32, _I32, _P, _SZ, _P]),
+    "oxc_causal_conv_step": (_I32, [_P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I32, _I32,
+                                    _P]),
+    "oxc_selective_scan_carry_size": (_I64, [_I64, _I64, _I64, _I64]),
+    "oxc_selective_scan_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _I32]),
+    "oxc_selective_scan_fwd": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I64,
+                                      _I64, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64,
+                                      _I64, _I64, _I32, _P, _SZ, _P]),
+    "oxc_selective_scan_bwd": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I64,
+                                      _I64, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _P, _P,
+                                      _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _P, _SZ,
+                                      _P]),
+    "oxc_selective_step": (_I32, [_P, _I64, _P, _I64, _P, _P, _I64, _P, _I64, _P, _P, _I64, _P, _P,
+                                  _P, _P, _I64, _I64, _I64, _I32, _P]),
+    "oxc_policy_loss": (_I32, [_P, _I64, _P, _P, _P, _P, _F32, _F32, _F32, _F32, _P, _P, _P, _P, _P,
+                               _I64, _I64, _I64, _I32, _P, _P]),
+    "oxc_clip_global_norm_workspace_size": (_SZ, [_I64]),
+    "oxc_global_norm": (_I32, [_P, _P, _P, _I64, _P, _P, _SZ, _P]),
+    "oxc_clip_global_norm": (_I32, [_P, _P, _P, _P, _I64, ctypes.c_double, _P, _P, _SZ, _P]),
 }
 
 NOALLOC_SCRATCH_BYTES = 16 * 1024 * 1024

@@ -991,3 +991,447 @@ def verify_draft(target, draft, tokens, uniform, race, lengths=None, flag=None):
         tokens.data_ptr(), _ptr(lengths), uniform.data_ptr(), race.data_ptr(), B, K, V,
         out.data_ptr(), accepted.data_ptr(), _ptr(flag), _stream()), "verify_draft")
     return out, accepted
+
+
+# ---- layers and losses of a selective state space model ----------------------------------
+#
+# What a model with selective state space layers needs beside the draft model's
+# operators above, in training and a token at a time; types, strides and gradients
+# as there.
+
+_ACTIVATIONS = {None: 0, "silu": 1}
+
+
+def _sequences(name, x):
+    dt = _dtype_id("x", x)
+    if x.dim() != 3:
+        raise ValueError(f"invalid argument: {name} expects [batch, length, dim], got {list(x.shape)}")
+    return dt
+
+
+def _recorded(*tensors):
+    """Whether autograd has to see a call on these tensors."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return _has_tangent(*[t for t in tensors if t is not None])
+
+
+# ---- short causal convolution --------------------------------------------------------------
+
+def _conv_args(name, x, shape, weight, bias, x0, activation):
+    dim = shape[-1]
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise ValueError(f"invalid argument: {name} expects weight [dim, width]")
+    width = weight.shape[1]
+    _operand("weight", weight, (dim, width), torch.float32, x.device)
+    if width < 1:
+        raise ValueError(f"invalid argument: {name} needs at least one tap")
+    if bias is not None:
+        _operand("bias", bias, (dim,), torch.float32, x.device)
+    if x0 is not None:
+        _operand("x0", x0, (shape[0], width - 1, dim), x.dtype, x.device)
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"invalid argument: unknown activation {activation!r}")
+    return width
+
+
+def causal_conv_fwd(x, weight, bias=None, x0=None, starts=None, activation="silu"):
+    """Returns (y, last)."""
+    dt = _sequences("causal_conv", x)
+    width = _conv_args("causal_conv", x, x.shape, weight, bias, x0, activation)
+    B, T, D = x.shape
+    x, starts = _sequence(x), _starts_tensor(starts, x)
+    weight, bias = dense(weight), None if bias is None else dense(bias)
+    x0 = None if x0 is None else _dense_any(x0)
+    y = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
+    last = torch.empty(B, width - 1, D, dtype=x.dtype, device=x.device)
+    N.check(N.load().oxc_causal_conv_fwd(
+        x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), _ptr(bias), _ptr(x0),
+        _ptr(starts), y.data_ptr(), last.data_ptr(), B, T, D, width, _ACTIVATIONS[activation], dt,
+        _stream()), "causal_conv")
+    return y, last
+
+
+def causal_conv_bwd(x, weight, bias=None, x0=None, dy=None, dlast=None, starts=None, activation="silu"):
+    """Returns (dx, dweight, dbias, dx0) for the gradients of y and of last (None = zero)."""
+    dt = _sequences("causal_conv", x)
+    width = _conv_args("causal_conv", x, x.shape, weight, bias, x0, activation)
+    B, T, D = x.shape
+    x, starts = _sequence(x), _starts_tensor(starts, x)
+    weight, bias = dense(weight), None if bias is None else dense(bias)
+    x0 = None if x0 is None else _dense_any(x0)
+    if dy is not None:
+        _operand("dy", dy, (B, T, D), x.dtype, x.device)
+        dy = _sequence(dy)
+    if dlast is not None:
+        _operand("dlast", dlast, (B, width - 1, D), x.dtype, x.device)
+        dlast = _dense_any(dlast)
+    dx = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
+    dx0 = torch.empty(B, width - 1, D, dtype=x.dtype, device=x.device)
+    dw = torch.empty(D * (width + 1), dtype=torch.float32, device=x.device)
+    L = N.load()
+    ws = _workspace(L.oxc_causal_conv_bwd_workspace_size(B, T, D, width), x.device)
+    ysb, yst = (0, 0) if dy is None else dy.stride()[:2]
+    N.check(L.oxc_causal_conv_bwd(
+        x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), _ptr(bias), _ptr(x0),
+        _ptr(starts), _ptr(dy), ysb, yst, _ptr(dlast), dx.data_ptr(), dx0.data_ptr(), dw.data_ptr(),
+        B, T, D, width, _ACTIVATIONS[activation], dt, ws.data_ptr(), ws.numel(), _stream()),
+        "causal_conv backward")
+    return dx, dw[:D * width].view(D, width), dw[D * width:], dx0
+
+
+class _CausalConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, x0, starts, activation):
+        y, last = causal_conv_fwd(x, weight, bias, x0, starts, activation)
+        ctx.save_for_backward(x, weight, bias, x0, starts)
+        ctx.activation = activation
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dlast):
+        if dy is None and dlast is None:
+            return None, None, None, None, None, None
+        x, weight, bias, x0, starts = ctx.saved_tensors
+        dx, dw, db, dx0 = causal_conv_bwd(x, weight, bias, x0, dy, dlast, starts, ctx.activation)
+        return dx, dw, None if bias is None else db, None if x0 is None else dx0, None, None
+
+
+def causal_conv(x, weight, bias=None, x0=None, starts=None, activation="silu"):
+    """A short causal convolution over dim 1 of x [batch, length, dim], channel by
+    channel: u_t = bias + sum_k weight[:, k] x_{t - width + 1 + k}, y = silu(u)
+    (``activation=None``: u).  Returns (y, last).
+
+    x is float32 or bfloat16 with any batch and time strides; weight [dim, width],
+    width 1 to 8, and bias [dim] are float32.  x0 [batch, width - 1, dim], of x's
+    type, holds the inputs before the first token (zeros if None), and last the
+    ones that a continuation of the rows takes as its x0.  ``starts`` (bool [batch,
+    length]) marks where a new sequence begins in a packed row: taps do not reach
+    before it, and last is zero there."""
+    if isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor) and _recorded(x, weight, bias, x0):
+        return _CausalConv.apply(x, weight, bias, x0, starts, activation)
+    return causal_conv_fwd(x, weight, bias, x0, starts, activation)
+
+
+def causal_conv_step(x, weight, bias, state, out=None, activation="silu"):
+    """One token of causal_conv for x [batch, dim] after the inputs in state [batch,
+    width - 1, dim]: returns y and writes the inputs for the next token to ``out``
+    (``state`` itself if None).  For inference: it has no gradient."""
+    dt = _dtype_id("x", x)
+    if x.dim() != 2:
+        raise ValueError(f"invalid argument: causal_conv_step expects [batch, dim], got {list(x.shape)}")
+    width = _conv_args("causal_conv_step", x, x.shape, weight, bias, None, activation)
+    _operand("state", state, (x.shape[0], width - 1, x.shape[1]), x.dtype, x.device)
+    out = _state_out(state, out)
+    if _recorded(x, weight, bias, state):
+        raise ValueError("invalid argument: causal_conv_step has no gradient; train with causal_conv")
+    x, weight, bias = _rows2d(x), dense(weight), None if bias is None else dense(bias)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    N.check(N.load().oxc_causal_conv_step(
+        x.data_ptr(), x.stride(0), weight.data_ptr(), _ptr(bias), state.data_ptr(), out.data_ptr(),
+        y.data_ptr(), x.shape[0], x.shape[1], width, _ACTIVATIONS[activation], dt, _stream()),
+        "causal_conv_step")
+    return y
+
+
+def _state_out(state, out):
+    """Where a step writes the state after it: `state`, or a tensor that does not overlap it."""
+    if out is None or out is state:
+        out = state
+    else:
+        _operand("out", out, state.shape, state.dtype, state.device)
+    if not (state.is_contiguous() and out.is_contiguous()):
+        raise ValueError("invalid argument: state and out must be contiguous")
+    if 0 < abs(out.data_ptr() - state.data_ptr()) < state.element_size() * state.numel():
+        raise ValueError("invalid argument: out must be state or not overlap it")
+    return out
+
+
+# ---- selective state space scan ------------------------------------------------------------
+
+def _selective_args(x, lead, delta, A, B, C, D, z, delta_bias):
+    """Checks everything but x and the states; `lead`: x's dims before the last."""
+    dim, dev = x.shape[-1], x.device
+    if not isinstance(A, torch.Tensor) or A.dim() != 2:
+        raise ValueError("invalid argument: A must be [dim, state]")
+    n = A.shape[1]
+    _operand("delta", delta, x.shape, x.dtype, dev)
+    _operand("A", A, (dim, n), torch.float32, dev)
+    _operand("B", B, (*lead, n), x.dtype, dev)
+    _operand("C", C, (*lead, n), x.dtype, dev)
+    if D is not None:
+        _operand("D", D, (dim,), torch.float32, dev)
+    if z is not None:
+        _operand("z", z, x.shape, x.dtype, dev)
+    if delta_bias is not None:
+        _operand("delta_bias", delta_bias, (dim,), torch.float32, dev)
+    return n
+
+
+def _dense_or_none(t):
+    return None if t is None else dense(t)
+
+
+def selective_scan_fwd(x, delta, A, B, C, D=None, z=None, delta_bias=None, h0=None, starts=None,
+                       save=True):
+    """Returns (y, last, carry); carry (None without ``save``) is what the VJP needs."""
+    dt = _sequences("selective_scan", x)
+    batch, length, dim = x.shape
+    n = _selective_args(x, (batch, length), delta, A, B, C, D, z, delta_bias)
+    if h0 is not None:
+        _operand("h0", h0, (batch, dim, n), torch.float32, x.device)
+    x, delta, B, C, starts = _sequence(x), _sequence(delta), _sequence(B), _sequence(C), _starts_tensor(starts, x)
+    z = None if z is None else _sequence(z)
+    A, D, delta_bias, h0 = dense(A), _dense_or_none(D), _dense_or_none(delta_bias), _dense_or_none(h0)
+    L = N.load()
+    y = torch.empty(batch, length, dim, dtype=x.dtype, device=x.device)
+    last = torch.empty(batch, dim, n, dtype=torch.float32, device=x.device)
+    carry = None
+    if save:
+        carry = torch.empty(L.oxc_selective_scan_carry_size(batch, length, dim, n), dtype=torch.float32,
+                            device=x.device)
+    ws = _workspace(L.oxc_selective_scan_workspace_size(batch, length, dim, n, 0), x.device)
+    zsb, zst = (0, 0) if z is None else z.stride()[:2]
+    N.check(L.oxc_selective_scan_fwd(
+        x.data_ptr(), x.stride(0), x.stride(1), delta.data_ptr(), delta.stride(0), delta.stride(1),
+        A.data_ptr(), B.data_ptr(), B.stride(0), B.stride(1), C.data_ptr(), C.stride(0), C.stride(1),
+        _ptr(D), _ptr(z), zsb, zst, _ptr(delta_bias), _ptr(starts), _ptr(h0), y.data_ptr(),
+        last.data_ptr(), _ptr(carry), batch, length, dim, n, dt, ws.data_ptr(), ws.numel(),
+        _stream()), "selective_scan")
+    return y, last, carry
+
+
+def selective_scan_bwd(x, delta, A, B, C, carry, D=None, z=None, delta_bias=None, starts=None,
+                       dy=None, dlast=None):
+    """Returns (dx, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dh0) for the gradients of y
+    and of the last state (None = zero); carry is selective_scan_fwd's.  dz is None
+    without z."""
+    dt = _sequences("selective_scan", x)
+    batch, length, dim = x.shape
+    n = _selective_args(x, (batch, length), delta, A, B, C, D, z, delta_bias)
+    L = N.load()
+    _operand("carry", carry, (L.oxc_selective_scan_carry_size(batch, length, dim, n),), torch.float32, x.device)
+    if not carry.is_contiguous():
+        raise ValueError("invalid argument: carry must be contiguous")
+    if dy is not None:
+        _operand("dy", dy, x.shape, x.dtype, x.device)
+        dy = _sequence(dy)
+    if dlast is not None:
+        _operand("dlast", dlast, (batch, dim, n), torch.float32, x.device)
+        dlast = dense(dlast)
+    x, delta, B, C, starts = _sequence(x), _sequence(delta), _sequence(B), _sequence(C), _starts_tensor(starts, x)
+    z = None if z is None else _sequence(z)
+    A, D, delta_bias = dense(A), _dense_or_none(D), _dense_or_none(delta_bias)
+
+    def like(*shape):
+        return torch.empty(shape, dtype=x.dtype, device=x.device)
+    dx, ddelta, dB, dC = like(*x.shape), like(*x.shape), like(batch, length, n), like(batch, length, n)
+    dz = None if z is None else like(*x.shape)
+    sums = torch.empty(dim * (n + 2), dtype=torch.float32, device=x.device)
+    dh0 = torch.empty(batch, dim, n, dtype=torch.float32, device=x.device)
+    ws = _workspace(L.oxc_selective_scan_workspace_size(batch, length, dim, n, 1), x.device)
+    zsb, zst = (0, 0) if z is None else z.stride()[:2]
+    ysb, yst = (0, 0) if dy is None else dy.stride()[:2]
+    N.check(L.oxc_selective_scan_bwd(
+        x.data_ptr(), x.stride(0), x.stride(1), delta.data_ptr(), delta.stride(0), delta.stride(1),
+        A.data_ptr(), B.data_ptr(), B.stride(0), B.stride(1), C.data_ptr(), C.stride(0), C.stride(1),
+        _ptr(D), _ptr(z), zsb, zst, _ptr(delta_bias), _ptr(starts), carry.data_ptr(), _ptr(dy), ysb,
+        yst, _ptr(dlast), dx.data_ptr(), ddelta.data_ptr(), sums.data_ptr(), dB.data_ptr(),
+        dC.data_ptr(), _ptr(dz), dh0.data_ptr(), batch, length, dim, n, dt, ws.data_ptr(),
+        ws.numel(), _stream()), "selective_scan backward")
+    dA, dD, dbias = sums.split((dim * n, dim, dim))
+    return dx, ddelta, dA.view(dim, n), dB, dC, dD, dz, dbias, dh0
+
+
+class _SelectiveScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, delta, A, B, C, D, z, delta_bias, h0, starts):
+        y, last, carry = selective_scan_fwd(x, delta, A, B, C, D, z, delta_bias, h0, starts)
+        ctx.save_for_backward(x, delta, A, B, C, carry, D, z, delta_bias, starts)
+        ctx.has_h0 = h0 is not None
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dlast):
+        if dy is None and dlast is None:
+            return (None,) * 10
+        x, delta, A, B, C, carry, D, z, delta_bias, starts = ctx.saved_tensors
+        dx, ddelta, dA, dB, dC, dD, dz, dbias, dh0 = selective_scan_bwd(
+            x, delta, A, B, C, carry, D, z, delta_bias, starts, dy, dlast)
+        return (dx, ddelta, dA, dB, dC, None if D is None else dD, dz,
+                None if delta_bias is None else dbias, dh0 if ctx.has_h0 else None, None)
+
+
+def selective_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, h0=None, starts=None):
+    """The selective state space scan over dim 1 of x [batch, length, dim]: with dt =
+    softplus(delta + delta_bias), the state h [dim, state] of a sequence is
+    h_t = exp(dt_t A) h_{t-1} + dt_t x_t B_t, and y_t = (sum over the states of C_t h_t
+    + D x_t) silu(z_t).  Returns (y, last), last [batch, dim, state] being the state
+    after the last token.
+
+    x, delta and z [batch, length, dim] and B and C [batch, length, state] have one type
+    (float32 or bfloat16) and any batch and time strides, so parts of one projection
+    need no copy; A [dim, state] (negative for a state that decays; state up to 128), D and
+    delta_bias [dim], the state h0 (zero if None) and last are float32.  D, z and
+    delta_bias may be None (no D x, no gate, no bias).  ``starts`` (bool [batch,
+    length]) marks where a new sequence begins in a packed row: the state before such
+    a token is zero."""
+    if (isinstance(x, torch.Tensor) and all(t is None or isinstance(t, torch.Tensor)
+                                            for t in (delta, A, B, C, D, z, delta_bias, h0))
+            and _recorded(x, delta, A, B, C, D, z, delta_bias, h0)):
+        return _SelectiveScan.apply(x, delta, A, B, C, D, z, delta_bias, h0, starts)
+    return selective_scan_fwd(x, delta, A, B, C, D, z, delta_bias, h0, starts, save=False)[:2]
+
+
+def selective_step(x, delta, A, B, C, state, D=None, z=None, delta_bias=None, out=None):
+    """One token of selective_scan for x, delta, z [batch, dim] and B, C [batch, state]:
+    writes the state after it to ``out`` (``state`` itself if None) and returns y.  For
+    inference: it has no gradient."""
+    dt = _dtype_id("x", x)
+    if x.dim() != 2:
+        raise ValueError(f"invalid argument: selective_step expects [batch, dim], got {list(x.shape)}")
+    batch, dim = x.shape
+    n = _selective_args(x, (batch,), delta, A, B, C, D, z, delta_bias)
+    _operand("state", state, (batch, dim, n), torch.float32, x.device)
+    out = _state_out(state, out)
+    if _recorded(x, delta, A, B, C, state, D, z, delta_bias):
+        raise ValueError("invalid argument: selective_step has no gradient; train with selective_scan")
+    x, delta, B, C = _rows2d(x), _rows2d(delta), _rows2d(B), _rows2d(C)
+    z = None if z is None else _rows2d(z)
+    A, D, delta_bias = dense(A), _dense_or_none(D), _dense_or_none(delta_bias)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    N.check(N.load().oxc_selective_step(
+        x.data_ptr(), x.stride(0), delta.data_ptr(), delta.stride(0), A.data_ptr(), B.data_ptr(),
+        B.stride(0), C.data_ptr(), C.stride(0), _ptr(D), _ptr(z), 0 if z is None else z.stride(0),
+        _ptr(delta_bias), state.data_ptr(), out.data_ptr(), y.data_ptr(), batch, dim, n, dt,
+        _stream()), "selective_step")
+    return y
+
+
+# ---- clipped policy loss -------------------------------------------------------------------
+
+def _sampled_tokens(name, logits, tokens):
+    dt = _dtype_id("logits", logits)
+    if logits.dim() < 2:
+        raise ValueError(f"invalid argument: {name} expects [n, classes] logits, got {list(logits.shape)}")
+    if not isinstance(tokens, torch.Tensor) or tokens.dtype not in (torch.int64, torch.int32):
+        raise ValueError("invalid argument: tokens must be an int64 or int32 tensor")
+    tokens = tokens.to(torch.int64).contiguous()
+    _operand("tokens", tokens, logits.shape[:-1], torch.int64, logits.device)
+    return dt, tokens
+
+
+def policy_loss_fwd(logits, tokens, old_logp, advantages, ref_logp=None, clip=0.2, kl_coef=0.0,
+                    temperature=1.0, total_rows=None, grad=True, grad_loss=None, flag=None):
+    """Returns (loss[1], logp, dlogits): the gradient (times grad_loss[0] if given)
+    comes from the same pass; None without ``grad``."""
+    dt, tok = _sampled_tokens("policy_loss", logits, tokens)
+    dev, lead = logits.device, logits.shape[:-1]
+    _operand("old_logp", old_logp, lead, torch.float32, dev)
+    _operand("advantages", advantages, lead, torch.float32, dev)
+    below, above = clip if isinstance(clip, (tuple, list)) else (clip, clip)
+    if not (below >= 0 and above >= 0 and 0 <= kl_coef < float("inf")):
+        raise ValueError(f"invalid argument: clip {clip} and kl_coef {kl_coef} must not be negative")
+    if ref_logp is not None:
+        _operand("ref_logp", ref_logp, lead, torch.float32, dev)
+    elif kl_coef > 0:
+        raise ValueError("invalid argument: the KL term needs ref_logp")
+    if grad_loss is not None:
+        one = isinstance(grad_loss, torch.Tensor) and grad_loss.numel() == 1
+        _operand("grad_loss", grad_loss, grad_loss.shape if one else (1,), torch.float32, dev)
+    if flag is not None:
+        _flag(flag, dev)
+    x, old, adv, ref = _rows2d(logits), dense(old_logp), dense(advantages), _dense_or_none(ref_logp)
+    rows, vocab = x.shape
+    loss = torch.empty(1, dtype=torch.float32, device=dev)
+    logp = torch.empty(lead, dtype=torch.float32, device=dev)
+    row_loss = torch.empty(rows, dtype=torch.float32, device=dev)
+    dlogits = torch.empty(logits.shape, dtype=x.dtype, device=dev) if grad else None
+    N.check(N.load().oxc_policy_loss(
+        x.data_ptr(), x.stride(0), tok.data_ptr(), old.data_ptr(), adv.data_ptr(), _ptr(ref),
+        float(below), float(above), float(kl_coef), float(temperature), _ptr(grad_loss),
+        loss.data_ptr(), logp.data_ptr(), row_loss.data_ptr(), _ptr(dlogits), rows, vocab,
+        int(total_rows or rows), dt, _ptr(flag), _stream()), "policy_loss")
+    return loss, logp, dlogits
+
+
+class _PolicyLoss(torch.autograd.Function):
+    """As _DistillLoss: the forward pass leaves the gradient for a loss gradient of 1,
+    backward hands it out, scaled on the device if it is another (in bfloat16 rounded a
+    second time then), and a second backward computes it again."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, old_logp, advantages, ref_logp, *args):
+        loss, logp, ctx.dlogits = policy_loss_fwd(logits, tokens, old_logp, advantages, ref_logp, *args)
+        ctx.save_for_backward(logits, tokens, old_logp, advantages, ref_logp)
+        ctx.args = args
+        ctx.mark_non_differentiable(logp)
+        ctx.set_materialize_grads(False)
+        return loss.reshape(()), logp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _):
+        if g is None:
+            return (None,) * 9
+        if g.dtype != torch.float32:
+            g = g.to(torch.float32)
+        d, ctx.dlogits = ctx.dlogits, None
+        if d is None:
+            d = policy_loss_fwd(*ctx.saved_tensors, *ctx.args)[2]
+        N.check(N.load().oxc_scale_by(d.data_ptr(), d.numel(), _DTYPES[d.dtype], g.data_ptr(),
+                                      _stream()), "policy_loss backward")
+        return d, None, None, None, None, None, None, None, None
+
+
+def policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, clip=0.2, kl_coef=0.0,
+                temperature=1.0, total_rows=None):
+    """The clipped policy loss of sampled tokens with a KL term towards a reference:
+    returns (loss, logp), logp [...] being each token's log-probability in
+    softmax(logits / temperature) (no gradient runs through it).  With r = exp(logp -
+    old_logp) the loss is the mean over rows of
+
+        -min(r A, clamp(r, 1 - clip, 1 + clip) A)
+        + kl_coef (exp(ref_logp - logp) - (ref_logp - logp) - 1).
+
+    logits [..., vocab] float32 or bfloat16; tokens [...] int64 or int32; old_logp,
+    advantages A and ref_logp [...] float32, which the gradient does not reach.  clip:
+    one number, or (below, above).  A row with a negative token (padding) adds 0 to the
+    mean and has a zero gradient and logp; a token >= vocab makes the loss NaN.
+    total_rows: the divisor of the mean (the rows of this call if None), as in a sharded
+    batch or where only unpadded tokens count.  In bfloat16 the gradient is rounded for
+    a factor of 1 on the loss and again when another one scales it."""
+    if isinstance(logits, torch.Tensor) and _recorded(logits):
+        for name, t in (("old_logp", old_logp), ("advantages", advantages), ("ref_logp", ref_logp)):
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                raise ValueError(f"invalid argument: {name} gets no gradient; detach it")
+        return _PolicyLoss.apply(logits, tokens, old_logp, advantages, ref_logp, clip, kl_coef,
+                                 temperature, total_rows)
+    loss, logp, _ = policy_loss_fwd(logits, tokens, old_logp, advantages, ref_logp, clip, kl_coef,
+                                    temperature, total_rows, grad=False)
+    return loss.reshape(()), logp
+
+
+def token_logprobs(logits, tokens, temperature=1.0, flag=None):
+    """Each token's log-probability [...] in softmax(logits / temperature), as
+    policy_loss returns it: its old_logp and ref_logp, from the logits of the policy
+    that sampled the tokens and of the reference.  It has no gradient."""
+    dt, tok = _sampled_tokens("token_logprobs", logits, tokens)
+    if _recorded(logits):
+        raise ValueError("invalid argument: token_logprobs has no gradient; train with policy_loss")
+    if flag is not None:
+        _flag(flag, logits.device)
+    x = _rows2d(logits)
+    logp = torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device)
+    rows, vocab = x.shape
+    N.check(N.load().oxc_policy_loss(
+        x.data_ptr(), x.stride(0), tok.data_ptr(), None, None, None, 0.0, 0.0, 0.0,
+        float(temperature), None, None, logp.data_ptr(), None, None, rows, vocab, max(rows, 1), dt,
+        _ptr(flag), _stream()), "token_logprobs")
+    return logp

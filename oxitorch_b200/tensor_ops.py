@@ -6,7 +6,8 @@ keepdim)`` with its VJP ``reduce_backward`` and the autograd helper
 ``unbroadcast`` (graph.rs:274-313), the whole-tensor
 ``sum_all``/``mean_all``/``reduce_all``, plus
 ``clip_grad_norm_`` and ``clip_grad_value_`` (python/oxitorch/optim.py:242-272)
-over device gradients.  Inputs are torch CUDA float32 tensors with any strides (views:
+over device gradients, and beyond the reference ``global_norm`` and
+``clip_global_norm_``, which do not wait for the device.  Inputs are torch CUDA float32 tensors with any strides (views:
 transposes, slices, zero-stride broadcasts); outputs are dense, like the
 reference's ``from_results``.  Every op is one call into liboxicuda.so.
 """
@@ -14,11 +15,12 @@ reference's ``from_results``.  Every op is one call into liboxicuda.so.
 from __future__ import annotations
 
 import ctypes
+from array import array
 
 import torch
 
 from . import _native as N
-from .functional import _require_cuda_f32, _stream, _workspace, dense
+from .functional import _DTYPES, _dtype_id, _require_cuda_f32, _stream, _workspace, dense
 
 BINARY_OPS = ["add", "sub", "mul", "div", "pow", "min", "max"]
 CMP_OPS = ["eq", "ne", "lt", "le", "gt", "ge"]
@@ -296,6 +298,95 @@ def clip_grad_value_(grads, clip_value):
                              "which needs dense storage")
         N.check(L.oxc_clip_grad_value(g.data_ptr(), g.numel(), clip_value, _stream()),
                 "clip_grad_value_")
+
+
+def _flat_operands(name, tensors):
+    """Checks dense float32 / bfloat16 tensors of the current device; returns their
+    addresses, sizes and dtype ids as arrays."""
+    device = torch._C._cuda_getDevice()
+    dtypes = []
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be torch CUDA tensors")
+        dt = _DTYPES.get(t.dtype)
+        if dt is None or t.get_device() != device:
+            _dtype_id(name, t)  # raises
+        if not t.is_contiguous() and not _permuted_dense(t):
+            raise ValueError(f"invalid argument: {name} must have dense storage")
+        dtypes.append(dt)
+    return (array("q", [t.data_ptr() for t in tensors]), array("q", [t.numel() for t in tensors]),
+            array("i", dtypes))
+
+
+def _permuted_dense(t):
+    """Whether t's elements fill a range of memory in some order of its dims."""
+    n = 1
+    for stride, size in sorted((s, d) for s, d in zip(t.stride(), t.shape) if d != 1):
+        if stride != n:
+            return False
+        n *= size
+    return True
+
+
+def global_norm(tensors):
+    """sqrt of the sum over all tensors of sum(v * v), summed in f64, as a 0-d float32
+    tensor: the host does not wait for it.  Tensors are float32 or bfloat16, dense, any
+    number of them; None is skipped."""
+    tensors = [t for t in tensors if t is not None]
+    ptrs, sizes, dtypes = _flat_operands("tensors", tensors)
+    if not tensors:
+        return torch.zeros((), device="cuda")
+    L = N.load()
+    norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
+    ws = _workspace(L.oxc_clip_global_norm_workspace_size(len(tensors)), norm.device)
+    N.check(L.oxc_global_norm(ptrs.buffer_info()[0], sizes.buffer_info()[0], dtypes.buffer_info()[0],
+                              len(tensors), norm.data_ptr(), ws.data_ptr(), ws.numel(), _stream()),
+            "global_norm")
+    return norm
+
+
+def clip_global_norm_(grads, max_norm, out=None):
+    """clip_grad_norm_ for p = 2 without waiting for the device, in two launches for up
+    to 640 tensors: where max_norm / (norm + 1e-6) < 1, every gradient is scaled by it
+    (in f32, rounded once), in place or into ``out``, a list of tensors of the same
+    shapes and types.  Returns the norm before, a 0-d float32 tensor (NaN or infinite
+    if the gradients are; a NaN norm leaves them as they are).
+
+    Gradients are float32 or bfloat16, dense and apart from each other, any number of
+    them; None is skipped (in ``out`` too).  A captured graph repeats the call on the same
+    addresses."""
+    grads = list(grads)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"invalid argument: max_norm must not be negative, got {max_norm}")
+    if out is not None:
+        out = list(out)
+        if len(out) != len(grads):
+            raise ValueError(f"invalid argument: {len(out)} outputs for {len(grads)} gradients")
+        out = [o for o, g in zip(out, grads) if g is not None]
+    grads = [g for g in grads if g is not None]
+    ptrs, sizes, dtypes = _flat_operands("gradients", grads)
+    for t in grads if out is None else out:
+        if isinstance(t, torch.Tensor) and t.requires_grad:
+            raise ValueError("invalid argument: clip_global_norm_ writes to tensors outside any graph")
+    if not grads:
+        return torch.zeros((), device="cuda")
+    to = None
+    if out is not None:
+        to = _flat_operands("outputs", out)[0]
+        for g, o in zip(grads, out):
+            if g.shape != o.shape or g.dtype != o.dtype or (
+                    not (g.is_contiguous() and o.is_contiguous()) and g.stride() != o.stride()):
+                raise ValueError(f"shape mismatch: an output {list(o.shape)} {o.dtype} for a gradient "
+                                 f"{list(g.shape)} {g.dtype}, or laid out otherwise")
+    L = N.load()
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    ws = _workspace(L.oxc_clip_global_norm_workspace_size(len(grads)), norm.device)
+    N.check(L.oxc_clip_global_norm(
+        ptrs.buffer_info()[0], None if to is None else to.buffer_info()[0], sizes.buffer_info()[0],
+        dtypes.buffer_info()[0], len(grads), max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(),
+        _stream()), "clip_global_norm_")
+    return norm
 
 
 def scale_(g, scale):
