@@ -1,138 +1,7 @@
-// selective_scan.cu -- the forward of the selective scan, its single-token step and
-// the C entries (the mathematics is in selective_scan.cuh).
+// selective_scan.cu -- the single-token step of the selective scan and the C entries (the mathematics is in selective_scan.cuh).
 #include "selective_scan.cuh"
 
 namespace oxc {
-
-// MAP: only finds what a segment does to the state.
-template <typename T, int SPT, int LPC, bool VEC, bool MAP>
-__global__ void __launch_bounds__(Layout<T, SPT, LPC>::kThreads)
-selective_fwd_kernel(SelectiveArgs<T> a) {
-  using L = Layout<T, SPT, LPC>;
-  constexpr int P = L::P, VW = VEC ? 4 : 1;
-  extern __shared__ __align__(16) float smem[];
-  float* s_dt = smem;                               // [kTile][kChannels]
-  float* s_dtx = s_dt + kTile * L::kChannels;       // dt x
-  float* s_y = s_dtx + kTile * L::kChannels;
-  float* s_B = s_y + (MAP ? 0 : kTile * L::kChannels);  // [kTile][NP]
-  float* s_C = s_B + kTile * L::NP;
-  const unsigned int ct = blockIdx.x % a.ctiles, rest = blockIdx.x / a.ctiles;
-  const int runs = MAP ? a.segments - 1 : a.segments;  // nothing follows the last
-  const int64_t b = rest / runs;
-  const int seg = rest % runs;
-  const int64_t d0 = (int64_t)ct * L::kChannels;
-  const Place<L> at(d0);
-  const int64_t tiles = (a.length + kTile - 1) / kTile;
-  const int64_t tile0 = (int64_t)seg * a.seg_tiles, tile1 = min(tiles, tile0 + a.seg_tiles);
-  if (!MAP) pdl_wait();
-  float2 A2[2][P], h[2][P];
-  load_decay<L>(A2, at, a);
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    if (MAP) {
-#pragma unroll
-      for (int i = 0; i < P; ++i) h[c][i] = both(0.0f);
-    } else {
-      at.load(h[c], a.h0, c, b, a.dim, a.N);
-    }
-  }
-  if (!MAP)
-    for (int k = 0; k < seg; ++k) through_segment<L>(h, A2, at, a, b, k);
-  float time[2] = {0.0f, 0.0f};
-  bool fresh = false;
-  for (int64_t tile = tile0; tile < tile1; ++tile) {
-    const int64_t t0 = tile * kTile;
-    each_vec<L, VW>([&](int t, int ch) {
-      const bool on = t0 + t < a.length && d0 + ch < a.dim;
-      float x[VW], dt[VW];
-      if (on) {
-        load_vec<VW>(x, a.x.p + b * a.x.sb + (t0 + t) * a.x.st + d0 + ch);
-        load_vec<VW>(dt, a.delta.p + b * a.delta.sb + (t0 + t) * a.delta.st + d0 + ch);
-      }
-#pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        // beyond the sequence dt = 0: the state stays
-        dt[k] = on ? softplus(dt[k] + (a.delta_bias ? a.delta_bias[d0 + ch + k] : 0.0f)) : 0.0f;
-        s_dt[t * L::kChannels + ch + k] = dt[k];
-        s_dtx[t * L::kChannels + ch + k] = on ? dt[k] * x[k] : 0.0f;
-      }
-    });
-    stage_rows<L>(s_B, a.B, b, t0, a.length, a.N);
-    if (!MAP) stage_rows<L>(s_C, a.C, b, t0, a.length, a.N);
-    const unsigned int starts = tile_starts(a.starts, b, t0, a.length);
-    __syncthreads();
-    if (!MAP && a.carry) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) at.store(h[c], a.carry, c, b * tiles + tile, a.dim, a.N);
-    }
-#pragma unroll 4
-    for (int t = 0; t < kTile; ++t) {
-      const float2 dt = *reinterpret_cast<const float2*>(s_dt + t * L::kChannels + at.ch);
-      const float2 dtx = *reinterpret_cast<const float2*>(s_dtx + t * L::kChannels + at.ch);
-      float2 B[P], C[P];
-      load_states<SPT>(B, s_B + t * L::NP + at.sl * SPT);
-      if (!MAP) load_states<SPT>(C, s_C + t * L::NP + at.sl * SPT);
-      float2 y[2] = {both(0.0f), both(0.0f)};
-      const bool start = (starts >> t) & 1u;
-      if (start) fresh = true;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float2 d2 = both(c ? dt.y : dt.x), u2 = both(c ? dtx.y : dtx.x);
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-          const float2 e = exp2_pair(__fmul2_rn(A2[c][i], d2));
-          const float2 u = __fmul2_rn(u2, B[i]);
-          h[c][i] = start ? u : __ffma2_rn(e, h[c][i], u);
-          if (!MAP) y[c] = __ffma2_rn(C[i], h[c][i], y[c]);
-        }
-      }
-      if (MAP) {
-        time[0] += dt.x;
-        time[1] += dt.y;
-      } else {
-        using Sum = LaneSum<2, 1, LPC>;
-        float v[2] = {y[0].x + y[0].y, y[1].x + y[1].y};
-        int first = 0;
-        Sum::run(v, at.sl, first);
-        if (at.sl < Sum::kUsed) {
-#pragma unroll
-          for (int i = 0; i < Sum::kKept; ++i) s_y[t * L::kChannels + at.ch + first + i] = v[i];
-        }
-      }
-    }
-    __syncthreads();
-    if (!MAP)
-      each_vec<L, VW>([&](int t, int ch) {
-        if (t0 + t >= a.length || d0 + ch >= a.dim) return;
-        float x[VW], y[VW];
-        load_vec<VW>(x, a.x.p + b * a.x.sb + (t0 + t) * a.x.st + d0 + ch);
-#pragma unroll
-        for (int k = 0; k < VW; ++k) {
-          y[k] = s_y[t * L::kChannels + ch + k];
-          if (a.D) y[k] = fmaf(a.D[d0 + ch + k], x[k], y[k]);
-        }
-        if (a.z.p) {
-          load_vec<VW>(x, a.z.p + b * a.z.sb + (t0 + t) * a.z.st + d0 + ch);
-#pragma unroll
-          for (int k = 0; k < VW; ++k) y[k] *= x[k] * sigmoid(x[k]);
-        }
-        store_from_f32<VW>(a.y + (b * a.length + t0 + t) * a.dim + d0 + ch, y);
-      });
-  }
-  if (MAP) {
-    const int64_t row = b * a.segments + seg;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      at.store(h[c], a.seg_state, c, row, a.dim, a.N);
-      if (at.sl == 0 && at.d + c < a.dim)
-        a.seg_time[row * a.dim + at.d + c] = fresh ? -1.0f : time[c];
-    }
-    pdl_launch_dependents();
-  } else if (seg == a.segments - 1 && a.last) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) at.store(h[c], a.last, c, b, a.dim, a.N);
-  }
-}
 
 // One token: LPC lanes a channel, four states a lane at a time.
 template <typename T, int LPC>
@@ -192,29 +61,6 @@ selective_step_kernel(const T* __restrict__ x, int64_t x_sb, const T* __restrict
 }
 
 template <typename T>
-static oxc_status selective_fwd_launch(const SelectiveArgs<T>& a, cudaStream_t s) {
-  const bool vec = a.dim % 4 == 0 && seq_vec(a.x) && seq_vec(a.delta) && seq_vec(a.z) &&
-                   aligned_to(a.y, 4 * sizeof(T));
-  const cudaError_t err = by_state(a.N, [&](auto spt, auto lpc) -> cudaError_t {
-    constexpr int SPT = decltype(spt)::value, LPC = decltype(lpc)::value;
-    using L = Layout<T, SPT, LPC>;
-    const size_t plane = kTile * L::kChannels * sizeof(float), row = kTile * L::NP * sizeof(float);
-    const unsigned int per = (unsigned int)(a.batch * a.ctiles);
-    if (a.segments > 1) {
-      auto map = vec ? selective_fwd_kernel<T, SPT, LPC, true, true>
-                     : selective_fwd_kernel<T, SPT, LPC, false, true>;
-      const cudaError_t e = launch_scan(map, per * (a.segments - 1), L::kThreads, 2 * plane + row, false, s, a);
-      if (e != cudaSuccess) return e;
-    }
-    auto kernel = vec ? selective_fwd_kernel<T, SPT, LPC, true, false>
-                      : selective_fwd_kernel<T, SPT, LPC, false, false>;
-    return launch_scan(kernel, per * a.segments, L::kThreads, 3 * plane + 2 * row, a.segments > 1, s, a);
-  });
-  return err == cudaSuccess ? check_launch("oxc_selective_scan_fwd")
-                            : cuda_fail(err, "oxc_selective_scan_fwd");
-}
-
-template <typename T>
 static oxc_status selective_step_launch(const void* x, int64_t x_sb, const void* delta,
                                         int64_t delta_sb, const float* A, const void* B,
                                         int64_t B_sb, const void* C, int64_t C_sb, const float* D,
@@ -252,7 +98,7 @@ int64_t oxc_selective_scan_carry_size(int64_t batch, int64_t length, int64_t dim
 size_t oxc_selective_scan_workspace_size(int64_t batch, int64_t length, int64_t dim, int64_t state,
                                          int32_t backward) {
   if (batch <= 0 || length <= 0 || dim <= 0 || state <= 0 || state > kMaxState) return 0;
-  const Plan p = selective_plan(batch, length, dim, state);
+  const Plan p = selective_plan(batch, length, dim, state, backward);
   size_t n = map_floats(p, batch, dim, state);
   if (backward)
     n += (size_t)batch * p.segments * (size_t)(dim * state + 2 * dim) +
@@ -307,7 +153,7 @@ oxc_status oxc_selective_scan_fwd(const void* x, int64_t x_sb, int64_t x_st, con
     a.length = length;
     a.dim = dim;
     a.N = (int)state;
-    selective_segments(a, selective_plan(batch, length, dim, state), static_cast<float*>(workspace));
+    selective_segments(a, selective_plan(batch, length, dim, state, false), static_cast<float*>(workspace));
     return selective_fwd_launch(a, s);
   };
   return dtype == OXC_BF16 ? go(bf16{}) : go(0.0f);
@@ -369,7 +215,7 @@ oxc_status oxc_selective_scan_bwd(const void* x, int64_t x_sb, int64_t x_st, con
     a.length = length;
     a.dim = dim;
     a.N = (int)state;
-    const Plan p = selective_plan(batch, length, dim, state);
+    const Plan p = selective_plan(batch, length, dim, state, true);
     float* ws = static_cast<float*>(workspace);
     a.sums = ws;  // first, as its parts of dA are read as vectors
     a.rows = a.sums + (size_t)batch * p.segments * (size_t)(dim * state + 2 * dim);

@@ -17,15 +17,15 @@
 //   dA = sum_{b,t} dt mu h_{t-1},  dD = sum e x,  ddelta_bias = sum ddelta
 //   dB_t[n] = sum_d lam dt x,  dC_t[n] = sum_d h e,  dz = dy inner silu'(z)
 //
-// A thread keeps SPT states of each of two channels in registers, LPC threads side
-// by side share a channel, and the CTA's threads walk through the tokens in tiles
-// of kTile: the tile's operands are staged in shared memory in f32 (dt and dt x
-// once per token and channel), sums over n are made across the LPC threads and
-// sums over d across the warp's other lanes, its warps and the CTAs.  The VJP gets
-// the state before each tile from the forward (`carry`) and goes through the tiles
-// from the last to the first: it runs the recurrence forward through a tile,
-// keeping the state every kBack tokens, and from the last of these backwards again
-// with the decays and states of kBack tokens in registers.
+// A thread keeps SPT states of each of CPT channels in registers, LPC threads side
+// by side share a channel, and the CTA's threads walk through the tokens in tiles of
+// kTile.  A tile's operands are copied to shared memory while the tile before it is
+// worked on, and turned into f32 steps (dt, dt x) there, once per token and channel.
+// Sums over n are made across the LPC threads, sums over d across the warp's other
+// lanes, its warps and the CTAs.  The VJP gets the state before each tile from the
+// forward (`carry`) and goes through the tiles from the last to the first: it runs the
+// recurrence forward through a tile, keeping the state every kBack tokens, and from the
+// last of these backwards again with the decays and states of kBack tokens in registers.
 //
 // Where batch and dim leave the GPU idle, the sequence is cut into segments.  A
 // first kernel finds what each does to the state (its decay, exp(A sum dt), and the
@@ -43,7 +43,7 @@ namespace oxc {
 constexpr int kTile = 16;     // tokens; the states that the VJP needs are saved as often
 constexpr int kBack = 4;      // tokens whose states the VJP holds in registers
 constexpr int kMaxState = 128;
-constexpr int kMaxSegments = 32;
+constexpr int kMaxSegments = 64;
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 
 // A [batch, length, n] operand: the last dim dense, strides in elements.
@@ -70,7 +70,7 @@ struct SelectiveArgs {
   float* seg_time;   // sum of dt; negative if a sequence starts in it
   int64_t batch, length, dim;
   int N, segments, seg_tiles;  // tiles per segment
-  unsigned int ctiles;
+  unsigned int ctiles, map_ctiles;  // of the VJP, and of its first kernel
 };
 
 __device__ __forceinline__ float ex2(float t) {
@@ -81,10 +81,33 @@ __device__ __forceinline__ float ex2(float t) {
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float2 exp2_pair(float2 t) { return make_float2(ex2(t.x), ex2(t.y)); }
 
-__device__ __forceinline__ float softplus(float v) {
-  return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v)));
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
-__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+__device__ __forceinline__ float sigmoid(float v) { return rcp(1.0f + ex2(-kLog2e * v)); }
+
+// log(1 + exp(v)) = max(v, 0) + log(1 + e), e = exp(-|v|).  e = 2^t exp(n - t ln 2) with
+// n = -|v| and t = n log2(e) rounded, the second factor to first order.  log(1 + e) = 2
+// artanh(s), s = e / (2 + e) <= 1/3, by the series in s^2 (2 s^17 / 17 is below 2^-26 of
+// it), so a small e keeps its relative accuracy.
+__device__ __forceinline__ float softplus(float v) {
+  float n = -fabsf(v);
+  n = n < -100.0f ? -100.0f : n;  // (a NaN stays)
+  const float t = n * kLog2e;
+  float e = ex2(t);
+  e = fmaf(e, fmaf(t, -kLn2, n), e);
+  const float s = e * rcp(2.0f + e), w = s * s;
+  float p = 2.0f / 15.0f;
+  p = fmaf(p, w, 2.0f / 13.0f);
+  p = fmaf(p, w, 2.0f / 11.0f);
+  p = fmaf(p, w, 2.0f / 9.0f);
+  p = fmaf(p, w, 2.0f / 7.0f);
+  p = fmaf(p, w, 2.0f / 5.0f);
+  p = fmaf(p, w, 2.0f / 3.0f);
+  return fmaf(s, fmaf(p, w, 2.0f), v > 0.0f ? v : 0.0f);
+}
 
 // Sums v over the lanes that differ in the bits FROM .. TO / 2 of their number, each
 // lane keeping a part of the values: halves are exchanged while the count is even.
@@ -133,13 +156,36 @@ __device__ __forceinline__ void load_states(float2 (&v)[SPT / 2], const float* p
   }
 }
 
-template <typename T, int SPT_, int LPC_>
+template <int SPT_, int LPC_, int CPT_, int WARPS>
 struct Layout {
-  static constexpr int SPT = SPT_, LPC = LPC_, P = SPT / 2;
-  static constexpr int kWarps = 8, kThreads = kWarps * 32;
-  static constexpr int kChannels = kWarps * 64 / LPC;  // a CTA's
-  static constexpr int NP = SPT * LPC;                 // states with their padding
+  static constexpr int SPT = SPT_, LPC = LPC_, CPT = CPT_, P = SPT / 2;
+  static constexpr int kWarps = WARPS, kThreads = kWarps * 32;
+  static constexpr int kLanes = 32 / LPC;               // of a warp, side by side over channels
+  static constexpr int kWarpChannels = kLanes * CPT;
+  static constexpr int kChannels = kWarps * kWarpChannels;  // a CTA's
+  static constexpr int NP = SPT * LPC;                  // states with their padding
 };
+
+// One element if `on`, else 0.  The load is predicated rather than branched around or
+// selected from, so that nothing waits for it before its value is used.
+__device__ __forceinline__ float load_if(const float* p, bool on) {
+  float v = 0.0f;
+  asm("{.reg .pred p; setp.ne.s32 p, %2, 0; @p ld.global.nc.f32 %0, [%1];}" : "+f"(v) : "l"(p), "r"((int)on));
+  return v;
+}
+__device__ __forceinline__ uint16_t load_if(const bf16* p, bool on) {
+  uint16_t v = 0;
+  asm("{.reg .pred p; setp.ne.s32 p, %2, 0; @p ld.global.nc.u16 %0, [%1];}" : "+h"(v) : "l"(p), "r"((int)on));
+  return v;
+}
+__device__ __forceinline__ float4 load_if(const float4* p, bool on) {
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  asm("{.reg .pred p; setp.ne.s32 p, %5, 0; @p ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];}"
+      : "+f"(v.x), "+f"(v.y), "+f"(v.z), "+f"(v.w) : "l"(p), "r"((int)on));
+  return v;
+}
+__device__ __forceinline__ float as_f32(float v) { return v; }
+__device__ __forceinline__ float as_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 
 // Where a thread's states are.
 template <class L>
@@ -149,7 +195,7 @@ struct Place {
   __device__ __forceinline__ Place(int64_t d0) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     sl = lane % L::LPC;
-    ch = (warp * (32 / L::LPC) + lane / L::LPC) * 2;
+    ch = (warp * L::kLanes + lane / L::LPC) * L::CPT;
     d = d0 + ch;
   }
   static __device__ __forceinline__ bool vectors(const float* p, int N) {
@@ -161,8 +207,7 @@ struct Place {
     const bool on = p && d + c < dim;
     const float* q = p + (row * dim + d + c) * N + sl * L::SPT;
     if (L::SPT == 4 && vectors(p, N)) {
-      float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (on && sl * L::SPT < N) t = *reinterpret_cast<const float4*>(q);
+      const float4 t = load_if(reinterpret_cast<const float4*>(q), on && sl * L::SPT < N);
       v[0] = make_float2(t.x, t.y);
       v[1] = make_float2(t.z, t.w);
       return;
@@ -170,8 +215,8 @@ struct Place {
 #pragma unroll
     for (int i = 0; i < L::P; ++i) {
       const int n = sl * L::SPT + 2 * i;
-      v[i].x = on && n < N ? q[2 * i] : 0.0f;
-      v[i].y = on && n + 1 < N ? q[2 * i + 1] : 0.0f;
+      v[i].x = load_if(q + 2 * i, on && n < N);
+      v[i].y = load_if(q + 2 * i + 1, on && n + 1 < N);
     }
   }
   __device__ __forceinline__ void store(const float2 (&v)[L::P], float* p, int c, int64_t row,
@@ -192,38 +237,162 @@ struct Place {
   }
 };
 
-// Four (VEC) or one consecutive elements, kept in the caches: the end of a tile reads
-// them again.
-template <int VW, typename T>
-__device__ __forceinline__ void load_vec(float (&v)[VW], const T* p) {
-  if constexpr (VW == 4 && sizeof(T) == 4) {
-    const float4 t = *reinterpret_cast<const float4*>(p);
-    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-  } else if constexpr (VW == 4) {
-    const uint2 t = *reinterpret_cast<const uint2*>(p);
-    v[0] = bf16_lo(t.x); v[1] = bf16_hi(t.x); v[2] = bf16_lo(t.y); v[3] = bf16_hi(t.y);
-  } else {
-    v[0] = to_f32(p[0]);
+// 4, 8 or 16 bytes to shared memory without passing the registers; zeros unless `on`.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool on) {
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(on ? 16 : 0) : "memory");
+  else if constexpr (BYTES == 8)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(src), "r"(on ? 8 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_sent() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+// A tile's operands as they are in memory, TENSORS of them twice over: thread i's
+// vectors lie where only thread i looks, so no barrier stands between its copies and
+// its reads.  A [kTile, kChannels] tile is cut into vectors of VW channels, dealt to the
+// threads token by token, kTurn tokens at a time: a thread's vectors are of the same
+// channels.  Where vectors are shorter than the 4 bytes that can be copied without
+// passing the registers, L2 is asked for the tile ahead and the copy made when it
+// begins.  DIR is 1 or -1, the direction through the tiles.
+template <class L, typename T, int VW, int TENSORS, int DIR>
+struct Raw {
+  static constexpr bool kAsync = VW * sizeof(T) >= 4;
+  static constexpr int kPer = L::kChannels / VW;  // vectors of a token
+  static constexpr int kVecs = kTile * kPer;
+  static constexpr int kMine = (kVecs + L::kThreads - 1) / L::kThreads;
+  static constexpr int kTurn = kVecs < L::kThreads ? kTile : L::kThreads / kPer;
+  static constexpr int kPitch = (kVecs < L::kThreads ? kVecs : L::kThreads) * VW;
+  static constexpr int kElements = 2 * TENSORS * kMine * kPitch;
+  static_assert(kVecs < L::kThreads || (L::kThreads % kPer == 0 && kVecs % L::kThreads == 0),
+                "a turn is a whole number of tokens");
+  T* s;
+  int t, ch;   // the first vector's token in the tile, and its channel there
+  bool has;    // whether the thread has vectors at all
+  bool in;     // and whether their channels exist
+  const T* p[TENSORS];  // it, in the tile to be fetched next
+  int64_t step[TENSORS];
+  __device__ __forceinline__ Raw(T* s, int64_t d0, int64_t dim)
+      : s(s), t(threadIdx.x / kPer), ch(threadIdx.x % kPer * VW),
+        has(kVecs >= L::kThreads || (int)threadIdx.x < kVecs), in(has && d0 + ch < dim) {}
+  __device__ __forceinline__ void open(int which, const SeqArg<T>& v, int64_t b, int64_t t0, int64_t d0) {
+    step[which] = v.st;
+    p[which] = v.p ? v.p + b * v.sb + (t0 + t) * v.st + d0 + ch : nullptr;
   }
+  __device__ __forceinline__ T* at(int buffer, int which, int k) const {
+    return s + ((buffer * TENSORS + which) * kMine + k) * kPitch + threadIdx.x * VW;
+  }
+  // Whether the thread's k-th vector is one of `left` tokens.
+  __device__ __forceinline__ bool on(int k, int left) const { return in && t + k * kTurn < left; }
+  // Asks for the next tile, `left` tokens of which are there; zeros for the others.
+  __device__ __forceinline__ void fetch(int which, int buffer, int left) {
+    if constexpr (kAsync) {
+#pragma unroll
+      for (int k = 0; k < kMine; ++k) {
+        if (!has) break;
+        const bool here = on(k, left);
+        const T* q = p[which] + k * kTurn * step[which];
+        copy_async<VW * (int)sizeof(T)>(at(buffer, which, k), here ? q : p[which], here);
+      }
+      p[which] += DIR * kTile * step[which];
+    } else {
+#pragma unroll
+      for (int k = 0; k < kMine; ++k)
+        if (on(k, left) && (threadIdx.x & 15) == 0)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(p[which] + k * kTurn * step[which]));
+    }
+  }
+  // The tile asked for last becomes readable.
+  __device__ __forceinline__ void land(int buffer, int left) {
+    if constexpr (kAsync) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    } else {
+      uint16_t v[TENSORS][kMine];
+#pragma unroll
+      for (int w = 0; w < TENSORS; ++w)
+#pragma unroll
+        for (int k = 0; k < kMine; ++k)
+          v[w][k] = load_if(p[w] + k * kTurn * step[w], p[w] && on(k, left));
+#pragma unroll
+      for (int w = 0; w < TENSORS; ++w) {
+        p[w] = p[w] ? p[w] + DIR * kTile * step[w] : nullptr;
+#pragma unroll
+        for (int k = 0; k < kMine; ++k)
+          if (has) *reinterpret_cast<uint16_t*>(at(buffer, w, k)) = v[w][k];
+      }
+    }
+  }
+  __device__ __forceinline__ void read(float (&f)[VW], int buffer, int which, int k) const {
+    const T* q = at(buffer, which, k);
+    if constexpr (VW == 4 && sizeof(T) == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(q);
+      f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    } else if constexpr (VW == 4) {
+      const uint2 v = *reinterpret_cast<const uint2*>(q);
+      f[0] = bf16_lo(v.x); f[1] = bf16_hi(v.x); f[2] = bf16_lo(v.y); f[3] = bf16_hi(v.y);
+    } else {
+      f[0] = to_f32(q[0]);
+    }
+  }
+};
+
+// VW entries of a [dim] vector from channel d on, `other` where there is none.
+template <int VW>
+__device__ __forceinline__ void load_channels(float (&v)[VW], const float* p, int64_t d, bool in,
+                                              float other) {
+#pragma unroll
+  for (int i = 0; i < VW; ++i) v[i] = p && in ? p[d + i] : other;
 }
 
-// Runs f(token of the tile, first channel of the tile, how many tokens in) for the
-// thread's vectors of a [kTile, kChannels] tile.
-template <class L, int VW, typename F>
-__device__ __forceinline__ void each_vec(F f) {
-  constexpr int kPer = L::kChannels / VW;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < kTile * kPer; i += L::kThreads) f(i / kPer, i % kPer * VW);
-}
-
-// The rows of B or C of a tile in f32, zero beyond N and the sequence.
-template <class L, typename T>
-__device__ __forceinline__ void stage_rows(float* s, const SeqArg<T>& v, int64_t b, int64_t t0,
-                                           int64_t length, int N) {
-  for (int i = threadIdx.x; i < kTile * L::NP; i += L::kThreads) {
-    const int t = i / L::NP, n = i % L::NP;
-    s[i] = n < N && t0 + t < length ? to_f32(v.p[b * v.sb + (t0 + t) * v.st + n]) : 0.0f;
+// The rows of B or C of a tile on the way to shared memory, zero beyond N and the
+// sequence: loaded a tile ahead.
+template <class L, typename T, int DIR>
+struct Rows {
+  static constexpr int kMine = (kTile * L::NP + L::kThreads - 1) / L::kThreads;
+  decltype(load_if((const T*)nullptr, true)) v[kMine];
+  const T* p;
+  int64_t step;
+  int t, n;
+  bool in;
+  __device__ __forceinline__ Rows(const SeqArg<T>& a, int64_t b, int64_t t0, int N) {
+    // a thread's entries are L::kThreads apart: its token and column by division where
+    // NP does not divide that
+    t = threadIdx.x / L::NP;
+    n = threadIdx.x % L::NP;
+    in = n < N;
+    step = a.st;
+    p = a.p + b * a.sb + t0 * a.st;
   }
+  __device__ __forceinline__ void load(int left, int N) {
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      if constexpr (L::kThreads % L::NP == 0) {
+        const int tk = t + k * (L::kThreads / L::NP);
+        v[k] = load_if(p + tk * step + n, in && tk < left);
+      } else {
+        const int i = k * L::kThreads + threadIdx.x, tk = i / L::NP, nk = i % L::NP;
+        v[k] = load_if(p + tk * step + nk, nk < N && tk < left);
+      }
+    }
+    p += DIR * kTile * step;
+  }
+  __device__ __forceinline__ void put(float* s) const {
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const int i = k * L::kThreads + threadIdx.x;
+      if (kTile * L::NP % L::kThreads == 0 || i < kTile * L::NP) s[i] = as_f32(v[k]);
+    }
+  }
+};
+
+// Runs f(std::true_type) where any of the tile's tokens starts a sequence, else
+// f(std::false_type), whose loops need no selects.
+template <typename F>
+__device__ __forceinline__ void by_fresh(unsigned int starts, F f) {
+  if (starts) f(std::true_type{});
+  else f(std::false_type{});
 }
 
 // The tile's tokens at which a sequence starts, a bit each (the same in all threads).
@@ -238,10 +407,10 @@ __device__ __forceinline__ unsigned int tile_starts(const uint8_t* starts, int64
 __device__ __forceinline__ float bounded(float v) { return v < -1e30f ? -1e30f : v > 1e30f ? 1e30f : v; }
 
 template <class L, typename T>
-__device__ __forceinline__ void load_decay(float2 (&A2)[2][L::P], const Place<L>& at,
+__device__ __forceinline__ void load_decay(float2 (&A2)[L::CPT][L::P], const Place<L>& at,
                                            const SelectiveArgs<T>& a) {
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < L::CPT; ++c) {
     at.load(A2[c], a.A, c, 0, a.dim, a.N);
 #pragma unroll
     for (int i = 0; i < L::P; ++i) {
@@ -254,12 +423,12 @@ __device__ __forceinline__ void load_decay(float2 (&A2)[2][L::P], const Place<L>
 
 // Takes a state from one end of segment `seg` to the other.
 template <class L, typename T>
-__device__ __forceinline__ void through_segment(float2 (&h)[2][L::P], const float2 (&A2)[2][L::P],
+__device__ __forceinline__ void through_segment(float2 (&h)[L::CPT][L::P], const float2 (&A2)[L::CPT][L::P],
                                                 const Place<L>& at, const SelectiveArgs<T>& a, int64_t b,
                                                 int seg) {
   const int64_t row = b * a.segments + seg;
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < L::CPT; ++c) {
     const float time = at.d + c < a.dim ? a.seg_time[row * a.dim + at.d + c] : 0.0f;
     float2 own[L::P];
     at.load(own, a.seg_state, c, row, a.dim, a.N);
@@ -291,24 +460,37 @@ inline auto by_state(int64_t N, F f) {
 #undef OXC_CASE
 }
 
-inline int64_t channel_tile(int64_t N) {
-  return by_state(N, [](auto spt, auto lpc) {
-    return (int64_t)Layout<float, decltype(spt)::value, decltype(lpc)::value>::kChannels;
-  });
-}
+template <int SPT, int LPC>
+using Forward = Layout<SPT, LPC, (LPC <= 4 ? 1 : 2), 8>;
+template <int SPT, int LPC>
+using Backward = Layout<SPT, LPC, 2, (LPC == 2 || SPT == 6 ? 4 : 8)>;
 
 struct Plan {
   int64_t ctiles;
   int segments, seg_tiles;
 };
 
-inline Plan selective_plan(int64_t batch, int64_t length, int64_t dim, int64_t N) {
+inline Plan selective_plan(int64_t batch, int64_t length, int64_t dim, int64_t N, bool backward) {
   Plan p;
-  const int64_t per = channel_tile(N);
+  const int64_t per = by_state(N, [&](auto spt, auto lpc) {
+    constexpr int SPT = decltype(spt)::value, LPC = decltype(lpc)::value;
+    return (int64_t)(backward ? Backward<SPT, LPC>::kChannels : Forward<SPT, LPC>::kChannels);
+  });
   p.ctiles = (dim + per - 1) / per;
   const int64_t tiles = std::max<int64_t>(1, selective_tiles(length));
-  int64_t segments = (2 * sm_count()) / std::max<int64_t>(1, batch * p.ctiles);
-  segments = std::max<int64_t>(1, std::min<int64_t>({segments, kMaxSegments, tiles / 4}));
+  const int64_t work = std::max<int64_t>(1, batch * p.ctiles), slots = (backward ? 1 : 2) * sm_count();
+  // the rounds of the grid, and the first kernel's share
+  const double map = backward ? 0.3 : 0.6;
+  double best = 0.0;
+  int64_t segments = 1;
+  for (int64_t k = 1; k <= std::min<int64_t>(kMaxSegments, std::max<int64_t>(1, tiles / 4)); ++k) {
+    const int64_t rounds = (work * k + slots - 1) / slots;
+    const double cost = (double)rounds / (double)k * (1.0 + map * (double)(k - 1) / (double)k);
+    if (k == 1 || cost < best * 0.98) {
+      best = cost;
+      segments = k;
+    }
+  }
   p.seg_tiles = (int)((tiles + segments - 1) / segments);
   p.segments = (int)((tiles + p.seg_tiles - 1) / p.seg_tiles);
   return p;
@@ -377,6 +559,8 @@ inline void selective_segments(SelectiveArgs<T>& a, const Plan& p, float* worksp
 }
 
 // Defined for each type by a file of its own.
+template <typename T>
+oxc_status selective_fwd_launch(const SelectiveArgs<T>& a, cudaStream_t s);
 template <typename T>
 oxc_status selective_bwd_launch(const SelectiveArgs<T>& a, float* out_sums, T* dB, T* dC, cudaStream_t s);
 
