@@ -19,8 +19,9 @@
 //
 // A thread keeps SPT states of each of CPT channels in registers, LPC threads side
 // by side share a channel, and the CTA's threads walk through the tokens in tiles of
-// kTile.  A tile's operands are copied to shared memory while the tile before it is
-// worked on, and turned into f32 steps (dt, dt x) there, once per token and channel.
+// kTile.  Four more warps prepare the tiles: they copy the operands to shared memory two
+// tiles ahead, turn them into f32 steps (dt, dt x) there, once per token and channel,
+// and finish and store a tile's outputs, while the others walk through the next one.
 // Sums over n are made across the LPC threads, sums over d across the warp's other
 // lanes, its warps and the CTAs.  The VJP gets the state before each tile from the
 // forward (`carry`) and goes through the tiles from the last to the first: it runs the
@@ -248,76 +249,106 @@ __device__ __forceinline__ void copy_async(void* dst, const void* src, bool on) 
   else
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(src), "r"(on ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ void copies_sent() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
-// A tile's operands as they are in memory, TENSORS of them twice over: thread i's
-// vectors lie where only thread i looks, so no barrier stands between its copies and
+// Barriers between the warps that prepare tiles and those that walk through them, one
+// pair for the even tiles and one for the odd: `full` when a tile is prepared, `done`
+// when it is walked through.  Who waits syncs, who goes on arrives.
+__device__ __forceinline__ void tile_sync(int id, int threads) {
+  __syncwarp();
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void tile_arrive(int id, int threads) {
+  __syncwarp();
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+constexpr int kFull = 1, kDone = 3;  // + the tile's parity
+
+// The threads that prepare tiles are behind those that walk through them.
+constexpr int kHelpers = 128;
+
+// A tile's operands as they are in memory, TENSORS of them DEPTH times over: helper i's
+// vectors lie where only helper i looks, so no barrier stands between its copies and
 // its reads.  A [kTile, kChannels] tile is cut into vectors of VW channels, dealt to the
-// threads token by token, kTurn tokens at a time: a thread's vectors are of the same
+// helpers token by token, kTurn tokens at a time: a thread's vectors are of the same
 // channels.  Where vectors are shorter than the 4 bytes that can be copied without
-// passing the registers, L2 is asked for the tile ahead and the copy made when it
-// begins.  DIR is 1 or -1, the direction through the tiles.
-template <class L, typename T, int VW, int TENSORS, int DIR>
+// passing the registers, they wait there if they are few; if not, L2 is asked for them
+// and the copy made when the tile begins.  DIR is 1 or -1, the direction through the
+// tiles.
+template <class L, typename T, int VW, int TENSORS, int DIR, int DEPTH>
 struct Raw {
+  static constexpr int kDepth = DEPTH;
   static constexpr bool kAsync = VW * sizeof(T) >= 4;
   static constexpr int kPer = L::kChannels / VW;  // vectors of a token
   static constexpr int kVecs = kTile * kPer;
-  static constexpr int kMine = (kVecs + L::kThreads - 1) / L::kThreads;
-  static constexpr int kTurn = kVecs < L::kThreads ? kTile : L::kThreads / kPer;
-  static constexpr int kPitch = (kVecs < L::kThreads ? kVecs : L::kThreads) * VW;
-  static constexpr int kElements = 2 * TENSORS * kMine * kPitch;
-  static_assert(kVecs < L::kThreads || (L::kThreads % kPer == 0 && kVecs % L::kThreads == 0),
+  static constexpr int kMine = (kVecs + kHelpers - 1) / kHelpers;
+  static constexpr int kTurn = kVecs < kHelpers ? kTile : kHelpers / kPer;
+  static constexpr int kPitch = (kVecs < kHelpers ? kVecs : kHelpers) * VW;
+  static constexpr int kElements = kDepth * TENSORS * kMine * kPitch;
+  static constexpr bool kHold = !kAsync && TENSORS * kMine <= 24;
+  static_assert(kVecs < kHelpers || (kHelpers % kPer == 0 && kVecs % kHelpers == 0),
                 "a turn is a whole number of tokens");
   T* s;
+  int me;      // the helper's number
   int t, ch;   // the first vector's token in the tile, and its channel there
   bool has;    // whether the thread has vectors at all
   bool in;     // and whether their channels exist
   const T* p[TENSORS];  // it, in the tile to be fetched next
   int64_t step[TENSORS];
-  __device__ __forceinline__ Raw(T* s, int64_t d0, int64_t dim)
-      : s(s), t(threadIdx.x / kPer), ch(threadIdx.x % kPer * VW),
-        has(kVecs >= L::kThreads || (int)threadIdx.x < kVecs), in(has && d0 + ch < dim) {}
+  uint16_t held[kHold ? TENSORS : 1][kHold ? kMine : 1];
+  __device__ __forceinline__ Raw(T* s, int me, int64_t d0, int64_t dim)
+      : s(s), me(me), t(me / kPer), ch(me % kPer * VW), has(kVecs >= kHelpers || me < kVecs),
+        in(has && d0 + ch < dim) {}
   __device__ __forceinline__ void open(int which, const SeqArg<T>& v, int64_t b, int64_t t0, int64_t d0) {
     step[which] = v.st;
     p[which] = v.p ? v.p + b * v.sb + (t0 + t) * v.st + d0 + ch : nullptr;
   }
   __device__ __forceinline__ T* at(int buffer, int which, int k) const {
-    return s + ((buffer * TENSORS + which) * kMine + k) * kPitch + threadIdx.x * VW;
+    return s + ((buffer * TENSORS + which) * kMine + k) * kPitch + me * VW;
   }
   // Whether the thread's k-th vector is one of `left` tokens.
   __device__ __forceinline__ bool on(int k, int left) const { return in && t + k * kTurn < left; }
-  // Asks for the next tile, `left` tokens of which are there; zeros for the others.
-  __device__ __forceinline__ void fetch(int which, int buffer, int left) {
-    if constexpr (kAsync) {
+  // Asks for the next tile, `left` tokens of which are there (none: the last was asked
+  // for already); zeros for the others.
+  __device__ __forceinline__ void fetch(int buffer, int left) {
+#pragma unroll
+    for (int w = 0; w < TENSORS; ++w) {
+      if (!p[w]) continue;
 #pragma unroll
       for (int k = 0; k < kMine; ++k) {
-        if (!has) break;
         const bool here = on(k, left);
-        const T* q = p[which] + k * kTurn * step[which];
-        copy_async<VW * (int)sizeof(T)>(at(buffer, which, k), here ? q : p[which], here);
+        const T* q = p[w] + k * kTurn * step[w];
+        if constexpr (kAsync) {
+          if (has && left > 0) copy_async<VW * (int)sizeof(T)>(at(buffer, w, k), here ? q : p[w], here);
+        } else if constexpr (kHold) {
+          held[w][k] = load_if(q, here);
+        } else {
+          if (here && (me & 15) == 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+        }
       }
-      p[which] += DIR * kTile * step[which];
-    } else {
-#pragma unroll
-      for (int k = 0; k < kMine; ++k)
-        if (on(k, left) && (threadIdx.x & 15) == 0)
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(p[which] + k * kTurn * step[which]));
+      if (kAsync || kHold) p[w] += DIR * kTile * step[w];
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  // The tile asked for last becomes readable.
+  // The oldest tile asked for becomes readable, of kDepth - 1 that are on the way (held
+  // ones: of one).
   __device__ __forceinline__ void land(int buffer, int left) {
     if constexpr (kAsync) {
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
     } else {
       uint16_t v[TENSORS][kMine];
 #pragma unroll
-      for (int w = 0; w < TENSORS; ++w)
+      for (int w = 0; w < TENSORS; ++w) {
+        if (!p[w]) continue;
 #pragma unroll
-        for (int k = 0; k < kMine; ++k)
-          v[w][k] = load_if(p[w] + k * kTurn * step[w], p[w] && on(k, left));
+        for (int k = 0; k < kMine; ++k) {
+          if constexpr (kHold) v[w][k] = held[w][k];
+          else v[w][k] = load_if(p[w] + k * kTurn * step[w], on(k, left));
+        }
+      }
 #pragma unroll
       for (int w = 0; w < TENSORS; ++w) {
-        p[w] = p[w] ? p[w] + DIR * kTile * step[w] : nullptr;
+        if (!p[w]) continue;
+        if (!kHold) p[w] += DIR * kTile * step[w];
 #pragma unroll
         for (int k = 0; k < kMine; ++k)
           if (has) *reinterpret_cast<uint16_t*>(at(buffer, w, k)) = v[w][k];
@@ -338,41 +369,32 @@ struct Raw {
   }
 };
 
-// VW entries of a [dim] vector from channel d on, `other` where there is none.
+// VW entries of a [dim] vector from channel d on, 0 where there is none.
 template <int VW>
-__device__ __forceinline__ void load_channels(float (&v)[VW], const float* p, int64_t d, bool in,
-                                              float other) {
+__device__ __forceinline__ void load_channels(float (&v)[VW], const float* p, int64_t d, bool in) {
 #pragma unroll
-  for (int i = 0; i < VW; ++i) v[i] = p && in ? p[d + i] : other;
+  for (int i = 0; i < VW; ++i) v[i] = p && in ? p[d + i] : 0.0f;
 }
 
 // The rows of B or C of a tile on the way to shared memory, zero beyond N and the
-// sequence: loaded a tile ahead.
+// sequence: in the helpers' registers from one tile to the next.
 template <class L, typename T, int DIR>
 struct Rows {
-  static constexpr int kMine = (kTile * L::NP + L::kThreads - 1) / L::kThreads;
+  static constexpr int kMine = (kTile * L::NP + kHelpers - 1) / kHelpers;
   decltype(load_if((const T*)nullptr, true)) v[kMine];
   const T* p;
   int64_t step;
-  int t, n;
-  bool in;
-  __device__ __forceinline__ Rows(const SeqArg<T>& a, int64_t b, int64_t t0, int N) {
-    // a thread's entries are L::kThreads apart: its token and column by division where
-    // NP does not divide that
-    t = threadIdx.x / L::NP;
-    n = threadIdx.x % L::NP;
-    in = n < N;
-    step = a.st;
-    p = a.p + b * a.sb + t0 * a.st;
-  }
+  int me, t, n;
+  __device__ __forceinline__ Rows(int me, const SeqArg<T>& a, int64_t b, int64_t t0)
+      : p(a.p + b * a.sb + t0 * a.st), step(a.st), me(me), t(me / L::NP), n(me % L::NP) {}
   __device__ __forceinline__ void load(int left, int N) {
 #pragma unroll
     for (int k = 0; k < kMine; ++k) {
-      if constexpr (L::kThreads % L::NP == 0) {
-        const int tk = t + k * (L::kThreads / L::NP);
-        v[k] = load_if(p + tk * step + n, in && tk < left);
+      if constexpr (kHelpers % L::NP == 0) {
+        const int tk = t + k * (kHelpers / L::NP);
+        v[k] = load_if(p + tk * step + n, n < N && tk < left);
       } else {
-        const int i = k * L::kThreads + threadIdx.x, tk = i / L::NP, nk = i % L::NP;
+        const int i = k * kHelpers + me, tk = i / L::NP, nk = i % L::NP;
         v[k] = load_if(p + tk * step + nk, nk < N && tk < left);
       }
     }
@@ -381,8 +403,8 @@ struct Rows {
   __device__ __forceinline__ void put(float* s) const {
 #pragma unroll
     for (int k = 0; k < kMine; ++k) {
-      const int i = k * L::kThreads + threadIdx.x;
-      if (kTile * L::NP % L::kThreads == 0 || i < kTile * L::NP) s[i] = as_f32(v[k]);
+      const int i = k * kHelpers + me;
+      if (kTile * L::NP % kHelpers == 0 || i < kTile * L::NP) s[i] = as_f32(v[k]);
     }
   }
 };
@@ -395,14 +417,29 @@ __device__ __forceinline__ void by_fresh(unsigned int starts, F f) {
   else f(std::false_type{});
 }
 
-// The tile's tokens at which a sequence starts, a bit each (the same in all threads).
-__device__ __forceinline__ unsigned int tile_starts(const uint8_t* starts, int64_t row, int64_t t0,
-                                                   int64_t length) {
-  if (!starts) return 0u;
-  const int lane = threadIdx.x & 31;
-  const bool s = lane < kTile && t0 + lane < length && starts[row * length + t0 + lane];
-  return __ballot_sync(0xffffffffu, s);
-}
+// A tile's tokens at which a sequence starts, a bit each (the same in all of a warp's
+// threads): read a tile ahead.
+struct Starts {
+  const uint8_t* row;
+  int64_t length;
+  uint8_t next;
+  __device__ __forceinline__ Starts(const uint8_t* starts, int64_t b, int64_t length, int64_t tile)
+      : row(starts ? starts + b * length : nullptr), length(length), next(0) {
+    load(tile);
+  }
+  __device__ __forceinline__ void load(int64_t tile) {
+    const int lane = threadIdx.x & 31;
+    const int64_t t = tile * kTile + lane;
+    if (row) next = lane < kTile && t >= 0 && t < length ? row[t] : (uint8_t)0;
+  }
+  // Those of the tile loaded last, and loads another.
+  __device__ __forceinline__ unsigned int bits(int64_t then) {
+    if (!row) return 0u;
+    const unsigned int b = __ballot_sync(0xffffffffu, next != 0);
+    load(then);
+    return b;
+  }
+};
 
 __device__ __forceinline__ float bounded(float v) { return v < -1e30f ? -1e30f : v > 1e30f ? 1e30f : v; }
 
@@ -462,8 +499,17 @@ inline auto by_state(int64_t N, F f) {
 
 template <int SPT, int LPC>
 using Forward = Layout<SPT, LPC, (LPC <= 4 ? 1 : 2), 8>;
-template <int SPT, int LPC>
-using Backward = Layout<SPT, LPC, 2, (LPC == 2 || SPT == 6 ? 4 : 8)>;
+// In the VJP 4 states a thread, the lanes a power of two.
+template <int LPC>
+using Backward = Layout<4, LPC, 2, (LPC == 2 ? 4 : 8)>;
+template <typename F>
+inline auto by_lanes(int64_t N, F f) {
+  if (N <= 8) return f(std::integral_constant<int, 2>{});
+  if (N <= 16) return f(std::integral_constant<int, 4>{});
+  if (N <= 32) return f(std::integral_constant<int, 8>{});
+  if (N <= 64) return f(std::integral_constant<int, 16>{});
+  return f(std::integral_constant<int, 32>{});
+}
 
 struct Plan {
   int64_t ctiles;
@@ -472,10 +518,11 @@ struct Plan {
 
 inline Plan selective_plan(int64_t batch, int64_t length, int64_t dim, int64_t N, bool backward) {
   Plan p;
-  const int64_t per = by_state(N, [&](auto spt, auto lpc) {
-    constexpr int SPT = decltype(spt)::value, LPC = decltype(lpc)::value;
-    return (int64_t)(backward ? Backward<SPT, LPC>::kChannels : Forward<SPT, LPC>::kChannels);
-  });
+  const int64_t per =
+      backward ? by_lanes(N, [](auto lpc) { return (int64_t)Backward<decltype(lpc)::value>::kChannels; })
+               : by_state(N, [](auto spt, auto lpc) {
+                   return (int64_t)Forward<decltype(spt)::value, decltype(lpc)::value>::kChannels;
+                 });
   p.ctiles = (dim + per - 1) / per;
   const int64_t tiles = std::max<int64_t>(1, selective_tiles(length));
   const int64_t work = std::max<int64_t>(1, batch * p.ctiles), slots = (backward ? 1 : 2) * sm_count();

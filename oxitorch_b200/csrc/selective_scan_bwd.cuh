@@ -6,41 +6,78 @@
 
 namespace oxc {
 
+template <class L, typename T, int VW>
+struct BackwardMapShared {
+  using R = Raw<L, T, VW, 3, -1, 2>;  // delta, dy, z
+  static constexpr int kIn = 2 * kTile * L::kChannels;  // dt, dy silu(z); twice, for the even tiles
+  static constexpr int kC = kTile * L::NP;              // and the odd, as C
+  static constexpr int kFloats = 2 * (kIn + kC);
+  static constexpr size_t kBytes = sizeof(float) * kFloats + sizeof(T) * R::kElements;
+};
+
 // What the segments from the second on do to mu, the gradient that flows out of
 // their first token.
 template <typename T, int SPT, int LPC, bool VEC>
-__global__ void __launch_bounds__(Forward<SPT, LPC>::kThreads)
+__global__ void __launch_bounds__(Forward<SPT, LPC>::kThreads + kHelpers, 2)
 selective_bwd_map_kernel(SelectiveArgs<T> a) {
   using L = Forward<SPT, LPC>;
-  constexpr int P = L::P, CPT = L::CPT, VW = VEC ? 4 : 1;
-  using R = Raw<L, T, VW, 3, -1>;  // delta, dy, z
+  constexpr int P = L::P, CPT = L::CPT, VW = VEC ? 4 : 1, kAll = L::kThreads + kHelpers;
+  using S = BackwardMapShared<L, T, VW>;
+  using R = typename S::R;
   extern __shared__ __align__(16) float smem[];
-  float2* s_in = reinterpret_cast<float2*>(smem);  // [kTile][kChannels] dt, dy silu(z)
-  float* s_C = smem + 2 * kTile * L::kChannels;
   const unsigned int ct = blockIdx.x % a.map_ctiles, rest = blockIdx.x / a.map_ctiles;
   const int64_t b = rest / (a.segments - 1);
   const int seg = 1 + rest % (a.segments - 1);
   const int64_t d0 = (int64_t)ct * L::kChannels;
-  const Place<L> at(d0);
   const int64_t tiles = (a.length + kTile - 1) / kTile;
-  const int64_t tile0 = (int64_t)seg * a.seg_tiles, tile1 = min(tiles, tile0 + a.seg_tiles);
-  R raw(reinterpret_cast<T*>(s_C + kTile * L::NP), d0, a.dim);
-  raw.open(0, a.delta, b, (tile1 - 1) * kTile, d0);
-  raw.open(1, a.dy, b, (tile1 - 1) * kTile, d0);
-  raw.open(2, a.z, b, (tile1 - 1) * kTile, d0);
-  Rows<L, T, -1> rows_C(a.C, b, (tile1 - 1) * kTile, a.N);
-  auto tokens = [&](int64_t tile) { return (int)min((int64_t)kTile, a.length - tile * kTile); };
-  auto fetch = [&](int64_t tile) {
-    const int left = tokens(tile), buffer = (int)tile & 1;
-    raw.fetch(0, buffer, left);
-    if (a.dy.p) raw.fetch(1, buffer, left);
-    if (a.z.p) raw.fetch(2, buffer, left);
-    copies_sent();
-    rows_C.load(left, a.N);
-  };
-  fetch(tile1 - 1);
-  float bias[VW];
-  load_channels(bias, a.delta_bias, d0 + raw.ch, raw.in, 0.0f);
+  const int64_t tile0 = (int64_t)seg * a.seg_tiles, end = min(tiles, tile0 + a.seg_tiles) - 1;
+  const int count = (int)(end + 1 - tile0);  // tile i of them is end - i
+  auto s_in = [&](int i) { return reinterpret_cast<float2*>(smem + (i & 1) * S::kIn); };
+  auto s_C = [&](int i) { return smem + 2 * S::kIn + (i & 1) * S::kC; };
+
+  if (threadIdx.x >= L::kThreads) {
+    const int me = threadIdx.x - L::kThreads;
+    R raw(reinterpret_cast<T*>(smem + S::kFloats), me, d0, a.dim);
+    raw.open(0, a.delta, b, end * kTile, d0);
+    raw.open(1, a.dy, b, end * kTile, d0);
+    raw.open(2, a.z, b, end * kTile, d0);
+    Rows<L, T, -1> rows_C(me, a.C, b, end * kTile);
+    auto tokens = [&](int i) {
+      return i < count ? (int)min((int64_t)kTile, a.length - (end - i) * kTile) : 0;
+    };
+    raw.fetch(0, tokens(0));
+    rows_C.load(tokens(0), a.N);
+    float bias[VW];
+    load_channels(bias, a.delta_bias, d0 + raw.ch, raw.in);
+    for (int i = 0; i < count; ++i) {
+      const int left = tokens(i), buffer = i & 1;
+      raw.land(buffer, left);
+      raw.fetch(buffer ^ 1, tokens(i + 1));
+      if (i > 1) tile_sync(kDone + (i & 1), kAll);
+#pragma unroll
+      for (int k = 0; k < R::kMine; ++k) {
+        if (!raw.has) break;
+        const bool on = raw.on(k, left);
+        float dt[VW], e[VW], z[VW];
+        raw.read(dt, buffer, 0, k);
+        if (a.dy.p) raw.read(e, buffer, 1, k);
+        if (a.z.p) raw.read(z, buffer, 2, k);
+#pragma unroll
+        for (int v = 0; v < VW; ++v) {
+          if (!a.dy.p) e[v] = 0.0f;
+          if (a.z.p) e[v] *= z[v] * sigmoid(z[v]);
+          dt[v] = on ? softplus(dt[v] + bias[v]) : 0.0f;
+          s_in(i)[(raw.t + k * R::kTurn) * L::kChannels + raw.ch + v] = make_float2(dt[v], e[v]);
+        }
+      }
+      rows_C.put(s_C(i));
+      tile_arrive(kFull + (i & 1), kAll);
+      rows_C.load(tokens(i + 1), a.N);
+    }
+    return;
+  }
+
+  const Place<L> at(d0);
   float2 A2[CPT][P], mu[CPT][P];
   load_decay<L>(A2, at, a);
   float time[CPT];
@@ -51,39 +88,22 @@ selective_bwd_map_kernel(SelectiveArgs<T> a) {
     for (int i = 0; i < P; ++i) mu[c][i] = both(0.0f);
   }
   bool fresh = false;
-  for (int64_t tile = tile1 - 1; tile >= tile0; --tile) {
-    const int left = tokens(tile), buffer = (int)tile & 1;
-    raw.land(buffer, left);
-#pragma unroll
-    for (int k = 0; k < R::kMine; ++k) {
-      if (!raw.has) break;
-      const bool on = raw.on(k, left);
-      float dt[VW], e[VW], z[VW];
-      raw.read(dt, buffer, 0, k);
-      if (a.dy.p) raw.read(e, buffer, 1, k);
-      if (a.z.p) raw.read(z, buffer, 2, k);
-#pragma unroll
-      for (int i = 0; i < VW; ++i) {
-        if (!a.dy.p) e[i] = 0.0f;
-        if (a.z.p) e[i] *= z[i] * sigmoid(z[i]);
-        dt[i] = on ? softplus(dt[i] + bias[i]) : 0.0f;
-        s_in[(raw.t + k * R::kTurn) * L::kChannels + raw.ch + i] = make_float2(dt[i], e[i]);
-      }
-    }
-    rows_C.put(s_C);
-    const unsigned int starts = tile_starts(a.starts, b, tile * kTile, a.length);
-    __syncthreads();
-    if (tile > tile0) fetch(tile - 1);
+  Starts ahead(a.starts, b, a.length, end);
+  for (int tile = 0; tile < count; ++tile) {
+    const unsigned int starts = ahead.bits(end - tile - 1);
     if (starts) fresh = true;
+    tile_sync(kFull + (tile & 1), kAll);
+    const float2* in_tile = s_in(tile) + at.ch;
+    const float* C_tile = s_C(tile) + at.sl * SPT;
     by_fresh(starts, [&](auto some) {
 #pragma unroll 4
       for (int t = kTile - 1; t >= 0; --t) {
         float2 C[P];
-        load_states<SPT>(C, s_C + t * L::NP + at.sl * SPT);
+        load_states<SPT>(C, C_tile + t * L::NP);
         const bool start = decltype(some)::value && ((starts >> t) & 1u);
 #pragma unroll
         for (int c = 0; c < CPT; ++c) {
-          const float2 in = s_in[t * L::kChannels + at.ch + c];
+          const float2 in = in_tile[t * L::kChannels + c];
 #pragma unroll
           for (int i = 0; i < P; ++i) {
             const float2 decay = exp2_pair(__fmul2_rn(A2[c][i], both(in.x)));
@@ -94,7 +114,7 @@ selective_bwd_map_kernel(SelectiveArgs<T> a) {
         }
       }
     });
-    __syncthreads();
+    if (tile + 2 < count) tile_arrive(kDone + (tile & 1), kAll);
   }
   const int64_t row = b * a.segments + seg;
 #pragma unroll
@@ -125,77 +145,195 @@ struct Shares {
 
 template <class L, typename T, int VW, bool GATED>
 struct BackwardShared {
-  using R = Raw<L, T, VW, GATED ? 4 : 3, -1>;
+  using R = Raw<L, T, VW, GATED ? 4 : 3, -1, 2>;  // x, delta, dy, z
   using S = Shares<L, GATED>;
   static constexpr int kParts = kTile / kBack;
-  static constexpr int kPlane = kTile * L::kChannels;
-  static constexpr int kIn = 4 * kPlane;                       // dt, dt x, e, -; later -, rate, -, through
-  static constexpr int kInner = GATED ? kPlane : 0;
-  static constexpr int kRows = L::kWarps * kTile * 2 * L::NP;  // dB, dC of each warp
-  static constexpr int kKept = kParts * L::CPT * L::SPT * L::kThreads;
-  static constexpr int kFloats =
-      kIn + kInner + 2 * kTile * L::NP + kRows + kKept + L::kWarps * S::kFloats;
+  // twice each, for the even tiles and the odd
+  static constexpr int kIn = 4 * kTile * L::kChannels;         // [kTile][kChannels] of four: dt, dt x, e,
+                                                               // nothing; afterwards dt, rate / ln 2,
+                                                               // inner - D x, through
+  static constexpr int kBC = 2 * kTile * L::NP;                // [kTile][NP]
+  static constexpr int kRows = L::kWarps * kTile * 2 * L::NP;  // [kWarps][kTile][2 NP]: dB, dC, once
+  static constexpr int kKept = (kParts - 1) * L::CPT * L::SPT * L::kThreads;  // [..][2 P][kThreads]
+  static constexpr int kFloats = 2 * (kIn + kBC) + kRows + kKept + L::kWarps * S::kFloats;
   static constexpr size_t kBytes = sizeof(float) * kFloats + sizeof(T) * R::kElements;
 };
 
-template <typename T, int SPT, int LPC, bool VEC, bool GATED>
-__global__ void __launch_bounds__(Backward<SPT, LPC>::kThreads)
+constexpr int kRowsFree = 5;  // the barrier after which the rows of the tile before are read
+
+// Of the registers that a CTA of 8 + 4 warps is launched with (168 a thread) the helpers
+// pass 80 each on: 256 x 208 + 128 x 88 = 384 x 168.
+template <bool TAKE>
+__device__ __forceinline__ void share_registers() {
+  if constexpr (TAKE) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+}
+
+template <typename T, int LPC, bool VEC, bool GATED>
+__global__ void __launch_bounds__(Backward<LPC>::kThreads + kHelpers, 1)
 selective_bwd_kernel(SelectiveArgs<T> a) {
-  using L = Backward<SPT, LPC>;
-  constexpr int P = L::P, CPT = L::CPT, VW = VEC ? 4 : 1;
-  static_assert(CPT == 2, "two channels a thread");
+  using L = Backward<LPC>;
+  constexpr int SPT = L::SPT, P = L::P, CPT = L::CPT, VW = VEC ? 4 : 1, kAll = L::kThreads + kHelpers;
+  static_assert(CPT == 2 && SPT == 4, "the shares are vectors");
   using M = BackwardShared<L, T, VW, GATED>;
-  using R = typename M::R;  // x, delta, dy, z
+  using R = typename M::R;
   using S = typename M::S;
   constexpr int kParts = M::kParts;
   extern __shared__ __align__(16) float smem[];
-  float4* s_in = reinterpret_cast<float4*>(smem);
-  float* s_inner = smem + M::kIn;          // inner - D x
-  float* s_B = s_inner + M::kInner;        // [kTile][NP]
-  float* s_C = s_B + kTile * L::NP;
-  float* s_rows = s_C + kTile * L::NP;     // [kWarps][kTile][2 NP]
-  float2* s_kept = reinterpret_cast<float2*>(s_rows + M::kRows);  // [kParts][2 P][kThreads]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cl = lane / LPC;
-  float* share_rows = s_rows + M::kRows + M::kKept + warp * S::kFloats;
-  float* share_sums = share_rows + S::kRowFloats;
+  float* s_rows = smem + 2 * (M::kIn + M::kBC);
   const unsigned int ct = blockIdx.x % a.ctiles, rest = blockIdx.x / a.ctiles;
   const int64_t b = rest / a.segments;
   const int seg = rest % a.segments;
   const int64_t d0 = (int64_t)ct * L::kChannels;
-  const Place<L> at(d0);
   const int64_t tiles = (a.length + kTile - 1) / kTile;
-  const int64_t tile0 = (int64_t)seg * a.seg_tiles, tile1 = min(tiles, tile0 + a.seg_tiles);
-  R raw(reinterpret_cast<T*>(smem + M::kFloats), d0, a.dim);
-  const int64_t end0 = (tile1 - 1) * kTile;
-  raw.open(0, a.x, b, end0, d0);
-  raw.open(1, a.delta, b, end0, d0);
-  raw.open(2, a.dy, b, end0, d0);
-  if (GATED) raw.open(GATED ? 3 : 0, a.z, b, end0, d0);
-  Rows<L, T, -1> rows_B(a.B, b, end0, a.N), rows_C(a.C, b, end0, a.N);
-  float2 enter[CPT][P];  // the state before the next tile
-  auto tokens = [&](int64_t tile) { return (int)min((int64_t)kTile, a.length - tile * kTile); };
-  auto fetch = [&](int64_t tile) {
-    const int left = tokens(tile), buffer = (int)tile & 1;
-    raw.fetch(0, buffer, left);
-    raw.fetch(1, buffer, left);
-    if (a.dy.p) raw.fetch(2, buffer, left);
-    if (GATED) raw.fetch(GATED ? 3 : 0, buffer, left);
-    copies_sent();
-    rows_B.load(left, a.N);
-    rows_C.load(left, a.N);
+  const int64_t tile0 = (int64_t)seg * a.seg_tiles, end = min(tiles, tile0 + a.seg_tiles) - 1;
+  const int count = (int)(end + 1 - tile0);  // tile i of them is end - i
+  auto in_of = [&](int i) { return reinterpret_cast<float4*>(smem + (i & 1) * M::kIn); };
+  auto B_of = [&](int i) { return smem + 2 * M::kIn + (i & 1) * M::kBC; };
+  float* sums = a.sums + (b * a.segments + seg) * (a.dim * a.N + 2 * a.dim);
+
+  if (threadIdx.x >= L::kThreads) {
+    if constexpr (L::kWarps == 8) share_registers<false>();
+    const int me = threadIdx.x - L::kThreads;
+    R raw(reinterpret_cast<T*>(smem + M::kFloats), me, d0, a.dim);
+    raw.open(0, a.x, b, end * kTile, d0);
+    raw.open(1, a.delta, b, end * kTile, d0);
+    raw.open(2, a.dy, b, end * kTile, d0);
+    if (GATED) raw.open(GATED ? 3 : 0, a.z, b, end * kTile, d0);
+    Rows<L, T, -1> rows_B(me, a.B, b, end * kTile), rows_C(me, a.C, b, end * kTile);
+    auto tokens = [&](int i) {
+      return i < count ? (int)min((int64_t)kTile, a.length - (end - i) * kTile) : 0;
+    };
+    raw.fetch(0, tokens(0));
+    rows_B.load(tokens(0), a.N);
+    rows_C.load(tokens(0), a.N);
+    float bias[VW], skip[VW];      // of the thread's vectors
+    float dD[VW], dbias[VW];       // and their sums
+    load_channels(bias, a.delta_bias, d0 + raw.ch, raw.in);
+    load_channels(skip, a.D, d0 + raw.ch, raw.in);
 #pragma unroll
-    for (int c = 0; c < CPT; ++c) at.load(enter[c], a.carry, c, b * tiles + tile, a.dim, a.N);
-  };
-  fetch(tile1 - 1);
-  float bias[VW], skip[VW];  // of the thread's vectors
-  load_channels(bias, a.delta_bias, d0 + raw.ch, raw.in, 0.0f);
-  load_channels(skip, a.D, d0 + raw.ch, raw.in, 0.0f);
-  int64_t out = (b * a.length + end0 + raw.t) * a.dim + d0 + raw.ch;
-  float2 A2[CPT][P], mu[CPT][P], dA[CPT][P];
+    for (int v = 0; v < VW; ++v) dD[v] = dbias[v] = 0.0f;
+    int64_t out = (b * a.length + end * kTile + raw.t) * a.dim + d0 + raw.ch;
+    float* row_out = a.rows + ((int64_t)ct * a.batch * a.length + b * a.length + end * kTile) * 2 * a.N;
+    for (int i = 0; i <= count; ++i) {
+      if (i < count) {
+        const int left = tokens(i), buffer = i & 1;
+        raw.land(buffer, left);
+#pragma unroll 2
+        for (int k = 0; k < R::kMine; ++k) {
+          if (!raw.has) break;
+          const bool on = raw.on(k, left);
+          float x[VW], dt[VW], e[VW], z[VW];
+          raw.read(x, buffer, 0, k);
+          raw.read(dt, buffer, 1, k);
+          if (a.dy.p) raw.read(e, buffer, 2, k);
+          if (GATED) raw.read(z, buffer, GATED ? 3 : 0, k);
+          float4* to = in_of(i) + (raw.t + k * R::kTurn) * L::kChannels + raw.ch;
+#pragma unroll
+          for (int v = 0; v < VW; ++v) {
+            if (!a.dy.p) e[v] = 0.0f;
+            if (GATED) e[v] *= z[v] * sigmoid(z[v]);
+            dt[v] = on ? softplus(dt[v] + bias[v]) : 0.0f;
+            to[v] = make_float4(dt[v], dt[v] * x[v], e[v], 0.0f);
+          }
+        }
+        rows_B.put(B_of(i));
+        rows_C.put(B_of(i) + kTile * L::NP);
+        tile_arrive(kFull + (i & 1), kAll);
+        rows_B.load(tokens(i + 1), a.N);
+        rows_C.load(tokens(i + 1), a.N);
+      }
+      if (i > 0) {
+        tile_sync(kDone + ((i - 1) & 1), kAll);
+        const int left = tokens(i - 1), buffer = (i - 1) & 1;
+        // dB and dC over the warps
+        for (int o = me; o < kTile * L::NP / 2; o += kHelpers) {
+          const int t = o / (L::NP / 2), n = o % (L::NP / 2) * 4;  // four at a time
+          const float* p = s_rows + t * 2 * L::NP + n;
+          float4 s = *reinterpret_cast<const float4*>(p);
+#pragma unroll
+          for (int w = 1; w < L::kWarps; ++w) {
+            const float4 q = *reinterpret_cast<const float4*>(p + w * kTile * 2 * L::NP);
+            s.x += q.x; s.y += q.y; s.z += q.z; s.w += q.w;
+          }
+          const int what = n / L::NP, first = n % L::NP;
+          float* to = row_out + t * 2 * a.N + what * a.N + first;
+          if (t < left) {
+            if (first < a.N) to[0] = s.x;
+            if (first + 1 < a.N) to[1] = s.y;
+            if (first + 2 < a.N) to[2] = s.z;
+            if (first + 3 < a.N) to[3] = s.w;
+          }
+        }
+        row_out -= kTile * 2 * a.N;
+        if (i < count) tile_arrive(kRowsFree, kAll);
+#pragma unroll 2
+        for (int k = 0; k < R::kMine; ++k) {
+          if (!raw.on(k, left)) break;
+          const float4* from = in_of(i - 1) + (raw.t + k * R::kTurn) * L::kChannels + raw.ch;
+          const int64_t to = out + k * R::kTurn * a.dim;
+          float x[VW], d[VW], dx[VW], e[VW], z[VW], dz[VW];
+          raw.read(x, buffer, 0, k);
+          raw.read(d, buffer, 1, k);
+          if (a.dy.p) raw.read(e, buffer, 2, k);
+          if (GATED) raw.read(z, buffer, GATED ? 3 : 0, k);
+#pragma unroll
+          for (int v = 0; v < VW; ++v) {
+            const float4 in = from[v];
+            if (!a.dy.p) e[v] = 0.0f;
+            if (GATED) {
+              const float s = sigmoid(z[v]);
+              dz[v] = e[v] * fmaf(skip[v], x[v], in.z) * fmaf(z[v] * s, 1.0f - s, s);
+              e[v] *= z[v] * s;
+            }
+            dx[v] = fmaf(in.x, in.w, skip[v] * e[v]);
+            const float ddt = fmaf(x[v], in.w, kLn2 * in.y);
+            d[v] = ddt * sigmoid(d[v] + bias[v]);
+            dD[v] = fmaf(e[v], x[v], dD[v]);
+            dbias[v] += d[v];
+          }
+          store_from_f32<VW>(a.dx + to, dx);
+          store_from_f32<VW>(a.ddelta + to, d);
+          if (GATED) store_from_f32<VW>(a.dz + to, dz);
+        }
+        out -= kTile * a.dim;
+      }
+      raw.fetch((i + 1) & 1, tokens(i + 1));  // where the tile just stored was
+    }
+    // dD and ddelta_bias over the threads with the same channels, where tile 0 or 1 was
+    float* s = smem;
+    sums += a.dim * a.N;
+    tile_sync(kRowsFree + 1, kHelpers);
+    if (raw.has) {
+#pragma unroll
+      for (int v = 0; v < VW; ++v) {
+        s[raw.t * L::kChannels + raw.ch + v] = dD[v];
+        s[(R::kTurn + raw.t) * L::kChannels + raw.ch + v] = dbias[v];
+      }
+    }
+    tile_sync(kRowsFree + 1, kHelpers);
+    for (int o = me; o < 2 * L::kChannels; o += kHelpers) {
+      const int ch = o % L::kChannels, what = o / L::kChannels;
+      float v = 0.0f;
+      for (int k = 0; k < R::kTurn; ++k) v += s[(what * R::kTurn + k) * L::kChannels + ch];
+      if (d0 + ch < a.dim) sums[what * a.dim + d0 + ch] = v;
+    }
+    pdl_launch_dependents();
+    return;
+  }
+
+  if constexpr (L::kWarps == 8) share_registers<true>();
+  const Place<L> at(d0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cl = lane / LPC;
+  float2* s_kept = reinterpret_cast<float2*>(s_rows + M::kRows);
+  float* share_rows = s_rows + M::kRows + M::kKept + warp * S::kFloats;
+  float* share_sums = share_rows + S::kRowFloats;
+  float2 A2[CPT][P], mu[CPT][P], dA[CPT][P], enter[CPT][P];  // enter: the state before the next tile
   load_decay<L>(A2, at, a);
 #pragma unroll
   for (int c = 0; c < CPT; ++c) {
     at.load(mu[c], a.dlast, c, b, a.dim, a.N);
+    at.load(enter[c], a.carry, c, b * tiles + end, a.dim, a.N);
 #pragma unroll
     for (int i = 0; i < P; ++i) dA[c][i] = both(0.0f);
   }
@@ -203,43 +341,24 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
     pdl_wait();
     for (int k = a.segments - 1; k > seg; --k) through_segment<L>(mu, A2, at, a, b, k);
   }
-  // this thread's columns of dD and ddelta_bias: those of its vectors
-  float dD[VW], dbias[VW];
-#pragma unroll
-  for (int k = 0; k < VW; ++k) dD[k] = dbias[k] = 0.0f;
-  for (int64_t tile = tile1 - 1; tile >= tile0; --tile) {
-    const int left = tokens(tile), buffer = (int)tile & 1;
-    raw.land(buffer, left);
-#pragma unroll
-    for (int k = 0; k < R::kMine; ++k) {
-      if (!raw.has) break;
-      const bool on = raw.on(k, left);
-      float x[VW], dt[VW], e[VW], z[VW];
-      raw.read(x, buffer, 0, k);
-      raw.read(dt, buffer, 1, k);
-      if (a.dy.p) raw.read(e, buffer, 2, k);
-      if (GATED) raw.read(z, buffer, GATED ? 3 : 0, k);
-#pragma unroll
-      for (int i = 0; i < VW; ++i) {
-        if (!a.dy.p) e[i] = 0.0f;
-        if (GATED) e[i] *= z[i] * sigmoid(z[i]);
-        dt[i] = on ? softplus(dt[i] + bias[i]) : 0.0f;
-        s_in[(raw.t + k * R::kTurn) * L::kChannels + raw.ch + i] = make_float4(dt[i], dt[i] * x[i], e[i], 0.0f);
-      }
-    }
-    rows_B.put(s_B);
-    rows_C.put(s_C);
-    const unsigned int starts = tile_starts(a.starts, b, tile * kTile, a.length);
+  auto kept = [&](int j, int c, int i) -> float2& {
+    return s_kept[((j * CPT + c) * P + i) * L::kThreads + threadIdx.x];
+  };
+  Starts ahead(a.starts, b, a.length, end);
+  for (int tile = 0; tile < count; ++tile) {
+    const unsigned int starts = ahead.bits(end - tile - 1);
     float2 h[CPT][P];
 #pragma unroll
     for (int c = 0; c < CPT; ++c)
 #pragma unroll
       for (int i = 0; i < P; ++i) h[c][i] = enter[c][i];
-    __syncthreads();
-    if (tile > tile0) fetch(tile - 1);
-    auto kept = [&](int j, int c, int i) -> float2& {
-      return s_kept[((j * CPT + c) * P + i) * L::kThreads + threadIdx.x];
-    };
+    if (tile + 1 < count) {
+#pragma unroll
+      for (int c = 0; c < CPT; ++c) at.load(enter[c], a.carry, c, b * tiles + end - tile - 1, a.dim, a.N);
+    }
+    float4* s_in = in_of(tile);
+    const float *s_B = B_of(tile), *s_C = s_B + kTile * L::NP;
+    tile_sync(kFull + (tile & 1), kAll);
     by_fresh(starts, [&](auto some) {
       constexpr bool kSome = decltype(some)::value;
       // the operands of kBack tokens: all read before anything is stored, as the compiler
@@ -279,6 +398,7 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
           forward(j * kBack, k, e, h);
         }
       }
+      if (tile > 0) tile_sync(kRowsFree, kAll);
 #pragma unroll 1
       for (int j = kParts - 1; j >= 0; --j) {
         float2 enters[CPT][P], decay[kBack][CPT][P], state[kBack][CPT][P], Cs[kBack][P];
@@ -335,16 +455,8 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
                 make_float2(inner[0].x + inner[0].y, inner[1].x + inner[1].y);
           float* row = L::kLanes > 1 ? share_rows + (slot * L::kLanes + cl) * S::kRow + at.sl * SPT
                                      : s_rows + (warp * kTile + t) * 2 * L::NP + at.sl * SPT;
-          if constexpr (SPT == 4) {
-            *reinterpret_cast<float4*>(row) = make_float4(dB[0].x, dB[0].y, dB[1].x, dB[1].y);
-            *reinterpret_cast<float4*>(row + L::NP) = make_float4(dC[0].x, dC[0].y, dC[1].x, dC[1].y);
-          } else {
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-              reinterpret_cast<float2*>(row)[i] = dB[i];
-              reinterpret_cast<float2*>(row + L::NP)[i] = dC[i];
-            }
-          }
+          *reinterpret_cast<float4*>(row) = make_float4(dB[0].x, dB[0].y, dB[1].x, dB[1].y);
+          *reinterpret_cast<float4*>(row + L::NP) = make_float4(dC[0].x, dC[0].y, dC[1].x, dC[1].y);
           if (slot) continue;
           // the sums of tokens t and t + 1
           __syncwarp();
@@ -375,88 +487,30 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
             float2 r = *reinterpret_cast<const float2*>(p);
 #pragma unroll
             for (int k = 1; k < LPC; ++k) r = __fadd2_rn(r, *reinterpret_cast<const float2*>(p + k * S::kSum));
-            const int to = (t + token) * L::kChannels + warp * L::kWarpChannels + ch;
-            if (what == 0) {  // dt x has been used
-              s_in[to].w = r.x;
-              s_in[to + 1].w = r.y;
-            } else if (what == 1) {
-              s_in[to].y = r.x;
-              s_in[to + 1].y = r.y;
+            float4* to = s_in + (t + token) * L::kChannels + warp * L::kWarpChannels + ch;
+            if (what == 0) {
+              to[0].w = r.x;
+              to[1].w = r.y;
+            } else if (what == 1) {  // dt x and e have been used
+              to[0].y = r.x;
+              to[1].y = r.y;
             } else {
-              *reinterpret_cast<float2*>(s_inner + to) = r;
+              to[0].z = r.x;
+              to[1].z = r.y;
             }
           }
           __syncwarp();
         }
       }
     });
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < R::kMine; ++k) {
-      if (!raw.on(k, left)) break;
-      const int at0 = (raw.t + k * R::kTurn) * L::kChannels + raw.ch;
-      const int64_t to = out + k * R::kTurn * a.dim;
-      float x[VW], v[VW], dx[VW], e[VW];
-      raw.read(x, buffer, 0, k);
-      raw.read(v, buffer, 1, k);
-#pragma unroll
-      for (int i = 0; i < VW; ++i) {
-        const float4 in = s_in[at0 + i];  // dt, rate / ln 2, e, through
-        dx[i] = fmaf(in.x, in.w, skip[i] * in.z);
-        const float ddt = fmaf(x[i], in.w, kLn2 * in.y);
-        v[i] = ddt * sigmoid(v[i] + bias[i]);
-        dD[i] = fmaf(in.z, x[i], dD[i]);
-        dbias[i] += v[i];
-      }
-      store_from_f32<VW>(a.dx + to, dx);
-      store_from_f32<VW>(a.ddelta + to, v);
-      if (GATED) {
-        raw.read(v, buffer, GATED ? 3 : 0, k);
-        if (a.dy.p) raw.read(e, buffer, 2, k);
-#pragma unroll
-        for (int i = 0; i < VW; ++i) {
-          const float s = sigmoid(v[i]), inner = fmaf(skip[i], x[i], s_inner[at0 + i]);
-          v[i] = (a.dy.p ? e[i] : 0.0f) * inner * fmaf(v[i] * s, 1.0f - s, s);
-        }
-        store_from_f32<VW>(a.dz + to, v);
-      }
-    }
-    out -= kTile * a.dim;
-    for (int i = threadIdx.x; i < kTile * 2 * L::NP; i += L::kThreads) {
-      const int t = i / (2 * L::NP), k = i % (2 * L::NP), n = k % L::NP;
-      if (t < left && n < a.N) {
-        float s = s_rows[i];
-#pragma unroll
-        for (int w = 1; w < L::kWarps; ++w) s += s_rows[w * kTile * 2 * L::NP + i];
-        a.rows[((int64_t)ct * a.batch * a.length + b * a.length + tile * kTile + t) * 2 * a.N +
-               (k < L::NP ? 0 : a.N) + n] = s;
-      }
-    }
-    __syncthreads();
+    tile_arrive(kDone + (tile & 1), kAll);
   }
   if (seg == 0) {
 #pragma unroll
     for (int c = 0; c < CPT; ++c) at.store(mu[c], a.dh0, c, b, a.dim, a.N);
   }
-  float* sums = a.sums + (b * a.segments + seg) * (a.dim * a.N + 2 * a.dim);
 #pragma unroll
   for (int c = 0; c < CPT; ++c) at.store(dA[c], sums, c, 0, a.dim, a.N);
-  // dD and ddelta_bias over the threads with the same channels
-  constexpr int kSame = R::kTurn;
-  sums += a.dim * a.N;
-#pragma unroll
-  for (int k = 0; k < VW; ++k) {
-    if (raw.t >= kSame) break;
-    smem[raw.t * L::kChannels + raw.ch + k] = dD[k];
-    smem[(kSame + raw.t) * L::kChannels + raw.ch + k] = dbias[k];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 2 * L::kChannels; i += L::kThreads) {
-    const int ch = i % L::kChannels, what = i / L::kChannels;
-    float s = 0.0f;
-    for (int k = 0; k < kSame; ++k) s += smem[(what * kSame + k) * L::kChannels + ch];
-    if (d0 + ch < a.dim) sums[what * a.dim + d0 + ch] = s;
-  }
   pdl_launch_dependents();
 }
 
@@ -476,14 +530,24 @@ __global__ void __launch_bounds__(256) selective_rows_kernel(const float* __rest
   (k < N ? dB : dC)[token * N + (k < N ? k : k - N)] = from_f32<T>(s);
 }
 
-template <typename T, int SPT, int LPC, bool VEC, bool GATED>
+template <typename T, int LPC, bool VEC, bool GATED>
 static cudaError_t selective_bwd_one(const SelectiveArgs<T>& a, cudaStream_t s) {
-  using L = Backward<SPT, LPC>;
-  constexpr size_t smem = BackwardShared<L, T, VEC ? 4 : 1, GATED>::kBytes;
-  static_assert(smem <= 227 * 1024, "a CTA's shared memory");
-  static_assert(sizeof(float) * 2 * L::kThreads * (VEC ? 4 : 1) <= smem, "dD and ddelta_bias fit");
-  return launch_scan(selective_bwd_kernel<T, SPT, LPC, VEC, GATED>,
-                     (unsigned int)(a.batch * a.ctiles) * a.segments, L::kThreads, smem,
+  using L = Backward<LPC>;
+  using M = BackwardShared<L, T, VEC ? 4 : 1, GATED>;
+  static_assert(M::kBytes <= 227 * 1024, "a CTA's shared memory");
+  static_assert(2 * M::R::kTurn * L::kChannels <= 2 * M::kIn, "dD and ddelta_bias fit");
+  if (L::kWarps == 8) {  // what share_registers deals out has to be there, or it would wait for ever
+    static int registers = 0;
+    if (registers == 0) {
+      cudaFuncAttributes attr;
+      const cudaError_t e = cudaFuncGetAttributes(&attr, selective_bwd_kernel<T, LPC, VEC, GATED>);
+      if (e != cudaSuccess) return e;
+      registers = attr.numRegs;
+    }
+    if (registers != 168) return cudaErrorLaunchOutOfResources;
+  }
+  return launch_scan(selective_bwd_kernel<T, LPC, VEC, GATED>,
+                     (unsigned int)(a.batch * a.ctiles) * a.segments, L::kThreads + kHelpers, M::kBytes,
                      a.segments > 1, s, a);
 }
 
@@ -493,23 +557,25 @@ oxc_status selective_bwd_launch(const SelectiveArgs<T>& a, float* out_sums, T* d
   const bool vec = a.dim % 4 == 0 && seq_vec(a.x) && seq_vec(a.delta) && seq_vec(a.z) &&
                    seq_vec(a.dy) && aligned_to(a.dx, 4 * sizeof(T)) &&
                    aligned_to(a.ddelta, 4 * sizeof(T)) && aligned_to(a.dz, 4 * sizeof(T));
-  cudaError_t err = by_state(a.N, [&](auto spt, auto lpc) -> cudaError_t {
-    constexpr int SPT = decltype(spt)::value, LPC = decltype(lpc)::value;
-    if (a.segments > 1) {
+  cudaError_t err = cudaSuccess;
+  if (a.segments > 1)
+    err = by_state(a.N, [&](auto spt, auto lpc) {
+      constexpr int SPT = decltype(spt)::value, LPC = decltype(lpc)::value;
       using L = Forward<SPT, LPC>;
       SelectiveArgs<T> m = a;
       m.map_ctiles = (unsigned int)((a.dim + L::kChannels - 1) / L::kChannels);
-      auto map = vec ? selective_bwd_map_kernel<T, SPT, LPC, true>
-                     : selective_bwd_map_kernel<T, SPT, LPC, false>;
-      const size_t smem = sizeof(float) * kTile * (2 * L::kChannels + L::NP) +
-                          sizeof(T) * (vec ? Raw<L, T, 4, 3, -1>::kElements : Raw<L, T, 1, 3, -1>::kElements);
-      const cudaError_t e = launch_scan(map, (unsigned int)a.batch * m.map_ctiles * (a.segments - 1),
-                                        L::kThreads, smem, false, s, m);
-      if (e != cudaSuccess) return e;
-    }
+      return launch_scan(vec ? selective_bwd_map_kernel<T, SPT, LPC, true>
+                             : selective_bwd_map_kernel<T, SPT, LPC, false>,
+                         (unsigned int)a.batch * m.map_ctiles * (a.segments - 1), L::kThreads + kHelpers,
+                         vec ? BackwardMapShared<L, T, 4>::kBytes : BackwardMapShared<L, T, 1>::kBytes,
+                         false, s, m);
+    });
+  if (err != cudaSuccess) return cuda_fail(err, "oxc_selective_scan_bwd");
+  err = by_lanes(a.N, [&](auto lpc) {
+    constexpr int LPC = decltype(lpc)::value;
     if (a.z.p)
-      return vec ? selective_bwd_one<T, SPT, LPC, true, true>(a, s) : selective_bwd_one<T, SPT, LPC, false, true>(a, s);
-    return vec ? selective_bwd_one<T, SPT, LPC, true, false>(a, s) : selective_bwd_one<T, SPT, LPC, false, false>(a, s);
+      return vec ? selective_bwd_one<T, LPC, true, true>(a, s) : selective_bwd_one<T, LPC, false, true>(a, s);
+    return vec ? selective_bwd_one<T, LPC, true, false>(a, s) : selective_bwd_one<T, LPC, false, false>(a, s);
   });
   if (err != cudaSuccess) return cuda_fail(err, "oxc_selective_scan_bwd");
   const int64_t tokens = a.batch * a.length, n = tokens * 2 * a.N;
