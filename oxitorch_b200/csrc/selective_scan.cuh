@@ -191,12 +191,17 @@ __device__ __forceinline__ float as_f32(uint16_t v) { return __uint_as_float((ui
 // Where a thread's states are.
 template <class L>
 struct Place {
-  int sl, ch;    // its lane among a channel's, its first channel in the tile
+  int sl, cl;    // its lane among a channel's, and over channels
+  int ch;        // its first channel in the tile; the others are kLanes apart
   int64_t d;     // and in the tensor
+  // Neighbouring lanes have the same states of neighbouring channels: they read the
+  // same 16 bytes of B and C, which costs 2.4 cycles of the SM's shared memory a load
+  // where four addresses taking turns (lane % 4) cost 4.
   __device__ __forceinline__ Place(int64_t d0) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    sl = lane % L::LPC;
-    ch = (warp * L::kLanes + lane / L::LPC) * L::CPT;
+    sl = lane / L::kLanes;
+    cl = lane % L::kLanes;
+    ch = warp * L::kWarpChannels + cl;
     d = d0 + ch;
   }
   static __device__ __forceinline__ bool vectors(const float* p, int N) {
@@ -205,8 +210,9 @@ struct Place {
   // states of channel c in a [.., dim, N] array, zero where there is none
   __device__ __forceinline__ void load(float2 (&v)[L::P], const float* p, int c, int64_t row,
                                        int64_t dim, int N) const {
-    const bool on = p && d + c < dim;
-    const float* q = p + (row * dim + d + c) * N + sl * L::SPT;
+    const int64_t dc = d + c * L::kLanes;
+    const bool on = p && dc < dim;
+    const float* q = p + (row * dim + dc) * N + sl * L::SPT;
     if (L::SPT == 4 && vectors(p, N)) {
       const float4 t = load_if(reinterpret_cast<const float4*>(q), on && sl * L::SPT < N);
       v[0] = make_float2(t.x, t.y);
@@ -222,8 +228,9 @@ struct Place {
   }
   __device__ __forceinline__ void store(const float2 (&v)[L::P], float* p, int c, int64_t row,
                                         int64_t dim, int N) const {
-    if (!p || d + c >= dim) return;
-    float* q = p + (row * dim + d + c) * N + sl * L::SPT;
+    const int64_t dc = d + c * L::kLanes;
+    if (!p || dc >= dim) return;
+    float* q = p + (row * dim + dc) * N + sl * L::SPT;
     if (L::SPT == 4 && vectors(p, N)) {
       if (sl * L::SPT < N)
         *reinterpret_cast<float4*>(q) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
@@ -369,6 +376,22 @@ struct Raw {
   }
 };
 
+// VW floats in shared memory.
+template <int VW>
+__device__ __forceinline__ void load_floats(float (&v)[VW], const float* p) {
+  if constexpr (VW == 4) {
+    const float4 t = *reinterpret_cast<const float4*>(p);
+    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+  } else {
+    v[0] = p[0];
+  }
+}
+template <int VW>
+__device__ __forceinline__ void store_floats(float* p, const float (&v)[VW]) {
+  if constexpr (VW == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else p[0] = v[0];
+}
+
 // VW entries of a [dim] vector from channel d on, 0 where there is none.
 template <int VW>
 __device__ __forceinline__ void load_channels(float (&v)[VW], const float* p, int64_t d, bool in) {
@@ -466,7 +489,8 @@ __device__ __forceinline__ void through_segment(float2 (&h)[L::CPT][L::P], const
   const int64_t row = b * a.segments + seg;
 #pragma unroll
   for (int c = 0; c < L::CPT; ++c) {
-    const float time = at.d + c < a.dim ? a.seg_time[row * a.dim + at.d + c] : 0.0f;
+    const int64_t d = at.d + c * L::kLanes;
+    const float time = d < a.dim ? a.seg_time[row * a.dim + d] : 0.0f;
     float2 own[L::P];
     at.load(own, a.seg_state, c, row, a.dim, a.N);
 #pragma unroll

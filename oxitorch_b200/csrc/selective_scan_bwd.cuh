@@ -103,7 +103,7 @@ selective_bwd_map_kernel(SelectiveArgs<T> a) {
         const bool start = decltype(some)::value && ((starts >> t) & 1u);
 #pragma unroll
         for (int c = 0; c < CPT; ++c) {
-          const float2 in = in_tile[t * L::kChannels + c];
+          const float2 in = in_tile[t * L::kChannels + c * L::kLanes];
 #pragma unroll
           for (int i = 0; i < P; ++i) {
             const float2 decay = exp2_pair(__fmul2_rn(A2[c][i], both(in.x)));
@@ -120,42 +120,25 @@ selective_bwd_map_kernel(SelectiveArgs<T> a) {
 #pragma unroll
   for (int c = 0; c < CPT; ++c) {
     at.store(mu[c], a.seg_state, c, row, a.dim, a.N);
-    if (at.sl == 0 && at.d + c < a.dim)
-      a.seg_time[row * a.dim + at.d + c] = fresh ? -1.0f : time[c];
+    const int64_t d = at.d + c * L::kLanes;
+    if (at.sl == 0 && d < a.dim) a.seg_time[row * a.dim + d] = fresh ? -1.0f : time[c];
   }
   pdl_launch_dependents();
 }
 
-// Where the sums of the VJP's kBack tokens are made, a warp by itself: every lane
-// leaves its share, and the shares are added up in vectors.  A few stores and loads
-// for kBack tokens in the place of a shuffle and two selects for each value and step.
-template <class L, bool GATED>
-struct Shares {
-  static constexpr int kBlock = 2;                    // tokens at a time
-  static constexpr int kSums = GATED ? 3 : 2;         // through, rate, inner
-  // [kBlock][kLanes][2 NP] dB and dC, rows apart by 16 banks
-  static constexpr int kRow = 2 * L::NP + (L::NP % 16 == 0 && L::kLanes > 1 ? 16 : 4);
-  static constexpr int kRowFloats = L::kLanes > 1 ? kBlock * L::kLanes * kRow : 0;
-  // [kBlock][LPC][kSums][kWarpChannels], rows apart by 8 banks while they are few
-  static constexpr int kSum = L::LPC <= 4 ? (kSums * L::kWarpChannels + 31) / 32 * 32 + 8
-                                          : kSums * L::kWarpChannels + 2;
-  static constexpr int kSumFloats = (kBlock * L::LPC * kSum + 3) / 4 * 4;
-  static constexpr int kFloats = kRowFloats + kSumFloats;
-};
-
 template <class L, typename T, int VW, bool GATED>
 struct BackwardShared {
   using R = Raw<L, T, VW, GATED ? 4 : 3, -1, 2>;  // x, delta, dy, z
-  using S = Shares<L, GATED>;
   static constexpr int kParts = kTile / kBack;
+  static constexpr int kPlane = kTile * L::kChannels;
   // twice each, for the even tiles and the odd
-  static constexpr int kIn = 4 * kTile * L::kChannels;         // [kTile][kChannels] of four: dt, dt x, e,
-                                                               // nothing; afterwards dt, rate / ln 2,
-                                                               // inner - D x, through
+  static constexpr int kIn = (GATED ? 4 : 3) * kPlane;         // planes [kTile][kChannels]: dt, dt x, e and
+                                                               // nothing; afterwards dt, through,
+                                                               // rate / ln 2, inner - D x
   static constexpr int kBC = 2 * kTile * L::NP;                // [kTile][NP]
   static constexpr int kRows = L::kWarps * kTile * 2 * L::NP;  // [kWarps][kTile][2 NP]: dB, dC, once
   static constexpr int kKept = (kParts - 1) * L::CPT * L::SPT * L::kThreads;  // [..][2 P][kThreads]
-  static constexpr int kFloats = 2 * (kIn + kBC) + kRows + kKept + L::kWarps * S::kFloats;
+  static constexpr int kFloats = 2 * (kIn + kBC) + kRows + kKept;
   static constexpr size_t kBytes = sizeof(float) * kFloats + sizeof(T) * R::kElements;
 };
 
@@ -174,10 +157,8 @@ __global__ void __launch_bounds__(Backward<LPC>::kThreads + kHelpers, 1)
 selective_bwd_kernel(SelectiveArgs<T> a) {
   using L = Backward<LPC>;
   constexpr int SPT = L::SPT, P = L::P, CPT = L::CPT, VW = VEC ? 4 : 1, kAll = L::kThreads + kHelpers;
-  static_assert(CPT == 2 && SPT == 4, "the shares are vectors");
   using M = BackwardShared<L, T, VW, GATED>;
   using R = typename M::R;
-  using S = typename M::S;
   constexpr int kParts = M::kParts;
   extern __shared__ __align__(16) float smem[];
   float* s_rows = smem + 2 * (M::kIn + M::kBC);
@@ -188,7 +169,7 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
   const int64_t tiles = (a.length + kTile - 1) / kTile;
   const int64_t tile0 = (int64_t)seg * a.seg_tiles, end = min(tiles, tile0 + a.seg_tiles) - 1;
   const int count = (int)(end + 1 - tile0);  // tile i of them is end - i
-  auto in_of = [&](int i) { return reinterpret_cast<float4*>(smem + (i & 1) * M::kIn); };
+  auto in_of = [&](int i) { return smem + (i & 1) * M::kIn; };
   auto B_of = [&](int i) { return smem + 2 * M::kIn + (i & 1) * M::kBC; };
   float* sums = a.sums + (b * a.segments + seg) * (a.dim * a.N + 2 * a.dim);
 
@@ -228,14 +209,17 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
           raw.read(dt, buffer, 1, k);
           if (a.dy.p) raw.read(e, buffer, 2, k);
           if (GATED) raw.read(z, buffer, GATED ? 3 : 0, k);
-          float4* to = in_of(i) + (raw.t + k * R::kTurn) * L::kChannels + raw.ch;
+          float* to = in_of(i) + (raw.t + k * R::kTurn) * L::kChannels + raw.ch;
 #pragma unroll
           for (int v = 0; v < VW; ++v) {
             if (!a.dy.p) e[v] = 0.0f;
             if (GATED) e[v] *= z[v] * sigmoid(z[v]);
             dt[v] = on ? softplus(dt[v] + bias[v]) : 0.0f;
-            to[v] = make_float4(dt[v], dt[v] * x[v], e[v], 0.0f);
+            x[v] *= dt[v];
           }
+          store_floats(to, dt);
+          store_floats(to + M::kPlane, x);
+          store_floats(to + 2 * M::kPlane, e);
         }
         rows_B.put(B_of(i));
         rows_C.put(B_of(i) + kTile * L::NP);
@@ -270,24 +254,27 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
 #pragma unroll 2
         for (int k = 0; k < R::kMine; ++k) {
           if (!raw.on(k, left)) break;
-          const float4* from = in_of(i - 1) + (raw.t + k * R::kTurn) * L::kChannels + raw.ch;
+          const float* from = in_of(i - 1) + (raw.t + k * R::kTurn) * L::kChannels + raw.ch;
           const int64_t to = out + k * R::kTurn * a.dim;
-          float x[VW], d[VW], dx[VW], e[VW], z[VW], dz[VW];
+          float x[VW], d[VW], dx[VW], e[VW], z[VW], dz[VW], through[VW], rate[VW];
+          load_floats(dx, from);  // dt
+          load_floats(through, from + M::kPlane);
+          load_floats(rate, from + 2 * M::kPlane);
+          if (GATED) load_floats(dz, from + (GATED ? 3 : 0) * M::kPlane);  // inner - D x
           raw.read(x, buffer, 0, k);
           raw.read(d, buffer, 1, k);
           if (a.dy.p) raw.read(e, buffer, 2, k);
           if (GATED) raw.read(z, buffer, GATED ? 3 : 0, k);
 #pragma unroll
           for (int v = 0; v < VW; ++v) {
-            const float4 in = from[v];
             if (!a.dy.p) e[v] = 0.0f;
             if (GATED) {
               const float s = sigmoid(z[v]);
-              dz[v] = e[v] * fmaf(skip[v], x[v], in.z) * fmaf(z[v] * s, 1.0f - s, s);
+              dz[v] = e[v] * fmaf(skip[v], x[v], dz[v]) * fmaf(z[v] * s, 1.0f - s, s);
               e[v] *= z[v] * s;
             }
-            dx[v] = fmaf(in.x, in.w, skip[v] * e[v]);
-            const float ddt = fmaf(x[v], in.w, kLn2 * in.y);
+            dx[v] = fmaf(dx[v], through[v], skip[v] * e[v]);
+            const float ddt = fmaf(x[v], through[v], kLn2 * rate[v]);
             d[v] = ddt * sigmoid(d[v] + bias[v]);
             dD[v] = fmaf(e[v], x[v], dD[v]);
             dbias[v] += d[v];
@@ -324,10 +311,8 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
 
   if constexpr (L::kWarps == 8) share_registers<true>();
   const Place<L> at(d0);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cl = lane / LPC;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float2* s_kept = reinterpret_cast<float2*>(s_rows + M::kRows);
-  float* share_rows = s_rows + M::kRows + M::kKept + warp * S::kFloats;
-  float* share_sums = share_rows + S::kRowFloats;
   float2 A2[CPT][P], mu[CPT][P], dA[CPT][P], enter[CPT][P];  // enter: the state before the next tile
   load_decay<L>(A2, at, a);
 #pragma unroll
@@ -356,21 +341,24 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
 #pragma unroll
       for (int c = 0; c < CPT; ++c) at.load(enter[c], a.carry, c, b * tiles + end - tile - 1, a.dim, a.N);
     }
-    float4* s_in = in_of(tile);
+    float* s_in = in_of(tile) + at.ch;
     const float *s_B = B_of(tile), *s_C = s_B + kTile * L::NP;
     tile_sync(kFull + (tile & 1), kAll);
     by_fresh(starts, [&](auto some) {
       constexpr bool kSome = decltype(some)::value;
       // the operands of kBack tokens: all read before anything is stored, as the compiler
       // cannot tell the stores from them
-      float4 in[kBack][CPT];
+      float2 in[kBack][CPT];
       float2 B[kBack][P];
       auto read = [&](int t) {
 #pragma unroll
         for (int k = 0; k < kBack; ++k) {
           load_states<SPT>(B[k], s_B + (t + k) * L::NP + at.sl * SPT);
 #pragma unroll
-          for (int c = 0; c < CPT; ++c) in[k][c] = s_in[(t + k) * L::kChannels + at.ch + c];
+          for (int c = 0; c < CPT; ++c) {
+            const float* p = s_in + (t + k) * L::kChannels + c * L::kLanes;
+            in[k][c] = make_float2(p[0], p[M::kPlane]);
+          }
         }
       };
       // one token forward: `e` the decay, h the state after it
@@ -402,9 +390,14 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
 #pragma unroll 1
       for (int j = kParts - 1; j >= 0; --j) {
         float2 enters[CPT][P], decay[kBack][CPT][P], state[kBack][CPT][P], Cs[kBack][P];
+        float es[kBack][CPT];
         read(j * kBack);
 #pragma unroll
-        for (int k = 0; k < kBack; ++k) load_states<SPT>(Cs[k], s_C + (j * kBack + k) * L::NP + at.sl * SPT);
+        for (int k = 0; k < kBack; ++k) {
+          load_states<SPT>(Cs[k], s_C + (j * kBack + k) * L::NP + at.sl * SPT);
+#pragma unroll
+          for (int c = 0; c < CPT; ++c) es[k][c] = s_in[2 * M::kPlane + (j * kBack + k) * L::kChannels + c * L::kLanes];
+        }
 #pragma unroll
         for (int c = 0; c < CPT; ++c)
 #pragma unroll
@@ -422,13 +415,12 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
         }
 #pragma unroll
         for (int back = kBack - 1; back >= 0; --back) {
-          const int t = j * kBack + back, slot = back % S::kBlock;
+          const int t = j * kBack + back;
           float2 dB[P], dC[P], through[CPT], rate[CPT], inner[CPT];
           const bool start = kSome && ((starts >> t) & 1u);
 #pragma unroll
           for (int c = 0; c < CPT; ++c) {
-            const float4 v = in[back][c];
-            const float2 dt2 = both(v.x), dtx2 = both(v.y), e2 = both(v.z);
+            const float2 dt2 = both(in[back][c].x), dtx2 = both(in[back][c].y), e2 = both(es[back][c]);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
               const float2 C = Cs[back][i], lam = __ffma2_rn(C, e2, mu[c][i]);
@@ -445,61 +437,51 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
               dA[c][i] = __ffma2_rn(q, dt2, dA[c][i]);
             }
           }
-          // this lane's shares
-          float* sum = share_sums + (slot * LPC + at.sl) * S::kSum + cl * CPT;
-          *reinterpret_cast<float2*>(sum) = make_float2(through[0].x + through[0].y, through[1].x + through[1].y);
-          *reinterpret_cast<float2*>(sum + L::kWarpChannels) =
-              make_float2(rate[0].x + rate[0].y, rate[1].x + rate[1].y);
-          if (GATED)
-            *reinterpret_cast<float2*>(sum + 2 * L::kWarpChannels) =
-                make_float2(inner[0].x + inner[0].y, inner[1].x + inner[1].y);
-          float* row = L::kLanes > 1 ? share_rows + (slot * L::kLanes + cl) * S::kRow + at.sl * SPT
-                                     : s_rows + (warp * kTile + t) * 2 * L::NP + at.sl * SPT;
-          *reinterpret_cast<float4*>(row) = make_float4(dB[0].x, dB[0].y, dB[1].x, dB[1].y);
-          *reinterpret_cast<float4*>(row + L::NP) = make_float4(dC[0].x, dC[0].y, dC[1].x, dC[1].y);
-          if (slot) continue;
-          // the sums of tokens t and t + 1
-          __syncwarp();
-          if constexpr (L::kLanes > 1) {
-            constexpr int kQuads = 2 * L::NP / 4;
+          float* to = s_in + t * L::kChannels;
+          {
+            using Sum = LaneSum<4, L::kLanes, 32>;
+            float v[4] = {through[0].x + through[0].y, through[1].x + through[1].y,
+                          rate[0].x + rate[0].y, rate[1].x + rate[1].y};
+            int first = 0;
+            Sum::run(v, lane, first);
+            if (lane < Sum::kUsed) {  // dt x and e have been used
 #pragma unroll
-            for (int o = lane; o < S::kBlock * kQuads; o += 32) {
-              const int token = o / kQuads, quad = o % kQuads;
-              const float* p = share_rows + token * L::kLanes * S::kRow + quad * 4;
-              float4 r = *reinterpret_cast<const float4*>(p);
-              float2 lo = make_float2(r.x, r.y), hi = make_float2(r.z, r.w);
+              for (int i = 0; i < Sum::kKept; ++i)
+                to[(1 + (first + i) / 2) * M::kPlane + (first + i) % 2 * L::kLanes] = v[i];
+            }
+          }
+          if (GATED) {
+            using Sum = LaneSum<2, L::kLanes, 32>;
+            float v[2] = {inner[0].x + inner[0].y, inner[1].x + inner[1].y};
+            int first = 0;
+            Sum::run(v, lane, first);
+            if (lane < Sum::kUsed) {
 #pragma unroll
-              for (int k = 1; k < L::kLanes; ++k) {
-                r = *reinterpret_cast<const float4*>(p + k * S::kRow);
-                lo = __fadd2_rn(lo, make_float2(r.x, r.y));
-                hi = __fadd2_rn(hi, make_float2(r.z, r.w));
+              for (int i = 0; i < Sum::kKept; ++i)
+                to[(GATED ? 3 : 0) * M::kPlane + (first + i) * L::kLanes] = v[i];
+            }
+          }
+          {
+            using Sum = LaneSum<2 * SPT, 1, L::kLanes>;
+            float v[2 * SPT];
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+              v[2 * i] = dB[i].x;
+              v[2 * i + 1] = dB[i].y;
+              v[SPT + 2 * i] = dC[i].x;
+              v[SPT + 2 * i + 1] = dC[i].y;
+            }
+            int first = 0;
+            Sum::run(v, lane, first);
+            if (at.cl < Sum::kUsed) {
+              float* row = s_rows + (warp * kTile + t) * 2 * L::NP + at.sl * SPT;
+#pragma unroll
+              for (int i = 0; i < Sum::kKept; ++i) {
+                const int k = first + i;
+                row[k < SPT ? k : L::NP + k - SPT] = v[i];
               }
-              *reinterpret_cast<float4*>(s_rows + (warp * kTile + t + token) * 2 * L::NP + quad * 4) =
-                  make_float4(lo.x, lo.y, hi.x, hi.y);
             }
           }
-          constexpr int kPairs = S::kSums * L::kWarpChannels / 2;
-#pragma unroll
-          for (int o = lane; o < S::kBlock * kPairs; o += 32) {
-            const int token = o / kPairs, pair = o % kPairs, what = pair / (L::kWarpChannels / 2),
-                      ch = pair % (L::kWarpChannels / 2) * 2;
-            const float* p = share_sums + token * LPC * S::kSum + what * L::kWarpChannels + ch;
-            float2 r = *reinterpret_cast<const float2*>(p);
-#pragma unroll
-            for (int k = 1; k < LPC; ++k) r = __fadd2_rn(r, *reinterpret_cast<const float2*>(p + k * S::kSum));
-            float4* to = s_in + (t + token) * L::kChannels + warp * L::kWarpChannels + ch;
-            if (what == 0) {
-              to[0].w = r.x;
-              to[1].w = r.y;
-            } else if (what == 1) {  // dt x and e have been used
-              to[0].y = r.x;
-              to[1].y = r.y;
-            } else {
-              to[0].z = r.x;
-              to[1].z = r.y;
-            }
-          }
-          __syncwarp();
         }
       }
     });

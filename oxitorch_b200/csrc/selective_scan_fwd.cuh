@@ -13,9 +13,11 @@ struct ForwardShared {
   static constexpr int kPlane = kTile * L::kChannels, kRow = kTile * L::NP;
   // twice each, for the even tiles and the odd
   static constexpr int kIn = 2 * kPlane;                    // [kTile][kChannels] dt, dt x
-  static constexpr int kY = MAP ? 0 : kLeft * kPlane;       // [kTile][kChannels][kLeft]
+  static constexpr int kYRow = L::kChannels + (L::kLanes < 4 ? 4 : L::kLanes);  // banks apart
+  static constexpr int kY = MAP ? 0 : kTile * kLeft * kYRow;  // [kTile][kLeft][kYRow]
   static constexpr int kBC = (MAP ? 1 : 2) * kRow;          // [kTile][NP]
   static constexpr int kFloats = 2 * (kIn + kY + kBC);
+  static_assert(kYRow % 4 == 0 && kIn % 4 == 0 && kBC % 4 == 0, "vectors of 16 bytes");
   static constexpr size_t kBytes = sizeof(float) * kFloats + sizeof(T) * R::kElements;
 };
 
@@ -100,17 +102,18 @@ selective_fwd_kernel(SelectiveArgs<T> a) {
 #pragma unroll
           for (int k = 0; k < R::kMine; ++k) {
             if (!raw.on(k, left)) break;
-            float x[VW], y[VW];
+            float x[VW], y[VW], part[VW];
             raw.read(x, before, 0, k);
+            const float* p = s + (raw.t + k * R::kTurn) * kLeft * S::kYRow + raw.ch;
+            load_floats(y, p);
+#pragma unroll
+            for (int m = 1; m < kLeft; ++m) {
+              load_floats(part, p + m * S::kYRow);
+#pragma unroll
+              for (int v = 0; v < VW; ++v) y[v] += part[v];
+            }
 #pragma unroll
             for (int v = 0; v < VW; ++v) {
-              const float* p = s + ((raw.t + k * R::kTurn) * L::kChannels + raw.ch + v) * kLeft;
-              if constexpr (kLeft == 4) {
-                const float4 q = *reinterpret_cast<const float4*>(p);
-                y[v] = (q.x + q.y) + (q.z + q.w);
-              } else {
-                y[v] = p[0] + p[kLeft - 1];
-              }
               if (a.D) y[v] = fmaf(skip[v], x[v], y[v]);
             }
             if (a.z.p) {
@@ -162,7 +165,7 @@ selective_fwd_kernel(SelectiveArgs<T> a) {
     tile_sync(kFull + (tile & 1), kAll);
     const float2* in_tile = s_in(tile) + at.ch;
     const float *B_tile = s_B(tile) + at.sl * SPT, *C_tile = B_tile + S::kRow;
-    float* y_tile = s_y(tile) + at.ch * kLeft + at.sl;
+    float* y_tile = s_y(tile) + at.sl * S::kYRow + at.ch;
     by_fresh(starts, [&](auto some) {
       // kAhead tokens at a time: all their reads before the first of their stores, which
       // the compiler cannot tell from them
@@ -174,13 +177,8 @@ selective_fwd_kernel(SelectiveArgs<T> a) {
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
           const int t = t1 + k;
-          if constexpr (CPT == 2) {
-            const float4 v = *reinterpret_cast<const float4*>(in_tile + t * L::kChannels);
-            in[k][0] = make_float2(v.x, v.y);
-            in[k][1] = make_float2(v.z, v.w);
-          } else {
-            in[k][0] = in_tile[t * L::kChannels];
-          }
+#pragma unroll
+          for (int c = 0; c < CPT; ++c) in[k][c] = in_tile[t * L::kChannels + c * L::kLanes];
           load_states<SPT>(B[k], B_tile + t * L::NP);
           if (!MAP) load_states<SPT>(C[k], C_tile + t * L::NP);
         }
@@ -207,8 +205,9 @@ selective_fwd_kernel(SelectiveArgs<T> a) {
 #pragma unroll
             for (int c = 0; c < CPT; ++c) {
 #pragma unroll
-              for (int m = kLeft; m < LPC; m *= 2) y[k][c] += __shfl_xor_sync(0xffffffffu, y[k][c], m);
-              if (LPC == kLeft || at.sl < kLeft) y_tile[((t1 + k) * L::kChannels + c) * kLeft] = y[k][c];
+              for (int m = kLeft; m < LPC; m *= 2)
+                y[k][c] += __shfl_xor_sync(0xffffffffu, y[k][c], m * L::kLanes);
+              if (LPC == kLeft || at.sl < kLeft) y_tile[(t1 + k) * kLeft * S::kYRow + c * L::kLanes] = y[k][c];
             }
         }
       }
@@ -220,8 +219,8 @@ selective_fwd_kernel(SelectiveArgs<T> a) {
 #pragma unroll
     for (int c = 0; c < CPT; ++c) {
       at.store(h[c], a.seg_state, c, row, a.dim, a.N);
-      if (at.sl == 0 && at.d + c < a.dim)
-        a.seg_time[row * a.dim + at.d + c] = fresh ? -1.0f : time[c];
+      const int64_t d = at.d + c * L::kLanes;
+      if (at.sl == 0 && d < a.dim) a.seg_time[row * a.dim + d] = fresh ? -1.0f : time[c];
     }
     pdl_launch_dependents();
   } else if (seg == a.segments - 1 && a.last) {
