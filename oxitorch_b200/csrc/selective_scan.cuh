@@ -25,8 +25,8 @@
 // Sums over n are made across the LPC threads, sums over d across the warp's other
 // lanes, its warps and the CTAs.  The VJP gets the state before each tile from the
 // forward (`carry`) and goes through the tiles from the last to the first: it runs the
-// recurrence forward through a tile, keeping the state every kBack tokens, and from the
-// last of these backwards again with the decays and states of kBack tokens in registers.
+// recurrence forward through a tile, keeping the state every few tokens, and from the last
+// of these backwards again with the decays and states of those few tokens in registers.
 //
 // Where batch and dim leave the GPU idle, the sequence is cut into segments.  A
 // first kernel finds what each does to the state (its decay, exp(A sum dt), and the
@@ -42,7 +42,6 @@
 namespace oxc {
 
 constexpr int kTile = 16;     // tokens; the states that the VJP needs are saved as often
-constexpr int kBack = 4;      // tokens whose states the VJP holds in registers
 constexpr int kMaxState = 128;
 constexpr int kMaxSegments = 64;
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
@@ -226,6 +225,12 @@ struct Place {
       v[i].y = load_if(q + 2 * i + 1, on && n + 1 < N);
     }
   }
+  // Asks L2 for what load will take.
+  __device__ __forceinline__ void ask(const float* p, int c, int64_t row, int64_t dim, int N) const {
+    const int64_t dc = d + c * L::kLanes;
+    if (dc < dim && sl * L::SPT < N)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p + (row * dim + dc) * N + sl * L::SPT));
+  }
   __device__ __forceinline__ void store(const float2 (&v)[L::P], float* p, int c, int64_t row,
                                         int64_t dim, int N) const {
     const int64_t dc = d + c * L::kLanes;
@@ -270,8 +275,18 @@ __device__ __forceinline__ void tile_arrive(int id, int threads) {
 }
 constexpr int kFull = 1, kDone = 3;  // + the tile's parity
 
-// The threads that prepare tiles are behind those that walk through them.
-constexpr int kHelpers = 128;
+// The threads that prepare tiles, behind those that walk through them: as many, since
+// their chains of dependent operations are as long.
+constexpr int kHelpers = 256;
+
+// Deals out the registers that a CTA is launched with: the warps that walk through tiles
+// need more of them than the helpers.  The shares have to add up to no more than those
+// at the launch, or the first of these would wait for ever.
+template <int REGISTERS, bool MORE>
+__device__ __forceinline__ void take_registers() {
+  if constexpr (MORE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGISTERS));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGISTERS));
+}
 
 // A tile's operands as they are in memory, TENSORS of them DEPTH times over: helper i's
 // vectors lie where only helper i looks, so no barrier stands between its copies and
@@ -525,7 +540,7 @@ template <int SPT, int LPC>
 using Forward = Layout<SPT, LPC, (LPC <= 4 ? 1 : 2), 8>;
 // In the VJP 4 states a thread, the lanes a power of two.
 template <int LPC>
-using Backward = Layout<4, LPC, 2, (LPC == 2 ? 4 : 8)>;
+using Backward = Layout<4, LPC, (LPC == 2 ? 1 : 2), 8>;
 template <typename F>
 inline auto by_lanes(int64_t N, F f) {
   if (N <= 8) return f(std::integral_constant<int, 2>{});

@@ -129,6 +129,7 @@ selective_bwd_map_kernel(SelectiveArgs<T> a) {
 template <class L, typename T, int VW, bool GATED>
 struct BackwardShared {
   using R = Raw<L, T, VW, GATED ? 4 : 3, -1, 2>;  // x, delta, dy, z
+  static constexpr int kBack = 4;  // tokens whose states are held in registers
   static constexpr int kParts = kTile / kBack;
   static constexpr int kPlane = kTile * L::kChannels;
   // twice each, for the even tiles and the odd
@@ -144,13 +145,15 @@ struct BackwardShared {
 
 constexpr int kRowsFree = 5;  // the barrier after which the rows of the tile before are read
 
-// Of the registers that a CTA of 8 + 4 warps is launched with (168 a thread) the helpers
-// pass 80 each on: 256 x 208 + 128 x 88 = 384 x 168.
-template <bool TAKE>
-__device__ __forceinline__ void share_registers() {
-  if constexpr (TAKE) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-}
+// Registers a thread: at the launch, then of those that walk and of the helpers.
+template <class L>
+struct Registers {
+  static constexpr int kAll = L::kThreads + kHelpers;
+  static constexpr int kLaunch = 65536 / kAll / 8 * 8;
+  static constexpr bool kDeal = L::CPT == 2;
+  static constexpr int kHelp = 88, kWalk = 168;
+  static_assert(!kDeal || L::kThreads * kWalk + kHelpers * kHelp <= kAll * kLaunch, "more than there are");
+};
 
 template <typename T, int LPC, bool VEC, bool GATED>
 __global__ void __launch_bounds__(Backward<LPC>::kThreads + kHelpers, 1)
@@ -159,7 +162,7 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
   constexpr int SPT = L::SPT, P = L::P, CPT = L::CPT, VW = VEC ? 4 : 1, kAll = L::kThreads + kHelpers;
   using M = BackwardShared<L, T, VW, GATED>;
   using R = typename M::R;
-  constexpr int kParts = M::kParts;
+  constexpr int kParts = M::kParts, kBack = M::kBack;
   extern __shared__ __align__(16) float smem[];
   float* s_rows = smem + 2 * (M::kIn + M::kBC);
   const unsigned int ct = blockIdx.x % a.ctiles, rest = blockIdx.x / a.ctiles;
@@ -174,7 +177,7 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
   float* sums = a.sums + (b * a.segments + seg) * (a.dim * a.N + 2 * a.dim);
 
   if (threadIdx.x >= L::kThreads) {
-    if constexpr (L::kWarps == 8) share_registers<false>();
+    if constexpr (Registers<L>::kDeal) take_registers<Registers<L>::kHelp, false>();
     const int me = threadIdx.x - L::kThreads;
     R raw(reinterpret_cast<T*>(smem + M::kFloats), me, d0, a.dim);
     raw.open(0, a.x, b, end * kTile, d0);
@@ -200,7 +203,7 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
       if (i < count) {
         const int left = tokens(i), buffer = i & 1;
         raw.land(buffer, left);
-#pragma unroll 2
+#pragma unroll 1
         for (int k = 0; k < R::kMine; ++k) {
           if (!raw.has) break;
           const bool on = raw.on(k, left);
@@ -251,7 +254,7 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
         }
         row_out -= kTile * 2 * a.N;
         if (i < count) tile_arrive(kRowsFree, kAll);
-#pragma unroll 2
+#pragma unroll 1
         for (int k = 0; k < R::kMine; ++k) {
           if (!raw.on(k, left)) break;
           const float* from = in_of(i - 1) + (raw.t + k * R::kTurn) * L::kChannels + raw.ch;
@@ -309,16 +312,15 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
     return;
   }
 
-  if constexpr (L::kWarps == 8) share_registers<true>();
+  if constexpr (Registers<L>::kDeal) take_registers<Registers<L>::kWalk, true>();
   const Place<L> at(d0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float2* s_kept = reinterpret_cast<float2*>(s_rows + M::kRows);
-  float2 A2[CPT][P], mu[CPT][P], dA[CPT][P], enter[CPT][P];  // enter: the state before the next tile
+  float2 A2[CPT][P], mu[CPT][P], dA[CPT][P];
   load_decay<L>(A2, at, a);
 #pragma unroll
   for (int c = 0; c < CPT; ++c) {
     at.load(mu[c], a.dlast, c, b, a.dim, a.N);
-    at.load(enter[c], a.carry, c, b * tiles + end, a.dim, a.N);
 #pragma unroll
     for (int i = 0; i < P; ++i) dA[c][i] = both(0.0f);
   }
@@ -332,14 +334,11 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
   Starts ahead(a.starts, b, a.length, end);
   for (int tile = 0; tile < count; ++tile) {
     const unsigned int starts = ahead.bits(end - tile - 1);
-    float2 h[CPT][P];
+    float2 h[CPT][P];  // the state before the tile; L2 is asked for the next one
 #pragma unroll
-    for (int c = 0; c < CPT; ++c)
-#pragma unroll
-      for (int i = 0; i < P; ++i) h[c][i] = enter[c][i];
-    if (tile + 1 < count) {
-#pragma unroll
-      for (int c = 0; c < CPT; ++c) at.load(enter[c], a.carry, c, b * tiles + end - tile - 1, a.dim, a.N);
+    for (int c = 0; c < CPT; ++c) {
+      at.load(h[c], a.carry, c, b * tiles + end - tile, a.dim, a.N);
+      if (tile + 1 < count) at.ask(a.carry, c, b * tiles + end - tile - 1, a.dim, a.N);
     }
     float* s_in = in_of(tile) + at.ch;
     const float *s_B = B_of(tile), *s_C = s_B + kTile * L::NP;
@@ -439,20 +438,26 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
           }
           float* to = s_in + t * L::kChannels;
           {
-            using Sum = LaneSum<4, L::kLanes, 32>;
-            float v[4] = {through[0].x + through[0].y, through[1].x + through[1].y,
-                          rate[0].x + rate[0].y, rate[1].x + rate[1].y};
+            using Sum = LaneSum<2 * CPT, L::kLanes, 32>;
+            float v[2 * CPT];
+#pragma unroll
+            for (int c = 0; c < CPT; ++c) {
+              v[c] = through[c].x + through[c].y;
+              v[CPT + c] = rate[c].x + rate[c].y;
+            }
             int first = 0;
             Sum::run(v, lane, first);
             if (lane < Sum::kUsed) {  // dt x and e have been used
 #pragma unroll
               for (int i = 0; i < Sum::kKept; ++i)
-                to[(1 + (first + i) / 2) * M::kPlane + (first + i) % 2 * L::kLanes] = v[i];
+                to[(1 + (first + i) / CPT) * M::kPlane + (first + i) % CPT * L::kLanes] = v[i];
             }
           }
           if (GATED) {
-            using Sum = LaneSum<2, L::kLanes, 32>;
-            float v[2] = {inner[0].x + inner[0].y, inner[1].x + inner[1].y};
+            using Sum = LaneSum<CPT, L::kLanes, 32>;
+            float v[CPT];
+#pragma unroll
+            for (int c = 0; c < CPT; ++c) v[c] = inner[c].x + inner[c].y;
             int first = 0;
             Sum::run(v, lane, first);
             if (lane < Sum::kUsed) {
@@ -518,16 +523,14 @@ static cudaError_t selective_bwd_one(const SelectiveArgs<T>& a, cudaStream_t s) 
   using M = BackwardShared<L, T, VEC ? 4 : 1, GATED>;
   static_assert(M::kBytes <= 227 * 1024, "a CTA's shared memory");
   static_assert(2 * M::R::kTurn * L::kChannels <= 2 * M::kIn, "dD and ddelta_bias fit");
-  if (L::kWarps == 8) {  // what share_registers deals out has to be there, or it would wait for ever
-    static int registers = 0;
-    if (registers == 0) {
-      cudaFuncAttributes attr;
-      const cudaError_t e = cudaFuncGetAttributes(&attr, selective_bwd_kernel<T, LPC, VEC, GATED>);
-      if (e != cudaSuccess) return e;
-      registers = attr.numRegs;
-    }
-    if (registers != 168) return cudaErrorLaunchOutOfResources;
+  static int registers = 0;  // those that take_registers counts on have to be there
+  if (registers == 0) {
+    cudaFuncAttributes attr;
+    const cudaError_t e = cudaFuncGetAttributes(&attr, selective_bwd_kernel<T, LPC, VEC, GATED>);
+    if (e != cudaSuccess) return e;
+    registers = attr.numRegs;
   }
+  if (Registers<L>::kDeal && registers != Registers<L>::kLaunch) return cudaErrorLaunchOutOfResources;
   return launch_scan(selective_bwd_kernel<T, LPC, VEC, GATED>,
                      (unsigned int)(a.batch * a.ctiles) * a.segments, L::kThreads + kHelpers, M::kBytes,
                      a.segments > 1, s, a);
