@@ -12,12 +12,16 @@
 //   dx_s = sum_k w_{W-1-k} du_{s+k}   (over the taps that y_{s+k} had)
 //   dw_{W-1-k} = sum_t du_t x_{t-k},  dbias = sum_t du_t
 //
-// A warp takes 128 channels, four a lane, and a run of tokens; the taps are a
-// window of registers that moves along it, so each input is read once, and the
-// W-1 tokens before a run (and in the VJP after it) a second time, from L2.
-// Weight gradients are summed along the run in registers, over the CTA's warps in
-// shared memory and over CTAs by a second kernel, each in a fixed order.  Bound by
-// HBM.
+// A warp takes 128 channels, four a lane in two pairs, and a run of tokens; the taps are
+// a window of registers that moves along it, so each input is read once, and the W-1
+// tokens before a run (and in the VJP after it) a second time, from L2.  A few tokens are
+// loaded ahead of those that are worked on.  Weight gradients are summed along the run in
+// registers, over the CTA's warps in shared memory and over CTAs by a second kernel, each
+// in a fixed order.
+//
+// Bound by HBM in f32 and by the exponentials and reciprocals of the SiLU in bf16: two of
+// 16 a cycle and SM for each element take longer than its 4 bytes, so two channels share
+// a reciprocal.
 #include <algorithm>
 #include <type_traits>
 
@@ -28,15 +32,57 @@ namespace oxc {
 constexpr int kConvWarps = 8;
 constexpr int kConvLaneCh = 4;                  // channels a lane
 constexpr int kConvChannels = 32 * kConvLaneCh;  // a warp
-constexpr int kConvStep = 4;                    // tokens loaded at a time
 constexpr int kConvRun = 64;                    // tokens of a forward run
 constexpr int kConvMaxWidth = 8;
 
-// A lane's four channels: consecutive ones, in one access (VEC), or 32 apart.
+// A lane's four channels as they are in memory: consecutive ones, in one access (VEC),
+// or 32 apart.  Loads are predicated, so that nothing waits for one before its use.
+template <typename T, bool VEC>
+struct ConvRaw;
+template <bool VEC>
+struct ConvRaw<float, VEC> {
+  float v[4];
+  __device__ __forceinline__ void load(const float* p, int live) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = 0.0f;
+    if constexpr (VEC) {
+      asm("{.reg .pred p; setp.gt.s32 p, %5, 0; @p ld.global.v4.f32 {%0, %1, %2, %3}, [%4];}"
+          : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]) : "l"(p), "r"(live));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        asm("{.reg .pred p; setp.gt.s32 p, %2, %3; @p ld.global.f32 %0, [%1];}"
+            : "+f"(v[k]) : "l"(p + 32 * k), "r"(live), "r"(k));
+    }
+  }
+  __device__ __forceinline__ float2 pair(int j) const { return make_float2(v[2 * j], v[2 * j + 1]); }
+};
+template <bool VEC>
+struct ConvRaw<bf16, VEC> {
+  uint32_t w[VEC ? 2 : 4];
+  __device__ __forceinline__ void load(const bf16* p, int live) {
+#pragma unroll
+    for (int k = 0; k < (VEC ? 2 : 4); ++k) w[k] = 0u;
+    if constexpr (VEC) {
+      asm("{.reg .pred p; setp.gt.s32 p, %3, 0; @p ld.global.v2.u32 {%0, %1}, [%2];}"
+          : "+r"(w[0]), "+r"(w[1]) : "l"(p), "r"(live));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        asm("{.reg .pred p; setp.gt.s32 p, %2, %3; @p ld.global.u16 %0, [%1];}"
+            : "+r"(w[k]) : "l"(p + 32 * k), "r"(live), "r"(k));
+    }
+  }
+  __device__ __forceinline__ float2 pair(int j) const {
+    if constexpr (VEC) return make_float2(bf16_lo(w[j]), bf16_hi(w[j]));
+    else return make_float2(bf16_lo(w[2 * j]), bf16_lo(w[2 * j + 1]));
+  }
+};
+
 template <typename T, bool VEC>
 struct ConvLane {
-  int64_t d;
-  int live;
+  int64_t d;  // the first channel
+  int live;   // how many exist
   __device__ __forceinline__ ConvLane(int64_t d0, int64_t dim) {
     const int lane = threadIdx.x & 31;
     d = VEC ? d0 + lane * kConvLaneCh : d0 + lane;
@@ -45,28 +91,14 @@ struct ConvLane {
     for (int k = 0; k < kConvLaneCh; ++k) live += d + at(k) < dim;
   }
   static __device__ __forceinline__ int at(int k) { return VEC ? k : 32 * k; }
-  __device__ __forceinline__ void load(float (&v)[kConvLaneCh], const T* row, bool on) const {
+  __device__ __forceinline__ void store(T* row, const float2 (&v)[2]) const {
+    const float f[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
     if constexpr (VEC) {
-      if (on && live) load_as_f32<kConvLaneCh>(v, row + d);
-      else
-#pragma unroll
-        for (int k = 0; k < kConvLaneCh; ++k) v[k] = 0.0f;
+      if (live) store_from_f32<4>(row + d, f);
     } else {
 #pragma unroll
-      for (int k = 0; k < kConvLaneCh; ++k) {
-        float one[1] = {0.0f};
-        if (on && k < live) load_as_f32<1>(one, row + d + 32 * k);
-        v[k] = one[0];
-      }
-    }
-  }
-  __device__ __forceinline__ void store(T* row, const float (&v)[kConvLaneCh]) const {
-    if constexpr (VEC) {
-      if (live) store_from_f32<kConvLaneCh>(row + d, v);
-    } else {
-#pragma unroll
-      for (int k = 0; k < kConvLaneCh; ++k) {
-        const float one[1] = {v[k]};
+      for (int k = 0; k < 4; ++k) {
+        const float one[1] = {f[k]};
         if (k < live) store_from_f32<1>(row + d + 32 * k, one);
       }
     }
@@ -95,87 +127,163 @@ struct ConvArgs {
   unsigned int ctiles, groups;  // channel tiles, groups of kConvWarps runs
 };
 
-__device__ __forceinline__ float sigmoid_f32(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
-
-// Tokens since the sequence of token t began, at most W - 1 (also where none of the
-// last W - 1 starts one: what lies before token 0 belongs to its sequence).
-template <int W>
-__device__ __forceinline__ int conv_age(const uint8_t* starts, int64_t row, int64_t t) {
-  int age = W - 1;
-  if (starts) {
-#pragma unroll
-    for (int k = W - 2; k >= 0; --k)
-      if (t - k >= 0 && starts[row + t - k]) age = k;
-  }
-  return age;
+__device__ __forceinline__ float ex2(float t) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return r;
+}
+__device__ __forceinline__ float rcp(float t) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return r;
+}
+__device__ __forceinline__ float sigmoid_f32(float v) { return rcp(1.0f + ex2(-1.44269504f * v)); }
+// Of two values: with a = 1 + exp(-v.x) and b = 1 + exp(-v.y), one reciprocal r = 1 / (a b)
+// gives both, b r and a r.  Where a b would pass f32's range (v below -40 in one of them),
+// one by one.
+__device__ __forceinline__ float2 sigmoid_pair(float2 v) {
+  const float a = 1.0f + ex2(-1.44269504f * v.x), b = 1.0f + ex2(-1.44269504f * v.y);
+  if (a > 0x1p60f || b > 0x1p60f) return make_float2(rcp(a), rcp(b));
+  const float r = rcp(a * b);
+  return make_float2(b * r, a * r);
 }
 
-// Reads token t of a batch row, one of x0 if t is negative, zero at the end.
-template <typename T, int W, bool VEC>
-__device__ __forceinline__ void conv_token(const ConvArgs<T>& a, const ConvLane<T, VEC>& lane,
-                                           int64_t b, int64_t t, float (&v)[kConvLaneCh]) {
-  if (t >= 0) lane.load(v, a.x + b * a.x_sb + t * a.x_st, t < a.length);
-  else lane.load(v, a.x0 + (b * (W - 1) + t + W - 1) * a.dim, a.x0 != nullptr);
+// The tokens at which a sequence starts, a bit each: bit l is token t - (W - 1) + l, of the
+// W - 1 tokens before a step of U tokens and the step.
+template <int W, int U>
+struct ConvStarts {
+  const uint8_t* row;
+  int64_t length;
+  uint8_t next;
+  __device__ __forceinline__ ConvStarts(const uint8_t* starts, int64_t row, int64_t length)
+      : row(starts ? starts + row : nullptr), length(length), next(0) {}
+  __device__ __forceinline__ void load(int64_t t) {
+    const int lane = threadIdx.x & 31;
+    const int64_t at = t - (W - 1) + lane;
+    if (row) next = lane < W - 1 + U && at >= 0 && at < length ? row[at] : (uint8_t)0;
+  }
+  __device__ __forceinline__ unsigned int bits() const {
+    return row ? __ballot_sync(0xffffffffu, next != 0) : 0u;
+  }
+};
+// Tokens since the sequence of the step's i-th token began, at most W - 1 (also where
+// none of the last W - 1 starts one: what lies before token 0 belongs to its sequence).
+template <int W>
+__device__ __forceinline__ int conv_age(unsigned int bits, int i) {
+  const unsigned int before = bits << (31 - (W - 1 + i));
+  return before ? min(W - 1, __clz(before)) : W - 1;
+}
+// Runs f(std::true_type) if any bit is set, else f(std::false_type), whose taps need no
+// tests.
+template <typename F>
+__device__ __forceinline__ void by_fresh(unsigned int bits, F f) {
+  if (bits) f(std::true_type{});
+  else f(std::false_type{});
+}
+
+// The weights and the bias of a lane's channels, in pairs.
+template <int W, bool VEC, typename T>
+__device__ __forceinline__ void conv_weights(float2 (&w)[W][2], float2 (&bias)[2], const ConvArgs<T>& a,
+                                             const ConvLane<T, VEC>& lane) {
+#pragma unroll
+  for (int c = 0; c < kConvLaneCh; ++c) {
+    const bool on = c < lane.live;
+    const int64_t d = lane.d + lane.at(c);
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const float v = on ? a.w[d * W + k] : 0.0f;
+      if (c & 1) w[k][c / 2].y = v;
+      else w[k][c / 2].x = v;
+    }
+    const float v = on && a.bias ? a.bias[d] : 0.0f;
+    if (c & 1) bias[c / 2].y = v;
+    else bias[c / 2].x = v;
+  }
+}
+
+// Token t of a batch row, one of x0 if t is negative.
+template <int W, bool VEC, typename T>
+__device__ __forceinline__ void conv_token(ConvRaw<T, VEC>& r, const ConvArgs<T>& a,
+                                           const ConvLane<T, VEC>& lane, int64_t b, int64_t t) {
+  if (t >= 0) r.load(a.x + b * a.x_sb + t * a.x_st + lane.d, t < a.length ? lane.live : 0);
+  else r.load(a.x0 + (b * (W - 1) + t + W - 1) * a.dim + lane.d, a.x0 ? lane.live : 0);
 }
 
 template <typename T, int W, bool VEC>
 __global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvArgs<T> a) {
-  constexpr int C = kConvLaneCh, U = kConvStep;
+  constexpr int U = 16 / (int)sizeof(T);  // tokens a step: 16 or 8 bytes each in flight a lane
+  using Raw = ConvRaw<T, VEC>;
   const unsigned int tile = blockIdx.x % a.ctiles, rest = blockIdx.x / a.ctiles;
   const int64_t b = rest / a.groups;
   const int64_t t0 = ((int64_t)(rest % a.groups) * kConvWarps + (threadIdx.x >> 5)) * kConvRun;
   if (t0 >= a.length && t0 > 0) return;
   const ConvLane<T, VEC> lane((int64_t)tile * kConvChannels, a.dim);
-  const int64_t row = b * a.length, end = min(a.length, t0 + kConvRun);
-  float w[W][C], bias[C];
+  const int left = (int)max((int64_t)0, min(a.length - t0, (int64_t)kConvRun));
+  float2 w[W][2], bias[2];
+  conv_weights<W, VEC>(w, bias, a, lane);
+  float2 xs[W - 1 + U][2];  // token t - (W - 1) first
+  Raw raw[U];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const bool on = c < lane.live;
-    const int64_t d = lane.d + lane.at(c);
-#pragma unroll
-    for (int k = 0; k < W; ++k) w[k][c] = on ? a.w[d * W + k] : 0.0f;
-    bias[c] = on && a.bias ? a.bias[d] : 0.0f;
+  for (int k = 0; k < W - 1; ++k) {
+    Raw r;
+    conv_token<W, VEC>(r, a, lane, b, t0 - (W - 1) + k);
+    xs[k][0] = r.pair(0);
+    xs[k][1] = r.pair(1);
   }
-  float xs[W - 1 + U][C];  // token t0 - (W - 1) first
+  ConvStarts<W, U> ahead(a.starts, b * a.length, a.length);
+  ahead.load(t0);
+  const T* px = a.x + b * a.x_sb + t0 * a.x_st + lane.d;
 #pragma unroll
-  for (int k = 0; k < W - 1; ++k) conv_token<T, W, VEC>(a, lane, b, t0 - (W - 1) + k, xs[k]);
-  for (int64_t t = t0; t < end; t += U) {
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-      lane.load(xs[W - 1 + i], a.x + b * a.x_sb + (t + i) * a.x_st, t + i < end);
+  for (int i = 0; i < U; ++i) raw[i].load(px + i * a.x_st, i < left ? lane.live : 0);
+  T* py = a.y + (b * a.length + t0) * a.dim;
+  for (int t = 0; t < left; t += U) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int age = a.starts && t + i < end ? conv_age<W>(a.starts, row, t + i) : W - 1;
-      float u[C];
-#pragma unroll
-      for (int c = 0; c < C; ++c) u[c] = bias[c];
-#pragma unroll
-      for (int k = 0; k < W; ++k)  // tap k, W - 1 - k tokens back
-        if (W - 1 - k <= age) {
-#pragma unroll
-          for (int c = 0; c < C; ++c) u[c] = fmaf(w[k][c], xs[i + k][c], u[c]);
-        }
-      if (a.silu) {
-#pragma unroll
-        for (int c = 0; c < C; ++c) u[c] *= sigmoid_f32(u[c]);
-      }
-      if (t + i < end) lane.store(a.y + (row + t + i) * a.dim, u);
+      xs[W - 1 + i][0] = raw[i].pair(0);
+      xs[W - 1 + i][1] = raw[i].pair(1);
     }
+    const unsigned int bits = ahead.bits();
+    px += U * a.x_st;
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k)
+    for (int i = 0; i < U; ++i) raw[i].load(px + i * a.x_st, t + U + i < left ? lane.live : 0);
+    ahead.load(t0 + t + U);
+    by_fresh(bits, [&](auto some) {
 #pragma unroll
-      for (int c = 0; c < C; ++c) xs[k][c] = xs[U + k][c];
-  }
-  if (a.last && end == a.length && (end > t0 || t0 == 0)) {  // the run of the last token
-    const int age = a.length > 0 ? conv_age<W>(a.starts, row, a.length - 1) : W - 1;
+      for (int i = 0; i < U; ++i) {
+        const int age = decltype(some)::value ? conv_age<W>(bits, i) : W - 1;
+        float2 u[2] = {bias[0], bias[1]};
+#pragma unroll
+        for (int k = 0; k < W; ++k)  // tap k, W - 1 - k tokens back
+          if (!decltype(some)::value || W - 1 - k <= age) {
+            u[0] = __ffma2_rn(w[k][0], xs[i + k][0], u[0]);
+            u[1] = __ffma2_rn(w[k][1], xs[i + k][1], u[1]);
+          }
+        if (a.silu) {
+          u[0] = __fmul2_rn(u[0], sigmoid_pair(u[0]));
+          u[1] = __fmul2_rn(u[1], sigmoid_pair(u[1]));
+        }
+        if (t + i < left) lane.store(py + i * a.dim, u);
+      }
+    });
+    py += U * a.dim;
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) {
-      float v[C];
-      conv_token<T, W, VEC>(a, lane, b, a.length - (W - 1) + k, v);
-      if (W - 2 - k > age) {
+      xs[k][0] = xs[U + k][0];
+      xs[k][1] = xs[U + k][1];
+    }
+  }
+  if (a.last && t0 + left == a.length) {  // the run of the last token
+    // bit l of the ballot: a start at token length - 1 - l
+    const int64_t at = a.length - 1 - (threadIdx.x & 31);
+    const unsigned int starts = __ballot_sync(
+        0xffffffffu, a.starts && at >= 0 && (threadIdx.x & 31) < W - 1 && a.starts[b * a.length + at]);
+    const int age = starts ? __ffs(starts) - 1 : W - 1;
 #pragma unroll
-        for (int c = 0; c < C; ++c) v[c] = 0.0f;
-      }
+    for (int k = 0; k < W - 1; ++k) {
+      Raw r;
+      conv_token<W, VEC>(r, a, lane, b, a.length - (W - 1) + k);
+      float2 v[2] = {r.pair(0), r.pair(1)};
+      if (W - 2 - k > age) v[0] = v[1] = make_float2(0.0f, 0.0f);
       lane.store(a.last + (b * (W - 1) + k) * a.dim, v);
     }
   }
@@ -184,102 +292,127 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvArgs<T> a
 // A run of the VJP owns R = kConvRun - (W - 1) tokens and goes through the W - 1
 // after them too, whose du its last tokens need.
 template <typename T, int W, bool VEC>
-__global__ void __launch_bounds__(kConvWarps * 32) conv_bwd_kernel(ConvArgs<T> a) {
-  constexpr int C = kConvLaneCh, U = kConvStep, R = kConvRun - (W - 1);
+__global__ void __launch_bounds__(kConvWarps * 32, W <= 4 ? 2 : 1) conv_bwd_kernel(ConvArgs<T> a) {
+  constexpr int U = sizeof(T) == 2 && VEC ? 4 : 2, R = kConvRun - (W - 1);
+  using Raw = ConvRaw<T, VEC>;
   __shared__ float sums[kConvWarps][kConvChannels];
   const unsigned int tile = blockIdx.x % a.ctiles, rest = blockIdx.x / a.ctiles;
   const int64_t b = rest / a.groups;
   const int warp = threadIdx.x >> 5;
   const int64_t t0 = ((int64_t)(rest % a.groups) * kConvWarps + warp) * R;
   const ConvLane<T, VEC> lane((int64_t)tile * kConvChannels, a.dim);
-  const int64_t row = b * a.length, own = min(a.length, t0 + R);
-  float w[W][C], bias[C], dw[W][C], db[C];
+  float2 dw[W][2], db[2];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const bool on = c < lane.live;
-    const int64_t d = lane.d + lane.at(c);
+  for (int c = 0; c < 2; ++c) {
+    db[c] = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int k = 0; k < W; ++k) {
-      w[k][c] = on ? a.w[d * W + k] : 0.0f;
-      dw[k][c] = 0.0f;
-    }
-    bias[c] = on && a.bias ? a.bias[d] : 0.0f;
-    db[c] = 0.0f;
+    for (int k = 0; k < W; ++k) dw[k][c] = make_float2(0.0f, 0.0f);
   }
   if (t0 < a.length || t0 == 0) {
-    float xs[W - 1 + U][C];   // token t - (W - 1) first
-    float acc[W - 1 + U][C];  // and its gradient
+    // tokens from t0 on that are there, that the run owns and that it goes through
+    const int there = (int)max((int64_t)0, min(a.length - t0, (int64_t)kConvRun));
+    const int own = min(there, R), through = (int)min(a.length + W - 1 - t0, (int64_t)kConvRun);
+    float2 w[W][2], bias[2];
+    conv_weights<W, VEC>(w, bias, a, lane);
+    float2 xs[W - 1 + U][2];   // token t - (W - 1) first
+    float2 acc[W - 1 + U][2];  // and its gradient
+    Raw rx[U], rd[U];
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) {
-      conv_token<T, W, VEC>(a, lane, b, t0 - (W - 1) + k, xs[k]);
+      Raw r;
+      conv_token<W, VEC>(r, a, lane, b, t0 - (W - 1) + k);
 #pragma unroll
-      for (int c = 0; c < C; ++c) acc[k][c] = 0.0f;
+      for (int c = 0; c < 2; ++c) {
+        xs[k][c] = r.pair(c);
+        acc[k][c] = make_float2(0.0f, 0.0f);
+      }
     }
-    const int last_age = a.dlast && a.length > 0 ? conv_age<W>(a.starts, row, a.length - 1) : W - 1;
-    // token s, whose gradient is complete but for dlast's share
-    auto emit = [&](int64_t s, float (&v)[C]) {
-      if (s < (t0 == 0 ? 1 - W : t0) || s >= own) return;
-      const int back = (int)min(a.length - 1 - s, (int64_t)W);  // tokens before the last
-      if (a.dlast && back < W - 1 && back <= last_age) {
-        float e[C];
-        lane.load(e, a.dlast + (b * (W - 1) + W - 2 - back) * a.dim, true);
+    ConvStarts<W, U> ahead(a.starts, b * a.length, a.length);
+    ahead.load(t0);
+    const T* px = a.x + b * a.x_sb + t0 * a.x_st + lane.d;
+    const T* pd = a.dy + b * a.dy_sb + t0 * a.dy_st + lane.d;
 #pragma unroll
-        for (int c = 0; c < C; ++c) v[c] += e[c];
+    for (int i = 0; i < U; ++i) {
+      rx[i].load(px + i * a.x_st, i < there ? lane.live : 0);
+      rd[i].load(pd + i * a.dy_st, i < there && a.dy ? lane.live : 0);
+    }
+    // token s from t0 on, whose gradient is complete but for dlast's share
+    auto emit = [&](int s, const float2 (&v)[2]) {
+      if (s >= own || s < (t0 == 0 ? 1 - W : 0)) return;
+      float2 o[2] = {v[0], v[1]};
+      if (a.dlast && t0 + s >= a.length - (W - 1)) {
+        const int back = (int)(a.length - 1 - t0 - s);  // tokens before the last
+        bool same = true;  // no sequence starts after it
+        for (int k = 0; k < back && a.starts; ++k) same = same && !(a.length - 1 - k >= 0 && a.starts[(b + 1) * a.length - 1 - k]);
+        Raw e;
+        e.load(a.dlast + (b * (W - 1) + W - 2 - back) * a.dim + lane.d, same ? lane.live : 0);
+        o[0] = __fadd2_rn(o[0], e.pair(0));
+        o[1] = __fadd2_rn(o[1], e.pair(1));
       }
-      if (s >= 0) lane.store(a.dx + (row + s) * a.dim, v);
-      else if (a.dx0) lane.store(a.dx0 + (b * (W - 1) + s + W - 1) * a.dim, v);
+      if (t0 + s >= 0) lane.store(a.dx + (b * a.length + t0 + s) * a.dim, o);
+      else if (a.dx0) lane.store(a.dx0 + (b * (W - 1) + s + W - 1) * a.dim, o);
     };
-    for (int64_t t = t0; t < t0 + kConvRun && t < a.length + W - 1; t += U) {
-      float dy[U][C];
+    for (int t = 0; t < through; t += U) {
+      Raw dy[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        lane.load(xs[W - 1 + i], a.x + b * a.x_sb + (t + i) * a.x_st, t + i < a.length);
-        lane.load(dy[i], a.dy + b * a.dy_sb + (t + i) * a.dy_st, t + i < a.length && a.dy);
+      for (int i = 0; i < U; ++i) dy[i] = rd[i];
 #pragma unroll
-        for (int c = 0; c < C; ++c) acc[W - 1 + i][c] = 0.0f;
-      }
+      for (int i = 0; i < U; ++i)
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        if (t + i >= a.length) continue;
-        const int age = a.starts ? conv_age<W>(a.starts, row, t + i) : W - 1;
-        float u[C];
-#pragma unroll
-        for (int c = 0; c < C; ++c) u[c] = bias[c];
-#pragma unroll
-        for (int k = 0; k < W; ++k)
-          if (W - 1 - k <= age) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) u[c] = fmaf(w[k][c], xs[i + k][c], u[c]);
-          }
-        if (a.silu) {  // (u s)' = s + u s (1 - s)
-#pragma unroll
-          for (int c = 0; c < C; ++c) {
-            const float s = sigmoid_f32(u[c]);
-            u[c] = dy[i][c] * fmaf(u[c] * s, 1.0f - s, s);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < C; ++c) u[c] = dy[i][c];
+        for (int c = 0; c < 2; ++c) {
+          xs[W - 1 + i][c] = rx[i].pair(c);
+          acc[W - 1 + i][c] = make_float2(0.0f, 0.0f);
         }
-        const bool mine = t + i < own;
+      const unsigned int bits = ahead.bits();
+      px += U * a.x_st;
+      pd += U * a.dy_st;
 #pragma unroll
-        for (int c = 0; c < C; ++c) db[c] += mine ? u[c] : 0.0f;
-#pragma unroll
-        for (int k = 0; k < W; ++k)
-          if (W - 1 - k <= age) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-              acc[i + k][c] = fmaf(w[k][c], u[c], acc[i + k][c]);
-              if (mine) dw[k][c] = fmaf(u[c], xs[i + k][c], dw[k][c]);
-            }
-          }
+      for (int i = 0; i < U; ++i) {
+        rx[i].load(px + i * a.x_st, t + U + i < there ? lane.live : 0);
+        rd[i].load(pd + i * a.dy_st, t + U + i < there && a.dy ? lane.live : 0);
       }
+      ahead.load(t0 + t + U);
+      by_fresh(bits, [&](auto some) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int age = decltype(some)::value ? conv_age<W>(bits, i) : W - 1;
+          float2 u[2] = {bias[0], bias[1]}, mine[2];
+#pragma unroll
+          for (int k = 0; k < W; ++k)
+            if (!decltype(some)::value || W - 1 - k <= age) {
+              u[0] = __ffma2_rn(w[k][0], xs[i + k][0], u[0]);
+              u[1] = __ffma2_rn(w[k][1], xs[i + k][1], u[1]);
+            }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            if (a.silu) {  // (u s)' = s + u s (1 - s)
+              const float2 s = sigmoid_pair(u[c]), us = __fmul2_rn(u[c], s);
+              const float2 rest = make_float2(1.0f - s.x, 1.0f - s.y);
+              u[c] = __fmul2_rn(dy[i].pair(c), __ffma2_rn(us, rest, s));
+            } else {
+              u[c] = dy[i].pair(c);
+            }
+            // (0 beyond the sequence, as dy is)
+            mine[c] = t + i < own ? u[c] : make_float2(0.0f, 0.0f);
+            db[c] = __fadd2_rn(db[c], mine[c]);
+          }
+#pragma unroll
+          for (int k = 0; k < W; ++k)
+            if (!decltype(some)::value || W - 1 - k <= age) {
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                acc[i + k][c] = __ffma2_rn(w[k][c], u[c], acc[i + k][c]);
+                dw[k][c] = __ffma2_rn(mine[c], xs[i + k][c], dw[k][c]);
+              }
+            }
+        }
+      });
 #pragma unroll
       for (int i = 0; i < U; ++i) emit(t + i - (W - 1), acc[i]);
 #pragma unroll
       for (int k = 0; k < W - 1; ++k)
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
+        for (int c = 0; c < 2; ++c) {
           xs[k][c] = xs[U + k][c];
           acc[k][c] = acc[U + k][c];
         }
@@ -287,12 +420,15 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_bwd_kernel(ConvArgs<T> a
   }
   // over the warps, then one row of partial sums a CTA: [dim][W], then [dim]
   float* part = a.parts + (int64_t)rest * a.dim * (W + 1);
+  const int first = VEC ? (threadIdx.x & 31) * kConvLaneCh : threadIdx.x & 31;
 #pragma unroll
   for (int k = 0; k <= W; ++k) {
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      sums[warp][VEC ? (threadIdx.x & 31) * C + c : (threadIdx.x & 31) + 32 * c] =
-          k < W ? dw[k < W ? k : 0][c] : db[c];
+    for (int c = 0; c < 2; ++c) {
+      const float2 v = k < W ? dw[k < W ? k : 0][c] : db[c];
+      sums[warp][first + ConvLane<T, VEC>::at(2 * c)] = v.x;
+      sums[warp][first + ConvLane<T, VEC>::at(2 * c + 1)] = v.y;
+    }
     __syncthreads();
     const int64_t d = (int64_t)tile * kConvChannels + threadIdx.x;
     if (threadIdx.x < kConvChannels && d < a.dim) {
