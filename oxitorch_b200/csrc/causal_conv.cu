@@ -19,9 +19,7 @@
 // registers, over the CTA's warps in shared memory and over CTAs by a second kernel, each
 // in a fixed order.
 //
-// Bound by HBM in f32 and by the exponentials and reciprocals of the SiLU in bf16: two of
-// 16 a cycle and SM for each element take longer than its 4 bytes, so two channels share
-// a reciprocal.
+// Bound by HBM in f32, by the issue of instructions in bf16.
 #include <algorithm>
 #include <type_traits>
 
@@ -30,45 +28,60 @@
 namespace oxc {
 
 constexpr int kConvWarps = 8;
-constexpr int kConvLaneCh = 4;                  // channels a lane
-constexpr int kConvChannels = 32 * kConvLaneCh;  // a warp
 constexpr int kConvRun = 64;                    // tokens of a forward run
 constexpr int kConvMaxWidth = 8;
 
+// Pairs of channels a lane and tokens a step, with as many registers as two CTAs an SM
+// leave (up to four taps).  Measured at [4, 2048, 4096], forward: 2 pairs and 8 tokens
+// 34 us in bf16 and 50 in f32; 2 and 4 39 and 54; 1 and 8 41 and 53.  VJP in bf16: 2 and 4
+// 70 us, 2 and 8 78, 1 and 8 78; single elements (4095 channels) 1 and 4 88, 2 and 4 232;
+// in f32 1 and 8 87, 1 and 4 97, 2 and 4 150.
+constexpr int kConvFwdPairs = 2, kConvFwdStep = 8;
+template <typename T, bool VEC>
+struct ConvBwd {
+  static constexpr int kPairs = sizeof(T) == 2 && VEC ? 2 : 1, kStep = sizeof(T) == 2 ? 4 : 8;
+};
+
 // A lane's four channels as they are in memory: consecutive ones, in one access (VEC),
 // or 32 apart.  Loads are predicated, so that nothing waits for one before its use.
-template <typename T, bool VEC>
+template <typename T, bool VEC, int NP>
 struct ConvRaw;
-template <bool VEC>
-struct ConvRaw<float, VEC> {
-  float v[4];
+template <bool VEC, int NP>
+struct ConvRaw<float, VEC, NP> {
+  float v[2 * NP];
   __device__ __forceinline__ void load(const float* p, int live) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = 0.0f;
-    if constexpr (VEC) {
+    for (int k = 0; k < 2 * NP; ++k) v[k] = 0.0f;
+    if constexpr (VEC && NP == 1) {
+      asm("{.reg .pred p; setp.gt.s32 p, %3, 0; @p ld.global.v2.f32 {%0, %1}, [%2];}"
+          : "+f"(v[0]), "+f"(v[1]) : "l"(p), "r"(live));
+    } else if constexpr (VEC) {
       asm("{.reg .pred p; setp.gt.s32 p, %5, 0; @p ld.global.v4.f32 {%0, %1, %2, %3}, [%4];}"
           : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]) : "l"(p), "r"(live));
     } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 2 * NP; ++k)
         asm("{.reg .pred p; setp.gt.s32 p, %2, %3; @p ld.global.f32 %0, [%1];}"
             : "+f"(v[k]) : "l"(p + 32 * k), "r"(live), "r"(k));
     }
   }
   __device__ __forceinline__ float2 pair(int j) const { return make_float2(v[2 * j], v[2 * j + 1]); }
 };
-template <bool VEC>
-struct ConvRaw<bf16, VEC> {
-  uint32_t w[VEC ? 2 : 4];
+template <bool VEC, int NP>
+struct ConvRaw<bf16, VEC, NP> {
+  uint32_t w[VEC ? NP : 2 * NP];
   __device__ __forceinline__ void load(const bf16* p, int live) {
 #pragma unroll
-    for (int k = 0; k < (VEC ? 2 : 4); ++k) w[k] = 0u;
-    if constexpr (VEC) {
+    for (int k = 0; k < (VEC ? NP : 2 * NP); ++k) w[k] = 0u;
+    if constexpr (VEC && NP == 1) {
+      asm("{.reg .pred p; setp.gt.s32 p, %2, 0; @p ld.global.u32 %0, [%1];}"
+          : "+r"(w[0]) : "l"(p), "r"(live));
+    } else if constexpr (VEC) {
       asm("{.reg .pred p; setp.gt.s32 p, %3, 0; @p ld.global.v2.u32 {%0, %1}, [%2];}"
           : "+r"(w[0]), "+r"(w[1]) : "l"(p), "r"(live));
     } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 2 * NP; ++k)
         asm("{.reg .pred p; setp.gt.s32 p, %2, %3; @p ld.global.u16 %0, [%1];}"
             : "+r"(w[k]) : "l"(p + 32 * k), "r"(live), "r"(k));
     }
@@ -79,25 +92,31 @@ struct ConvRaw<bf16, VEC> {
   }
 };
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, int NP>
 struct ConvLane {
+  static constexpr int kMine = 2 * NP, kChannels = 32 * kMine;  // a lane's and a warp's
   int64_t d;  // the first channel
   int live;   // how many exist
   __device__ __forceinline__ ConvLane(int64_t d0, int64_t dim) {
     const int lane = threadIdx.x & 31;
-    d = VEC ? d0 + lane * kConvLaneCh : d0 + lane;
+    d = VEC ? d0 + lane * kMine : d0 + lane;
     live = 0;
 #pragma unroll
-    for (int k = 0; k < kConvLaneCh; ++k) live += d + at(k) < dim;
+    for (int k = 0; k < kMine; ++k) live += d + at(k) < dim;
   }
   static __device__ __forceinline__ int at(int k) { return VEC ? k : 32 * k; }
-  __device__ __forceinline__ void store(T* row, const float2 (&v)[2]) const {
-    const float f[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
+  __device__ __forceinline__ void store(T* row, const float2 (&v)[NP]) const {
+    float f[kMine];
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      f[2 * j] = v[j].x;
+      f[2 * j + 1] = v[j].y;
+    }
     if constexpr (VEC) {
-      if (live) store_from_f32<4>(row + d, f);
+      if (live) store_from_f32<kMine>(row + d, f);
     } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kMine; ++k) {
         const float one[1] = {f[k]};
         if (k < live) store_from_f32<1>(row + d + 32 * k, one);
       }
@@ -123,7 +142,6 @@ struct ConvArgs {
   T* dx0;
   float* parts;  // [batch * groups of runs, dim * (W + 1)]
   int64_t batch, length, dim;
-  int silu;
   unsigned int ctiles, groups;  // channel tiles, groups of kConvWarps runs
 };
 
@@ -138,16 +156,6 @@ __device__ __forceinline__ float rcp(float t) {
   return r;
 }
 __device__ __forceinline__ float sigmoid_f32(float v) { return rcp(1.0f + ex2(-1.44269504f * v)); }
-// Of two values: with a = 1 + exp(-v.x) and b = 1 + exp(-v.y), one reciprocal r = 1 / (a b)
-// gives both, b r and a r.  Where a b would pass f32's range (v below -40 in one of them),
-// one by one.
-__device__ __forceinline__ float2 sigmoid_pair(float2 v) {
-  const float a = 1.0f + ex2(-1.44269504f * v.x), b = 1.0f + ex2(-1.44269504f * v.y);
-  if (a > 0x1p60f || b > 0x1p60f) return make_float2(rcp(a), rcp(b));
-  const float r = rcp(a * b);
-  return make_float2(b * r, a * r);
-}
-
 // The tokens at which a sequence starts, a bit each: bit l is token t - (W - 1) + l, of the
 // W - 1 tokens before a step of U tokens and the step.
 template <int W, int U>
@@ -182,11 +190,11 @@ __device__ __forceinline__ void by_fresh(unsigned int bits, F f) {
 }
 
 // The weights and the bias of a lane's channels, in pairs.
-template <int W, bool VEC, typename T>
-__device__ __forceinline__ void conv_weights(float2 (&w)[W][2], float2 (&bias)[2], const ConvArgs<T>& a,
-                                             const ConvLane<T, VEC>& lane) {
+template <int W, bool VEC, int NP, typename T>
+__device__ __forceinline__ void conv_weights(float2 (&w)[W][NP], float2 (&bias)[NP], const ConvArgs<T>& a,
+                                             const ConvLane<T, VEC, NP>& lane) {
 #pragma unroll
-  for (int c = 0; c < kConvLaneCh; ++c) {
+  for (int c = 0; c < 2 * NP; ++c) {
     const bool on = c < lane.live;
     const int64_t d = lane.d + lane.at(c);
 #pragma unroll
@@ -202,33 +210,34 @@ __device__ __forceinline__ void conv_weights(float2 (&w)[W][2], float2 (&bias)[2
 }
 
 // Token t of a batch row, one of x0 if t is negative.
-template <int W, bool VEC, typename T>
-__device__ __forceinline__ void conv_token(ConvRaw<T, VEC>& r, const ConvArgs<T>& a,
-                                           const ConvLane<T, VEC>& lane, int64_t b, int64_t t) {
+template <int W, bool VEC, int NP, typename T>
+__device__ __forceinline__ void conv_token(ConvRaw<T, VEC, NP>& r, const ConvArgs<T>& a,
+                                           const ConvLane<T, VEC, NP>& lane, int64_t b, int64_t t) {
   if (t >= 0) r.load(a.x + b * a.x_sb + t * a.x_st + lane.d, t < a.length ? lane.live : 0);
   else r.load(a.x0 + (b * (W - 1) + t + W - 1) * a.dim + lane.d, a.x0 ? lane.live : 0);
 }
 
-template <typename T, int W, bool VEC>
-__global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvArgs<T> a) {
-  constexpr int U = 16 / (int)sizeof(T);  // tokens a step: 16 or 8 bytes each in flight a lane
-  using Raw = ConvRaw<T, VEC>;
+template <typename T, int W, bool VEC, bool SILU>
+__global__ void __launch_bounds__(kConvWarps * 32, W <= 4 ? 2 : 1) conv_fwd_kernel(ConvArgs<T> a) {
+  constexpr int U = kConvFwdStep, NP = kConvFwdPairs;
+  using Raw = ConvRaw<T, VEC, NP>;
   const unsigned int tile = blockIdx.x % a.ctiles, rest = blockIdx.x / a.ctiles;
   const int64_t b = rest / a.groups;
   const int64_t t0 = ((int64_t)(rest % a.groups) * kConvWarps + (threadIdx.x >> 5)) * kConvRun;
   if (t0 >= a.length && t0 > 0) return;
-  const ConvLane<T, VEC> lane((int64_t)tile * kConvChannels, a.dim);
+  using Lane = ConvLane<T, VEC, NP>;
+  const Lane lane((int64_t)tile * Lane::kChannels, a.dim);
   const int left = (int)max((int64_t)0, min(a.length - t0, (int64_t)kConvRun));
-  float2 w[W][2], bias[2];
-  conv_weights<W, VEC>(w, bias, a, lane);
-  float2 xs[W - 1 + U][2];  // token t - (W - 1) first
+  float2 w[W][NP], bias[NP];
+  conv_weights<W, VEC, NP>(w, bias, a, lane);
+  float2 xs[W - 1 + U][NP];  // token t - (W - 1) first
   Raw raw[U];
 #pragma unroll
   for (int k = 0; k < W - 1; ++k) {
     Raw r;
-    conv_token<W, VEC>(r, a, lane, b, t0 - (W - 1) + k);
-    xs[k][0] = r.pair(0);
-    xs[k][1] = r.pair(1);
+    conv_token<W, VEC, NP>(r, a, lane, b, t0 - (W - 1) + k);
+#pragma unroll
+    for (int c = 0; c < NP; ++c) xs[k][c] = r.pair(c);
   }
   ConvStarts<W, U> ahead(a.starts, b * a.length, a.length);
   ahead.load(t0);
@@ -238,10 +247,9 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvArgs<T> a
   T* py = a.y + (b * a.length + t0) * a.dim;
   for (int t = 0; t < left; t += U) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      xs[W - 1 + i][0] = raw[i].pair(0);
-      xs[W - 1 + i][1] = raw[i].pair(1);
-    }
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int c = 0; c < NP; ++c) xs[W - 1 + i][c] = raw[i].pair(c);
     const unsigned int bits = ahead.bits();
     px += U * a.x_st;
 #pragma unroll
@@ -251,26 +259,23 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvArgs<T> a
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int age = decltype(some)::value ? conv_age<W>(bits, i) : W - 1;
-        float2 u[2] = {bias[0], bias[1]};
+        float2 u[NP];
 #pragma unroll
-        for (int k = 0; k < W; ++k)  // tap k, W - 1 - k tokens back
-          if (!decltype(some)::value || W - 1 - k <= age) {
-            u[0] = __ffma2_rn(w[k][0], xs[i + k][0], u[0]);
-            u[1] = __ffma2_rn(w[k][1], xs[i + k][1], u[1]);
-          }
-        if (a.silu) {
-          u[0] = __fmul2_rn(u[0], sigmoid_pair(u[0]));
-          u[1] = __fmul2_rn(u[1], sigmoid_pair(u[1]));
+        for (int c = 0; c < NP; ++c) {
+          u[c] = bias[c];
+#pragma unroll
+          for (int k = 0; k < W; ++k)  // tap k, W - 1 - k tokens back
+            if (!decltype(some)::value || W - 1 - k <= age) u[c] = __ffma2_rn(w[k][c], xs[i + k][c], u[c]);
+          if (SILU) u[c] = make_float2(u[c].x * sigmoid_f32(u[c].x), u[c].y * sigmoid_f32(u[c].y));
         }
         if (t + i < left) lane.store(py + i * a.dim, u);
       }
     });
     py += U * a.dim;
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k) {
-      xs[k][0] = xs[U + k][0];
-      xs[k][1] = xs[U + k][1];
-    }
+    for (int k = 0; k < W - 1; ++k)
+#pragma unroll
+      for (int c = 0; c < NP; ++c) xs[k][c] = xs[U + k][c];
   }
   if (a.last && t0 + left == a.length) {  // the run of the last token
     // bit l of the ballot: a start at token length - 1 - l
@@ -281,9 +286,10 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvArgs<T> a
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) {
       Raw r;
-      conv_token<W, VEC>(r, a, lane, b, a.length - (W - 1) + k);
-      float2 v[2] = {r.pair(0), r.pair(1)};
-      if (W - 2 - k > age) v[0] = v[1] = make_float2(0.0f, 0.0f);
+      conv_token<W, VEC, NP>(r, a, lane, b, a.length - (W - 1) + k);
+      float2 v[NP];
+#pragma unroll
+      for (int c = 0; c < NP; ++c) v[c] = W - 2 - k > age ? make_float2(0.0f, 0.0f) : r.pair(c);
       lane.store(a.last + (b * (W - 1) + k) * a.dim, v);
     }
   }
@@ -291,19 +297,20 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvArgs<T> a
 
 // A run of the VJP owns R = kConvRun - (W - 1) tokens and goes through the W - 1
 // after them too, whose du its last tokens need.
-template <typename T, int W, bool VEC>
+template <typename T, int W, bool VEC, bool SILU>
 __global__ void __launch_bounds__(kConvWarps * 32, W <= 4 ? 2 : 1) conv_bwd_kernel(ConvArgs<T> a) {
-  constexpr int U = sizeof(T) == 2 && VEC ? 4 : 2, R = kConvRun - (W - 1);
-  using Raw = ConvRaw<T, VEC>;
-  __shared__ float sums[kConvWarps][kConvChannels];
+  constexpr int NP = ConvBwd<T, VEC>::kPairs, U = ConvBwd<T, VEC>::kStep, R = kConvRun - (W - 1);
+  using Raw = ConvRaw<T, VEC, NP>;
+  __shared__ float sums[kConvWarps][64 * NP];
   const unsigned int tile = blockIdx.x % a.ctiles, rest = blockIdx.x / a.ctiles;
   const int64_t b = rest / a.groups;
   const int warp = threadIdx.x >> 5;
   const int64_t t0 = ((int64_t)(rest % a.groups) * kConvWarps + warp) * R;
-  const ConvLane<T, VEC> lane((int64_t)tile * kConvChannels, a.dim);
-  float2 dw[W][2], db[2];
+  using Lane = ConvLane<T, VEC, NP>;
+  const Lane lane((int64_t)tile * Lane::kChannels, a.dim);
+  float2 dw[W][NP], db[NP];
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < NP; ++c) {
     db[c] = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < W; ++k) dw[k][c] = make_float2(0.0f, 0.0f);
@@ -312,17 +319,17 @@ __global__ void __launch_bounds__(kConvWarps * 32, W <= 4 ? 2 : 1) conv_bwd_kern
     // tokens from t0 on that are there, that the run owns and that it goes through
     const int there = (int)max((int64_t)0, min(a.length - t0, (int64_t)kConvRun));
     const int own = min(there, R), through = (int)min(a.length + W - 1 - t0, (int64_t)kConvRun);
-    float2 w[W][2], bias[2];
-    conv_weights<W, VEC>(w, bias, a, lane);
-    float2 xs[W - 1 + U][2];   // token t - (W - 1) first
-    float2 acc[W - 1 + U][2];  // and its gradient
+    float2 w[W][NP], bias[NP];
+    conv_weights<W, VEC, NP>(w, bias, a, lane);
+    float2 xs[W - 1 + U][NP];   // token t - (W - 1) first
+    float2 acc[W - 1 + U][NP];  // and its gradient
     Raw rx[U], rd[U];
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) {
       Raw r;
-      conv_token<W, VEC>(r, a, lane, b, t0 - (W - 1) + k);
+      conv_token<W, VEC, NP>(r, a, lane, b, t0 - (W - 1) + k);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < NP; ++c) {
         xs[k][c] = r.pair(c);
         acc[k][c] = make_float2(0.0f, 0.0f);
       }
@@ -337,17 +344,19 @@ __global__ void __launch_bounds__(kConvWarps * 32, W <= 4 ? 2 : 1) conv_bwd_kern
       rd[i].load(pd + i * a.dy_st, i < there && a.dy ? lane.live : 0);
     }
     // token s from t0 on, whose gradient is complete but for dlast's share
-    auto emit = [&](int s, const float2 (&v)[2]) {
+    auto emit = [&](int s, const float2 (&v)[NP]) {
       if (s >= own || s < (t0 == 0 ? 1 - W : 0)) return;
-      float2 o[2] = {v[0], v[1]};
+      float2 o[NP];
+#pragma unroll
+      for (int c = 0; c < NP; ++c) o[c] = v[c];
       if (a.dlast && t0 + s >= a.length - (W - 1)) {
         const int back = (int)(a.length - 1 - t0 - s);  // tokens before the last
         bool same = true;  // no sequence starts after it
         for (int k = 0; k < back && a.starts; ++k) same = same && !(a.length - 1 - k >= 0 && a.starts[(b + 1) * a.length - 1 - k]);
         Raw e;
         e.load(a.dlast + (b * (W - 1) + W - 2 - back) * a.dim + lane.d, same ? lane.live : 0);
-        o[0] = __fadd2_rn(o[0], e.pair(0));
-        o[1] = __fadd2_rn(o[1], e.pair(1));
+#pragma unroll
+        for (int c = 0; c < NP; ++c) o[c] = __fadd2_rn(o[c], e.pair(c));
       }
       if (t0 + s >= 0) lane.store(a.dx + (b * a.length + t0 + s) * a.dim, o);
       else if (a.dx0) lane.store(a.dx0 + (b * (W - 1) + s + W - 1) * a.dim, o);
@@ -359,7 +368,7 @@ __global__ void __launch_bounds__(kConvWarps * 32, W <= 4 ? 2 : 1) conv_bwd_kern
 #pragma unroll
       for (int i = 0; i < U; ++i)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < NP; ++c) {
           xs[W - 1 + i][c] = rx[i].pair(c);
           acc[W - 1 + i][c] = make_float2(0.0f, 0.0f);
         }
@@ -376,17 +385,15 @@ __global__ void __launch_bounds__(kConvWarps * 32, W <= 4 ? 2 : 1) conv_bwd_kern
 #pragma unroll
         for (int i = 0; i < U; ++i) {
           const int age = decltype(some)::value ? conv_age<W>(bits, i) : W - 1;
-          float2 u[2] = {bias[0], bias[1]}, mine[2];
+          float2 u[NP], mine[NP];
 #pragma unroll
-          for (int k = 0; k < W; ++k)
-            if (!decltype(some)::value || W - 1 - k <= age) {
-              u[0] = __ffma2_rn(w[k][0], xs[i + k][0], u[0]);
-              u[1] = __ffma2_rn(w[k][1], xs[i + k][1], u[1]);
-            }
+          for (int c = 0; c < NP; ++c) {
+            u[c] = bias[c];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            if (a.silu) {  // (u s)' = s + u s (1 - s)
-              const float2 s = sigmoid_pair(u[c]), us = __fmul2_rn(u[c], s);
+            for (int k = 0; k < W; ++k)
+              if (!decltype(some)::value || W - 1 - k <= age) u[c] = __ffma2_rn(w[k][c], xs[i + k][c], u[c]);
+            if (SILU) {  // (u s)' = s + u s (1 - s)
+              const float2 s = make_float2(sigmoid_f32(u[c].x), sigmoid_f32(u[c].y)), us = __fmul2_rn(u[c], s);
               const float2 rest = make_float2(1.0f - s.x, 1.0f - s.y);
               u[c] = __fmul2_rn(dy[i].pair(c), __ffma2_rn(us, rest, s));
             } else {
@@ -400,19 +407,26 @@ __global__ void __launch_bounds__(kConvWarps * 32, W <= 4 ? 2 : 1) conv_bwd_kern
           for (int k = 0; k < W; ++k)
             if (!decltype(some)::value || W - 1 - k <= age) {
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
+              for (int c = 0; c < NP; ++c) {
                 acc[i + k][c] = __ffma2_rn(w[k][c], u[c], acc[i + k][c]);
                 dw[k][c] = __ffma2_rn(mine[c], xs[i + k][c], dw[k][c]);
               }
             }
         }
       });
+      const int first = t - (W - 1);
+      if (first >= 0 && first + U <= own && (!a.dlast || t0 + first + U <= a.length - (W - 1))) {
+        T* to = a.dx + (b * a.length + t0 + first) * a.dim;
 #pragma unroll
-      for (int i = 0; i < U; ++i) emit(t + i - (W - 1), acc[i]);
+        for (int i = 0; i < U; ++i) lane.store(to + i * a.dim, acc[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < U; ++i) emit(first + i, acc[i]);
+      }
 #pragma unroll
       for (int k = 0; k < W - 1; ++k)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < NP; ++c) {
           xs[k][c] = xs[U + k][c];
           acc[k][c] = acc[U + k][c];
         }
@@ -420,18 +434,18 @@ __global__ void __launch_bounds__(kConvWarps * 32, W <= 4 ? 2 : 1) conv_bwd_kern
   }
   // over the warps, then one row of partial sums a CTA: [dim][W], then [dim]
   float* part = a.parts + (int64_t)rest * a.dim * (W + 1);
-  const int first = VEC ? (threadIdx.x & 31) * kConvLaneCh : threadIdx.x & 31;
+  const int first = VEC ? (threadIdx.x & 31) * 2 * NP : threadIdx.x & 31;
 #pragma unroll
   for (int k = 0; k <= W; ++k) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < NP; ++c) {
       const float2 v = k < W ? dw[k < W ? k : 0][c] : db[c];
-      sums[warp][first + ConvLane<T, VEC>::at(2 * c)] = v.x;
-      sums[warp][first + ConvLane<T, VEC>::at(2 * c + 1)] = v.y;
+      sums[warp][first + Lane::at(2 * c)] = v.x;
+      sums[warp][first + Lane::at(2 * c + 1)] = v.y;
     }
     __syncthreads();
-    const int64_t d = (int64_t)tile * kConvChannels + threadIdx.x;
-    if (threadIdx.x < kConvChannels && d < a.dim) {
+    const int64_t d = (int64_t)tile * Lane::kChannels + threadIdx.x;
+    if (threadIdx.x < Lane::kChannels && d < a.dim) {
       float s = sums[0][threadIdx.x];
 #pragma unroll
       for (int i = 1; i < kConvWarps; ++i) s += sums[i][threadIdx.x];
@@ -465,9 +479,8 @@ __global__ void __launch_bounds__(128) conv_step_kernel(const T* __restrict__ x,
 }
 
 template <typename T>
-static bool conv_vector(const T* p, int64_t sb, int64_t st) {
-  constexpr size_t n = kConvLaneCh * sizeof(T);
-  return !p || (aligned_to(p, n) && sb % kConvLaneCh == 0 && st % kConvLaneCh == 0);
+static bool conv_vector(const T* p, int64_t sb, int64_t st, int channels) {
+  return !p || (aligned_to(p, channels * sizeof(T)) && sb % channels == 0 && st % channels == 0);
 }
 
 // Calls f with the width as a compile-time number.
@@ -491,14 +504,17 @@ static int64_t conv_groups(int64_t length, int64_t run) {
 }
 
 template <typename T>
-static oxc_status conv_launch(ConvArgs<T> a, int64_t width, bool backward, cudaStream_t s) {
-  const bool vec = a.dim % kConvLaneCh == 0 && conv_vector(a.x, a.x_sb, a.x_st) &&
-                   conv_vector(a.dy, a.dy_sb, a.dy_st) && conv_vector(a.x0, 0, 0) &&
-                   conv_vector(a.dlast, 0, 0) && conv_vector<T>(a.y, 0, 0) &&
-                   conv_vector<T>(a.last, 0, 0) && conv_vector<T>(a.dx, 0, 0) &&
-                   conv_vector<T>(a.dx0, 0, 0);
+static oxc_status conv_launch(ConvArgs<T> a, int64_t width, bool silu, bool backward, cudaStream_t s) {
+  // a lane's channels where it reads vectors
+  const int wide = 2 * (backward ? ConvBwd<T, true>::kPairs : kConvFwdPairs);
+  const bool vec = a.dim % wide == 0 && conv_vector(a.x, a.x_sb, a.x_st, wide) &&
+                   conv_vector(a.dy, a.dy_sb, a.dy_st, wide) && conv_vector(a.x0, 0, 0, wide) &&
+                   conv_vector(a.dlast, 0, 0, wide) && conv_vector<T>(a.y, 0, 0, wide) &&
+                   conv_vector<T>(a.last, 0, 0, wide) && conv_vector<T>(a.dx, 0, 0, wide) &&
+                   conv_vector<T>(a.dx0, 0, 0, wide);
+  const int channels = vec || !backward ? wide : 2 * ConvBwd<T, false>::kPairs;
   const int64_t run = backward ? kConvRun - (width - 1) : kConvRun;
-  const int64_t ctiles = (a.dim + kConvChannels - 1) / kConvChannels;
+  const int64_t ctiles = (a.dim + 32 * channels - 1) / (32 * channels);
   const int64_t groups = conv_groups(a.length, run);
   if (ctiles * groups > 0x7fffffff / std::max<int64_t>(a.batch, 1))
     return fail(OXC_ERR_NOT_IMPLEMENTED, "not implemented: causal_conv: more than 2^31 blocks");
@@ -507,13 +523,11 @@ static oxc_status conv_launch(ConvArgs<T> a, int64_t width, bool backward, cudaS
   const unsigned int grid = (unsigned int)(a.batch * ctiles * groups);
   by_width(width, [&](auto w) {
     constexpr int W = decltype(w)::value;
-    if (backward) {
-      if (vec) conv_bwd_kernel<T, W, true><<<grid, kConvWarps * 32, 0, s>>>(a);
-      else conv_bwd_kernel<T, W, false><<<grid, kConvWarps * 32, 0, s>>>(a);
-    } else {
-      if (vec) conv_fwd_kernel<T, W, true><<<grid, kConvWarps * 32, 0, s>>>(a);
-      else conv_fwd_kernel<T, W, false><<<grid, kConvWarps * 32, 0, s>>>(a);
-    }
+    auto kernel = backward ? (silu ? (vec ? conv_bwd_kernel<T, W, true, true> : conv_bwd_kernel<T, W, false, true>)
+                                   : (vec ? conv_bwd_kernel<T, W, true, false> : conv_bwd_kernel<T, W, false, false>))
+                           : (silu ? (vec ? conv_fwd_kernel<T, W, true, true> : conv_fwd_kernel<T, W, false, true>)
+                                   : (vec ? conv_fwd_kernel<T, W, true, false> : conv_fwd_kernel<T, W, false, false>));
+    kernel<<<grid, kConvWarps * 32, 0, s>>>(a);
   });
   return check_launch("oxc_causal_conv");
 }
@@ -578,8 +592,7 @@ oxc_status oxc_causal_conv_fwd(const void* x, int64_t x_sb, int64_t x_st, const 
     a.batch = batch;
     a.length = length;
     a.dim = dim;
-    a.silu = silu;
-    return conv_launch<T>(a, width, false, s);
+    return conv_launch<T>(a, width, silu != 0, false, s);
   };
   return dtype == OXC_BF16 ? go(bf16{}) : go(0.0f);
 }
@@ -629,8 +642,7 @@ oxc_status oxc_causal_conv_bwd(const void* x, int64_t x_sb, int64_t x_st, const 
     a.batch = batch;
     a.length = length;
     a.dim = dim;
-    a.silu = silu;
-    return conv_launch<T>(a, width, true, s);
+    return conv_launch<T>(a, width, silu != 0, true, s);
   };
   const oxc_status r = dtype == OXC_BF16 ? go(bf16{}) : go(0.0f);
   if (r) return r;
