@@ -27,8 +27,7 @@
 namespace oxc {
 
 constexpr int kPolicyThreads = 256;            // per CTA at most
-constexpr int kPolicyCopies = 4;               // bulk copies per part of a row
-constexpr int kPolicyPart = 100 * 1024;        // bytes of a row per CTA, if a cluster can
+constexpr int kPolicyCopies = 2;               // bulk copies per part of a row
 constexpr int kPolicyMaxPart = 160 * 1024;     // and at most
 constexpr int kPolicyCluster = 8;              // CTAs per row at most
 
@@ -91,8 +90,10 @@ __device__ __forceinline__ PolicyTerm policy_term(const PolicyArgs& a, const Sam
 // sends to every CTA of the cluster, and a second the gradient; then the copies of the
 // next row's part are started, whose bytes L2 was asked for when the second pass began.
 // Every thread works out the row's term by itself.
+// (With registers for four CTAs of 256 threads an SM, not fewer: 334 us against 353 at f32
+// [8192, 32000].  Those of 128 threads lose by it: 134 us against 122 at bf16 [16384, 8000].)
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1)
 policy_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restrict__ dlogits,
                       PolicyArgs a) {
   namespace cg = cooperative_groups;
@@ -314,12 +315,13 @@ __global__ void __launch_bounds__(512) policy_wide_kernel(const T* __restrict__ 
   }
 }
 
-// CTAs per row: parts of up to 100 KB, two or more resident on an SM, as long as a
-// cluster of 8 holds the row, larger ones beyond; 0 if they would be too large.
-// More CTAs than the row needs while that leaves SMs idle and each has some work.
-static int policy_cluster(int64_t rows, int64_t bytes) {
+// CTAs per row: parts of up to 40 KB in f32 and 100 KB in bf16 as long as a cluster of 8
+// holds the row, larger ones beyond; 0 if they would be too large.  ([8192, 32000]: f32
+// in parts of 32 KB 344 us and of 64 KB 371, bf16 of 32 KB 224 and of 64 KB 200.)  More
+// CTAs than the row needs while that leaves SMs idle and each has some work.
+static int policy_cluster(int64_t rows, int64_t bytes, int64_t most) {
   int size = 1;
-  while (size < kPolicyCluster && bytes > (int64_t)size * kPolicyPart) size *= 2;
+  while (size < kPolicyCluster && bytes > size * most) size *= 2;
   if (bytes > (int64_t)size * kPolicyMaxPart) return 0;
   while (size < kPolicyCluster && rows * size * 2 <= sm_count() &&
          bytes >= (int64_t)size * 2 * kPolicyThreads * 16)
@@ -332,7 +334,7 @@ static oxc_status policy_launch(const void* logits, int64_t stride, void* dlogit
                                 const PolicyArgs& a, cudaStream_t s) {
   const T* x = static_cast<const T*>(logits);
   T* d = static_cast<T*>(dlogits);
-  const int size = policy_cluster(a.rows, (int64_t)a.vocab * sizeof(T));
+  const int size = policy_cluster(a.rows, (int64_t)a.vocab * sizeof(T), (sizeof(T) == 4 ? 40 : 100) * 1024);
   if (size == 0) {
     policy_wide_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, (int64_t)sm_count() * 4), 512, 0, s>>>(x, stride, d, a);
     return check_launch("oxc_policy_loss");

@@ -20,6 +20,7 @@ mathematical gradient.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
@@ -1015,7 +1016,33 @@ def _recorded(*tensors):
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    return _has_tangent(*[t for t in tensors if t is not None])
+    # tangents exist only within a level of forward-mode differentiation
+    return forward_ad._current_level >= 0 and _has_tangent(*[t for t in tensors if t is not None])
+
+
+def _fits(name, t, shape, dtype, device):
+    """_operand, with the checks that a fitting tensor passes first: a step takes ten of them."""
+    if (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape
+            or t.get_device() != device.index):
+        _operand(name, t, shape, dtype, device)
+
+
+def _lines(t):
+    """A [rows, cols] operand whose last dim is dense; others are copied."""
+    return t if t.stride(1) == 1 else _rows2d(t)
+
+
+def _flat(t):
+    """A float32 operand that is dense, None or copied."""
+    return t if t is None or t.is_contiguous() else dense(t)
+
+
+def _scratch(nbytes, device):
+    """(tensor, address, bytes) of a workspace; nothing where none is needed."""
+    if not nbytes:
+        return None, None, 0
+    ws = _workspace(nbytes, device)
+    return ws, ws.data_ptr(), ws.numel()
 
 
 # ---- short causal convolution --------------------------------------------------------------
@@ -1025,13 +1052,13 @@ def _conv_args(name, x, shape, weight, bias, x0, activation):
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError(f"invalid argument: {name} expects weight [dim, width]")
     width = weight.shape[1]
-    _operand("weight", weight, (dim, width), torch.float32, x.device)
+    _fits("weight", weight, (dim, width), torch.float32, x.device)
     if width < 1:
         raise ValueError(f"invalid argument: {name} needs at least one tap")
     if bias is not None:
-        _operand("bias", bias, (dim,), torch.float32, x.device)
+        _fits("bias", bias, (dim,), torch.float32, x.device)
     if x0 is not None:
-        _operand("x0", x0, (shape[0], width - 1, dim), x.dtype, x.device)
+        _fits("x0", x0, (shape[0], width - 1, dim), x.dtype, x.device)
     if activation not in _ACTIVATIONS:
         raise ValueError(f"invalid argument: unknown activation {activation!r}")
     return width
@@ -1043,7 +1070,7 @@ def causal_conv_fwd(x, weight, bias=None, x0=None, starts=None, activation="silu
     width = _conv_args("causal_conv", x, x.shape, weight, bias, x0, activation)
     B, T, D = x.shape
     x, starts = _sequence(x), _starts_tensor(starts, x)
-    weight, bias = dense(weight), None if bias is None else dense(bias)
+    weight, bias = _flat(weight), _flat(bias)
     x0 = None if x0 is None else _dense_any(x0)
     y = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
     last = torch.empty(B, width - 1, D, dtype=x.dtype, device=x.device)
@@ -1060,13 +1087,13 @@ def causal_conv_bwd(x, weight, bias=None, x0=None, dy=None, dlast=None, starts=N
     width = _conv_args("causal_conv", x, x.shape, weight, bias, x0, activation)
     B, T, D = x.shape
     x, starts = _sequence(x), _starts_tensor(starts, x)
-    weight, bias = dense(weight), None if bias is None else dense(bias)
+    weight, bias = _flat(weight), _flat(bias)
     x0 = None if x0 is None else _dense_any(x0)
     if dy is not None:
-        _operand("dy", dy, (B, T, D), x.dtype, x.device)
+        _fits("dy", dy, (B, T, D), x.dtype, x.device)
         dy = _sequence(dy)
     if dlast is not None:
-        _operand("dlast", dlast, (B, width - 1, D), x.dtype, x.device)
+        _fits("dlast", dlast, (B, width - 1, D), x.dtype, x.device)
         dlast = _dense_any(dlast)
     dx = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
     dx0 = torch.empty(B, width - 1, D, dtype=x.dtype, device=x.device)
@@ -1125,11 +1152,11 @@ def causal_conv_step(x, weight, bias, state, out=None, activation="silu"):
     if x.dim() != 2:
         raise ValueError(f"invalid argument: causal_conv_step expects [batch, dim], got {list(x.shape)}")
     width = _conv_args("causal_conv_step", x, x.shape, weight, bias, None, activation)
-    _operand("state", state, (x.shape[0], width - 1, x.shape[1]), x.dtype, x.device)
+    _fits("state", state, (x.shape[0], width - 1, x.shape[1]), x.dtype, x.device)
     out = _state_out(state, out)
     if _recorded(x, weight, bias, state):
         raise ValueError("invalid argument: causal_conv_step has no gradient; train with causal_conv")
-    x, weight, bias = _rows2d(x), dense(weight), None if bias is None else dense(bias)
+    x, weight, bias = _lines(x), _flat(weight), _flat(bias)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     N.check(N.load().oxc_causal_conv_step(
         x.data_ptr(), x.stride(0), weight.data_ptr(), _ptr(bias), state.data_ptr(), out.data_ptr(),
@@ -1143,7 +1170,7 @@ def _state_out(state, out):
     if out is None or out is state:
         out = state
     else:
-        _operand("out", out, state.shape, state.dtype, state.device)
+        _fits("out", out, state.shape, state.dtype, state.device)
     if not (state.is_contiguous() and out.is_contiguous()):
         raise ValueError("invalid argument: state and out must be contiguous")
     if 0 < abs(out.data_ptr() - state.data_ptr()) < state.element_size() * state.numel():
@@ -1159,21 +1186,17 @@ def _selective_args(x, lead, delta, A, B, C, D, z, delta_bias):
     if not isinstance(A, torch.Tensor) or A.dim() != 2:
         raise ValueError("invalid argument: A must be [dim, state]")
     n = A.shape[1]
-    _operand("delta", delta, x.shape, x.dtype, dev)
-    _operand("A", A, (dim, n), torch.float32, dev)
-    _operand("B", B, (*lead, n), x.dtype, dev)
-    _operand("C", C, (*lead, n), x.dtype, dev)
+    _fits("delta", delta, x.shape, x.dtype, dev)
+    _fits("A", A, (dim, n), torch.float32, dev)
+    _fits("B", B, (*lead, n), x.dtype, dev)
+    _fits("C", C, (*lead, n), x.dtype, dev)
     if D is not None:
-        _operand("D", D, (dim,), torch.float32, dev)
+        _fits("D", D, (dim,), torch.float32, dev)
     if z is not None:
-        _operand("z", z, x.shape, x.dtype, dev)
+        _fits("z", z, x.shape, x.dtype, dev)
     if delta_bias is not None:
-        _operand("delta_bias", delta_bias, (dim,), torch.float32, dev)
+        _fits("delta_bias", delta_bias, (dim,), torch.float32, dev)
     return n
-
-
-def _dense_or_none(t):
-    return None if t is None else dense(t)
 
 
 def selective_scan_fwd(x, delta, A, B, C, D=None, z=None, delta_bias=None, h0=None, starts=None,
@@ -1183,10 +1206,10 @@ def selective_scan_fwd(x, delta, A, B, C, D=None, z=None, delta_bias=None, h0=No
     batch, length, dim = x.shape
     n = _selective_args(x, (batch, length), delta, A, B, C, D, z, delta_bias)
     if h0 is not None:
-        _operand("h0", h0, (batch, dim, n), torch.float32, x.device)
+        _fits("h0", h0, (batch, dim, n), torch.float32, x.device)
     x, delta, B, C, starts = _sequence(x), _sequence(delta), _sequence(B), _sequence(C), _starts_tensor(starts, x)
     z = None if z is None else _sequence(z)
-    A, D, delta_bias, h0 = dense(A), _dense_or_none(D), _dense_or_none(delta_bias), _dense_or_none(h0)
+    A, D, delta_bias, h0 = _flat(A), _flat(D), _flat(delta_bias), _flat(h0)
     L = N.load()
     y = torch.empty(batch, length, dim, dtype=x.dtype, device=x.device)
     last = torch.empty(batch, dim, n, dtype=torch.float32, device=x.device)
@@ -1194,14 +1217,13 @@ def selective_scan_fwd(x, delta, A, B, C, D=None, z=None, delta_bias=None, h0=No
     if save:
         carry = torch.empty(L.oxc_selective_scan_carry_size(batch, length, dim, n), dtype=torch.float32,
                             device=x.device)
-    ws = _workspace(L.oxc_selective_scan_workspace_size(batch, length, dim, n, 0), x.device)
+    ws, at, nbytes = _scratch(L.oxc_selective_scan_workspace_size(batch, length, dim, n, 0), x.device)
     zsb, zst = (0, 0) if z is None else z.stride()[:2]
     N.check(L.oxc_selective_scan_fwd(
         x.data_ptr(), x.stride(0), x.stride(1), delta.data_ptr(), delta.stride(0), delta.stride(1),
         A.data_ptr(), B.data_ptr(), B.stride(0), B.stride(1), C.data_ptr(), C.stride(0), C.stride(1),
         _ptr(D), _ptr(z), zsb, zst, _ptr(delta_bias), _ptr(starts), _ptr(h0), y.data_ptr(),
-        last.data_ptr(), _ptr(carry), batch, length, dim, n, dt, ws.data_ptr(), ws.numel(),
-        _stream()), "selective_scan")
+        last.data_ptr(), _ptr(carry), batch, length, dim, n, dt, at, nbytes, _stream()), "selective_scan")
     return y, last, carry
 
 
@@ -1214,18 +1236,18 @@ def selective_scan_bwd(x, delta, A, B, C, carry, D=None, z=None, delta_bias=None
     batch, length, dim = x.shape
     n = _selective_args(x, (batch, length), delta, A, B, C, D, z, delta_bias)
     L = N.load()
-    _operand("carry", carry, (L.oxc_selective_scan_carry_size(batch, length, dim, n),), torch.float32, x.device)
+    _fits("carry", carry, (L.oxc_selective_scan_carry_size(batch, length, dim, n),), torch.float32, x.device)
     if not carry.is_contiguous():
         raise ValueError("invalid argument: carry must be contiguous")
     if dy is not None:
-        _operand("dy", dy, x.shape, x.dtype, x.device)
+        _fits("dy", dy, x.shape, x.dtype, x.device)
         dy = _sequence(dy)
     if dlast is not None:
-        _operand("dlast", dlast, (batch, dim, n), torch.float32, x.device)
+        _fits("dlast", dlast, (batch, dim, n), torch.float32, x.device)
         dlast = dense(dlast)
     x, delta, B, C, starts = _sequence(x), _sequence(delta), _sequence(B), _sequence(C), _starts_tensor(starts, x)
     z = None if z is None else _sequence(z)
-    A, D, delta_bias = dense(A), _dense_or_none(D), _dense_or_none(delta_bias)
+    A, D, delta_bias = _flat(A), _flat(D), _flat(delta_bias)
 
     def like(*shape):
         return torch.empty(shape, dtype=x.dtype, device=x.device)
@@ -1298,13 +1320,13 @@ def selective_step(x, delta, A, B, C, state, D=None, z=None, delta_bias=None, ou
         raise ValueError(f"invalid argument: selective_step expects [batch, dim], got {list(x.shape)}")
     batch, dim = x.shape
     n = _selective_args(x, (batch,), delta, A, B, C, D, z, delta_bias)
-    _operand("state", state, (batch, dim, n), torch.float32, x.device)
+    _fits("state", state, (batch, dim, n), torch.float32, x.device)
     out = _state_out(state, out)
     if _recorded(x, delta, A, B, C, state, D, z, delta_bias):
         raise ValueError("invalid argument: selective_step has no gradient; train with selective_scan")
-    x, delta, B, C = _rows2d(x), _rows2d(delta), _rows2d(B), _rows2d(C)
-    z = None if z is None else _rows2d(z)
-    A, D, delta_bias = dense(A), _dense_or_none(D), _dense_or_none(delta_bias)
+    x, delta, B, C = _lines(x), _lines(delta), _lines(B), _lines(C)
+    z = None if z is None else _lines(z)
+    A, D, delta_bias = _flat(A), _flat(D), _flat(delta_bias)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     N.check(N.load().oxc_selective_step(
         x.data_ptr(), x.stride(0), delta.data_ptr(), delta.stride(0), A.data_ptr(), B.data_ptr(),
@@ -1323,7 +1345,7 @@ def _sampled_tokens(name, logits, tokens):
     if not isinstance(tokens, torch.Tensor) or tokens.dtype not in (torch.int64, torch.int32):
         raise ValueError("invalid argument: tokens must be an int64 or int32 tensor")
     tokens = tokens.to(torch.int64).contiguous()
-    _operand("tokens", tokens, logits.shape[:-1], torch.int64, logits.device)
+    _fits("tokens", tokens, logits.shape[:-1], torch.int64, logits.device)
     return dt, tokens
 
 
@@ -1333,21 +1355,21 @@ def policy_loss_fwd(logits, tokens, old_logp, advantages, ref_logp=None, clip=0.
     comes from the same pass; None without ``grad``."""
     dt, tok = _sampled_tokens("policy_loss", logits, tokens)
     dev, lead = logits.device, logits.shape[:-1]
-    _operand("old_logp", old_logp, lead, torch.float32, dev)
-    _operand("advantages", advantages, lead, torch.float32, dev)
+    _fits("old_logp", old_logp, lead, torch.float32, dev)
+    _fits("advantages", advantages, lead, torch.float32, dev)
     below, above = clip if isinstance(clip, (tuple, list)) else (clip, clip)
     if not (below >= 0 and above >= 0 and 0 <= kl_coef < float("inf")):
         raise ValueError(f"invalid argument: clip {clip} and kl_coef {kl_coef} must not be negative")
     if ref_logp is not None:
-        _operand("ref_logp", ref_logp, lead, torch.float32, dev)
+        _fits("ref_logp", ref_logp, lead, torch.float32, dev)
     elif kl_coef > 0:
         raise ValueError("invalid argument: the KL term needs ref_logp")
     if grad_loss is not None:
         one = isinstance(grad_loss, torch.Tensor) and grad_loss.numel() == 1
-        _operand("grad_loss", grad_loss, grad_loss.shape if one else (1,), torch.float32, dev)
+        _fits("grad_loss", grad_loss, grad_loss.shape if one else (1,), torch.float32, dev)
     if flag is not None:
         _flag(flag, dev)
-    x, old, adv, ref = _rows2d(logits), dense(old_logp), dense(advantages), _dense_or_none(ref_logp)
+    x, old, adv, ref = _rows2d(logits), dense(old_logp), dense(advantages), _flat(ref_logp)
     rows, vocab = x.shape
     loss = torch.empty(1, dtype=torch.float32, device=dev)
     logp = torch.empty(lead, dtype=torch.float32, device=dev)

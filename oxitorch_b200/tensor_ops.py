@@ -302,18 +302,19 @@ def clip_grad_value_(grads, clip_value):
 
 def _flat_operands(name, tensors):
     """Checks dense float32 / bfloat16 tensors of the current device; returns their
-    addresses, sizes and dtype ids as arrays."""
+    addresses, sizes and dtype ids as arrays.  (A list at a time: a model has hundreds.)"""
     device = torch._C._cuda_getDevice()
-    dtypes = []
-    for t in tensors:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be torch CUDA tensors")
-        dt = _DTYPES.get(t.dtype)
-        if dt is None or t.get_device() != device:
+    try:
+        dtypes = [_DTYPES[t.dtype] for t in tensors]
+        if any([t.get_device() != device for t in tensors]):
+            raise KeyError
+        flat = all([t.is_contiguous() for t in tensors])
+    except (AttributeError, KeyError):
+        for t in tensors:
             _dtype_id(name, t)  # raises
-        if not t.is_contiguous() and not _permuted_dense(t):
-            raise ValueError(f"invalid argument: {name} must have dense storage")
-        dtypes.append(dt)
+        raise
+    if not flat and not all(t.is_contiguous() or _permuted_dense(t) for t in tensors):
+        raise ValueError(f"invalid argument: {name} must have dense storage")
     return (array("q", [t.data_ptr() for t in tensors]), array("q", [t.numel() for t in tensors]),
             array("i", dtypes))
 
@@ -349,7 +350,7 @@ def clip_global_norm_(grads, max_norm, out=None):
     """clip_grad_norm_ for p = 2 without waiting for the device, in two launches for up
     to 640 tensors: where max_norm / (norm + 1e-6) < 1, every gradient is scaled by it
     (in f32, rounded once), in place or into ``out``, a list of tensors of the same
-    shapes and types.  Returns the norm before, a 0-d float32 tensor (NaN or infinite
+    sizes and types.  Returns the norm before, a 0-d float32 tensor (NaN or infinite
     if the gradients are; a NaN norm leaves them as they are).
 
     Gradients are float32 or bfloat16, dense and apart from each other, any number of
@@ -366,19 +367,19 @@ def clip_global_norm_(grads, max_norm, out=None):
         out = [o for o, g in zip(out, grads) if g is not None]
     grads = [g for g in grads if g is not None]
     ptrs, sizes, dtypes = _flat_operands("gradients", grads)
-    for t in grads if out is None else out:
-        if isinstance(t, torch.Tensor) and t.requires_grad:
-            raise ValueError("invalid argument: clip_global_norm_ writes to tensors outside any graph")
     if not grads:
         return torch.zeros((), device="cuda")
     to = None
     if out is not None:
-        to = _flat_operands("outputs", out)[0]
-        for g, o in zip(grads, out):
-            if g.shape != o.shape or g.dtype != o.dtype or (
-                    not (g.is_contiguous() and o.is_contiguous()) and g.stride() != o.stride()):
-                raise ValueError(f"shape mismatch: an output {list(o.shape)} {o.dtype} for a gradient "
-                                 f"{list(g.shape)} {g.dtype}, or laid out otherwise")
+        to, counts, same = _flat_operands("outputs", out)
+        if same != dtypes or counts != sizes or not all([t.is_contiguous() for t in grads + out]):
+            for g, o in zip(grads, out):
+                if g.numel() != o.numel() or g.dtype != o.dtype or (
+                        not (g.is_contiguous() and o.is_contiguous()) and (g.shape, g.stride()) != (o.shape, o.stride())):
+                    raise ValueError(f"shape mismatch: an output {list(o.shape)} {o.dtype} for a gradient "
+                                     f"{list(g.shape)} {g.dtype}, or laid out otherwise")
+    if any([t.requires_grad for t in (grads if out is None else out)]):
+        raise ValueError("invalid argument: clip_global_norm_ writes to tensors outside any graph")
     L = N.load()
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
     ws = _workspace(L.oxc_clip_global_norm_workspace_size(len(grads)), norm.device)
