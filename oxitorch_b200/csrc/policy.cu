@@ -361,13 +361,23 @@ static oxc_status policy_launch(const void* logits, int64_t stride, void* dlogit
   cfg.numAttrs = 1;
   // as many clusters as are resident at once: with more, the rest would run as a
   // second wave (a cluster's CTAs share a GPC, so not every SM can be used)
-  int64_t resident = (int64_t)sm_count() * occupancy((const void*)kernel, threads, part) / size;
-  if (size > 1 && a.rows > resident / 2) {
-    int n = 0;
-    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, (const void*)kernel, &cfg);
-    if (e != cudaSuccess) return cuda_fail(e, "oxc_policy_loss");
-    resident = n;
+  static thread_local struct { int device = -1, part = 0, size = 0; int64_t resident = 0; } known;
+  int device = 0;
+  cudaGetDevice(&device);
+  if (known.device != device || known.part != part || known.size != size) {
+    int64_t resident = (int64_t)sm_count() * occupancy((const void*)kernel, threads, part) / size;
+    if (size > 1) {
+      int n = 0;
+      const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, (const void*)kernel, &cfg);
+      if (e != cudaSuccess) return cuda_fail(e, "oxc_policy_loss");
+      resident = n;
+    }
+    known.device = device;
+    known.part = part;
+    known.size = size;
+    known.resident = resident;
   }
+  const int64_t resident = known.resident;
   cfg.gridDim = dim3((unsigned)(std::min<int64_t>(a.rows, std::max<int64_t>(resident, 1)) * size));
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, x, stride, d, a);
   return e == cudaSuccess ? check_launch("oxc_policy_loss") : cuda_fail(e, "oxc_policy_loss");

@@ -1020,6 +1020,15 @@ def _recorded(*tensors):
     return forward_ad._current_level >= 0 and _has_tangent(*[t for t in tensors if t is not None])
 
 
+def _once(backward):
+    """once_differentiable, entered only where a gradient of the gradient is recorded."""
+    refusing = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (refusing if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run
+
+
 def _fits(name, t, shape, dtype, device):
     """_operand, with the checks that a fitting tensor passes first: a step takes ten of them."""
     if (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape
@@ -1083,48 +1092,54 @@ def causal_conv_fwd(x, weight, bias=None, x0=None, starts=None, activation="silu
 
 def causal_conv_bwd(x, weight, bias=None, x0=None, dy=None, dlast=None, starts=None, activation="silu"):
     """Returns (dx, dweight, dbias, dx0) for the gradients of y and of last (None = zero)."""
-    dt = _sequences("causal_conv", x)
+    _sequences("causal_conv", x)
     width = _conv_args("causal_conv", x, x.shape, weight, bias, x0, activation)
-    B, T, D = x.shape
-    x, starts = _sequence(x), _starts_tensor(starts, x)
-    weight, bias = _flat(weight), _flat(bias)
-    x0 = None if x0 is None else _dense_any(x0)
     if dy is not None:
-        _fits("dy", dy, (B, T, D), x.dtype, x.device)
-        dy = _sequence(dy)
+        _fits("dy", dy, x.shape, x.dtype, x.device)
     if dlast is not None:
-        _fits("dlast", dlast, (B, width - 1, D), x.dtype, x.device)
-        dlast = _dense_any(dlast)
-    dx = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
-    dx0 = torch.empty(B, width - 1, D, dtype=x.dtype, device=x.device)
-    dw = torch.empty(D * (width + 1), dtype=torch.float32, device=x.device)
+        _fits("dlast", dlast, (x.shape[0], width - 1, x.shape[2]), x.dtype, x.device)
+    return _causal_conv_bwd(x, weight, bias, x0, dy, dlast, _starts_tensor(starts, x), activation)
+
+
+def _causal_conv_bwd(x, weight, bias, x0, dy, dlast, starts, activation):
+    (B, T, D), width, dev = x.shape, weight.shape[1], x.device
+    x, weight, bias = _sequence(x), _flat(weight), _flat(bias)
+    x0 = None if x0 is None else _dense_any(x0)
+    dy = None if dy is None else _sequence(dy)
+    dlast = None if dlast is None else _dense_any(dlast)
+    dx = torch.empty(B, T, D, dtype=x.dtype, device=dev)
+    dx0 = torch.empty(B, width - 1, D, dtype=x.dtype, device=dev)
+    dw = torch.empty(D * (width + 1), dtype=torch.float32, device=dev)
     L = N.load()
-    ws = _workspace(L.oxc_causal_conv_bwd_workspace_size(B, T, D, width), x.device)
+    ws = _workspace(L.oxc_causal_conv_bwd_workspace_size(B, T, D, width), dev)
     ysb, yst = (0, 0) if dy is None else dy.stride()[:2]
+    xsb, xst, _ = x.stride()
     N.check(L.oxc_causal_conv_bwd(
-        x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), _ptr(bias), _ptr(x0),
-        _ptr(starts), _ptr(dy), ysb, yst, _ptr(dlast), dx.data_ptr(), dx0.data_ptr(), dw.data_ptr(),
-        B, T, D, width, _ACTIVATIONS[activation], dt, ws.data_ptr(), ws.numel(), _stream()),
+        x.data_ptr(), xsb, xst, weight.data_ptr(), _ptr(bias), _ptr(x0), _ptr(starts), _ptr(dy), ysb,
+        yst, _ptr(dlast), dx.data_ptr(), dx0.data_ptr(), dw.data_ptr(), B, T, D, width,
+        _ACTIVATIONS[activation], _DTYPES[x.dtype], ws.data_ptr(), ws.numel(), _stream()),
         "causal_conv backward")
-    return dx, dw[:D * width].view(D, width), dw[D * width:], dx0
+    dw, db = dw.split((D * width, D))
+    return dx, dw.view(D, width), db, dx0
 
 
 class _CausalConv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, x0, starts, activation):
         y, last = causal_conv_fwd(x, weight, bias, x0, starts, activation)
+        starts = _starts_tensor(starts, x)
         ctx.save_for_backward(x, weight, bias, x0, starts)
         ctx.activation = activation
         ctx.set_materialize_grads(False)
         return y, last
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dlast):
         if dy is None and dlast is None:
             return None, None, None, None, None, None
         x, weight, bias, x0, starts = ctx.saved_tensors
-        dx, dw, db, dx0 = causal_conv_bwd(x, weight, bias, x0, dy, dlast, starts, ctx.activation)
+        dx, dw, db, dx0 = _causal_conv_bwd(x, weight, bias, x0, dy, dlast, starts, ctx.activation)
         return dx, dw, None if bias is None else db, None if x0 is None else dx0, None, None
 
 
@@ -1232,30 +1247,34 @@ def selective_scan_bwd(x, delta, A, B, C, carry, D=None, z=None, delta_bias=None
     """Returns (dx, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dh0) for the gradients of y
     and of the last state (None = zero); carry is selective_scan_fwd's.  dz is None
     without z."""
-    dt = _sequences("selective_scan", x)
+    _sequences("selective_scan", x)
     batch, length, dim = x.shape
     n = _selective_args(x, (batch, length), delta, A, B, C, D, z, delta_bias)
-    L = N.load()
-    _fits("carry", carry, (L.oxc_selective_scan_carry_size(batch, length, dim, n),), torch.float32, x.device)
+    _fits("carry", carry, (N.load().oxc_selective_scan_carry_size(batch, length, dim, n),), torch.float32, x.device)
     if not carry.is_contiguous():
         raise ValueError("invalid argument: carry must be contiguous")
     if dy is not None:
         _fits("dy", dy, x.shape, x.dtype, x.device)
-        dy = _sequence(dy)
     if dlast is not None:
         _fits("dlast", dlast, (batch, dim, n), torch.float32, x.device)
-        dlast = dense(dlast)
-    x, delta, B, C, starts = _sequence(x), _sequence(delta), _sequence(B), _sequence(C), _starts_tensor(starts, x)
-    z = None if z is None else _sequence(z)
-    A, D, delta_bias = _flat(A), _flat(D), _flat(delta_bias)
+    return _selective_scan_bwd(x, delta, A, B, C, carry, D, z, delta_bias, _starts_tensor(starts, x), dy, dlast)
 
-    def like(*shape):
-        return torch.empty(shape, dtype=x.dtype, device=x.device)
-    dx, ddelta, dB, dC = like(*x.shape), like(*x.shape), like(batch, length, n), like(batch, length, n)
-    dz = None if z is None else like(*x.shape)
-    sums = torch.empty(dim * (n + 2), dtype=torch.float32, device=x.device)
-    dh0 = torch.empty(batch, dim, n, dtype=torch.float32, device=x.device)
-    ws = _workspace(L.oxc_selective_scan_workspace_size(batch, length, dim, n, 1), x.device)
+
+def _selective_scan_bwd(x, delta, A, B, C, carry, D, z, delta_bias, starts, dy, dlast):
+    (batch, length, dim), n, dev = x.shape, A.shape[1], x.device
+    x, delta, B, C = _sequence(x), _sequence(delta), _sequence(B), _sequence(C)
+    z = None if z is None else _sequence(z)
+    dy = None if dy is None else _sequence(dy)
+    A, D, delta_bias, dlast = _flat(A), _flat(D), _flat(delta_bias), _flat(dlast)
+    wide = (batch, length, dim)
+    dx, ddelta = torch.empty(wide, dtype=x.dtype, device=dev), torch.empty(wide, dtype=x.dtype, device=dev)
+    dB = torch.empty(batch, length, n, dtype=x.dtype, device=dev)
+    dC = torch.empty(batch, length, n, dtype=x.dtype, device=dev)
+    dz = None if z is None else torch.empty(wide, dtype=x.dtype, device=dev)
+    sums = torch.empty(dim * (n + 2), dtype=torch.float32, device=dev)
+    dh0 = torch.empty(batch, dim, n, dtype=torch.float32, device=dev)
+    L = N.load()
+    ws = _workspace(L.oxc_selective_scan_workspace_size(batch, length, dim, n, 1), dev)
     zsb, zst = (0, 0) if z is None else z.stride()[:2]
     ysb, yst = (0, 0) if dy is None else dy.stride()[:2]
     N.check(L.oxc_selective_scan_bwd(
@@ -1263,8 +1282,8 @@ def selective_scan_bwd(x, delta, A, B, C, carry, D=None, z=None, delta_bias=None
         A.data_ptr(), B.data_ptr(), B.stride(0), B.stride(1), C.data_ptr(), C.stride(0), C.stride(1),
         _ptr(D), _ptr(z), zsb, zst, _ptr(delta_bias), _ptr(starts), carry.data_ptr(), _ptr(dy), ysb,
         yst, _ptr(dlast), dx.data_ptr(), ddelta.data_ptr(), sums.data_ptr(), dB.data_ptr(),
-        dC.data_ptr(), _ptr(dz), dh0.data_ptr(), batch, length, dim, n, dt, ws.data_ptr(),
-        ws.numel(), _stream()), "selective_scan backward")
+        dC.data_ptr(), _ptr(dz), dh0.data_ptr(), batch, length, dim, n, _DTYPES[x.dtype],
+        ws.data_ptr(), ws.numel(), _stream()), "selective_scan backward")
     dA, dD, dbias = sums.split((dim * n, dim, dim))
     return dx, ddelta, dA.view(dim, n), dB, dC, dD, dz, dbias, dh0
 
@@ -1273,18 +1292,18 @@ class _SelectiveScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, delta, A, B, C, D, z, delta_bias, h0, starts):
         y, last, carry = selective_scan_fwd(x, delta, A, B, C, D, z, delta_bias, h0, starts)
-        ctx.save_for_backward(x, delta, A, B, C, carry, D, z, delta_bias, starts)
+        ctx.save_for_backward(x, delta, A, B, C, carry, D, z, delta_bias, _starts_tensor(starts, x))
         ctx.has_h0 = h0 is not None
         ctx.set_materialize_grads(False)
         return y, last
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dlast):
         if dy is None and dlast is None:
             return (None,) * 10
         x, delta, A, B, C, carry, D, z, delta_bias, starts = ctx.saved_tensors
-        dx, ddelta, dA, dB, dC, dD, dz, dbias, dh0 = selective_scan_bwd(
+        dx, ddelta, dA, dB, dC, dD, dz, dbias, dh0 = _selective_scan_bwd(
             x, delta, A, B, C, carry, D, z, delta_bias, starts, dy, dlast)
         return (dx, ddelta, dA, dB, dC, None if D is None else dD, dz,
                 None if delta_bias is None else dbias, dh0 if ctx.has_h0 else None, None)
@@ -1398,7 +1417,7 @@ class _PolicyLoss(torch.autograd.Function):
         return loss.reshape(()), logp
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g, _):
         if g is None:
             return (None,) * 9
