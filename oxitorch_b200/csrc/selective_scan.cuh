@@ -17,16 +17,25 @@
 //   dA = sum_{b,t} dt mu h_{t-1},  dD = sum e x,  ddelta_bias = sum ddelta
 //   dB_t[n] = sum_d lam dt x,  dC_t[n] = sum_d h e,  dz = dy inner silu'(z)
 //
-// A thread keeps SPT states of each of CPT channels in registers, LPC threads side
-// by side share a channel, and the CTA's threads walk through the tokens in tiles of
-// kTile.  Four more warps prepare the tiles: they copy the operands to shared memory two
-// tiles ahead, turn them into f32 steps (dt, dt x) there, once per token and channel,
-// and finish and store a tile's outputs, while the others walk through the next one.
-// Sums over n are made across the LPC threads, sums over d across the warp's other
-// lanes, its warps and the CTAs.  The VJP gets the state before each tile from the
+// A thread keeps SPT states of each of CPT channels in registers, LPC lanes of a warp
+// share a channel, and the CTA's threads walk through the tokens in tiles of kTile.
+// Eight more warps, the helpers, prepare the tiles: they copy the operands to shared
+// memory a tile or two ahead, turn them into f32 steps (dt, dt x) there, once per token
+// and channel, and finish and store a tile's outputs, while the others walk through the
+// next one.  (Without helpers, and with the copies a tile ahead, f32 [4, 2048, 4096] with
+// 16 states took 408 us forward and 1135 VJP, half of it the tiles' preparation.)  Sums
+// over n are made across the LPC lanes, sums over d across the warp's other lanes, its
+// warps and the CTAs.  The VJP gets the state before each tile from the
 // forward (`carry`) and goes through the tiles from the last to the first: it runs the
 // recurrence forward through a tile, keeping the state every few tokens, and from the last
 // of these backwards again with the decays and states of those few tokens in registers.
+//
+// What bounds it, at f32 [4, 2048, 4096] with 16 states, 2^29 exponentials: at 16 a cycle
+// and SM they take 120 us forward and 210 in the VJP (1.75 for each state), the operands
+// 82 and 143 us of HBM.  Shared memory, which hands the operands around (26 of its cycles
+// for 256 states forward, 49 in the VJP), and the issue of instructions (99 and 228 of
+// them, 4 a cycle) are as busy as the exponentials, and the CTAs are 256 and 128 for 148
+// SMs: 279 us forward (294 with the states saved), 777 VJP; bf16 the same.
 //
 // Where batch and dim leave the GPU idle, the sequence is cut into segments.  A
 // first kernel finds what each does to the state (its decay, exp(A sum dt), and the
@@ -275,8 +284,9 @@ __device__ __forceinline__ void tile_arrive(int id, int threads) {
 }
 constexpr int kFull = 1, kDone = 3;  // + the tile's parity
 
-// The threads that prepare tiles, behind those that walk through them: as many, since
-// their chains of dependent operations are as long.
+// The threads that prepare tiles, behind those that walk through them.  (With 128, whose
+// chains of dependent operations then were what the others waited for: bf16 [3, 4097,
+// 1001] with 24 states 390 us forward and 943 VJP instead of 280 and 719.)
 constexpr int kHelpers = 256;
 
 // Deals out the registers that a CTA is launched with: the warps that walk through tiles
@@ -506,12 +516,14 @@ __device__ __forceinline__ void through_segment(float2 (&h)[L::CPT][L::P], const
   for (int c = 0; c < L::CPT; ++c) {
     const int64_t d = at.d + c * L::kLanes;
     const float time = d < a.dim ? a.seg_time[row * a.dim + d] : 0.0f;
-    float2 own[L::P];
-    at.load(own, a.seg_state, c, row, a.dim, a.N);
+    // plain loads: the kernel before this one wrote them, so none may move above the wait
+    const float* q = a.seg_state + (row * a.dim + d) * a.N + at.sl * L::SPT;
+    const int there = d < a.dim ? a.N - at.sl * L::SPT : 0;
 #pragma unroll
     for (int i = 0; i < L::P; ++i) {
+      const float2 own = make_float2(2 * i < there ? q[2 * i] : 0.0f, 2 * i + 1 < there ? q[2 * i + 1] : 0.0f);
       const float2 e = exp2_pair(__fmul2_rn(A2[c][i], both(time)));
-      h[c][i] = time < 0.0f ? own[i] : __ffma2_rn(e, h[c][i], own[i]);
+      h[c][i] = time < 0.0f ? own : __ffma2_rn(e, h[c][i], own);
     }
   }
 }
@@ -565,7 +577,8 @@ inline Plan selective_plan(int64_t batch, int64_t length, int64_t dim, int64_t N
   p.ctiles = (dim + per - 1) / per;
   const int64_t tiles = std::max<int64_t>(1, selective_tiles(length));
   const int64_t work = std::max<int64_t>(1, batch * p.ctiles), slots = (backward ? 1 : 2) * sm_count();
-  // the rounds of the grid, and the first kernel's share
+  // the fewest segments for which the rounds of the grid, and the first kernel's work
+  // beside the other's, come to the least
   const double map = backward ? 0.3 : 0.6;
   double best = 0.0;
   int64_t segments = 1;

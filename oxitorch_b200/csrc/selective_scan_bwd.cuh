@@ -145,7 +145,8 @@ struct BackwardShared {
 
 constexpr int kRowsFree = 5;  // the barrier after which the rows of the tile before are read
 
-// Registers a thread: at the launch, then of those that walk and of the helpers.
+// Registers a thread: at the launch, then of those that walk and of the helpers.  (88
+// for the helpers: f32 [4, 2048, 4096] 777 us; 80: 786; 72: 812; 64, which spills: 960.)
 template <class L>
 struct Registers {
   static constexpr int kAll = L::kThreads + kHelpers;

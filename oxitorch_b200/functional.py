@@ -8,8 +8,9 @@ torch CUDA float32 tensors: torch supplies device memory, the stream and the
 autograd graph bookkeeping (``torch.autograd.Function``); all arithmetic on
 the path is ours.
 
-The last part of the file, the layers of a recurrent draft model, has no
-counterpart in the reference and takes bfloat16 activations too.
+The last parts of the file, the layers of a recurrent draft model and those of a
+selective state space model with its policy loss, have no counterpart in the
+reference and take bfloat16 activations too.
 
 ``grad_mode`` selects the backward semantics of the norms:
 ``"ref"`` (default) reproduces the reference graph, where ``rsqrt`` is
@@ -1014,10 +1015,10 @@ def _recorded(*tensors):
     """Whether autograd has to see a call on these tensors."""
     if torch.is_grad_enabled():
         for t in tensors:
-            if t is not None and t.requires_grad:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
                 return True
     # tangents exist only within a level of forward-mode differentiation
-    return forward_ad._current_level >= 0 and _has_tangent(*[t for t in tensors if t is not None])
+    return forward_ad._current_level >= 0 and _has_tangent(*[t for t in tensors if isinstance(t, torch.Tensor)])
 
 
 def _once(backward):
@@ -1154,7 +1155,7 @@ def causal_conv(x, weight, bias=None, x0=None, starts=None, activation="silu"):
     ones that a continuation of the rows takes as its x0.  ``starts`` (bool [batch,
     length]) marks where a new sequence begins in a packed row: taps do not reach
     before it, and last is zero there."""
-    if isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor) and _recorded(x, weight, bias, x0):
+    if _recorded(x, weight, bias, x0):
         return _CausalConv.apply(x, weight, bias, x0, starts, activation)
     return causal_conv_fwd(x, weight, bias, x0, starts, activation)
 
@@ -1323,9 +1324,7 @@ def selective_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, h0=None, 
     delta_bias may be None (no D x, no gate, no bias).  ``starts`` (bool [batch,
     length]) marks where a new sequence begins in a packed row: the state before such
     a token is zero."""
-    if (isinstance(x, torch.Tensor) and all(t is None or isinstance(t, torch.Tensor)
-                                            for t in (delta, A, B, C, D, z, delta_bias, h0))
-            and _recorded(x, delta, A, B, C, D, z, delta_bias, h0)):
+    if _recorded(x, delta, A, B, C, D, z, delta_bias, h0):
         return _SelectiveScan.apply(x, delta, A, B, C, D, z, delta_bias, h0, starts)
     return selective_scan_fwd(x, delta, A, B, C, D, z, delta_bias, h0, starts, save=False)[:2]
 
