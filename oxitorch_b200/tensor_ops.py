@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 from array import array
+from operator import attrgetter
 
 import torch
 
@@ -300,23 +301,35 @@ def clip_grad_value_(grads, clip_value):
                 "clip_grad_value_")
 
 
+_TENSORS = {torch.Tensor, torch.nn.Parameter}
+_dtype_of, _requires_grad = attrgetter("dtype"), attrgetter("requires_grad")
+
+
 def _flat_operands(name, tensors):
     """Checks dense float32 / bfloat16 tensors of the current device; returns their
-    addresses, sizes and dtype ids as arrays.  (A list at a time: a model has hundreds.)"""
-    device = torch._C._cuda_getDevice()
-    try:
-        dtypes = [_DTYPES[t.dtype] for t in tensors]
-        if any([t.get_device() != device for t in tensors]):
-            raise KeyError
-        flat = all([t.is_contiguous() for t in tensors])
-    except (AttributeError, KeyError):
+    addresses, sizes and dtype ids as arrays, and whether all are contiguous.  (By whole
+    lists, as a model has hundreds: 0.3 us a tensor.)"""
+    tensor = torch.Tensor
+    if not _TENSORS.issuperset(map(type, tensors)) and not all(isinstance(t, tensor) for t in tensors):
+        raise TypeError(f"{name} must be torch CUDA tensors")
+    kinds = set(map(_dtype_of, tensors))
+    if not kinds <= _DTYPES.keys() or not {torch._C._cuda_getDevice()}.issuperset(map(tensor.get_device, tensors)):
         for t in tensors:
             _dtype_id(name, t)  # raises
-        raise
+    flat = all(map(tensor.is_contiguous, tensors))
     if not flat and not all(t.is_contiguous() or _permuted_dense(t) for t in tensors):
         raise ValueError(f"invalid argument: {name} must have dense storage")
-    return (array("q", [t.data_ptr() for t in tensors]), array("q", [t.numel() for t in tensors]),
-            array("i", dtypes))
+    if len(kinds) == 1:
+        dtypes = array("i", (_DTYPES[kinds.pop()],)) * len(tensors)
+    else:
+        dtypes = array("i", [_DTYPES[t.dtype] for t in tensors])
+    return array("q", map(tensor.data_ptr, tensors)), array("q", map(tensor.numel, tensors)), dtypes, flat
+
+
+def _listed(tensors):
+    """The tensors of a list that are there."""
+    tensors = list(tensors)
+    return [t for t in tensors if t is not None] if type(None) in set(map(type, tensors)) else tensors
 
 
 def _permuted_dense(t):
@@ -333,8 +346,8 @@ def global_norm(tensors):
     """sqrt of the sum over all tensors of sum(v * v), summed in f64, as a 0-d float32
     tensor: the host does not wait for it.  Tensors are float32 or bfloat16, dense, any
     number of them; None is skipped."""
-    tensors = [t for t in tensors if t is not None]
-    ptrs, sizes, dtypes = _flat_operands("tensors", tensors)
+    tensors = _listed(tensors)
+    ptrs, sizes, dtypes, _ = _flat_operands("tensors", tensors)
     if not tensors:
         return torch.zeros((), device="cuda")
     L = N.load()
@@ -364,21 +377,22 @@ def clip_global_norm_(grads, max_norm, out=None):
         out = list(out)
         if len(out) != len(grads):
             raise ValueError(f"invalid argument: {len(out)} outputs for {len(grads)} gradients")
-        out = [o for o, g in zip(out, grads) if g is not None]
-    grads = [g for g in grads if g is not None]
-    ptrs, sizes, dtypes = _flat_operands("gradients", grads)
+        if type(None) in set(map(type, grads)):
+            out = [o for o, g in zip(out, grads) if g is not None]
+    grads = _listed(grads)
+    ptrs, sizes, dtypes, flat = _flat_operands("gradients", grads)
     if not grads:
         return torch.zeros((), device="cuda")
     to = None
     if out is not None:
-        to, counts, same = _flat_operands("outputs", out)
-        if same != dtypes or counts != sizes or not all([t.is_contiguous() for t in grads + out]):
+        to, counts, same, flat_too = _flat_operands("outputs", out)
+        if same != dtypes or counts != sizes or not (flat and flat_too):
             for g, o in zip(grads, out):
                 if g.numel() != o.numel() or g.dtype != o.dtype or (
                         not (g.is_contiguous() and o.is_contiguous()) and (g.shape, g.stride()) != (o.shape, o.stride())):
                     raise ValueError(f"shape mismatch: an output {list(o.shape)} {o.dtype} for a gradient "
                                      f"{list(g.shape)} {g.dtype}, or laid out otherwise")
-    if any([t.requires_grad for t in (grads if out is None else out)]):
+    if any(map(_requires_grad, grads if out is None else out)):
         raise ValueError("invalid argument: clip_global_norm_ writes to tensors outside any graph")
     L = N.load()
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
