@@ -581,17 +581,16 @@ inline Plan selective_plan(int64_t batch, int64_t length, int64_t dim, int64_t N
   // beside the other's, come to the least
   const double map = backward ? 0.3 : 0.6;
   double best = 0.0;
-  int64_t segments = 1;
-  for (int64_t k = 1; k <= std::min<int64_t>(kMaxSegments, std::max<int64_t>(1, tiles / 4)); ++k) {
+  for (int64_t want = 1; want <= std::min<int64_t>(kMaxSegments, std::max<int64_t>(1, tiles / 4)); ++want) {
+    const int64_t each = (tiles + want - 1) / want, k = (tiles + each - 1) / each;
     const int64_t rounds = (work * k + slots - 1) / slots;
-    const double cost = (double)rounds / (double)k * (1.0 + map * (double)(k - 1) / (double)k);
-    if (k == 1 || cost < best * 0.98) {
+    const double cost = (double)(rounds * each) * (1.0 + map * (double)(k - 1) / (double)k);
+    if (want == 1 || cost < best * 0.98) {
       best = cost;
-      segments = k;
+      p.seg_tiles = (int)each;
+      p.segments = (int)k;
     }
   }
-  p.seg_tiles = (int)((tiles + segments - 1) / segments);
-  p.segments = (int)((tiles + p.seg_tiles - 1) / p.seg_tiles);
   return p;
 }
 
