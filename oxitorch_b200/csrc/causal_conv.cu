@@ -28,7 +28,6 @@
 namespace oxc {
 
 constexpr int kConvWarps = 8;
-constexpr int kConvRun = 64;                    // tokens of a forward run
 constexpr int kConvMaxWidth = 8;
 
 // Pairs of channels a lane and tokens a step, with as many registers as two CTAs an SM
@@ -142,6 +141,7 @@ struct ConvArgs {
   T* dx0;
   float* parts;  // [batch * groups of runs, dim * (W + 1)]
   int64_t batch, length, dim;
+  int run;  // tokens that a warp goes through
   unsigned int ctiles, groups;  // channel tiles, groups of kConvWarps runs
 };
 
@@ -223,11 +223,11 @@ __global__ void __launch_bounds__(kConvWarps * 32, W <= 4 ? 2 : 1) conv_fwd_kern
   using Raw = ConvRaw<T, VEC, NP>;
   const unsigned int tile = blockIdx.x % a.ctiles, rest = blockIdx.x / a.ctiles;
   const int64_t b = rest / a.groups;
-  const int64_t t0 = ((int64_t)(rest % a.groups) * kConvWarps + (threadIdx.x >> 5)) * kConvRun;
+  const int64_t t0 = ((int64_t)(rest % a.groups) * kConvWarps + (threadIdx.x >> 5)) * a.run;
   if (t0 >= a.length && t0 > 0) return;
   using Lane = ConvLane<T, VEC, NP>;
   const Lane lane((int64_t)tile * Lane::kChannels, a.dim);
-  const int left = (int)max((int64_t)0, min(a.length - t0, (int64_t)kConvRun));
+  const int left = (int)max((int64_t)0, min(a.length - t0, (int64_t)a.run));
   float2 w[W][NP], bias[NP];
   conv_weights<W, VEC, NP>(w, bias, a, lane);
   float2 xs[W - 1 + U][NP];  // token t - (W - 1) first
@@ -295,16 +295,16 @@ __global__ void __launch_bounds__(kConvWarps * 32, W <= 4 ? 2 : 1) conv_fwd_kern
   }
 }
 
-// A run of the VJP owns R = kConvRun - (W - 1) tokens and goes through the W - 1
+// A run of the VJP owns R = a.run - (W - 1) tokens and goes through the W - 1
 // after them too, whose du its last tokens need.
 template <typename T, int W, bool VEC, bool SILU>
 __global__ void __launch_bounds__(kConvWarps * 32, W <= 4 ? 2 : 1) conv_bwd_kernel(ConvArgs<T> a) {
-  constexpr int NP = ConvBwd<T, VEC>::kPairs, U = ConvBwd<T, VEC>::kStep, R = kConvRun - (W - 1);
+  constexpr int NP = ConvBwd<T, VEC>::kPairs, U = ConvBwd<T, VEC>::kStep;
   using Raw = ConvRaw<T, VEC, NP>;
   __shared__ float sums[kConvWarps][64 * NP];
   const unsigned int tile = blockIdx.x % a.ctiles, rest = blockIdx.x / a.ctiles;
   const int64_t b = rest / a.groups;
-  const int warp = threadIdx.x >> 5;
+  const int warp = threadIdx.x >> 5, R = a.run - (W - 1);
   const int64_t t0 = ((int64_t)(rest % a.groups) * kConvWarps + warp) * R;
   using Lane = ConvLane<T, VEC, NP>;
   const Lane lane((int64_t)tile * Lane::kChannels, a.dim);
@@ -317,8 +317,8 @@ __global__ void __launch_bounds__(kConvWarps * 32, W <= 4 ? 2 : 1) conv_bwd_kern
   }
   if (t0 < a.length || t0 == 0) {
     // tokens from t0 on that are there, that the run owns and that it goes through
-    const int there = (int)max((int64_t)0, min(a.length - t0, (int64_t)kConvRun));
-    const int own = min(there, R), through = (int)min(a.length + W - 1 - t0, (int64_t)kConvRun);
+    const int there = (int)max((int64_t)0, min(a.length - t0, (int64_t)a.run));
+    const int own = min(there, R), through = (int)min(a.length + W - 1 - t0, (int64_t)a.run);
     float2 w[W][NP], bias[NP];
     conv_weights<W, VEC, NP>(w, bias, a, lane);
     float2 xs[W - 1 + U][NP];   // token t - (W - 1) first
@@ -498,13 +498,40 @@ static void by_width(int64_t width, F f) {
   }
 }
 
-static int64_t conv_groups(int64_t length, int64_t run) {
-  const int64_t per = run * kConvWarps;
-  return std::max<int64_t>(1, (length + per - 1) / per);
+// How a call is cut: tokens that a warp goes through, and groups of warps along a row.
+struct ConvCut {
+  int run;
+  int64_t ctiles, groups;
+};
+
+// The longest run among those whose grid takes the least time: its rounds on the GPU, at
+// a run's tokens each and some for its beginning.  (Against runs of 64, bf16, four taps:
+// [1, 512, 2048] 6.5 us instead of 12.6 forward and 12.4 instead of 25 VJP; [4, 2048, 4096]
+// 31.7 instead of 35 and 66 instead of 72; f32 there 51.5 instead of 50.6, HBM-bound, and 82
+// instead of 88.  At most 128 tokens: the VJPs 70 and 88.  At least 32: [1, 512, 2048] 8.5
+// and 16.6.)
+static ConvCut conv_cut(int64_t batch, int64_t length, int64_t dim, int64_t width, int channels,
+                        bool backward) {
+  constexpr int kLeast = 16, kMost = 256, kBeginning = 24;
+  ConvCut best{0, (dim + 32 * channels - 1) / (32 * channels), 1};
+  const int64_t slots = (width <= 4 ? 2 : 1) * sm_count(), tiles = batch * best.ctiles;
+  int64_t least = 0;
+  for (int run = kLeast; run <= kMost; run += 8) {
+    const int64_t per = (backward ? run - (width - 1) : run) * kConvWarps;
+    const int64_t groups = std::max<int64_t>(1, (length + per - 1) / per);
+    const int64_t cost = (tiles * groups + slots - 1) / slots * (run + kBeginning);
+    if (!best.run || cost <= least) {
+      least = cost;
+      best.run = run;
+      best.groups = groups;
+    }
+  }
+  return best;
 }
 
 template <typename T>
-static oxc_status conv_launch(ConvArgs<T> a, int64_t width, bool silu, bool backward, cudaStream_t s) {
+static oxc_status conv_launch(ConvArgs<T> a, int64_t width, bool silu, bool backward, cudaStream_t s,
+                              int64_t* sums = nullptr) {
   // a lane's channels where it reads vectors
   const int wide = 2 * (backward ? ConvBwd<T, true>::kPairs : kConvFwdPairs);
   const bool vec = a.dim % wide == 0 && conv_vector(a.x, a.x_sb, a.x_st, wide) &&
@@ -513,14 +540,14 @@ static oxc_status conv_launch(ConvArgs<T> a, int64_t width, bool silu, bool back
                    conv_vector<T>(a.last, 0, 0, wide) && conv_vector<T>(a.dx, 0, 0, wide) &&
                    conv_vector<T>(a.dx0, 0, 0, wide);
   const int channels = vec || !backward ? wide : 2 * ConvBwd<T, false>::kPairs;
-  const int64_t run = backward ? kConvRun - (width - 1) : kConvRun;
-  const int64_t ctiles = (a.dim + 32 * channels - 1) / (32 * channels);
-  const int64_t groups = conv_groups(a.length, run);
-  if (ctiles * groups > 0x7fffffff / std::max<int64_t>(a.batch, 1))
+  const ConvCut cut = conv_cut(a.batch, a.length, a.dim, width, channels, backward);
+  if (cut.ctiles * cut.groups > 0x7fffffff / std::max<int64_t>(a.batch, 1))
     return fail(OXC_ERR_NOT_IMPLEMENTED, "not implemented: causal_conv: more than 2^31 blocks");
-  a.ctiles = (unsigned int)ctiles;
-  a.groups = (unsigned int)groups;
-  const unsigned int grid = (unsigned int)(a.batch * ctiles * groups);
+  a.run = cut.run;
+  a.ctiles = (unsigned int)cut.ctiles;
+  a.groups = (unsigned int)cut.groups;
+  if (sums) *sums = a.batch * cut.groups;
+  const unsigned int grid = (unsigned int)(a.batch * cut.ctiles * cut.groups);
   by_width(width, [&](auto w) {
     constexpr int W = decltype(w)::value;
     auto kernel = backward ? (silu ? (vec ? conv_bwd_kernel<T, W, true, true> : conv_bwd_kernel<T, W, false, true>)
@@ -599,8 +626,10 @@ oxc_status oxc_causal_conv_fwd(const void* x, int64_t x_sb, int64_t x_st, const 
 
 size_t oxc_causal_conv_bwd_workspace_size(int64_t batch, int64_t length, int64_t dim, int64_t width) {
   if (batch <= 0 || length < 0 || dim <= 0 || width < 1 || width > kConvMaxWidth) return 0;
-  return sizeof(float) * (size_t)(batch * conv_groups(length, kConvRun - (width - 1))) *
-         (size_t)(dim * (width + 1));
+  int64_t groups = 1;
+  for (int pairs = 1; pairs <= 2; ++pairs)  // of every ConvBwd
+    groups = std::max(groups, conv_cut(batch, length, dim, width, 2 * pairs, true).groups);
+  return sizeof(float) * (size_t)(batch * groups) * (size_t)(dim * (width + 1));
 }
 
 oxc_status oxc_causal_conv_bwd(const void* x, int64_t x_sb, int64_t x_st, const float* w,
@@ -622,6 +651,7 @@ oxc_status oxc_causal_conv_bwd(const void* x, int64_t x_sb, int64_t x_st, const 
   }
   if (!workspace || workspace_bytes < oxc_causal_conv_bwd_workspace_size(batch, length, dim, width))
     return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: causal_conv backward: workspace too small");
+  int64_t sums = 0;  // rows of partial sums
   auto go = [&](auto zero) {
     using T = decltype(zero);
     ConvArgs<T> a{};
@@ -642,12 +672,11 @@ oxc_status oxc_causal_conv_bwd(const void* x, int64_t x_sb, int64_t x_st, const 
     a.batch = batch;
     a.length = length;
     a.dim = dim;
-    return conv_launch<T>(a, width, silu != 0, true, s);
+    return conv_launch<T>(a, width, silu != 0, true, s, &sums);
   };
   const oxc_status r = dtype == OXC_BF16 ? go(bf16{}) : go(0.0f);
   if (r) return r;
-  launch_colsum_partials(static_cast<const float*>(workspace),
-                         (int)(batch * conv_groups(length, kConvRun - (width - 1))), cols, dw, s);
+  launch_colsum_partials(static_cast<const float*>(workspace), (int)sums, cols, dw, s);
   return check_launch("oxc_causal_conv_bwd (sums)");
 }
 
