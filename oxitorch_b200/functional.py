@@ -1055,6 +1055,10 @@ def _scratch(nbytes, device):
     return ws, ws.data_ptr(), ws.numel()
 
 
+def _dense_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 # ---- short causal convolution --------------------------------------------------------------
 
 def _conv_args(name, x, shape, weight, bias, x0, activation):
@@ -1082,8 +1086,7 @@ def causal_conv_fwd(x, weight, bias=None, x0=None, starts=None, activation="silu
     x, starts = _sequence(x), _starts_tensor(starts, x)
     weight, bias = _flat(weight), _flat(bias)
     x0 = None if x0 is None else _dense_any(x0)
-    y = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
-    last = torch.empty(B, width - 1, D, dtype=x.dtype, device=x.device)
+    y, last = _dense_like(x), x.new_empty((B, width - 1, D))
     N.check(N.load().oxc_causal_conv_fwd(
         x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), _ptr(bias), _ptr(x0),
         _ptr(starts), y.data_ptr(), last.data_ptr(), B, T, D, width, _ACTIVATIONS[activation], dt,
@@ -1108,9 +1111,7 @@ def _causal_conv_bwd(x, weight, bias, x0, dy, dlast, starts, activation):
     x0 = None if x0 is None else _dense_any(x0)
     dy = None if dy is None else _sequence(dy)
     dlast = None if dlast is None else _dense_any(dlast)
-    dx = torch.empty(B, T, D, dtype=x.dtype, device=dev)
-    dx0 = torch.empty(B, width - 1, D, dtype=x.dtype, device=dev)
-    dw = torch.empty(D * (width + 1), dtype=torch.float32, device=dev)
+    dx, dx0, dw = _dense_like(x), x.new_empty((B, width - 1, D)), weight.new_empty(D * (width + 1))
     L = N.load()
     ws = _workspace(L.oxc_causal_conv_bwd_workspace_size(B, T, D, width), dev)
     ysb, yst = (0, 0) if dy is None else dy.stride()[:2]
@@ -1173,7 +1174,7 @@ def causal_conv_step(x, weight, bias, state, out=None, activation="silu"):
     if _recorded(x, weight, bias, state):
         raise ValueError("invalid argument: causal_conv_step has no gradient; train with causal_conv")
     x, weight, bias = _lines(x), _flat(weight), _flat(bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _dense_like(x)
     N.check(N.load().oxc_causal_conv_step(
         x.data_ptr(), x.stride(0), weight.data_ptr(), _ptr(bias), state.data_ptr(), out.data_ptr(),
         y.data_ptr(), x.shape[0], x.shape[1], width, _ACTIVATIONS[activation], dt, _stream()),
@@ -1227,12 +1228,8 @@ def selective_scan_fwd(x, delta, A, B, C, D=None, z=None, delta_bias=None, h0=No
     z = None if z is None else _sequence(z)
     A, D, delta_bias, h0 = _flat(A), _flat(D), _flat(delta_bias), _flat(h0)
     L = N.load()
-    y = torch.empty(batch, length, dim, dtype=x.dtype, device=x.device)
-    last = torch.empty(batch, dim, n, dtype=torch.float32, device=x.device)
-    carry = None
-    if save:
-        carry = torch.empty(L.oxc_selective_scan_carry_size(batch, length, dim, n), dtype=torch.float32,
-                            device=x.device)
+    y, last = _dense_like(x), A.new_empty((batch, dim, n))
+    carry = A.new_empty(L.oxc_selective_scan_carry_size(batch, length, dim, n)) if save else None
     ws, at, nbytes = _scratch(L.oxc_selective_scan_workspace_size(batch, length, dim, n, 0), x.device)
     zsb, zst = (0, 0) if z is None else z.stride()[:2]
     N.check(L.oxc_selective_scan_fwd(
@@ -1267,13 +1264,9 @@ def _selective_scan_bwd(x, delta, A, B, C, carry, D, z, delta_bias, starts, dy, 
     z = None if z is None else _sequence(z)
     dy = None if dy is None else _sequence(dy)
     A, D, delta_bias, dlast = _flat(A), _flat(D), _flat(delta_bias), _flat(dlast)
-    wide = (batch, length, dim)
-    dx, ddelta = torch.empty(wide, dtype=x.dtype, device=dev), torch.empty(wide, dtype=x.dtype, device=dev)
-    dB = torch.empty(batch, length, n, dtype=x.dtype, device=dev)
-    dC = torch.empty(batch, length, n, dtype=x.dtype, device=dev)
-    dz = None if z is None else torch.empty(wide, dtype=x.dtype, device=dev)
-    sums = torch.empty(dim * (n + 2), dtype=torch.float32, device=dev)
-    dh0 = torch.empty(batch, dim, n, dtype=torch.float32, device=dev)
+    dx, ddelta, dz = _dense_like(x), _dense_like(x), None if z is None else _dense_like(x)
+    dB, dC = _dense_like(B), _dense_like(B)
+    sums, dh0 = A.new_empty(dim * (n + 2)), A.new_empty((batch, dim, n))
     L = N.load()
     ws = _workspace(L.oxc_selective_scan_workspace_size(batch, length, dim, n, 1), dev)
     zsb, zst = (0, 0) if z is None else z.stride()[:2]
@@ -1345,7 +1338,7 @@ def selective_step(x, delta, A, B, C, state, D=None, z=None, delta_bias=None, ou
     x, delta, B, C = _lines(x), _lines(delta), _lines(B), _lines(C)
     z = None if z is None else _lines(z)
     A, D, delta_bias = _flat(A), _flat(D), _flat(delta_bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _dense_like(x)
     N.check(N.load().oxc_selective_step(
         x.data_ptr(), x.stride(0), delta.data_ptr(), delta.stride(0), A.data_ptr(), B.data_ptr(),
         B.stride(0), C.data_ptr(), C.stride(0), _ptr(D), _ptr(z), 0 if z is None else z.stride(0),
@@ -1389,10 +1382,8 @@ def policy_loss_fwd(logits, tokens, old_logp, advantages, ref_logp=None, clip=0.
         _flag(flag, dev)
     x, old, adv, ref = _rows2d(logits), dense(old_logp), dense(advantages), _flat(ref_logp)
     rows, vocab = x.shape
-    loss = torch.empty(1, dtype=torch.float32, device=dev)
-    logp = torch.empty(lead, dtype=torch.float32, device=dev)
-    row_loss = torch.empty(rows, dtype=torch.float32, device=dev)
-    dlogits = torch.empty(logits.shape, dtype=x.dtype, device=dev) if grad else None
+    loss, logp, row_loss = old.new_empty(1), _dense_like(old), old.new_empty(rows)
+    dlogits = _dense_like(logits) if grad else None
     N.check(N.load().oxc_policy_loss(
         x.data_ptr(), x.stride(0), tok.data_ptr(), old.data_ptr(), adv.data_ptr(), _ptr(ref),
         float(below), float(above), float(kl_coef), float(temperature), _ptr(grad_loss),
