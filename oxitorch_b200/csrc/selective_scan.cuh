@@ -506,7 +506,9 @@ __device__ __forceinline__ void load_decay(float2 (&A2)[L::CPT][L::P], const Pla
   }
 }
 
-// Takes a state from one end of segment `seg` to the other.
+// Takes a state from one end of segment `seg` to the other.  Where rates above zero take
+// the decay beyond f32, the state may still be small or zero: two factors of half the
+// time, and a zero stays one.
 template <class L, typename T>
 __device__ __forceinline__ void through_segment(float2 (&h)[L::CPT][L::P], const float2 (&A2)[L::CPT][L::P],
                                                 const Place<L>& at, const SelectiveArgs<T>& a, int64_t b,
@@ -522,8 +524,10 @@ __device__ __forceinline__ void through_segment(float2 (&h)[L::CPT][L::P], const
 #pragma unroll
     for (int i = 0; i < L::P; ++i) {
       const float2 own = make_float2(2 * i < there ? q[2 * i] : 0.0f, 2 * i + 1 < there ? q[2 * i + 1] : 0.0f);
-      const float2 e = exp2_pair(__fmul2_rn(A2[c][i], both(time)));
-      h[c][i] = time < 0.0f ? own : __ffma2_rn(e, h[c][i], own);
+      const float2 e = exp2_pair(__fmul2_rn(A2[c][i], both(0.5f * time)));
+      const float2 to = __ffma2_rn(e, __fmul2_rn(e, h[c][i]), own);
+      h[c][i].x = time < 0.0f || h[c][i].x == 0.0f ? own.x : to.x;
+      h[c][i].y = time < 0.0f || h[c][i].y == 0.0f ? own.y : to.y;
     }
   }
 }

@@ -293,6 +293,46 @@ def test_selective_scan_extremes(dtype):
     np.testing.assert_allclose(_n(last), ref.last, rtol=1e-4, atol=1e-4)
 
 
+def test_selective_scan_grows_over_segments():
+    """With rates above zero the decay of a segment is beyond f32 (exp(128) and exp(89)
+    here) where the states are not: zero before the last tokens and behind the first
+    ones, or tiny.  A step's factor is off by 2^-24 of an exponent of 3 a few times and by
+    ex2's 2^-22, over 64 steps by 2^-14."""
+    import torch
+    from oxitorch_b200 import functional as F
+    args, _, dy, _ = _scan_inputs(1, 4096, 8, 4, "float32", False)
+    args = {**args, "h0": None, "z": None, "delta_bias": None}
+    args["A"].fill_(2.0)
+    args["delta"].fill_(float(np.log(np.expm1(1.0))))  # steps of 1
+    args["x"][:, :-20] = 0.0
+    dy[:, 20:] = 0.0
+    leaves = [args[k].requires_grad_() for k in ("x", "delta", "A", "B", "C")]
+    y, last = F.selective_scan(**args)
+    got = torch.autograd.grad(y, leaves, dy)
+    assert not y[:, :-20].any() and torch.isfinite(y).all()
+    ref = R.Scan(**{k: None if t is None else _n(t.detach()) for k, t in args.items()})
+    _check(last, ref.last, ref.last_bound, "last")
+    back = torch.zeros(8, 4, device="cuda", dtype=torch.float64)  # lam_t for t from 19 to 0
+    want = torch.zeros(20, 8, device="cuda", dtype=torch.float64)
+    B, C = args["B"].detach()[0].double(), args["C"].detach()[0].double()
+    for t in range(19, -1, -1):
+        back = back * np.exp(2.0) + C[t] * dy[0, t].double()[:, None]
+        want[t] = back @ B[t] + args["D"].double() * dy[0, t].double()
+    scale = want.abs().max()
+    assert (got[0][0, :20] - want).abs().max() <= 2.0 ** -13 * scale and not got[0][:, 20:].any()
+    assert not any(g.any() for g in got[1:])
+
+    args = {k: None if t is None else t.detach()[:, :128].contiguous() if t.dim() == 3 else t.detach()
+            for k, t in args.items()}
+    args["x"].zero_()
+    args["A"].fill_(1.39)
+    args["delta"][:, 64:] = -200.0  # steps of 0
+    args["h0"] = torch.full((1, 8, 4), 1e-37, device="cuda")
+    y, last = F.selective_scan(**args)
+    want = float(np.float32(1e-37)) * np.exp(64 * float(np.float32(1.39)))
+    np.testing.assert_allclose(_n(last), np.full((1, 8, 4), want), rtol=2.0 ** -13)
+
+
 def test_selective_scan_nan_reaches_all_that_follows():
     import torch
     from oxitorch_b200 import functional as F
