@@ -69,6 +69,38 @@ def test_causal_conv_without_its_options(dtype):
     _conv_check(x.clone(), w.clone(), None, x0.clone(), starts, None, dlast)
 
 
+@pytest.mark.parametrize("D", [3052, 1510])
+def test_causal_conv_of_long_runs(D):
+    """As many tokens as fill the GPU with long runs a warp, against 64 bits on the device.
+    With m = |bias| + sum |w x|: u is off by 5 roundings of m, and SiLU and its derivative,
+    whose slopes are below 1.1 and 0.5, by 2^-21 more from ex2 and the reciprocal: 2^-20
+    (1 + m) together.  A weight's sum adds up to 256 terms of a run, then 20 partial sums."""
+    import torch
+    from oxitorch_b200 import functional as F
+    T, W = 24000, 4
+    g = torch.Generator(device="cuda").manual_seed(D)
+    x, dy = (torch.randn(1, T, D, device="cuda", generator=g) for _ in range(2))
+    w, bias = torch.randn(D, W, device="cuda", generator=g), torch.randn(D, device="cuda", generator=g)
+    y, _ = F.causal_conv_fwd(x, w, bias)
+    dx, dw, db, _ = F.causal_conv_bwd(x, w, bias, None, dy)
+    pad = torch.nn.functional.pad(x[0].double(), (0, 0, W - 1, 0))
+    wd, d = w.double(), dy[0].double()
+    u = bias.double() + sum(wd[:, k] * pad[k:k + T] for k in range(W))
+    m = bias.double().abs() + sum((wd[:, k] * pad[k:k + T]).abs() for k in range(W))
+    s = torch.sigmoid(u)
+    assert ((y[0] - u * s).abs() <= 2.0 ** -20 * (1 + m)).all()
+    du, mag = d * (s + u * s * (1 - s)), d.abs() * (1 + m)
+    later = lambda t: torch.nn.functional.pad(t, (0, 0, 0, W - 1))  # noqa: E731
+    dus, mags = later(du), later(mag)
+    want = sum(wd[:, W - 1 - k] * dus[k:k + T] for k in range(W))
+    size = sum((wd[:, W - 1 - k] * mags[k:k + T]).abs() for k in range(W))
+    assert ((dx[0] - want).abs() <= 2.0 ** -19 * size).all()
+    for k in range(W):
+        tap = pad[k:k + T]
+        assert ((dw[:, k] - (du * tap).sum(0)).abs() <= 2.0 ** -15 * (mag * tap.abs()).sum(0)).all()
+    assert ((db - du.sum(0)).abs() <= 2.0 ** -15 * mag.sum(0)).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("offset", [0, 1, 4])
 def test_causal_conv_reads_parts_of_a_projection(dtype, offset):
