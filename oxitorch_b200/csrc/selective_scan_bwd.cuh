@@ -204,6 +204,7 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
       if (i < count) {
         const int left = tokens(i), buffer = i & 1;
         raw.land(buffer, left);
+        if constexpr (!R::kAsync) raw.fetch(buffer ^ 1, tokens(i + 1));
 #pragma unroll 1
         for (int k = 0; k < R::kMine; ++k) {
           if (!raw.has) break;
@@ -289,7 +290,7 @@ selective_bwd_kernel(SelectiveArgs<T> a) {
         }
         out -= kTile * a.dim;
       }
-      raw.fetch((i + 1) & 1, tokens(i + 1));  // where the tile just stored was
+      if constexpr (R::kAsync) raw.fetch((i + 1) & 1, tokens(i + 1));  // where the tile just stored was
     }
     // dD and ddelta_bias over the threads with the same channels, where tile 0 or 1 was
     float* s = smem;

@@ -67,6 +67,7 @@ selective_fwd_kernel(SelectiveArgs<T> a) {
       if (i < count) {
         const int left = tokens(i);
         raw.land(buffer, left);
+        if constexpr (!R::kAsync) raw.fetch(next, tokens(i + 1));
 #pragma unroll
         for (int k = 0; k < R::kMine; ++k) {
           if (!raw.has) break;
@@ -126,7 +127,7 @@ selective_fwd_kernel(SelectiveArgs<T> a) {
           out += kTile * a.dim;
         }
       }
-      raw.fetch(next, tokens(i + kAhead));  // where the tile just stored was
+      if constexpr (R::kAsync) raw.fetch(next, tokens(i + kAhead));  // where the tile just stored was
       before = buffer;
       buffer = buffer + 1 == R::kDepth ? 0 : buffer + 1;
       next = next + 1 == R::kDepth ? 0 : next + 1;
