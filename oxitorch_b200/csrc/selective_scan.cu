@@ -3,7 +3,8 @@
 
 namespace oxc {
 
-// One token: LPC lanes a channel, four states a lane at a time.
+// One token: LPC lanes a channel, four states a lane at a time.  Rates are bounded as the
+// scan bounds them, so that an infinite one times a step of zero is zero here too.
 template <typename T, int LPC>
 __global__ void __launch_bounds__(128)
 selective_step_kernel(const T* __restrict__ x, int64_t x_sb, const T* __restrict__ delta,
@@ -33,15 +34,15 @@ selective_step_kernel(const T* __restrict__ x, int64_t x_sb, const T* __restrict
         bv[k] = to_f32(Bb[s + k]);
         cv[k] = to_f32(Cb[s + k]);
       }
-      h.x = fmaf(ex2(dt * (r.x * kLog2e)), h.x, dtx * bv[0]);
-      h.y = fmaf(ex2(dt * (r.y * kLog2e)), h.y, dtx * bv[1]);
-      h.z = fmaf(ex2(dt * (r.z * kLog2e)), h.z, dtx * bv[2]);
-      h.w = fmaf(ex2(dt * (r.w * kLog2e)), h.w, dtx * bv[3]);
+      h.x = fmaf(ex2(dt * bounded(r.x * kLog2e)), h.x, dtx * bv[0]);
+      h.y = fmaf(ex2(dt * bounded(r.y * kLog2e)), h.y, dtx * bv[1]);
+      h.z = fmaf(ex2(dt * bounded(r.z * kLog2e)), h.z, dtx * bv[2]);
+      h.w = fmaf(ex2(dt * bounded(r.w * kLog2e)), h.w, dtx * bv[3]);
       sum = fmaf(cv[0], h.x, fmaf(cv[1], h.y, fmaf(cv[2], h.z, fmaf(cv[3], h.w, sum))));
       *reinterpret_cast<float4*>(out + o) = h;
     } else {
       for (int k = 0; k < 4 && s + k < N; ++k) {
-        const float h = fmaf(ex2(dt * (A[d * N + s + k] * kLog2e)), state[o + k],
+        const float h = fmaf(ex2(dt * bounded(A[d * N + s + k] * kLog2e)), state[o + k],
                              dtx * to_f32(Bb[s + k]));
         sum = fmaf(to_f32(Cb[s + k]), h, sum);
         out[o + k] = h;

@@ -491,6 +491,8 @@ struct Starts {
   }
 };
 
+// A rate (times log2(e)): an infinite one times a step of zero, as of a padded token, is
+// then zero too.
 __device__ __forceinline__ float bounded(float v) { return v < -1e30f ? -1e30f : v > 1e30f ? 1e30f : v; }
 
 template <class L, typename T>
@@ -501,7 +503,6 @@ __device__ __forceinline__ void load_decay(float2 (&A2)[L::CPT][L::P], const Pla
     at.load(A2[c], a.A, c, 0, a.dim, a.N);
 #pragma unroll
     for (int i = 0; i < L::P; ++i) {
-      // an infinite rate times a step of zero, as of a padded token, is zero too
       A2[c][i].x = bounded(A2[c][i].x * kLog2e);
       A2[c][i].y = bounded(A2[c][i].y * kLog2e);
     }
