@@ -67,6 +67,7 @@ typedef struct oxc_view {
 #define OXC_ACT_GELU_TANH 1 /* python/oxitorch/nn/functional.py:194-199 */
 
 /* ---- library ---------------------------------------------------------- */
+/* 2: oxc_policy_loss takes clip_below, clip_above, kl_coef and temperature as doubles. */
 int32_t oxc_abi_version(void);
 /* Message of the last failing call on this thread ("" if none). */
 const char* oxc_last_error(void);
@@ -792,19 +793,19 @@ oxc_status oxc_selective_step(const void* x, int64_t x_sb, const void* delta, in
 /* Clipped policy loss of sampled tokens: with logp the token's log-probability in
  * softmax(logits / temperature) and r = exp(logp - old_logp), loss[0] = 1 / total_rows *
  * sum_rows -min(r A, clamp(r, 1 - clip_below, 1 + clip_above) A) + kl_coef *
- * (exp(ref_logp - logp) - (ref_logp - logp) - 1), A the row's advantage, and (unless
- * dlogits is NULL) dlogits = grad_loss[0] * d loss / d logits, dense, in the same
- * pass; grad_loss NULL = 1.  logp [rows] is written too.  A row with a negative token
+ * (exp(ref_logp - logp) - (ref_logp - logp) - 1), A the row's advantage (next to
+ * where it is clipped, r is taken in f64), and (unless dlogits is NULL) dlogits =
+ * grad_loss[0] * d loss / d logits, dense, in the same pass; grad_loss NULL = 1.  logp [rows] is written too.  A row with a negative token
  * is padding: loss, gradient and logp 0.  A token >= vocab is recorded in err_flag
  * (int32[4], may be NULL) and makes them NaN.  ref_logp may be NULL where kl_coef is
  * 0.  loss NULL: only logp is computed (advantages, old_logp, row_loss are not used,
  * dlogits is NULL).  row_loss: `rows` floats of scratch. */
 oxc_status oxc_policy_loss(const void* logits, int64_t logits_stride, const int64_t* tokens,
                            const float* old_logp, const float* advantages, const float* ref_logp,
-                           float clip_below, float clip_above, float kl_coef, float temperature,
-                           const float* grad_loss, float* loss, float* logp, float* row_loss,
-                           void* dlogits, int64_t rows, int64_t vocab, int64_t total_rows,
-                           int32_t dtype, int32_t* err_flag, void* stream);
+                           double clip_below, double clip_above, double kl_coef,
+                           double temperature, const float* grad_loss, float* loss, float* logp,
+                           float* row_loss, void* dlogits, int64_t rows, int64_t vocab,
+                           int64_t total_rows, int32_t dtype, int32_t* err_flag, void* stream);
 
 /* The norm over `count` dense tensors (addresses, element counts and dtypes in host
  * arrays), summed in f64, into norm[0] on the device; and the clipping by it: out[i] =

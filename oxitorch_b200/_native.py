@@ -98,7 +98,7 @@ class PlaneMap(ctypes.Structure):
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
-_F32 = ctypes.c_float
+_F32, _F64 = ctypes.c_float, ctypes.c_double
 _SZ = ctypes.c_size_t
 _VP = ctypes.POINTER(View)
 _U32 = ctypes.c_uint32
@@ -236,11 +236,11 @@ SIGNATURES = {
                                       _P]),
     "oxc_selective_step": (_I32, [_P, _I64, _P, _I64, _P, _P, _I64, _P, _I64, _P, _P, _I64, _P, _P,
                                   _P, _P, _I64, _I64, _I64, _I32, _P]),
-    "oxc_policy_loss": (_I32, [_P, _I64, _P, _P, _P, _P, _F32, _F32, _F32, _F32, _P, _P, _P, _P, _P,
+    "oxc_policy_loss": (_I32, [_P, _I64, _P, _P, _P, _P, _F64, _F64, _F64, _F64, _P, _P, _P, _P, _P,
                                _I64, _I64, _I64, _I32, _P, _P]),
     "oxc_clip_global_norm_workspace_size": (_SZ, [_I64]),
     "oxc_global_norm": (_I32, [_P, _P, _P, _I64, _P, _P, _SZ, _P]),
-    "oxc_clip_global_norm": (_I32, [_P, _P, _P, _P, _I64, ctypes.c_double, _P, _P, _SZ, _P]),
+    "oxc_clip_global_norm": (_I32, [_P, _P, _P, _P, _I64, _F64, _P, _P, _SZ, _P]),
 }
 
 NOALLOC_SCRATCH_BYTES = 16 * 1024 * 1024

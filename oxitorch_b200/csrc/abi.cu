@@ -131,7 +131,7 @@ static int32_t lookup(const char* const (&table)[N], const char* name) {
 
 extern "C" {
 
-int32_t oxc_abi_version(void) { return 1; }
+int32_t oxc_abi_version(void) { return 2; }
 
 const char* oxc_last_error(void) { return g_last_error; }
 

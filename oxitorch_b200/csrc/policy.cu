@@ -36,7 +36,8 @@ constexpr int kPolicyCluster = 8;              // CTAs per row at most
 struct PolicyArgs {
   const int64_t* tokens;
   const float *old_logp, *adv, *ref_logp;  // adv NULL: only logp is asked for
-  float low, high;    // 1 - below, 1 + above
+  float low, high, log_low, log_high;  // 1 - below, 1 + above and their logarithms
+  double low64, high64, inv_tau64;     // as they were given
   float kl;
   float inv_tau, c;   // c = log2(e) / tau
   float grad_scale;   // 1 / (total_rows tau)
@@ -67,21 +68,41 @@ struct PolicyTerm {
   float logp, loss, by;  // by = d loss / d logp
 };
 
+// exp(logp - old) in 64 bits.  Not inlined, as few rows need it: the registers of log and
+// exp would be those of every row.
+__device__ __noinline__ double policy_ratio(float logit, float2 row, float old, double inv_tau) {
+  return exp(((double)logit - (double)row.x) * inv_tau - log((double)row.y) - (double)old);
+}
+
 // From the token's logit and the row's (max, sum of exponentials).  Comparisons are
 // written so that a NaN reaches both the loss and the gradient.
+// In 32 bits the ratio's logarithm is off by up to 2^-24 (5 |logp| + |old| + 4): three
+// roundings of the scaled logit, logf's, and those of the two differences.  Whether the
+// row is clipped, and so whether it has a gradient, may hang on less: a ratio that lies
+// so near to an edge is taken in 64 bits.  (Log-probability and ratio of every row in 64
+// bits: f32 [8192, 32000] 361 us for 342, in sums of two floats 359; the row waits for it.)
 __device__ __forceinline__ PolicyTerm policy_term(const PolicyArgs& a, const Sample& s, float logit,
                                                   float2 row) {
   PolicyTerm t;
   t.logp = (logit - row.x) * a.inv_tau - logf(row.y);
   t.loss = t.by = 0.0f;
   if (!a.adv) return t;
-  const float r = expf(t.logp - s.old);
-  const float held = (r < a.low ? a.low : r > a.high ? a.high : r) * s.adv, free = r * s.adv;
-  t.loss = free > held ? -held : -free;
-  t.by = free > held ? 0.0f : -free;
+  const float gap = t.logp - s.old;
+  const float near = 0x1p-21f * (1.0f + fabsf(t.logp) + fabsf(s.old)), r = expf(gap);
+  float held = (r < a.low ? a.low : r > a.high ? a.high : r) * s.adv, free = r * s.adv;
+  bool clipped = free > held;
+  if (fabsf(gap - a.log_low) < near || fabsf(gap - a.log_high) < near) {
+    const double q = policy_ratio(logit, row, s.old, a.inv_tau64), f = q * (double)s.adv;
+    const double h = (q < a.low64 ? a.low64 : q > a.high64 ? a.high64 : q) * (double)s.adv;
+    clipped = f > h;
+    free = (float)f;
+    held = (float)h;
+  }
+  t.loss = clipped ? -held : -free;
+  t.by = clipped ? 0.0f : -free;
   if (a.ref_logp) {
-    const float gap = s.ref - t.logp, e = expm1f(gap);
-    t.loss = fmaf(a.kl, e - gap, t.loss);
+    const float to_ref = s.ref - t.logp, e = expm1f(to_ref);
+    t.loss = fmaf(a.kl, e - to_ref, t.loss);
     t.by = fmaf(-a.kl, e, t.by);
   }
   return t;
@@ -93,9 +114,10 @@ __device__ __forceinline__ PolicyTerm policy_term(const PolicyArgs& a, const Sam
 // next row's part are started, whose bytes L2 was asked for when the second pass began.
 // Every thread works out the row's term by itself.
 // (With registers for four CTAs of 256 threads an SM, not fewer: 334 us against 353 at f32
-// [8192, 32000].  Those of 128 threads lose by it: 134 us against 122 at bf16 [16384, 8000].)
+// [8192, 32000].  Those of 128 threads lose by it: 134 us against 122 at bf16 [16384, 8000];
+// there with registers for seven 120, for six 125.)
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1)
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : sizeof(T) == 2 ? 7 : 1)
 policy_cluster_kernel(const T* __restrict__ logits, int64_t stride, T* __restrict__ dlogits,
                       PolicyArgs a) {
   namespace cg = cooperative_groups;
@@ -393,10 +415,10 @@ extern "C" {
 
 oxc_status oxc_policy_loss(const void* logits, int64_t logits_stride, const int64_t* tokens,
                            const float* old_logp, const float* advantages, const float* ref_logp,
-                           float clip_below, float clip_above, float kl_coef, float temperature,
-                           const float* grad_loss, float* loss, float* logp, float* row_loss,
-                           void* dlogits, int64_t rows, int64_t vocab, int64_t total_rows,
-                           int32_t dtype, int32_t* err_flag, void* stream) {
+                           double clip_below, double clip_above, double kl_coef,
+                           double temperature, const float* grad_loss, float* loss, float* logp,
+                           float* row_loss, void* dlogits, int64_t rows, int64_t vocab,
+                           int64_t total_rows, int32_t dtype, int32_t* err_flag, void* stream) {
   if (!known_dtype(dtype))
     return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: policy_loss: unknown dtype %d", dtype);
   if (rows < 0 || vocab < 0)
@@ -405,14 +427,14 @@ oxc_status oxc_policy_loss(const void* logits, int64_t logits_stride, const int6
     return fail(OXC_ERR_INVALID_ARGUMENT,
                 "invalid argument: policy_loss: total_rows %lld must cover the %lld local rows",
                 (long long)total_rows, (long long)rows);
-  if (!(temperature > 0.0f) || isinf(temperature))
+  const float c = (float)(1.4426950408889634 / temperature);  // log2(e) / tau
+  if (!(temperature > 0.0) || isinf((float)temperature) || isinf(c))
     return fail(OXC_ERR_INVALID_ARGUMENT,
-                "invalid argument: policy_loss: temperature must be positive, got %g",
-                (double)temperature);
-  if (!(clip_below >= 0.0f) || !(clip_above >= 0.0f) || !(kl_coef >= 0.0f) || isinf(kl_coef))
+                "invalid argument: policy_loss: temperature must be positive, got %g", temperature);
+  if (!(clip_below >= 0.0) || !(clip_above >= 0.0) || !(kl_coef >= 0.0) || isinf((float)kl_coef))
     return fail(OXC_ERR_INVALID_ARGUMENT,
                 "invalid argument: policy_loss: clip (%g, %g) and kl_coef %g must not be negative",
-                (double)clip_below, (double)clip_above, (double)kl_coef);
+                clip_below, clip_above, kl_coef);
   if (vocab > 0x7fffffff - 1024)  // a thread's int index steps past the last token
     return fail(OXC_ERR_NOT_IMPLEMENTED, "not implemented: policy_loss: rows wider than 2^31");
   if (rows > 0 && vocab == 0)
@@ -421,20 +443,24 @@ oxc_status oxc_policy_loss(const void* logits, int64_t logits_stride, const int6
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (rows > 0) {
     if (!logits || !tokens || !logp || (term && (!advantages || !old_logp || !row_loss)) ||
-        (!term && dlogits) || (term && kl_coef > 0.0f && !ref_logp))
+        (!term && dlogits) || (term && kl_coef > 0.0 && !ref_logp))
       return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: policy_loss: null pointer");
-    const double tau = (double)temperature;
     PolicyArgs a{};
     a.tokens = tokens;
     a.old_logp = old_logp;
     a.adv = term ? advantages : nullptr;
-    a.ref_logp = kl_coef > 0.0f ? ref_logp : nullptr;
-    a.low = (float)(1.0 - (double)clip_below);
-    a.high = (float)(1.0 + (double)clip_above);
-    a.kl = kl_coef;
-    a.inv_tau = (float)(1.0 / tau);
-    a.c = (float)(1.4426950408889634 / tau);
-    a.grad_scale = (float)(1.0 / (tau * (double)total_rows));
+    a.ref_logp = kl_coef > 0.0 ? ref_logp : nullptr;
+    a.low = (float)(1.0 - clip_below);
+    a.high = (float)(1.0 + clip_above);
+    a.log_low = clip_below < 1.0 ? (float)log1p(-clip_below) : -INFINITY;
+    a.log_high = (float)log1p(clip_above);
+    a.low64 = 1.0 - clip_below;
+    a.high64 = 1.0 + clip_above;
+    a.kl = (float)kl_coef;
+    a.inv_tau = (float)(1.0 / temperature);
+    a.inv_tau64 = 1.0 / temperature;
+    a.c = c;
+    a.grad_scale = (float)(1.0 / (temperature * (double)total_rows));
     a.grad_loss = grad_loss;
     a.logp = logp;
     a.row_loss = term ? row_loss : nullptr;

@@ -1,5 +1,6 @@
 """The operators of a selective state space model where they can go wrong: rates
-without bound in a single step.  Error bounds come from tests/selective_reference.py."""
+without bound in a single step, and ratios next to where they are clipped.  Error
+bounds come from tests/selective_reference.py."""
 
 import numpy as np
 import pytest
@@ -38,3 +39,61 @@ def test_selective_step_keeps_its_state_beside_unbounded_rates(N, rate, dtype):
         y = F.selective_step(**at, A=args["A"], D=args["D"], delta_bias=args["delta_bias"], state=state)
         _check(y, want[:, t], bound[:, t], f"y {t}")
         _check(state, ref.h[:, t], ref.e[:, t], f"state {t}")
+
+
+# ---- policy_loss ---------------------------------------------------------------------
+
+def _edge_rows(vocab, far, tau, clip, seed):
+    """Rows of `vocab` logits, the first c of them 0 and the token's `far`, the others
+    -inf, whose sum of exponentials is c in f32 (exp(far / tau) is below 2^-40) and off by
+    less than 1e-12 in truth; old log-probabilities with which the ratio lies within 1e-6 of
+    where it is clipped, but no nearer than 2e-8, on either side."""
+    g = np.random.default_rng(seed)
+    rows = []
+    for c in g.permutation(np.arange(500, vocab)):
+        at = c - 1 if far == 0 else c
+        if at >= vocab:
+            continue
+        logp = far / tau - np.log(float(c))
+        for edge in (1 - clip[0], 1 + clip[1]):
+            old = np.float32(logp - np.log(edge))
+            for old in (old, np.nextafter(old, np.float32(0)), np.nextafter(old, np.float32(-1e9))):
+                off = np.exp(logp - np.float64(old)) / edge - 1
+                if 2e-8 < abs(off) < 1e-6:
+                    rows.append((c, at, old, logp, edge, off))
+        if len(rows) > 600:
+            break
+    return rows
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [2000, 20011])
+@pytest.mark.parametrize("far,tau,clip", [(0.0, 1.0, (0.2, 0.28)), (-30.0, 1.0, (0.2, 0.2)), (-30.0, 0.7, (0.2, 0.28)),
+                                          (-30.0, 0.9, (0.3, 0.1))])
+def test_policy_loss_ratios_next_to_where_they_are_clipped(far, tau, clip, vocab, dtype):
+    """Whether a row is clipped decides whether it has a gradient.  A log-probability of
+    -7 to -50 in f32 is off by 5e-7 to 4e-6, more than these ratios lie from the edge: the
+    side has to be the one that 64 bits say.  Rows of -inf beside 0 have an exact sum."""
+    import torch
+    from oxitorch_b200 import functional as F
+    rows = _edge_rows(vocab, far, tau, clip, vocab)
+    assert len(rows) > 300
+    c, at, old, logp, edge, off = (np.array(v) for v in zip(*rows))
+    assert (off > 0).any() and (off < 0).any() and len(set(edge)) == 2
+    n = len(rows)
+    x = torch.arange(vocab, device="cuda") < torch.from_numpy(c).cuda()[:, None]
+    x = torch.where(x, 0.0, -float("inf"))
+    x[torch.arange(n), torch.from_numpy(at).cuda()] = far
+    x = x.to(getattr(torch, dtype))
+    old_t = torch.from_numpy(old.astype(np.float32)).cuda()
+    tokens = torch.from_numpy(at).cuda()
+    for sign in (1.0, -1.0):
+        adv = torch.full((n,), sign, device="cuda")
+        _, got, d = F.policy_loss_fwd(x, tokens, old_t, adv, clip=clip, temperature=tau, total_rows=n)
+        # with z = (logit - max) / tau: the difference, 1 / tau and their product are off by
+        # 2^-24 |z| each, logf by 2^-23 of log c, the sum by 2^-24 |logp|; |logp| = |z| + log c
+        _check(got, logp, 2.0 ** -22 * np.abs(logp) + 1e-10, "logp")
+        r = np.exp(logp - old.astype(np.float64))
+        clipped = r > 1 + clip[1] if sign > 0 else r < 1 - clip[0]
+        have = d.float().abs().sum(1).cpu().numpy() > 0
+        assert np.array_equal(have, ~clipped), f"{(have == clipped).sum()} of {n} rows on the wrong side"
