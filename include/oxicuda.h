@@ -795,11 +795,12 @@ oxc_status oxc_selective_step(const void* x, int64_t x_sb, const void* delta, in
  * sum_rows -min(r A, clamp(r, 1 - clip_below, 1 + clip_above) A) + kl_coef *
  * (exp(ref_logp - logp) - (ref_logp - logp) - 1), A the row's advantage (next to
  * where it is clipped, r is taken in f64), and (unless dlogits is NULL) dlogits =
- * grad_loss[0] * d loss / d logits, dense, in the same pass; grad_loss NULL = 1.  logp [rows] is written too.  A row with a negative token
- * is padding: loss, gradient and logp 0.  A token >= vocab is recorded in err_flag
- * (int32[4], may be NULL) and makes them NaN.  ref_logp may be NULL where kl_coef is
- * 0.  loss NULL: only logp is computed (advantages, old_logp, row_loss are not used,
- * dlogits is NULL).  row_loss: `rows` floats of scratch. */
+ * grad_loss[0] * d loss / d logits, dense, in the same pass; grad_loss NULL = 1.
+ * logp [rows] is written too.  A row with a negative token is padding: loss, gradient
+ * and logp 0.  A token >= vocab is recorded in err_flag (int32[4], may be NULL) and
+ * makes them NaN.  ref_logp may be NULL where kl_coef is 0.  loss NULL: only logp is
+ * computed (advantages, old_logp, row_loss are not used, dlogits is NULL).  row_loss:
+ * `rows` floats of scratch. */
 oxc_status oxc_policy_loss(const void* logits, int64_t logits_stride, const int64_t* tokens,
                            const float* old_logp, const float* advantages, const float* ref_logp,
                            double clip_below, double clip_above, double kl_coef,
@@ -809,8 +810,8 @@ oxc_status oxc_policy_loss(const void* logits, int64_t logits_stride, const int6
 
 /* The norm over `count` dense tensors (addresses, element counts and dtypes in host
  * arrays), summed in f64, into norm[0] on the device; and the clipping by it: out[i] =
- * tensor i times max_norm / (norm + 1e-6) where that is below 1 (the tensor itself
- * where it is not, also when the norm is NaN).  out NULL: in place.  The tensors do
+ * tensor i times max_norm / (norm + 1e-6), of the f64 norm, where that is below 1 (the
+ * tensor itself where it is not, also when the norm is NaN).  out NULL: in place.  The tensors do
  * not overlap; out[i] is tensor i or overlaps none. */
 size_t oxc_clip_global_norm_workspace_size(int64_t count);
 oxc_status oxc_global_norm(const int64_t* tensors, const int64_t* sizes, const int32_t* dtypes,

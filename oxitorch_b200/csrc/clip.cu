@@ -116,16 +116,18 @@ __device__ __forceinline__ double total_squares(const double* sums, int n, doubl
   return block_sum(s, scratch);
 }
 
-template <typename T>
-__device__ __forceinline__ void chunk_scale(const T* p, T* out, int64_t n, float f) {
+// F: float, or double for factors that f32 does not hold.
+template <typename T, typename F>
+__device__ __forceinline__ void chunk_scale(const T* p, T* out, int64_t n, F f) {
   constexpr int kVec = 16 / sizeof(T), U = 4;
   int64_t i = threadIdx.x;
+  auto times = [f](float v) { return (float)((F)v * f); };
   auto scaled = [&](const uint4& q) {
     uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if constexpr (sizeof(T) == 4) w[k] = __float_as_uint(__uint_as_float(w[k]) * f);
-      else w[k] = pack_bf16(bf16_lo(w[k]) * f, bf16_hi(w[k]) * f);
+      if constexpr (sizeof(T) == 4) w[k] = __float_as_uint(times(__uint_as_float(w[k])));
+      else w[k] = pack_bf16(times(bf16_lo(w[k])), times(bf16_hi(w[k])));
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   };
@@ -143,7 +145,7 @@ __device__ __forceinline__ void chunk_scale(const T* p, T* out, int64_t n, float
     for (; i < nv; i += kClipThreads) __stcs(o + i, scaled(__ldcs(v + i)));
     i = nv * kVec + threadIdx.x;
   }
-  for (; i < n; i += kClipThreads) out[i] = from_f32<T>(to_f32(p[i]) * f);
+  for (; i < n; i += kClipThreads) out[i] = from_f32<T>(times(to_f32(p[i])));
 }
 
 template <int CAP>
@@ -157,6 +159,8 @@ clip_scale_kernel(const __grid_constant__ ClipList<CAP> list, const double* __re
   const double factor = max_norm / (norm + 1e-6);
   const bool scale = factor < 1.0;  // not with a NaN
   const float f = scale ? (float)factor : 1.0f;
+  // large gradients clipped to a small norm: in f32 such a factor has few bits or none
+  const bool tiny = factor > 0.0 && factor < 0x1p-126;
   const int chunks = list.first[list.count];
   for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= (int)gridDim.x) {
     const int i = list.find(c);
@@ -165,10 +169,14 @@ clip_scale_kernel(const __grid_constant__ ClipList<CAP> list, const double* __re
     const bool half = list.is_bf16(i);
     const int64_t each = kClipBytes / (half ? 2 : 4), from = (int64_t)(c - list.first[i]) * each;
     const int64_t n = min(each, t.n - from);
-    if (half)
-      chunk_scale(static_cast<const bf16*>(t.in) + from, static_cast<bf16*>(t.out) + from, n, f);
-    else
-      chunk_scale(static_cast<const float*>(t.in) + from, static_cast<float*>(t.out) + from, n, f);
+    auto by = [&](auto factor) {
+      if (half)
+        chunk_scale(static_cast<const bf16*>(t.in) + from, static_cast<bf16*>(t.out) + from, n, factor);
+      else
+        chunk_scale(static_cast<const float*>(t.in) + from, static_cast<float*>(t.out) + from, n, factor);
+    };
+    if (tiny) by(factor);
+    else by(f);
   }
 }
 

@@ -364,7 +364,8 @@ def clip_global_norm_(grads, max_norm, out=None):
     to 640 tensors: where max_norm / (norm + 1e-6) < 1, every gradient is scaled by it
     (in f32, rounded once), in place or into ``out``, a list of tensors of the same
     sizes and types.  Returns the norm before, a 0-d float32 tensor (NaN or infinite
-    if the gradients are; a NaN norm leaves them as they are).
+    if the gradients are; a NaN norm leaves them as they are).  The factor comes from the
+    norm in f64, also where that is beyond float32.
 
     Gradients are float32 or bfloat16, dense and apart from each other, any number of
     them; None is skipped (in ``out`` too).  A captured graph repeats the call on the same

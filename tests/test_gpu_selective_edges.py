@@ -1,13 +1,13 @@
 """The operators of a selective state space model where they can go wrong: rates
-without bound in a single step, and ratios next to where they are clipped.  Error
-bounds come from tests/selective_reference.py."""
+without bound in a single step, factors below the smallest normal f32, and ratios
+next to where they are clipped.  Error bounds come from tests/selective_reference.py."""
 
 import numpy as np
 import pytest
 
 import selective_reference as R
 from test_gpu_draft import DTYPES, _check, _n, _t
-from test_gpu_selective import _scan_inputs
+from test_gpu_selective import _clip_check, _gradients, _scan_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -39,6 +39,49 @@ def test_selective_step_keeps_its_state_beside_unbounded_rates(N, rate, dtype):
         y = F.selective_step(**at, A=args["A"], D=args["D"], delta_bias=args["delta_bias"], state=state)
         _check(y, want[:, t], bound[:, t], f"y {t}")
         _check(state, ref.h[:, t], ref.e[:, t], f"state {t}")
+
+
+# ---- clip_global_norm_ ---------------------------------------------------------------
+
+def test_global_norm_beyond_32_bits():
+    """Squares that f32 does not hold, a norm that it holds, and one that it does not."""
+    import torch
+    from oxitorch_b200 import tensor_ops as T
+    grads = _gradients([1000, 77], ["float32"], 1e37)
+    norm, _ = R.clip([_n(g) for g in grads], 1.0)
+    assert norm < 2.0 ** 128
+    got = T.global_norm(grads).item()
+    assert abs(got - norm) <= 2.0 ** -23 * norm  # finite, and the 64-bit value
+    assert torch.isinf(T.global_norm(grads * 2000))
+    assert torch.isfinite(T.global_norm([g.bfloat16() for g in grads]))
+
+
+@pytest.mark.parametrize("dtypes", [["float32"], ["bfloat16"], ["float32", "bfloat16"]])
+@pytest.mark.parametrize("max_norm", [1.0, 1e-3, 1e-6, 1e-20])
+def test_clip_global_norm_by_factors_below_the_smallest_normal(max_norm, dtypes):
+    """Gradients of 1e36 clipped to norms down to 1e-20: the factor, 6e-39 to 6e-59, is
+    one that f32 holds with few bits or not at all; the clipped values are ordinary."""
+    import torch
+    sizes = [1000, 77, 5, 4096, 20001]
+    _clip_check(_gradients(sizes, dtypes, 1e36), max_norm)
+    grads = _gradients(sizes, dtypes, 1e36)
+    _clip_check(grads, max_norm, out=[torch.full_like(g, float("nan")) for g in grads])
+    wide = torch.zeros(20010, device="cuda", dtype=grads[-1].dtype)
+    wide[3:20004] = grads[-1]
+    _clip_check([wide[3:20004]], max_norm)  # rows off their 16 bytes
+    assert not wide[:3].any() and not wide[20004:].any()
+
+
+def test_clip_global_norm_where_the_norm_is_beyond_32_bits():
+    """The norm returned is infinite, the factor is not zero: it comes from the 64-bit norm."""
+    import torch
+    from oxitorch_b200 import tensor_ops as T
+    grads = _gradients([4001] * 500, ["float32"], 1e37)
+    norm, want = R.clip([_n(g) for g in grads], 2.0)
+    assert norm > 2.0 ** 128
+    assert torch.isinf(T.clip_global_norm_(grads, 2.0))
+    for g, w in zip(grads, want):
+        _check(g, w, 2.0 ** -23 * np.abs(w), "clipped")
 
 
 # ---- policy_loss ---------------------------------------------------------------------
