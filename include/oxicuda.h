@@ -798,9 +798,10 @@ oxc_status oxc_selective_step(const void* x, int64_t x_sb, const void* delta, in
  * grad_loss[0] * d loss / d logits, dense, in the same pass; grad_loss NULL = 1.
  * logp [rows] is written too.  A row with a negative token is padding: loss, gradient
  * and logp 0.  A token >= vocab is recorded in err_flag (int32[4], may be NULL) and
- * makes them NaN.  ref_logp may be NULL where kl_coef is 0.  loss NULL: only logp is
- * computed (advantages, old_logp, row_loss are not used, dlogits is NULL).  row_loss:
- * `rows` floats of scratch. */
+ * makes them NaN.  total_rows: any number above 0, as of the rows of a sharded batch, or
+ * of those that are no padding.  ref_logp may be NULL where kl_coef is 0.  loss NULL:
+ * only logp is computed (advantages, old_logp, row_loss are not used, dlogits is NULL).
+ * row_loss: `rows` floats of scratch. */
 oxc_status oxc_policy_loss(const void* logits, int64_t logits_stride, const int64_t* tokens,
                            const float* old_logp, const float* advantages, const float* ref_logp,
                            double clip_below, double clip_above, double kl_coef,

@@ -423,10 +423,9 @@ oxc_status oxc_policy_loss(const void* logits, int64_t logits_stride, const int6
     return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: policy_loss: unknown dtype %d", dtype);
   if (rows < 0 || vocab < 0)
     return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: policy_loss: negative shape");
-  if (total_rows < rows || total_rows <= 0)
-    return fail(OXC_ERR_INVALID_ARGUMENT,
-                "invalid argument: policy_loss: total_rows %lld must cover the %lld local rows",
-                (long long)total_rows, (long long)rows);
+  if (total_rows <= 0)
+    return fail(OXC_ERR_INVALID_ARGUMENT, "invalid argument: policy_loss: total_rows %lld must be positive",
+                (long long)total_rows);
   const float c = (float)(1.4426950408889634 / temperature);  // log2(e) / tau
   if (!(temperature > 0.0) || isinf((float)temperature) || isinf(c))
     return fail(OXC_ERR_INVALID_ARGUMENT,

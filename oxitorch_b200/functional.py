@@ -1360,6 +1360,22 @@ def _sampled_tokens(name, logits, tokens):
     return dt, tokens
 
 
+def _mean_divisor(name, total_rows, tokens):
+    """The divisor of a mean over rows, of which those with a negative token do not count.
+    One below the number of rows is compared with the rows that count, for which the host
+    waits for the device; while a graph is captured their tokens are not there yet, and it
+    is taken as it is."""
+    rows = tokens.numel()
+    if total_rows is None:
+        return max(rows, 1)
+    total = int(total_rows)
+    if 0 < total < rows and not torch.cuda.is_current_stream_capturing():
+        count = int((tokens >= 0).sum())
+        if total < count:
+            raise ValueError(f"invalid argument: {name}: total_rows {total} must cover the {count} rows that count")
+    return total
+
+
 def policy_loss_fwd(logits, tokens, old_logp, advantages, ref_logp=None, clip=0.2, kl_coef=0.0,
                     temperature=1.0, total_rows=None, grad=True, grad_loss=None, flag=None):
     """Returns (loss[1], logp, dlogits): the gradient (times grad_loss[0] if given)
@@ -1381,14 +1397,15 @@ def policy_loss_fwd(logits, tokens, old_logp, advantages, ref_logp=None, clip=0.
     if flag is not None:
         _flag(flag, dev)
     x, old, adv, ref = _rows2d(logits), dense(old_logp), dense(advantages), _flat(ref_logp)
-    rows, vocab = x.shape
+    rows, vocab = tok.numel(), logits.shape[-1]
+    total = _mean_divisor("policy_loss", total_rows, tok)
     loss, logp, row_loss = old.new_empty(1), _dense_like(old), old.new_empty(rows)
     dlogits = _dense_like(logits) if grad else None
     N.check(N.load().oxc_policy_loss(
         x.data_ptr(), x.stride(0), tok.data_ptr(), old.data_ptr(), adv.data_ptr(), _ptr(ref),
         float(below), float(above), float(kl_coef), float(temperature), _ptr(grad_loss),
-        loss.data_ptr(), logp.data_ptr(), row_loss.data_ptr(), _ptr(dlogits), rows, vocab,
-        int(total_rows or rows), dt, _ptr(flag), _stream()), "policy_loss")
+        loss.data_ptr(), logp.data_ptr(), row_loss.data_ptr(), _ptr(dlogits), rows, vocab, total, dt,
+        _ptr(flag), _stream()), "policy_loss")
     return loss, logp, dlogits
 
 
@@ -1436,7 +1453,9 @@ def policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, clip=0.2, k
     one number, or (below, above).  A row with a negative token (padding) adds 0 to the
     mean and has a zero gradient and logp; a token >= vocab makes the loss NaN.
     total_rows: the divisor of the mean (the rows of this call if None), as in a sharded
-    batch or where only unpadded tokens count.  In bfloat16 the gradient is rounded for
+    batch, or, where only unpadded tokens count, their number: one below the rows of the
+    call has to cover those that are no padding, and the host waits for the tokens to see
+    that it does (not while a graph is captured).  In bfloat16 the gradient is rounded for
     a factor of 1 on the loss and again when another one scales it."""
     if isinstance(logits, torch.Tensor) and _recorded(logits):
         for name, t in (("old_logp", old_logp), ("advantages", advantages), ("ref_logp", ref_logp)):

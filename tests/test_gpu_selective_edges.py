@@ -1,13 +1,14 @@
 """The operators of a selective state space model where they can go wrong: rates
-without bound in a single step, factors below the smallest normal f32, and ratios
-next to where they are clipped.  Error bounds come from tests/selective_reference.py."""
+without bound in a single step, factors below the smallest normal f32, ratios next to
+where they are clipped, and divisors of the policy loss.  Error bounds come from
+tests/selective_reference.py."""
 
 import numpy as np
 import pytest
 
 import selective_reference as R
 from test_gpu_draft import DTYPES, _check, _n, _t
-from test_gpu_selective import _clip_check, _gradients, _scan_inputs
+from test_gpu_selective import _clip_check, _gradients, _policy_check, _policy_inputs, _scan_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +141,73 @@ def test_policy_loss_ratios_next_to_where_they_are_clipped(far, tau, clip, vocab
         clipped = r > 1 + clip[1] if sign > 0 else r < 1 - clip[0]
         have = d.float().abs().sum(1).cpu().numpy() > 0
         assert np.array_equal(have, ~clipped), f"{(have == clipped).sum()} of {n} rows on the wrong side"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,vocab", [(64, 1003), (7, 32001), (5, 330001)])
+def test_policy_loss_mean_over_the_tokens_that_count(n, vocab, dtype):
+    """total_rows as the number of rows that are no padding: below the rows of the call."""
+    if vocab == 330001 and dtype == "bfloat16":
+        vocab = 660001  # beyond what a cluster holds
+    logits, tokens, old, ref, adv = _policy_inputs(n, vocab, dtype)
+    tokens[::3] = -1
+    count = int((tokens >= 0).sum())
+    assert 0 < count < n
+    _policy_check(logits, tokens, old, adv, ref, kl=0.1, total=count)
+    _policy_check(logits, tokens, old, adv, total=count)
+    _policy_check(logits, tokens, old, adv, ref, kl=0.1, tau=0.7, total=count + 1)
+
+
+def test_policy_loss_mean_over_the_tokens_that_count_twice_backward_and_captured():
+    """The gradient computed again has the same divisor; a captured call takes it as given."""
+    import torch
+    from oxitorch_b200 import functional as F
+    logits, tokens, old, ref, adv = _policy_inputs(40, 1003, "float32")
+    tokens[::4] = -1
+    count = int((tokens >= 0).sum())
+    dev = lambda a: torch.from_numpy(np.asarray(a)).cuda()  # noqa: E731
+    x, rest = logits.requires_grad_(), [dev(v) for v in (tokens, old, adv, ref)]
+    loss, _ = F.policy_loss(x, *rest, kl_coef=0.1, total_rows=count)
+    a, = torch.autograd.grad(loss, x, retain_graph=True)
+    b, = torch.autograd.grad(loss, x)
+    assert torch.equal(a, b)
+    x = x.detach()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        F.policy_loss_fwd(x, *rest, kl_coef=0.1, total_rows=count)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got, _, d = F.policy_loss_fwd(x, *rest, kl_coef=0.1, total_rows=count)
+    torch.cuda.current_stream().wait_stream(side)
+    graph.replay()
+    assert torch.equal(got.reshape(()), loss.detach()) and torch.equal(d, a)
+
+
+def test_policy_loss_divisors():
+    """No rows with the default divisor, a batch of padding alone, and the divisors that
+    are refused: 0, negative ones, and fewer than the tokens that count."""
+    import torch
+    from oxitorch_b200 import functional as F
+    x = torch.zeros(0, 5, device="cuda", requires_grad=True)
+    none, no = torch.zeros(0, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda")
+    loss, logp = F.policy_loss(x, no, none, none)
+    assert loss == 0 and logp.shape == (0,)
+    assert torch.autograd.grad(loss, x)[0].shape == (0, 5)
+    assert F.policy_loss(x.detach(), no, none, none)[0] == 0
+    x, v = torch.randn(4, 5, device="cuda"), torch.ones(4, device="cuda")
+    pad = torch.full((4,), -1, device="cuda")
+    loss, _, d = F.policy_loss_fwd(x, pad, v, v, total_rows=1)
+    assert loss == 0 and not d.any()
+    tokens = torch.tensor([1, -1, 3, 0], device="cuda")
+    F.policy_loss(x, tokens, -v, v, total_rows=3)
+    for args in ((x, tokens), (x[:0], tokens[:0])):
+        n = len(args[0])
+        for bad in (0, -1, -3):
+            with pytest.raises(ValueError):
+                F.policy_loss(*args, v[:n], v[:n], total_rows=bad)
+    for total in (2, 1):
+        with pytest.raises(ValueError, match="total_rows"):
+            F.policy_loss(x, tokens, v, v, total_rows=total)
+        with pytest.raises(ValueError, match="total_rows"):
+            F.policy_loss(x.clone().requires_grad_(), tokens, v, v, total_rows=total)
