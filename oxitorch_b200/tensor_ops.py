@@ -19,9 +19,10 @@ from array import array
 from operator import attrgetter
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
-from .functional import _DTYPES, _dtype_id, _require_cuda_f32, _stream, _workspace, dense
+from .functional import _DTYPES, _dtype_id, _has_tangent, _require_cuda_f32, _stream, _workspace, dense
 
 BINARY_OPS = ["add", "sub", "mul", "div", "pow", "min", "max"]
 CMP_OPS = ["eq", "ne", "lt", "le", "gt", "ge"]
@@ -332,6 +333,12 @@ def _listed(tensors):
     return [t for t in tensors if t is not None] if type(None) in set(map(type, tensors)) else tensors
 
 
+def _any_recorded(tensors):
+    """_recorded, by the whole list."""
+    return (torch.is_grad_enabled() and any(map(_requires_grad, tensors))) or (
+        forward_ad._current_level >= 0 and _has_tangent(*tensors))
+
+
 def _permuted_dense(t):
     """Whether t's elements fill a range of memory in some order of its dims."""
     n = 1
@@ -345,9 +352,12 @@ def _permuted_dense(t):
 def global_norm(tensors):
     """sqrt of the sum over all tensors of sum(v * v), summed in f64, as a 0-d float32
     tensor: the host does not wait for it.  Tensors are float32 or bfloat16, dense, any
-    number of them; None is skipped."""
+    number of them; None is skipped.  It has no gradient: parameters are measured under
+    torch.no_grad or detached."""
     tensors = _listed(tensors)
     ptrs, sizes, dtypes, _ = _flat_operands("tensors", tensors)
+    if _any_recorded(tensors):
+        raise ValueError("invalid argument: global_norm has no gradient; detach its tensors")
     if not tensors:
         return torch.zeros((), device="cuda")
     L = N.load()
@@ -393,8 +403,8 @@ def clip_global_norm_(grads, max_norm, out=None):
                         not (g.is_contiguous() and o.is_contiguous()) and (g.shape, g.stride()) != (o.shape, o.stride())):
                     raise ValueError(f"shape mismatch: an output {list(o.shape)} {o.dtype} for a gradient "
                                      f"{list(g.shape)} {g.dtype}, or laid out otherwise")
-    if any(map(_requires_grad, grads if out is None else out)):
-        raise ValueError("invalid argument: clip_global_norm_ writes to tensors outside any graph")
+    if any(map(_requires_grad, grads if out is None else out)) or _any_recorded(grads):
+        raise ValueError("invalid argument: clip_global_norm_ has no gradient and writes to tensors outside any graph")
     L = N.load()
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
     ws = _workspace(L.oxc_clip_global_norm_workspace_size(len(grads)), norm.device)

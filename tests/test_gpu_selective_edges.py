@@ -1,7 +1,7 @@
 """The operators of a selective state space model where they can go wrong: rates
 without bound in a single step, factors below the smallest normal f32, ratios next to
-where they are clipped, and divisors of the policy loss.  Error bounds come from
-tests/selective_reference.py."""
+where they are clipped, divisors of the policy loss, and derivatives that there are
+none of.  Error bounds come from tests/selective_reference.py."""
 
 import numpy as np
 import pytest
@@ -83,6 +83,29 @@ def test_clip_global_norm_where_the_norm_is_beyond_32_bits():
     assert torch.isinf(T.clip_global_norm_(grads, 2.0))
     for g, w in zip(grads, want):
         _check(g, w, 2.0 ** -23 * np.abs(w), "clipped")
+
+
+def test_global_norm_refuses_what_it_has_no_gradient_for():
+    import torch
+    from torch.autograd import forward_ad
+    from oxitorch_b200 import tensor_ops as T
+    a, b = _gradients([12, 20], ["float32"])
+    want = T.global_norm([a, b])
+    for bad in ([a.clone().requires_grad_(), b], [b, a.clone().requires_grad_() * 2], [torch.nn.Parameter(a.clone())]):
+        with pytest.raises(ValueError, match="gradient"):
+            T.global_norm(bad)
+        with torch.no_grad():
+            T.global_norm(bad)
+    assert torch.equal(T.global_norm([a, None, torch.nn.Parameter(b, requires_grad=False)]), want)
+    for bad in ([a.clone().requires_grad_(), b], [b, a.clone().requires_grad_() * 2]):
+        with pytest.raises(ValueError, match="gradient"):  # also beside an output of its own
+            T.clip_global_norm_(bad, 1.0, out=[torch.empty_like(g) for g in bad])
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(a, torch.ones_like(a))
+        for call in (T.global_norm, lambda g: T.clip_global_norm_(g, 1.0)):
+            with pytest.raises(ValueError, match="gradient"):
+                call([b, dual])
+        assert torch.equal(T.global_norm([a, b]), want)
 
 
 # ---- policy_loss ---------------------------------------------------------------------
