@@ -1457,10 +1457,11 @@ def policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, clip=0.2, k
     call has to cover those that are no padding, and the host waits for the tokens to see
     that it does (not while a graph is captured).  In bfloat16 the gradient is rounded for
     a factor of 1 on the loss and again when another one scales it."""
-    if isinstance(logits, torch.Tensor) and _recorded(logits):
+    if _recorded(old_logp, advantages, ref_logp):
         for name, t in (("old_logp", old_logp), ("advantages", advantages), ("ref_logp", ref_logp)):
-            if isinstance(t, torch.Tensor) and t.requires_grad:
+            if _recorded(t):
                 raise ValueError(f"invalid argument: {name} gets no gradient; detach it")
+    if _recorded(logits):
         return _PolicyLoss.apply(logits, tokens, old_logp, advantages, ref_logp, clip, kl_coef,
                                  temperature, total_rows)
     loss, logp, _ = policy_loss_fwd(logits, tokens, old_logp, advantages, ref_logp, clip, kl_coef,

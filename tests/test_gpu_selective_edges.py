@@ -234,3 +234,24 @@ def test_policy_loss_divisors():
             F.policy_loss(x, tokens, v, v, total_rows=total)
         with pytest.raises(ValueError, match="total_rows"):
             F.policy_loss(x.clone().requires_grad_(), tokens, v, v, total_rows=total)
+
+
+@pytest.mark.parametrize("name", ["old_logp", "advantages", "ref_logp"])
+def test_policy_loss_refuses_what_it_has_no_gradient_for(name):
+    """Also where the logits need none: the loss would leave the graph without a word."""
+    import torch
+    from torch.autograd import forward_ad
+    from oxitorch_b200 import functional as F
+    x, tokens = torch.randn(3, 5, device="cuda"), torch.tensor([0, 4, -1], device="cuda")
+    v = torch.ones(3, device="cuda")
+    args = dict(old_logp=-v, advantages=v, ref_logp=-v, kl_coef=0.1)
+    for logits in (x, x.clone().requires_grad_()):
+        with pytest.raises(ValueError, match=name):
+            F.policy_loss(logits, tokens, **{**args, name: args[name].clone().requires_grad_()})
+        with torch.no_grad():
+            F.policy_loss(logits, tokens, **{**args, name: args[name].clone().requires_grad_()})
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(args[name], torch.ones_like(v))
+            with pytest.raises(ValueError, match=name):
+                F.policy_loss(logits, tokens, **{**args, name: dual})
+            F.policy_loss(logits, tokens, **args)
