@@ -1480,7 +1480,7 @@ def token_logprobs(logits, tokens, temperature=1.0, flag=None):
         _flag(flag, logits.device)
     x = _rows2d(logits)
     logp = torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device)
-    rows, vocab = x.shape
+    rows, vocab = tok.numel(), logits.shape[-1]
     N.check(N.load().oxc_policy_loss(
         x.data_ptr(), x.stride(0), tok.data_ptr(), None, None, None, 0.0, 0.0, 0.0,
         float(temperature), None, None, logp.data_ptr(), None, None, rows, vocab, max(rows, 1), dt,

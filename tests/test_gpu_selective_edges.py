@@ -255,3 +255,19 @@ def test_policy_loss_refuses_what_it_has_no_gradient_for(name):
             with pytest.raises(ValueError, match=name):
                 F.policy_loss(logits, tokens, **{**args, name: dual})
             F.policy_loss(logits, tokens, **args)
+
+
+def test_token_logprobs_over_no_classes():
+    """Refused where there are rows, as policy_loss refuses it; no rows are no matter."""
+    import torch
+    from oxitorch_b200 import functional as F
+    for lead in ((3,), (2, 3), (1,)):
+        tokens = torch.zeros(lead, dtype=torch.int64, device="cuda")
+        with pytest.raises(ValueError, match="zero classes"):
+            F.token_logprobs(torch.zeros(*lead, 0, device="cuda"), tokens)
+        with pytest.raises(ValueError, match="zero classes"):
+            F.policy_loss(torch.zeros(*lead, 0, device="cuda"), tokens, tokens.float(), tokens.float())
+    for vocab in (0, 5):
+        none = torch.zeros(0, dtype=torch.int64, device="cuda")
+        assert F.token_logprobs(torch.zeros(0, vocab, device="cuda"), none).shape == (0,)
+        assert F.policy_loss(torch.zeros(0, vocab, device="cuda"), none, none.float(), none.float())[0] == 0
