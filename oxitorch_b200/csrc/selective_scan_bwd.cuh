@@ -2,6 +2,8 @@
 // selective_scan.cuh).
 #pragma once
 
+#include <atomic>
+
 #include "selective_scan.cuh"
 
 namespace oxc {
@@ -525,12 +527,15 @@ static cudaError_t selective_bwd_one(const SelectiveArgs<T>& a, cudaStream_t s) 
   using M = BackwardShared<L, T, VEC ? 4 : 1, GATED>;
   static_assert(M::kBytes <= 227 * 1024, "a CTA's shared memory");
   static_assert(2 * M::R::kTurn * L::kChannels <= 2 * M::kIn, "dD and ddelta_bias fit");
-  static int registers = 0;  // those that take_registers counts on have to be there
+  // those that take_registers counts on have to be there; threads may ask at once
+  static std::atomic<int> known{0};
+  int registers = known.load(std::memory_order_relaxed);
   if (registers == 0) {
     cudaFuncAttributes attr;
     const cudaError_t e = cudaFuncGetAttributes(&attr, selective_bwd_kernel<T, LPC, VEC, GATED>);
     if (e != cudaSuccess) return e;
     registers = attr.numRegs;
+    known.store(registers, std::memory_order_relaxed);
   }
   if (Registers<L>::kDeal && registers != Registers<L>::kLaunch) return cudaErrorLaunchOutOfResources;
   return launch_scan(selective_bwd_kernel<T, LPC, VEC, GATED>,

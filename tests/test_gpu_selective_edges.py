@@ -3,6 +3,8 @@ without bound in a single step, factors below the smallest normal f32, ratios ne
 where they are clipped, divisors of the policy loss, and derivatives that there are
 none of.  Error bounds come from tests/selective_reference.py."""
 
+import threading
+
 import numpy as np
 import pytest
 
@@ -271,3 +273,35 @@ def test_token_logprobs_over_no_classes():
         none = torch.zeros(0, dtype=torch.int64, device="cuda")
         assert F.token_logprobs(torch.zeros(0, vocab, device="cuda"), none).shape == (0,)
         assert F.policy_loss(torch.zeros(0, vocab, device="cuda"), none, none.float(), none.float())[0] == 0
+
+
+# ---- selective_scan ------------------------------------------------------------------
+
+def test_selective_scan_backward_in_two_threads():
+    """Two threads that call the VJP at once, each on a stream of its own."""
+    import torch
+    from oxitorch_b200 import functional as F
+    args, _, dy, dlast = _scan_inputs(1, 200, 24, 16, "float32", False)
+    carry = F.selective_scan_fwd(**args)[2]
+    del args["h0"]
+    want = F.selective_scan_bwd(**args, carry=carry, dy=dy, dlast=dlast)
+    torch.cuda.synchronize()
+    found, failed = {}, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    found[i] = F.selective_scan_bwd(**args, carry=carry, dy=dy, dlast=dlast)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # shown by the assertion below
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for got in found.values():
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
