@@ -1,7 +1,8 @@
 """The operators of a selective state space model where they can go wrong: rates
 without bound in a single step, factors below the smallest normal f32, ratios next to
-where they are clipped, divisors of the policy loss, and derivatives that there are
-none of.  Error bounds come from tests/selective_reference.py."""
+where they are clipped, divisors of the policy loss, derivatives that there are none
+of, and rows cut into segments in every layout of the states.  Error bounds come from
+tests/selective_reference.py."""
 
 import threading
 
@@ -10,7 +11,7 @@ import pytest
 
 import selective_reference as R
 from test_gpu_draft import DTYPES, _check, _n, _t
-from test_gpu_selective import _clip_check, _gradients, _policy_check, _policy_inputs, _scan_inputs
+from test_gpu_selective import _clip_check, _gradients, _policy_check, _policy_inputs, _scan_check, _scan_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -276,6 +277,51 @@ def test_token_logprobs_over_no_classes():
 
 
 # ---- selective_scan ------------------------------------------------------------------
+
+# the channels of a CTA of the VJP
+_BACKWARD_CHANNELS = ((8, 128), (16, 128), (32, 64), (64, 32), (128, 16))
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("T,D,N", [(300, 20, 7), (260, 21, 8), (300, 20, 10), (230, 19, 12), (290, 140, 16), (300, 20, 24),
+                                   (211, 17, 23), (300, 36, 31), (260, 20, 40), (300, 19, 48), (260, 20, 64), (200, 33, 57),
+                                   (260, 12, 90), (200, 15, 96), (260, 20, 128), (300, 13, 101)])
+def test_selective_scan_of_segments_in_every_layout(T, D, N, gated, dtype, packed):
+    """One row, cut into segments in both directions, for every number of states a lane
+    and of lanes a channel, at widths that vectors fit and that they do not."""
+    from oxitorch_b200 import _native
+    size = _native.load().oxc_selective_scan_workspace_size
+    channels = next(c for n, c in _BACKWARD_CHANNELS if N <= n)
+    one = 4 * (D * (N + 2) + -(-D // channels) * T * 2 * N)
+    assert size(1, T, D, N, 0) > 0 and size(1, T, D, N, 1) > one
+    _scan_check(*_scan_inputs(1, T, D, N, dtype, packed, gated=gated))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,D,N", [(1, 40, 300, 64), (2, 33, 150, 128), (1, 35, 515, 40), (2, 20, 260, 96)])
+def test_selective_scan_many_states_over_many_channels(B, T, D, N, dtype):
+    """dB and dC summed over several tiles of channels where a CTA holds few of them.
+
+    With rates of -128 some decays lie below 2^-126, where the exponential gives 0: what is
+    lost of a gradient is below 2^-126 times one of a token (below 2^9: two normal variates,
+    a gate and another), the states (2^6), rates (2^8) and tokens (2^6) that it is summed
+    over; with 2^-126 for the states themselves, 2^-90 covers all."""
+    import torch
+    from oxitorch_b200 import functional as F
+    args, starts, dy, dlast = _scan_inputs(B, T, D, N, dtype, True)
+    leaves = [t.requires_grad_() for t in args.values()]
+    y, last = F.selective_scan(**args, starts=torch.from_numpy(starts).cuda())
+    ref = R.Scan(**{k: _n(t) for k, t in args.items()}, starts=starts)
+    want, bound = ref.out()
+    _check(y, want, bound + 2.0 ** -90, "y")
+    _check(last, ref.last, ref.last_bound + 2.0 ** -90, "last")
+    got = torch.autograd.grad((y, last), leaves, (dy, dlast))
+    want, bound = ref.grad(_n(dy), _n(dlast))
+    for k, d in zip(args, got):
+        _check(d, want[k], bound[k] + 2.0 ** -90, "d" + k)
+
 
 def test_selective_scan_backward_in_two_threads():
     """Two threads that call the VJP at once, each on a stream of its own."""
