@@ -368,7 +368,10 @@ static oxc_status policy_launch(const void* logits, int64_t stride, void* dlogit
   const int threads = part <= 128 * 16 * 8 ? 128 : 256;
   auto kernel = threads == 128 ? policy_cluster_kernel<T, 128> : policy_cluster_kernel<T, 256>;
   if (part > 40 * 1024) {  // beyond what a kernel may use unasked
-    const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, part);
+    // the most that any call asks for: a smaller limit, set by another thread between this
+    // and the launch, would refuse it
+    const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               kPolicyMaxPart);
     if (e != cudaSuccess) return cuda_fail(e, "oxc_policy_loss");
   }
   cudaLaunchConfig_t cfg = {};
