@@ -712,9 +712,10 @@ static oxc_status add_rms_bwd_launch(const float* r, const float* w, const float
   do {                                                                                          \
     auto kernel = exact ? add_rms_bwd_rows_kernel<T, VPT, MAXT, OXC_GRAD_EXACT, EDGE>           \
                         : add_rms_bwd_rows_kernel<T, VPT, MAXT, OXC_GRAD_REF, EDGE>;            \
-    if (smem > 40 * 1024) {                                                                     \
+    if (smem > 40 * 1024) { /* the most that any width asks for, as threads may ask at once */  \
       const cudaError_t e = cudaFuncSetAttribute(                                               \
-          (const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);         \
+          (const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,                     \
+          VPT * MAXT * (int)sizeof(float4) * (VPT <= 4 ? 2 : 1));                               \
       if (e != cudaSuccess) return cuda_fail(e, "oxc_add_rms_norm_bwd");                        \
     }                                                                                           \
     kernel<<<(unsigned)ctas, g.threads(), smem, s>>>(                                           \

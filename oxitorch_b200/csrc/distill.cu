@@ -502,7 +502,10 @@ static oxc_status distill_launch(const void* logits, int64_t stride, void* dlogi
   auto cluster = threads == 128 ? distill_cluster_kernel<T, 128> : distill_cluster_kernel<T, 256>;
   const void* kernel = size ? (const void*)cluster : (const void*)distill_wide_kernel<T>;
   if (smem > 40 * 1024) {  // beyond what a kernel may use unasked
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // the most that any call asks for: a smaller limit, set by another thread between this
+    // and the launch, would refuse it
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               size ? kDistillSmem : (int)teacher_smem(kDistillMaxTop));
     if (e != cudaSuccess) return cuda_fail(e, "oxc_distill_loss");
   }
   *losses = size ? size : 1;

@@ -540,9 +540,11 @@ static int pipe_vpt(int64_t cols, int nwg, int max_vpt) {
   return 0;
 }
 
+// All that a CTA can have, whatever this call needs: a smaller limit, set by another
+// thread between this and the launch, would refuse the call.
 template <typename K>
-static void allow_smem(K kernel, size_t bytes) {
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+static void allow_smem(K kernel) {
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)max_smem_optin());
 }
 
 static int64_t ln_bwd_ctas(int64_t rows) {
@@ -681,12 +683,12 @@ oxc_status oxc_layer_norm_bwd(const float* x, const float* w, const float* b, co
   do {                                                                                        \
     if (sacc) {                                                                               \
       auto k = ln_bwd_pipe_kernel<kBwdNG, kBwdNWG, VPT, ACT, MODE, true>;                     \
-      allow_smem(k, smem);                                                                    \
+      allow_smem(k);                                                                          \
       k<<<(unsigned)ctas, block, smem, s>>>(x, w, b, mean, rstd, dy, dx, parts, rows,         \
                                             (int)cols, chunk, stages, gc);                    \
     } else {                                                                                  \
       auto k = ln_bwd_pipe_kernel<kBwdNG, kBwdNWG, VPT, ACT, MODE, false>;                    \
-      allow_smem(k, smem);                                                                    \
+      allow_smem(k);                                                                          \
       k<<<(unsigned)ctas, block, smem, s>>>(x, w, b, mean, rstd, dy, dx, parts, rows,         \
                                             (int)cols, chunk, stages, gc);                    \
     }                                                                                         \

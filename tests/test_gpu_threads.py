@@ -50,7 +50,65 @@ def _policy(vocab):
     return call
 
 
-@pytest.mark.parametrize("make,sizes", [(_policy, (98304, 200000, 320000))], ids=["policy_loss"])
+def _distill(vocab):
+    import torch
+    from oxitorch_b200 import _native as N
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x, teacher = (torch.randn(2, n, device="cuda", generator=g) for n in (vocab, 8))
+    ids = torch.arange(16, device="cuda").view(2, 8)
+    loss, rows, d = x.new_empty(1), x.new_empty(2 * N.DISTILL_PARTS), torch.empty_like(x)
+    args = (x.data_ptr(), vocab, teacher.data_ptr(), ids.data_ptr(), 8, 1.0, None, loss.data_ptr(), rows.data_ptr(),
+            d.data_ptr(), 2, vocab, 2, 0, None, torch.cuda.current_stream().cuda_stream)
+    entry = N.load().oxc_distill_loss
+
+    def call():
+        N.check(entry(*args), "distill_loss")
+        return x, teacher, ids, loss, rows[:2], d
+    return call
+
+
+def _add_rms_norm(cols):
+    import torch
+    from oxitorch_b200 import _native as N
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    r, dy, dr = (torch.randn(16, cols, device="cuda", generator=g) for _ in range(3))
+    w, rstd = torch.randn(cols, device="cuda", generator=g), torch.rand(16, device="cuda", generator=g) + 0.5
+    dx, dw = torch.empty_like(r), torch.empty_like(w)
+    L = N.load()
+    ws = torch.empty(L.oxc_add_rms_norm_bwd_workspace_size(16, cols), dtype=torch.uint8, device="cuda")
+    args = (r.data_ptr(), w.data_ptr(), rstd.data_ptr(), dy.data_ptr(), cols, dr.data_ptr(), cols, dx.data_ptr(),
+            dx.data_ptr(), dw.data_ptr(), 16, cols, 0, 0, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
+
+    def call():
+        N.check(L.oxc_add_rms_norm_bwd(*args), "add_rms_norm backward")
+        return r, w, rstd, dy, dr, dx, dw
+    return call
+
+
+def _layer_norm(cols):
+    import torch
+    from oxitorch_b200 import _native as N
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    x, dy = (torch.randn(16, cols, device="cuda", generator=g) for _ in range(2))
+    w, b = (torch.randn(cols, device="cuda", generator=g) for _ in range(2))
+    mean, rstd = x.mean(1), 1 / x.std(1)
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(w)
+    L = N.load()
+    ws = torch.empty(L.oxc_layer_norm_bwd_workspace_size(16, cols), dtype=torch.uint8, device="cuda")
+    args = (x.data_ptr(), w.data_ptr(), b.data_ptr(), mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dx.data_ptr(),
+            dw.data_ptr(), db.data_ptr(), 16, cols, 0, 0, ws.data_ptr(), ws.numel(),
+            torch.cuda.current_stream().cuda_stream)
+
+    def call():
+        N.check(L.oxc_layer_norm_bwd(*args), "layer_norm backward")
+        return x, w, b, mean, rstd, dy, dx, dw, db
+    return call
+
+
+@pytest.mark.parametrize("make,sizes", [(_policy, (98304, 200000, 320000)), (_distill, (98304, 200000, 280000)),
+                                        (_add_rms_norm, (18000, 24576, 32768)), (_add_rms_norm, (8704, 10000, 12288)),
+                                        (_layer_norm, (3104, 3200, 4096))],
+                         ids=["policy_loss", "distill_loss", "add_rms_norm", "add_rms_norm, narrower", "layer_norm"])
 def test_threads_with_different_shared_memory(make, sizes):
     import torch
     found, failed = _at_once([lambda n=n: make(n) for n in 2 * sizes], 4000)
