@@ -306,12 +306,13 @@ _TENSORS = {torch.Tensor, torch.nn.Parameter}
 _dtype_of, _requires_grad = attrgetter("dtype"), attrgetter("requires_grad")
 
 
-def _flat_operands(name, tensors):
+def _flat_operands(name, tensors, types=None):
     """Checks dense float32 / bfloat16 tensors of the current device; returns their
-    addresses, sizes and dtype ids as arrays, and whether all are contiguous.  (By whole
-    lists, as a model has hundreds: 0.3 us a tensor.)"""
+    addresses, sizes and dtype ids as arrays, and whether all are contiguous.  ``types``:
+    the set of their types, if known.  (By whole lists, as a model has hundreds: 0.3 us a
+    tensor.)"""
     tensor = torch.Tensor
-    if not _TENSORS.issuperset(map(type, tensors)) and not all(isinstance(t, tensor) for t in tensors):
+    if not _TENSORS.issuperset(types or map(type, tensors)) and not all(isinstance(t, tensor) for t in tensors):
         raise TypeError(f"{name} must be torch CUDA tensors")
     kinds = set(map(_dtype_of, tensors))
     if not kinds <= _DTYPES.keys() or not {torch._C._cuda_getDevice()}.issuperset(map(tensor.get_device, tensors)):
@@ -325,12 +326,6 @@ def _flat_operands(name, tensors):
     else:
         dtypes = array("i", [_DTYPES[t.dtype] for t in tensors])
     return array("q", map(tensor.data_ptr, tensors)), array("q", map(tensor.numel, tensors)), dtypes, flat
-
-
-def _listed(tensors):
-    """The tensors of a list that are there."""
-    tensors = list(tensors)
-    return [t for t in tensors if t is not None] if type(None) in set(map(type, tensors)) else tensors
 
 
 def _any_recorded(tensors):
@@ -354,8 +349,12 @@ def global_norm(tensors):
     tensor: the host does not wait for it.  Tensors are float32 or bfloat16, dense, any
     number of them; None is skipped.  It has no gradient: parameters are measured under
     torch.no_grad or detached."""
-    tensors = _listed(tensors)
-    ptrs, sizes, dtypes, _ = _flat_operands("tensors", tensors)
+    tensors = list(tensors)
+    types = set(map(type, tensors))
+    if type(None) in types:
+        types.discard(type(None))
+        tensors = [t for t in tensors if t is not None]
+    ptrs, sizes, dtypes, _ = _flat_operands("tensors", tensors, types)
     if _any_recorded(tensors):
         raise ValueError("invalid argument: global_norm has no gradient; detach its tensors")
     if not tensors:
@@ -388,10 +387,13 @@ def clip_global_norm_(grads, max_norm, out=None):
         out = list(out)
         if len(out) != len(grads):
             raise ValueError(f"invalid argument: {len(out)} outputs for {len(grads)} gradients")
-        if type(None) in set(map(type, grads)):
+    types = set(map(type, grads))
+    if type(None) in types:
+        types.discard(type(None))
+        if out is not None:
             out = [o for o, g in zip(out, grads) if g is not None]
-    grads = _listed(grads)
-    ptrs, sizes, dtypes, flat = _flat_operands("gradients", grads)
+        grads = [g for g in grads if g is not None]
+    ptrs, sizes, dtypes, flat = _flat_operands("gradients", grads, types)
     if not grads:
         return torch.zeros((), device="cuda")
     to = None
