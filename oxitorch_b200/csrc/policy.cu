@@ -91,7 +91,7 @@ __device__ __forceinline__ PolicyTerm policy_term(const PolicyArgs& a, const Sam
   const float near = 0x1p-21f * (1.0f + fabsf(t.logp) + fabsf(s.old)), r = expf(gap);
   float held = (r < a.low ? a.low : r > a.high ? a.high : r) * s.adv, free = r * s.adv;
   bool clipped = free > held;
-  if (fabsf(gap - a.log_low) < near || fabsf(gap - a.log_high) < near) {
+  if (__builtin_expect(fminf(fabsf(gap - a.log_low), fabsf(gap - a.log_high)) < near, 0)) {
     const double q = policy_ratio(logit, row, s.old, a.inv_tau64), f = q * (double)s.adv;
     const double h = (q < a.low64 ? a.low64 : q > a.high64 ? a.high64 : q) * (double)s.adv;
     clipped = f > h;
