@@ -13,8 +13,8 @@
 //
 // Bound by HBM: each element is read for the norm, and read again and written for the
 // scaling; the second read comes from L2 as far as that goes (126 MB).  473 million f32:
-// the norm 270 us, with the scaling 944 to 972, 89 to 92% of the copy bandwidth for three
-// passes; 83 tensors of a small model 10 us in a captured graph (78 by the host).
+// the norm 270 us, with the scaling 944 to 982, 88 to 92% of the copy bandwidth for three
+// passes; 83 tensors of a small model 11 us in a captured graph (79 by the host).
 #include <algorithm>
 #include <new>
 

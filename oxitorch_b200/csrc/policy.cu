@@ -16,8 +16,8 @@
 // Bound by HBM: 2 sizeof(T) bytes a logit, the row read once and its gradient
 // written once.  As in distill.cu a row stays in shared memory between the two,
 // shared by a cluster of 1 to 8 CTAs that exchange (max, sum) pairs; rows wider
-// than that take the kernel of three passes.  f32 [8192, 32000] takes 337 us, 95% of the
-// copy bandwidth; bf16 [8192, 131072] 788 us, 83%: there the two exponentials a logit keep
+// than that take the kernel of three passes.  f32 [8192, 32000] takes 342 us, 94% of the
+// copy bandwidth; bf16 [8192, 131072] 816 us, 80%: there the two exponentials a logit keep
 // their unit busy for 60% of that time, and issue and barriers come to as much.
 #include <cooperative_groups.h>
 #include <math.h>

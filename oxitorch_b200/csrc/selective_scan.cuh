@@ -286,7 +286,7 @@ constexpr int kFull = 1, kDone = 3;  // + the tile's parity
 
 // The threads that prepare tiles, behind those that walk through them.  (With 128, whose
 // chains of dependent operations then were what the others waited for: bf16 [3, 4097,
-// 1001] with 24 states 390 us forward and 943 VJP instead of 280 and 719.)
+// 1001] with 24 states 390 us forward and 943 VJP instead of 280 and 719; now 264 and 709.)
 constexpr int kHelpers = 256;
 
 // Deals out the registers that a CTA is launched with: the warps that walk through tiles
