@@ -328,9 +328,9 @@ def _flat_operands(name, tensors, types=None):
     return array("q", map(tensor.data_ptr, tensors)), array("q", map(tensor.numel, tensors)), dtypes, flat
 
 
-def _any_recorded(tensors):
-    """_recorded, by the whole list."""
-    return (torch.is_grad_enabled() and any(map(_requires_grad, tensors))) or (
+def _any_recorded(tensors, known=False):
+    """_recorded, by the whole list; ``known``: none of them requires a gradient."""
+    return (not known and torch.is_grad_enabled() and any(map(_requires_grad, tensors))) or (
         forward_ad._current_level >= 0 and _has_tangent(*tensors))
 
 
@@ -405,7 +405,8 @@ def clip_global_norm_(grads, max_norm, out=None):
                         not (g.is_contiguous() and o.is_contiguous()) and (g.shape, g.stride()) != (o.shape, o.stride())):
                     raise ValueError(f"shape mismatch: an output {list(o.shape)} {o.dtype} for a gradient "
                                      f"{list(g.shape)} {g.dtype}, or laid out otherwise")
-    if any(map(_requires_grad, grads if out is None else out)) or _any_recorded(grads):
+    # (in place the first question has answered the second but for tangents)
+    if any(map(_requires_grad, grads if out is None else out)) or _any_recorded(grads, out is None):
         raise ValueError("invalid argument: clip_global_norm_ has no gradient and writes to tensors outside any graph")
     L = N.load()
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
